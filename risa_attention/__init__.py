@@ -11,7 +11,7 @@ __all__ = list(_impl.__all__)
 __version__ = _impl.__version__
 
 for _name in ("attention", "dense", "sparse", "reference", "permutation", "_backend", "_execution",
-              "_quantization", "_types", "_validation", "_key_mask"):
+              "_quantization", "_types", "_validation", "_key_mask", "serving"):
     sys.modules[f"{__name__}.{_name}"] = importlib.import_module(f"risaattention_b200.{_name}")
 if _impl._backend._C is not None:
     sys.modules[f"{__name__}._C"] = _impl._backend._C

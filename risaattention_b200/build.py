@@ -8,6 +8,7 @@ from __future__ import annotations
 
 import concurrent.futures
 import os
+import re
 import subprocess
 import sys
 from pathlib import Path
@@ -16,7 +17,10 @@ PKG = Path(__file__).resolve().parent
 CSRC = PKG / "csrc"
 OBJ = CSRC / "_obj"
 LIB = PKG / "librisa_b200.so"
-UNITS = ["prep_qk", "prep_v", "misc", "attention_api", "attention_rows", "attention_tc"]
+UNITS = ["prep_qk", "prep_v", "misc", "attention_api", "attention_rows", "attention_tc", "cache_ops",
+         "paged_rows"]
+# these share no numeric contract with other kernels: their arithmetic is as written
+EXACT_UNITS = {"cache_ops", "paged_rows"}
 # measurement probe (INT8 issue-loop ceiling used by bench.py), its own library
 PROBE_LIB = PKG / "librisa_b200_probe.so"
 PROBE_UNITS = ["mma_peak"]
@@ -28,16 +32,24 @@ NVCC_FLAGS = [
 ]
 
 
-def _newest_header() -> float:
-    headers = list(CSRC.glob("*.cuh")) + list((PKG.parent / "include").glob("*.h"))
-    return max(p.stat().st_mtime for p in headers)
+def _newest(source: Path, seen: set[Path] | None = None) -> float:
+    """Latest modification of a source and of every file that it includes by a relative name."""
+    seen = set() if seen is None else seen
+    seen.add(source)
+    newest = source.stat().st_mtime
+    for name in re.findall(r'^\s*#include "([^"]+)"', source.read_text(), re.MULTILINE):
+        header = (source.parent / name).resolve()
+        if header.exists() and header not in seen:
+            newest = max(newest, _newest(header, seen))
+    return newest
 
 
 def _compile(unit: str, force: bool, verbose: bool) -> str | None:
     src, obj = CSRC / f"{unit}.cu", OBJ / f"{unit}.o"
-    if not force and obj.exists() and obj.stat().st_mtime > max(src.stat().st_mtime, _newest_header()):
+    if not force and obj.exists() and obj.stat().st_mtime > _newest(src):
         return None
-    cmd = ["nvcc", *NVCC_FLAGS, "-c", str(src), "-o", str(obj)]
+    flags = [f for f in NVCC_FLAGS if f != "--use_fast_math" or unit not in EXACT_UNITS]
+    cmd = ["nvcc", *flags, "-c", str(src), "-o", str(obj)]
     if verbose:
         cmd[1:1] = ["-Xptxas", "-v"]
     proc = subprocess.run(cmd, capture_output=True, text=True)
@@ -47,7 +59,7 @@ def _compile(unit: str, force: bool, verbose: bool) -> str | None:
 
 
 def build_torch_extension(force: bool = False) -> Path:
-    """Compiles csrc/torch_binding.cpp into the in-tree module ``risaattention_b200/_C*.so``: the
+    """Compiles csrc/torch_binding.cpp and csrc/cache_binding.cpp into the in-tree module ``risaattention_b200/_C*.so``: the
     PyTorch C++ extension through which the Python runtime reaches the C-ABI library (linked by
     relative run path, so the pair can be moved together)."""
     import sysconfig
@@ -57,22 +69,33 @@ def build_torch_extension(force: bool = False) -> Path:
     from torch.utils import cpp_extension
 
     target = PKG / f"_C{sysconfig.get_config_var('EXT_SUFFIX')}"
-    src = CSRC / "torch_binding.cpp"
-    newest = max(src.stat().st_mtime, (PKG.parent / "include" / "risa_b200.h").stat().st_mtime)
-    if not force and target.exists() and target.stat().st_mtime > newest:
+    sources = [CSRC / "torch_binding.cpp", CSRC / "cache_binding.cpp"]
+    if not force and target.exists() and target.stat().st_mtime > max(map(_newest, sources)):
         return target
+    objects = [OBJ / f"{source.stem}.o" for source in sources]
     includes = [*cpp_extension.include_paths(), pybind11.get_include(),
                 sysconfig.get_paths()["include"], "/usr/local/cuda/include"]
     torch_lib = str(Path(torch.__file__).resolve().parent / "lib")
-    cmd = ["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-fvisibility=hidden",
-           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
-           "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
-           *[f"-I{path}" for path in includes], str(src), "-o", str(target),
-           f"-L{PKG}", "-lrisa_b200", f"-L{torch_lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu",
-           "-lc10", "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"]
-    proc = subprocess.run(cmd, capture_output=True, text=True)
-    if proc.returncode != 0:
-        raise RuntimeError(f"g++ failed for torch_binding.cpp:\n{proc.stdout}\n{proc.stderr}")
+    compile_flags = ["-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden",
+                     f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+                     "-DTORCH_EXTENSION_NAME=_C", "-DTORCH_API_INCLUDE_EXTENSION_H",
+                     *[f"-I{path}" for path in includes]]
+
+    def run(what, cmd):
+        proc = subprocess.run(cmd, capture_output=True, text=True)
+        if proc.returncode != 0:
+            raise RuntimeError(f"g++ failed for {what}:\n{proc.stdout}\n{proc.stderr}")
+
+    def compile_source(pair):
+        source, obj = pair
+        if force or not obj.exists() or obj.stat().st_mtime <= _newest(source):
+            run(source.name, ["g++", *compile_flags, "-c", str(source), "-o", str(obj)])
+
+    with concurrent.futures.ThreadPoolExecutor(max_workers=len(sources)) as pool:
+        list(pool.map(compile_source, zip(sources, objects)))
+    run(target.name, ["g++", "-shared", *map(str, objects), "-o", str(target), f"-L{PKG}", "-lrisa_b200",
+                      f"-L{torch_lib}", "-ltorch_python", "-ltorch", "-ltorch_cpu", "-lc10",
+                      "-Wl,-rpath,$ORIGIN", f"-Wl,-rpath,{torch_lib}"])
     return target
 
 

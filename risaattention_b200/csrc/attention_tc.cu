@@ -2306,6 +2306,12 @@ int attention_tc_split_parts(int ctas, int n_k, int cta_k, int sms) {
 
 }  // namespace risa_b200
 
+namespace risa_b200 {
+namespace serving {
+int device_status();  // what the serving kernels recorded (cache_ops.cu)
+}
+}  // namespace risa_b200
+
 extern "C" int risa_b200_device_status(void) {
   unsigned int status = 0, zero = 0;
   if (cudaMemcpyFromSymbol(&status, risa_b200::tc::g_wait_status, sizeof(status)) != cudaSuccess)
@@ -2317,7 +2323,7 @@ extern "C" int risa_b200_device_status(void) {
                            "attention kernel gave up waiting at site %u (bounded wait expired)",
                            status);
   }
-  return RISA_B200_OK;
+  return risa_b200::serving::device_status();
 }
 
 extern "C" int risa_b200_bounded_wait_self_test(uint64_t limit_ns, void* stream) {

@@ -24,6 +24,8 @@
 
 namespace py = pybind11;
 
+void bind_cache(py::module_& m);  // the serving operators (cache_binding.cpp)
+
 namespace {
 
 void check(int status) {
@@ -754,4 +756,5 @@ PYBIND11_MODULE(_C, m) {
     check(risa_b200_bounded_wait_self_test(limit_ns, stream_of(stream_ptr)));
   });
   m.def("abi_version", [] { return risa_b200_abi_version(); });
+  bind_cache(m);
 }
