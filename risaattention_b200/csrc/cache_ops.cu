@@ -1,5 +1,6 @@
 // Rotary positions, the append that fills a paged key/value cache, and eviction from it: the serving
 // operators that move data.  All are bounded by memory traffic (large) or by launch latency (steps).
+#include "paged_tc.cuh"
 #include "serving.cuh"
 
 namespace risa_b200 {
@@ -18,6 +19,9 @@ unsigned int* status_word() {
 
 // Reports (and clears) what the kernels recorded.
 int device_status() {
+  const int site = paged_tc_wait_status();
+  if (site < 0) return fail(RISA_B200_CUDA, "device status: %s", cudaGetErrorString(cudaGetLastError()));
+  if (site > 0) return fail(RISA_B200_DEVICE, "paged attention kernel gave up waiting at site %d (bounded wait expired)", site);
   unsigned int status = 0, zero = 0;
   if (cudaMemcpyFromSymbol(&status, g_bad_page, sizeof(status)) != cudaSuccess)
     return fail(RISA_B200_CUDA, "device status: %s", cudaGetErrorString(cudaGetLastError()));

@@ -8,18 +8,17 @@
 // heads), keeps running maximum, sum and output in registers, and adds V^T P^T in the same orientation.
 // Codes become 16-bit values in registers on the way to the matrix instruction: whole numbers up to 128 are
 // exact in bf16 and fp16, so K's scale multiplies the score and V's the probability, both in 32 bits.
+#include "paged_tc.cuh"
 #include "serving_plan.cuh"
+
+#include <climits>
+#include <type_traits>
 
 namespace risa_b200 {
 namespace serving {
 namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-// Where a running maximum starts: below every score (in units of log 2) that 16-bit operands of use
-// produce, and finite, so that a row that has seen nothing yet needs no case of its own.
-constexpr float kNoMaximum = -1e30f;
-
 struct RowsArgs {
   LineArgs line;
   const void* q;
@@ -305,8 +304,7 @@ __device__ __forceinline__ int channel_of(int mt, int second) {
 template <typename C>
 __global__ __launch_bounds__(kThreads) void paged_rows_kernel(const RowsArgs a) {
   extern __shared__ __align__(128) char smem[];
-  __shared__ BlockScan<kThreads> scan;
-  __shared__ Place found;
+  __shared__ LineShared<kThreads> shared;
   __shared__ float warp_max[kWarps][C::R], warp_sum[kWarps][C::R];
   using T = typename C::T;
   using W = Walk<C, true>;
@@ -326,25 +324,15 @@ __global__ __launch_bounds__(kThreads) void paged_rows_kernel(const RowsArgs a) 
         for (int h = threadIdx.x; h < heads; h += kThreads) a.lse[int64_t(token) * heads + h] = -INFINITY;
     }
   }
-  const int64_t total = line_total<kThreads>(a.line, scan);
-  const int workers = int(min(int64_t(gridDim.x), (total + a.min_steps - 1) / a.min_steps));
+  const int64_t total = line_total<kThreads>(a.line, shared);
+  const int workers = workers_of(total, gridDim.x, a.min_steps);
   if (int(blockIdx.x) >= workers) return;
-  int64_t at = border(total, blockIdx.x, workers);
-  const int64_t end = border(total, blockIdx.x + 1, workers);
-  const Place start = line_place<kThreads>(a.line, at, scan, found);
-  int s = start.sequence;
-  int64_t offset = start.offset;
-  while (at < end) {
-    const Sequence seq = sequence_of(a.line.step, s);
-    const Share share = share_of(a.line, seq);
-    if (offset >= work_of(a.line, share)) {
-      ++s;
-      offset = 0;
-      continue;
-    }
-    const int unit = int(offset / share.steps), step0 = int(offset - int64_t(unit) * share.steps);
-    const int take = int(min(int64_t(share.steps - step0), end - at));
-    const int head = unit / share.blocks, row0 = (unit - head * share.blocks) * R, rows = seq.count * a.line.group;
+  const int64_t begin = border(total, blockIdx.x, workers);
+  Pieces pieces{border(total, blockIdx.x + 1, workers) - begin, line_place<kThreads>(a.line, begin, shared)};
+  Piece piece;
+  while (pieces.next(a.line, piece)) {
+    const Sequence seq = piece.seq;
+    const int s = piece.sequence, head = piece.head, row0 = piece.block * R, rows = seq.count * a.line.group, take = piece.count;
 
     uint32_t qf[NT][C::KS][2];
     load_queries<C>(a, seq, head, row0, rows, qf);
@@ -364,7 +352,7 @@ __global__ __launch_bounds__(kThreads) void paged_rows_kernel(const RowsArgs a) 
     const int all_lo = visible(seq.length - seq.count + last_row / a.line.group, seq.length, a.line.causal, a.line.window).lo;
     const int low = a.line.window > 0 ? visible(seq.length - seq.count, seq.length, true, a.line.window).lo : 0;
 
-    W walk{a, a.line.step.table + int64_t(s) * a.line.step.width, head, (share.first_step + step0 + warp) * 16, low, seq.length,
+    W walk{a, a.line.step.table + int64_t(s) * a.line.step.width, head, (piece.first + warp) * 16, low, seq.length,
            take > warp ? (take - warp + kWarps - 1) / kWarps : 0, s};
     walk.base = ring;
     walk.start();
@@ -481,8 +469,8 @@ __global__ __launch_bounds__(kThreads) void paged_rows_kernel(const RowsArgs a) 
         for (int i = 0; i < 4; ++i) mine[(nt * 8 + 2 * t + (i & 1)) * kRowStride + channel_of<C>(mt, i >> 1)] = o[nt][mt][i];
     }
     __syncthreads();
-    const bool whole = take == share.steps;
-    float* slot = whole ? nullptr : a.parts + (int64_t(blockIdx.x) * 2 + (step0 == 0 ? 1 : 0)) * (R * D + 2 * R);
+    const bool whole = piece.whole;
+    float* slot = whole ? nullptr : a.parts + (int64_t(blockIdx.x) * 2 + (piece.opens ? 1 : 0)) * slot_floats(R, D);
     for (int i = threadIdx.x; i < R * (D / 4); i += kThreads) {
       const int r = i / (D / 4), c = (i % (D / 4)) * 4;
       if (row0 + r >= rows) continue;
@@ -520,63 +508,6 @@ __global__ __launch_bounds__(kThreads) void paged_rows_kernel(const RowsArgs a) 
       }
     }
     __syncthreads();
-    at += take;
-    offset += take;
-  }
-}
-
-// One CTA per (border between two workers, query row): the first border inside a unit joins that unit's
-// parts in the order of their keys, so that results do not depend on which worker ended first.
-template <typename T, int D>
-__global__ __launch_bounds__(kThreads) void join_parts_kernel(const RowsArgs a, int max_workers) {
-  __shared__ BlockScan<kThreads> scan;
-  __shared__ Place found;
-  chain_wait();
-  chain_release();
-  const int64_t total = line_total<kThreads>(a.line, scan);
-  const int workers = int(min(int64_t(max_workers), (total + a.min_steps - 1) / a.min_steps));
-  const int c = blockIdx.x, R = a.line.rows;
-  if (c + 1 >= workers) return;
-  const int64_t edge = border(total, c + 1, workers), previous = border(total, c, workers);
-  const Place place = line_place<kThreads>(a.line, edge, scan, found);
-  const Sequence seq = sequence_of(a.line.step, place.sequence);
-  const Share share = share_of(a.line, seq);
-  const int unit = int(place.offset / share.steps);
-  const int64_t inside = place.offset - int64_t(unit) * share.steps, unit_start = edge - inside, unit_end = unit_start + share.steps;
-  if (inside == 0 || previous > unit_start) return;  // no unit is cut here, or an earlier border joins it
-  const int head = unit / share.blocks, r = blockIdx.y, row = (unit - head * share.blocks) * R + r;
-  if (row >= seq.count * a.line.group) return;
-  const int64_t slot_size = int64_t(R) * D + 2 * R;
-  int parts = 1;
-  while (c + parts < workers && border(total, c + parts, workers) < unit_end) ++parts;
-  // parts c (second slot), c + 1, ... (first slots)
-  auto slot_of = [&](int i) { return a.parts + (int64_t(c + i) * 2 + (i == 0 ? 1 : 0)) * slot_size; };
-  float top = kNoMaximum;
-  for (int i = threadIdx.x; i < parts; i += kThreads) top = fmaxf(top, slot_of(i)[R * D + r]);
-  __shared__ float tops[kWarps];
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
-  if ((threadIdx.x & 31) == 0) tops[threadIdx.x >> 5] = top;
-  __syncthreads();
-  top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
-  constexpr int PER = D > kThreads ? D / kThreads : 1;
-  float sum[PER] = {}, norm = 0.f;
-  if (int(threadIdx.x) * PER < D) {
-#pragma unroll 8
-    for (int i = 0; i < parts; ++i) {
-      const float* slot = slot_of(i);
-      const float f = ex2_approx(slot[R * D + r] - top);
-      norm += f * slot[R * D + R + r];
-#pragma unroll
-      for (int e = 0; e < PER; ++e) sum[e] += f * slot[r * D + threadIdx.x + e * kThreads];
-    }
-    const float f = norm == 0.f ? 0.f : 1.0f / norm;
-    const int token = row / a.line.group, h = head * a.line.group + row % a.line.group;
-    T* out = static_cast<T*>(a.out) + int64_t(seq.first + token) * a.on + int64_t(h) * a.oh;
-#pragma unroll
-    for (int e = 0; e < PER; ++e) out[threadIdx.x + e * kThreads] = static_cast<T>(sum[e] * f);
-    if (threadIdx.x == 0 && a.lse != nullptr)
-      a.lse[int64_t(seq.first + token) * (a.line.kv_heads * a.line.group) + h] = norm == 0.f ? -INFINITY : top * kLn2 + logf(norm);
   }
 }
 
@@ -586,8 +517,7 @@ __global__ __launch_bounds__(kThreads) void join_parts_kernel(const RowsArgs a, 
 template <typename C>
 __global__ __launch_bounds__(kThreads) void weigh_rows_kernel(const RowsArgs a) {
   extern __shared__ __align__(128) char smem[];
-  __shared__ BlockScan<kThreads> scan;
-  __shared__ Place found;
+  __shared__ LineShared<kThreads> shared;
   using W = Walk<C, false>;
   constexpr int NT = C::NT, R = C::R;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
@@ -598,36 +528,26 @@ __global__ __launch_bounds__(kThreads) void weigh_rows_kernel(const RowsArgs a) 
   // what no step covers: in front of the window, behind the length
   for (int64_t u = blockIdx.x; u < int64_t(a.line.step.batch) * a.line.kv_heads; u += gridDim.x) {
     const Sequence seq = sequence_of(a.line.step, int(u / a.line.kv_heads));
-    if (a.line.max_rows > 0 && seq.count * a.line.group > a.line.max_rows) continue;
-    const Share share = share_of(a.line, seq);
-    const int from = share.blocks == 0 ? 0 : min(share.first_step * 16, slots);
-    const int to = share.blocks == 0 ? 0 : min((share.first_step + share.steps) * 16, slots);
+    const int rows = seq.count * a.line.group;
+    if (rows > a.line.max_rows) continue;
+    const StepRange range = rows == 0 ? StepRange{0, 0} : steps_of(a.line, seq, 0);
+    const int from = min(range.first * 16, slots), to = min((range.first + range.count) * 16, slots);
     for (int i = threadIdx.x; i < slots - (to - from); i += kThreads) {
       const int key = i < from ? i : i + (to - from);
       a.weights[u * slots + key] = a.previous != nullptr ? a.previous[u * slots + key] : 0.f;
     }
   }
-  const int64_t total = line_total<kThreads>(a.line, scan);
-  const int workers = int(min(int64_t(gridDim.x), (total + a.min_steps - 1) / a.min_steps));
+  const int64_t total = line_total<kThreads>(a.line, shared);
+  const int workers = workers_of(total, gridDim.x, a.min_steps);
   if (int(blockIdx.x) >= workers) return;
-  int64_t at = border(total, blockIdx.x, workers);
-  const int64_t end = border(total, blockIdx.x + 1, workers);
-  const Place start = line_place<kThreads>(a.line, at, scan, found);
-  int s = start.sequence;
-  int64_t offset = start.offset;
-  while (at < end) {
-    const Sequence seq = sequence_of(a.line.step, s);
-    const Share share = share_of(a.line, seq);
-    if (offset >= work_of(a.line, share)) {
-      ++s;
-      offset = 0;
-      continue;
-    }
-    const int head = int(offset / share.steps), step0 = int(offset - int64_t(head) * share.steps);
-    const int take = int(min(int64_t(share.steps - step0), end - at));
-    const int rows = seq.count * a.line.group, blocks = (rows + R - 1) / R;
+  const int64_t begin = border(total, blockIdx.x, workers);
+  Pieces pieces{border(total, blockIdx.x + 1, workers) - begin, line_place<kThreads>(a.line, begin, shared)};
+  Piece piece;
+  while (pieces.next(a.line, piece)) {
+    const Sequence seq = piece.seq;
+    const int s = piece.sequence, head = piece.head, rows = seq.count * a.line.group, blocks = (rows + R - 1) / R, take = piece.count;
     const int low = a.line.window > 0 ? visible(seq.length - seq.count, seq.length, true, a.line.window).lo : 0;
-    W walk{a, a.line.step.table + int64_t(s) * a.line.step.width, head, (share.first_step + step0 + warp) * 16, low, seq.length,
+    W walk{a, a.line.step.table + int64_t(s) * a.line.step.width, head, (piece.first + warp) * 16, low, seq.length,
            take > warp ? (take - warp + kWarps - 1) / kWarps : 0, s};
     walk.base = ring;
     walk.start();
@@ -697,8 +617,6 @@ __global__ __launch_bounds__(kThreads) void weigh_rows_kernel(const RowsArgs a) 
     }
     copies_wait<0>();
     __syncwarp();
-    at += take;
-    offset += take;
   }
 }
 
@@ -747,7 +665,7 @@ RowsArgs rows_args(const risa_b200_cache* cache, const risa_b200_step* step, con
                    float scale, int is_causal, int window, unsigned int* status) {
   RowsArgs a{};
   const int group = q_heads / cache->kv_heads;
-  a.line = {view_of(*step, cache->page_size), cache->kv_heads, group, 8 * column_blocks_of(*step, group), 0, 16, is_causal != 0, window};
+  a.line = {view_of(*step, cache->page_size), cache->kv_heads, group, 8 * column_blocks_of(*step, group), 1, INT_MAX, 16, is_causal != 0, window};
   a.q = q;
   a.qn = qs[0];
   a.qh = qs[1];
@@ -776,10 +694,21 @@ int allow_shared(K kernel, int bytes, const char* what) {
 using namespace risa_b200;
 using namespace risa_b200::serving;
 
+// Whether a step can hold sequences for the tensor-core kernel.
+static bool takes_tensor_cores(const risa_b200_cache& cache, const risa_b200_step& step, int group) {
+  const int64_t most = step.query_offsets == nullptr ? group : int64_t(step.tokens) * group;
+  return cache.head_dim <= 128 && most >= kTcFewestRows;
+}
+static size_t rows_scratch(const risa_b200_cache& cache, const risa_b200_step& step, int group) {
+  return size_t(kMaxWorkers) * 2 * slot_floats(8 * column_blocks_of(step, group), cache.head_dim) * sizeof(float);
+}
+
 extern "C" size_t risa_b200_paged_attention_scratch_size(const risa_b200_cache* cache, const risa_b200_step* step, int q_heads) {
   if (cache == nullptr || step == nullptr || cache->kv_heads <= 0 || q_heads <= 0) return 0;
-  const int r = 8 * column_blocks_of(*step, q_heads / cache->kv_heads);
-  return size_t(kMaxWorkers) * 2 * (size_t(r) * cache->head_dim + 2 * r) * sizeof(float);
+  const int group = q_heads / cache->kv_heads;
+  size_t bytes = rows_scratch(*cache, *step, group);
+  if (takes_tensor_cores(*cache, *step, group)) bytes += size_t(kTcWorkers) * 2 * slot_floats(paged_tc_rows(), cache->head_dim) * sizeof(float);
+  return bytes;
 }
 
 extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const risa_b200_step* step, const void* q,
@@ -802,15 +731,25 @@ extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const ris
   a.clear_rest = clear_rest;
   a.parts = static_cast<float*>(scratch);
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  const int bad = with_tile(dtype_code, cache->dtype_code == kInt8, cache->head_dim, a.line.rows / 8, [&](auto tile) {
+  const bool tensor_cores = takes_tensor_cores(*cache, *step, a.line.group);
+  if (tensor_cores) a.line.max_rows = kTcFewestRows - 1;
+  int bad = with_tile(dtype_code, cache->dtype_code == kInt8, cache->head_dim, a.line.rows / 8, [&](auto tile) {
     using C = decltype(tile);
     constexpr int bytes = kWarps * Walk<C, true>::STAGE * Walk<C, true>::STAGES;
     if (const int bad = allow_shared(paged_rows_kernel<C>, bytes, "paged attention")) return bad;
     const int workers = C::D == 256 && !C::INT8 ? kMaxWorkers / 2 : kMaxWorkers;
     launch_chained(paged_rows_kernel<C>, dim3(workers), dim3(kThreads), bytes, stream, a);
-    launch_chained(join_parts_kernel<typename C::T, C::D>, dim3(workers - 1, C::R), dim3(kThreads), 0, stream, a, workers);
+    const JoinArgs join{a.line, a.parts, workers, a.min_steps, out, a.on, a.oh, lse};
+    launch_chained(join_parts_kernel<typename C::T, C::D>, dim3(workers - 1, C::R / 4), dim3(128), 0, stream, join);
     return RISA_B200_OK;
   });
+  if (bad == RISA_B200_OK && tensor_cores) {
+    TcArgs t{a.line, q, a.qn, a.qh, out, a.on, a.oh, lse, a.keys, a.values, a.key_scales, a.value_scales, a.pages, a.scale_log2,
+             a.parts + rows_scratch(*cache, *step, a.line.group) / sizeof(float), 2, status};
+    t.line.min_rows = kTcFewestRows;
+    t.line.max_rows = INT_MAX;
+    bad = paged_tc(t, dtype_code, cache->dtype_code == kInt8, cache->head_dim, stream);
+  }
   return bad ? bad : check_launch("paged attention");
 }
 

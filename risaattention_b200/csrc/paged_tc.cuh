@@ -1,0 +1,35 @@
+// Arguments of the tensor-core kernels over a paged cache (paged_tc.cu), as their callers fill them.
+#pragma once
+#include "serving_plan.cuh"
+
+namespace risa_b200 {
+namespace serving {
+
+constexpr int kTcWorkers = 148;  // one CTA per SM
+// Sequences with at least so many query rows per key head are theirs.
+constexpr int kTcFewestRows = 33;
+
+struct TcArgs {
+  LineArgs line;  // rows and keys are the kernel's own
+  const void* q;
+  int64_t qn, qh;
+  void* out;
+  int64_t on, oh;
+  float* lse;
+  const char* keys;
+  const char* values;
+  const float* key_scales;
+  const float* value_scales;
+  int pages;
+  float scale_log2;
+  float* parts;
+  int min_steps;
+  unsigned int* status;
+};
+
+int paged_tc_rows();
+int paged_tc(TcArgs args, int dtype_code, bool codes, int head_dim, cudaStream_t stream);
+int paged_tc_wait_status();
+
+}  // namespace serving
+}  // namespace risa_b200

@@ -1,8 +1,9 @@
 // How the work of a step is divided among the CTAs of a launch.  Lengths live on the device, so every CTA
-// computes the division itself from the lengths of all sequences: the units of a sequence (key head x
-// block of query rows) hold equally many key steps, all steps of all units in their order form one line, and
-// worker c of n takes [W c / n, W (c + 1) / n) of it.  A unit that a border cuts is finished by several
-// workers, each leaving a partial result in a slot of its own; a second launch joins them in order.
+// computes the division itself: the units (sequence, key head, block of query rows) with their key steps,
+// laid end to end, form one line, and worker c of n takes [W c / n, W (c + 1) / n) of it.  A unit that a
+// border cuts is finished by several workers, each leaving a partial result in a slot of its own; a second
+// launch joins them in order.  Equal shares whatever the lengths, at most two partial results per worker,
+// and the same division (so the same bits) every time.
 #pragma once
 #include "serving.cuh"
 
@@ -11,29 +12,38 @@ namespace serving {
 
 struct LineArgs {
   StepView step;
-  int kv_heads, group;  // query heads per key head
-  int rows;             // query rows of a unit
-  int max_rows;         // sequences with more query rows per key head belong to another launch (0: none do)
-  int keys;             // keys of a step
+  int kv_heads, group;     // query heads per key head
+  int rows;                // query rows of a block
+  int min_rows, max_rows;  // sequences with fewer or more query rows per key head belong to another launch
+  int keys;                // keys of a step
   int causal, window;
 };
 
-// One sequence's share of the line.
+// Key steps [first, first + count) of a block: those with a key that one of its rows sees, at least one.
+struct StepRange {
+  int first, count;
+};
+__device__ __forceinline__ StepRange steps_of(const LineArgs& a, const Sequence& q, int block) {
+  const int rows = q.count * a.group, row0 = block * a.rows;
+  const int token0 = row0 / a.group, token1 = (min(row0 + min(a.rows, rows - row0), rows) - 1) / a.group;
+  const KeyRange oldest = visible(q.length - q.count + token0, q.length, a.causal, a.window);
+  const KeyRange newest = visible(q.length - q.count + token1, q.length, a.causal, a.window);
+  const int first = oldest.lo / a.keys, end = (newest.hi + a.keys - 1) / a.keys;
+  return {first, max(end - first, 1)};
+}
+
+// One sequence's share of the line: blocks per key head (0: nothing to do) and steps of one head's blocks.
 struct Share {
-  int blocks;      // blocks of query rows per key head (0: nothing to do)
-  int first_step;  // key step where its units start
-  int steps;       // steps of each unit
+  int blocks;
+  int64_t per_head;
 };
 __device__ __forceinline__ Share share_of(const LineArgs& a, const Sequence& q) {
   const int rows = q.count * a.group;
-  if (rows == 0 || (a.max_rows > 0 && rows > a.max_rows)) return {0, 0, 0};
-  // the first new token sees the oldest keys
-  const int lo = a.window > 0 ? visible(q.length - q.count, q.length, true, a.window).lo : 0;
-  const int first = lo / a.keys, end = (q.length + a.keys - 1) / a.keys;
-  return {(rows + a.rows - 1) / a.rows, first, max(end - first, 1)};
-}
-__device__ __forceinline__ int64_t work_of(const LineArgs& a, const Share& h) {
-  return int64_t(h.blocks) * a.kv_heads * h.steps;
+  if (rows == 0 || rows < a.min_rows || rows > a.max_rows) return {0, 0};
+  const int blocks = rows <= a.rows ? 1 : (rows + a.rows - 1) / a.rows;
+  int64_t sum = 0;
+  for (int b = 0; b < blocks; ++b) sum += steps_of(a, q, b).count;
+  return {blocks, sum};
 }
 
 // Whole-block sums for blocks of NT threads (NT a multiple of 32, at most 1024).
@@ -62,37 +72,171 @@ __device__ __forceinline__ int64_t block_inclusive_scan(int64_t v, BlockScan<NT>
   return v + before;
 }
 
+// A step of the line: its unit and how many of the unit's steps lie in front of it.
+struct Place {
+  int sequence, head, block, inside;
+};
 template <int NT>
-__device__ __forceinline__ int64_t line_total(const LineArgs& a, BlockScan<NT>& s) {
+struct LineShared {
+  BlockScan<NT> scan;
+  int sequence;
+  int64_t offset, per_head;
+};
+
+template <int NT>
+__device__ __forceinline__ int64_t line_total(const LineArgs& a, LineShared<NT>& s) {
   int64_t sum = 0, total;
-  for (int i = threadIdx.x; i < a.step.batch; i += NT) sum += work_of(a, share_of(a, sequence_of(a.step, i)));
-  block_inclusive_scan<NT>(sum, s, total);
+  for (int i = threadIdx.x; i < a.step.batch; i += NT) sum += share_of(a, sequence_of(a.step, i)).per_head * a.kv_heads;
+  block_inclusive_scan<NT>(sum, s.scan, total);
   return total;
 }
 
-// Where `at` (inside the line) lies: its sequence and the distance from where that sequence starts.
-struct Place {
-  int sequence;
-  int64_t offset;
-};
+// Where step `at` (inside the line) lies; every thread of the block calls it.
 template <int NT>
-__device__ __forceinline__ Place line_place(const LineArgs& a, int64_t at, BlockScan<NT>& s, Place& shared) {
+__device__ __forceinline__ Place line_place(const LineArgs& a, int64_t at, LineShared<NT>& s) {
   int64_t base = 0;
   for (int i0 = 0; i0 < a.step.batch; i0 += NT) {
     const int i = i0 + threadIdx.x;
-    const int64_t w = i < a.step.batch ? work_of(a, share_of(a, sequence_of(a.step, i))) : 0;
+    const int64_t per_head = i < a.step.batch ? share_of(a, sequence_of(a.step, i)).per_head : 0;
     int64_t total;
-    const int64_t through = base + block_inclusive_scan<NT>(w, s, total);
-    if (through - w <= at && at < through) shared = {i, at - (through - w)};
+    const int64_t w = per_head * a.kv_heads, through = base + block_inclusive_scan<NT>(w, s.scan, total);
+    if (through - w <= at && at < through) {
+      s.sequence = i;
+      s.offset = at - (through - w);
+      s.per_head = per_head;
+    }
     base += total;
     if (base > at) break;
   }
   __syncthreads();
-  return shared;
+  Place p{s.sequence, int(s.offset / s.per_head), 0, 0};
+  int64_t rest = s.offset - p.head * s.per_head;
+  const Sequence q = sequence_of(a.step, p.sequence);
+  for (;; ++p.block) {
+    const int count = steps_of(a, q, p.block).count;
+    if (rest < count) break;
+    rest -= count;
+  }
+  p.inside = int(rest);
+  __syncthreads();  // the shared words may be written again
+  return p;
 }
 
 // Border of worker c on a line of w steps.
 __device__ __forceinline__ int64_t border(int64_t w, int c, int workers) { return w * c / workers; }
+__device__ __forceinline__ int workers_of(int64_t w, int most, int min_steps) {
+  return int(min(int64_t(most), (w + min_steps - 1) / min_steps));
+}
+
+// What a worker does next: steps [first, first + count) of one block; whole: all of the block's, opens: its
+// first ones.
+struct Piece {
+  Sequence seq;
+  int sequence, head, block;
+  int first, count;
+  bool whole, opens;
+};
+// Walks the pieces of one worker; every role of a CTA keeps a walk of its own.
+struct Pieces {
+  int64_t left;  // steps to go
+  Place at;
+  __device__ __forceinline__ bool next(const LineArgs& a, Piece& p) {
+    if (left <= 0) return false;
+    p.seq = sequence_of(a.step, at.sequence);
+    int rows = p.seq.count * a.group;
+    while (at.block * int64_t(a.rows) >= rows || rows < a.min_rows || rows > a.max_rows) {
+      at.block = 0;
+      if (++at.head >= a.kv_heads || rows == 0 || rows < a.min_rows || rows > a.max_rows) {
+        at.head = 0;
+        ++at.sequence;  // the line has steps left, so a sequence with work follows
+        p.seq = sequence_of(a.step, at.sequence);
+        rows = p.seq.count * a.group;
+      }
+    }
+    const StepRange range = steps_of(a, p.seq, at.block);
+    p.sequence = at.sequence;
+    p.head = at.head;
+    p.block = at.block;
+    p.first = range.first + at.inside;
+    p.count = int(min(int64_t(range.count - at.inside), left));
+    p.opens = at.inside == 0;
+    p.whole = p.count == range.count;
+    left -= p.count;
+    at.inside += p.count;
+    if (at.inside == range.count) {
+      at.inside = 0;
+      ++at.block;
+    }
+    return true;
+  }
+};
+
+// ---- joining the parts of a cut unit ------------------------------------------------------------------------
+// A slot holds a part's unnormalised output [rows][head_dim], its maxima [rows] (in units of log 2) and its sums
+// [rows].  A worker's first slot takes a part of a unit that began before it, its second a unit's first part.
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// Where a running maximum starts: below every score (in units of log 2) that 16-bit operands of use produce,
+// and finite, so that a row that has seen nothing yet needs no case of its own.
+constexpr float kNoMaximum = -1e30f;
+
+struct JoinArgs {
+  LineArgs line;
+  const float* parts;
+  int max_workers, min_steps;
+  void* out;
+  int64_t on, oh;
+  float* lse;
+};
+__host__ __device__ __forceinline__ int64_t slot_floats(int rows, int head_dim) { return int64_t(rows) * (head_dim + 2); }
+
+// Borders are grid x, groups of four rows (a warp each) grid y.  The first border inside a unit joins that unit's
+// parts in the order of their keys, so that results do not depend on which worker ended first.
+template <typename T, int D>
+__global__ __launch_bounds__(128) void join_parts_kernel(const JoinArgs a) {
+  __shared__ LineShared<128> shared;
+  chain_wait();
+  chain_release();
+  const int64_t total = line_total<128>(a.line, shared);
+  const int workers = workers_of(total, a.max_workers, a.min_steps), c = blockIdx.x, R = a.line.rows;
+  if (c + 1 >= workers) return;
+  const int64_t edge = border(total, c + 1, workers), previous = border(total, c, workers);
+  const Place place = line_place<128>(a.line, edge, shared);
+  const Sequence seq = sequence_of(a.line.step, place.sequence);
+  const int64_t unit_start = edge - place.inside, unit_end = unit_start + steps_of(a.line, seq, place.block).count;
+  if (place.inside == 0 || previous > unit_start) return;  // no unit is cut here, or an earlier border joins it
+  const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, row = place.block * R + r;
+  if (r >= R || row >= seq.count * a.line.group) return;
+  int parts = 1;
+  while (c + parts < workers && border(total, c + parts, workers) < unit_end) ++parts;
+  const int64_t slot = slot_floats(R, D);
+  auto slot_of = [&](int i) { return a.parts + (int64_t(c + i) * 2 + (i == 0 ? 1 : 0)) * slot; };
+  float top = kNoMaximum;
+  for (int i = lane; i < parts; i += 32) top = fmaxf(top, slot_of(i)[R * D + r]);
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+  constexpr int PER = D / 32;
+  float sum[PER] = {}, norm = 0.f;
+#pragma unroll 8
+  for (int i = 0; i < parts; ++i) {
+    const float* s = slot_of(i);
+    const float f = ex2_approx(s[R * D + r] - top);
+    norm += f * s[R * D + R + r];
+#pragma unroll
+    for (int e = 0; e < PER / 2; ++e) {
+      const float2 x = *reinterpret_cast<const float2*>(s + r * D + e * 64 + lane * 2);
+      sum[2 * e] += f * x.x;
+      sum[2 * e + 1] += f * x.y;
+    }
+  }
+  const float f = norm == 0.f ? 0.f : 1.0f / norm;
+  const int token = row / a.line.group, h = place.head * a.line.group + row % a.line.group;
+  T* out = static_cast<T*>(a.out) + int64_t(seq.first + token) * a.on + int64_t(h) * a.oh;
+#pragma unroll
+  for (int e = 0; e < PER / 2; ++e)
+    *reinterpret_cast<uint32_t*>(out + e * 64 + lane * 2) = Half2<T>::pack(sum[2 * e] * f, sum[2 * e + 1] * f);
+  if (lane == 0 && a.lse != nullptr)
+    a.lse[int64_t(seq.first + token) * (a.line.kv_heads * a.line.group) + h] = norm == 0.f ? -INFINITY : top * kLn2 + logf(norm);
+}
 
 }  // namespace serving
 }  // namespace risa_b200

@@ -351,7 +351,7 @@ def assert_weights(b, got, lse, previous=None, **options):
     n terms of one sign adds 2^-24 n at most."""
     want, size = U.weights(b, lse, **options)
     terms = max(b.chunks) * b.q.shape[1]
-    score = size * (b.q.shape[-1] * 2.0 ** -23 + (torch.finfo(b.q.dtype).eps / 16 if b.cache.quantized else 0)) + 2.0 ** -20 * (1 + size)
+    score = size * b.q.shape[-1] * 2.0 ** -23 + 2.0 ** -20 * (1 + size)
     bound = want * (1.1 * score + terms * 2.0 ** -24)
     if previous is not None:
         want = want + previous.double()
