@@ -18,9 +18,9 @@ CSRC = PKG / "csrc"
 OBJ = CSRC / "_obj"
 LIB = PKG / "librisa_b200.so"
 UNITS = ["prep_qk", "prep_v", "misc", "attention_api", "attention_rows", "attention_tc", "cache_ops",
-         "paged_rows", "paged_tc"]
+         "paged_rows", "paged_tc", "weigh_tc"]
 # these share no numeric contract with other kernels: their arithmetic is as written
-EXACT_UNITS = {"cache_ops", "paged_rows", "paged_tc"}
+EXACT_UNITS = {"cache_ops", "paged_rows", "paged_tc", "weigh_tc"}
 # measurement probe (INT8 issue-loop ceiling used by bench.py), its own library
 PROBE_LIB = PKG / "librisa_b200_probe.so"
 PROBE_UNITS = ["mma_peak"]

@@ -19,9 +19,10 @@ unsigned int* status_word() {
 
 // Reports (and clears) what the kernels recorded.
 int device_status() {
-  const int site = paged_tc_wait_status();
+  const int attention_site = paged_tc_wait_status(), weigh_site = weigh_tc_wait_status();
+  const int site = attention_site != 0 ? attention_site : weigh_site;
   if (site < 0) return fail(RISA_B200_CUDA, "device status: %s", cudaGetErrorString(cudaGetLastError()));
-  if (site > 0) return fail(RISA_B200_DEVICE, "paged attention kernel gave up waiting at site %d (bounded wait expired)", site);
+  if (site > 0) return fail(RISA_B200_DEVICE, "kernel over a paged cache gave up waiting at site %d (bounded wait expired)", site);
   unsigned int status = 0, zero = 0;
   if (cudaMemcpyFromSymbol(&status, g_bad_page, sizeof(status)) != cudaSuccess)
     return fail(RISA_B200_CUDA, "device status: %s", cudaGetErrorString(cudaGetLastError()));

@@ -753,12 +753,19 @@ extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const ris
   return bad ? bad : check_launch("paged attention");
 }
 
-extern "C" size_t risa_b200_key_weights_scratch_size(const risa_b200_cache*, const risa_b200_step*, int) { return 0; }
+static bool weighs_on_tensor_cores(const risa_b200_step& step, int group) {
+  return (step.query_offsets == nullptr ? group : int64_t(step.tokens) * group) >= kTcFewestRows;
+}
+
+extern "C" size_t risa_b200_key_weights_scratch_size(const risa_b200_cache* cache, const risa_b200_step* step, int q_heads) {
+  if (cache == nullptr || step == nullptr || cache->kv_heads <= 0 || q_heads <= 0) return 0;
+  return weighs_on_tensor_cores(*step, q_heads / cache->kv_heads) ? weigh_tc_scratch() : 0;
+}
 
 extern "C" int risa_b200_key_weights(const risa_b200_cache* cache, const risa_b200_step* step, const void* q,
                                      const int64_t q_strides[2], int q_heads, int dtype_code, const float* lse, float scale,
-                                     int is_causal, int window, const float* previous, float* weights, void*, size_t,
-                                     void* stream_ptr) {
+                                     int is_causal, int window, const float* previous, float* weights, void* scratch,
+                                     size_t scratch_bytes, void* stream_ptr) {
   if (const int bad = check_queries(cache, step, q, q_strides, q_heads, dtype_code, scale, is_causal, window, "key weights")) return bad;
   RISA_REQUIRE(lse != nullptr && weights != nullptr, "key weights: null tensor");
   unsigned int* status = status_word();
@@ -766,16 +773,37 @@ extern "C" int risa_b200_key_weights(const risa_b200_cache* cache, const risa_b2
   RowsArgs a = rows_args(cache, step, q, q_strides, q_heads, scale, is_causal, window, status);
   const int column_blocks = a.line.rows / 8;
   a.line.rows = 1 << 30;  // all rows of a key head are one unit
+  const bool tensor_cores = weighs_on_tensor_cores(*step, a.line.group);
+  RISA_REQUIRE(!tensor_cores || (scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 16 == 0 && scratch_bytes >= weigh_tc_scratch()),
+               "key weights: the scratch is too small");
+  if (tensor_cores) a.line.max_rows = kTcFewestRows - 1;
+  const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   a.row_lse = lse;
   a.previous = previous;
   a.weights = weights;
-  const int bad = with_tile(dtype_code, cache->dtype_code == kInt8, cache->head_dim, column_blocks, [&](auto tile) {
+  int bad = with_tile(dtype_code, cache->dtype_code == kInt8, cache->head_dim, column_blocks, [&](auto tile) {
     using C = decltype(tile);
     constexpr int bytes = kWarps * Walk<C, false>::STAGE * Walk<C, false>::STAGES;
     if (const int bad = allow_shared(weigh_rows_kernel<C>, bytes, "key weights")) return bad;
     launch_chained(weigh_rows_kernel<C>, dim3(C::D == 256 && !C::INT8 ? kMaxWorkers / 2 : kMaxWorkers), dim3(kThreads), bytes,
-                   static_cast<cudaStream_t>(stream_ptr), a);
+                   stream, a);
     return RISA_B200_OK;
   });
+  if (bad == RISA_B200_OK && tensor_cores) {
+    TcArgs t{};
+    t.line = a.line;
+    t.line.min_rows = kTcFewestRows;
+    t.q = q;
+    t.qn = a.qn;
+    t.qh = a.qh;
+    t.keys = a.keys;
+    t.key_scales = a.key_scales;
+    t.pages = a.pages;
+    t.scale_log2 = a.scale_log2;
+    t.parts = static_cast<float*>(scratch);
+    t.min_steps = 2;
+    t.status = status;
+    bad = weigh_tc(t, lse, previous, weights, dtype_code, cache->dtype_code == kInt8, cache->head_dim, stream);
+  }
   return bad ? bad : check_launch("key weights");
 }

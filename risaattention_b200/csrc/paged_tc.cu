@@ -12,9 +12,7 @@
 // them (and owns tensor memory).  13-15 idle, so that registers can be dealt per warpgroup.
 #include "serving_plan.cuh"
 #include "paged_tc.cuh"
-#include "tc_ptx.cuh"
-
-#include <type_traits>
+#include "tc_f16.cuh"
 
 namespace risa_b200 {
 namespace serving {
@@ -54,66 +52,7 @@ struct Barriers {
   uint64_t q_full[kGroups], s_full[kGroups], p_full[kGroups], o_full[kGroups], o_free[kGroups], drained;
 };
 
-// kind::f16 with fp32 accumulators, M = 128: types of A and B, B's major axis, N.
-template <typename T> __host__ __device__ constexpr uint32_t idesc_f16(bool b_mn_major, int n) {
-  const uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
-  return (1u << 4) | (type << 7) | (type << 10) | ((b_mn_major ? 1u : 0u) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
-}
-// Operand descriptors as a constant upper half and a lower half to which offsets (in units of 16 bytes) are added.
-// Rows of 64 channels are 128 bytes wide and swizzled, eight of them 1024 bytes; the next 64 channels are one block of
-// 128 rows further.  Q and K are read with the MMA's K axis along a row (the leading offset is unused), V with it across
-// the rows (the leading offset leads to the next 64 channels).
-constexpr uint32_t kDescHigh = (1024 >> 4) | 1u << 14 | 2u << 29;
-__device__ __forceinline__ uint64_t descriptor(uint32_t low) { return uint64_t(kDescHigh) << 32 | low; }
-__device__ __forceinline__ uint32_t along_row(uint32_t address) { return (address & 0x3ffffu) >> 4 | 1u << 16; }
-__device__ __forceinline__ uint32_t across_rows(uint32_t address) { return (address & 0x3ffffu) >> 4 | uint32_t(16384 >> 4) << 16; }
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
-      : "memory");
-}
-__device__ __forceinline__ void mma_f16_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
-  asm volatile(
-      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
-      : "memory");
-}
-
-__device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t* r) {
-  asm volatile(
-      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(address),
-      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
-      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-      : "memory");
-}
-
-__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
-}
-__device__ __forceinline__ void store16(uint32_t to, uint4 v) {
-  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
-}
-// Byte offset of the 16-byte piece `piece` of row `row` in a tile of 128 rows.
-__device__ __forceinline__ uint32_t tile_offset(int row, int piece) {
-  return uint32_t((piece >> 3) * 16384 + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
-}
-
-// Two codes of a word (bytes 2 i and 2 i + 1 of `word` with the sign bits flipped) times the scale: 2^23 + u is exact,
-// so the difference to 2^23 + 128 is the code.
-template <typename T>
-__device__ __forceinline__ uint32_t scaled_pair(uint32_t word, int i, float scale) {
-  const float a = __uint_as_float(__byte_perm(word, 0x4b000000u, i ? 0x7442 : 0x7440)) - 8388736.0f;
-  const float b = __uint_as_float(__byte_perm(word, 0x4b000000u, i ? 0x7443 : 0x7441)) - 8388736.0f;
-  return Half2<T>::pack(a * scale, b * scale);
-}
-
 // ---- the fetching warpgroup -----------------------------------------------------------------------------------
-// Page numbers of a tile's eight runs of 16 keys.
-struct TilePages {
-  int id[8];
-};
-
 template <typename C>
 struct Fetcher {
   const TcArgs& a;
@@ -124,88 +63,8 @@ struct Fetcher {
   uint32_t issued;  // tiles so far
   RingPos<C::STAGES> k, v;
 
-  __device__ __forceinline__ TilePages look_up(const int32_t* row, int key0, int low, int length) const {
-    TilePages t;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int key = key0 + 16 * i;
-      t.id[i] = key < length && key + 16 > low ? __ldg(row + (key >> a.line.step.page_shift)) : -1;
-    }
-    return t;
-  }
-  // Runs of the tile whose page is outside the pool although a key of theirs exists.
-  __device__ __forceinline__ uint32_t bad_runs(const TilePages& t, int key0, int low, int length) const {
-    uint32_t bad = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int key = key0 + 16 * i;
-      if (key < length && key + 16 > low && (t.id[i] < 0 || t.id[i] >= a.pages)) bad |= 1u << i;
-    }
-    return bad;
-  }
-  __device__ __forceinline__ int64_t line_of(const TilePages& t, int i, int key0, int head) const {
-    return ((int64_t(t.id[i]) * a.line.kv_heads + head) << a.line.step.page_shift) + ((key0 + 16 * i) & ((1 << a.line.step.page_shift) - 1));
-  }
   __device__ __forceinline__ bool wait_stage(uint64_t* empty, int stage, uint32_t phase, unsigned site) const {
     return mbar_wait(smem_u32(empty + stage), phase ^ 1, gave_up, site);
-  }
-};
-
-// 16-bit rows: 16 bytes at a time straight into place; rows that are not there become zeros (a stale NaN in V would
-// spoil the product with a probability of 0).
-template <typename C>
-__device__ __forceinline__ void copy_tile(const Fetcher<C>& f, const char* pool, uint32_t to, const TilePages& t, uint32_t bad,
-                                          int key0, int low, int length, int head) {
-  constexpr int PIECES = C::D / 8;              // of a row
-  constexpr int PER_RUN = 16 * PIECES / 128;    // pieces of a run of 16 rows per thread
-#pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const bool run = !(bad >> i & 1) && t.id[i] >= 0;
-    const char* from = pool + (run ? f.line_of(t, i, key0, head) * (C::D * 2) : 0);
-#pragma unroll
-    for (int j = 0; j < PER_RUN; ++j) {
-      const int index = j * 128 + f.p, r = index / PIECES, piece = index % PIECES, key = key0 + 16 * i + r;
-      copy16(to + tile_offset(16 * i + r, piece), from + index * 16, run && key >= low && key < length);
-    }
-  }
-}
-
-// Codes: 16 of them per load, times their row's scale, rounded to the queries' type (half a step, as if the cache had
-// held 16-bit values), written as two pieces.
-template <typename C>
-struct CodeTile {
-  static constexpr int PIECES = C::D / 16, LOADS = 128 * PIECES / 128;
-  uint4 codes[LOADS];
-  float scale[LOADS];
-  __device__ __forceinline__ void load(const Fetcher<C>& f, const char* pool, const float* scales, const TilePages& t, uint32_t bad,
-                                       int key0, int low, int length, int head) {
-#pragma unroll
-    for (int n = 0; n < LOADS; ++n) {
-      const int index = n * 128 + f.p, row = index / PIECES, piece = index % PIECES, i = row >> 4, key = key0 + row;
-      // the run of a load is a constant where a run takes whole loads (64 channels: two runs per load)
-      const int run0 = n * 128 / PIECES >> 4;
-      const int id = 128 / PIECES <= 16 ? t.id[run0] : (i == run0 ? t.id[run0] : t.id[run0 + 1 < 8 ? run0 + 1 : 7]);
-      const bool there = !(bad >> i & 1) && id >= 0 && key >= low && key < length;
-      const int64_t line = ((int64_t(id) * f.a.line.kv_heads + head) << f.a.line.step.page_shift) + (key & ((1 << f.a.line.step.page_shift) - 1));
-      codes[n] = there ? *reinterpret_cast<const uint4*>(pool + line * C::D + piece * 16) : make_uint4(0, 0, 0, 0);
-      scale[n] = there ? scales[line] : 0.f;
-    }
-  }
-  __device__ __forceinline__ void store(const Fetcher<C>& f, uint32_t to) const {
-#pragma unroll
-    for (int n = 0; n < LOADS; ++n) {
-      const int index = n * 128 + f.p, row = index / PIECES, piece = index % PIECES;
-      const uint32_t w[4] = {codes[n].x ^ 0x80808080u, codes[n].y ^ 0x80808080u, codes[n].z ^ 0x80808080u, codes[n].w ^ 0x80808080u};
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        uint4 v;
-        v.x = scaled_pair<typename C::T>(w[2 * h], 0, scale[n]);
-        v.y = scaled_pair<typename C::T>(w[2 * h], 1, scale[n]);
-        v.z = scaled_pair<typename C::T>(w[2 * h + 1], 0, scale[n]);
-        v.w = scaled_pair<typename C::T>(w[2 * h + 1], 1, scale[n]);
-        store16(to + tile_offset(row, 2 * piece + h), v);
-      }
-    }
   }
 };
 
@@ -236,29 +95,32 @@ __device__ __forceinline__ void fetch_tiles(Fetcher<C>& f, Pieces pieces) {
     const int32_t* row = a.line.step.table + int64_t(piece.sequence) * a.line.step.width;
     const int length = piece.seq.length;
     const int low = a.line.window > 0 ? visible(piece.seq.length - piece.seq.count, length, true, a.line.window).lo : 0;
-    TilePages ahead = f.look_up(row, piece.first * kTileKeys, low, length);
+    const PoolView keys{a.keys, a.key_scales, a.line.kv_heads, a.line.step.page_shift}, values{a.values, a.value_scales, a.line.kv_heads, a.line.step.page_shift};
+    KeyRuns ahead;
+    ahead.look_up(row, a.line.step.page_shift, piece.first * kTileKeys, low, length);
     for (int i = 0; i < piece.count; ++i) {
       const int key0 = (piece.first + i) * kTileKeys;
-      const TilePages t = ahead;
-      if (i + 1 < piece.count) ahead = f.look_up(row, key0 + kTileKeys, low, length);
-      const uint32_t bad = f.bad_runs(t, key0, low, length);
+      const KeyRuns t = ahead;
+      if (i + 1 < piece.count) ahead.look_up(row, a.line.step.page_shift, key0 + kTileKeys, low, length);
+      const uint32_t bad = t.bad(a.pages);
       const uint32_t note = bad | (i == 0 ? kFirst : 0u) | (i + 1 == piece.count ? kLast : 0u) |
                             (piece.seq.count * a.line.group - piece.block * kRows > 128 ? kTwoGroups : 0u);
       const uint32_t k_to = f.k_ring + f.k.stage * C::SIDE, v_to = f.v_ring + f.v.stage * C::SIDE;
       if constexpr (C::INT8) {
-        CodeTile<C> codes;
-        codes.load(f, a.keys, a.key_scales, t, bad, key0, low, length, piece.head);
+        // scaled and rounded to the queries' type (half a step), as if the cache had held 16-bit values
+        CodeTile<typename C::T, C::D, true> codes;
+        codes.load(keys, t, bad, piece.head, f.p);
         if (!f.wait_stage(f.bars->k_empty, f.k.stage, f.k.phase, 1001)) return;
         if (f.p == 0) {
           f.notes[f.issued % kNotes] = note;
           if (bad) atomicCAS(a.status, 0u, unsigned(piece.sequence) + 1u);
         }
-        codes.store(f, k_to);
+        codes.store(k_to, f.p);
         fence_async_smem();
         mbar_arrive(smem_u32(f.bars->k_full + f.k.stage));
-        codes.load(f, a.values, a.value_scales, t, bad, key0, low, length, piece.head);
+        codes.load(values, t, bad, piece.head, f.p);
         if (!f.wait_stage(f.bars->v_empty, f.v.stage, f.v.phase, 1002)) return;
-        codes.store(f, v_to);
+        codes.store(v_to, f.p);
         fence_async_smem();
         mbar_arrive(smem_u32(f.bars->v_full + f.v.stage));
       } else {
@@ -267,12 +129,12 @@ __device__ __forceinline__ void fetch_tiles(Fetcher<C>& f, Pieces pieces) {
           f.notes[f.issued % kNotes] = note;
           if (bad) atomicCAS(a.status, 0u, unsigned(piece.sequence) + 1u);
         }
-        copy_tile<C>(f, a.keys, k_to, t, bad, key0, low, length, piece.head);
+        copy_keys<C::D>(keys, t, bad, piece.head, k_to, f.p);
         asm volatile("cp.async.commit_group;" ::: "memory");
         ++owed;
         settle(false);
         if (!f.wait_stage(f.bars->v_empty, f.v.stage, f.v.phase, 1002)) break;
-        copy_tile<C>(f, a.values, v_to, t, bad, key0, low, length, piece.head);
+        copy_keys<C::D>(values, t, bad, piece.head, v_to, f.p);
         asm volatile("cp.async.commit_group;" ::: "memory");
         ++owed;
         settle(false);

@@ -31,5 +31,11 @@ int paged_tc_rows();
 int paged_tc(TcArgs args, int dtype_code, bool codes, int head_dim, cudaStream_t stream);
 int paged_tc_wait_status();
 
+// Key weights (weigh_tc.cu); `out`, `lse` and `values` of the arguments are not used.
+size_t weigh_tc_scratch();
+int weigh_tc(const TcArgs& args, const float* row_lse, const float* previous, float* weights, int dtype_code, bool codes, int head_dim,
+             cudaStream_t stream);
+int weigh_tc_wait_status();
+
 }  // namespace serving
 }  // namespace risa_b200

@@ -19,31 +19,34 @@ struct LineArgs {
   int causal, window;
 };
 
-// Key steps [first, first + count) of a block: those with a key that one of its rows sees, at least one.
+// Steps [first, first + count) of a block.
 struct StepRange {
   int first, count;
 };
+// How many blocks a sequence has per key head (0: nothing to do).  The functions of a line that know what its
+// blocks and steps are: blocks_of and steps_of; here blocks of query rows and steps of keys.
+__device__ __forceinline__ int blocks_of(const LineArgs& a, const Sequence& q) {
+  const int rows = q.count * a.group;
+  if (rows == 0 || rows < a.min_rows || rows > a.max_rows) return 0;
+  return rows <= a.rows ? 1 : (rows + a.rows - 1) / a.rows;
+}
+// The key steps with a key that one of the block's rows sees, at least one.
 __device__ __forceinline__ StepRange steps_of(const LineArgs& a, const Sequence& q, int block) {
   const int rows = q.count * a.group, row0 = block * a.rows;
-  const int token0 = row0 / a.group, token1 = (min(row0 + min(a.rows, rows - row0), rows) - 1) / a.group;
+  const int token0 = row0 / a.group, token1 = (row0 + min(a.rows, rows - row0) - 1) / a.group;
   const KeyRange oldest = visible(q.length - q.count + token0, q.length, a.causal, a.window);
   const KeyRange newest = visible(q.length - q.count + token1, q.length, a.causal, a.window);
   const int first = oldest.lo / a.keys, end = (newest.hi + a.keys - 1) / a.keys;
   return {first, max(end - first, 1)};
 }
 
-// One sequence's share of the line: blocks per key head (0: nothing to do) and steps of one head's blocks.
-struct Share {
-  int blocks;
-  int64_t per_head;
-};
-__device__ __forceinline__ Share share_of(const LineArgs& a, const Sequence& q) {
-  const int rows = q.count * a.group;
-  if (rows == 0 || rows < a.min_rows || rows > a.max_rows) return {0, 0};
-  const int blocks = rows <= a.rows ? 1 : (rows + a.rows - 1) / a.rows;
+// Steps of one key head's blocks.
+template <typename L>
+__device__ __forceinline__ int64_t head_steps(const L& a, const Sequence& q) {
+  const int blocks = blocks_of(a, q);
   int64_t sum = 0;
   for (int b = 0; b < blocks; ++b) sum += steps_of(a, q, b).count;
-  return {blocks, sum};
+  return sum;
 }
 
 // Whole-block sums for blocks of NT threads (NT a multiple of 32, at most 1024).
@@ -83,21 +86,21 @@ struct LineShared {
   int64_t offset, per_head;
 };
 
-template <int NT>
-__device__ __forceinline__ int64_t line_total(const LineArgs& a, LineShared<NT>& s) {
+template <int NT, typename L>
+__device__ __forceinline__ int64_t line_total(const L& a, LineShared<NT>& s) {
   int64_t sum = 0, total;
-  for (int i = threadIdx.x; i < a.step.batch; i += NT) sum += share_of(a, sequence_of(a.step, i)).per_head * a.kv_heads;
+  for (int i = threadIdx.x; i < a.step.batch; i += NT) sum += head_steps(a, sequence_of(a.step, i)) * a.kv_heads;
   block_inclusive_scan<NT>(sum, s.scan, total);
   return total;
 }
 
 // Where step `at` (inside the line) lies; every thread of the block calls it.
-template <int NT>
-__device__ __forceinline__ Place line_place(const LineArgs& a, int64_t at, LineShared<NT>& s) {
+template <int NT, typename L>
+__device__ __forceinline__ Place line_place(const L& a, int64_t at, LineShared<NT>& s) {
   int64_t base = 0;
   for (int i0 = 0; i0 < a.step.batch; i0 += NT) {
     const int i = i0 + threadIdx.x;
-    const int64_t per_head = i < a.step.batch ? share_of(a, sequence_of(a.step, i)).per_head : 0;
+    const int64_t per_head = i < a.step.batch ? head_steps(a, sequence_of(a.step, i)) : 0;
     int64_t total;
     const int64_t w = per_head * a.kv_heads, through = base + block_inclusive_scan<NT>(w, s.scan, total);
     if (through - w <= at && at < through) {
@@ -140,17 +143,18 @@ struct Piece {
 struct Pieces {
   int64_t left;  // steps to go
   Place at;
-  __device__ __forceinline__ bool next(const LineArgs& a, Piece& p) {
+  template <typename L>
+  __device__ __forceinline__ bool next(const L& a, Piece& p) {
     if (left <= 0) return false;
     p.seq = sequence_of(a.step, at.sequence);
-    int rows = p.seq.count * a.group;
-    while (at.block * int64_t(a.rows) >= rows || rows < a.min_rows || rows > a.max_rows) {
+    int blocks = blocks_of(a, p.seq);
+    while (at.block >= blocks) {
       at.block = 0;
-      if (++at.head >= a.kv_heads || rows == 0 || rows < a.min_rows || rows > a.max_rows) {
+      if (blocks == 0 || ++at.head == a.kv_heads) {
         at.head = 0;
         ++at.sequence;  // the line has steps left, so a sequence with work follows
         p.seq = sequence_of(a.step, at.sequence);
-        rows = p.seq.count * a.group;
+        blocks = blocks_of(a, p.seq);
       }
     }
     const StepRange range = steps_of(a, p.seq, at.block);

@@ -1,0 +1,152 @@
+// 16-bit tensor-core pieces shared by the kernels over a paged cache: operand descriptors, the matrix instructions with
+// fp32 accumulators, tiles in shared memory and what fills them.
+#pragma once
+#include <type_traits>
+
+#include "serving.cuh"
+#include "tc_ptx.cuh"
+
+namespace risa_b200 {
+namespace serving {
+
+// kind::f16 with fp32 accumulators, M = 128: types of A and B, B's major axis, N.
+template <typename T> __host__ __device__ constexpr uint32_t idesc_f16(bool b_mn_major, int n) {
+  const uint32_t type = std::is_same<T, __half>::value ? 0u : 1u;
+  return (1u << 4) | (type << 7) | (type << 10) | ((b_mn_major ? 1u : 0u) << 16) | (uint32_t(n >> 3) << 17) | (uint32_t(128 >> 4) << 24);
+}
+// Operand descriptors as a constant upper half and a lower half to which offsets (in units of 16 bytes) are added.
+// Rows of 64 channels are 128 bytes wide and swizzled, eight of them 1024 bytes; the next 64 channels are one block of
+// 128 rows further.  Q and K are read with the MMA's K axis along a row (the leading offset is unused), V with it across
+// the rows (the leading offset leads to the next 64 channels).
+constexpr uint32_t kDescHigh = (1024 >> 4) | 1u << 14 | 2u << 29;
+__device__ __forceinline__ uint64_t descriptor(uint32_t low) { return uint64_t(kDescHigh) << 32 | low; }
+__device__ __forceinline__ uint32_t along_row(uint32_t address) { return (address & 0x3ffffu) >> 4 | 1u << 16; }
+__device__ __forceinline__ uint32_t across_rows(uint32_t address) { return (address & 0x3ffffu) >> 4 | uint32_t(16384 >> 4) << 16; }
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+// A from tensor memory: two 16-bit values along K per column.
+__device__ __forceinline__ void mma_f16_tmem(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+  asm volatile(
+      "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n}\n" ::"r"(d), "r"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      : "memory");
+}
+
+__device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t* r) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, %16};" ::"r"(address),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]),
+      "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
+      : "memory");
+}
+
+__device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void store16(uint32_t to, uint4 v) {
+  asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
+}
+// Byte offset of the 16-byte piece `piece` of row `row` in a tile of 128 rows.
+__device__ __forceinline__ uint32_t tile_offset(int row, int piece) {
+  return uint32_t((piece >> 3) * 16384 + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
+}
+
+// Codes 2 i and 2 i + 1 of a word whose sign bits have been flipped, times the scale: 2^23 + u is exact, so its
+// difference to 2^23 + 128 is the code.
+template <typename T>
+__device__ __forceinline__ uint32_t scaled_pair(uint32_t word, int i, float scale) {
+  const float a = __uint_as_float(__byte_perm(word, 0x4b000000u, i ? 0x7442 : 0x7440)) - 8388736.0f;
+  const float b = __uint_as_float(__byte_perm(word, 0x4b000000u, i ? 0x7443 : 0x7441)) - 8388736.0f;
+  return Half2<T>::pack(a * scale, b * scale);
+}
+
+// ---- 128 keys of a paged sequence into a tile, by the 128 threads of a warpgroup ----------------------------------------
+// Page numbers of eight runs of 16 keys, and where they lie.
+struct KeyRuns {
+  int id[8];
+  int key0, low, length;  // keys [low, length) exist
+  __device__ __forceinline__ bool exists(int i) const { return key0 + 16 * i < length && key0 + 16 * i + 16 > low; }
+  __device__ __forceinline__ void look_up(const int32_t* row, int page_shift, int first_key, int first_existing, int sequence_length) {
+    key0 = first_key;
+    low = first_existing;
+    length = sequence_length;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) id[i] = exists(i) ? __ldg(row + ((key0 + 16 * i) >> page_shift)) : -1;
+  }
+  // Runs whose page is outside the pool although a key of theirs exists.
+  __device__ __forceinline__ uint32_t bad(int pages) const {
+    uint32_t bits = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+      if (exists(i) && (id[i] < 0 || id[i] >= pages)) bits |= 1u << i;
+    return bits;
+  }
+};
+struct PoolView {
+  const char* rows;
+  const float* scales;
+  int kv_heads, page_shift;
+  // Row of key `key` of a sequence in page `id`.
+  __device__ __forceinline__ int64_t line(int id, int head, int key) const {
+    return ((int64_t(id) * kv_heads + head) << page_shift) + (key & ((1 << page_shift) - 1));
+  }
+};
+
+// 16-bit rows: 16 bytes at a time straight into place; rows that are not there become zeros (a stale NaN in V would spoil
+// the product with a probability of 0).
+template <int D>
+__device__ __forceinline__ void copy_keys(const PoolView& pool, const KeyRuns& k, uint32_t bad, int head, uint32_t to, int thread) {
+  constexpr int PIECES = D / 8;             // of a row
+  constexpr int PER_RUN = 16 * PIECES / 128;  // pieces of a run per thread
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const bool run = !(bad >> i & 1) && k.id[i] >= 0;
+    const char* from = pool.rows + (run ? pool.line(k.id[i], head, k.key0 + 16 * i) * (D * 2) : 0);
+#pragma unroll
+    for (int j = 0; j < PER_RUN; ++j) {
+      const int index = j * 128 + thread, r = index / PIECES, piece = index % PIECES, key = k.key0 + 16 * i + r;
+      copy16(to + tile_offset(16 * i + r, piece), from + index * 16, run && key >= k.low && key < k.length);
+    }
+  }
+}
+
+// Codes: 16 of them per load; `store` multiplies by their row's scale (SCALED) and rounds to T.
+template <typename T, int D, bool SCALED>
+struct CodeTile {
+  static constexpr int PIECES = D / 16, LOADS = PIECES;
+  uint4 codes[LOADS];
+  float scale[SCALED ? LOADS : 1];
+  __device__ __forceinline__ void load(const PoolView& pool, const KeyRuns& k, uint32_t bad, int head, int thread) {
+#pragma unroll
+    for (int n = 0; n < LOADS; ++n) {
+      const int index = n * 128 + thread, row = index / PIECES, piece = index % PIECES, i = row >> 4, key = k.key0 + row;
+      // a load of the warpgroup covers 128 / PIECES rows: one run of 16, or two at 64 channels
+      constexpr int RUNS = 128 / PIECES / 16;
+      const int id = RUNS <= 1 ? k.id[n * 128 / PIECES / 16] : (i == n * 2 ? k.id[(n * 2) & 7] : k.id[(n * 2 + 1) & 7]);
+      const bool there = !(bad >> i & 1) && id >= 0 && key >= k.low && key < k.length;
+      const int64_t line = pool.line(id, head, key);
+      codes[n] = there ? *reinterpret_cast<const uint4*>(pool.rows + line * D + piece * 16) : make_uint4(0, 0, 0, 0);
+      if (SCALED) scale[n] = there ? pool.scales[line] : 0.f;
+    }
+  }
+  __device__ __forceinline__ void store(uint32_t to, int thread) const {
+#pragma unroll
+    for (int n = 0; n < LOADS; ++n) {
+      const int index = n * 128 + thread, row = index / PIECES, piece = index % PIECES;
+      const float s = SCALED ? scale[n] : 1.0f;
+      const uint32_t w[4] = {codes[n].x ^ 0x80808080u, codes[n].y ^ 0x80808080u, codes[n].z ^ 0x80808080u, codes[n].w ^ 0x80808080u};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        store16(to + tile_offset(row, 2 * piece + h),
+                make_uint4(scaled_pair<T>(w[2 * h], 0, s), scaled_pair<T>(w[2 * h], 1, s), scaled_pair<T>(w[2 * h + 1], 0, s),
+                           scaled_pair<T>(w[2 * h + 1], 1, s)));
+    }
+  }
+};
+
+}  // namespace serving
+}  // namespace risa_b200

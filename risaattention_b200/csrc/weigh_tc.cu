@@ -1,0 +1,452 @@
+// The attention that cached keys receive from many query rows, on the tensor cores.
+//
+// With the rows' log-sum-exp known a weight needs no maximum and no order: w_j = sum over rows of 2^(s_rj - lse_r).  So
+// the roles of the attention kernel turn around: 256 keys stay (the A operand, two groups of 128), query rows stream
+// past them (128 at a time, the B operand), scores S = K Q^T arrive with a key per lane of tensor memory, and the
+// thread that owns a key adds up its row of exponentials in a register.  K is read once, nothing is written but the
+// weights.  What bounds it is the exponentials: one per (key, row) and 16 per clock and SM, 2048 clocks for 256 keys x
+// 128 rows, against 1024 of the matrix instruction at 128 channels.
+//
+// Warps 0-3, 4-7: the two groups' sums.  8-11: fetch keys and query rows.  12: issues the products.  13-15 idle.
+#include "paged_tc.cuh"
+#include "tc_f16.cuh"
+
+#include <climits>
+
+namespace risa_b200 {
+namespace serving {
+
+using namespace tc;
+
+namespace {
+
+constexpr int kThreads = 512;
+constexpr int kBlockKeys = 256;
+constexpr int kFetcher = 8, kIssuer = 12;
+// Notes and log-sum-exps of the tiles in flight.  A slot is written again kDepth tiles later, by when the sums have
+// left it: the fetchers are at most the query stages ahead of the issuer, the issuer two tiles ahead of the sums.
+constexpr int kDepth = 8;
+// Bits of a note: first and last tile of a block, whether the block has more than 128 keys, and from kBadRuns on the runs of
+// 16 keys whose page is outside the pool.
+constexpr uint32_t kFirst = 1u, kLast = 2u, kTwoGroups = 4u, kBadRuns = 8;
+
+// Blocks of 256 keys and steps of query rows (serving_plan.cuh's line the other way round).
+struct WeighLine {
+  StepView step;
+  int kv_heads, group, min_rows, tile_rows;
+  int causal, window;
+};
+__device__ __forceinline__ int first_seen(const WeighLine& a, const Sequence& q) {
+  return a.window > 0 ? visible(q.length - q.count, q.length, true, a.window).lo : 0;
+}
+__device__ __forceinline__ int blocks_of(const WeighLine& a, const Sequence& q) {
+  if (q.count == 0 || q.count * a.group < a.min_rows || q.length == 0) return 0;
+  return (q.length + kBlockKeys - 1) / kBlockKeys - first_seen(a, q) / kBlockKeys;
+}
+// Rows [lo, hi) of the sequence that see a key; hi is INT_MAX where no window ends them.
+struct RowRange {
+  int lo, hi;
+};
+__device__ __forceinline__ RowRange rows_of(const WeighLine& a, const Sequence& q, int key) {
+  if (!a.causal) return {0, INT_MAX};
+  const int base = q.length - q.count;  // place of the first new token
+  const int lo = min(max(key - base, 0), q.count) * a.group;
+  if (a.window == 0) return {lo, INT_MAX};
+  const int64_t end = int64_t(key) + a.window - base;
+  return {lo, end <= 0 ? 0 : end >= q.count ? INT_MAX : int(end) * a.group};
+}
+__device__ __forceinline__ StepRange steps_of(const WeighLine& a, const Sequence& q, int block) {
+  const int key0 = (first_seen(a, q) / kBlockKeys + block) * kBlockKeys;
+  const int rows = q.count * a.group, from = rows_of(a, q, key0).lo, to = min(rows_of(a, q, key0 + kBlockKeys - 1).hi, rows);
+  const int first = min(from, rows - 1) / a.tile_rows, end = (to + a.tile_rows - 1) / a.tile_rows;
+  return {first, max(end - first, 1)};
+}
+
+struct WeighArgs {
+  WeighLine line;
+  const void* q;
+  int64_t qn, qh;
+  const float* row_lse;
+  PoolView keys;
+  int pages;
+  float scale_log2;
+  const float* previous;
+  float* weights;
+  float* parts;  // two slots of 256 floats per worker
+  int min_steps;
+  unsigned int* status;
+};
+
+template <typename T_, bool INT8_, int D_>
+struct Shape {
+  using T = T_;
+  static constexpr bool INT8 = INT8_;
+  static constexpr int D = D_;
+  static constexpr int ROWS = D == 256 ? 64 : 128;  // query rows of a tile
+  static constexpr int GROUP = 128 * D * 2;         // 128 keys
+  static constexpr int KEYS = 2 * GROUP, KEY_BUFFERS = D == 256 ? 1 : 2;
+  static constexpr int TILE = ROWS * D * 2, STAGES = D == 64 ? 4 : 2;
+  static constexpr int SMEM = KEY_BUFFERS * KEYS + STAGES * TILE + 1024;
+  static_assert(STAGES + 2 < kDepth, "notes outlive their readers");
+};
+
+struct Barriers {
+  uint64_t k_full[2], k_empty[2], q_full[4], q_empty[4], s_full[2][2], s_free[2][2], drained;
+};
+
+// Byte offset of piece `piece` of row `row` in a tile of ROWS query rows.
+template <int ROWS>
+__device__ __forceinline__ uint32_t query_offset(int row, int piece) {
+  return uint32_t((piece >> 3) * (ROWS * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
+}
+
+struct Notes {
+  uint32_t tile[kDepth];
+  float minus_lse[kDepth][128];  // in units of log 2; -infinity for rows that give nothing
+};
+
+template <typename C>
+__device__ __forceinline__ void fetch(const WeighArgs& a, Pieces pieces, Barriers* bars, volatile Notes* notes, uint32_t keys, uint32_t queries,
+                                      uint32_t gave_up) {
+  const int p = threadIdx.x - kFetcher * 32;
+  RingPos<C::KEY_BUFFERS> kb;
+  RingPos<C::STAGES> st;
+  uint32_t tile = 0;
+  // copy groups under way, oldest first, and the barriers that wait for them
+  uint32_t owed[2] = {0, 0};
+  int count = 0;
+  auto hand_over = [&] {
+    if (count == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
+    else asm volatile("cp.async.wait_group 0;" ::: "memory");
+    fence_async_smem();
+    mbar_arrive(owed[0]);
+    owed[0] = owed[1];
+    --count;
+  };
+  auto close = [&](uint32_t barrier) {
+    asm volatile("cp.async.commit_group;" ::: "memory");
+    owed[count++] = barrier;
+    if (count == 2) hand_over();
+  };
+  Piece piece;
+  bool alive = true;
+  while (alive && pieces.next(a.line, piece)) {
+    const Sequence& seq = piece.seq;
+    const int32_t* row = a.line.step.table + int64_t(piece.sequence) * a.line.step.width;
+    const int low = first_seen(a.line, seq), key0 = (low / kBlockKeys + piece.block) * kBlockKeys, rows = seq.count * a.line.group;
+    // with a single key buffer its block must be read out first, to its last tile
+    if (C::KEY_BUFFERS == 1)
+      while (count > 0) hand_over();
+    if (!mbar_wait(smem_u32(bars->k_empty + kb.stage), kb.phase ^ 1, gave_up, 1101)) break;
+    uint32_t bad = 0;
+#pragma unroll 1
+    for (int g = 0; g < 2; ++g) {
+      KeyRuns runs;
+      runs.look_up(row, a.line.step.page_shift, key0 + 128 * g, low, seq.length);
+      const uint32_t b = runs.bad(a.pages);
+      bad |= b << (8 * g);
+      const uint32_t to = keys + kb.stage * C::KEYS + g * C::GROUP;
+      if constexpr (C::INT8) {
+        // codes as they are: a key's scale multiplies its scores in 32 bits
+        CodeTile<typename C::T, C::D, false> codes;
+        codes.load(a.keys, runs, b, piece.head, p);
+        codes.store(to, p);
+      } else {
+        copy_keys<C::D>(a.keys, runs, b, piece.head, to, p);
+      }
+    }
+    if (p == 0 && bad) atomicCAS(a.status, 0u, unsigned(piece.sequence) + 1u);
+    close(smem_u32(bars->k_full + kb.stage));
+    kb.next();
+    for (int i = 0; i < piece.count; ++i, ++tile) {
+      if (!mbar_wait(smem_u32(bars->q_empty + st.stage), st.phase ^ 1, gave_up, 1102)) {
+        alive = false;
+        break;
+      }
+      const int row0 = (piece.first + i) * C::ROWS;
+      if (p == 0)
+        notes->tile[tile % kDepth] = (i == 0 ? kFirst : 0u) | (i + 1 == piece.count ? kLast : 0u) | (seq.length - key0 > 128 ? kTwoGroups : 0u) | bad << kBadRuns;
+      if (p < C::ROWS) {
+        const int r = row0 + p;
+        float x = -INFINITY;
+        if (r < rows) {
+          const int token = r / a.line.group;
+          x = __ldg(a.row_lse + int64_t(seq.first + token) * (a.line.kv_heads * a.line.group) + piece.head * a.line.group + r - token * a.line.group);
+        }
+        notes->minus_lse[tile % kDepth][p] = x == -INFINITY ? -INFINITY : -x * kLog2e;
+      }
+      constexpr int PIECES = C::D / 8;
+      const uint32_t to = queries + st.stage * C::TILE;
+#pragma unroll 4
+      for (int n = 0; n < C::ROWS * PIECES / 128; ++n) {
+        const int index = n * 128 + p, r = index / PIECES, c = index % PIECES;
+        const bool there = row0 + r < rows;
+        const int token = there ? (row0 + r) / a.line.group : 0, h = there ? row0 + r - token * a.line.group : 0;
+        copy16(to + query_offset<C::ROWS>(r, c),
+               static_cast<const typename C::T*>(a.q) + int64_t(seq.first + token) * a.qn + int64_t(piece.head * a.line.group + h) * a.qh + c * 8, there);
+      }
+      close(smem_u32(bars->q_full + st.stage));
+      st.next();
+    }
+  }
+  while (count > 0) hand_over();
+}
+
+template <typename C>
+__device__ __forceinline__ void issue(int tiles, Barriers* bars, const volatile Notes* notes, uint32_t tmem, uint32_t keys, uint32_t queries,
+                                      uint32_t gave_up) {
+  constexpr uint32_t kScores = idesc_f16<typename C::T>(false, C::ROWS);
+  RingPos<C::KEY_BUFFERS> kb;
+  RingPos<C::STAGES> st;
+  RingPos<2> buffer;
+  const bool elected = elect_one();
+  for (int tile = 0; tile < tiles; ++tile) {
+    if (!mbar_wait(smem_u32(bars->q_full + st.stage), st.phase, gave_up, 1110)) return;
+    const uint32_t note = notes->tile[tile % kDepth];
+    if ((note & kFirst) && !mbar_wait(smem_u32(bars->k_full + kb.stage), kb.phase, gave_up, 1111)) return;
+    const int groups = note & kTwoGroups ? 2 : 1;
+    for (int g = 0; g < 2; ++g) {
+      // both groups' buffers take turns together, so a group that sits out hands its buffer on
+      if (!mbar_wait(smem_u32(&bars->s_free[g][buffer.stage]), buffer.phase ^ 1, gave_up, 1112 + g)) return;
+      tc_fence_after();
+      if (!elected) continue;
+      if (g < groups) {
+        const uint32_t rows_k = along_row(keys + kb.stage * C::KEYS + g * C::GROUP), rows_q = along_row(queries + st.stage * C::TILE);
+#pragma unroll
+        for (int c = 0; c < C::D / 16; ++c)
+          mma_f16(tmem + (g * 2 + buffer.stage) * 128, descriptor(rows_k + (c >> 2) * 1024 + (c & 3) * 2),
+                  descriptor(rows_q + (c >> 2) * (C::ROWS * 8) + (c & 3) * 2), kScores, c > 0);
+      }
+      mma_commit(smem_u32(&bars->s_full[g][buffer.stage]));
+    }
+    if (elected) {
+      mma_commit(smem_u32(bars->q_empty + st.stage));
+      if (note & kLast) mma_commit(smem_u32(bars->k_empty + kb.stage));
+    }
+    if (note & kLast) kb.next();
+    st.next();
+    buffer.next();
+  }
+}
+
+template <typename C>
+__device__ __forceinline__ void add_up(const WeighArgs& a, Pieces pieces, Barriers* bars, uint32_t tmem, int g, const volatile Notes* notes,
+                                       uint32_t minus_lse, uint32_t gave_up) {
+  const int lane = threadIdx.x & 127;
+  const uint32_t columns = tmem + (uint32_t(lane & ~31) << 16) + g * 256;
+  const int slots = a.line.step.width << a.line.step.page_shift;
+  RingPos<2> buffer;
+  uint32_t tile = 0;
+  Piece piece;
+  while (pieces.next(a.line, piece)) {
+    const Sequence& seq = piece.seq;
+    const int low = first_seen(a.line, seq), key0 = (low / kBlockKeys + piece.block) * kBlockKeys + g * 128, key = key0 + lane;
+    const bool takes_part = g == 0 || seq.length - key0 > 0;
+    RowRange mine = rows_of(a.line, seq, key);
+    const int all_lo = rows_of(a.line, seq, key0 + 127).lo, all_hi = rows_of(a.line, seq, key0).hi;
+    bool whole_group = key0 >= low && key0 + 128 <= seq.length;
+    if (key < low || key >= seq.length) mine.hi = 0;
+    float factor = a.scale_log2;
+    if (C::INT8 && key >= low && key < seq.length) {
+      const int id = __ldg(a.line.step.table + int64_t(piece.sequence) * a.line.step.width + (key >> a.line.step.page_shift));
+      if (id >= 0 && id < a.pages) factor *= __ldg(a.keys.scales + a.keys.line(id, piece.head, key));
+    }
+    const uint64_t factor2 = pack_f32x2(factor, factor);
+    uint64_t sum[4] = {0, 0, 0, 0};
+    for (int i = 0; i < piece.count; ++i, ++tile) {
+      if (!mbar_wait(smem_u32(&bars->s_full[g][buffer.stage]), buffer.phase, gave_up, 1120 + g)) return;
+      tc_fence_after();
+      if (i == 0) {
+        const uint32_t bad = notes->tile[tile % kDepth] >> (kBadRuns + 8 * g) & 0xff;
+        if (bad != 0) whole_group = false;
+        if (bad >> (lane >> 4) & 1) mine.hi = 0;
+      }
+      const uint32_t s = columns + buffer.stage * 128, lse = minus_lse + (tile % kDepth) * 512;
+      if (takes_part) {
+        const int row0 = (piece.first + i) * C::ROWS;
+        const bool every = whole_group && row0 >= all_lo && row0 <= all_hi - C::ROWS;
+        uint32_t x[2][32];
+        tmem_load32(s, x[0]);
+#pragma unroll
+        for (int c = 0; c < C::ROWS / 32; ++c) {
+          tmem_load_wait();
+          tmem_regs_ready<32>(x[c & 1]);
+          if (c + 1 < C::ROWS / 32) tmem_load32(s + (c + 1) * 32, x[(c + 1) & 1]);
+          else {
+            tc_fence_before();
+            mbar_arrive_warp(smem_u32(&bars->s_free[g][buffer.stage]));
+          }
+          uint32_t* v = x[c & 1];
+#pragma unroll
+          for (int e = 0; e < 32; e += 4) {
+            uint64_t l01, l23;
+            asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(l01), "=l"(l23) : "r"(lse + (c * 32 + e) * 4) : "memory");
+            float u[4];
+            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), factor2, l01), u[0], u[1]);
+            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), factor2, l23), u[2], u[3]);
+            if (!every) {
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (row0 + c * 32 + e + j < mine.lo || row0 + c * 32 + e + j >= mine.hi) u[j] = -INFINITY;
+            }
+#pragma unroll
+            for (int j = 0; j < 4; ++j) u[j] = ex2_approx(u[j]);
+            sum[e / 2 & 3] = add_f32x2(sum[e / 2 & 3], pack_f32x2(u[0], u[1]));
+            sum[(e / 2 + 1) & 3] = add_f32x2(sum[(e / 2 + 1) & 3], pack_f32x2(u[2], u[3]));
+          }
+        }
+      } else {
+        mbar_arrive_warp(smem_u32(&bars->s_free[g][buffer.stage]));
+      }
+      buffer.next();
+    }
+    float x0, x1, total;
+    unpack_f32x2(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])), x0, x1);
+    total = x0 + x1;
+    if (!piece.whole) {
+      a.parts[(int64_t(blockIdx.x) * 2 + (piece.opens ? 1 : 0)) * kBlockKeys + g * 128 + lane] = total;
+    } else if (key < slots) {
+      const int64_t index = (int64_t(piece.sequence) * a.line.kv_heads + piece.head) * slots + key;
+      a.weights[index] = total + (a.previous != nullptr ? a.previous[index] : 0.f);
+    }
+  }
+}
+
+template <typename C>
+__global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a) {
+  extern __shared__ char smem_raw[];
+  __shared__ Barriers bars;
+  __shared__ LineShared<kThreads> shared;
+  __shared__ uint32_t tmem_base, gave_up_word;
+  __shared__ __align__(16) Notes notes;
+  const int warp = threadIdx.x >> 5;
+  const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
+  const uint32_t keys = smem, queries = keys + C::KEY_BUFFERS * C::KEYS, gave_up = smem_u32(&gave_up_word);
+  if (threadIdx.x == 0) {
+    gave_up_word = 0;
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(bars.k_full + i), 128);
+      mbar_init(smem_u32(bars.k_empty + i), 1);
+      for (int g = 0; g < 2; ++g) {
+        mbar_init(smem_u32(&bars.s_full[g][i]), 1);
+        mbar_init(smem_u32(&bars.s_free[g][i]), 4);
+      }
+    }
+    for (int i = 0; i < 4; ++i) {
+      mbar_init(smem_u32(bars.q_full + i), 128);
+      mbar_init(smem_u32(bars.q_empty + i), 1);
+    }
+    mbar_init(smem_u32(&bars.drained), 1);
+    mbar_init_fence();
+  }
+  chain_wait();
+  chain_release();
+  // what no block covers: in front of the window, behind the length
+  const int slots = a.line.step.width << a.line.step.page_shift;
+  for (int64_t u = blockIdx.x; u < int64_t(a.line.step.batch) * a.line.kv_heads; u += gridDim.x) {
+    const Sequence seq = sequence_of(a.line.step, int(u / a.line.kv_heads));
+    if (seq.count * a.line.group < a.line.min_rows) continue;
+    const int blocks = blocks_of(a.line, seq), block0 = first_seen(a.line, seq) / kBlockKeys;
+    const int from = blocks == 0 ? 0 : block0 * kBlockKeys, to = blocks == 0 ? 0 : min((block0 + blocks) * kBlockKeys, slots);
+    for (int i = threadIdx.x; i < slots - (to - from); i += kThreads) {
+      const int64_t index = u * slots + (i < from ? i : i + (to - from));
+      a.weights[index] = a.previous != nullptr ? a.previous[index] : 0.f;
+    }
+  }
+  const int64_t total = line_total<kThreads>(a.line, shared);
+  const int workers = workers_of(total, gridDim.x, a.min_steps);
+  if (int(blockIdx.x) >= workers) return;
+  const int64_t begin = border(total, blockIdx.x, workers);
+  const Pieces pieces{border(total, blockIdx.x + 1, workers) - begin, line_place<kThreads>(a.line, begin, shared)};
+  if (warp == kIssuer) tmem_alloc(smem_u32(&tmem_base), 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base;
+  if (warp < kFetcher) {
+    add_up<C>(a, pieces, &bars, tmem, warp >> 2, &notes, smem_u32(&notes.minus_lse[0][0]), gave_up);
+  } else if (warp < kIssuer) {
+    fetch<C>(a, pieces, &bars, &notes, keys, queries, gave_up);
+  } else if (warp == kIssuer) {
+    issue<C>(int(pieces.left), &bars, &notes, tmem, keys, queries, gave_up);
+    __syncwarp();
+    // nothing of this CTA is in flight when tensor memory is handed back, also after a wait that ran out
+    if (elect_one()) mma_commit(smem_u32(&bars.drained));
+    __syncwarp();
+    mbar_drain(smem_u32(&bars.drained), 0);
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  if (warp == kIssuer) tmem_dealloc(tmem, 512);
+  if (gave_up_word != 0 && threadIdx.x < kBlockKeys) {
+    // a wait ran out: this worker's weights are marked
+    Pieces all = pieces;
+    Piece piece;
+    while (all.next(a.line, piece)) {
+      const int key = (first_seen(a.line, piece.seq) / kBlockKeys + piece.block) * kBlockKeys + threadIdx.x;
+      if (!piece.whole) a.parts[(int64_t(blockIdx.x) * 2 + (piece.opens ? 1 : 0)) * kBlockKeys + threadIdx.x] = NAN;
+      else if (key < slots) a.weights[(int64_t(piece.sequence) * a.line.kv_heads + piece.head) * slots + key] = NAN;
+    }
+  }
+}
+
+// One CTA per border between two workers: the first border inside a block of keys adds up its parts in order.
+__global__ __launch_bounds__(kBlockKeys) void join_weights_kernel(const WeighArgs a, int max_workers) {
+  __shared__ LineShared<kBlockKeys> shared;
+  chain_wait();
+  chain_release();
+  const int64_t total = line_total<kBlockKeys>(a.line, shared);
+  const int workers = workers_of(total, max_workers, a.min_steps), c = blockIdx.x;
+  if (c + 1 >= workers) return;
+  const int64_t edge = border(total, c + 1, workers), previous = border(total, c, workers);
+  const Place place = line_place<kBlockKeys>(a.line, edge, shared);
+  const Sequence seq = sequence_of(a.line.step, place.sequence);
+  const int64_t start = edge - place.inside, end = start + steps_of(a.line, seq, place.block).count;
+  if (place.inside == 0 || previous > start) return;
+  float sum = a.parts[(int64_t(c) * 2 + 1) * kBlockKeys + threadIdx.x];
+  for (int i = 1; c + i < workers && border(total, c + i, workers) < end; ++i) sum += a.parts[int64_t(c + i) * 2 * kBlockKeys + threadIdx.x];
+  const int slots = a.line.step.width << a.line.step.page_shift;
+  const int key = (first_seen(a.line, seq) / kBlockKeys + place.block) * kBlockKeys + threadIdx.x;
+  if (key >= slots) return;
+  const int64_t index = (int64_t(place.sequence) * a.line.kv_heads + place.head) * slots + key;
+  a.weights[index] = sum + (a.previous != nullptr ? a.previous[index] : 0.f);
+}
+
+template <typename C>
+int launch(WeighArgs a, cudaStream_t stream) {
+  a.line.tile_rows = C::ROWS;
+  if (cudaFuncSetAttribute(weigh_tc_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
+    return fail(RISA_B200_CUDA, "key weights: %s", cudaGetErrorString(cudaGetLastError()));
+  launch_chained(weigh_tc_kernel<C>, dim3(kTcWorkers), dim3(kThreads), C::SMEM, stream, a);
+  launch_chained(join_weights_kernel, dim3(kTcWorkers - 1), dim3(kBlockKeys), 0, stream, a, kTcWorkers);
+  return RISA_B200_OK;
+}
+template <typename T>
+int launch_for(const WeighArgs& a, bool codes, int head_dim, cudaStream_t stream) {
+  if (head_dim == 64) return codes ? launch<Shape<T, true, 64>>(a, stream) : launch<Shape<T, false, 64>>(a, stream);
+  if (head_dim == 128) return codes ? launch<Shape<T, true, 128>>(a, stream) : launch<Shape<T, false, 128>>(a, stream);
+  return codes ? launch<Shape<T, true, 256>>(a, stream) : launch<Shape<T, false, 256>>(a, stream);
+}
+
+}  // namespace
+
+size_t weigh_tc_scratch() { return size_t(kTcWorkers) * 2 * kBlockKeys * sizeof(float); }
+
+int weigh_tc(const TcArgs& t, const float* row_lse, const float* previous, float* weights, int dtype_code, bool codes, int head_dim,
+             cudaStream_t stream) {
+  const WeighArgs a{{t.line.step, t.line.kv_heads, t.line.group, t.line.min_rows, 0, t.line.causal, t.line.window},
+                    t.q, t.qn, t.qh, row_lse, {t.keys, t.key_scales, t.line.kv_heads, t.line.step.page_shift}, t.pages, t.scale_log2,
+                    previous, weights, t.parts, t.min_steps, t.status};
+  return dtype_code == 1 ? launch_for<__half>(a, codes, head_dim, stream) : launch_for<__nv_bfloat16>(a, codes, head_dim, stream);
+}
+
+int weigh_tc_wait_status() {
+  unsigned int status = 0, zero = 0;
+  if (cudaMemcpyFromSymbol(&status, g_wait_status, sizeof(status)) != cudaSuccess) return -1;
+  if (status != 0) cudaMemcpyToSymbol(g_wait_status, &zero, sizeof(zero));
+  return int(status);
+}
+
+}  // namespace serving
+}  // namespace risa_b200
