@@ -665,7 +665,8 @@ RowsArgs rows_args(const risa_b200_cache* cache, const risa_b200_step* step, con
                    float scale, int is_causal, int window, unsigned int* status) {
   RowsArgs a{};
   const int group = q_heads / cache->kv_heads;
-  a.line = {view_of(*step, cache->page_size), cache->kv_heads, group, 8 * column_blocks_of(*step, group), 1, INT_MAX, 16, is_causal != 0, window};
+  a.line = {view_of(*step, cache->page_size), cache->kv_heads, Divisor(group), Divisor(8 * column_blocks_of(*step, group)), 1, INT_MAX, Divisor(16),
+            is_causal != 0, window};
   a.q = q;
   a.qn = qs[0];
   a.qh = qs[1];
@@ -772,7 +773,7 @@ extern "C" int risa_b200_key_weights(const risa_b200_cache* cache, const risa_b2
   if (status == nullptr) return RISA_B200_CUDA;
   RowsArgs a = rows_args(cache, step, q, q_strides, q_heads, scale, is_causal, window, status);
   const int column_blocks = a.line.rows / 8;
-  a.line.rows = 1 << 30;  // all rows of a key head are one unit
+  a.line.rows = Divisor(1 << 30);  // all rows of a key head are one unit
   const bool tensor_cores = weighs_on_tensor_cores(*step, a.line.group);
   RISA_REQUIRE(!tensor_cores || (scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 16 == 0 && scratch_bytes >= weigh_tc_scratch()),
                "key weights: the scratch is too small");

@@ -72,25 +72,6 @@ template <typename C>
 __device__ __forceinline__ void fetch_tiles(Fetcher<C>& f, Pieces pieces) {
   const TcArgs& a = f.a;
   Piece piece;
-  // cp.async groups in flight whose arrival is still owed: K and V alternate, at most two
-  int owed = 0, owed_k = 0, owed_v = 0;
-  bool next_is_k = true;
-  auto settle = [&](bool all) {  // the oldest group (or all of them) has landed: hand it over
-    while (owed > (all ? 0 : 1)) {
-      if (owed >= 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-      else asm volatile("cp.async.wait_group 0;" ::: "memory");
-      fence_async_smem();
-      if (next_is_k) {
-        mbar_arrive(smem_u32(f.bars->k_full + owed_k));
-        owed_k = owed_k + 1 == C::STAGES ? 0 : owed_k + 1;
-      } else {
-        mbar_arrive(smem_u32(f.bars->v_full + owed_v));
-        owed_v = owed_v + 1 == C::STAGES ? 0 : owed_v + 1;
-      }
-      next_is_k = !next_is_k;
-      --owed;
-    }
-  };
   while (pieces.next(a.line, piece)) {
     const int32_t* row = a.line.step.table + int64_t(piece.sequence) * a.line.step.width;
     const int length = piece.seq.length;
@@ -111,10 +92,6 @@ __device__ __forceinline__ void fetch_tiles(Fetcher<C>& f, Pieces pieces) {
         CodeTile<typename C::T, C::D, true> codes;
         codes.load(keys, t, bad, piece.head, f.p);
         if (!f.wait_stage(f.bars->k_empty, f.k.stage, f.k.phase, 1001)) return;
-        if (f.p == 0) {
-          f.notes[f.issued % kNotes] = note;
-          if (bad) atomicCAS(a.status, 0u, unsigned(piece.sequence) + 1u);
-        }
         codes.store(k_to, f.p);
         fence_async_smem();
         mbar_arrive(smem_u32(f.bars->k_full + f.k.stage));
@@ -124,28 +101,24 @@ __device__ __forceinline__ void fetch_tiles(Fetcher<C>& f, Pieces pieces) {
         fence_async_smem();
         mbar_arrive(smem_u32(f.bars->v_full + f.v.stage));
       } else {
-        if (!f.wait_stage(f.bars->k_empty, f.k.stage, f.k.phase, 1001)) break;
-        if (f.p == 0) {
-          f.notes[f.issued % kNotes] = note;
-          if (bad) atomicCAS(a.status, 0u, unsigned(piece.sequence) + 1u);
-        }
+        if (!f.wait_stage(f.bars->k_empty, f.k.stage, f.k.phase, 1001)) return copies_drain();
         copy_keys<C::D>(keys, t, bad, piece.head, k_to, f.p);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        ++owed;
-        settle(false);
-        if (!f.wait_stage(f.bars->v_empty, f.v.stage, f.v.phase, 1002)) break;
+        copies_arrive(smem_u32(f.bars->k_full + f.k.stage));
+        if (!f.wait_stage(f.bars->v_empty, f.v.stage, f.v.phase, 1002)) return copies_drain();
         copy_keys<C::D>(values, t, bad, piece.head, v_to, f.p);
-        asm volatile("cp.async.commit_group;" ::: "memory");
-        ++owed;
-        settle(false);
+        copies_arrive(smem_u32(f.bars->v_full + f.v.stage));
+      }
+      if (f.p == 0) {
+        f.notes[f.issued % kNotes] = note;
+        if (bad) atomicCAS(a.status, 0u, unsigned(piece.sequence) + 1u);
+        mbar_arrive(smem_u32(f.bars->k_full + f.k.stage));  // the note is there
       }
       f.k.next();
       f.v.next();
       ++f.issued;
     }
-    if (!C::INT8 && gave_up_read(f.gave_up) != 0) break;
   }
-  if (!C::INT8) settle(true);
+  if (!C::INT8) copies_drain();
 }
 
 // ---- the issuing warp ---------------------------------------------------------------------------------------------
@@ -159,6 +132,7 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
   uint32_t q_phase = 0, p_phase = 0, o_phase = 3;  // a bit per group
   const bool elected = elect_one();
   auto scores = [&](int g) {
+    fence_async_smem();  // K's copies, which the barrier has told of
     if (!elected) return;
     const uint32_t rows_q = along_row(q + g * C::SIDE), rows_k = along_row(k_ring + k.stage * C::SIDE);
 #pragma unroll
@@ -192,6 +166,7 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
       if (!mbar_wait(smem_u32(bars->p_full + g), p_phase >> g & 1, gave_up, 1014)) return;
       p_phase ^= 1u << g;
       tc_fence_after();
+      fence_async_smem();  // V's copies
       if (elected) {
         const uint32_t rows_v = across_rows(v_ring + v.stage * C::SIDE);
 #pragma unroll
@@ -409,7 +384,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const TcArgs a) {
   if (threadIdx.x == 0) {
     gave_up_word = 0;
     for (int i = 0; i < 4; ++i) {
-      mbar_init(smem_u32(bars.k_full + i), 128);
+      mbar_init(smem_u32(bars.k_full + i), 129);
       mbar_init(smem_u32(bars.v_full + i), 128);
       mbar_init(smem_u32(bars.k_empty + i), 1);
       mbar_init(smem_u32(bars.v_empty + i), 1);
@@ -498,8 +473,8 @@ int launch(const TcArgs& a, cudaStream_t stream) {
 int paged_tc_rows() { return kRows; }
 
 int paged_tc(TcArgs a, int dtype_code, bool codes, int head_dim, cudaStream_t stream) {
-  a.line.rows = kRows;
-  a.line.keys = kTileKeys;
+  a.line.rows = Divisor(kRows);
+  a.line.keys = Divisor(kTileKeys);
   if (dtype_code == 1)
     return head_dim == 64 ? (codes ? launch<Shape<__half, true, 64>>(a, stream) : launch<Shape<__half, false, 64>>(a, stream))
                           : (codes ? launch<Shape<__half, true, 128>>(a, stream) : launch<Shape<__half, false, 128>>(a, stream));

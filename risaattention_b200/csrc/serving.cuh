@@ -43,6 +43,22 @@ inline int check_step(const risa_b200_step* s, const risa_b200_cache* c, const c
 
 #ifdef __CUDACC__
 
+// A divisor known to the host: numbers below 2^31 are divided by a multiplication.
+struct Divisor {
+  int value;
+  uint32_t mul, shift;
+  __host__ __device__ Divisor() : value(1), mul(0), shift(0) {}
+  explicit Divisor(int d) : value(d) {
+    uint32_t l = 0;
+    while ((int64_t(1) << l) < d) ++l;
+    mul = uint32_t((uint64_t(1) << (31 + l)) / uint32_t(d) + 1);
+    shift = 31 + l;
+  }
+  __host__ __device__ __forceinline__ operator int() const { return value; }
+};
+__device__ __forceinline__ int operator/(int n, const Divisor& d) { return int((uint64_t(uint32_t(n)) * d.mul) >> d.shift); }
+__device__ __forceinline__ int operator%(int n, const Divisor& d) { return n - (n / d) * d.value; }
+
 // ---- a step as the kernels see it -----------------------------------------------------------------
 struct StepView {
   const int32_t* table;

@@ -12,10 +12,11 @@ namespace serving {
 
 struct LineArgs {
   StepView step;
-  int kv_heads, group;     // query heads per key head
-  int rows;                // query rows of a block
+  int kv_heads;
+  Divisor group;           // query heads per key head
+  Divisor rows;            // query rows of a block
   int min_rows, max_rows;  // sequences with fewer or more query rows per key head belong to another launch
-  int keys;                // keys of a step
+  Divisor keys;            // keys of a step
   int causal, window;
 };
 
@@ -33,19 +34,28 @@ __device__ __forceinline__ int blocks_of(const LineArgs& a, const Sequence& q) {
 // The key steps with a key that one of the block's rows sees, at least one.
 __device__ __forceinline__ StepRange steps_of(const LineArgs& a, const Sequence& q, int block) {
   const int rows = q.count * a.group, row0 = block * a.rows;
-  const int token0 = row0 / a.group, token1 = (row0 + min(a.rows, rows - row0) - 1) / a.group;
+  const int token0 = row0 / a.group, token1 = (row0 + min(a.rows.value, rows - row0) - 1) / a.group;
   const KeyRange oldest = visible(q.length - q.count + token0, q.length, a.causal, a.window);
   const KeyRange newest = visible(q.length - q.count + token1, q.length, a.causal, a.window);
   const int first = oldest.lo / a.keys, end = (newest.hi + a.keys - 1) / a.keys;
   return {first, max(end - first, 1)};
 }
 
-// Steps of one key head's blocks.
+// Steps of one key head's blocks: one thread's sum, or a warp's (the same in every lane).
 template <typename L>
 __device__ __forceinline__ int64_t head_steps(const L& a, const Sequence& q) {
   const int blocks = blocks_of(a, q);
   int64_t sum = 0;
   for (int b = 0; b < blocks; ++b) sum += steps_of(a, q, b).count;
+  return sum;
+}
+template <typename L>
+__device__ __forceinline__ int64_t head_steps_of_warp(const L& a, const Sequence& q) {
+  const int blocks = blocks_of(a, q);
+  int64_t sum = 0;
+  for (int b = threadIdx.x & 31; b < blocks; b += 32) sum += steps_of(a, q, b).count;
+#pragma unroll
+  for (int off = 16; off > 0; off >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, off);
   return sum;
 }
 
@@ -82,45 +92,82 @@ struct Place {
 template <int NT>
 struct LineShared {
   BlockScan<NT> scan;
+  int64_t steps[NT / 32];
   int sequence;
   int64_t offset, per_head;
 };
 
+// Few sequences may have many blocks each: a warp adds up one of them.  Many sequences: a thread each.
 template <int NT, typename L>
 __device__ __forceinline__ int64_t line_total(const L& a, LineShared<NT>& s) {
+  const int warp = threadIdx.x >> 5;
   int64_t sum = 0, total;
-  for (int i = threadIdx.x; i < a.step.batch; i += NT) sum += head_steps(a, sequence_of(a.step, i)) * a.kv_heads;
+  if (a.step.batch <= NT / 32) {
+    const int64_t steps = warp < a.step.batch ? head_steps_of_warp(a, sequence_of(a.step, warp)) : 0;
+    if ((threadIdx.x & 31) == 0) {
+      s.steps[warp] = steps;
+      sum = steps * a.kv_heads;
+    }
+  } else {
+    for (int i = threadIdx.x; i < a.step.batch; i += NT) sum += head_steps(a, sequence_of(a.step, i)) * a.kv_heads;
+  }
   block_inclusive_scan<NT>(sum, s.scan, total);
   return total;
 }
 
-// Where step `at` (inside the line) lies; every thread of the block calls it.
+// Where step `at` (inside the line) lies; every thread of the block calls it, after line_total.
 template <int NT, typename L>
 __device__ __forceinline__ Place line_place(const L& a, int64_t at, LineShared<NT>& s) {
   int64_t base = 0;
-  for (int i0 = 0; i0 < a.step.batch; i0 += NT) {
-    const int i = i0 + threadIdx.x;
-    const int64_t per_head = i < a.step.batch ? head_steps(a, sequence_of(a.step, i)) : 0;
-    int64_t total;
-    const int64_t w = per_head * a.kv_heads, through = base + block_inclusive_scan<NT>(w, s.scan, total);
-    if (through - w <= at && at < through) {
-      s.sequence = i;
-      s.offset = at - (through - w);
-      s.per_head = per_head;
+  if (a.step.batch <= NT / 32) {
+    int i = 0;
+    for (; i + 1 < a.step.batch; ++i) {
+      const int64_t w = s.steps[i] * a.kv_heads;
+      if (at < base + w) break;
+      base += w;
     }
-    base += total;
-    if (base > at) break;
+    if (threadIdx.x == 0) {
+      s.sequence = i;
+      s.offset = at - base;
+      s.per_head = s.steps[i];
+    }
+  } else {
+    for (int i0 = 0; i0 < a.step.batch; i0 += NT) {
+      const int i = i0 + threadIdx.x;
+      const int64_t per_head = i < a.step.batch ? head_steps(a, sequence_of(a.step, i)) : 0;
+      int64_t total;
+      const int64_t w = per_head * a.kv_heads, through = base + block_inclusive_scan<NT>(w, s.scan, total);
+      if (through - w <= at && at < through) {
+        s.sequence = i;
+        s.offset = at - (through - w);
+        s.per_head = per_head;
+      }
+      base += total;
+      if (base > at) break;
+    }
   }
   __syncthreads();
   Place p{s.sequence, int(s.offset / s.per_head), 0, 0};
   int64_t rest = s.offset - p.head * s.per_head;
   const Sequence q = sequence_of(a.step, p.sequence);
-  for (;; ++p.block) {
-    const int count = steps_of(a, q, p.block).count;
-    if (rest < count) break;
-    rest -= count;
+  const int blocks = blocks_of(a, q), lane = threadIdx.x & 31;
+  for (;; p.block += 32) {  // 32 blocks at a time; every warp by itself
+    const int b = p.block + lane, count = b < blocks ? steps_of(a, q, b).count : 0;
+    int64_t through = count;
+#pragma unroll
+    for (int off = 1; off < 32; off <<= 1) {
+      const int64_t below = __shfl_up_sync(0xffffffffu, through, off);
+      if (lane >= off) through += below;
+    }
+    const unsigned int behind = __ballot_sync(0xffffffffu, rest < through);
+    if (behind != 0) {
+      const int first = __ffs(behind) - 1;
+      p.block += first;
+      p.inside = int(rest - __shfl_sync(0xffffffffu, through - count, first));
+      break;
+    }
+    rest -= __shfl_sync(0xffffffffu, through, 31);
   }
-  p.inside = int(rest);
   __syncthreads();  // the shared words may be written again
   return p;
 }

@@ -47,6 +47,12 @@ __device__ __forceinline__ void tmem_store16(uint32_t address, const uint32_t* r
 __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there) {
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
+// The thread's arrival on a barrier once all its copies so far have landed; nothing waits for it here.  The copies are
+// written through the generic proxy: whoever waits on the barrier fences before a matrix instruction reads them.
+__device__ __forceinline__ void copies_arrive(uint32_t barrier) {
+  asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(barrier) : "memory");
+}
+__device__ __forceinline__ void copies_drain() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ void store16(uint32_t to, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }

@@ -33,7 +33,10 @@ constexpr uint32_t kFirst = 1u, kLast = 2u, kTwoGroups = 4u, kBadRuns = 8;
 // Blocks of 256 keys and steps of query rows (serving_plan.cuh's line the other way round).
 struct WeighLine {
   StepView step;
-  int kv_heads, group, min_rows, tile_rows;
+  int kv_heads;
+  Divisor group;
+  int min_rows;
+  Divisor tile_rows;  // query rows of a step
   int causal, window;
 };
 __device__ __forceinline__ int first_seen(const WeighLine& a, const Sequence& q) {
@@ -112,32 +115,19 @@ __device__ __forceinline__ void fetch(const WeighArgs& a, Pieces pieces, Barrier
   RingPos<C::KEY_BUFFERS> kb;
   RingPos<C::STAGES> st;
   uint32_t tile = 0;
-  // copy groups under way, oldest first, and the barriers that wait for them
-  uint32_t owed[2] = {0, 0};
-  int count = 0;
-  auto hand_over = [&] {
-    if (count == 2) asm volatile("cp.async.wait_group 1;" ::: "memory");
-    else asm volatile("cp.async.wait_group 0;" ::: "memory");
-    fence_async_smem();
-    mbar_arrive(owed[0]);
-    owed[0] = owed[1];
-    --count;
-  };
-  auto close = [&](uint32_t barrier) {
-    asm volatile("cp.async.commit_group;" ::: "memory");
-    owed[count++] = barrier;
-    if (count == 2) hand_over();
-  };
   Piece piece;
-  bool alive = true;
-  while (alive && pieces.next(a.line, piece)) {
+  auto lse_of = [&](const Piece& at, int tile) {  // this thread's row of a tile
+    const int r = tile * C::ROWS + p, rows = at.seq.count * a.line.group;
+    if (p >= C::ROWS || r >= rows) return -INFINITY;
+    const int token = r / a.line.group;
+    return __ldg(a.row_lse + int64_t(at.seq.first + token) * (a.line.kv_heads * a.line.group) + at.head * a.line.group + r - token * a.line.group);
+  };
+  while (pieces.next(a.line, piece)) {
     const Sequence& seq = piece.seq;
     const int32_t* row = a.line.step.table + int64_t(piece.sequence) * a.line.step.width;
     const int low = first_seen(a.line, seq), key0 = (low / kBlockKeys + piece.block) * kBlockKeys, rows = seq.count * a.line.group;
-    // with a single key buffer its block must be read out first, to its last tile
-    if (C::KEY_BUFFERS == 1)
-      while (count > 0) hand_over();
-    if (!mbar_wait(smem_u32(bars->k_empty + kb.stage), kb.phase ^ 1, gave_up, 1101)) break;
+    float lse = lse_of(piece, piece.first);
+    if (!mbar_wait(smem_u32(bars->k_empty + kb.stage), kb.phase ^ 1, gave_up, 1101)) return copies_drain();
     uint32_t bad = 0;
 #pragma unroll 1
     for (int g = 0; g < 2; ++g) {
@@ -156,40 +146,44 @@ __device__ __forceinline__ void fetch(const WeighArgs& a, Pieces pieces, Barrier
       }
     }
     if (p == 0 && bad) atomicCAS(a.status, 0u, unsigned(piece.sequence) + 1u);
-    close(smem_u32(bars->k_full + kb.stage));
+    if (C::INT8) {
+      fence_async_smem();
+      mbar_arrive(smem_u32(bars->k_full + kb.stage));
+    } else {
+      copies_arrive(smem_u32(bars->k_full + kb.stage));
+    }
     kb.next();
     for (int i = 0; i < piece.count; ++i, ++tile) {
-      if (!mbar_wait(smem_u32(bars->q_empty + st.stage), st.phase ^ 1, gave_up, 1102)) {
-        alive = false;
-        break;
-      }
-      const int row0 = (piece.first + i) * C::ROWS;
-      if (p == 0)
-        notes->tile[tile % kDepth] = (i == 0 ? kFirst : 0u) | (i + 1 == piece.count ? kLast : 0u) | (seq.length - key0 > 128 ? kTwoGroups : 0u) | bad << kBadRuns;
-      if (p < C::ROWS) {
-        const int r = row0 + p;
-        float x = -INFINITY;
-        if (r < rows) {
-          const int token = r / a.line.group;
-          x = __ldg(a.row_lse + int64_t(seq.first + token) * (a.line.kv_heads * a.line.group) + piece.head * a.line.group + r - token * a.line.group);
-        }
-        notes->minus_lse[tile % kDepth][p] = x == -INFINITY ? -INFINITY : -x * kLog2e;
-      }
-      constexpr int PIECES = C::D / 8;
+      const float x = lse;
+      if (i + 1 < piece.count) lse = lse_of(piece, piece.first + i + 1);
+      if (!mbar_wait(smem_u32(bars->q_empty + st.stage), st.phase ^ 1, gave_up, 1102)) return copies_drain();
+      constexpr int PIECES = C::D / 8, ROWS_EACH = 128 / PIECES;  // rows that the warpgroup copies at a time
+      const int c = p % PIECES;
+      int r = p / PIECES, row = (piece.first + i) * C::ROWS + r, token = row / a.line.group, h = row - token * a.line.group;
+      const int tokens_each = ROWS_EACH / a.line.group, heads_each = ROWS_EACH - tokens_each * a.line.group;
       const uint32_t to = queries + st.stage * C::TILE;
 #pragma unroll 4
-      for (int n = 0; n < C::ROWS * PIECES / 128; ++n) {
-        const int index = n * 128 + p, r = index / PIECES, c = index % PIECES;
-        const bool there = row0 + r < rows;
-        const int token = there ? (row0 + r) / a.line.group : 0, h = there ? row0 + r - token * a.line.group : 0;
+      for (int n = 0; n < C::ROWS / ROWS_EACH; ++n, r += ROWS_EACH, row += ROWS_EACH) {
+        const bool there = row < rows;
         copy16(to + query_offset<C::ROWS>(r, c),
-               static_cast<const typename C::T*>(a.q) + int64_t(seq.first + token) * a.qn + int64_t(piece.head * a.line.group + h) * a.qh + c * 8, there);
+               static_cast<const typename C::T*>(a.q) + (there ? int64_t(seq.first + token) * a.qn + int64_t(piece.head * a.line.group + h) * a.qh + c * 8 : 0),
+               there);
+        token += tokens_each;
+        h += heads_each;
+        if (h >= a.line.group) {
+          h -= a.line.group;
+          ++token;
+        }
       }
-      close(smem_u32(bars->q_full + st.stage));
+      copies_arrive(smem_u32(bars->q_full + st.stage));
+      if (p < C::ROWS) notes->minus_lse[tile % kDepth][p] = x == -INFINITY ? -INFINITY : -x * kLog2e;
+      if (p == 0)
+        notes->tile[tile % kDepth] = (i == 0 ? kFirst : 0u) | (i + 1 == piece.count ? kLast : 0u) | (seq.length - key0 > 128 ? kTwoGroups : 0u) | bad << kBadRuns;
+      mbar_arrive_warp(smem_u32(bars->q_full + st.stage));  // the notes are there
       st.next();
     }
   }
-  while (count > 0) hand_over();
+  copies_drain();
 }
 
 template <typename C>
@@ -204,6 +198,7 @@ __device__ __forceinline__ void issue(int tiles, Barriers* bars, const volatile 
     if (!mbar_wait(smem_u32(bars->q_full + st.stage), st.phase, gave_up, 1110)) return;
     const uint32_t note = notes->tile[tile % kDepth];
     if ((note & kFirst) && !mbar_wait(smem_u32(bars->k_full + kb.stage), kb.phase, gave_up, 1111)) return;
+    fence_async_smem();  // the copies that the barriers have told of
     const int groups = note & kTwoGroups ? 2 : 1;
     for (int g = 0; g < 2; ++g) {
       // both groups' buffers take turns together, so a group that sits out hands its buffer on
@@ -333,7 +328,7 @@ __global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a
       }
     }
     for (int i = 0; i < 4; ++i) {
-      mbar_init(smem_u32(bars.q_full + i), 128);
+      mbar_init(smem_u32(bars.q_full + i), 128 + 4);
       mbar_init(smem_u32(bars.q_empty + i), 1);
     }
     mbar_init(smem_u32(&bars.drained), 1);
@@ -415,7 +410,7 @@ __global__ __launch_bounds__(kBlockKeys) void join_weights_kernel(const WeighArg
 
 template <typename C>
 int launch(WeighArgs a, cudaStream_t stream) {
-  a.line.tile_rows = C::ROWS;
+  a.line.tile_rows = Divisor(C::ROWS);
   if (cudaFuncSetAttribute(weigh_tc_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
     return fail(RISA_B200_CUDA, "key weights: %s", cudaGetErrorString(cudaGetLastError()));
   launch_chained(weigh_tc_kernel<C>, dim3(kTcWorkers), dim3(kThreads), C::SMEM, stream, a);
@@ -435,7 +430,7 @@ size_t weigh_tc_scratch() { return size_t(kTcWorkers) * 2 * kBlockKeys * sizeof(
 
 int weigh_tc(const TcArgs& t, const float* row_lse, const float* previous, float* weights, int dtype_code, bool codes, int head_dim,
              cudaStream_t stream) {
-  const WeighArgs a{{t.line.step, t.line.kv_heads, t.line.group, t.line.min_rows, 0, t.line.causal, t.line.window},
+  const WeighArgs a{{t.line.step, t.line.kv_heads, t.line.group, t.line.min_rows, Divisor(), t.line.causal, t.line.window},
                     t.q, t.qn, t.qh, row_lse, {t.keys, t.key_scales, t.line.kv_heads, t.line.step.page_shift}, t.pages, t.scale_log2,
                     previous, weights, t.parts, t.min_steps, t.status};
   return dtype_code == 1 ? launch_for<__half>(a, codes, head_dim, stream) : launch_for<__nv_bfloat16>(a, codes, head_dim, stream);
