@@ -89,7 +89,7 @@ __device__ __forceinline__ void fetch_tiles(Fetcher<C>& f, Pieces pieces) {
       const uint32_t k_to = f.k_ring + f.k.stage * C::SIDE, v_to = f.v_ring + f.v.stage * C::SIDE;
       if constexpr (C::INT8) {
         // scaled and rounded to the queries' type (half a step), as if the cache had held 16-bit values
-        CodeTile<typename C::T, C::D, true> codes;
+        CodeTile<typename C::T, C::D> codes;
         codes.load(keys, t, bad, piece.head, f.p);
         if (!f.wait_stage(f.bars->k_empty, f.k.stage, f.k.phase, 1001)) return;
         codes.store(k_to, f.p);

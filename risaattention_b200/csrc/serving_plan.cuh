@@ -41,6 +41,17 @@ __device__ __forceinline__ StepRange steps_of(const LineArgs& a, const Sequence&
   return {first, max(end - first, 1)};
 }
 
+// Quotients of numbers that are rarely past 32 bits (a 64-bit division is some hundred instructions).
+__device__ __forceinline__ int64_t quotient(int64_t n, int64_t d) {
+  return ((n | d) >> 32) == 0 ? int64_t(uint32_t(n) / uint32_t(d)) : n / d;
+}
+// Border of worker c on a line of w steps, and the first worker whose border is not in front of step `at`.
+__device__ __forceinline__ int64_t border(int64_t w, int c, int workers) { return quotient(w * c, workers); }
+__device__ __forceinline__ int worker_from(int64_t w, int64_t at, int workers) { return int(quotient(at * workers + w - 1, w)); }
+__device__ __forceinline__ int workers_of(int64_t w, int most, int min_steps) {
+  return int(min(int64_t(most), quotient(w + min_steps - 1, min_steps)));
+}
+
 // Steps of one key head's blocks: one thread's sum, or a warp's (the same in every lane).
 template <typename L>
 __device__ __forceinline__ int64_t head_steps(const L& a, const Sequence& q) {
@@ -147,7 +158,7 @@ __device__ __forceinline__ Place line_place(const L& a, int64_t at, LineShared<N
     }
   }
   __syncthreads();
-  Place p{s.sequence, int(s.offset / s.per_head), 0, 0};
+  Place p{s.sequence, int(quotient(s.offset, s.per_head)), 0, 0};
   int64_t rest = s.offset - p.head * s.per_head;
   const Sequence q = sequence_of(a.step, p.sequence);
   const int blocks = blocks_of(a, q), lane = threadIdx.x & 31;
@@ -172,11 +183,6 @@ __device__ __forceinline__ Place line_place(const L& a, int64_t at, LineShared<N
   return p;
 }
 
-// Border of worker c on a line of w steps.
-__device__ __forceinline__ int64_t border(int64_t w, int c, int workers) { return w * c / workers; }
-__device__ __forceinline__ int workers_of(int64_t w, int most, int min_steps) {
-  return int(min(int64_t(most), (w + min_steps - 1) / min_steps));
-}
 
 // What a worker does next: steps [first, first + count) of one block; whole: all of the block's, opens: its
 // first ones.
@@ -257,8 +263,7 @@ __global__ __launch_bounds__(128) void join_parts_kernel(const JoinArgs a) {
   if (place.inside == 0 || previous > unit_start) return;  // no unit is cut here, or an earlier border joins it
   const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, row = place.block * R + r;
   if (r >= R || row >= seq.count * a.line.group) return;
-  int parts = 1;
-  while (c + parts < workers && border(total, c + parts, workers) < unit_end) ++parts;
+  const int parts = min(worker_from(total, unit_end, workers), workers) - c;
   const int64_t slot = slot_floats(R, D);
   auto slot_of = [&](int i) { return a.parts + (int64_t(c + i) * 2 + (i == 0 ? 1 : 0)) * slot; };
   float top = kNoMaximum;

@@ -70,6 +70,17 @@ __device__ __forceinline__ uint32_t scaled_pair(uint32_t word, int i, float scal
   return Half2<T>::pack(a * scale, b * scale);
 }
 
+// The 16 codes `w` of a row as 16-bit values: two pieces of its tile.
+template <typename T>
+__device__ __forceinline__ void store_codes(uint32_t tile, int row, int piece, uint4 w, float scale) {
+  const uint32_t u[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
+#pragma unroll
+  for (int h = 0; h < 2; ++h)
+    store16(tile + tile_offset(row, 2 * piece + h),
+            make_uint4(scaled_pair<T>(u[2 * h], 0, scale), scaled_pair<T>(u[2 * h], 1, scale), scaled_pair<T>(u[2 * h + 1], 0, scale),
+                       scaled_pair<T>(u[2 * h + 1], 1, scale)));
+}
+
 // ---- 128 keys of a paged sequence into a tile, by the 128 threads of a warpgroup ----------------------------------------
 // Page numbers of eight runs of 16 keys, and where they lie.
 struct KeyRuns {
@@ -120,12 +131,12 @@ __device__ __forceinline__ void copy_keys(const PoolView& pool, const KeyRuns& k
   }
 }
 
-// Codes: 16 of them per load; `store` multiplies by their row's scale (SCALED) and rounds to T.
-template <typename T, int D, bool SCALED>
+// Codes: 16 of them per load; `store` multiplies by their row's scale and rounds to T.
+template <typename T, int D>
 struct CodeTile {
   static constexpr int PIECES = D / 16, LOADS = PIECES;
   uint4 codes[LOADS];
-  float scale[SCALED ? LOADS : 1];
+  float scale[LOADS];
   __device__ __forceinline__ void load(const PoolView& pool, const KeyRuns& k, uint32_t bad, int head, int thread) {
 #pragma unroll
     for (int n = 0; n < LOADS; ++n) {
@@ -136,20 +147,14 @@ struct CodeTile {
       const bool there = !(bad >> i & 1) && id >= 0 && key >= k.low && key < k.length;
       const int64_t line = pool.line(id, head, key);
       codes[n] = there ? *reinterpret_cast<const uint4*>(pool.rows + line * D + piece * 16) : make_uint4(0, 0, 0, 0);
-      if (SCALED) scale[n] = there ? pool.scales[line] : 0.f;
+      scale[n] = there ? pool.scales[line] : 0.f;
     }
   }
   __device__ __forceinline__ void store(uint32_t to, int thread) const {
 #pragma unroll
     for (int n = 0; n < LOADS; ++n) {
       const int index = n * 128 + thread, row = index / PIECES, piece = index % PIECES;
-      const float s = SCALED ? scale[n] : 1.0f;
-      const uint32_t w[4] = {codes[n].x ^ 0x80808080u, codes[n].y ^ 0x80808080u, codes[n].z ^ 0x80808080u, codes[n].w ^ 0x80808080u};
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        store16(to + tile_offset(row, 2 * piece + h),
-                make_uint4(scaled_pair<T>(w[2 * h], 0, s), scaled_pair<T>(w[2 * h], 1, s), scaled_pair<T>(w[2 * h + 1], 0, s),
-                           scaled_pair<T>(w[2 * h + 1], 1, s)));
+      store_codes<T>(to, row, piece, codes[n], scale[n]);
     }
   }
 };

@@ -7,7 +7,9 @@
 // weights.  What bounds it is the exponentials: one per (key, row) and 16 per clock and SM, 2048 clocks for 256 keys x
 // 128 rows, against 1024 of the matrix instruction at 128 channels.
 //
-// Warps 0-3, 4-7: the two groups' sums.  8-11: fetch keys and query rows.  12: issues the products.  13-15 idle.
+// Warps 0-15: the sums, four warpgroups: two for each group of keys, each with half of a tile's rows (four warps a
+// scheduler hide the latencies of tensor memory and the exponential; two left a third of the time idle).  16-19: fetch
+// query rows.  20-23: fetch keys.  24: issues the products.
 #include "paged_tc.cuh"
 #include "tc_f16.cuh"
 
@@ -20,15 +22,14 @@ using namespace tc;
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 800;
 constexpr int kBlockKeys = 256;
-constexpr int kFetcher = 8, kIssuer = 12;
+constexpr int kFetcher = 16, kKeyFetcher = 20, kIssuer = 24;
 // Notes and log-sum-exps of the tiles in flight.  A slot is written again kDepth tiles later, by when the sums have
 // left it: the fetchers are at most the query stages ahead of the issuer, the issuer two tiles ahead of the sums.
 constexpr int kDepth = 8;
-// Bits of a note: first and last tile of a block, whether the block has more than 128 keys, and from kBadRuns on the runs of
-// 16 keys whose page is outside the pool.
-constexpr uint32_t kFirst = 1u, kLast = 2u, kTwoGroups = 4u, kBadRuns = 8;
+// Bits of a note: first and last tile of a block, whether the block has more than 128 keys.
+constexpr uint32_t kFirst = 1u, kLast = 2u, kTwoGroups = 4u;
 
 // Blocks of 256 keys and steps of query rows (serving_plan.cuh's line the other way round).
 struct WeighLine {
@@ -94,7 +95,7 @@ struct Shape {
 };
 
 struct Barriers {
-  uint64_t k_full[2], k_empty[2], q_full[4], q_empty[4], s_full[2][2], s_free[2][2], drained;
+  uint64_t k_full[2], k_empty[2], q_full[4], q_empty[4], s_full[2][2], s_free[2][2], half_full[2], drained;
 };
 
 // Byte offset of piece `piece` of row `row` in a tile of ROWS query rows.
@@ -105,14 +106,68 @@ __device__ __forceinline__ uint32_t query_offset(int row, int piece) {
 
 struct Notes {
   uint32_t tile[kDepth];
+  uint32_t bad[kDepth];          // runs of 16 keys whose page is outside the pool, of the last blocks
   float minus_lse[kDepth][128];  // in units of log 2; -infinity for rows that give nothing
+  // What the second half of the rows adds to a key, of the last four blocks: the warpgroup that writes it is at most two
+  // tiles ahead of the one that reads it.
+  float half[4][2][128];
 };
 
+// A worker's key blocks.  A short loop: it runs once in many tiles, and unrolled it was 7 us of instruction fetches in front
+// of the first product.
 template <typename C>
-__device__ __forceinline__ void fetch(const WeighArgs& a, Pieces pieces, Barriers* bars, volatile Notes* notes, uint32_t keys, uint32_t queries,
+__device__ __forceinline__ void fetch_keys(const WeighArgs& a, Pieces pieces, Barriers* bars, volatile Notes* notes, uint32_t keys, uint32_t gave_up) {
+  constexpr int PIECES = C::D / (C::INT8 ? 16 : 8), EACH = 128 / PIECES;  // rows that the warpgroup fetches at a time
+  const int p = threadIdx.x - kKeyFetcher * 32, lane = p & 31, piece = p % PIECES;
+  RingPos<C::KEY_BUFFERS> kb;
+  uint32_t block = 0;
+  Piece at;
+  while (pieces.next(a.line, at)) {
+    const int32_t* row = a.line.step.table + int64_t(at.sequence) * a.line.step.width;
+    const int low = first_seen(a.line, at.seq), length = at.seq.length, key0 = (low / kBlockKeys + at.block) * kBlockKeys;
+    // lane i knows the page of the block's i-th run of 16 keys
+    const int run = key0 + 16 * lane;
+    const bool exists = lane < kBlockKeys / 16 && run < length && run + 16 > low;
+    int id = exists ? __ldg(row + (run >> a.line.step.page_shift)) : -1;
+    const uint32_t bad = __ballot_sync(0xffffffffu, exists && (id < 0 || id >= a.pages));
+    if (id >= a.pages) id = -1;
+    if (!mbar_wait(smem_u32(bars->k_empty + kb.stage), kb.phase ^ 1, gave_up, 1101)) break;
+    if (p == 0) {
+      notes->bad[block % kDepth] = bad;
+      if (bad) atomicCAS(a.status, 0u, unsigned(at.sequence) + 1u);
+    }
+#pragma unroll 4
+    for (int r = p / PIECES; r < kBlockKeys; r += EACH) {
+      const int key = key0 + r, page = __shfl_sync(0xffffffffu, id, r >> 4);
+      const bool there = page >= 0 && key >= low && key < length;
+      const int64_t line = there ? a.keys.line(page, at.head, key) : 0;
+      const uint32_t to = keys + kb.stage * C::KEYS + (r >> 7) * C::GROUP;
+      if (C::INT8) {
+        // codes as they are: a key's scale multiplies its scores in 32 bits
+        uint4 w = make_uint4(0, 0, 0, 0);
+        if (there) w = *reinterpret_cast<const uint4*>(a.keys.rows + line * C::D + piece * 16);
+        store_codes<typename C::T>(to, r & 127, piece, w, 1.0f);
+      } else {
+        copy16(to + tile_offset(r & 127, piece), a.keys.rows + line * (C::D * 2) + piece * 16, there);
+      }
+    }
+    if (C::INT8) {
+      fence_async_smem();
+      mbar_arrive(smem_u32(bars->k_full + kb.stage));
+    } else {
+      copies_arrive(smem_u32(bars->k_full + kb.stage));
+    }
+    mbar_arrive_warp(smem_u32(bars->k_full + kb.stage));  // the note is there
+    kb.next();
+    ++block;
+  }
+  copies_drain();
+}
+
+template <typename C>
+__device__ __forceinline__ void fetch_queries(const WeighArgs& a, Pieces pieces, Barriers* bars, volatile Notes* notes, uint32_t queries,
                                       uint32_t gave_up) {
   const int p = threadIdx.x - kFetcher * 32;
-  RingPos<C::KEY_BUFFERS> kb;
   RingPos<C::STAGES> st;
   uint32_t tile = 0;
   Piece piece;
@@ -122,63 +177,47 @@ __device__ __forceinline__ void fetch(const WeighArgs& a, Pieces pieces, Barrier
     const int token = r / a.line.group;
     return __ldg(a.row_lse + int64_t(at.seq.first + token) * (a.line.kv_heads * a.line.group) + at.head * a.line.group + r - token * a.line.group);
   };
-  while (pieces.next(a.line, piece)) {
-    const Sequence& seq = piece.seq;
-    const int32_t* row = a.line.step.table + int64_t(piece.sequence) * a.line.step.width;
-    const int low = first_seen(a.line, seq), key0 = (low / kBlockKeys + piece.block) * kBlockKeys, rows = seq.count * a.line.group;
-    float lse = lse_of(piece, piece.first);
-    if (!mbar_wait(smem_u32(bars->k_empty + kb.stage), kb.phase ^ 1, gave_up, 1101)) return copies_drain();
-    uint32_t bad = 0;
-#pragma unroll 1
-    for (int g = 0; g < 2; ++g) {
-      KeyRuns runs;
-      runs.look_up(row, a.line.step.page_shift, key0 + 128 * g, low, seq.length);
-      const uint32_t b = runs.bad(a.pages);
-      bad |= b << (8 * g);
-      const uint32_t to = keys + kb.stage * C::KEYS + g * C::GROUP;
-      if constexpr (C::INT8) {
-        // codes as they are: a key's scale multiplies its scores in 32 bits
-        CodeTile<typename C::T, C::D, false> codes;
-        codes.load(a.keys, runs, b, piece.head, p);
-        codes.store(to, p);
-      } else {
-        copy_keys<C::D>(a.keys, runs, b, piece.head, to, p);
-      }
-    }
-    if (p == 0 && bad) atomicCAS(a.status, 0u, unsigned(piece.sequence) + 1u);
-    if (C::INT8) {
-      fence_async_smem();
-      mbar_arrive(smem_u32(bars->k_full + kb.stage));
-    } else {
-      copies_arrive(smem_u32(bars->k_full + kb.stage));
-    }
-    kb.next();
-    for (int i = 0; i < piece.count; ++i, ++tile) {
+  bool more = pieces.next(a.line, piece);
+  float lse = lse_of(piece, piece.first);
+  while (more) {
+    const Piece now = piece;
+    const Sequence& seq = now.seq;
+    const int key0 = (first_seen(a.line, seq) / kBlockKeys + now.block) * kBlockKeys, rows = seq.count * a.line.group;
+    more = pieces.next(a.line, piece);
+    constexpr int PIECES = C::D / 8, ROWS_EACH = 128 / PIECES;  // rows that the warpgroup copies at a time
+    constexpr int COPIES = C::ROWS / ROWS_EACH;
+    static_assert(ROWS_EACH == 4 || ROWS_EACH % 8 == 0, "a thread's rows lie alike in the swizzle");
+    const int c = p % PIECES, r0 = p / PIECES;
+    const int tokens_each = ROWS_EACH / a.line.group;
+    const int64_t each = tokens_each * a.qn + (ROWS_EACH - tokens_each * a.line.group) * a.qh, wrap = a.qn - a.line.group * a.qh;
+    for (int i = 0; i < now.count; ++i, ++tile) {
       const float x = lse;
-      if (i + 1 < piece.count) lse = lse_of(piece, piece.first + i + 1);
+      if (i + 1 < now.count) lse = lse_of(now, now.first + i + 1);
+      else if (more) lse = lse_of(piece, piece.first);
       if (!mbar_wait(smem_u32(bars->q_empty + st.stage), st.phase ^ 1, gave_up, 1102)) return copies_drain();
-      constexpr int PIECES = C::D / 8, ROWS_EACH = 128 / PIECES;  // rows that the warpgroup copies at a time
-      const int c = p % PIECES;
-      int r = p / PIECES, row = (piece.first + i) * C::ROWS + r, token = row / a.line.group, h = row - token * a.line.group;
-      const int tokens_each = ROWS_EACH / a.line.group, heads_each = ROWS_EACH - tokens_each * a.line.group;
+      int row = (now.first + i) * C::ROWS + r0;
+      const int token = row / a.line.group;
+      int h = row - token * a.line.group;
+      const typename C::T* from = static_cast<const typename C::T*>(a.q) + int64_t(seq.first + token) * a.qn + int64_t(now.head * a.line.group + h) * a.qh + c * 8;
       const uint32_t to = queries + st.stage * C::TILE;
-#pragma unroll 4
-      for (int n = 0; n < C::ROWS / ROWS_EACH; ++n, r += ROWS_EACH, row += ROWS_EACH) {
+#pragma unroll
+      for (int n = 0; n < COPIES; ++n) {
+        // a row that does not exist is not read; the address then is the queries' own
         const bool there = row < rows;
-        copy16(to + query_offset<C::ROWS>(r, c),
-               static_cast<const typename C::T*>(a.q) + (there ? int64_t(seq.first + token) * a.qn + int64_t(piece.head * a.line.group + h) * a.qh + c * 8 : 0),
-               there);
-        token += tokens_each;
-        h += heads_each;
+        copy16(to + (ROWS_EACH % 8 == 0 ? query_offset<C::ROWS>(r0, c) + n * ROWS_EACH * 128 : query_offset<C::ROWS>(r0 + n * ROWS_EACH, c)),
+               there ? from : static_cast<const typename C::T*>(a.q), there);
+        row += ROWS_EACH;
+        from += each;
+        h += ROWS_EACH - tokens_each * a.line.group;
         if (h >= a.line.group) {
           h -= a.line.group;
-          ++token;
+          from += wrap;
         }
       }
       copies_arrive(smem_u32(bars->q_full + st.stage));
       if (p < C::ROWS) notes->minus_lse[tile % kDepth][p] = x == -INFINITY ? -INFINITY : -x * kLog2e;
       if (p == 0)
-        notes->tile[tile % kDepth] = (i == 0 ? kFirst : 0u) | (i + 1 == piece.count ? kLast : 0u) | (seq.length - key0 > 128 ? kTwoGroups : 0u) | bad << kBadRuns;
+        notes->tile[tile % kDepth] = (i == 0 ? kFirst : 0u) | (i + 1 == now.count ? kLast : 0u) | (seq.length - key0 > 128 ? kTwoGroups : 0u);
       mbar_arrive_warp(smem_u32(bars->q_full + st.stage));  // the notes are there
       st.next();
     }
@@ -224,14 +263,52 @@ __device__ __forceinline__ void issue(int tiles, Barriers* bars, const volatile 
   }
 }
 
+// Adds the exponentials of ROWS query rows (from column `from` on) to a key's sum.  Every row sees the key, or (MASKED) rows
+// [lo, hi) of the sequence do, the first column being row `row0`.
+template <int ROWS, bool MASKED>
+__device__ __forceinline__ void add_rows(uint32_t columns, const float* minus_lse, float factor, int row0, const RowRange& seen, float (&sum)[4],
+                                         uint32_t freed) {
+#pragma unroll
+  for (int c = 0; c < ROWS; c += 32) {
+    uint32_t x[32];
+    tmem_load32(columns + c, x);
+    tmem_load_wait();
+    tmem_regs_ready<32>(x);
+    if (c + 32 == ROWS) {
+      tc_fence_before();
+      mbar_arrive_warp(freed);
+    }
+    float u[32];
+#pragma unroll
+    for (int e = 0; e < 32; e += 4) {
+      const float4 l = *reinterpret_cast<const float4*>(minus_lse + c + e);
+      u[e] = fmaf(__uint_as_float(x[e]), factor, l.x);
+      u[e + 1] = fmaf(__uint_as_float(x[e + 1]), factor, l.y);
+      u[e + 2] = fmaf(__uint_as_float(x[e + 2]), factor, l.z);
+      u[e + 3] = fmaf(__uint_as_float(x[e + 3]), factor, l.w);
+    }
+    if (MASKED) {
+      const int lo = seen.lo - row0 - c, hi = seen.hi - row0 - c;
+#pragma unroll
+      for (int e = 0; e < 32; ++e)
+        if (e < lo || e >= hi) u[e] = -INFINITY;
+    }
+#pragma unroll
+    for (int e = 0; e < 32; ++e) u[e] = ex2_approx(u[e]);
+#pragma unroll
+    for (int e = 0; e < 32; ++e) sum[e & 3] += u[e];
+  }
+}
+
 template <typename C>
-__device__ __forceinline__ void add_up(const WeighArgs& a, Pieces pieces, Barriers* bars, uint32_t tmem, int g, const volatile Notes* notes,
-                                       uint32_t minus_lse, uint32_t gave_up) {
+__device__ __forceinline__ void add_up(const WeighArgs& a, Pieces pieces, Barriers* bars, uint32_t tmem, int g, int half, Notes* notes,
+                                       uint32_t gave_up) {
+  constexpr int ROWS = C::ROWS / 2;
   const int lane = threadIdx.x & 127;
-  const uint32_t columns = tmem + (uint32_t(lane & ~31) << 16) + g * 256;
+  const uint32_t columns = tmem + (uint32_t(lane & ~31) << 16) + g * 256 + half * ROWS;
   const int slots = a.line.step.width << a.line.step.page_shift;
   RingPos<2> buffer;
-  uint32_t tile = 0;
+  uint32_t tile = 0, block = 0;
   Piece piece;
   while (pieces.next(a.line, piece)) {
     const Sequence& seq = piece.seq;
@@ -246,58 +323,40 @@ __device__ __forceinline__ void add_up(const WeighArgs& a, Pieces pieces, Barrie
       const int id = __ldg(a.line.step.table + int64_t(piece.sequence) * a.line.step.width + (key >> a.line.step.page_shift));
       if (id >= 0 && id < a.pages) factor *= __ldg(a.keys.scales + a.keys.line(id, piece.head, key));
     }
-    const uint64_t factor2 = pack_f32x2(factor, factor);
-    uint64_t sum[4] = {0, 0, 0, 0};
+    float sum[4] = {0.f, 0.f, 0.f, 0.f};
     for (int i = 0; i < piece.count; ++i, ++tile) {
       if (!mbar_wait(smem_u32(&bars->s_full[g][buffer.stage]), buffer.phase, gave_up, 1120 + g)) return;
       tc_fence_after();
       if (i == 0) {
-        const uint32_t bad = notes->tile[tile % kDepth] >> (kBadRuns + 8 * g) & 0xff;
+        const uint32_t bad = notes->bad[block % kDepth] >> (8 * g) & 0xff;
         if (bad != 0) whole_group = false;
         if (bad >> (lane >> 4) & 1) mine.hi = 0;
       }
-      const uint32_t s = columns + buffer.stage * 128, lse = minus_lse + (tile % kDepth) * 512;
+      const uint32_t freed = smem_u32(&bars->s_free[g][buffer.stage]);
       if (takes_part) {
-        const int row0 = (piece.first + i) * C::ROWS;
-        const bool every = whole_group && row0 >= all_lo && row0 <= all_hi - C::ROWS;
-        uint32_t x[2][32];
-        tmem_load32(s, x[0]);
-#pragma unroll
-        for (int c = 0; c < C::ROWS / 32; ++c) {
-          tmem_load_wait();
-          tmem_regs_ready<32>(x[c & 1]);
-          if (c + 1 < C::ROWS / 32) tmem_load32(s + (c + 1) * 32, x[(c + 1) & 1]);
-          else {
-            tc_fence_before();
-            mbar_arrive_warp(smem_u32(&bars->s_free[g][buffer.stage]));
-          }
-          uint32_t* v = x[c & 1];
-#pragma unroll
-          for (int e = 0; e < 32; e += 4) {
-            uint64_t l01, l23;
-            asm volatile("ld.shared.v2.u64 {%0, %1}, [%2];" : "=l"(l01), "=l"(l23) : "r"(lse + (c * 32 + e) * 4) : "memory");
-            float u[4];
-            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[e]), __uint_as_float(v[e + 1])), factor2, l01), u[0], u[1]);
-            unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(v[e + 2]), __uint_as_float(v[e + 3])), factor2, l23), u[2], u[3]);
-            if (!every) {
-#pragma unroll
-              for (int j = 0; j < 4; ++j)
-                if (row0 + c * 32 + e + j < mine.lo || row0 + c * 32 + e + j >= mine.hi) u[j] = -INFINITY;
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) u[j] = ex2_approx(u[j]);
-            sum[e / 2 & 3] = add_f32x2(sum[e / 2 & 3], pack_f32x2(u[0], u[1]));
-            sum[(e / 2 + 1) & 3] = add_f32x2(sum[(e / 2 + 1) & 3], pack_f32x2(u[2], u[3]));
-          }
+        const int row0 = (piece.first + i) * C::ROWS + half * ROWS;
+        const float* lse = notes->minus_lse[tile % kDepth] + half * ROWS;
+        if (whole_group && row0 >= all_lo && row0 <= all_hi - ROWS) {
+          add_rows<ROWS, false>(columns + buffer.stage * 128, lse, factor, row0, mine, sum, freed);
+        } else {
+          add_rows<ROWS, true>(columns + buffer.stage * 128, lse, factor, row0, mine, sum, freed);
         }
       } else {
-        mbar_arrive_warp(smem_u32(&bars->s_free[g][buffer.stage]));
+        mbar_arrive_warp(freed);
       }
       buffer.next();
     }
-    float x0, x1, total;
-    unpack_f32x2(add_f32x2(add_f32x2(sum[0], sum[1]), add_f32x2(sum[2], sum[3])), x0, x1);
-    total = x0 + x1;
+    float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
+    float* other = &notes->half[block & 3][g][lane];
+    const uint32_t parity = block & 1;
+    ++block;
+    if (half == 1) {
+      *other = total;
+      mbar_arrive_warp(smem_u32(bars->half_full + g));
+      continue;
+    }
+    if (!mbar_wait(smem_u32(bars->half_full + g), parity, gave_up, 1122 + g)) return;
+    total += *other;
     if (!piece.whole) {
       a.parts[(int64_t(blockIdx.x) * 2 + (piece.opens ? 1 : 0)) * kBlockKeys + g * 128 + lane] = total;
     } else if (key < slots) {
@@ -320,11 +379,12 @@ __global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a
   if (threadIdx.x == 0) {
     gave_up_word = 0;
     for (int i = 0; i < 2; ++i) {
-      mbar_init(smem_u32(bars.k_full + i), 128);
+      mbar_init(smem_u32(bars.k_full + i), 128 + 4);
       mbar_init(smem_u32(bars.k_empty + i), 1);
+      mbar_init(smem_u32(bars.half_full + i), 4);
       for (int g = 0; g < 2; ++g) {
         mbar_init(smem_u32(&bars.s_full[g][i]), 1);
-        mbar_init(smem_u32(&bars.s_free[g][i]), 4);
+        mbar_init(smem_u32(&bars.s_free[g][i]), 8);
       }
     }
     for (int i = 0; i < 4; ++i) {
@@ -359,9 +419,11 @@ __global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a
   tc_fence_after();
   const uint32_t tmem = tmem_base;
   if (warp < kFetcher) {
-    add_up<C>(a, pieces, &bars, tmem, warp >> 2, &notes, smem_u32(&notes.minus_lse[0][0]), gave_up);
+    add_up<C>(a, pieces, &bars, tmem, warp >> 3, (warp >> 2) & 1, &notes, gave_up);
+  } else if (warp < kKeyFetcher) {
+    fetch_queries<C>(a, pieces, &bars, &notes, queries, gave_up);
   } else if (warp < kIssuer) {
-    fetch<C>(a, pieces, &bars, &notes, keys, queries, gave_up);
+    fetch_keys<C>(a, pieces, &bars, &notes, keys, gave_up);
   } else if (warp == kIssuer) {
     issue<C>(int(pieces.left), &bars, &notes, tmem, keys, queries, gave_up);
     __syncwarp();
@@ -400,7 +462,8 @@ __global__ __launch_bounds__(kBlockKeys) void join_weights_kernel(const WeighArg
   const int64_t start = edge - place.inside, end = start + steps_of(a.line, seq, place.block).count;
   if (place.inside == 0 || previous > start) return;
   float sum = a.parts[(int64_t(c) * 2 + 1) * kBlockKeys + threadIdx.x];
-  for (int i = 1; c + i < workers && border(total, c + i, workers) < end; ++i) sum += a.parts[int64_t(c + i) * 2 * kBlockKeys + threadIdx.x];
+  const int last = min(worker_from(total, end, workers), workers);
+  for (int i = c + 1; i < last; ++i) sum += a.parts[int64_t(i) * 2 * kBlockKeys + threadIdx.x];
   const int slots = a.line.step.width << a.line.step.page_shift;
   const int key = (first_seen(a.line, seq) / kBlockKeys + place.block) * kBlockKeys + threadIdx.x;
   if (key >= slots) return;
