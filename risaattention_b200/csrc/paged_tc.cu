@@ -1,15 +1,20 @@
 // Attention of many query rows (chunks of prompts) over a paged cache on the tensor cores.
 //
 // A unit is 256 query rows of one key head, rows in the order (token, head of the group), so that all heads of a
-// group share every key tile; two groups of 128 rows (one softmax warpgroup and one accumulator each) take turns on
-// the tensor pipe: while one group's scores become probabilities, the other's matrix products run.  Per 128-key tile
-// and group: S = Q K^T (128 x 128 x head_dim, fp32 in tensor memory), the thread that owns a row reads it, keeps
-// running maximum and sum without a shuffle, writes P (16 bits) over the columns of S, and O += P V takes P from
-// tensor memory and V from shared memory as it lies there (keys along K, channels contiguous).
+// group share every key tile; two groups of 128 rows, each with accumulators of its own, take turns on the tensor pipe:
+// while one group's scores become probabilities, the other's matrix products run.  Per 128-key tile and group:
+// S = Q K^T (128 x 128 x head_dim, fp32 in tensor memory); two threads own a row, each reads 64 of its scores into
+// registers, they exchange maxima (lanes of tensor memory are rows, so sums need no shuffle) and write P (16 bits) over
+// the first half of S's columns; O += P V takes P from tensor memory and V from shared memory as it lies there (keys
+// along K, channels contiguous).
 //
-// Warps 0-3, 4-7: softmax, query loads, epilogue of their row group.  8-11: fetch K and V tiles from the pages
-// (cp.async, or codes converted on the way) into the 128-byte-swizzled layout of the matrix instructions.  12: issues
-// them (and owns tensor memory).  13-15 idle, so that registers can be dealt per warpgroup.
+// What bounds it: per tile and group the tensor pipe works 1024 clocks (head_dim 128) and the special-function unit
+// 1024, and what one group's products and the other's softmax do not hide of each other is the chain of both.  With one
+// thread for a row the chain was 2080 (softmax) + 1630 clocks and a tile of both groups took 3710.
+//
+// Warps 0-15: softmax, query loads and epilogue, four for each half of the columns of each row group.  16-19: fetch K
+// and V tiles from the pages (cp.async, or codes converted on the way) into the 128-byte-swizzled layout of the matrix
+// instructions.  20: issues them (and owns tensor memory).  21-23 idle, so that registers can be dealt per warpgroup.
 #include "serving_plan.cuh"
 #include "paged_tc.cuh"
 #include "tc_f16.cuh"
@@ -21,12 +26,12 @@ using namespace tc;
 
 namespace {
 
-constexpr int kThreads = 512;
+constexpr int kThreads = 768;
 constexpr int kTileKeys = 128, kGroups = 2, kRows = 128 * kGroups;
-constexpr int kProducer = 8, kIssuer = 12;  // first warps of their roles
-// The SM's 65,536 registers at 512 threads are 128 each; the softmax warps hold a row of 128 scores.
-constexpr int kRegsLaunch = 128, kRegsSoftmax = 192, kRegsProducer = 88, kRegsIssuer = 40;
-static_assert(128 * (2 * kRegsSoftmax + kRegsProducer + kRegsIssuer) <= kThreads * kRegsLaunch, "register budget");
+constexpr int kProducer = 16, kIssuer = 20;  // first warps of their roles
+// 768 threads of at most 85 registers are launched with 80; the softmax warps hold 64 scores of a row.
+constexpr int kRegsLaunch = 80, kRegsSoftmax = 96, kRegsProducer = 56, kRegsIssuer = 40;
+static_assert(128 * (4 * kRegsSoftmax + kRegsProducer + kRegsIssuer) <= kThreads * kRegsLaunch, "register budget");
 // A note for each tile in flight: runs of 16 keys that are hidden because their page is outside the pool, whether the
 // tile is the first or the last of its unit, and whether the unit has more than 128 rows.
 constexpr int kNotes = 16;
@@ -41,7 +46,6 @@ struct Shape {
   static constexpr bool INT8 = INT8_;
   static constexpr int D = D_;
   static constexpr int SIDE = kTileKeys * D * 2;  // a K or V tile as the matrix instructions read it
-  static constexpr int HALVES = D / 64;           // blocks of 64 channels: 128 rows of 128 bytes
   static constexpr int STAGES = D == 128 ? 2 : 4;
   static constexpr int Q = kGroups * SIDE;
   static constexpr int SMEM = Q + 2 * STAGES * SIDE + 1024;  // + alignment
@@ -51,82 +55,90 @@ struct Barriers {
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
   uint64_t q_full[kGroups], s_full[kGroups], p_full[kGroups], o_full[kGroups], o_free[kGroups], drained;
 };
-
-// ---- the fetching warpgroup -----------------------------------------------------------------------------------
-template <typename C>
-struct Fetcher {
-  const TcArgs& a;
-  Barriers* bars;
-  volatile uint32_t* notes;
-  uint32_t v_ring, k_ring, gave_up;
-  int p;            // thread of the group
-  uint32_t issued;  // tiles so far
-  RingPos<C::STAGES> k, v;
-
-  __device__ __forceinline__ bool wait_stage(uint64_t* empty, int stage, uint32_t phase, unsigned site) const {
-    return mbar_wait(smem_u32(empty + stage), phase ^ 1, gave_up, site);
-  }
+// What the two threads of a row tell each other: maxima (of tiles in turn) and sums.
+struct Exchange {
+  float maximum[2][kGroups][2][128];
+  float sum[kGroups][2][128];
 };
 
+// ---- the fetching warpgroup -----------------------------------------------------------------------------------
+// Tiles of 16-bit rows that all exist come by TMA, a box of 64 channels x a page at a time: 128 threads that copy 16
+// bytes each took 2800 clocks for a tile in a scheduler's company of four softmax warps.  The others (a sequence's end, the
+// front of a window, pages outside the pool) are copied piece by piece with zeros in place of what is not there.
 template <typename C>
-__device__ __forceinline__ void fetch_tiles(Fetcher<C>& f, Pieces pieces) {
-  const TcArgs& a = f.a;
+__device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* key_map, const CUtensorMap* value_map, Pieces pieces, Barriers* bars,
+                                            volatile uint32_t* notes, uint32_t k_ring, uint32_t v_ring, uint32_t gave_up) {
+  const int p = threadIdx.x - kProducer * 32;
+  uint32_t issued = 0;
+  RingPos<C::STAGES> stage;  // of both rings
   Piece piece;
+  const PoolView keys{a.keys, a.key_scales, a.line.kv_heads, a.line.step.page_shift}, values{a.values, a.value_scales, a.line.kv_heads, a.line.step.page_shift};
   while (pieces.next(a.line, piece)) {
     const int32_t* row = a.line.step.table + int64_t(piece.sequence) * a.line.step.width;
     const int length = piece.seq.length;
     const int low = a.line.window > 0 ? visible(piece.seq.length - piece.seq.count, length, true, a.line.window).lo : 0;
-    const PoolView keys{a.keys, a.key_scales, a.line.kv_heads, a.line.step.page_shift}, values{a.values, a.value_scales, a.line.kv_heads, a.line.step.page_shift};
+    const uint32_t two = piece.seq.count * a.line.group - piece.block * kRows > 128 ? kTwoGroups : 0u;
     KeyRuns ahead;
-    ahead.look_up(row, a.line.step.page_shift, piece.first * kTileKeys, low, length);
+    ahead.look_up(row, a.line.step.page_shift, a.pages, 8, piece.first * kTileKeys, low, length);
+#pragma unroll 1
     for (int i = 0; i < piece.count; ++i) {
-      const int key0 = (piece.first + i) * kTileKeys;
-      const KeyRuns t = ahead;
-      if (i + 1 < piece.count) ahead.look_up(row, a.line.step.page_shift, key0 + kTileKeys, low, length);
-      const uint32_t bad = t.bad(a.pages);
-      const uint32_t note = bad | (i == 0 ? kFirst : 0u) | (i + 1 == piece.count ? kLast : 0u) |
-                            (piece.seq.count * a.line.group - piece.block * kRows > 128 ? kTwoGroups : 0u);
-      const uint32_t k_to = f.k_ring + f.k.stage * C::SIDE, v_to = f.v_ring + f.v.stage * C::SIDE;
-      if constexpr (C::INT8) {
-        // scaled and rounded to the queries' type (half a step), as if the cache had held 16-bit values
-        CodeTile<typename C::T, C::D> codes;
-        codes.load(keys, t, bad, piece.head, f.p);
-        if (!f.wait_stage(f.bars->k_empty, f.k.stage, f.k.phase, 1001)) return;
-        codes.store(k_to, f.p);
-        fence_async_smem();
-        mbar_arrive(smem_u32(f.bars->k_full + f.k.stage));
-        codes.load(values, t, bad, piece.head, f.p);
-        if (!f.wait_stage(f.bars->v_empty, f.v.stage, f.v.phase, 1002)) return;
-        codes.store(v_to, f.p);
-        fence_async_smem();
-        mbar_arrive(smem_u32(f.bars->v_full + f.v.stage));
-      } else {
-        if (!f.wait_stage(f.bars->k_empty, f.k.stage, f.k.phase, 1001)) return copies_drain();
-        copy_keys<C::D>(keys, t, bad, piece.head, k_to, f.p);
-        copies_arrive(smem_u32(f.bars->k_full + f.k.stage));
-        if (!f.wait_stage(f.bars->v_empty, f.v.stage, f.v.phase, 1002)) return copies_drain();
-        copy_keys<C::D>(values, t, bad, piece.head, v_to, f.p);
-        copies_arrive(smem_u32(f.bars->v_full + f.v.stage));
+      const KeyRuns runs = ahead;
+      if (i + 1 < piece.count) ahead.look_up(row, a.line.step.page_shift, a.pages, 8, runs.key0 + kTileKeys, low, length);
+#pragma unroll 1
+      for (int side = 0; side < 2; ++side) {  // K, then V
+        uint64_t* full = side ? bars->v_full : bars->k_full;
+        uint64_t* empty = side ? bars->v_empty : bars->k_empty;
+        const uint32_t to = (side ? v_ring : k_ring) + stage.stage * C::SIDE;
+        if (!mbar_wait(smem_u32(empty + stage.stage), stage.phase ^ 1, gave_up, 1001 + side)) {
+          // what is under way lands before the CTA ends (a stage that was never filled passes at once)
+          copies_drain();
+          for (int i = 0; i < C::STAGES; ++i) {
+            mbar_drain(smem_u32(bars->k_full + i), i < stage.stage + side ? stage.phase : stage.phase ^ 1);
+            mbar_drain(smem_u32(bars->v_full + i), i < stage.stage ? stage.phase : stage.phase ^ 1);
+          }
+          return;
+        }
+        if constexpr (C::INT8) {
+          // scaled and rounded to the queries' type (half a step), as if the cache had held 16-bit values
+          convert_keys<typename C::T, C::D, kTileKeys, true>(side ? values : keys, runs, piece.head, to, 0, p);
+          fence_async_smem();
+          mbar_arrive(smem_u32(full + stage.stage));
+        } else if (runs.bad == 0 && runs.key0 >= low && runs.key0 + kTileKeys <= length) {
+          const uint32_t bar = smem_u32(full + stage.stage);
+          const int shift = a.line.step.page_shift, page = __shfl_sync(0xffffffffu, runs.id, (p << (shift - 4)) & 31);
+          if (p == 0) mbar_expect_tx(bar, C::SIDE);
+          else mbar_arrive(bar);
+          __syncwarp();
+          if (p < kTileKeys >> shift) {
+#pragma unroll
+            for (int c = 0; c < C::D; c += 64)
+              tma_load_3d(to + (c >> 6) * 16384 + (p << shift) * 128, side ? value_map : key_map, bar, c, 0, page * a.line.kv_heads + piece.head);
+          }
+        } else {
+          copy_keys<C::D, kTileKeys>(side ? values : keys, runs, piece.head, to, 0, p);
+          copies_arrive(smem_u32(full + stage.stage));
+        }
+        if (side == 0 && p == 0) {
+          notes[issued % kNotes] = runs.bad | (i == 0 ? kFirst : 0u) | (i + 1 == piece.count ? kLast : 0u) | two;
+          if (runs.bad) atomicCAS(a.status, 0u, unsigned(piece.sequence) + 1u);
+          mbar_arrive(smem_u32(bars->k_full + stage.stage));  // the note is there
+        }
       }
-      if (f.p == 0) {
-        f.notes[f.issued % kNotes] = note;
-        if (bad) atomicCAS(a.status, 0u, unsigned(piece.sequence) + 1u);
-        mbar_arrive(smem_u32(f.bars->k_full + f.k.stage));  // the note is there
-      }
-      f.k.next();
-      f.v.next();
-      ++f.issued;
+      stage.next();
+      ++issued;
     }
   }
-  if (!C::INT8) copies_drain();
+  copies_drain();
 }
 
 // ---- the issuing warp ---------------------------------------------------------------------------------------------
-// Goes by the tiles' notes alone (written before K is handed over): where a unit's tiles begin and end, and whether its
-// second row group has rows.
+// It goes by the tiles' notes alone (written before K is handed over): where a unit's tiles begin and end, and whether the
+// second row group has rows.  One warp issues for both groups, in a fixed order, so that they take turns: with a warp each the
+// pipe served both at half speed, the groups' softmaxes fell into step and fought for the special-function unit (tile period
+// 5500 clocks).
 template <typename C>
-__device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const volatile uint32_t* notes, uint32_t tmem, uint32_t q,
-                                               uint32_t k_ring, uint32_t v_ring, uint32_t gave_up) {
+__device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const volatile uint32_t* notes, uint32_t tmem, uint32_t q, uint32_t k_ring,
+                                               uint32_t v_ring, uint32_t gave_up) {
   constexpr uint32_t kScores = idesc_f16<typename C::T>(false, kTileKeys), kOutput = idesc_f16<typename C::T>(true, C::D);
   RingPos<C::STAGES> k, v;
   uint32_t q_phase = 0, p_phase = 0, o_phase = 3;  // a bit per group
@@ -134,19 +146,21 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
   auto scores = [&](int g) {
     fence_async_smem();  // K's copies, which the barrier has told of
     if (!elected) return;
-    const uint32_t rows_q = along_row(q + g * C::SIDE), rows_k = along_row(k_ring + k.stage * C::SIDE);
+    const uint32_t rows_q = along_row(q + g * C::SIDE), rows_k = along_row(k_ring + k.stage * C::SIDE), to = tmem + g * kTileKeys;
+    mma_f16<false>(to, descriptor(rows_q), descriptor(rows_k), kScores);
 #pragma unroll
-    for (int c = 0; c < C::D / 16; ++c) {
+    for (int c = 1; c < C::D / 16; ++c) {
       const uint32_t at = (c >> 2) * 1024 + (c & 3) * 2;
-      mma_f16(tmem + g * kTileKeys, descriptor(rows_q + at), descriptor(rows_k + at), kScores, c > 0);
+      mma_f16<true>(to, descriptor(rows_q + at), descriptor(rows_k + at), kScores);
     }
     mma_commit(smem_u32(bars->s_full + g));
   };
   for (int tile = 0; tile < tiles; ++tile) {
     if (tile == 0 && !mbar_wait(smem_u32(bars->k_full + k.stage), k.phase, gave_up, 1010)) return;
     const uint32_t note = notes[tile % kNotes];
+    const bool first = note & kFirst, last = note & kLast;
     const int groups = note & kTwoGroups ? 2 : 1;
-    if (note & kFirst) {
+    if (first) {
       for (int g = 0; g < groups; ++g) {
         if (!mbar_wait(smem_u32(bars->q_full + g), q_phase >> g & 1, gave_up, 1011)) return;
         q_phase ^= 1u << g;
@@ -156,10 +170,9 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
       if (elected) mma_commit(smem_u32(bars->k_empty + k.stage));
       k.next();
     }
-    const bool last = note & kLast;
     for (int g = 0; g < groups; ++g) {
       if (g == 0 && !mbar_wait(smem_u32(bars->v_full + v.stage), v.phase, gave_up, 1012)) return;
-      if (note & kFirst) {  // the previous unit's output has been read
+      if (first) {  // the previous unit's output has been read
         if (!mbar_wait(smem_u32(bars->o_free + g), o_phase >> g & 1, gave_up, 1013)) return;
         o_phase ^= 1u << g;
       }
@@ -171,14 +184,13 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
         const uint32_t rows_v = across_rows(v_ring + v.stage * C::SIDE);
 #pragma unroll
         for (int c = 0; c < kTileKeys / 16; ++c)
-          mma_f16_tmem(tmem + kGroups * kTileKeys + g * C::D, tmem + g * kTileKeys + c * 8, descriptor(rows_v + c * 128), kOutput,
-                       c > 0 || !(note & kFirst));
+          mma_f16_tmem(tmem + kGroups * kTileKeys + g * C::D, tmem + g * kTileKeys + c * 8, descriptor(rows_v + c * 128), kOutput, c > 0 || !first);
         if (last) mma_commit(smem_u32(bars->o_full + g));
         if (g == groups - 1) mma_commit(smem_u32(bars->v_empty + v.stage));
       }
       if (!last) {
         if (g == 0 && !mbar_wait(smem_u32(bars->k_full + k.stage), k.phase, gave_up, 1015)) return;
-        scores(g);
+        scores(g);  // behind the product that reads P from these columns
         if (g == groups - 1) {
           if (elected) mma_commit(smem_u32(bars->k_empty + k.stage));
           k.next();
@@ -190,17 +202,22 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
   }
 }
 
-// ---- a softmax warpgroup ---------------------------------------------------------------------------------------------
-// Query rows of group g: 16-byte pieces, neighbouring threads along a row.  A negative scale flips their signs, so that
-// the maximum of the scores is the maximum of the scaled ones.
+// ---- the softmax warpgroups -------------------------------------------------------------------------------------------
+// A meeting of the two warps that own the same 32 rows.  One that leaves early arrives once more on its way out, so the
+// other is never kept waiting.
+__device__ __forceinline__ void meet(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void leave(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
+
+// Query rows of group g, by the 256 threads of its two warpgroups: 16-byte pieces, neighbouring threads along a row.  A
+// negative scale flips their signs, so that the maximum of the scores is the maximum of the scaled ones.
 template <typename C>
 __device__ __forceinline__ void load_query_rows(const TcArgs& a, const Piece& piece, int g, uint32_t to) {
-  constexpr int PIECES = C::D / 8;
-  const int t = threadIdx.x & 127, rows = piece.seq.count * a.line.group;
+  constexpr int PIECES = C::D / 8, EACH = 256 / PIECES;
+  const int t = threadIdx.x & 255, rows = piece.seq.count * a.line.group, c = t % PIECES;
   const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
 #pragma unroll 4
-  for (int n = 0; n < PIECES; ++n) {
-    const int index = n * 128 + t, r = index / PIECES, c = index % PIECES, row = piece.block * kRows + g * 128 + r;
+  for (int r = t / PIECES; r < 128; r += EACH) {
+    const int row = piece.block * kRows + g * 128 + r;
     uint4 v = make_uint4(0, 0, 0, 0);
     if (row < rows) {
       const int token = row / a.line.group, h = row - token * a.line.group;
@@ -217,13 +234,13 @@ __device__ __forceinline__ void load_query_rows(const TcArgs& a, const Piece& pi
 }
 
 template <typename C>
-__device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Barriers* bars, uint32_t tmem, uint32_t q, int g,
+__device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Barriers* bars, Exchange* exchange, uint32_t tmem, uint32_t q, int g, int half,
                                              const volatile uint32_t* notes, uint32_t gave_up) {
-  constexpr int D = C::D;
+  constexpr int D = C::D, KEYS = kTileKeys / 2;
   using T = typename C::T;
-  const int r = threadIdx.x & 127;
+  const int r = threadIdx.x & 127, meeting = 1 + g * 4 + (r >> 5);
   const uint32_t lanes = tmem + (uint32_t(r & ~31) << 16);
-  const uint32_t s_columns = lanes + g * kTileKeys, o_columns = lanes + kGroups * kTileKeys + g * D;
+  const uint32_t s_columns = lanes + g * kTileKeys, o_columns = lanes + kGroups * kTileKeys + g * D + half * (D / 2);
   const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // a scale of 0 must leave hidden scores at -inf
   uint32_t s_phase = 0, o_phase = 0, tile = 0;
   Piece piece;
@@ -242,61 +259,66 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
       continue;
     }
     const int rows = piece.seq.count * a.line.group, row = piece.block * kRows + g * 128 + r;
-    const int token = row / a.line.group, h = piece.head * a.line.group + row - token * a.line.group;
-    KeyRange seen = visible(piece.seq.length - piece.seq.count + token, piece.seq.length, a.line.causal, a.line.window);
+    KeyRange seen = visible(piece.seq.length - piece.seq.count + row / a.line.group, piece.seq.length, a.line.causal, a.line.window);
     if (row >= rows) seen = {0, 0};
     // keys that every row of the group sees need no test
     const int token0 = (piece.block * kRows + g * 128) / a.line.group, token1 = (min(piece.block * kRows + g * 128 + 128, rows) - 1) / a.line.group;
     const int all_hi = visible(piece.seq.length - piece.seq.count + token0, piece.seq.length, a.line.causal, a.line.window).hi;
     const int all_lo = visible(piece.seq.length - piece.seq.count + token1, piece.seq.length, a.line.causal, a.line.window).lo;
     float m = kNoMaximum, l = 0.f;
+#pragma unroll 1
     for (int i = 0; i < piece.count; ++i, ++tile) {
-      const int key0 = (piece.first + i) * kTileKeys;
-      if (!mbar_wait(smem_u32(bars->s_full + g), s_phase, gave_up, 1020 + g)) return;
+      const int key0 = (piece.first + i) * kTileKeys + half * KEYS;
+      if (!mbar_wait(smem_u32(bars->s_full + g), s_phase, gave_up, 1020 + g)) return leave(meeting);
       s_phase ^= 1;
       tc_fence_after();
-      uint32_t x[kTileKeys];
-#pragma unroll
-      for (int c = 0; c < kTileKeys / 32; ++c) tmem_load32(s_columns + c * 32, x + c * 32);
-      const uint32_t gone = notes[tile % kNotes] & kHiddenRuns;
+      uint32_t x[KEYS];
+      tmem_load32(s_columns + half * KEYS, x);
+      tmem_load32(s_columns + half * KEYS + 32, x + 32);
+      const uint32_t gone = notes[tile % kNotes] >> (half * 4) & (kHiddenRuns >> 4);
       tmem_load_wait();
-      tmem_regs_ready<kTileKeys>(x);
-      if (gone != 0 || key0 < all_lo || key0 + kTileKeys > all_hi) {
+      tmem_regs_ready<KEYS>(x);
+      if (gone != 0 || key0 < all_lo || key0 + KEYS > all_hi) {
+        asm volatile("" ::: "memory");  // a branch of its own: as selects in the common path it cost a quarter of the time
         const int lo = seen.lo - key0, hi = seen.hi - key0;
 #pragma unroll
-        for (int c = 0; c < kTileKeys; ++c)
+        for (int c = 0; c < KEYS; ++c)
           if (c < lo || c >= hi || (gone >> (c >> 4) & 1)) x[c] = 0xff800000u;
       }
       float top[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
 #pragma unroll
-      for (int c = 4; c < kTileKeys; c += 8)
+      for (int c = 4; c < KEYS; c += 8)
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-          top[e] = c + 4 + e < kTileKeys ? fmaxf(fmaxf(top[e], __uint_as_float(x[c + e])), __uint_as_float(x[c + 4 + e]))
-                                         : fmaxf(top[e], __uint_as_float(x[c + e]));
-      const float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+          top[e] = c + 4 + e < KEYS ? fmaxf(fmaxf(top[e], __uint_as_float(x[c + e])), __uint_as_float(x[c + 4 + e]))
+                                    : fmaxf(top[e], __uint_as_float(x[c + e]));
+      float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+      // also: from here on both halves of the scores are in registers, and P may be written over them
+      exchange->maximum[tile & 1][g][half][r] = best;
+      meet(meeting);
+      best = fmaxf(best, exchange->maximum[tile & 1][g][half ^ 1][r]);
       const bool moves = best > m + kStale;
       if (__any_sync(0xffffffffu, moves)) {
         const float to = moves ? best : m, keep = ex2_approx(m - to);
         m = to;
         l *= keep;
         if (i > 0) {  // scores of this tile were issued behind the product with the last one, so that is complete
-#pragma unroll
-          for (int c = 0; c < D / 16; ++c) {
+#pragma unroll 1
+          for (int c = 0; c < D / 2; c += 16) {
             uint32_t o[16];
-            tmem_load16(o_columns + c * 16, o);
+            tmem_load16(o_columns + c, o);
             tmem_load_wait();
             tmem_regs_ready<16>(o);
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[e] = __float_as_uint(__uint_as_float(o[e]) * keep);
-            tmem_store16(o_columns + c * 16, o);
+            tmem_store16(o_columns + c, o);
           }
         }
       }
       const uint64_t scale2 = pack_f32x2(scale, scale), minus_m = pack_f32x2(-m, -m);
       uint64_t sum[2] = {0, 0};
 #pragma unroll
-      for (int part = 0; part < 4; ++part) {
+      for (int part = 0; part < KEYS / 32; ++part) {
         uint32_t p[16];
 #pragma unroll
         for (int c = 0; c < 16; ++c) {
@@ -308,7 +330,7 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
           sum[c & 1] = add_f32x2(sum[c & 1], pack_f32x2(u, w));
           p[c] = Half2<T>::pack(u, w);
         }
-        tmem_store16(s_columns + part * 16, p);
+        tmem_store16(s_columns + half * (KEYS / 2) + part * 16, p);
       }
       float s0, s1;
       unpack_f32x2(add_f32x2(sum[0], sum[1]), s0, s1);
@@ -321,50 +343,48 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
     const Piece done = piece;
     more = pieces.next(a.line, piece);
     if (more && mine(piece)) fetch(piece);
-    if (!mbar_wait(smem_u32(bars->o_full + g), o_phase, gave_up, 1022 + g)) return;
+    exchange->sum[g][half][r] = l;
+    meet(meeting);
+    l += exchange->sum[g][half ^ 1][r];
+    if (!mbar_wait(smem_u32(bars->o_full + g), o_phase, gave_up, 1022 + g)) return leave(meeting);
     o_phase ^= 1;
     tc_fence_after();
     const bool there = row < rows;
-    if (done.whole) {
-      const float f = l == 0.f ? 0.f : 1.0f / l;
-      T* out = static_cast<T*>(a.out) + int64_t(done.seq.first + token) * a.on + int64_t(h) * a.oh;
+    const int token = row / a.line.group, h = done.head * a.line.group + row - token * a.line.group;
+    const float f = l == 0.f ? 0.f : 1.0f / l;
+    T* out = static_cast<T*>(a.out) + int64_t(done.seq.first + token) * a.on + int64_t(h) * a.oh + half * (D / 2);
+    float* slot = a.parts + (int64_t(blockIdx.x) * 2 + (done.opens ? 1 : 0)) * slot_floats(kRows, D);
+    const int in_block = g * 128 + r;
+#pragma unroll 1
+    for (int c = 0; c < D / 2; c += 16) {
+      uint32_t o[16];
+      tmem_load16(o_columns + c, o);
+      tmem_load_wait();
+      tmem_regs_ready<16>(o);
+      if (!there) continue;
+      if (done.whole) {
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_load32(o_columns + c * 32, o);
-        tmem_load_wait();
-        tmem_regs_ready<32>(o);
-        if (there) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            uint4 w;
-            w.x = Half2<T>::pack(__uint_as_float(o[8 * e]) * f, __uint_as_float(o[8 * e + 1]) * f);
-            w.y = Half2<T>::pack(__uint_as_float(o[8 * e + 2]) * f, __uint_as_float(o[8 * e + 3]) * f);
-            w.z = Half2<T>::pack(__uint_as_float(o[8 * e + 4]) * f, __uint_as_float(o[8 * e + 5]) * f);
-            w.w = Half2<T>::pack(__uint_as_float(o[8 * e + 6]) * f, __uint_as_float(o[8 * e + 7]) * f);
-            *reinterpret_cast<uint4*>(out + c * 32 + e * 8) = w;
-          }
+        for (int e = 0; e < 16; e += 8) {
+          uint4 w;
+          w.x = Half2<T>::pack(__uint_as_float(o[e]) * f, __uint_as_float(o[e + 1]) * f);
+          w.y = Half2<T>::pack(__uint_as_float(o[e + 2]) * f, __uint_as_float(o[e + 3]) * f);
+          w.z = Half2<T>::pack(__uint_as_float(o[e + 4]) * f, __uint_as_float(o[e + 5]) * f);
+          w.w = Half2<T>::pack(__uint_as_float(o[e + 6]) * f, __uint_as_float(o[e + 7]) * f);
+          *reinterpret_cast<uint4*>(out + c + e) = w;
         }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+          *reinterpret_cast<uint4*>(slot + int64_t(in_block) * D + half * (D / 2) + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
       }
-      if (there && a.lse != nullptr)
+    }
+    if (half == 0 && there) {
+      if (!done.whole) {
+        slot[kRows * D + in_block] = m;
+        slot[kRows * D + kRows + in_block] = l;
+      } else if (a.lse != nullptr) {
         a.lse[int64_t(done.seq.first + token) * (a.line.kv_heads * a.line.group) + h] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
-    } else {
-      float* slot = a.parts + (int64_t(blockIdx.x) * 2 + (done.opens ? 1 : 0)) * slot_floats(kRows, D);
-      const int in_block = g * 128 + r;
-#pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        uint32_t o[32];
-        tmem_load32(o_columns + c * 32, o);
-        tmem_load_wait();
-        tmem_regs_ready<32>(o);
-        if (there) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e)
-            *reinterpret_cast<uint4*>(slot + int64_t(in_block) * D + c * 32 + e * 4) = make_uint4(o[4 * e], o[4 * e + 1], o[4 * e + 2], o[4 * e + 3]);
-        }
       }
-      slot[kRows * D + in_block] = m;
-      slot[kRows * D + kRows + in_block] = l;
     }
     tc_fence_before();
     mbar_arrive_warp(smem_u32(bars->o_free + g));
@@ -372,9 +392,10 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
 }
 
 template <typename C>
-__global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const TcArgs a) {
+__global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_constant__ CUtensorMap key_map, const __grid_constant__ CUtensorMap value_map, const TcArgs a) {
   extern __shared__ char smem_raw[];
   __shared__ Barriers bars;
+  __shared__ Exchange exchange;
   __shared__ LineShared<kThreads> shared;
   __shared__ uint32_t tmem_base, gave_up_word;
   __shared__ volatile uint32_t notes[kNotes];
@@ -390,11 +411,11 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const TcArgs a) {
       mbar_init(smem_u32(bars.v_empty + i), 1);
     }
     for (int g = 0; g < kGroups; ++g) {
-      mbar_init(smem_u32(bars.q_full + g), 4);
+      mbar_init(smem_u32(bars.q_full + g), 8);
       mbar_init(smem_u32(bars.s_full + g), 1);
-      mbar_init(smem_u32(bars.p_full + g), 4);
+      mbar_init(smem_u32(bars.p_full + g), 8);
       mbar_init(smem_u32(bars.o_full + g), 1);
-      mbar_init(smem_u32(bars.o_free + g), 4);
+      mbar_init(smem_u32(bars.o_free + g), 8);
     }
     mbar_init(smem_u32(&bars.drained), 1);
     mbar_init_fence();
@@ -413,11 +434,10 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const TcArgs a) {
   const uint32_t tmem = tmem_base;
   if (warp < kProducer) {
     regs_inc<kRegsSoftmax>();
-    softmax_rows<C>(a, pieces, &bars, tmem, q, warp >> 2, notes, gave_up);
+    softmax_rows<C>(a, pieces, &bars, &exchange, tmem, q, warp >> 3, (warp >> 2) & 1, notes, gave_up);
   } else if (warp < kIssuer) {
     regs_dec<kRegsProducer>();
-    Fetcher<C> f{a, &bars, notes, v_ring, k_ring, gave_up, int(threadIdx.x) - kProducer * 32, 0};
-    fetch_tiles<C>(f, pieces);
+    fetch_tiles<C>(a, &key_map, &value_map, pieces, &bars, notes, k_ring, v_ring, gave_up);
   } else {
     regs_dec<kRegsIssuer>();
     if (warp == kIssuer) {
@@ -433,7 +453,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const TcArgs a) {
   __syncthreads();
   tc_fence_after();
   if (warp == kIssuer) tmem_dealloc(tmem, 512);
-  if (gave_up_word != 0 && threadIdx.x < 256) {
+  if (gave_up_word != 0 && threadIdx.x < kRows) {
     // a wait ran out: the rows of this worker's whole units are marked, parts poison their join
     Pieces all = pieces;
     Piece piece;
@@ -452,8 +472,35 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const TcArgs a) {
   }
 }
 
+// The pool as {channels, a page's rows, pages x heads}, in boxes of 64 channels x a page with the 128-byte swizzle.
+using EncodeFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                              const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeFn encode_fn() {
+  static const EncodeFn fn = [] {
+    void* ptr = nullptr;
+    cudaDriverEntryPointQueryResult result;
+    const bool good = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &result) == cudaSuccess && result == cudaDriverEntryPointSuccess;
+    return good ? reinterpret_cast<EncodeFn>(ptr) : nullptr;
+  }();
+  return fn;
+}
+template <typename C>
+bool pool_map(CUtensorMap* map, const char* pool, const TcArgs& a) {
+  const cuuint64_t dims[3] = {cuuint64_t(C::D), cuuint64_t(1) << a.line.step.page_shift, cuuint64_t(a.pages) * a.line.kv_heads};
+  const cuuint64_t strides[2] = {cuuint64_t(C::D) * 2, (cuuint64_t(C::D) * 2) << a.line.step.page_shift};
+  const cuuint32_t box[3] = {64, 1u << a.line.step.page_shift, 1}, ones[3] = {1, 1, 1};
+  return encode_fn()(map, std::is_same<typename C::T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
+                     const_cast<char*>(pool), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                     CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <typename C>
 int launch(const TcArgs& a, cudaStream_t stream) {
+  CUtensorMap key_map{}, value_map{};
+  RISA_REQUIRE(int64_t(a.pages) * a.line.kv_heads < (int64_t(1) << 31), "paged attention: the pool has too many pages");
+  if (!C::INT8)
+    if (encode_fn() == nullptr || !pool_map<C>(&key_map, a.keys, a) || !pool_map<C>(&value_map, a.values, a))
+      return fail(RISA_B200_CUDA, "paged attention: no tensor map of the pool");
   if (cudaFuncSetAttribute(paged_tc_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
     return fail(RISA_B200_CUDA, "paged attention: %s", cudaGetErrorString(cudaGetLastError()));
   // setmaxnreg deals out what the CTA was launched with; a smaller launch count would block its waits for ever
@@ -462,7 +509,7 @@ int launch(const TcArgs& a, cudaStream_t stream) {
     return cudaFuncGetAttributes(&attributes, paged_tc_kernel<C>) == cudaSuccess && attributes.numRegs == kRegsLaunch;
   }();
   RISA_REQUIRE(budget, "paged attention: the tensor-core kernel was not compiled for %d registers", kRegsLaunch);
-  launch_chained(paged_tc_kernel<C>, dim3(kTcWorkers), dim3(kThreads), C::SMEM, stream, a);
+  launch_chained(paged_tc_kernel<C>, dim3(kTcWorkers), dim3(kThreads), C::SMEM, stream, key_map, value_map, a);
   const JoinArgs join{a.line, a.parts, kTcWorkers, a.min_steps, a.out, a.on, a.oh, a.lse};
   launch_chained(join_parts_kernel<typename C::T, C::D>, dim3(kTcWorkers - 1, kRows / 4), dim3(128), 0, stream, join);
   return RISA_B200_OK;

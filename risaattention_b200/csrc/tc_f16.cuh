@@ -22,10 +22,12 @@ constexpr uint32_t kDescHigh = (1024 >> 4) | 1u << 14 | 2u << 29;
 __device__ __forceinline__ uint64_t descriptor(uint32_t low) { return uint64_t(kDescHigh) << 32 | low; }
 __device__ __forceinline__ uint32_t along_row(uint32_t address) { return (address & 0x3ffffu) >> 4 | 1u << 16; }
 __device__ __forceinline__ uint32_t across_rows(uint32_t address) { return (address & 0x3ffffu) >> 4 | uint32_t(16384 >> 4) << 16; }
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
+// One thread issues.
+template <bool ACCUMULATE>
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
   asm volatile(
       "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "n"(ACCUMULATE ? 1 : 0)
       : "memory");
 }
 // A from tensor memory: two 16-bit values along K per column.
@@ -81,28 +83,9 @@ __device__ __forceinline__ void store_codes(uint32_t tile, int row, int piece, u
                        scaled_pair<T>(u[2 * h + 1], 1, scale)));
 }
 
-// ---- 128 keys of a paged sequence into a tile, by the 128 threads of a warpgroup ----------------------------------------
-// Page numbers of eight runs of 16 keys, and where they lie.
-struct KeyRuns {
-  int id[8];
-  int key0, low, length;  // keys [low, length) exist
-  __device__ __forceinline__ bool exists(int i) const { return key0 + 16 * i < length && key0 + 16 * i + 16 > low; }
-  __device__ __forceinline__ void look_up(const int32_t* row, int page_shift, int first_key, int first_existing, int sequence_length) {
-    key0 = first_key;
-    low = first_existing;
-    length = sequence_length;
-#pragma unroll
-    for (int i = 0; i < 8; ++i) id[i] = exists(i) ? __ldg(row + ((key0 + 16 * i) >> page_shift)) : -1;
-  }
-  // Runs whose page is outside the pool although a key of theirs exists.
-  __device__ __forceinline__ uint32_t bad(int pages) const {
-    uint32_t bits = 0;
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-      if (exists(i) && (id[i] < 0 || id[i] >= pages)) bits |= 1u << i;
-    return bits;
-  }
-};
+// ---- keys of a paged sequence into tiles, by the 128 threads of a warpgroup ------------------------------------------------
+// The code is short on purpose: what a CTA runs for the first time it first has to fetch, and unrolled copies were 10 us of
+// instruction fetches in front of the first product.
 struct PoolView {
   const char* rows;
   const float* scales;
@@ -112,52 +95,61 @@ struct PoolView {
     return ((int64_t(id) * kv_heads + head) << page_shift) + (key & ((1 << page_shift) - 1));
   }
 };
+// Keys [low, length) of a sequence exist.  Lane i of every warp knows the page of the i-th run of 16 keys from key0 on, -1
+// where there is none; `bad`: runs whose page is outside the pool although a key of theirs exists.
+struct KeyRuns {
+  int key0, low, length, id;
+  uint32_t bad;
+  __device__ __forceinline__ void look_up(const int32_t* row, int page_shift, int pages, int runs, int first_key, int first_existing, int sequence_length) {
+    key0 = first_key;
+    low = first_existing;
+    length = sequence_length;
+    const int lane = threadIdx.x & 31, key = key0 + 16 * lane;
+    const bool exists = lane < runs && key < length && key + 16 > low;
+    id = exists ? __ldg(row + (key >> page_shift)) : -1;
+    bad = __ballot_sync(0xffffffffu, exists && (id < 0 || id >= pages));
+    if (id >= pages) id = -1;
+  }
+};
 
-// 16-bit rows: 16 bytes at a time straight into place; rows that are not there become zeros (a stale NaN in V would spoil
-// the product with a probability of 0).
-template <int D>
-__device__ __forceinline__ void copy_keys(const PoolView& pool, const KeyRuns& k, uint32_t bad, int head, uint32_t to, int thread) {
-  constexpr int PIECES = D / 8;             // of a row
-  constexpr int PER_RUN = 16 * PIECES / 128;  // pieces of a run per thread
+// 16-bit rows: 16 bytes at a time straight into place, ROWS of them (tiles of 128 lie `tile_bytes` apart); rows that are not
+// there become zeros (a stale NaN in V would spoil the product with a probability of 0).
+template <int D, int ROWS>
+__device__ __forceinline__ void copy_keys(const PoolView& pool, const KeyRuns& k, int head, uint32_t to, int tile_bytes, int thread) {
+  constexpr int PIECES = D / 8, EACH = 128 / PIECES;  // rows that the warpgroup copies at a time
+  const int piece = thread % PIECES;
+#pragma unroll 4
+  for (int r = thread / PIECES; r < ROWS; r += EACH) {
+    const int key = k.key0 + r, page = __shfl_sync(0xffffffffu, k.id, r >> 4);
+    const bool there = page >= 0 && key >= k.low && key < k.length;
+    const int64_t line = there ? pool.line(page, head, key) : 0;
+    copy16(to + (ROWS > 128 ? (r >> 7) * tile_bytes : 0) + tile_offset(r & 127, piece), pool.rows + line * (D * 2) + piece * 16, there);
+  }
+}
+// Codes: 16 of them per load, as 16-bit values; with SCALED times their row's scale.
+template <typename T, int D, int ROWS, bool SCALED>
+__device__ __forceinline__ void convert_keys(const PoolView& pool, const KeyRuns& k, int head, uint32_t to, int tile_bytes, int thread) {
+  constexpr int PIECES = D / 16, EACH = 128 / PIECES, BATCH = 4;
+  const int piece = thread % PIECES;
+#pragma unroll 1
+  for (int r0 = thread / PIECES; r0 < ROWS; r0 += BATCH * EACH) {
+    uint4 codes[BATCH];
+    float scale[BATCH];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const bool run = !(bad >> i & 1) && k.id[i] >= 0;
-    const char* from = pool.rows + (run ? pool.line(k.id[i], head, k.key0 + 16 * i) * (D * 2) : 0);
+    for (int n = 0; n < BATCH; ++n) {
+      const int r = r0 + n * EACH, key = k.key0 + r, page = __shfl_sync(0xffffffffu, k.id, r >> 4);
+      const bool there = page >= 0 && key >= k.low && key < k.length;
+      const int64_t line = there ? pool.line(page, head, key) : 0;
+      codes[n] = there ? *reinterpret_cast<const uint4*>(pool.rows + line * D + piece * 16) : make_uint4(0, 0, 0, 0);
+      scale[n] = !SCALED ? 1.0f : there ? pool.scales[line] : 0.f;
+    }
 #pragma unroll
-    for (int j = 0; j < PER_RUN; ++j) {
-      const int index = j * 128 + thread, r = index / PIECES, piece = index % PIECES, key = k.key0 + 16 * i + r;
-      copy16(to + tile_offset(16 * i + r, piece), from + index * 16, run && key >= k.low && key < k.length);
+    for (int n = 0; n < BATCH; ++n) {
+      const int r = r0 + n * EACH;
+      store_codes<T>(to + (ROWS > 128 ? (r >> 7) * tile_bytes : 0), r & 127, piece, codes[n], scale[n]);
     }
   }
 }
-
-// Codes: 16 of them per load; `store` multiplies by their row's scale and rounds to T.
-template <typename T, int D>
-struct CodeTile {
-  static constexpr int PIECES = D / 16, LOADS = PIECES;
-  uint4 codes[LOADS];
-  float scale[LOADS];
-  __device__ __forceinline__ void load(const PoolView& pool, const KeyRuns& k, uint32_t bad, int head, int thread) {
-#pragma unroll
-    for (int n = 0; n < LOADS; ++n) {
-      const int index = n * 128 + thread, row = index / PIECES, piece = index % PIECES, i = row >> 4, key = k.key0 + row;
-      // a load of the warpgroup covers 128 / PIECES rows: one run of 16, or two at 64 channels
-      constexpr int RUNS = 128 / PIECES / 16;
-      const int id = RUNS <= 1 ? k.id[n * 128 / PIECES / 16] : (i == n * 2 ? k.id[(n * 2) & 7] : k.id[(n * 2 + 1) & 7]);
-      const bool there = !(bad >> i & 1) && id >= 0 && key >= k.low && key < k.length;
-      const int64_t line = pool.line(id, head, key);
-      codes[n] = there ? *reinterpret_cast<const uint4*>(pool.rows + line * D + piece * 16) : make_uint4(0, 0, 0, 0);
-      scale[n] = there ? pool.scales[line] : 0.f;
-    }
-  }
-  __device__ __forceinline__ void store(uint32_t to, int thread) const {
-#pragma unroll
-    for (int n = 0; n < LOADS; ++n) {
-      const int index = n * 128 + thread, row = index / PIECES, piece = index % PIECES;
-      store_codes<T>(to, row, piece, codes[n], scale[n]);
-    }
-  }
-};
 
 }  // namespace serving
 }  // namespace risa_b200

@@ -113,44 +113,27 @@ struct Notes {
   float half[4][2][128];
 };
 
-// A worker's key blocks.  A short loop: it runs once in many tiles, and unrolled it was 7 us of instruction fetches in front
-// of the first product.
+// A worker's key blocks.
 template <typename C>
 __device__ __forceinline__ void fetch_keys(const WeighArgs& a, Pieces pieces, Barriers* bars, volatile Notes* notes, uint32_t keys, uint32_t gave_up) {
-  constexpr int PIECES = C::D / (C::INT8 ? 16 : 8), EACH = 128 / PIECES;  // rows that the warpgroup fetches at a time
-  const int p = threadIdx.x - kKeyFetcher * 32, lane = p & 31, piece = p % PIECES;
+  const int p = threadIdx.x - kKeyFetcher * 32;
   RingPos<C::KEY_BUFFERS> kb;
   uint32_t block = 0;
   Piece at;
   while (pieces.next(a.line, at)) {
     const int32_t* row = a.line.step.table + int64_t(at.sequence) * a.line.step.width;
     const int low = first_seen(a.line, at.seq), length = at.seq.length, key0 = (low / kBlockKeys + at.block) * kBlockKeys;
-    // lane i knows the page of the block's i-th run of 16 keys
-    const int run = key0 + 16 * lane;
-    const bool exists = lane < kBlockKeys / 16 && run < length && run + 16 > low;
-    int id = exists ? __ldg(row + (run >> a.line.step.page_shift)) : -1;
-    const uint32_t bad = __ballot_sync(0xffffffffu, exists && (id < 0 || id >= a.pages));
-    if (id >= a.pages) id = -1;
+    KeyRuns runs;
+    runs.look_up(row, a.line.step.page_shift, a.pages, kBlockKeys / 16, key0, low, length);
     if (!mbar_wait(smem_u32(bars->k_empty + kb.stage), kb.phase ^ 1, gave_up, 1101)) break;
     if (p == 0) {
-      notes->bad[block % kDepth] = bad;
-      if (bad) atomicCAS(a.status, 0u, unsigned(at.sequence) + 1u);
+      notes->bad[block % kDepth] = runs.bad;
+      if (runs.bad) atomicCAS(a.status, 0u, unsigned(at.sequence) + 1u);
     }
-#pragma unroll 4
-    for (int r = p / PIECES; r < kBlockKeys; r += EACH) {
-      const int key = key0 + r, page = __shfl_sync(0xffffffffu, id, r >> 4);
-      const bool there = page >= 0 && key >= low && key < length;
-      const int64_t line = there ? a.keys.line(page, at.head, key) : 0;
-      const uint32_t to = keys + kb.stage * C::KEYS + (r >> 7) * C::GROUP;
-      if (C::INT8) {
-        // codes as they are: a key's scale multiplies its scores in 32 bits
-        uint4 w = make_uint4(0, 0, 0, 0);
-        if (there) w = *reinterpret_cast<const uint4*>(a.keys.rows + line * C::D + piece * 16);
-        store_codes<typename C::T>(to, r & 127, piece, w, 1.0f);
-      } else {
-        copy16(to + tile_offset(r & 127, piece), a.keys.rows + line * (C::D * 2) + piece * 16, there);
-      }
-    }
+    const uint32_t to = keys + kb.stage * C::KEYS;
+    // codes as they are: a key's scale multiplies its scores in 32 bits
+    if constexpr (C::INT8) convert_keys<typename C::T, C::D, kBlockKeys, false>(a.keys, runs, at.head, to, C::GROUP, p);
+    else copy_keys<C::D, kBlockKeys>(a.keys, runs, at.head, to, C::GROUP, p);
     if (C::INT8) {
       fence_async_smem();
       mbar_arrive(smem_u32(bars->k_full + kb.stage));
@@ -246,10 +229,11 @@ __device__ __forceinline__ void issue(int tiles, Barriers* bars, const volatile 
       if (!elected) continue;
       if (g < groups) {
         const uint32_t rows_k = along_row(keys + kb.stage * C::KEYS + g * C::GROUP), rows_q = along_row(queries + st.stage * C::TILE);
+        const uint32_t to = tmem + (g * 2 + buffer.stage) * 128;
+        mma_f16<false>(to, descriptor(rows_k), descriptor(rows_q), kScores);
 #pragma unroll
-        for (int c = 0; c < C::D / 16; ++c)
-          mma_f16(tmem + (g * 2 + buffer.stage) * 128, descriptor(rows_k + (c >> 2) * 1024 + (c & 3) * 2),
-                  descriptor(rows_q + (c >> 2) * (C::ROWS * 8) + (c & 3) * 2), kScores, c > 0);
+        for (int c = 1; c < C::D / 16; ++c)
+          mma_f16<true>(to, descriptor(rows_k + (c >> 2) * 1024 + (c & 3) * 2), descriptor(rows_q + (c >> 2) * (C::ROWS * 8) + (c & 3) * 2), kScores);
       }
       mma_commit(smem_u32(&bars->s_full[g][buffer.stage]));
     }
