@@ -116,7 +116,9 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
           }
         } else {
           copy_keys<C::D, kTileKeys>(side ? values : keys, runs, piece.head, to, 0, p);
-          copies_arrive(smem_u32(full + stage.stage));
+          copies_drain();
+          fence_async_smem();
+          mbar_arrive(smem_u32(full + stage.stage));
         }
         if (side == 0 && p == 0) {
           notes[issued % kNotes] = runs.bad | (i == 0 ? kFirst : 0u) | (i + 1 == piece.count ? kLast : 0u) | two;
@@ -144,14 +146,12 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
   uint32_t q_phase = 0, p_phase = 0, o_phase = 3;  // a bit per group
   const bool elected = elect_one();
   auto scores = [&](int g) {
-    fence_async_smem();  // K's copies, which the barrier has told of
     if (!elected) return;
     const uint32_t rows_q = along_row(q + g * C::SIDE), rows_k = along_row(k_ring + k.stage * C::SIDE), to = tmem + g * kTileKeys;
-    mma_f16<false>(to, descriptor(rows_q), descriptor(rows_k), kScores);
-#pragma unroll
-    for (int c = 1; c < C::D / 16; ++c) {
+#pragma unroll 2
+    for (int c = 0; c < C::D / 16; ++c) {
       const uint32_t at = (c >> 2) * 1024 + (c & 3) * 2;
-      mma_f16<true>(to, descriptor(rows_q + at), descriptor(rows_k + at), kScores);
+      mma_f16(to, descriptor(rows_q + at), descriptor(rows_k + at), kScores, c > 0);
     }
     mma_commit(smem_u32(bars->s_full + g));
   };
@@ -179,10 +179,9 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
       if (!mbar_wait(smem_u32(bars->p_full + g), p_phase >> g & 1, gave_up, 1014)) return;
       p_phase ^= 1u << g;
       tc_fence_after();
-      fence_async_smem();  // V's copies
       if (elected) {
         const uint32_t rows_v = across_rows(v_ring + v.stage * C::SIDE);
-#pragma unroll
+#pragma unroll 2
         for (int c = 0; c < kTileKeys / 16; ++c)
           mma_f16_tmem(tmem + kGroups * kTileKeys + g * C::D, tmem + g * kTileKeys + c * 8, descriptor(rows_v + c * 128), kOutput, c > 0 || !first);
         if (last) mma_commit(smem_u32(bars->o_full + g));

@@ -23,11 +23,10 @@ __device__ __forceinline__ uint64_t descriptor(uint32_t low) { return uint64_t(k
 __device__ __forceinline__ uint32_t along_row(uint32_t address) { return (address & 0x3ffffu) >> 4 | 1u << 16; }
 __device__ __forceinline__ uint32_t across_rows(uint32_t address) { return (address & 0x3ffffu) >> 4 | uint32_t(16384 >> 4) << 16; }
 // One thread issues.
-template <bool ACCUMULATE>
-__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc) {
+__device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
       "{\n.reg .pred p;\nsetp.ne.b32 p, %4, 0;\n"
-      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "n"(ACCUMULATE ? 1 : 0)
+      "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n}\n" ::"r"(d), "l"(a), "l"(b), "r"(idesc), "r"(accumulate ? 1u : 0u)
       : "memory");
 }
 // A from tensor memory: two 16-bit values along K per column.
@@ -50,7 +49,8 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(to), "l"(from), "r"(there ? 16 : 0) : "memory");
 }
 // The thread's arrival on a barrier once all its copies so far have landed; nothing waits for it here.  The copies are
-// written through the generic proxy: whoever waits on the barrier fences before a matrix instruction reads them.
+// written through the generic proxy: whoever waits on the barrier fences before a matrix instruction reads them (or the
+// thread itself waits, fences and arrives).
 __device__ __forceinline__ void copies_arrive(uint32_t barrier) {
   asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(barrier) : "memory");
 }

@@ -230,10 +230,9 @@ __device__ __forceinline__ void issue(int tiles, Barriers* bars, const volatile 
       if (g < groups) {
         const uint32_t rows_k = along_row(keys + kb.stage * C::KEYS + g * C::GROUP), rows_q = along_row(queries + st.stage * C::TILE);
         const uint32_t to = tmem + (g * 2 + buffer.stage) * 128;
-        mma_f16<false>(to, descriptor(rows_k), descriptor(rows_q), kScores);
-#pragma unroll
-        for (int c = 1; c < C::D / 16; ++c)
-          mma_f16<true>(to, descriptor(rows_k + (c >> 2) * 1024 + (c & 3) * 2), descriptor(rows_q + (c >> 2) * (C::ROWS * 8) + (c & 3) * 2), kScores);
+#pragma unroll 2
+        for (int c = 0; c < C::D / 16; ++c)
+          mma_f16(to, descriptor(rows_k + (c >> 2) * 1024 + (c & 3) * 2), descriptor(rows_q + (c >> 2) * (C::ROWS * 8) + (c & 3) * 2), kScores, c > 0);
       }
       mma_commit(smem_u32(&bars->s_full[g][buffer.stage]));
     }
