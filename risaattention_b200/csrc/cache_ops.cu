@@ -84,6 +84,24 @@ __device__ __forceinline__ void store8<float>(float* p, const float* x) {
   reinterpret_cast<float4*>(p)[1] = make_float4(x[4], x[5], x[6], x[7]);
 }
 
+// The same as it was loaded: as many of them as registers hold are on their way at once.
+template <typename T>
+struct Run {
+  uint4 raw;
+  __device__ __forceinline__ void load(const T* p) { raw = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void zero() { raw = make_uint4(0, 0, 0, 0); }
+  __device__ __forceinline__ void values(float* x) const { load8(reinterpret_cast<const T*>(&raw), x); }
+};
+template <>
+struct Run<float> {
+  float4 raw[2];
+  __device__ __forceinline__ void load(const float* p) {
+    raw[0] = reinterpret_cast<const float4*>(p)[0];
+    raw[1] = reinterpret_cast<const float4*>(p)[1];
+  }
+  __device__ __forceinline__ void values(float* x) const { load8(reinterpret_cast<const float*>(raw), x); }
+};
+
 // ---- rotation ----------------------------------------------------------------------------------------------
 struct RotateArgs {
   const void* x;
@@ -99,6 +117,7 @@ struct RotateArgs {
 // A thread owns eight pairs of one token (two runs of eight channels) in `heads_each` heads, so that
 // its eight cosines and sines serve them all; behind the pairs come the threads that copy eight
 // channels each.  Consecutive threads are consecutive runs of a row, then rows of consecutive tokens.
+constexpr int kHeadsAhead = 4;
 template <typename T>
 __global__ __launch_bounds__(256) void rotate_kernel(const RotateArgs a) {
   chain_wait();
@@ -113,11 +132,14 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotateArgs a) {
   if (item >= pairs) {
     if (a.out == a.x) return;
     const int c = a.rotary_dim + (item - pairs) * 8;
-#pragma unroll 4
-    for (int h = h0; h < h1; ++h) {
-      float v[8];
-      load8(x + h * a.xh + c, v);
-      store8(out + h * a.oh + c, v);
+    for (int h = h0; h < h1; h += 8) {  // eight at a time on their way
+      Run<T> v[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (h + i < h1) v[i].load(x + (h + i) * a.xh + c);
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+        if (h + i < h1) *reinterpret_cast<Run<T>*>(out + (h + i) * a.oh + c) = v[i];
     }
     return;
   }
@@ -130,11 +152,7 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotateArgs a) {
   }
   const int c0 = a.interleaved ? item * 16 : item * 8;
   const int c1 = a.interleaved ? c0 + 8 : a.rotary_dim / 2 + item * 8;
-#pragma unroll 2
-  for (int h = h0; h < h1; ++h) {
-    float u[8], v[8];
-    load8(x + h * a.xh + c0, u);
-    load8(x + h * a.xh + c1, v);
+  auto turn = [&](float (&u)[8], float (&v)[8]) {
     if (a.interleaved) {
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -153,6 +171,30 @@ __global__ __launch_bounds__(256) void rotate_kernel(const RotateArgs a) {
         v[i] = q * cs[i] + p * sn[i];
       }
     }
+  };
+  int h = h0;
+  for (; h + kHeadsAhead <= h1; h += kHeadsAhead) {
+    Run<T> u[kHeadsAhead], v[kHeadsAhead];
+#pragma unroll
+    for (int i = 0; i < kHeadsAhead; ++i) {
+      u[i].load(x + (h + i) * a.xh + c0);
+      v[i].load(x + (h + i) * a.xh + c1);
+    }
+#pragma unroll
+    for (int i = 0; i < kHeadsAhead; ++i) {
+      float p[8], q[8];
+      u[i].values(p);
+      v[i].values(q);
+      turn(p, q);
+      store8(out + (h + i) * a.oh + c0, p);
+      store8(out + (h + i) * a.oh + c1, q);
+    }
+  }
+  for (; h < h1; ++h) {
+    float u[8], v[8];
+    load8(x + h * a.xh + c0, u);
+    load8(x + h * a.xh + c1, v);
+    turn(u, v);
     store8(out + h * a.oh + c0, u);
     store8(out + h * a.oh + c1, v);
   }
@@ -219,24 +261,21 @@ __device__ __forceinline__ float row_absmax(const float* x, int lanes) {
 // the token's query heads, key heads and value heads with the cosines and sines of the lane's channels
 // kept in registers (a token of 32 + 8 rotated heads would compute each of them 40 times otherwise).
 // The second channel of a pair sits in the same lane (interleaved) or in the lane half a rotated row
-// away, whose channels come by shuffle.  Codes: absolute maximum over 127, rounded to nearest even
-// after one true division per channel; a row of zeros has scale 0, a row with an infinity or a NaN reads
-// back as NaN.
+// away, whose channels come by shuffle.  Codes: absolute maximum over 127, rounded to nearest even; a row of
+// zeros has scale 0, a row with an infinity or a NaN reads back as NaN.
+constexpr int kRowsAhead = 6;  // rows of a slot on their way at once: all of a token of 32 + 2 x 8 heads of 128
 template <typename T, bool INT8>
 __global__ __launch_bounds__(128) void append_kernel(const AppendArgs a) {
   chain_wait();
   chain_release();
   const int token = blockIdx.x, lanes = a.head_dim >> 3;
   const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes, slots = 128 / lanes;
-  // the sequence whose tokens include this one, by bisection of the offsets
+  // the sequence whose tokens include this one: as many as end in front of it, counted 128 at a time
   int s = token;
   if (a.step.offsets != nullptr) {
-    int lo = 0, hi = a.step.batch;  // first sequence whose end lies behind the token
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (__ldg(a.step.offsets + mid + 1) > token) hi = mid; else lo = mid + 1;
-    }
-    s = lo;
+    s = 0;
+    for (int i = 0; i < a.step.batch; i += 128)
+      s += __syncthreads_count(i + int(threadIdx.x) < a.step.batch && __ldg(a.step.offsets + i + threadIdx.x + 1) <= token);
   }
   int place = -1;
   bool belongs = false;
@@ -282,53 +321,72 @@ __global__ __launch_bounds__(128) void append_kernel(const AppendArgs a) {
   }
   const int slot_in_page = place & ((1 << a.step.page_shift) - 1);
   const int rows = a.q_heads + 2 * a.kv_heads;
-  for (int r0 = 0; r0 < rows; r0 += slots) {
-    const int r = r0 + slot;
-    const bool there = r < rows;
-    const int kind = r < a.q_heads ? 0 : r < a.q_heads + a.kv_heads ? 1 : 2;
-    const int h = kind == 0 ? r : kind == 1 ? r - a.q_heads : r - a.q_heads - a.kv_heads;
-    float x[8] = {};
-    if (there) {
-      const T* from = kind == 0 ? static_cast<const T*>(a.q) + token * a.qn + h * a.qh
-                    : kind == 1 ? static_cast<const T*>(a.k) + token * a.kn + h * a.kh
-                                : static_cast<const T*>(a.v) + token * a.vn + h * a.vh;
-      load8(from + channel, x);
-    }
-    if (a.turns != nullptr) {
-      if (a.interleaved) {
-        if (turned && kind < 2) {
+  // where row r comes from
+  auto source = [&](int r) {
+    return r < a.q_heads ? static_cast<const T*>(a.q) + token * a.qn + r * a.qh
+           : r < a.q_heads + a.kv_heads ? static_cast<const T*>(a.k) + token * a.kn + (r - a.q_heads) * a.kh
+                                        : static_cast<const T*>(a.v) + token * a.vn + (r - a.q_heads - a.kv_heads) * a.vh;
+  };
+  for (int r0 = 0; r0 < rows; r0 += slots * kRowsAhead) {
+    Run<T> run[kRowsAhead];
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float p = x[2 * i], q = x[2 * i + 1];
-            x[2 * i] = p * cs[i] - q * sn[i];
-            x[2 * i + 1] = q * cs[i] + p * sn[i];
+    for (int j = 0; j < kRowsAhead; ++j) {
+      const int r = r0 + j * slots + slot;
+      run[j].zero();
+      if (r < rows) run[j].load(source(r) + channel);
+    }
+#pragma unroll
+    for (int j = 0; j < kRowsAhead; ++j) {
+      if (r0 + j * slots >= rows) break;  // the same for the whole CTA
+      const int r = r0 + j * slots + slot;
+      const bool there = r < rows;
+      const int kind = r < a.q_heads ? 0 : r < a.q_heads + a.kv_heads ? 1 : 2;
+      const int h = kind == 0 ? r : kind == 1 ? r - a.q_heads : r - a.q_heads - a.kv_heads;
+      float x[8];
+      run[j].values(x);
+      if (a.turns != nullptr && __any_sync(0xffffffffu, kind < 2)) {
+        if (a.interleaved) {
+          if (turned && kind < 2) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float p = x[2 * i], q = x[2 * i + 1];
+              x[2 * i] = p * cs[i] - q * sn[i];
+              x[2 * i + 1] = q * cs[i] + p * sn[i];
+            }
+          }
+        } else {
+          Run<T> other;
+          other.raw.x = __shfl_sync(0xffffffffu, run[j].raw.x, partner);
+          other.raw.y = __shfl_sync(0xffffffffu, run[j].raw.y, partner);
+          other.raw.z = __shfl_sync(0xffffffffu, run[j].raw.z, partner);
+          other.raw.w = __shfl_sync(0xffffffffu, run[j].raw.w, partner);
+          if (turned && kind < 2) {
+            float y[8];
+            other.values(y);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = x[i] * cs[i] - y[i] * sn[i];
           }
         }
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-          const float other = __shfl_sync(0xffffffffu, x[i], partner);
-          if (turned && kind < 2) x[i] = x[i] * cs[i] - other * sn[i];
-        }
       }
-    }
-    if (INT8) {
-      const float scale = row_absmax(x, lanes) / 127.0f;
-      if (there && kind > 0 && page >= 0) {
-        float c[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) c[i] = scale > 0.f ? x[i] / scale : 0.f;
-        const int64_t row = ((page * a.kv_heads + h) << a.step.page_shift) + slot_in_page;
-        char* codes = static_cast<char*>(kind == 1 ? a.keys : a.values);
-        *reinterpret_cast<uint2*>(codes + row * a.head_dim + channel) =
-            make_uint2(pack4_s8(c[0], c[1], c[2], c[3]), pack4_s8(c[4], c[5], c[6], c[7]));
-        if (lane == 0) (kind == 1 ? a.key_scales : a.value_scales)[row] = scale;
-      }
-    } else if (there && kind > 0 && page >= 0) {
       const int64_t row = ((page * a.kv_heads + h) << a.step.page_shift) + slot_in_page;
-      store8(static_cast<T*>(kind == 1 ? a.keys : a.values) + row * a.head_dim + channel, x);
+      if (INT8 && __any_sync(0xffffffffu, kind > 0)) {
+        const float most = row_absmax(x, lanes), scale = most / 127.0f;
+        if (there && kind > 0 && page >= 0) {
+          // one reciprocal for the row; rows so small that it would overflow are divided
+          const float inverse = 127.0f / most;
+          float c[8];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) c[i] = most > 1e-35f ? x[i] * inverse : scale > 0.f ? x[i] / scale : 0.f;
+          char* codes = static_cast<char*>(kind == 1 ? a.keys : a.values);
+          *reinterpret_cast<uint2*>(codes + row * a.head_dim + channel) =
+              make_uint2(pack4_s8(c[0], c[1], c[2], c[3]), pack4_s8(c[4], c[5], c[6], c[7]));
+          if (lane == 0) (kind == 1 ? a.key_scales : a.value_scales)[row] = scale;
+        }
+      } else if (!INT8 && there && kind > 0 && page >= 0) {
+        store8(static_cast<T*>(kind == 1 ? a.keys : a.values) + row * a.head_dim + channel, x);
+      }
+      if (there && kind == 0) store8(static_cast<T*>(a.q_out) + token * a.on + h * a.oh + channel, x);
     }
-    if (there && kind == 0) store8(static_cast<T*>(a.q_out) + token * a.on + h * a.oh + channel, x);
   }
 }
 

@@ -34,6 +34,7 @@ struct RowsArgs {
   float scale_log2;
   int clear_rest;
   float* parts;   // two slots per worker: of a unit that began before it, of one that goes on after it
+  JoinNote* notes;
   int min_steps;  // fewest steps that make a worker worth its share of the join
   unsigned int* status;
   // key weights only
@@ -326,9 +327,12 @@ __global__ __launch_bounds__(kThreads) void paged_rows_kernel(const RowsArgs a) 
   }
   const int64_t total = line_total<kThreads>(a.line, shared);
   const int workers = workers_of(total, gridDim.x, a.min_steps);
-  if (int(blockIdx.x) >= workers) return;
-  const int64_t begin = border(total, blockIdx.x, workers);
-  Pieces pieces{border(total, blockIdx.x + 1, workers) - begin, line_place<kThreads>(a.line, begin, shared)};
+  if (int(blockIdx.x) >= workers) {
+    if (threadIdx.x == 0) a.notes[blockIdx.x] = JoinNote{};
+    return;
+  }
+  const int64_t begin = border(total, blockIdx.x, workers), end = border(total, blockIdx.x + 1, workers);
+  Pieces pieces{end - begin, line_place<kThreads>(a.line, begin, shared)};
   Piece piece;
   while (pieces.next(a.line, piece)) {
     const Sequence seq = piece.seq;
@@ -509,6 +513,7 @@ __global__ __launch_bounds__(kThreads) void paged_rows_kernel(const RowsArgs a) 
     }
     __syncthreads();
   }
+  if (threadIdx.x == 0) a.notes[blockIdx.x] = join_note(a.line, piece, total, end, blockIdx.x, workers);
 }
 
 // ---- key weights -------------------------------------------------------------------------------------------
@@ -701,14 +706,14 @@ static bool takes_tensor_cores(const risa_b200_cache& cache, const risa_b200_ste
   return cache.head_dim <= 128 && most >= kTcFewestRows;
 }
 static size_t rows_scratch(const risa_b200_cache& cache, const risa_b200_step& step, int group) {
-  return size_t(kMaxWorkers) * 2 * slot_floats(8 * column_blocks_of(step, group), cache.head_dim) * sizeof(float);
+  return size_t(kMaxWorkers) * (2 * slot_floats(8 * column_blocks_of(step, group), cache.head_dim) * sizeof(float) + sizeof(JoinNote));
 }
 
 extern "C" size_t risa_b200_paged_attention_scratch_size(const risa_b200_cache* cache, const risa_b200_step* step, int q_heads) {
   if (cache == nullptr || step == nullptr || cache->kv_heads <= 0 || q_heads <= 0) return 0;
   const int group = q_heads / cache->kv_heads;
   size_t bytes = rows_scratch(*cache, *step, group);
-  if (takes_tensor_cores(*cache, *step, group)) bytes += size_t(kTcWorkers) * 2 * slot_floats(paged_tc_rows(), cache->head_dim) * sizeof(float);
+  if (takes_tensor_cores(*cache, *step, group)) bytes += paged_tc_scratch(cache->head_dim);
   return bytes;
 }
 
@@ -731,6 +736,7 @@ extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const ris
   a.lse = lse;
   a.clear_rest = clear_rest;
   a.parts = static_cast<float*>(scratch);
+  a.notes = reinterpret_cast<JoinNote*>(a.parts + size_t(kMaxWorkers) * 2 * slot_floats(a.line.rows, cache->head_dim));
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   const bool tensor_cores = takes_tensor_cores(*cache, *step, a.line.group);
   if (tensor_cores) a.line.max_rows = kTcFewestRows - 1;
@@ -740,13 +746,13 @@ extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const ris
     if (const int bad = allow_shared(paged_rows_kernel<C>, bytes, "paged attention")) return bad;
     const int workers = C::D == 256 && !C::INT8 ? kMaxWorkers / 2 : kMaxWorkers;
     launch_chained(paged_rows_kernel<C>, dim3(workers), dim3(kThreads), bytes, stream, a);
-    const JoinArgs join{a.line, a.parts, workers, a.min_steps, out, a.on, a.oh, lse};
-    launch_chained(join_parts_kernel<typename C::T, C::D>, dim3(workers - 1, C::R / 4), dim3(128), 0, stream, join);
+    const JoinArgs join{a.parts, a.notes, C::R, a.line.group, q_heads, out, a.on, a.oh, lse};
+    launch_chained(join_parts_kernel<typename C::T, C::D, true>, dim3(workers - 1, C::R), dim3(128), 0, stream, join);
     return RISA_B200_OK;
   });
   if (bad == RISA_B200_OK && tensor_cores) {
     TcArgs t{a.line, q, a.qn, a.qh, out, a.on, a.oh, lse, a.keys, a.values, a.key_scales, a.value_scales, a.pages, a.scale_log2,
-             a.parts + rows_scratch(*cache, *step, a.line.group) / sizeof(float), 2, status};
+             a.parts + rows_scratch(*cache, *step, a.line.group) / sizeof(float), nullptr, 2, status};
     t.line.min_rows = kTcFewestRows;
     t.line.max_rows = INT_MAX;
     bad = paged_tc(t, dtype_code, cache->dtype_code == kInt8, cache->head_dim, stream);

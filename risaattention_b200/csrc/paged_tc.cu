@@ -423,9 +423,12 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
   chain_release();
   const int64_t total = line_total<kThreads>(a.line, shared);
   const int workers = workers_of(total, gridDim.x, a.min_steps);
-  if (int(blockIdx.x) >= workers) return;
-  const int64_t begin = border(total, blockIdx.x, workers);
-  const Pieces pieces{border(total, blockIdx.x + 1, workers) - begin, line_place<kThreads>(a.line, begin, shared)};
+  if (int(blockIdx.x) >= workers) {
+    if (threadIdx.x == 0) a.notes[blockIdx.x] = JoinNote{};
+    return;
+  }
+  const int64_t begin = border(total, blockIdx.x, workers), finish = border(total, blockIdx.x + 1, workers);
+  const Pieces pieces{finish - begin, line_place<kThreads>(a.line, begin, shared)};
   if (warp == kIssuer) tmem_alloc(smem_u32(&tmem_base), 512);
   tc_fence_before();
   __syncthreads();
@@ -439,6 +442,12 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
     fetch_tiles<C>(a, &key_map, &value_map, pieces, &bars, notes, k_ring, v_ring, gave_up);
   } else {
     regs_dec<kRegsIssuer>();
+    if (warp == kIssuer + 1 && (threadIdx.x & 31) == 0) {
+      Pieces all = pieces;
+      Piece piece;
+      while (all.next(a.line, piece)) {}
+      a.notes[blockIdx.x] = join_note(a.line, piece, total, finish, blockIdx.x, workers);
+    }
     if (warp == kIssuer) {
       issue_products<C>(int(pieces.left), &bars, notes, tmem, q, k_ring, v_ring, gave_up);
       __syncwarp();
@@ -509,18 +518,19 @@ int launch(const TcArgs& a, cudaStream_t stream) {
   }();
   RISA_REQUIRE(budget, "paged attention: the tensor-core kernel was not compiled for %d registers", kRegsLaunch);
   launch_chained(paged_tc_kernel<C>, dim3(kTcWorkers), dim3(kThreads), C::SMEM, stream, key_map, value_map, a);
-  const JoinArgs join{a.line, a.parts, kTcWorkers, a.min_steps, a.out, a.on, a.oh, a.lse};
-  launch_chained(join_parts_kernel<typename C::T, C::D>, dim3(kTcWorkers - 1, kRows / 4), dim3(128), 0, stream, join);
+  const JoinArgs join{a.parts, a.notes, kRows, a.line.group, a.line.kv_heads * a.line.group, a.out, a.on, a.oh, a.lse};
+  launch_chained(join_parts_kernel<typename C::T, C::D, false>, dim3(kTcWorkers - 1, kRows / 16), dim3(128), 0, stream, join);
   return RISA_B200_OK;
 }
 
 }  // namespace
 
-int paged_tc_rows() { return kRows; }
+size_t paged_tc_scratch(int head_dim) { return size_t(kTcWorkers) * (2 * slot_floats(kRows, head_dim) * sizeof(float) + sizeof(JoinNote)); }
 
 int paged_tc(TcArgs a, int dtype_code, bool codes, int head_dim, cudaStream_t stream) {
   a.line.rows = Divisor(kRows);
   a.line.keys = Divisor(kTileKeys);
+  a.notes = reinterpret_cast<JoinNote*>(a.parts + size_t(kTcWorkers) * 2 * slot_floats(kRows, head_dim));
   if (dtype_code == 1)
     return head_dim == 64 ? (codes ? launch<Shape<__half, true, 64>>(a, stream) : launch<Shape<__half, false, 64>>(a, stream))
                           : (codes ? launch<Shape<__half, true, 128>>(a, stream) : launch<Shape<__half, false, 128>>(a, stream));

@@ -23,11 +23,12 @@ struct TcArgs {
   int pages;
   float scale_log2;
   float* parts;
+  JoinNote* notes;  // set by the kernel's own launcher
   int min_steps;
   unsigned int* status;
 };
 
-int paged_tc_rows();
+size_t paged_tc_scratch(int head_dim);
 int paged_tc(TcArgs args, int dtype_code, bool codes, int head_dim, cudaStream_t stream);
 int paged_tc_wait_status();
 

@@ -236,62 +236,110 @@ constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 // and finite, so that a row that has seen nothing yet needs no case of its own.
 constexpr float kNoMaximum = -1e30f;
 
+__host__ __device__ __forceinline__ int64_t slot_floats(int rows, int head_dim) { return int64_t(rows) * (head_dim + 2); }
+// What a worker leaves for the join: the unit whose first part it ended with, and over how many workers that unit goes
+// (parts 0: it ended with a whole unit, or inside one that began before it).  Every CTA of a launch writes one.
+struct JoinNote {
+  int first_token, rows, head, block, parts, sequence;
+};
+
 struct JoinArgs {
-  LineArgs line;
   const float* parts;
-  int max_workers, min_steps;
+  const JoinNote* notes;
+  int unit_rows;
+  Divisor group;
+  int heads;
   void* out;
   int64_t on, oh;
   float* lse;
 };
-__host__ __device__ __forceinline__ int64_t slot_floats(int rows, int head_dim) { return int64_t(rows) * (head_dim + 2); }
 
-// Borders are grid x, groups of four rows (a warp each) grid y.  The first border inside a unit joins that unit's
-// parts in the order of their keys, so that results do not depend on which worker ended first.
-template <typename T, int D>
+// Written once the walk over the pieces has come to its end (`at` behind the last step, `done` the last piece).
+__device__ __forceinline__ JoinNote join_note(const LineArgs& a, const Piece& last, int64_t total, int64_t end, int worker, int workers) {
+  if (!last.opens || last.whole) return {0, 0, 0, 0, 0, 0};
+  const int64_t unit_end = end - last.count + steps_of(a, last.seq, last.block).count;
+  return {last.seq.first, last.seq.count * a.group, last.head, last.block, min(worker_from(total, unit_end, workers), workers) - worker, last.sequence};
+}
+
+// Worker c's unit (grid x) is joined from the second slot of c and the first slots of those behind it, in the order of
+// their keys, so that results do not depend on which worker ended first.  MANY: units of few rows and up to a hundred
+// parts; a CTA joins one row (grid y), its warps a quarter of the parts each.  Else few parts: a warp joins four rows.
+template <typename T, int D, bool MANY>
 __global__ __launch_bounds__(128) void join_parts_kernel(const JoinArgs a) {
-  __shared__ LineShared<128> shared;
+  __shared__ float tops[4], norms[4], sums[MANY ? 4 : 1][D];
   chain_wait();
   chain_release();
-  const int64_t total = line_total<128>(a.line, shared);
-  const int workers = workers_of(total, a.max_workers, a.min_steps), c = blockIdx.x, R = a.line.rows;
-  if (c + 1 >= workers) return;
-  const int64_t edge = border(total, c + 1, workers), previous = border(total, c, workers);
-  const Place place = line_place<128>(a.line, edge, shared);
-  const Sequence seq = sequence_of(a.line.step, place.sequence);
-  const int64_t unit_start = edge - place.inside, unit_end = unit_start + steps_of(a.line, seq, place.block).count;
-  if (place.inside == 0 || previous > unit_start) return;  // no unit is cut here, or an earlier border joins it
-  const int r = blockIdx.y * 4 + (threadIdx.x >> 5), lane = threadIdx.x & 31, row = place.block * R + r;
-  if (r >= R || row >= seq.count * a.line.group) return;
-  const int parts = min(worker_from(total, unit_end, workers), workers) - c;
+  const JoinNote note = a.notes[blockIdx.x];
+  if (note.parts == 0) return;
+  const int c = blockIdx.x, R = a.unit_rows, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int64_t slot = slot_floats(R, D);
   auto slot_of = [&](int i) { return a.parts + (int64_t(c + i) * 2 + (i == 0 ? 1 : 0)) * slot; };
-  float top = kNoMaximum;
-  for (int i = lane; i < parts; i += 32) top = fmaxf(top, slot_of(i)[R * D + r]);
-#pragma unroll
-  for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
   constexpr int PER = D / 32;
-  float sum[PER] = {}, norm = 0.f;
-#pragma unroll 8
-  for (int i = 0; i < parts; ++i) {
-    const float* s = slot_of(i);
-    const float f = ex2_approx(s[R * D + r] - top);
-    norm += f * s[R * D + R + r];
+  // this warp's share of one row's parts [from, to)
+  auto add = [&](int r, int from, int to, float& top, float& norm, float (&sum)[PER]) {
+    top = kNoMaximum;
+    for (int i = from + lane; i < to; i += 32) top = fmaxf(top, slot_of(i)[R * D + r]);
 #pragma unroll
-    for (int e = 0; e < PER / 2; ++e) {
-      const float2 x = *reinterpret_cast<const float2*>(s + r * D + e * 64 + lane * 2);
-      sum[2 * e] += f * x.x;
-      sum[2 * e + 1] += f * x.y;
+    for (int off = 16; off > 0; off >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, off));
+    norm = 0.f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) sum[e] = 0.f;
+#pragma unroll(MANY ? 8 : 2)
+    for (int i = from; i < to; ++i) {
+      const float* s = slot_of(i);
+      const float f = ex2_approx(s[R * D + r] - top);
+      norm += f * s[R * D + R + r];
+#pragma unroll
+      for (int e = 0; e < PER / 2; ++e) {
+        const float2 x = *reinterpret_cast<const float2*>(s + r * D + e * 64 + lane * 2);
+        sum[2 * e] += f * x.x;
+        sum[2 * e + 1] += f * x.y;
+      }
+    }
+  };
+  auto write = [&](int row, float top, float norm, const float (&sum)[PER]) {
+    const float f = norm == 0.f ? 0.f : 1.0f / norm;
+    const int token = row / a.group, h = note.head * a.group + row - token * a.group;
+    T* out = static_cast<T*>(a.out) + int64_t(note.first_token + token) * a.on + int64_t(h) * a.oh;
+#pragma unroll
+    for (int e = 0; e < PER / 2; ++e)
+      *reinterpret_cast<uint32_t*>(out + e * 64 + lane * 2) = Half2<T>::pack(sum[2 * e] * f, sum[2 * e + 1] * f);
+    if (lane == 0 && a.lse != nullptr)
+      a.lse[int64_t(note.first_token + token) * a.heads + h] = norm == 0.f ? -INFINITY : top * kLn2 + logf(norm);
+  };
+  float top, norm, sum[PER];
+  if (MANY) {
+    const int r = blockIdx.y, row = note.block * R + r;
+    if (row >= note.rows) return;
+    add(r, note.parts * warp / 4, note.parts * (warp + 1) / 4, top, norm, sum);
+    if (lane == 0) {
+      tops[warp] = top;
+      norms[warp] = norm;
+    }
+#pragma unroll
+    for (int e = 0; e < PER; ++e) sums[warp][e * 32 + lane] = sum[e];
+    __syncthreads();
+    if (warp != 0) return;
+    top = fmaxf(fmaxf(tops[0], tops[1]), fmaxf(tops[2], tops[3]));
+    norm = 0.f;
+#pragma unroll
+    for (int e = 0; e < PER; ++e) sum[e] = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = ex2_approx(tops[w] - top);
+      norm += f * norms[w];
+#pragma unroll
+      for (int e = 0; e < PER; ++e) sum[e] += f * sums[w][e * 32 + lane];
+    }
+    write(row, top, norm, sum);
+  } else {
+    for (int i = 0; i < 4; ++i) {
+      const int r = (blockIdx.y * 4 + warp) * 4 + i, row = note.block * R + r;
+      if (row >= note.rows) return;
+      add(r, 0, note.parts, top, norm, sum);
+      write(row, top, norm, sum);
     }
   }
-  const float f = norm == 0.f ? 0.f : 1.0f / norm;
-  const int token = row / a.line.group, h = place.head * a.line.group + row % a.line.group;
-  T* out = static_cast<T*>(a.out) + int64_t(seq.first + token) * a.on + int64_t(h) * a.oh;
-#pragma unroll
-  for (int e = 0; e < PER / 2; ++e)
-    *reinterpret_cast<uint32_t*>(out + e * 64 + lane * 2) = Half2<T>::pack(sum[2 * e] * f, sum[2 * e + 1] * f);
-  if (lane == 0 && a.lse != nullptr)
-    a.lse[int64_t(seq.first + token) * (a.line.kv_heads * a.line.group) + h] = norm == 0.f ? -INFINITY : top * kLn2 + logf(norm);
 }
 
 }  // namespace serving

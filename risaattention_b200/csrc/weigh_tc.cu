@@ -77,6 +77,7 @@ struct WeighArgs {
   const float* previous;
   float* weights;
   float* parts;  // two slots of 256 floats per worker
+  JoinNote* notes;  // as attention's, but for `rows`: the block's first key
   int min_steps;
   unsigned int* status;
 };
@@ -393,9 +394,12 @@ __global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a
   }
   const int64_t total = line_total<kThreads>(a.line, shared);
   const int workers = workers_of(total, gridDim.x, a.min_steps);
-  if (int(blockIdx.x) >= workers) return;
-  const int64_t begin = border(total, blockIdx.x, workers);
-  const Pieces pieces{border(total, blockIdx.x + 1, workers) - begin, line_place<kThreads>(a.line, begin, shared)};
+  if (int(blockIdx.x) >= workers) {
+    if (threadIdx.x == 0) a.notes[blockIdx.x] = JoinNote{};
+    return;
+  }
+  const int64_t begin = border(total, blockIdx.x, workers), finish = border(total, blockIdx.x + 1, workers);
+  const Pieces pieces{finish - begin, line_place<kThreads>(a.line, begin, shared)};
   if (warp == kIssuer) tmem_alloc(smem_u32(&tmem_base), 512);
   tc_fence_before();
   __syncthreads();
@@ -408,6 +412,19 @@ __global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a
   } else if (warp < kIssuer) {
     fetch_keys<C>(a, pieces, &bars, &notes, keys, gave_up);
   } else if (warp == kIssuer) {
+    if ((threadIdx.x & 31) == 0) {
+      Pieces all = pieces;
+      Piece last;
+      while (all.next(a.line, last)) {}
+      JoinNote note{};
+      if (last.opens && !last.whole) {
+        const int64_t end = finish - last.count + steps_of(a.line, last.seq, last.block).count;
+        note = {last.seq.first, (first_seen(a.line, last.seq) / kBlockKeys + last.block) * kBlockKeys, last.head, last.block,
+                min(worker_from(total, end, workers), workers) - int(blockIdx.x), last.sequence};
+      }
+      a.notes[blockIdx.x] = note;
+    }
+    __syncwarp();
     issue<C>(int(pieces.left), &bars, &notes, tmem, keys, queries, gave_up);
     __syncwarp();
     // nothing of this CTA is in flight when tensor memory is handed back, also after a wait that ran out
@@ -431,26 +448,17 @@ __global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a
   }
 }
 
-// One CTA per border between two workers: the first border inside a block of keys adds up its parts in order.
-__global__ __launch_bounds__(kBlockKeys) void join_weights_kernel(const WeighArgs a, int max_workers) {
-  __shared__ LineShared<kBlockKeys> shared;
+// The parts of the block that worker blockIdx.x ended with, added up in order.
+__global__ __launch_bounds__(kBlockKeys) void join_weights_kernel(const WeighArgs a) {
   chain_wait();
   chain_release();
-  const int64_t total = line_total<kBlockKeys>(a.line, shared);
-  const int workers = workers_of(total, max_workers, a.min_steps), c = blockIdx.x;
-  if (c + 1 >= workers) return;
-  const int64_t edge = border(total, c + 1, workers), previous = border(total, c, workers);
-  const Place place = line_place<kBlockKeys>(a.line, edge, shared);
-  const Sequence seq = sequence_of(a.line.step, place.sequence);
-  const int64_t start = edge - place.inside, end = start + steps_of(a.line, seq, place.block).count;
-  if (place.inside == 0 || previous > start) return;
-  float sum = a.parts[(int64_t(c) * 2 + 1) * kBlockKeys + threadIdx.x];
-  const int last = min(worker_from(total, end, workers), workers);
-  for (int i = c + 1; i < last; ++i) sum += a.parts[int64_t(i) * 2 * kBlockKeys + threadIdx.x];
-  const int slots = a.line.step.width << a.line.step.page_shift;
-  const int key = (first_seen(a.line, seq) / kBlockKeys + place.block) * kBlockKeys + threadIdx.x;
+  const JoinNote note = a.notes[blockIdx.x];
+  if (note.parts == 0) return;
+  float sum = a.parts[(int64_t(blockIdx.x) * 2 + 1) * kBlockKeys + threadIdx.x];
+  for (int i = 1; i < note.parts; ++i) sum += a.parts[(int64_t(blockIdx.x) + i) * 2 * kBlockKeys + threadIdx.x];
+  const int slots = a.line.step.width << a.line.step.page_shift, key = note.rows + threadIdx.x;
   if (key >= slots) return;
-  const int64_t index = (int64_t(place.sequence) * a.line.kv_heads + place.head) * slots + key;
+  const int64_t index = (int64_t(note.sequence) * a.line.kv_heads + note.head) * slots + key;
   a.weights[index] = sum + (a.previous != nullptr ? a.previous[index] : 0.f);
 }
 
@@ -460,7 +468,7 @@ int launch(WeighArgs a, cudaStream_t stream) {
   if (cudaFuncSetAttribute(weigh_tc_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
     return fail(RISA_B200_CUDA, "key weights: %s", cudaGetErrorString(cudaGetLastError()));
   launch_chained(weigh_tc_kernel<C>, dim3(kTcWorkers), dim3(kThreads), C::SMEM, stream, a);
-  launch_chained(join_weights_kernel, dim3(kTcWorkers - 1), dim3(kBlockKeys), 0, stream, a, kTcWorkers);
+  launch_chained(join_weights_kernel, dim3(kTcWorkers - 1), dim3(kBlockKeys), 0, stream, a);
   return RISA_B200_OK;
 }
 template <typename T>
@@ -472,13 +480,13 @@ int launch_for(const WeighArgs& a, bool codes, int head_dim, cudaStream_t stream
 
 }  // namespace
 
-size_t weigh_tc_scratch() { return size_t(kTcWorkers) * 2 * kBlockKeys * sizeof(float); }
+size_t weigh_tc_scratch() { return size_t(kTcWorkers) * (2 * kBlockKeys * sizeof(float) + sizeof(JoinNote)); }
 
 int weigh_tc(const TcArgs& t, const float* row_lse, const float* previous, float* weights, int dtype_code, bool codes, int head_dim,
              cudaStream_t stream) {
   const WeighArgs a{{t.line.step, t.line.kv_heads, t.line.group, t.line.min_rows, Divisor(), t.line.causal, t.line.window},
                     t.q, t.qn, t.qh, row_lse, {t.keys, t.key_scales, t.line.kv_heads, t.line.step.page_shift}, t.pages, t.scale_log2,
-                    previous, weights, t.parts, t.min_steps, t.status};
+                    previous, weights, t.parts, reinterpret_cast<JoinNote*>(t.parts + size_t(kTcWorkers) * 2 * kBlockKeys), t.min_steps, t.status};
   return dtype_code == 1 ? launch_for<__half>(a, codes, head_dim, stream) : launch_for<__nv_bfloat16>(a, codes, head_dim, stream);
 }
 
