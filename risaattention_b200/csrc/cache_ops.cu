@@ -269,7 +269,23 @@ __global__ __launch_bounds__(128) void append_kernel(const AppendArgs a) {
   chain_wait();
   chain_release();
   const int token = blockIdx.x, lanes = a.head_dim >> 3;
-  const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes, slots = 128 / lanes;
+  const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes, slots = 128 / lanes, channel = lane * 8;
+  const int rows = a.q_heads + 2 * a.kv_heads;
+  // Rows are on their way before their place is looked up: kRowsAhead of them from r0 on.
+  Run<T> run[kRowsAhead];
+  auto load_rows = [&](int r0) {
+#pragma unroll
+    for (int j = 0; j < kRowsAhead; ++j) {
+      const int r = r0 + j * slots + slot;
+      run[j].zero();
+      if (r < rows)
+        run[j].load((r < a.q_heads ? static_cast<const T*>(a.q) + token * a.qn + r * a.qh
+                     : r < a.q_heads + a.kv_heads ? static_cast<const T*>(a.k) + token * a.kn + (r - a.q_heads) * a.kh
+                                                  : static_cast<const T*>(a.v) + token * a.vn + (r - a.q_heads - a.kv_heads) * a.vh) +
+                    channel);
+    }
+  };
+  load_rows(0);
   // the sequence whose tokens include this one: as many as end in front of it, counted 128 at a time
   int s = token;
   if (a.step.offsets != nullptr) {
@@ -300,7 +316,6 @@ __global__ __launch_bounds__(128) void append_kernel(const AppendArgs a) {
   } else if (place >= 0 && threadIdx.x == 0) {
     atomicCAS(a.status, 0u, unsigned(s) + 1u);  // longer than its row of the table
   }
-  const int channel = lane * 8;
   const bool turned = a.turns != nullptr && channel < a.rotary_dim;
   float cs[8], sn[8];
   int partner = threadIdx.x & 31;
@@ -320,21 +335,8 @@ __global__ __launch_bounds__(128) void append_kernel(const AppendArgs a) {
     if (!a.interleaved) partner = (threadIdx.x & 31) + (second ? -(half >> 3) : (half >> 3));
   }
   const int slot_in_page = place & ((1 << a.step.page_shift) - 1);
-  const int rows = a.q_heads + 2 * a.kv_heads;
-  // where row r comes from
-  auto source = [&](int r) {
-    return r < a.q_heads ? static_cast<const T*>(a.q) + token * a.qn + r * a.qh
-           : r < a.q_heads + a.kv_heads ? static_cast<const T*>(a.k) + token * a.kn + (r - a.q_heads) * a.kh
-                                        : static_cast<const T*>(a.v) + token * a.vn + (r - a.q_heads - a.kv_heads) * a.vh;
-  };
   for (int r0 = 0; r0 < rows; r0 += slots * kRowsAhead) {
-    Run<T> run[kRowsAhead];
-#pragma unroll
-    for (int j = 0; j < kRowsAhead; ++j) {
-      const int r = r0 + j * slots + slot;
-      run[j].zero();
-      if (r < rows) run[j].load(source(r) + channel);
-    }
+    if (r0 > 0) load_rows(r0);
 #pragma unroll
     for (int j = 0; j < kRowsAhead; ++j) {
       if (r0 + j * slots >= rows) break;  // the same for the whole CTA
