@@ -6,8 +6,11 @@
 // its own (no barrier between warps, several KB in flight per warp), forms scores as K Q^T with the keys as
 // the 16 rows of the matrix instruction and up to 8 query rows as its columns (no padding for groups of 8
 // heads), keeps running maximum, sum and output in registers, and adds V^T P^T in the same orientation.
-// Codes become 16-bit values in registers on the way to the matrix instruction: whole numbers up to 128 are
-// exact in bf16 and fp16, so K's scale multiplies the score and V's the probability, both in 32 bits.
+// Codes become fp16 in registers on the way to the matrix instruction (whole numbers up to 128 are exact, and fp16 takes
+// half the instructions of bf16), so K's scale multiplies the score and V's the probability, both in 32 bits.  Queries
+// in bf16 become fp16 too, their row multiplied by a power of two that brings its largest value to 2^14: nothing is lost
+// but what is 2^-38 of that value.  Probability times scale fits fp16 because the running maximum is not that of the
+// scores s but of s + log2(scale): what is rounded is at most 1, and exact relative to the largest contribution.
 #include "paged_tc.cuh"
 #include "serving_plan.cuh"
 
@@ -48,14 +51,17 @@ struct Tile {
   using T = T_;
   static constexpr bool INT8 = INT8_;
   static constexpr int D = D_, NT = NT_, R = 8 * NT_;
+  using M = std::conditional_t<INT8_, __half, T_>;  // type of the matrix instructions' operands
   static constexpr int ROW = D * (INT8 ? 1 : 2);  // bytes of a key
   static constexpr int CHUNKS = ROW / 16;
   static constexpr int SIDE = 16 * ROW;  // the 16 keys (or values) of a step
   static constexpr int SCALES = INT8 ? 128 : 0;
   static constexpr int KS = D / 16;
-  // Two CTAs of four warps share an SM's shared memory (one at 16-bit rows of 256 channels): what hides
-  // the latency of HBM is bytes in flight, 96 KB or more per SM.
-  static constexpr int BUDGET = D == 256 && !INT8 ? 48 * 1024 : 24 * 1024;  // per warp
+  // CTAs of four warps that share an SM's shared memory: what hides the latency of HBM is bytes in flight, 96 KB or
+  // more per SM.  Codes, whose conversion keeps the schedulers busy, gain from a third CTA (32 requests of up to 32K
+  // keys: 280 us with two, 247 with three, 267 with four); 16-bit rows of 256 channels leave room for one.
+  static constexpr int CTAS = D == 256 && !INT8 ? 1 : INT8 && D <= 128 && NT == 1 ? 3 : 2;
+  static constexpr int BUDGET = 48 * 1024 / CTAS;  // per warp
   __host__ __device__ static constexpr int stages(int sides) {
     const int n = BUDGET / (sides * SIDE + SCALES);
     return n > 8 ? 8 : n;
@@ -113,22 +119,15 @@ __device__ __forceinline__ float read_float(uint32_t address) {
   return v;
 }
 
-// Two signed codes in the low bytes of the halves of `pair` (the high bytes are ignored) as 16-bit numbers.
-// bf16: 0x4300 + m is 128 + m for m < 128, so (low seven bits) - (sign bit ? 128 : 0) is the difference of
-// two such numbers; both and the result are exact.  fp16: 0x6400 + u is 1024 + u, so the code plus 128 less
-// 1152.
-template <typename T> __device__ __forceinline__ uint32_t codes_to(uint32_t pair);
-template <> __device__ __forceinline__ uint32_t codes_to<__nv_bfloat16>(uint32_t pair) {
-  const uint32_t low = (pair & 0x007f007fu) | 0x43004300u, sign = (pair & 0x00800080u) | 0x43004300u;
-  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&low), *reinterpret_cast<const __nv_bfloat162*>(&sign));
-  return *reinterpret_cast<const uint32_t*>(&d);
-}
-template <> __device__ __forceinline__ uint32_t codes_to<__half>(uint32_t pair) {
-  const uint32_t u = ((pair ^ 0x00800080u) & 0x00ff00ffu) | 0x64006400u;
+// Codes as fp16: 0x6400 + u is 1024 + u, so (code + 128 as u) less 1152 is the code.  Bytes 2 i and 2 i + 1 of a word whose
+// sign bits have been flipped; or two codes in the low bytes of the halves of a word (the high bytes are ignored).
+__device__ __forceinline__ uint32_t less_1152(uint32_t u) {
   const uint32_t bias = 0x64806480u;
   const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&bias));
   return *reinterpret_cast<const uint32_t*>(&d);
 }
+__device__ __forceinline__ uint32_t pair_of_flipped(uint32_t word, int i) { return less_1152(__byte_perm(word, 0x64646464u, i ? 0x4342 : 0x4140)); }
+__device__ __forceinline__ uint32_t pair_of_halves(uint32_t pair) { return less_1152((pair & 0x00ff00ffu) ^ 0x64806480u); }
 
 // ---- a warp's walk over its steps -----------------------------------------------------------------------
 // Steps first, first + kWarps, ... of one unit.  Page numbers are looked up 32 steps at a time, one set
@@ -195,9 +194,10 @@ struct Walk {
 // Query rows as the B operand: [nt][ks][2].  With codes the channels of a 64-channel run are dealt so that
 // a lane's 16 bytes of K serve four instructions: instruction 4 b + j takes channels 64 b + 16 t + 4 j ..
 // + 3 from lane t; the sum over channels does not mind the order.
+// factor: what multiplies the scores of rows 2 t and 2 t + 1 (the softmax scale in units of log 2, and the row's own).
 template <typename C>
-__device__ __forceinline__ void load_queries(const RowsArgs& a, const Sequence& seq, int head, int row0, int rows,
-                                             uint32_t (&qf)[C::NT][C::KS][2]) {
+__device__ __forceinline__ void load_queries(const RowsArgs& a, const Sequence& seq, int head, int row0, int rows, uint32_t (&qf)[C::NT][C::KS][2],
+                                             float (&factor)[C::NT][2]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < C::NT; ++nt) {
@@ -212,6 +212,28 @@ __device__ __forceinline__ void load_queries(const RowsArgs& a, const Sequence& 
       const int c1 = C::INT8 ? c0 + 2 : c0 + 8;
       qf[nt][ks][0] = there ? *reinterpret_cast<const uint32_t*>(q + c0) : 0u;
       qf[nt][ks][1] = there ? *reinterpret_cast<const uint32_t*>(q + c1) : 0u;
+    }
+    factor[nt][0] = factor[nt][1] = a.scale_log2;
+    if constexpr (C::INT8 && std::is_same<typename C::T, __nv_bfloat16>::value) {
+      uint32_t most = 0;  // bits of the largest magnitude
+#pragma unroll
+      for (int ks = 0; ks < C::KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) most = max(most, max((qf[nt][ks][i] & 0x7fffu) << 16, qf[nt][ks][i] & 0x7fff0000u));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 1));
+      most = max(most, __shfl_xor_sync(0xffffffffu, most, 2));
+      // exponent e of the largest value: the row times 2^(14 - e), an infinity or a NaN stays one
+      const int e = most == 0 ? 14 : min(max(int(most >> 23) - 127, -112), 126);
+      const float up = __uint_as_float(uint32_t(127 + 14 - e) << 23), down = __uint_as_float(uint32_t(127 - 14 + e) << 23);
+#pragma unroll
+      for (int ks = 0; ks < C::KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const float2 x = Half2<__nv_bfloat16>::unpack(qf[nt][ks][i]);
+          qf[nt][ks][i] = Half2<__half>::pack(x.x * up, x.y * up);
+        }
+      factor[nt][0] *= __shfl_sync(0xffffffffu, down, 8 * t);
+      factor[nt][1] *= __shfl_sync(0xffffffffu, down, 8 * t + 4);
     }
   }
 }
@@ -232,10 +254,10 @@ __device__ __forceinline__ void score_step(uint32_t keys, const uint32_t (&qf)[C
       const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const uint32_t af[4] = {codes_to<typename C::T>(__byte_perm(wl[j], 0, 0x4140)), codes_to<typename C::T>(__byte_perm(wh[j], 0, 0x4140)),
-                                codes_to<typename C::T>(__byte_perm(wl[j], 0, 0x4342)), codes_to<typename C::T>(__byte_perm(wh[j], 0, 0x4342))};
+        const uint32_t l = wl[j] ^ 0x80808080u, h = wh[j] ^ 0x80808080u;
+        const uint32_t af[4] = {pair_of_flipped(l, 0), pair_of_flipped(h, 0), pair_of_flipped(l, 1), pair_of_flipped(h, 1)};
 #pragma unroll
-        for (int nt = 0; nt < C::NT; ++nt) mma16816<typename C::T>(acc[nt], af, qf[nt][b * 4 + j]);
+        for (int nt = 0; nt < C::NT; ++nt) mma16816<__half>(acc[nt], af, qf[nt][b * 4 + j]);
       }
     }
   } else {
@@ -276,10 +298,10 @@ __device__ __forceinline__ void value_step(uint32_t values, const uint32_t (&p)[
 #pragma unroll
         for (int e = 0; e < 2; ++e) {  // channels 4 j + 2 e and + 1 of the run
           const int lo = e ? 0x4642 : 0x4440, hi = e ? 0x4743 : 0x4541;
-          const uint32_t af[4] = {codes_to<__nv_bfloat16>(__byte_perm(w[0][j], w[1][j], lo)), codes_to<__nv_bfloat16>(__byte_perm(w[0][j], w[1][j], hi)),
-                                  codes_to<__nv_bfloat16>(__byte_perm(w[2][j], w[3][j], lo)), codes_to<__nv_bfloat16>(__byte_perm(w[2][j], w[3][j], hi))};
+          const uint32_t af[4] = {pair_of_halves(__byte_perm(w[0][j], w[1][j], lo)), pair_of_halves(__byte_perm(w[0][j], w[1][j], hi)),
+                                  pair_of_halves(__byte_perm(w[2][j], w[3][j], lo)), pair_of_halves(__byte_perm(w[2][j], w[3][j], hi))};
 #pragma unroll
-          for (int nt = 0; nt < C::NT; ++nt) mma16816<__nv_bfloat16>(out[nt][run * 8 + j * 2 + e], af, p[nt]);
+          for (int nt = 0; nt < C::NT; ++nt) mma16816<__half>(out[nt][run * 8 + j * 2 + e], af, p[nt]);
         }
     }
   } else {
@@ -303,7 +325,7 @@ __device__ __forceinline__ int channel_of(int mt, int second) {
 
 // ---- attention --------------------------------------------------------------------------------------------
 template <typename C>
-__global__ __launch_bounds__(kThreads) void paged_rows_kernel(const RowsArgs a) {
+__global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const RowsArgs a) {
   extern __shared__ __align__(128) char smem[];
   __shared__ LineShared<kThreads> shared;
   __shared__ float warp_max[kWarps][C::R], warp_sum[kWarps][C::R];
@@ -339,7 +361,8 @@ __global__ __launch_bounds__(kThreads) void paged_rows_kernel(const RowsArgs a) 
     const int s = piece.sequence, head = piece.head, row0 = piece.block * R, rows = seq.count * a.line.group, take = piece.count;
 
     uint32_t qf[NT][C::KS][2];
-    load_queries<C>(a, seq, head, row0, rows, qf);
+    float factor[NT][2];
+    load_queries<C>(a, seq, head, row0, rows, qf, factor);
     int lo[NT][2], hi[NT][2];  // visible keys of rows 2 t and 2 t + 1
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
@@ -385,20 +408,20 @@ __global__ __launch_bounds__(kThreads) void paged_rows_kernel(const RowsArgs a) 
       const bool hidden = walk.hidden >> stage & 1;
       float acc[NT][4];
       score_step<C>(data, qf, acc);
-      float ks0 = a.scale_log2, ks1 = a.scale_log2, vs0 = 1.f, vs1 = 1.f;
+      float ks0 = 1.f, ks1 = 1.f, vs0 = 1.f, vs1 = 1.f, lift0 = 0.f, lift1 = 0.f;
       if (C::INT8) {
-        ks0 *= read_float(data + 2 * C::SIDE + g * 4);
-        ks1 *= read_float(data + 2 * C::SIDE + (g + 8) * 4);
+        ks0 = read_float(data + 2 * C::SIDE + g * 4);
+        ks1 = read_float(data + 2 * C::SIDE + (g + 8) * 4);
         vs0 = read_float(data + 2 * C::SIDE + 64 + g * 4);
         vs1 = read_float(data + 2 * C::SIDE + 64 + (g + 8) * 4);
+        // a row of zeros must not let its own probability overflow
+        lift0 = lg2_approx(fmaxf(vs0, 0x1p-100f));
+        lift1 = lg2_approx(fmaxf(vs1, 0x1p-100f));
       }
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt) {
-        acc[nt][0] *= ks0;
-        acc[nt][1] *= ks0;
-        acc[nt][2] *= ks1;
-        acc[nt][3] *= ks1;
-      }
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) acc[nt][e] *= C::INT8 ? (e < 2 ? ks0 : ks1) * factor[nt][e & 1] : factor[nt][e & 1];
       if (hidden || key < all_lo || key + 16 > all_hi) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -414,7 +437,7 @@ __global__ __launch_bounds__(kThreads) void paged_rows_kernel(const RowsArgs a) 
         float top[2], keep[2];
 #pragma unroll
         for (int i2 = 0; i2 < 2; ++i2) {
-          float x = fmaxf(acc[nt][i2], acc[nt][2 + i2]);
+          float x = fmaxf(acc[nt][i2] + lift0, acc[nt][2 + i2] + lift1);
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -441,11 +464,9 @@ __global__ __launch_bounds__(kThreads) void paged_rows_kernel(const RowsArgs a) 
         for (int i2 = 0; i2 < 4; ++i2) e[i2] = ex2_approx(acc[nt][i2] - m[nt][i2 & 1]);
         l[nt][0] += e[0] + e[2];
         l[nt][1] += e[1] + e[3];
-        // Probabilities leave 32 bits here (relative error 2^-9 in bf16, 2^-12 in fp16); with codes always to
-        // bf16, whose range holds probability times scale however small the scale is.
-        using P = std::conditional_t<C::INT8, __nv_bfloat16, T>;
-        p[nt][0] = transposed8x8(Half2<P>::pack(e[0] * vs0, e[1] * vs0));
-        p[nt][1] = transposed8x8(Half2<P>::pack(e[2] * vs1, e[3] * vs1));
+        // Probabilities (times scales) leave 32 bits here: half a step, 2^-8 of the value in bf16, 2^-11 in fp16.
+        p[nt][0] = transposed8x8(Half2<typename C::M>::pack(C::INT8 ? e[0] * vs0 : e[0], C::INT8 ? e[1] * vs0 : e[1]));
+        p[nt][1] = transposed8x8(Half2<typename C::M>::pack(C::INT8 ? e[2] * vs1 : e[2], C::INT8 ? e[3] * vs1 : e[3]));
       }
       value_step<C>(data + C::SIDE, p, o);
       stage = stage + 1 == W::STAGES ? 0 : stage + 1;
@@ -520,7 +541,7 @@ __global__ __launch_bounds__(kThreads) void paged_rows_kernel(const RowsArgs a) 
 // The same walk over K alone.  A key's weight is a sum over query rows, so a unit is (sequence, key head)
 // with all its rows, a warp's 16 keys are its own and nothing is joined.
 template <typename C>
-__global__ __launch_bounds__(kThreads) void weigh_rows_kernel(const RowsArgs a) {
+__global__ __launch_bounds__(kThreads, C::CTAS) void weigh_rows_kernel(const RowsArgs a) {
   extern __shared__ __align__(128) char smem[];
   __shared__ LineShared<kThreads> shared;
   using W = Walk<C, false>;
@@ -560,9 +581,9 @@ __global__ __launch_bounds__(kThreads) void weigh_rows_kernel(const RowsArgs a) 
     for (int i = 0; i < W::STAGES - 1; ++i) walk.fetch(i, i);
     uint32_t qf[NT][C::KS][2];
     int lo[NT][2], hi[NT][2];
-    float lse2[NT][2];
+    float lse2[NT][2], factor[NT][2];
     auto load_block = [&](int block) {
-      load_queries<C>(a, seq, head, block * R, rows, qf);
+      load_queries<C>(a, seq, head, block * R, rows, qf, factor);
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -587,10 +608,10 @@ __global__ __launch_bounds__(kThreads) void weigh_rows_kernel(const RowsArgs a) 
       const uint32_t data = ring + stage * W::STAGE;
       const int key = walk.key_of(i);
       const bool hidden = walk.hidden >> stage & 1;
-      float ks0 = a.scale_log2, ks1 = a.scale_log2;
+      float ks0 = 1.f, ks1 = 1.f;
       if (C::INT8) {
-        ks0 *= read_float(data + C::SIDE + g * 4);
-        ks1 *= read_float(data + C::SIDE + (g + 8) * 4);
+        ks0 = read_float(data + C::SIDE + g * 4);
+        ks1 = read_float(data + C::SIDE + (g + 8) * 4);
       }
       float sum0 = 0.f, sum1 = 0.f;
       for (int block = 0; block < blocks; ++block) {
@@ -603,7 +624,8 @@ __global__ __launch_bounds__(kThreads) void weigh_rows_kernel(const RowsArgs a) 
           for (int e = 0; e < 4; ++e) {
             const int k = key + g + (e >> 1) * 8;
             const bool seen = !hidden && k >= lo[nt][e & 1] && k < hi[nt][e & 1];
-            const float w = seen ? ex2_approx(fmaf(acc[nt][e], e < 2 ? ks0 : ks1, -lse2[nt][e & 1])) : 0.f;
+            const float f = C::INT8 ? (e < 2 ? ks0 : ks1) * factor[nt][e & 1] : factor[nt][e & 1];
+            const float w = seen ? ex2_approx(fmaf(acc[nt][e], f, -lse2[nt][e & 1])) : 0.f;
             if (e < 2) sum0 += w; else sum1 += w;
           }
       }
@@ -626,7 +648,7 @@ __global__ __launch_bounds__(kThreads) void weigh_rows_kernel(const RowsArgs a) 
 }
 
 // ---- launches ------------------------------------------------------------------------------------------------
-constexpr int kMaxWorkers = 148 * 2;
+constexpr int kSms = 148, kMaxWorkers = kSms * 3;
 
 template <typename F>
 int with_tile(int dtype_code, bool codes, int head_dim, int column_blocks, F&& f) {
@@ -744,7 +766,7 @@ extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const ris
     using C = decltype(tile);
     constexpr int bytes = kWarps * Walk<C, true>::STAGE * Walk<C, true>::STAGES;
     if (const int bad = allow_shared(paged_rows_kernel<C>, bytes, "paged attention")) return bad;
-    const int workers = C::D == 256 && !C::INT8 ? kMaxWorkers / 2 : kMaxWorkers;
+    const int workers = kSms * C::CTAS;
     launch_chained(paged_rows_kernel<C>, dim3(workers), dim3(kThreads), bytes, stream, a);
     const JoinArgs join{a.parts, a.notes, C::R, a.line.group, q_heads, out, a.on, a.oh, lse};
     launch_chained(join_parts_kernel<typename C::T, C::D, true>, dim3(workers - 1, C::R), dim3(128), 0, stream, join);
@@ -792,7 +814,7 @@ extern "C" int risa_b200_key_weights(const risa_b200_cache* cache, const risa_b2
     using C = decltype(tile);
     constexpr int bytes = kWarps * Walk<C, false>::STAGE * Walk<C, false>::STAGES;
     if (const int bad = allow_shared(weigh_rows_kernel<C>, bytes, "key weights")) return bad;
-    launch_chained(weigh_rows_kernel<C>, dim3(C::D == 256 && !C::INT8 ? kMaxWorkers / 2 : kMaxWorkers), dim3(kThreads), bytes,
+    launch_chained(weigh_rows_kernel<C>, dim3(kSms * C::CTAS), dim3(kThreads), bytes,
                    stream, a);
     return RISA_B200_OK;
   });
