@@ -411,11 +411,12 @@ struct SelectArgs {
 
 constexpr int kSelectThreads = 1024;
 
-// One CTA per (sequence, key head).  The count-th largest of the unprotected weights is found digit by
-// digit (11 + 11 + 10 bits) from histograms in shared memory; counters are whole numbers, so no order of
-// the atomics shows in the result.  Then each warp walks its own run of the sequence twice: counting
-// what it keeps, and (after a scan over the warps) writing it, so that kept tokens stay in order and
-// ties go to the lowest index.
+// One CTA per (sequence, key head).  Warp w owns the tokens of one run, in rounds of 32; the first kHeld rounds' weights stay in
+// registers between the passes over them, what is longer is read again.  The count-th largest of the unprotected weights is
+// found digit by digit (11 + 11 + 10 bits) from histograms in shared memory; counters are whole numbers, so no order of the
+// atomics shows in the result.  Then each warp goes over its run twice: counting what it keeps, and (after a scan over the
+// warps) writing it, so that kept tokens stay in order and ties go to the lowest index.
+constexpr int kHeld = 16;
 __global__ __launch_bounds__(kSelectThreads) void select_kept_kernel(const SelectArgs a) {
   __shared__ unsigned int histogram[2048];
   __shared__ unsigned int warp_totals[2][32];
@@ -433,9 +434,27 @@ __global__ __launch_bounds__(kSelectThreads) void select_kept_kernel(const Selec
   if (head == 0 && tid == 0) a.new_lengths[s] = count;
   const int open = length - recent;         // tokens that compete
   const unsigned int wanted = count - recent;  // of which so many stay
+  const int rounds = ((length + 31) / 32 + 31) / 32, begin = warp * rounds * 32;
+  float held[kHeld];
+#pragma unroll
+  for (int n = 0; n < kHeld; ++n) {
+    const int i = begin + n * 32 + lane;
+    held[n] = n < rounds && i < length ? weights[i] : 0.f;
+  }
+  // f(token, weight) for every round of this warp, whole warps at a time
+  auto each = [&](auto&& f) {
+#pragma unroll
+    for (int n = 0; n < kHeld; ++n)
+      if (n < rounds) f(begin + n * 32 + lane, held[n]);
+    for (int n = kHeld; n < rounds; ++n) {
+      const int i = begin + n * 32 + lane;
+      f(i, i < length ? weights[i] : 0.f);
+    }
+  };
   uint32_t threshold = 0;                    // larger ones stay,
   unsigned int equal_wanted = 0;             // and so many of those equal to it
-  if (wanted > 0 && int(wanted) < open) {
+  const bool all = int(wanted) >= open, none = wanted == 0;
+  if (!all && !none) {
     unsigned int above = 0;  // tokens known to be larger than every one with the prefix
     uint32_t prefix = 0;
     int shift = 21;
@@ -444,13 +463,12 @@ __global__ __launch_bounds__(kSelectThreads) void select_kept_kernel(const Selec
       const int bits = digit == 2 ? 10 : 11, bins = 1 << bits;
       for (int i = tid; i < bins; i += kSelectThreads) histogram[i] = 0;
       __syncthreads();
-      for (int i = tid; i < open; i += kSelectThreads) {
-        const uint32_t o = order_of(weights[i]);
-        if (digit == 0 || (o >> (shift + bits)) == prefix) atomicAdd(&histogram[(o >> shift) & (bins - 1)], 1u);
-      }
+      each([&](int i, float w) {
+        const uint32_t o = order_of(w);
+        if (i < open && (digit == 0 || (o >> (shift + bits)) == prefix)) atomicAdd(&histogram[(o >> shift) & (bins - 1)], 1u);
+      });
       __syncthreads();
-      // suffix sums over the bins: the bin that holds the wanted-th largest.  A thread takes two bins,
-      // from the top down.
+      // suffix sums over the bins: the bin that holds the wanted-th largest.  A thread takes two bins, from the top down.
       const int top = bins - 1 - 2 * tid;
       const unsigned int h0 = top >= 0 ? histogram[top] : 0, h1 = top >= 1 ? histogram[top - 1] : 0;
       unsigned int sum = h0 + h1;
@@ -461,8 +479,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_kept_kernel(const Selec
       }
       if (lane == 31) warp_totals[0][warp] = sum;
       __syncthreads();
-      unsigned int before = above;
-      for (int w = 0; w < warp; ++w) before += warp_totals[0][w];
+      const unsigned int before = above + __reduce_add_sync(0xffffffffu, lane < warp ? warp_totals[0][lane] : 0u);
       const unsigned int through = before + sum, until = through - h0 - h1;  // tokens above these two bins
       if (until < wanted && through >= wanted) {
         const bool first = until + h0 >= wanted;
@@ -478,39 +495,25 @@ __global__ __launch_bounds__(kSelectThreads) void select_kept_kernel(const Selec
     threshold = prefix;
     equal_wanted = wanted - above;
   }
-  const bool all = int(wanted) >= open;
-  // runs of whole warps' strides: warp w owns tokens [begin, end)
-  const int run = ((length + 31) / 32 + 31) / 32 * 32;
-  const int begin = min(warp * run, length), end = min(begin + run, length);
-  unsigned int larger = 0, equal = 0;
-  for (int i0 = begin; i0 < end; i0 += 32) {
-    const int i = i0 + lane;
-    const uint32_t o = i < end && i < open ? order_of(weights[i]) : 0;
-    const bool in = i < end && i < open;
-    larger += __popc(__ballot_sync(0xffffffffu, i < end && (i >= open || all || (wanted > 0 && o > threshold))));
-    equal += __popc(__ballot_sync(0xffffffffu, in && !all && wanted > 0 && o == threshold));
-  }
+  // stays for certain / ties with the threshold
+  auto larger = [&](int i, float w) { return i < length && (i >= open || all || (!none && order_of(w) > threshold)); };
+  auto equal = [&](int i, float w) { return i < open && !all && !none && order_of(w) == threshold; };
+  unsigned int larger_count = 0, equal_count = 0;
+  each([&](int i, float w) {
+    larger_count += __popc(__ballot_sync(0xffffffffu, larger(i, w)));
+    equal_count += __popc(__ballot_sync(0xffffffffu, equal(i, w)));
+  });
   if (lane == 0) {
-    warp_totals[0][warp] = larger;
-    warp_totals[1][warp] = equal;
+    warp_totals[0][warp] = larger_count;
+    warp_totals[1][warp] = equal_count;
   }
   __syncthreads();
-  unsigned int at = 0, equal_before = 0;
-  for (int w = 0; w < warp; ++w) {
-    at += warp_totals[0][w];
-    equal_before += warp_totals[1][w];
-  }
-  at += min(equal_before, equal_wanted);
-  for (int i0 = begin; i0 < end; i0 += 32) {
-    const int i = i0 + lane;
-    const bool in = i < end && i < open;
-    const float w = i < end ? weights[i] : 0.f;
-    const uint32_t o = order_of(w);
-    const bool ties = in && !all && wanted > 0 && o == threshold;
-    const unsigned int tied = __ballot_sync(0xffffffffu, ties);
-    const unsigned int below = (1u << lane) - 1;
-    bool stays = i < end && (i >= open || all || (wanted > 0 && o > threshold));
-    if (ties && equal_before + __popc(tied & below) < equal_wanted) stays = true;
+  unsigned int equal_before = __reduce_add_sync(0xffffffffu, lane < warp ? warp_totals[1][lane] : 0u);
+  unsigned int at = __reduce_add_sync(0xffffffffu, lane < warp ? warp_totals[0][lane] : 0u) + min(equal_before, equal_wanted);
+  each([&](int i, float w) {
+    const bool ties = equal(i, w);
+    const unsigned int tied = __ballot_sync(0xffffffffu, ties), below = (1u << lane) - 1;
+    const bool stays = larger(i, w) || (ties && equal_before + __popc(tied & below) < equal_wanted);
     const unsigned int mask = __ballot_sync(0xffffffffu, stays);
     if (stays) {
       const unsigned int to = at + __popc(mask & below);
@@ -519,7 +522,7 @@ __global__ __launch_bounds__(kSelectThreads) void select_kept_kernel(const Selec
     }
     at += __popc(mask);
     equal_before += __popc(tied);
-  }
+  });
   for (int i = count + tid; i < a.budget; i += kSelectThreads) kept[i] = -1;
   for (int i = count + tid; i < a.target_slots; i += kSelectThreads) new_weights[i] = 0.f;
 }

@@ -762,23 +762,30 @@ extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const ris
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   const bool tensor_cores = takes_tensor_cores(*cache, *step, a.line.group);
   if (tensor_cores) a.line.max_rows = kTcFewestRows - 1;
-  int bad = with_tile(dtype_code, cache->dtype_code == kInt8, cache->head_dim, a.line.rows / 8, [&](auto tile) {
+  const bool codes = cache->dtype_code == kInt8;
+  int bad = with_tile(dtype_code, codes, cache->head_dim, a.line.rows / 8, [&](auto tile) {
     using C = decltype(tile);
     constexpr int bytes = kWarps * Walk<C, true>::STAGE * Walk<C, true>::STAGES;
     if (const int bad = allow_shared(paged_rows_kernel<C>, bytes, "paged attention")) return bad;
-    const int workers = kSms * C::CTAS;
-    launch_chained(paged_rows_kernel<C>, dim3(workers), dim3(kThreads), bytes, stream, a);
-    const JoinArgs join{a.parts, a.notes, C::R, a.line.group, q_heads, out, a.on, a.oh, lse};
-    launch_chained(join_parts_kernel<typename C::T, C::D, true>, dim3(workers - 1, C::R), dim3(128), 0, stream, join);
+    launch_chained(paged_rows_kernel<C>, dim3(kSms * C::CTAS), dim3(kThreads), bytes, stream, a);
     return RISA_B200_OK;
   });
+  TcArgs t{};
   if (bad == RISA_B200_OK && tensor_cores) {
-    TcArgs t{a.line, q, a.qn, a.qh, out, a.on, a.oh, lse, a.keys, a.values, a.key_scales, a.value_scales, a.pages, a.scale_log2,
-             a.parts + rows_scratch(*cache, *step, a.line.group) / sizeof(float), nullptr, 2, status};
+    t = paged_tc_args(TcArgs{a.line, q, a.qn, a.qh, out, a.on, a.oh, lse, a.keys, a.values, a.key_scales, a.value_scales, a.pages, a.scale_log2,
+                             a.parts + rows_scratch(*cache, *step, a.line.group) / sizeof(float), nullptr, 2, status}, cache->head_dim);
     t.line.min_rows = kTcFewestRows;
     t.line.max_rows = INT_MAX;
-    bad = paged_tc(t, dtype_code, cache->dtype_code == kInt8, cache->head_dim, stream);
+    bad = paged_tc(t, dtype_code, codes, cache->head_dim, stream);
   }
+  if (bad == RISA_B200_OK)
+    bad = with_tile(dtype_code, codes, cache->head_dim, a.line.rows / 8, [&](auto tile) {
+      using C = decltype(tile);
+      const JoinArgs join{a.parts, a.notes, C::R, a.line.group, q_heads, out, a.on, a.oh, lse};
+      launch_chained(join_parts_kernel<typename C::T, C::D, true>, dim3(kSms * C::CTAS - 1, C::R), dim3(128), 0, stream, join);
+      return RISA_B200_OK;
+    });
+  if (bad == RISA_B200_OK && tensor_cores) bad = paged_tc_join(t, dtype_code, cache->head_dim, stream);
   return bad ? bad : check_launch("paged attention");
 }
 

@@ -419,12 +419,14 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
     mbar_init(smem_u32(&bars.drained), 1);
     mbar_init_fence();
   }
-  chain_wait();
+  // The launch in front is this call's own, for the sequences of few rows, and its start waited for everything before
+  // it; nothing it writes is read here.  So this one need not wait for it, only end behind it (the joins wait for this).
   chain_release();
   const int64_t total = line_total<kThreads>(a.line, shared);
   const int workers = workers_of(total, gridDim.x, a.min_steps);
   if (int(blockIdx.x) >= workers) {
     if (threadIdx.x == 0) a.notes[blockIdx.x] = JoinNote{};
+    chain_wait();
     return;
   }
   const int64_t begin = border(total, blockIdx.x, workers), finish = border(total, blockIdx.x + 1, workers);
@@ -478,6 +480,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
       }
     }
   }
+  chain_wait();
 }
 
 // The pool as {channels, a page's rows, pages x heads}, in boxes of 64 channels x a page with the 128-byte swizzle.
@@ -502,6 +505,13 @@ bool pool_map(CUtensorMap* map, const char* pool, const TcArgs& a) {
                      CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
+template <typename T, int D>
+int join(const TcArgs& a, cudaStream_t stream) {
+  const JoinArgs join{a.parts, a.notes, kRows, a.line.group, a.line.kv_heads * a.line.group, a.out, a.on, a.oh, a.lse};
+  launch_chained(join_parts_kernel<T, D, false>, dim3(kTcWorkers - 1, kRows / 16), dim3(128), 0, stream, join);
+  return RISA_B200_OK;
+}
+
 template <typename C>
 int launch(const TcArgs& a, cudaStream_t stream) {
   CUtensorMap key_map{}, value_map{};
@@ -518,8 +528,6 @@ int launch(const TcArgs& a, cudaStream_t stream) {
   }();
   RISA_REQUIRE(budget, "paged attention: the tensor-core kernel was not compiled for %d registers", kRegsLaunch);
   launch_chained(paged_tc_kernel<C>, dim3(kTcWorkers), dim3(kThreads), C::SMEM, stream, key_map, value_map, a);
-  const JoinArgs join{a.parts, a.notes, kRows, a.line.group, a.line.kv_heads * a.line.group, a.out, a.on, a.oh, a.lse};
-  launch_chained(join_parts_kernel<typename C::T, C::D, false>, dim3(kTcWorkers - 1, kRows / 16), dim3(128), 0, stream, join);
   return RISA_B200_OK;
 }
 
@@ -527,15 +535,22 @@ int launch(const TcArgs& a, cudaStream_t stream) {
 
 size_t paged_tc_scratch(int head_dim) { return size_t(kTcWorkers) * (2 * slot_floats(kRows, head_dim) * sizeof(float) + sizeof(JoinNote)); }
 
-int paged_tc(TcArgs a, int dtype_code, bool codes, int head_dim, cudaStream_t stream) {
+TcArgs paged_tc_args(TcArgs a, int head_dim) {
   a.line.rows = Divisor(kRows);
   a.line.keys = Divisor(kTileKeys);
   a.notes = reinterpret_cast<JoinNote*>(a.parts + size_t(kTcWorkers) * 2 * slot_floats(kRows, head_dim));
+  return a;
+}
+int paged_tc(const TcArgs& a, int dtype_code, bool codes, int head_dim, cudaStream_t stream) {
   if (dtype_code == 1)
     return head_dim == 64 ? (codes ? launch<Shape<__half, true, 64>>(a, stream) : launch<Shape<__half, false, 64>>(a, stream))
                           : (codes ? launch<Shape<__half, true, 128>>(a, stream) : launch<Shape<__half, false, 128>>(a, stream));
   return head_dim == 64 ? (codes ? launch<Shape<__nv_bfloat16, true, 64>>(a, stream) : launch<Shape<__nv_bfloat16, false, 64>>(a, stream))
                         : (codes ? launch<Shape<__nv_bfloat16, true, 128>>(a, stream) : launch<Shape<__nv_bfloat16, false, 128>>(a, stream));
+}
+int paged_tc_join(const TcArgs& a, int dtype_code, int head_dim, cudaStream_t stream) {
+  if (dtype_code == 1) return head_dim == 64 ? join<__half, 64>(a, stream) : join<__half, 128>(a, stream);
+  return head_dim == 64 ? join<__nv_bfloat16, 64>(a, stream) : join<__nv_bfloat16, 128>(a, stream);
 }
 
 // Site of the first wait of these kernels that ran out since the last call (0: none), or -1 on a CUDA error.

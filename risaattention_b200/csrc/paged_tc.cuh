@@ -10,7 +10,7 @@ constexpr int kTcWorkers = 148;  // one CTA per SM
 constexpr int kTcFewestRows = 33;
 
 struct TcArgs {
-  LineArgs line;  // rows and keys are the kernel's own
+  LineArgs line;  // rows, keys and notes are the kernel's own: paged_tc_args
   const void* q;
   int64_t qn, qh;
   void* out;
@@ -23,16 +23,19 @@ struct TcArgs {
   int pages;
   float scale_log2;
   float* parts;
-  JoinNote* notes;  // set by the kernel's own launcher
+  JoinNote* notes;  // behind the parts
   int min_steps;
   unsigned int* status;
 };
 
 size_t paged_tc_scratch(int head_dim);
-int paged_tc(TcArgs args, int dtype_code, bool codes, int head_dim, cudaStream_t stream);
+// The kernel runs beside the launch in front of it, which has to be one of the same call; the join comes behind both.
+TcArgs paged_tc_args(TcArgs args, int head_dim);
+int paged_tc(const TcArgs& args, int dtype_code, bool codes, int head_dim, cudaStream_t stream);
+int paged_tc_join(const TcArgs& args, int dtype_code, int head_dim, cudaStream_t stream);
 int paged_tc_wait_status();
 
-// Key weights (weigh_tc.cu); `out`, `lse` and `values` of the arguments are not used.
+// Key weights (weigh_tc.cu), likewise beside the launch in front; `out`, `lse` and `values` of the arguments are not used.
 size_t weigh_tc_scratch();
 int weigh_tc(const TcArgs& args, const float* row_lse, const float* previous, float* weights, int dtype_code, bool codes, int head_dim,
              cudaStream_t stream);

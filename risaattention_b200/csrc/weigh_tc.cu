@@ -378,8 +378,7 @@ __global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a
     mbar_init(smem_u32(&bars.drained), 1);
     mbar_init_fence();
   }
-  chain_wait();
-  chain_release();
+  chain_release();  // and no wait: see paged_tc_kernel
   // what no block covers: in front of the window, behind the length
   const int slots = a.line.step.width << a.line.step.page_shift;
   for (int64_t u = blockIdx.x; u < int64_t(a.line.step.batch) * a.line.kv_heads; u += gridDim.x) {
@@ -396,6 +395,7 @@ __global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a
   const int workers = workers_of(total, gridDim.x, a.min_steps);
   if (int(blockIdx.x) >= workers) {
     if (threadIdx.x == 0) a.notes[blockIdx.x] = JoinNote{};
+    chain_wait();
     return;
   }
   const int64_t begin = border(total, blockIdx.x, workers), finish = border(total, blockIdx.x + 1, workers);
@@ -446,6 +446,7 @@ __global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a
       else if (key < slots) a.weights[(int64_t(piece.sequence) * a.line.kv_heads + piece.head) * slots + key] = NAN;
     }
   }
+  chain_wait();
 }
 
 // The parts of the block that worker blockIdx.x ended with, added up in order.
