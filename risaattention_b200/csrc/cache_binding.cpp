@@ -41,6 +41,11 @@ int code_of(const at::Tensor& t) {
   }
 }
 
+// No two elements of a tensor that is written may share memory.
+void require_distinct(const at::Tensor& t, const char* what) {
+  for (int64_t i = 0; i < t.dim(); ++i) require(t.size(i) <= 1 || t.stride(i) != 0, std::string(what) + " must not be an expanded view");
+}
+
 // Rows of eight channels that start on 16-byte boundaries: the tensor itself, or a packed copy.
 at::Tensor rows_of(const at::Tensor& t) {
   bool good = t.stride(-1) == 1 && reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0;
@@ -163,6 +168,7 @@ at::Tensor rotate(const at::Tensor& x, const at::Tensor& positions, const at::Te
   require(x.stride(-1) == 1 || d == 1, "the last dimension of x must be contiguous");
   if (out_given.has_value()) {
     require(out_given->sizes() == x.sizes() && (out_given->stride(-1) == 1 || d == 1), "out must have the shape of x and contiguous rows");
+    require_distinct(*out_given, "out");
     require_type(out_given->scalar_type() == x.scalar_type(), "out must have the dtype of x");
     require(out_given->device() == x.device(), "out must be on the device of x");
     require(out_given->data_ptr() != x.data_ptr() || out_given->strides() == x.strides(), "out may be x itself, not another view of its memory");
@@ -258,6 +264,7 @@ py::tuple paged_attention(const at::Tensor& q, const at::Tensor& cache_keys, con
     require(out_given->sizes() == q.sizes() && out_given->stride(2) == 1 && (q.size(0) <= 1 || out_given->stride(0) % 8 == 0) &&
                 (q.size(1) <= 1 || out_given->stride(1) % 8 == 0),
             "out must have the shape of q and rows that start on 16-byte boundaries");
+    require_distinct(*out_given, "out");
     require_type(out_given->scalar_type() == q.scalar_type(), "out must have the dtype of q");
   }
   const Step step(cache, table, lengths, offsets, q.size(0));

@@ -414,9 +414,9 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
         ks1 = read_float(data + 2 * C::SIDE + (g + 8) * 4);
         vs0 = read_float(data + 2 * C::SIDE + 64 + g * 4);
         vs1 = read_float(data + 2 * C::SIDE + 64 + (g + 8) * 4);
-        // a row of zeros must not let its own probability overflow
-        lift0 = lg2_approx(fmaxf(vs0, 0x1p-100f));
-        lift1 = lg2_approx(fmaxf(vs1, 0x1p-100f));
+        // a row of zeros must not let its own probability overflow, nor one that is not finite let the others vanish
+        lift0 = vs0 < INFINITY ? lg2_approx(fmaxf(vs0, 0x1p-100f)) : 0.f;
+        lift1 = vs1 < INFINITY ? lg2_approx(fmaxf(vs1, 0x1p-100f)) : 0.f;
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)

@@ -43,6 +43,7 @@ constexpr float kStale = 8.0f;
 template <typename T_, bool INT8_, int D_>
 struct Shape {
   using T = T_;
+  using M = std::conditional_t<INT8_, __half, T_>;  // type of the matrix instructions' operands
   static constexpr bool INT8 = INT8_;
   static constexpr int D = D_;
   static constexpr int SIDE = kTileKeys * D * 2;  // a K or V tile as the matrix instructions read it
@@ -60,6 +61,14 @@ struct Exchange {
   float maximum[2][kGroups][2][128];
   float sum[kGroups][2][128];
 };
+// Over a cache of codes: scales of the tiles in flight (a slot is written again kScaleDepth tiles later, by when the softmax
+// that read it has handed over its probabilities), the largest of each 32 values' scales in units of log 2, and what the
+// queries' rows were divided by, of this unit and the one before.
+constexpr int kScaleDepth = 8;
+struct Scales {
+  float key[kScaleDepth][kTileKeys], value[kScaleDepth][kTileKeys], lift[kScaleDepth][4];
+  float row[2][kGroups][128];
+};
 
 // ---- the fetching warpgroup -----------------------------------------------------------------------------------
 // Tiles of 16-bit rows that all exist come by TMA, a box of 64 channels x a page at a time: 128 threads that copy 16
@@ -67,7 +76,7 @@ struct Exchange {
 // front of a window, pages outside the pool) are copied piece by piece with zeros in place of what is not there.
 template <typename C>
 __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* key_map, const CUtensorMap* value_map, Pieces pieces, Barriers* bars,
-                                            volatile uint32_t* notes, uint32_t k_ring, uint32_t v_ring, uint32_t gave_up) {
+                                            volatile uint32_t* notes, Scales* scales, uint32_t k_ring, uint32_t v_ring, uint32_t gave_up) {
   const int p = threadIdx.x - kProducer * 32;
   uint32_t issued = 0;
   RingPos<C::STAGES> stage;  // of both rings
@@ -99,8 +108,20 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
           return;
         }
         if constexpr (C::INT8) {
-          // scaled and rounded to the queries' type (half a step), as if the cache had held 16-bit values
-          convert_keys<typename C::T, C::D, kTileKeys, true>(side ? values : keys, runs, piece.head, to, 0, p);
+          // codes as they are; the softmax multiplies scores and probabilities by their keys' scales, in 32 bits
+          if (side == 0) {
+            const int key = runs.key0 + p, page = __shfl_sync(0xffffffffu, runs.id, p >> 4), slot = issued % kScaleDepth;
+            const bool there = page >= 0 && key >= low && key < length;
+            const int64_t line = there ? keys.line(page, piece.head, key) : 0;
+            const float v = there ? __ldg(values.scales + line) : 0.f;
+            scales->key[slot][p] = there ? __ldg(keys.scales + line) : 0.f;
+            scales->value[slot][p] = v;
+            float most = v < INFINITY ? fmaxf(v, 0x1p-100f) : 0x1p-100f;  // one that is not finite must not let the others vanish
+#pragma unroll
+            for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
+            if ((p & 31) == 0) scales->lift[slot][p >> 5] = lg2_approx(most);
+          }
+          convert_keys<__half, C::D, kTileKeys>(side ? values : keys, runs, piece.head, to, 0, p);
           fence_async_smem();
           mbar_arrive(smem_u32(full + stage.stage));
         } else if (runs.bad == 0 && runs.key0 >= low && runs.key0 + kTileKeys <= length) {
@@ -141,7 +162,7 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
 template <typename C>
 __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const volatile uint32_t* notes, uint32_t tmem, uint32_t q, uint32_t k_ring,
                                                uint32_t v_ring, uint32_t gave_up) {
-  constexpr uint32_t kScores = idesc_f16<typename C::T>(false, kTileKeys), kOutput = idesc_f16<typename C::T>(true, C::D);
+  constexpr uint32_t kScores = idesc_f16<typename C::M>(false, kTileKeys), kOutput = idesc_f16<typename C::M>(true, C::D);
   RingPos<C::STAGES> k, v;
   uint32_t q_phase = 0, p_phase = 0, o_phase = 3;  // a bit per group
   const bool elected = elect_one();
@@ -210,7 +231,7 @@ __device__ __forceinline__ void leave(int id) { asm volatile("bar.arrive %0, 64;
 // Query rows of group g, by the 256 threads of its two warpgroups: 16-byte pieces, neighbouring threads along a row.  A
 // negative scale flips their signs, so that the maximum of the scores is the maximum of the scaled ones.
 template <typename C>
-__device__ __forceinline__ void load_query_rows(const TcArgs& a, const Piece& piece, int g, uint32_t to) {
+__device__ __forceinline__ void load_query_rows(const TcArgs& a, const Piece& piece, int g, uint32_t to, float* row_scale) {
   constexpr int PIECES = C::D / 8, EACH = 256 / PIECES;
   const int t = threadIdx.x & 255, rows = piece.seq.count * a.line.group, c = t % PIECES;
   const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
@@ -222,31 +243,36 @@ __device__ __forceinline__ void load_query_rows(const TcArgs& a, const Piece& pi
       const int token = row / a.line.group, h = row - token * a.line.group;
       v = *reinterpret_cast<const uint4*>(static_cast<const typename C::T*>(a.q) + int64_t(piece.seq.first + token) * a.qn +
                                           int64_t(piece.head * a.line.group + h) * a.qh + c * 8);
-      v.x ^= flip;
-      v.y ^= flip;
-      v.z ^= flip;
-      v.w ^= flip;
     }
+    if constexpr (C::INT8 && std::is_same<typename C::T, __nv_bfloat16>::value) {
+      const float down = row_to_half<PIECES>(v);
+      if (c == 0) row_scale[r] = down;
+    }
+    v.x ^= flip;
+    v.y ^= flip;
+    v.z ^= flip;
+    v.w ^= flip;
     store16(to + tile_offset(r, c), v);
   }
   fence_async_smem();
 }
 
 template <typename C>
-__device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Barriers* bars, Exchange* exchange, uint32_t tmem, uint32_t q, int g, int half,
+__device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Barriers* bars, Exchange* exchange, Scales* scales, uint32_t tmem, uint32_t q, int g, int half,
                                              const volatile uint32_t* notes, uint32_t gave_up) {
   constexpr int D = C::D, KEYS = kTileKeys / 2;
   using T = typename C::T;
   const int r = threadIdx.x & 127, meeting = 1 + g * 4 + (r >> 5);
   const uint32_t lanes = tmem + (uint32_t(r & ~31) << 16);
   const uint32_t s_columns = lanes + g * kTileKeys, o_columns = lanes + kGroups * kTileKeys + g * D + half * (D / 2);
-  const float scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // a scale of 0 must leave hidden scores at -inf
-  uint32_t s_phase = 0, o_phase = 0, tile = 0;
+  const float call_scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // a scale of 0 must leave hidden scores at -inf
+  uint32_t s_phase = 0, o_phase = 0, tile = 0, turn = 0;
   Piece piece;
   bool more = pieces.next(a.line, piece);
   auto mine = [&](const Piece& p) { return p.seq.count * a.line.group - p.block * kRows > g * 128; };
   auto fetch = [&](const Piece& p) {
-    load_query_rows<C>(a, p, g, q + g * C::SIDE);
+    turn ^= 1;
+    load_query_rows<C>(a, p, g, q + g * C::SIDE, C::INT8 ? scales->row[turn][g] : nullptr);
     mbar_arrive_warp(smem_u32(bars->q_full + g));
   };
   if (more && mine(piece)) fetch(piece);
@@ -264,7 +290,8 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
     const int token0 = (piece.block * kRows + g * 128) / a.line.group, token1 = (min(piece.block * kRows + g * 128 + 128, rows) - 1) / a.line.group;
     const int all_hi = visible(piece.seq.length - piece.seq.count + token0, piece.seq.length, a.line.causal, a.line.window).hi;
     const int all_lo = visible(piece.seq.length - piece.seq.count + token1, piece.seq.length, a.line.causal, a.line.window).lo;
-    float m = kNoMaximum, l = 0.f;
+    float m = kNoMaximum, l = 0.f, scale = call_scale;
+    const uint32_t mine_turn = turn;
 #pragma unroll 1
     for (int i = 0; i < piece.count; ++i, ++tile) {
       const int key0 = (piece.first + i) * kTileKeys + half * KEYS;
@@ -277,6 +304,20 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
       const uint32_t gone = notes[tile % kNotes] >> (half * 4) & (kHiddenRuns >> 4);
       tmem_load_wait();
       tmem_regs_ready<KEYS>(x);
+      const int slot_of_tile = tile % kScaleDepth;
+      if constexpr (C::INT8) {
+        if (std::is_same<T, __nv_bfloat16>::value && i == 0) scale = call_scale * scales->row[mine_turn][g][r];
+        const ulonglong2* k = reinterpret_cast<const ulonglong2*>(scales->key[slot_of_tile] + half * KEYS);
+#pragma unroll
+        for (int c = 0; c < KEYS; c += 4) {
+          const ulonglong2 s = k[c / 4];
+          float u[4];
+          unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), s.x), u[0], u[1]);
+          unpack_f32x2(mul_f32x2(pack_f32x2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])), s.y), u[2], u[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[c + e] = __float_as_uint(u[e]);
+        }
+      }
       if (gone != 0 || key0 < all_lo || key0 + KEYS > all_hi) {
         asm volatile("" ::: "memory");  // a branch of its own: as selects in the common path it cost a quarter of the time
         const int lo = seen.lo - key0, hi = seen.hi - key0;
@@ -292,6 +333,11 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
           top[e] = c + 4 + e < KEYS ? fmaxf(fmaxf(top[e], __uint_as_float(x[c + e])), __uint_as_float(x[c + 4 + e]))
                                     : fmaxf(top[e], __uint_as_float(x[c + e]));
       float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+      if constexpr (C::INT8) {
+        // the maximum is that of probability times scale, or a little above it: at most 1 is rounded
+        const float4 lift = *reinterpret_cast<const float4*>(scales->lift[slot_of_tile]);
+        best += fmaxf(fmaxf(lift.x, lift.y), fmaxf(lift.z, lift.w));
+      }
       // also: from here on both halves of the scores are in registers, and P may be written over them
       exchange->maximum[tile & 1][g][half][r] = best;
       meet(meeting);
@@ -327,7 +373,12 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
           u = ex2_approx(u);
           w = ex2_approx(w);
           sum[c & 1] = add_f32x2(sum[c & 1], pack_f32x2(u, w));
-          p[c] = Half2<T>::pack(u, w);
+          if constexpr (C::INT8) {
+            const float2 v = *reinterpret_cast<const float2*>(scales->value[slot_of_tile] + half * KEYS + at);
+            u *= v.x;
+            w *= v.y;
+          }
+          p[c] = Half2<typename C::M>::pack(u, w);
         }
         tmem_store16(s_columns + half * (KEYS / 2) + part * 16, p);
       }
@@ -395,6 +446,8 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
   extern __shared__ char smem_raw[];
   __shared__ Barriers bars;
   __shared__ Exchange exchange;
+  __shared__ __align__(16) typename std::conditional<C::INT8, Scales, char>::type scales_memory;
+  Scales* scales = reinterpret_cast<Scales*>(&scales_memory);
   __shared__ LineShared<kThreads> shared;
   __shared__ uint32_t tmem_base, gave_up_word;
   __shared__ volatile uint32_t notes[kNotes];
@@ -438,10 +491,10 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
   const uint32_t tmem = tmem_base;
   if (warp < kProducer) {
     regs_inc<kRegsSoftmax>();
-    softmax_rows<C>(a, pieces, &bars, &exchange, tmem, q, warp >> 3, (warp >> 2) & 1, notes, gave_up);
+    softmax_rows<C>(a, pieces, &bars, &exchange, scales, tmem, q, warp >> 3, (warp >> 2) & 1, notes, gave_up);
   } else if (warp < kIssuer) {
     regs_dec<kRegsProducer>();
-    fetch_tiles<C>(a, &key_map, &value_map, pieces, &bars, notes, k_ring, v_ring, gave_up);
+    fetch_tiles<C>(a, &key_map, &value_map, pieces, &bars, notes, scales, k_ring, v_ring, gave_up);
   } else {
     regs_dec<kRegsIssuer>();
     if (warp == kIssuer + 1 && (threadIdx.x & 31) == 0) {

@@ -63,24 +63,49 @@ __device__ __forceinline__ uint32_t tile_offset(int row, int piece) {
   return uint32_t((piece >> 3) * 16384 + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
 }
 
-// Codes 2 i and 2 i + 1 of a word whose sign bits have been flipped, times the scale: 2^23 + u is exact, so its
-// difference to 2^23 + 128 is the code.
-template <typename T>
-__device__ __forceinline__ uint32_t scaled_pair(uint32_t word, int i, float scale) {
-  const float a = __uint_as_float(__byte_perm(word, 0x4b000000u, i ? 0x7442 : 0x7440)) - 8388736.0f;
-  const float b = __uint_as_float(__byte_perm(word, 0x4b000000u, i ? 0x7443 : 0x7441)) - 8388736.0f;
-  return Half2<T>::pack(a * scale, b * scale);
+// Codes are whole numbers of at most 128, exact in both 16-bit types.  Codes 2 i and 2 i + 1 of a word whose sign bits have
+// been flipped (u = code + 128).  fp16: 0x6400 + u is 1024 + u, less 1152.  bf16, whose numbers from 128 to 256 are whole
+// ones: 128 + the low seven bits, less 128 or 256 as the top bit says; two instructions more.
+template <typename M> __device__ __forceinline__ uint32_t code_pair(uint32_t word, int i);
+template <> __device__ __forceinline__ uint32_t code_pair<__half>(uint32_t word, int i) {
+  const uint32_t u = __byte_perm(word, 0x64646464u, i ? 0x4342 : 0x4140), bias = 0x64806480u;
+  const __half2 d = __hsub2(*reinterpret_cast<const __half2*>(&u), *reinterpret_cast<const __half2*>(&bias));
+  return *reinterpret_cast<const uint32_t*>(&d);
 }
-
-// The 16 codes `w` of a row as 16-bit values: two pieces of its tile.
-template <typename T>
-__device__ __forceinline__ void store_codes(uint32_t tile, int row, int piece, uint4 w, float scale) {
+template <> __device__ __forceinline__ uint32_t code_pair<__nv_bfloat16>(uint32_t word, int i) {
+  const uint32_t u = __byte_perm(word, 0, i ? 0x4342 : 0x4140);
+  const uint32_t low = (u & 0x007f007fu) | 0x43004300u, less = (u & 0x00800080u) ^ 0x43804380u;
+  const __nv_bfloat162 d = __hsub2(*reinterpret_cast<const __nv_bfloat162*>(&low), *reinterpret_cast<const __nv_bfloat162*>(&less));
+  return *reinterpret_cast<const uint32_t*>(&d);
+}
+// The 16 codes `w` of a row as numbers of type M: two pieces of its tile.
+template <typename M>
+__device__ __forceinline__ void store_codes(uint32_t tile, int row, int piece, uint4 w) {
   const uint32_t u[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
 #pragma unroll
   for (int h = 0; h < 2; ++h)
     store16(tile + tile_offset(row, 2 * piece + h),
-            make_uint4(scaled_pair<T>(u[2 * h], 0, scale), scaled_pair<T>(u[2 * h], 1, scale), scaled_pair<T>(u[2 * h + 1], 0, scale),
-                       scaled_pair<T>(u[2 * h + 1], 1, scale)));
+            make_uint4(code_pair<M>(u[2 * h], 0), code_pair<M>(u[2 * h], 1), code_pair<M>(u[2 * h + 1], 0), code_pair<M>(u[2 * h + 1], 1)));
+}
+// Queries in bf16 that meet codes become fp16: a row, held by LANES neighbouring threads as 16-byte pieces, is multiplied by
+// the power of two that brings its largest value to 2^14 (what is lost is 2^-38 of that value; an infinity or a NaN stays
+// one).  Returns the power's reciprocal.
+template <int LANES>
+__device__ __forceinline__ float row_to_half(uint4& v) {
+  uint32_t* w = reinterpret_cast<uint32_t*>(&v);
+  uint32_t most = 0;  // bits of the largest magnitude
+#pragma unroll
+  for (int i = 0; i < 4; ++i) most = max(most, max((w[i] & 0x7fffu) << 16, w[i] & 0x7fff0000u));
+#pragma unroll
+  for (int off = 1; off < LANES; off <<= 1) most = max(most, __shfl_xor_sync(0xffffffffu, most, off));
+  const int e = most == 0 ? 14 : min(max(int(most >> 23) - 127, -112), 126);
+  const float up = __uint_as_float(uint32_t(127 + 14 - e) << 23);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 x = Half2<__nv_bfloat16>::unpack(w[i]);
+    w[i] = Half2<__half>::pack(x.x * up, x.y * up);
+  }
+  return __uint_as_float(uint32_t(127 - 14 + e) << 23);
 }
 
 // ---- keys of a paged sequence into tiles, by the 128 threads of a warpgroup ------------------------------------------------
@@ -126,27 +151,24 @@ __device__ __forceinline__ void copy_keys(const PoolView& pool, const KeyRuns& k
     copy16(to + (ROWS > 128 ? (r >> 7) * tile_bytes : 0) + tile_offset(r & 127, piece), pool.rows + line * (D * 2) + piece * 16, there);
   }
 }
-// Codes: 16 of them per load, as 16-bit values; with SCALED times their row's scale.
-template <typename T, int D, int ROWS, bool SCALED>
+// Codes, 16 of them per load, as numbers of type M.
+template <typename M, int D, int ROWS>
 __device__ __forceinline__ void convert_keys(const PoolView& pool, const KeyRuns& k, int head, uint32_t to, int tile_bytes, int thread) {
   constexpr int PIECES = D / 16, EACH = 128 / PIECES, BATCH = 4;
   const int piece = thread % PIECES;
 #pragma unroll 1
   for (int r0 = thread / PIECES; r0 < ROWS; r0 += BATCH * EACH) {
     uint4 codes[BATCH];
-    float scale[BATCH];
 #pragma unroll
     for (int n = 0; n < BATCH; ++n) {
       const int r = r0 + n * EACH, key = k.key0 + r, page = __shfl_sync(0xffffffffu, k.id, r >> 4);
       const bool there = page >= 0 && key >= k.low && key < k.length;
-      const int64_t line = there ? pool.line(page, head, key) : 0;
-      codes[n] = there ? *reinterpret_cast<const uint4*>(pool.rows + line * D + piece * 16) : make_uint4(0, 0, 0, 0);
-      scale[n] = !SCALED ? 1.0f : there ? pool.scales[line] : 0.f;
+      codes[n] = there ? *reinterpret_cast<const uint4*>(pool.rows + pool.line(page, head, key) * D + piece * 16) : make_uint4(0, 0, 0, 0);
     }
 #pragma unroll
     for (int n = 0; n < BATCH; ++n) {
       const int r = r0 + n * EACH;
-      store_codes<T>(to + (ROWS > 128 ? (r >> 7) * tile_bytes : 0), r & 127, piece, codes[n], scale[n]);
+      store_codes<M>(to + (ROWS > 128 ? (r >> 7) * tile_bytes : 0), r & 127, piece, codes[n]);
     }
   }
 }

@@ -133,7 +133,7 @@ __device__ __forceinline__ void fetch_keys(const WeighArgs& a, Pieces pieces, Ba
     }
     const uint32_t to = keys + kb.stage * C::KEYS;
     // codes as they are: a key's scale multiplies its scores in 32 bits
-    if constexpr (C::INT8) convert_keys<typename C::T, C::D, kBlockKeys, false>(a.keys, runs, at.head, to, C::GROUP, p);
+    if constexpr (C::INT8) convert_keys<typename C::T, C::D, kBlockKeys>(a.keys, runs, at.head, to, C::GROUP, p);
     else copy_keys<C::D, kBlockKeys>(a.keys, runs, at.head, to, C::GROUP, p);
     if (C::INT8) {
       fence_async_smem();

@@ -107,18 +107,16 @@ def attention(batch, *, scale=None, causal=True, window=None):
 def assert_attention(batch, out, lse, **options):
     """Errors counted: scores are sums of head_dim products in 32 bits whose terms add up to ``size`` at most
     (2^-23 of it for each addition, and 2^-20 for the exponent's own scaling and exponential), which moves a probability
-    by that relative amount, twice with the denominator; a probability is rounded once (half a step of its type); over a
-    cache of codes keys and values may be rounded to the queries' type too: half a step each, so a score moves by at most
-    sum |q| |k| half = half * ``size``; the output is rounded once."""
+    by that relative amount, twice with the denominator; a probability is rounded once (half a step of its type; over a
+    cache of codes that is fp16); the output is rounded once.  Codes themselves are exact."""
     want, want_lse, spread, size = attention(batch, **options)
     half = torch.finfo(out.dtype).eps / 2
-    part = torch.finfo(torch.bfloat16).eps / 2 if batch.cache.quantized else half
-    rounded_keys = half if batch.cache.quantized else 0.0
-    score = size * (out.shape[-1] * 2.0 ** -23 + rounded_keys) + 2.0 ** -20 * (1 + size)
+    part = torch.finfo(torch.float16).eps / 2 if batch.cache.quantized else half
+    score = size * out.shape[-1] * 2.0 ** -23 + 2.0 ** -20 * (1 + size)
     assert torch.equal(torch.isneginf(lse.double()), torch.isneginf(want_lse))
     visible = ~torch.isneginf(want_lse)
     assert ((lse.double() - want_lse).abs()[visible] <= (score + 2.0 ** -22 * (1 + want_lse.abs()))[visible]).all()
-    bound = half * want.abs() + spread * (part + (half if batch.cache.quantized else 0.0) + 2.1 * score[..., None]) + torch.finfo(out.dtype).tiny
+    bound = half * want.abs() + spread * (part + 2.1 * score[..., None]) + torch.finfo(out.dtype).tiny
     error = (out.double() - want).abs()
     assert (error <= bound).all(), f"{float((error / bound.clamp_min(1e-300)).max()):.2f} of the bound"
     assert (out[~visible] == 0).all()

@@ -345,6 +345,34 @@ def test_attention_of_offsets_past_32_bits():
         U.assert_attention(b, out, lse)
 
 
+@pytest.mark.parametrize("chunk", [1, 50])
+def test_attention_over_codes_of_any_scale(chunk):
+    """Scales of values that differ by 2^60 or more within a sequence, zeros among them: what is rounded is relative to the
+    largest contribution, and the sums hold."""
+    b = U.batch_of([300], [chunk], q_heads=4, kv_heads=2, head_dim=128, page=16, quantized=True, seed=4)
+    used = b.table[0].long()
+    g = torch.Generator("cuda").manual_seed(0)
+    scales = torch.pow(2.0, torch.randint(-30, 31, b.cache.value_scales[used].shape, device="cuda", generator=g).float())
+    scales[0, :, 3:9] = 0
+    if chunk > 1:  # there what is rounded is relative to the largest scale of a tile: below 2^-14 of it steps are 2^-24 of it
+        scales = scales.clamp(2.0 ** -6, 2.0 ** 6)
+    b.cache.value_scales[used] = scales
+    out, lse = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets, return_lse=True)
+    U.assert_attention(b, out, lse)
+
+
+@pytest.mark.parametrize("chunk", [1, 18])
+def test_values_that_are_not_finite_leave_lse_and_other_heads(chunk):
+    b = U.batch_of([40], [chunk], q_heads=4, kv_heads=2, head_dim=64, page=16, quantized=True)
+    want, lse = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets, return_lse=True)
+    for bad in (math.inf, math.nan):
+        b.cache.value_scales[b.table[0, 1].long(), 0, 5] = bad
+        out, same = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets, return_lse=True)
+        assert not torch.isfinite(out[:, :2]).any() and torch.equal(out[:, 2:], want[:, 2:])
+        # the sum of two numbers of up to 16 each, one of them a logarithm of 32 bits
+        assert ((same - lse).abs() <= 3 * 2.0 ** -23 * 16).all()
+
+
 # ---- key weights ------------------------------------------------------------------------------------------------
 def assert_weights(b, got, lse, previous=None, **options):
     """An exponent is off by the score's error (see assert_attention) and lse's, whose rounding is the input's own; a sum of

@@ -75,6 +75,8 @@ def test_rotation_refusals():
         rotate(x(2, 3, 8), ints(2), table, out=x(2, 3, 9))
     with pytest.raises(TypeError, match="out"):
         rotate(x(2, 3, 8), ints(2), table, out=x(2, 3, 8, dtype=torch.float16))
+    with pytest.raises(ValueError, match="expanded"):
+        rotate(x(2, 3, 8), ints(2), table, out=x(2, 1, 8).expand(2, 3, 8))
     with pytest.raises(ValueError, match="gradient"):
         rotate(x(2, 3, 8, dtype=torch.float32).requires_grad_(), ints(2), table, out=x(2, 3, 8, dtype=torch.float32))
     with pytest.raises(ValueError, match="CUDA device"):
@@ -139,6 +141,7 @@ def test_attention_refusals(cache):
     refuses(ValueError, attend, x(3, 4, 64), cache, *step, out=x(3, 4, 32), match="out")
     refuses(TypeError, attend, x(3, 4, 64), cache, *step, out=x(3, 4, 64, dtype=torch.float16), match="out")
     refuses(ValueError, attend, x(3, 4, 64), cache, *step, out=x(3, 4, 65)[..., 1:], match="out")
+    refuses(ValueError, attend, x(3, 4, 64), cache, *step, out=x(1, 4, 64).expand(3, 4, 64), match="expanded")
 
 
 def test_append_refusals(cache):
