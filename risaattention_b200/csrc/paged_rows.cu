@@ -1,4 +1,4 @@
-// Attention of few query rows over a paged cache (single tokens, short chunks), the join of its partial
+// Attention of few query rows over a paged cache (single tokens, chunks of few tokens), the join of its partial
 // results, and the attention weight that cached keys receive from few rows.
 //
 // What bounds it is reading the cache once: 2 * keys * head_dim values per key head for a handful of
@@ -723,9 +723,8 @@ using namespace risa_b200;
 using namespace risa_b200::serving;
 
 // Whether a step can hold sequences for the tensor-core kernel.
-static bool takes_tensor_cores(const risa_b200_cache& cache, const risa_b200_step& step, int group) {
-  const int64_t most = step.query_offsets == nullptr ? group : int64_t(step.tokens) * group;
-  return cache.head_dim <= 128 && most >= kTcFewestRows;
+static bool takes_tensor_cores(const risa_b200_step& step, int group) {
+  return (step.query_offsets == nullptr ? group : int64_t(step.tokens) * group) >= kTcFewestRows;
 }
 static size_t rows_scratch(const risa_b200_cache& cache, const risa_b200_step& step, int group) {
   return size_t(kMaxWorkers) * (2 * slot_floats(8 * column_blocks_of(step, group), cache.head_dim) * sizeof(float) + sizeof(JoinNote));
@@ -735,7 +734,7 @@ extern "C" size_t risa_b200_paged_attention_scratch_size(const risa_b200_cache* 
   if (cache == nullptr || step == nullptr || cache->kv_heads <= 0 || q_heads <= 0) return 0;
   const int group = q_heads / cache->kv_heads;
   size_t bytes = rows_scratch(*cache, *step, group);
-  if (takes_tensor_cores(*cache, *step, group)) bytes += paged_tc_scratch(cache->head_dim);
+  if (takes_tensor_cores(*step, group)) bytes += paged_tc_scratch(cache->head_dim);
   return bytes;
 }
 
@@ -760,7 +759,7 @@ extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const ris
   a.parts = static_cast<float*>(scratch);
   a.notes = reinterpret_cast<JoinNote*>(a.parts + size_t(kMaxWorkers) * 2 * slot_floats(a.line.rows, cache->head_dim));
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  const bool tensor_cores = takes_tensor_cores(*cache, *step, a.line.group);
+  const bool tensor_cores = takes_tensor_cores(*step, a.line.group);
   if (tensor_cores) a.line.max_rows = kTcFewestRows - 1;
   const bool codes = cache->dtype_code == kInt8;
   int bad = with_tile(dtype_code, codes, cache->head_dim, a.line.rows / 8, [&](auto tile) {
@@ -789,13 +788,9 @@ extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const ris
   return bad ? bad : check_launch("paged attention");
 }
 
-static bool weighs_on_tensor_cores(const risa_b200_step& step, int group) {
-  return (step.query_offsets == nullptr ? group : int64_t(step.tokens) * group) >= kTcFewestRows;
-}
-
 extern "C" size_t risa_b200_key_weights_scratch_size(const risa_b200_cache* cache, const risa_b200_step* step, int q_heads) {
   if (cache == nullptr || step == nullptr || cache->kv_heads <= 0 || q_heads <= 0) return 0;
-  return weighs_on_tensor_cores(*step, q_heads / cache->kv_heads) ? weigh_tc_scratch() : 0;
+  return takes_tensor_cores(*step, q_heads / cache->kv_heads) ? weigh_tc_scratch() : 0;
 }
 
 extern "C" int risa_b200_key_weights(const risa_b200_cache* cache, const risa_b200_step* step, const void* q,
@@ -809,7 +804,7 @@ extern "C" int risa_b200_key_weights(const risa_b200_cache* cache, const risa_b2
   RowsArgs a = rows_args(cache, step, q, q_strides, q_heads, scale, is_causal, window, status);
   const int column_blocks = a.line.rows / 8;
   a.line.rows = Divisor(1 << 30);  // all rows of a key head are one unit
-  const bool tensor_cores = weighs_on_tensor_cores(*step, a.line.group);
+  const bool tensor_cores = takes_tensor_cores(*step, a.line.group);
   RISA_REQUIRE(!tensor_cores || (scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 16 == 0 && scratch_bytes >= weigh_tc_scratch()),
                "key weights: the scratch is too small");
   if (tensor_cores) a.line.max_rows = kTcFewestRows - 1;

@@ -12,12 +12,18 @@
 // 1024, and what one group's products and the other's softmax do not hide of each other is the chain of both.  With one
 // thread for a row the chain was 2080 (softmax) + 1630 clocks and a tile of both groups took 3710.
 //
+// Heads of 256 channels leave room for the outputs of 128 rows only.  There the two groups have the same rows and half of
+// the channels of V each, over tiles of 64 keys; the scores are computed twice (3 products for 2) in exchange for the same
+// taking of turns.
+//
 // Warps 0-15: softmax, query loads and epilogue, four for each half of the columns of each row group.  16-19: fetch K
 // and V tiles from the pages (cp.async, or codes converted on the way) into the 128-byte-swizzled layout of the matrix
 // instructions.  20: issues them (and owns tensor memory).  21-23 idle, so that registers can be dealt per warpgroup.
 #include "serving_plan.cuh"
 #include "paged_tc.cuh"
 #include "tc_f16.cuh"
+
+#include <algorithm>
 
 namespace risa_b200 {
 namespace serving {
@@ -27,7 +33,7 @@ using namespace tc;
 namespace {
 
 constexpr int kThreads = 768;
-constexpr int kTileKeys = 128, kGroups = 2, kRows = 128 * kGroups;
+constexpr int kGroups = 2;
 constexpr int kProducer = 16, kIssuer = 20;  // first warps of their roles
 // 768 threads of at most 85 registers are launched with 80; the softmax warps hold 64 scores of a row.
 constexpr int kRegsLaunch = 80, kRegsSoftmax = 96, kRegsProducer = 56, kRegsIssuer = 40;
@@ -46,15 +52,20 @@ struct Shape {
   using M = std::conditional_t<INT8_, __half, T_>;  // type of the matrix instructions' operands
   static constexpr bool INT8 = INT8_;
   static constexpr int D = D_;
-  static constexpr int SIDE = kTileKeys * D * 2;  // a K or V tile as the matrix instructions read it
-  static constexpr int STAGES = D == 128 ? 2 : 4;
-  static constexpr int Q = kGroups * SIDE;
+  static constexpr bool SHARED = D == 256;             // both groups have the same rows
+  static constexpr int KEYS = SHARED ? 64 : 128;       // of a tile
+  static constexpr int ROWS = SHARED ? 128 : 256;      // of a unit
+  static constexpr int OUT = SHARED ? D / 2 : D;       // channels of a group's output
+  static constexpr int SIDE = KEYS * D * 2;            // a K or V tile as the matrix instructions read it
+  static constexpr int BLOCK = KEYS * 128;             // 64 channels of it
+  static constexpr int STAGES = D == 64 ? 4 : 2;
+  static constexpr int QUERIES = 128 * D * 2, Q = (SHARED ? 1 : kGroups) * QUERIES;
   static constexpr int SMEM = Q + 2 * STAGES * SIDE + 1024;  // + alignment
 };
 
 struct Barriers {
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
-  uint64_t q_full[kGroups], s_full[kGroups], p_full[kGroups], o_full[kGroups], o_free[kGroups], drained;
+  uint64_t q_full[kGroups], s_full[kGroups], p_full[kGroups], o_full[kGroups], o_free[kGroups], q_empty, drained;
 };
 // What the two threads of a row tell each other: maxima (of tiles in turn) and sums.
 struct Exchange {
@@ -66,7 +77,7 @@ struct Exchange {
 // queries' rows were divided by, of this unit and the one before.
 constexpr int kScaleDepth = 8;
 struct Scales {
-  float key[kScaleDepth][kTileKeys], value[kScaleDepth][kTileKeys], lift[kScaleDepth][4];
+  float key[kScaleDepth][128], value[kScaleDepth][128], lift[kScaleDepth][4];
   float row[2][kGroups][128];
 };
 
@@ -86,13 +97,13 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
     const int32_t* row = a.line.step.table + int64_t(piece.sequence) * a.line.step.width;
     const int length = piece.seq.length;
     const int low = a.line.window > 0 ? visible(piece.seq.length - piece.seq.count, length, true, a.line.window).lo : 0;
-    const uint32_t two = piece.seq.count * a.line.group - piece.block * kRows > 128 ? kTwoGroups : 0u;
+    const uint32_t two = C::SHARED || piece.seq.count * a.line.group - piece.block * C::ROWS > 128 ? kTwoGroups : 0u;
     KeyRuns ahead;
-    ahead.look_up(row, a.line.step.page_shift, a.pages, 8, piece.first * kTileKeys, low, length);
+    ahead.look_up(row, a.line.step.page_shift, a.pages, C::KEYS / 16, piece.first * C::KEYS, low, length);
 #pragma unroll 1
     for (int i = 0; i < piece.count; ++i) {
       const KeyRuns runs = ahead;
-      if (i + 1 < piece.count) ahead.look_up(row, a.line.step.page_shift, a.pages, 8, runs.key0 + kTileKeys, low, length);
+      if (i + 1 < piece.count) ahead.look_up(row, a.line.step.page_shift, a.pages, C::KEYS / 16, runs.key0 + C::KEYS, low, length);
 #pragma unroll 1
       for (int side = 0; side < 2; ++side) {  // K, then V
         uint64_t* full = side ? bars->v_full : bars->k_full;
@@ -121,22 +132,24 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
             for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
             if ((p & 31) == 0) scales->lift[slot][p >> 5] = lg2_approx(most);
           }
-          convert_keys<__half, C::D, kTileKeys>(side ? values : keys, runs, piece.head, to, 0, p);
+          convert_keys<__half, C::D, C::KEYS>(side ? values : keys, runs, piece.head, to, 0, p);
           fence_async_smem();
           mbar_arrive(smem_u32(full + stage.stage));
-        } else if (runs.bad == 0 && runs.key0 >= low && runs.key0 + kTileKeys <= length) {
+        } else if (runs.bad == 0 && runs.key0 >= low && runs.key0 + C::KEYS <= length) {
           const uint32_t bar = smem_u32(full + stage.stage);
-          const int shift = a.line.step.page_shift, page = __shfl_sync(0xffffffffu, runs.id, (p << (shift - 4)) & 31);
+          // boxes of a page's rows, or of the tile's where a page is larger
+          const int shift = min(a.line.step.page_shift, C::KEYS == 64 ? 6 : 7), page = __shfl_sync(0xffffffffu, runs.id, (p << (shift - 4)) & 31);
+          const int in_page = runs.key0 & ((1 << a.line.step.page_shift) - 1) & ~((1 << shift) - 1);
           if (p == 0) mbar_expect_tx(bar, C::SIDE);
           else mbar_arrive(bar);
           __syncwarp();
-          if (p < kTileKeys >> shift) {
+          if (p < C::KEYS >> shift) {
 #pragma unroll
             for (int c = 0; c < C::D; c += 64)
-              tma_load_3d(to + (c >> 6) * 16384 + (p << shift) * 128, side ? value_map : key_map, bar, c, 0, page * a.line.kv_heads + piece.head);
+              tma_load_3d(to + (c >> 6) * C::BLOCK + (p << shift) * 128, side ? value_map : key_map, bar, c, in_page, page * a.line.kv_heads + piece.head);
           }
         } else {
-          copy_keys<C::D, kTileKeys>(side ? values : keys, runs, piece.head, to, 0, p);
+          copy_keys<C::D, C::KEYS>(side ? values : keys, runs, piece.head, to, 0, p);
           copies_drain();
           fence_async_smem();
           mbar_arrive(smem_u32(full + stage.stage));
@@ -162,18 +175,16 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
 template <typename C>
 __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const volatile uint32_t* notes, uint32_t tmem, uint32_t q, uint32_t k_ring,
                                                uint32_t v_ring, uint32_t gave_up) {
-  constexpr uint32_t kScores = idesc_f16<typename C::M>(false, kTileKeys), kOutput = idesc_f16<typename C::M>(true, C::D);
+  constexpr uint32_t kScores = idesc_f16<typename C::M>(false, C::KEYS), kOutput = idesc_f16<typename C::M>(true, C::OUT);
   RingPos<C::STAGES> k, v;
   uint32_t q_phase = 0, p_phase = 0, o_phase = 3;  // a bit per group
   const bool elected = elect_one();
   auto scores = [&](int g) {
     if (!elected) return;
-    const uint32_t rows_q = along_row(q + g * C::SIDE), rows_k = along_row(k_ring + k.stage * C::SIDE), to = tmem + g * kTileKeys;
+    const uint32_t rows_q = along_row(q + (C::SHARED ? 0 : g * C::QUERIES)), rows_k = along_row(k_ring + k.stage * C::SIDE), to = tmem + g * C::KEYS;
 #pragma unroll 2
-    for (int c = 0; c < C::D / 16; ++c) {
-      const uint32_t at = (c >> 2) * 1024 + (c & 3) * 2;
-      mma_f16(to, descriptor(rows_q + at), descriptor(rows_k + at), kScores, c > 0);
-    }
+    for (int c = 0; c < C::D / 16; ++c)
+      mma_f16(to, descriptor(rows_q + (c >> 2) * 1024 + (c & 3) * 2), descriptor(rows_k + (c >> 2) * (C::BLOCK >> 4) + (c & 3) * 2), kScores, c > 0);
     mma_commit(smem_u32(bars->s_full + g));
   };
   for (int tile = 0; tile < tiles; ++tile) {
@@ -182,8 +193,11 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
     const bool first = note & kFirst, last = note & kLast;
     const int groups = note & kTwoGroups ? 2 : 1;
     if (first) {
+      if (C::SHARED)
+        for (int g = 0; g < 2; ++g)
+          if (!mbar_wait(smem_u32(bars->q_full + g), q_phase >> g & 1, gave_up, 1011)) return;
       for (int g = 0; g < groups; ++g) {
-        if (!mbar_wait(smem_u32(bars->q_full + g), q_phase >> g & 1, gave_up, 1011)) return;
+        if (!C::SHARED && !mbar_wait(smem_u32(bars->q_full + g), q_phase >> g & 1, gave_up, 1011)) return;
         q_phase ^= 1u << g;
         tc_fence_after();
         scores(g);
@@ -191,6 +205,7 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
       if (elected) mma_commit(smem_u32(bars->k_empty + k.stage));
       k.next();
     }
+    if (C::SHARED && last && elected) mma_commit(smem_u32(&bars->q_empty));  // both groups' last scores are issued
     for (int g = 0; g < groups; ++g) {
       if (g == 0 && !mbar_wait(smem_u32(bars->v_full + v.stage), v.phase, gave_up, 1012)) return;
       if (first) {  // the previous unit's output has been read
@@ -201,10 +216,10 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
       p_phase ^= 1u << g;
       tc_fence_after();
       if (elected) {
-        const uint32_t rows_v = across_rows(v_ring + v.stage * C::SIDE);
+        const uint32_t rows_v = across_rows<C::KEYS>(v_ring + v.stage * C::SIDE + (C::SHARED ? g * 2 * C::BLOCK : 0));
 #pragma unroll 2
-        for (int c = 0; c < kTileKeys / 16; ++c)
-          mma_f16_tmem(tmem + kGroups * kTileKeys + g * C::D, tmem + g * kTileKeys + c * 8, descriptor(rows_v + c * 128), kOutput, c > 0 || !first);
+        for (int c = 0; c < C::KEYS / 16; ++c)
+          mma_f16_tmem(tmem + kGroups * C::KEYS + g * C::OUT, tmem + g * C::KEYS + c * 8, descriptor(rows_v + c * 128), kOutput, c > 0 || !first);
         if (last) mma_commit(smem_u32(bars->o_full + g));
         if (g == groups - 1) mma_commit(smem_u32(bars->v_empty + v.stage));
       }
@@ -228,16 +243,18 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
 __device__ __forceinline__ void meet(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 __device__ __forceinline__ void leave(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
 
-// Query rows of group g, by the 256 threads of its two warpgroups: 16-byte pieces, neighbouring threads along a row.  A
+// Query rows of group g (half of the rows that both groups share), by the 256 threads of its two warpgroups: 16-byte pieces,
+// neighbouring threads along a row.  A
 // negative scale flips their signs, so that the maximum of the scores is the maximum of the scaled ones.
 template <typename C>
 __device__ __forceinline__ void load_query_rows(const TcArgs& a, const Piece& piece, int g, uint32_t to, float* row_scale) {
   constexpr int PIECES = C::D / 8, EACH = 256 / PIECES;
   const int t = threadIdx.x & 255, rows = piece.seq.count * a.line.group, c = t % PIECES;
   const uint32_t flip = a.scale_log2 < 0.f ? 0x80008000u : 0u;
+  const int first = C::SHARED ? g * 64 : 0, end = C::SHARED ? first + 64 : 128;
 #pragma unroll 4
-  for (int r = t / PIECES; r < 128; r += EACH) {
-    const int row = piece.block * kRows + g * 128 + r;
+  for (int r = first + t / PIECES; r < end; r += EACH) {
+    const int row = piece.block * C::ROWS + (C::SHARED ? 0 : g * 128) + r;
     uint4 v = make_uint4(0, 0, 0, 0);
     if (row < rows) {
       const int token = row / a.line.group, h = row - token * a.line.group;
@@ -260,19 +277,20 @@ __device__ __forceinline__ void load_query_rows(const TcArgs& a, const Piece& pi
 template <typename C>
 __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Barriers* bars, Exchange* exchange, Scales* scales, uint32_t tmem, uint32_t q, int g, int half,
                                              const volatile uint32_t* notes, uint32_t gave_up) {
-  constexpr int D = C::D, KEYS = kTileKeys / 2;
+  constexpr int D = C::D, KEYS = C::KEYS / 2, OUT = C::OUT;
   using T = typename C::T;
   const int r = threadIdx.x & 127, meeting = 1 + g * 4 + (r >> 5);
   const uint32_t lanes = tmem + (uint32_t(r & ~31) << 16);
-  const uint32_t s_columns = lanes + g * kTileKeys, o_columns = lanes + kGroups * kTileKeys + g * D + half * (D / 2);
+  const uint32_t s_columns = lanes + g * C::KEYS, o_columns = lanes + kGroups * C::KEYS + g * OUT + half * (OUT / 2);
+  const int group_row = C::SHARED ? 0 : g * 128;  // of the group's first row in the unit
   const float call_scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // a scale of 0 must leave hidden scores at -inf
-  uint32_t s_phase = 0, o_phase = 0, tile = 0, turn = 0;
+  uint32_t s_phase = 0, o_phase = 0, q_phase = 0, tile = 0, turn = 0;
   Piece piece;
   bool more = pieces.next(a.line, piece);
-  auto mine = [&](const Piece& p) { return p.seq.count * a.line.group - p.block * kRows > g * 128; };
+  auto mine = [&](const Piece& p) { return p.seq.count * a.line.group - p.block * C::ROWS > group_row; };
   auto fetch = [&](const Piece& p) {
     turn ^= 1;
-    load_query_rows<C>(a, p, g, q + g * C::SIDE, C::INT8 ? scales->row[turn][g] : nullptr);
+    load_query_rows<C>(a, p, g, q + (C::SHARED ? 0 : g * C::QUERIES), C::INT8 ? scales->row[turn][C::SHARED ? 0 : g] : nullptr);
     mbar_arrive_warp(smem_u32(bars->q_full + g));
   };
   if (more && mine(piece)) fetch(piece);
@@ -283,30 +301,30 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
       if (more && mine(piece)) fetch(piece);
       continue;
     }
-    const int rows = piece.seq.count * a.line.group, row = piece.block * kRows + g * 128 + r;
+    const int rows = piece.seq.count * a.line.group, row = piece.block * C::ROWS + group_row + r;
     KeyRange seen = visible(piece.seq.length - piece.seq.count + row / a.line.group, piece.seq.length, a.line.causal, a.line.window);
     if (row >= rows) seen = {0, 0};
     // keys that every row of the group sees need no test
-    const int token0 = (piece.block * kRows + g * 128) / a.line.group, token1 = (min(piece.block * kRows + g * 128 + 128, rows) - 1) / a.line.group;
+    const int row0 = piece.block * C::ROWS + group_row, token0 = row0 / a.line.group, token1 = (min(row0 + 128, rows) - 1) / a.line.group;
     const int all_hi = visible(piece.seq.length - piece.seq.count + token0, piece.seq.length, a.line.causal, a.line.window).hi;
     const int all_lo = visible(piece.seq.length - piece.seq.count + token1, piece.seq.length, a.line.causal, a.line.window).lo;
     float m = kNoMaximum, l = 0.f, scale = call_scale;
     const uint32_t mine_turn = turn;
 #pragma unroll 1
     for (int i = 0; i < piece.count; ++i, ++tile) {
-      const int key0 = (piece.first + i) * kTileKeys + half * KEYS;
+      const int key0 = (piece.first + i) * C::KEYS + half * KEYS;
       if (!mbar_wait(smem_u32(bars->s_full + g), s_phase, gave_up, 1020 + g)) return leave(meeting);
       s_phase ^= 1;
       tc_fence_after();
       uint32_t x[KEYS];
-      tmem_load32(s_columns + half * KEYS, x);
-      tmem_load32(s_columns + half * KEYS + 32, x + 32);
-      const uint32_t gone = notes[tile % kNotes] >> (half * 4) & (kHiddenRuns >> 4);
+#pragma unroll
+      for (int c = 0; c < KEYS; c += 32) tmem_load32(s_columns + half * KEYS + c, x + c);
+      const uint32_t gone = notes[tile % kNotes] >> (half * (KEYS / 16)) & ((1u << (KEYS / 16)) - 1);
       tmem_load_wait();
       tmem_regs_ready<KEYS>(x);
       const int slot_of_tile = tile % kScaleDepth;
       if constexpr (C::INT8) {
-        if (std::is_same<T, __nv_bfloat16>::value && i == 0) scale = call_scale * scales->row[mine_turn][g][r];
+        if (std::is_same<T, __nv_bfloat16>::value && i == 0) scale = call_scale * scales->row[mine_turn][C::SHARED ? 0 : g][r];
         const ulonglong2* k = reinterpret_cast<const ulonglong2*>(scales->key[slot_of_tile] + half * KEYS);
 #pragma unroll
         for (int c = 0; c < KEYS; c += 4) {
@@ -349,7 +367,7 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
         l *= keep;
         if (i > 0) {  // scores of this tile were issued behind the product with the last one, so that is complete
 #pragma unroll 1
-          for (int c = 0; c < D / 2; c += 16) {
+          for (int c = 0; c < OUT / 2; c += 16) {
             uint32_t o[16];
             tmem_load16(o_columns + c, o);
             tmem_load_wait();
@@ -392,6 +410,10 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
     // the last scores are here, so the queries have been read
     const Piece done = piece;
     more = pieces.next(a.line, piece);
+    if (C::SHARED) {  // and by the other group
+      if (!mbar_wait(smem_u32(&bars->q_empty), q_phase, gave_up, 1024 + g)) return leave(meeting);
+      q_phase ^= 1;
+    }
     if (more && mine(piece)) fetch(piece);
     exchange->sum[g][half][r] = l;
     meet(meeting);
@@ -402,11 +424,11 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
     const bool there = row < rows;
     const int token = row / a.line.group, h = done.head * a.line.group + row - token * a.line.group;
     const float f = l == 0.f ? 0.f : 1.0f / l;
-    T* out = static_cast<T*>(a.out) + int64_t(done.seq.first + token) * a.on + int64_t(h) * a.oh + half * (D / 2);
-    float* slot = a.parts + (int64_t(blockIdx.x) * 2 + (done.opens ? 1 : 0)) * slot_floats(kRows, D);
-    const int in_block = g * 128 + r;
+    const int channel0 = (C::SHARED ? g * OUT : 0) + half * (OUT / 2), in_block = group_row + r;
+    T* out = static_cast<T*>(a.out) + int64_t(done.seq.first + token) * a.on + int64_t(h) * a.oh + channel0;
+    float* slot = a.parts + (int64_t(blockIdx.x) * 2 + (done.opens ? 1 : 0)) * slot_floats(C::ROWS, D);
 #pragma unroll 1
-    for (int c = 0; c < D / 2; c += 16) {
+    for (int c = 0; c < OUT / 2; c += 16) {
       uint32_t o[16];
       tmem_load16(o_columns + c, o);
       tmem_load_wait();
@@ -425,13 +447,13 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
       } else {
 #pragma unroll
         for (int e = 0; e < 16; e += 4)
-          *reinterpret_cast<uint4*>(slot + int64_t(in_block) * D + half * (D / 2) + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
+          *reinterpret_cast<uint4*>(slot + int64_t(in_block) * D + channel0 + c + e) = make_uint4(o[e], o[e + 1], o[e + 2], o[e + 3]);
       }
     }
-    if (half == 0 && there) {
+    if (half == 0 && there && (!C::SHARED || g == 0)) {
       if (!done.whole) {
-        slot[kRows * D + in_block] = m;
-        slot[kRows * D + kRows + in_block] = l;
+        slot[C::ROWS * D + in_block] = m;
+        slot[C::ROWS * D + C::ROWS + in_block] = l;
       } else if (a.lse != nullptr) {
         a.lse[int64_t(done.seq.first + token) * (a.line.kv_heads * a.line.group) + h] = l == 0.f ? -INFINITY : m * kLn2 + logf(l);
       }
@@ -469,6 +491,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
       mbar_init(smem_u32(bars.o_full + g), 1);
       mbar_init(smem_u32(bars.o_free + g), 8);
     }
+    mbar_init(smem_u32(&bars.q_empty), 1);
     mbar_init(smem_u32(&bars.drained), 1);
     mbar_init_fence();
   }
@@ -516,20 +539,20 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
   __syncthreads();
   tc_fence_after();
   if (warp == kIssuer) tmem_dealloc(tmem, 512);
-  if (gave_up_word != 0 && threadIdx.x < kRows) {
+  if (gave_up_word != 0 && threadIdx.x < C::ROWS) {
     // a wait ran out: the rows of this worker's whole units are marked, parts poison their join
     Pieces all = pieces;
     Piece piece;
     while (all.next(a.line, piece)) {
-      const int rows = piece.seq.count * a.line.group, row = piece.block * kRows + threadIdx.x;
+      const int rows = piece.seq.count * a.line.group, row = piece.block * C::ROWS + threadIdx.x;
       if (piece.whole) {
         if (row >= rows) continue;
         const int token = row / a.line.group, h = piece.head * a.line.group + row % a.line.group;
         typename C::T* out = static_cast<typename C::T*>(a.out) + int64_t(piece.seq.first + token) * a.on + int64_t(h) * a.oh;
         for (int c = 0; c < C::D; ++c) out[c] = static_cast<typename C::T>(NAN);
       } else {
-        float* slot = a.parts + (int64_t(blockIdx.x) * 2 + (piece.opens ? 1 : 0)) * slot_floats(kRows, C::D);
-        slot[kRows * C::D + kRows + threadIdx.x] = NAN;
+        float* slot = a.parts + (int64_t(blockIdx.x) * 2 + (piece.opens ? 1 : 0)) * slot_floats(C::ROWS, C::D);
+        slot[C::ROWS * C::D + C::ROWS + threadIdx.x] = NAN;
       }
     }
   }
@@ -552,7 +575,7 @@ template <typename C>
 bool pool_map(CUtensorMap* map, const char* pool, const TcArgs& a) {
   const cuuint64_t dims[3] = {cuuint64_t(C::D), cuuint64_t(1) << a.line.step.page_shift, cuuint64_t(a.pages) * a.line.kv_heads};
   const cuuint64_t strides[2] = {cuuint64_t(C::D) * 2, (cuuint64_t(C::D) * 2) << a.line.step.page_shift};
-  const cuuint32_t box[3] = {64, 1u << a.line.step.page_shift, 1}, ones[3] = {1, 1, 1};
+  const cuuint32_t box[3] = {64, std::min(1u << a.line.step.page_shift, cuuint32_t(C::KEYS)), 1}, ones[3] = {1, 1, 1};
   return encode_fn()(map, std::is_same<typename C::T, __half>::value ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3,
                      const_cast<char*>(pool), dims, strides, box, ones, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
                      CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -560,6 +583,7 @@ bool pool_map(CUtensorMap* map, const char* pool, const TcArgs& a) {
 
 template <typename T, int D>
 int join(const TcArgs& a, cudaStream_t stream) {
+  constexpr int kRows = Shape<T, false, D>::ROWS;
   const JoinArgs join{a.parts, a.notes, kRows, a.line.group, a.line.kv_heads * a.line.group, a.out, a.on, a.oh, a.lse};
   launch_chained(join_parts_kernel<T, D, false>, dim3(kTcWorkers - 1, kRows / 16), dim3(128), 0, stream, join);
   return RISA_B200_OK;
@@ -586,24 +610,34 @@ int launch(const TcArgs& a, cudaStream_t stream) {
 
 }  // namespace
 
-size_t paged_tc_scratch(int head_dim) { return size_t(kTcWorkers) * (2 * slot_floats(kRows, head_dim) * sizeof(float) + sizeof(JoinNote)); }
+namespace {
+int rows_of_unit(int head_dim) { return head_dim == 256 ? Shape<__half, false, 256>::ROWS : Shape<__half, false, 128>::ROWS; }
+template <typename T>
+int launch_for(const TcArgs& a, bool codes, int head_dim, cudaStream_t stream) {
+  if (head_dim == 64) return codes ? launch<Shape<T, true, 64>>(a, stream) : launch<Shape<T, false, 64>>(a, stream);
+  if (head_dim == 128) return codes ? launch<Shape<T, true, 128>>(a, stream) : launch<Shape<T, false, 128>>(a, stream);
+  return codes ? launch<Shape<T, true, 256>>(a, stream) : launch<Shape<T, false, 256>>(a, stream);
+}
+template <typename T>
+int join_for(const TcArgs& a, int head_dim, cudaStream_t stream) {
+  return head_dim == 64 ? join<T, 64>(a, stream) : head_dim == 128 ? join<T, 128>(a, stream) : join<T, 256>(a, stream);
+}
+}  // namespace
 
+size_t paged_tc_scratch(int head_dim) {
+  return size_t(kTcWorkers) * (2 * slot_floats(rows_of_unit(head_dim), head_dim) * sizeof(float) + sizeof(JoinNote));
+}
 TcArgs paged_tc_args(TcArgs a, int head_dim) {
-  a.line.rows = Divisor(kRows);
-  a.line.keys = Divisor(kTileKeys);
-  a.notes = reinterpret_cast<JoinNote*>(a.parts + size_t(kTcWorkers) * 2 * slot_floats(kRows, head_dim));
+  a.line.rows = Divisor(rows_of_unit(head_dim));
+  a.line.keys = Divisor(head_dim == 256 ? Shape<__half, false, 256>::KEYS : Shape<__half, false, 128>::KEYS);
+  a.notes = reinterpret_cast<JoinNote*>(a.parts + size_t(kTcWorkers) * 2 * slot_floats(a.line.rows, head_dim));
   return a;
 }
 int paged_tc(const TcArgs& a, int dtype_code, bool codes, int head_dim, cudaStream_t stream) {
-  if (dtype_code == 1)
-    return head_dim == 64 ? (codes ? launch<Shape<__half, true, 64>>(a, stream) : launch<Shape<__half, false, 64>>(a, stream))
-                          : (codes ? launch<Shape<__half, true, 128>>(a, stream) : launch<Shape<__half, false, 128>>(a, stream));
-  return head_dim == 64 ? (codes ? launch<Shape<__nv_bfloat16, true, 64>>(a, stream) : launch<Shape<__nv_bfloat16, false, 64>>(a, stream))
-                        : (codes ? launch<Shape<__nv_bfloat16, true, 128>>(a, stream) : launch<Shape<__nv_bfloat16, false, 128>>(a, stream));
+  return dtype_code == 1 ? launch_for<__half>(a, codes, head_dim, stream) : launch_for<__nv_bfloat16>(a, codes, head_dim, stream);
 }
 int paged_tc_join(const TcArgs& a, int dtype_code, int head_dim, cudaStream_t stream) {
-  if (dtype_code == 1) return head_dim == 64 ? join<__half, 64>(a, stream) : join<__half, 128>(a, stream);
-  return head_dim == 64 ? join<__nv_bfloat16, 64>(a, stream) : join<__nv_bfloat16, 128>(a, stream);
+  return dtype_code == 1 ? join_for<__half>(a, head_dim, stream) : join_for<__nv_bfloat16>(a, head_dim, stream);
 }
 
 // Site of the first wait of these kernels that ran out since the last call (0: none), or -1 on a CUDA error.

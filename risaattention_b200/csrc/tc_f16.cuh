@@ -16,12 +16,13 @@ template <typename T> __host__ __device__ constexpr uint32_t idesc_f16(bool b_mn
 }
 // Operand descriptors as a constant upper half and a lower half to which offsets (in units of 16 bytes) are added.
 // Rows of 64 channels are 128 bytes wide and swizzled, eight of them 1024 bytes; the next 64 channels are one block of
-// 128 rows further.  Q and K are read with the MMA's K axis along a row (the leading offset is unused), V with it across
+// the tile's rows further.  Q and K are read with the MMA's K axis along a row (the leading offset is unused), V with it across
 // the rows (the leading offset leads to the next 64 channels).
 constexpr uint32_t kDescHigh = (1024 >> 4) | 1u << 14 | 2u << 29;
 __device__ __forceinline__ uint64_t descriptor(uint32_t low) { return uint64_t(kDescHigh) << 32 | low; }
 __device__ __forceinline__ uint32_t along_row(uint32_t address) { return (address & 0x3ffffu) >> 4 | 1u << 16; }
-__device__ __forceinline__ uint32_t across_rows(uint32_t address) { return (address & 0x3ffffu) >> 4 | uint32_t(16384 >> 4) << 16; }
+template <int ROWS>
+__device__ __forceinline__ uint32_t across_rows(uint32_t address) { return (address & 0x3ffffu) >> 4 | uint32_t(ROWS * 128 >> 4) << 16; }
 // One thread issues.
 __device__ __forceinline__ void mma_f16(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, bool accumulate) {
   asm volatile(
@@ -58,9 +59,10 @@ __device__ __forceinline__ void copies_drain() { asm volatile("cp.async.wait_all
 __device__ __forceinline__ void store16(uint32_t to, uint4 v) {
   asm volatile("st.shared.v4.u32 [%0], {%1,%2,%3,%4};" ::"r"(to), "r"(v.x), "r"(v.y), "r"(v.z), "r"(v.w) : "memory");
 }
-// Byte offset of the 16-byte piece `piece` of row `row` in a tile of 128 rows.
+// Byte offset of the 16-byte piece `piece` of row `row` in a tile of ROWS rows: blocks of 64 channels.
+template <int ROWS = 128>
 __device__ __forceinline__ uint32_t tile_offset(int row, int piece) {
-  return uint32_t((piece >> 3) * 16384 + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
+  return uint32_t((piece >> 3) * (ROWS * 128) + row * 128 + (((piece & 7) ^ (row & 7)) << 4));
 }
 
 // Codes are whole numbers of at most 128, exact in both 16-bit types.  Codes 2 i and 2 i + 1 of a word whose sign bits have
@@ -79,12 +81,12 @@ template <> __device__ __forceinline__ uint32_t code_pair<__nv_bfloat16>(uint32_
   return *reinterpret_cast<const uint32_t*>(&d);
 }
 // The 16 codes `w` of a row as numbers of type M: two pieces of its tile.
-template <typename M>
+template <typename M, int ROWS>
 __device__ __forceinline__ void store_codes(uint32_t tile, int row, int piece, uint4 w) {
   const uint32_t u[4] = {w.x ^ 0x80808080u, w.y ^ 0x80808080u, w.z ^ 0x80808080u, w.w ^ 0x80808080u};
 #pragma unroll
   for (int h = 0; h < 2; ++h)
-    store16(tile + tile_offset(row, 2 * piece + h),
+    store16(tile + tile_offset<ROWS>(row, 2 * piece + h),
             make_uint4(code_pair<M>(u[2 * h], 0), code_pair<M>(u[2 * h], 1), code_pair<M>(u[2 * h + 1], 0), code_pair<M>(u[2 * h + 1], 1)));
 }
 // Queries in bf16 that meet codes become fp16: a row, held by LANES neighbouring threads as 16-byte pieces, is multiplied by
@@ -148,7 +150,7 @@ __device__ __forceinline__ void copy_keys(const PoolView& pool, const KeyRuns& k
     const int key = k.key0 + r, page = __shfl_sync(0xffffffffu, k.id, r >> 4);
     const bool there = page >= 0 && key >= k.low && key < k.length;
     const int64_t line = there ? pool.line(page, head, key) : 0;
-    copy16(to + (ROWS > 128 ? (r >> 7) * tile_bytes : 0) + tile_offset(r & 127, piece), pool.rows + line * (D * 2) + piece * 16, there);
+    copy16(to + (ROWS > 128 ? (r >> 7) * tile_bytes : 0) + tile_offset<(ROWS > 128 ? 128 : ROWS)>(r & 127, piece), pool.rows + line * (D * 2) + piece * 16, there);
   }
 }
 // Codes, 16 of them per load, as numbers of type M.
@@ -168,7 +170,7 @@ __device__ __forceinline__ void convert_keys(const PoolView& pool, const KeyRuns
 #pragma unroll
     for (int n = 0; n < BATCH; ++n) {
       const int r = r0 + n * EACH;
-      store_codes<M>(to + (ROWS > 128 ? (r >> 7) * tile_bytes : 0), r & 127, piece, codes[n]);
+      store_codes<M, (ROWS > 128 ? 128 : ROWS)>(to + (ROWS > 128 ? (r >> 7) * tile_bytes : 0), r & 127, piece, codes[n]);
     }
   }
 }
