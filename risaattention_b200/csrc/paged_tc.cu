@@ -100,6 +100,9 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
     const uint32_t two = C::SHARED || piece.seq.count * a.line.group - piece.block * C::ROWS > 128 ? kTwoGroups : 0u;
     KeyRuns ahead;
     ahead.look_up(row, a.line.step.page_shift, a.pages, C::KEYS / 16, piece.first * C::KEYS, low, length);
+    // over codes: the next batch is on its way while one is converted
+    CodeBatch<C::D> batch;
+    if (C::INT8) batch.load(keys, ahead, piece.head, 0, p);
 #pragma unroll 1
     for (int i = 0; i < piece.count; ++i) {
       const KeyRuns runs = ahead;
@@ -132,7 +135,15 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
             for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
             if ((p & 31) == 0) scales->lift[slot][p >> 5] = lg2_approx(most);
           }
-          convert_keys<__half, C::D, C::KEYS>(side ? values : keys, runs, piece.head, to, 0, p);
+#pragma unroll 1
+          for (int from = 0; from < C::KEYS; from += CodeBatch<C::D>::ROWS) {
+            CodeBatch<C::D> next = batch;
+            if (from + CodeBatch<C::D>::ROWS < C::KEYS) next.load(side ? values : keys, runs, piece.head, from + CodeBatch<C::D>::ROWS, p);
+            else if (side == 0) next.load(values, runs, piece.head, 0, p);
+            else if (i + 1 < piece.count) next.load(keys, ahead, piece.head, 0, p);
+            batch.template store<__half, C::KEYS>(to, 0, from, p);
+            batch = next;
+          }
           fence_async_smem();
           mbar_arrive(smem_u32(full + stage.stage));
         } else if (runs.bad == 0 && runs.key0 >= low && runs.key0 + C::KEYS <= length) {

@@ -153,27 +153,31 @@ __device__ __forceinline__ void copy_keys(const PoolView& pool, const KeyRuns& k
     copy16(to + (ROWS > 128 ? (r >> 7) * tile_bytes : 0) + tile_offset<(ROWS > 128 ? 128 : ROWS)>(r & 127, piece), pool.rows + line * (D * 2) + piece * 16, there);
   }
 }
-// Codes, 16 of them per load, as numbers of type M.
-template <typename M, int D, int ROWS>
-__device__ __forceinline__ void convert_keys(const PoolView& pool, const KeyRuns& k, int head, uint32_t to, int tile_bytes, int thread) {
-  constexpr int PIECES = D / 16, EACH = 128 / PIECES, BATCH = 4;
-  const int piece = thread % PIECES;
-#pragma unroll 1
-  for (int r0 = thread / PIECES; r0 < ROWS; r0 += BATCH * EACH) {
-    uint4 codes[BATCH];
+// Codes, 16 of them per load; a batch is what a thread has on its way at once, from row `from` of the tile on.
+template <int D>
+struct CodeBatch {
+  static constexpr int PIECES = D / 16, EACH = 128 / PIECES, COUNT = 4, ROWS = COUNT * EACH;
+  uint4 codes[COUNT];
+  __device__ __forceinline__ void load(const PoolView& pool, const KeyRuns& k, int head, int from, int thread) {
+    const int piece = thread % PIECES;
 #pragma unroll
-    for (int n = 0; n < BATCH; ++n) {
-      const int r = r0 + n * EACH, key = k.key0 + r, page = __shfl_sync(0xffffffffu, k.id, r >> 4);
+    for (int n = 0; n < COUNT; ++n) {
+      const int r = from + thread / PIECES + n * EACH, key = k.key0 + r, page = __shfl_sync(0xffffffffu, k.id, r >> 4);
       const bool there = page >= 0 && key >= k.low && key < k.length;
       codes[n] = there ? *reinterpret_cast<const uint4*>(pool.rows + pool.line(page, head, key) * D + piece * 16) : make_uint4(0, 0, 0, 0);
     }
+  }
+  // As numbers of type M, into tiles of TILE rows that lie `tile_bytes` apart.
+  template <typename M, int TILE>
+  __device__ __forceinline__ void store(uint32_t to, int tile_bytes, int from, int thread) const {
+    const int piece = thread % PIECES;
 #pragma unroll
-    for (int n = 0; n < BATCH; ++n) {
-      const int r = r0 + n * EACH;
-      store_codes<M, (ROWS > 128 ? 128 : ROWS)>(to + (ROWS > 128 ? (r >> 7) * tile_bytes : 0), r & 127, piece, codes[n]);
+    for (int n = 0; n < COUNT; ++n) {
+      const int r = from + thread / PIECES + n * EACH;
+      store_codes<M, TILE>(to + r / TILE * tile_bytes, r % TILE, piece, codes[n]);
     }
   }
-}
+};
 
 }  // namespace serving
 }  // namespace risa_b200

@@ -133,8 +133,18 @@ __device__ __forceinline__ void fetch_keys(const WeighArgs& a, Pieces pieces, Ba
     }
     const uint32_t to = keys + kb.stage * C::KEYS;
     // codes as they are: a key's scale multiplies its scores in 32 bits
-    if constexpr (C::INT8) convert_keys<typename C::T, C::D, kBlockKeys>(a.keys, runs, at.head, to, C::GROUP, p);
-    else copy_keys<C::D, kBlockKeys>(a.keys, runs, at.head, to, C::GROUP, p);
+    if constexpr (C::INT8) {
+      CodeBatch<C::D> batch, next;
+      batch.load(a.keys, runs, at.head, 0, p);
+#pragma unroll 1
+      for (int from = 0; from < kBlockKeys; from += CodeBatch<C::D>::ROWS) {
+        if (from + CodeBatch<C::D>::ROWS < kBlockKeys) next.load(a.keys, runs, at.head, from + CodeBatch<C::D>::ROWS, p);
+        batch.template store<typename C::T, 128>(to, C::GROUP, from, p);
+        batch = next;
+      }
+    } else {
+      copy_keys<C::D, kBlockKeys>(a.keys, runs, at.head, to, C::GROUP, p);
+    }
     if (C::INT8) {
       fence_async_smem();
       mbar_arrive(smem_u32(bars->k_full + kb.stage));
