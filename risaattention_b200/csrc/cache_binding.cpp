@@ -5,6 +5,7 @@
 #include <torch/extension.h>
 
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/VirtualGuardImpl.h>
 
 #include <optional>
 #include <string>
@@ -192,6 +193,36 @@ at::Tensor rotate(const at::Tensor& x, const at::Tensor& positions, const at::Te
   return out;
 }
 
+// The rotation is linear: its gradient is the transposed rotation of the output's gradient, whose own gradient is the rotation
+// again.  (A Function in Python took 88 us for a small tensor's forward and backward pass.)
+struct Rotation : public torch::autograd::Function<Rotation> {
+  // the stream that is current on the tensors' device: in a backward pass the one that the forward pass ran on
+  static uintptr_t stream_on(const c10::Device& device) {
+    const c10::impl::VirtualGuardImpl devices(device.type());
+    return reinterpret_cast<uintptr_t>(devices.getStream(device).native_handle());
+  }
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& positions, const at::Tensor& turns,
+                            double magnitude, bool interleaved, bool transposed) {
+    ctx->save_for_backward({positions, turns});
+    ctx->saved_data["magnitude"] = magnitude;
+    ctx->saved_data["interleaved"] = interleaved;
+    ctx->saved_data["transposed"] = transposed;
+    return rotate(x, positions, turns, magnitude, interleaved, transposed, std::nullopt, x.is_cuda() ? stream_on(x.device()) : 0);
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    // gradients of sums and broadcasts arrive as expanded views
+    const at::Tensor grad = grads[0].stride(-1) == 1 ? grads[0] : grads[0].contiguous();
+    return {Rotation::apply(grad, saved[0], saved[1], ctx->saved_data["magnitude"].toDouble(), ctx->saved_data["interleaved"].toBool(),
+                            !ctx->saved_data["transposed"].toBool()),
+            at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+  }
+};
+at::Tensor rotate_with_gradient(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& turns, double magnitude, bool interleaved,
+                                bool transposed) {
+  return Rotation::apply(x, positions, turns, magnitude, interleaved, transposed);
+}
+
 // Writes k and v [tokens, kv_heads, head_dim]; returns q rotated, or None.
 MaybeTensor cache_append(const at::Tensor& cache_keys, const at::Tensor& cache_values, const MaybeTensor& key_scales,
                          const MaybeTensor& value_scales, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
@@ -348,6 +379,7 @@ py::tuple cache_evict(const at::Tensor& cache_keys, const at::Tensor& cache_valu
 
 void bind_cache(py::module_& m) {
   m.def("rotate", &rotate);
+  m.def("rotate_with_gradient", &rotate_with_gradient);
   m.def("cache_append", &cache_append);
   m.def("paged_attention", &paged_attention);
   m.def("key_weights", &key_weights);

@@ -111,31 +111,6 @@ def _check_table(rotary):
         raise TypeError(f"rotary must be a RotaryTable, got {type(rotary).__name__}")
 
 
-def _rotated(x, positions, rotary, interleaved, transposed, out=None):
-    return _native(x.device).rotate(x, positions, rotary.turns, rotary.magnitude, interleaved, transposed, out,
-                                    _stream(x.device))
-
-
-class _Rotation(torch.autograd.Function):
-    """The rotation is linear: its gradient is the transposed rotation of the output's gradient, whose own
-    gradient is the rotation again."""
-
-    @staticmethod
-    def forward(ctx, x, positions, rotary, interleaved, transposed):
-        ctx.save_for_backward(positions, rotary.turns)
-        ctx.options = rotary.magnitude, interleaved, transposed
-        return _rotated(x, positions, rotary, interleaved, transposed)
-
-    @staticmethod
-    def backward(ctx, grad):
-        positions, turns = ctx.saved_tensors
-        magnitude, interleaved, transposed = ctx.options
-        if grad.stride(-1) != 1:
-            grad = grad.contiguous()  # gradients of sums and broadcasts arrive as expanded views
-        table = RotaryTable(turns, magnitude)
-        return _Rotation.apply(grad, positions, table, interleaved, not transposed), None, None, None, None
-
-
 def rotate_positions(x, positions, rotary, *, interleaved=False, transposed=False, out=None):
     """Rotates the first ``rotary.rotary_dim`` channels of every row of ``x`` by its position; the others
     are copied.
@@ -152,8 +127,10 @@ def rotate_positions(x, positions, rotary, *, interleaved=False, transposed=Fals
     if torch.is_grad_enabled() and x.requires_grad:
         if out is not None:
             raise ValueError("out cannot be given where x requires a gradient")
-        return _Rotation.apply(x, positions, rotary, bool(interleaved), bool(transposed))
-    return _rotated(x, positions, rotary, bool(interleaved), bool(transposed), out)
+        return _native(x.device).rotate_with_gradient(x, positions, rotary.turns, rotary.magnitude,
+                                                      bool(interleaved), bool(transposed))
+    return _native(x.device).rotate(x, positions, rotary.turns, rotary.magnitude, bool(interleaved),
+                                    bool(transposed), out, _stream(x.device))
 
 
 # ---- the cache --------------------------------------------------------------------------------------------

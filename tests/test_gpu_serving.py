@@ -113,6 +113,33 @@ def test_rotation_gradient(interleaved):
         assert torch.equal(second, risa.rotate_positions(direction, positions, table, interleaved=interleaved))
 
 
+def test_rotation_gradient_on_another_stream_and_in_a_graph():
+    table = risa.rotary_table(64)
+    positions = torch.arange(40, device="cuda")
+    x = torch.randn(40, 3, 64, device="cuda").requires_grad_()
+    grad = torch.randn_like(x)
+    want, = torch.autograd.grad(risa.rotate_positions(x, positions, table), x, grad)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        got, = torch.autograd.grad(risa.rotate_positions(x, positions, table), x, grad)
+    torch.cuda.synchronize()
+    assert torch.equal(got, want)
+    leaf = x.detach().clone().requires_grad_()
+    with torch.cuda.stream(side):
+        torch.autograd.grad(risa.rotate_positions(leaf, positions, table), leaf, grad)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured, = torch.autograd.grad(risa.rotate_positions(leaf, positions, table), leaf, grad)
+    grad.mul_(2)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(captured, 2 * want)
+    with pytest.raises(ValueError):
+        risa.rotate_positions(x, positions[:3], table)
+
+
 # ---- append -------------------------------------------------------------------------------------------------
 APPENDS = [
     # lengths, chunks, heads, head_dim, page, rotary_dim
