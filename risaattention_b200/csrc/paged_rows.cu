@@ -11,6 +11,10 @@
 // in bf16 become fp16 too, their row multiplied by a power of two that brings its largest value to 2^14: nothing is lost
 // but what is 2^-38 of that value.  Probability times scale fits fp16 because the running maximum is not that of the
 // scores s but of s + log2(scale): what is rounded is at most 1, and exact relative to the largest contribution.
+//
+// Measured: 16 requests of up to 16K keys, 8 key heads of 128 bf16 channels, 110 us (6.1 TB/s, 95 % of a plain copy's rate);
+// 32 requests of up to 32K keys as codes 246 us at full clocks (5.6 TB/s), 282 in long runs, where the conversion's
+// instructions (schedulers 61 % busy) feel the lower clock.
 #include "paged_tc.cuh"
 #include "serving_plan.cuh"
 
