@@ -327,6 +327,41 @@ def test_attention_of_many_sequences():
     U.assert_attention(b, out, lse)
 
 
+@pytest.mark.parametrize("head_dim,page,quantized", [(256, 128, False), (256, 16, True), (256, 128, True), (64, 128, False), (128, 16, True)])
+@pytest.mark.parametrize("window", [None, 50])
+def test_chunks_of_other_shapes(head_dim, page, quantized, window):
+    """Pages larger than a tile and smaller, a group of three heads, blocks of query rows that end anywhere."""
+    b = U.batch_of([257, 64, 500, 129], [100, 64, 11, 43], q_heads=6, kv_heads=2, head_dim=head_dim, page=page, quantized=quantized, seed=head_dim)
+    out, lse = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets, window=window, return_lse=True)
+    U.assert_attention(b, out, lse, window=window)
+    assert_weights(b, risa.cached_key_weights(b.q, lse, b.cache, b.table, b.lengths, query_offsets=b.offsets, window=window), lse, window=window)
+
+
+def test_many_sequences_of_chunks_and_single_tokens():
+    lengths = [20 + (53 * i) % 150 for i in range(70)]
+    chunks = [(1, 0, 9, 20, 3)[i % 5] for i in range(70)]
+    b = U.batch_of(lengths, chunks, q_heads=8, kv_heads=2, head_dim=64, page=16)
+    out, lse = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets, return_lse=True)
+    U.assert_attention(b, out, lse)
+    assert_weights(b, risa.cached_key_weights(b.q, lse, b.cache, b.table, b.lengths, query_offsets=b.offsets), lse)
+
+
+def test_two_calls_at_once():
+    batches = [U.batch_of([2000 + 300 * i, 90], [1 + 60 * i, 40], q_heads=8, kv_heads=2, head_dim=128, page=16, seed=i, quantized=i == 1) for i in range(2)]
+    attend = lambda b: risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets, return_lse=True)  # noqa: E731
+    want = [attend(b) for b in batches]
+    streams = [torch.cuda.Stream() for _ in batches]
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        for b, stream in zip(batches, streams):
+            with torch.cuda.stream(stream):
+                got.append(attend(b))
+    torch.cuda.synchronize()
+    for i, (out, lse) in enumerate(got):
+        assert torch.equal(out, want[i % 2][0]) and torch.equal(lse, want[i % 2][1])
+
+
 def test_attention_gives_the_same_bits_again_and_on_another_stream():
     b = U.batch_of([3000, 70, 900], [1, 60, 300], q_heads=8, kv_heads=2, head_dim=128, page=64)
     first = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets, return_lse=True)
@@ -417,7 +452,7 @@ def assert_weights(b, got, lse, previous=None, **options):
 
 @pytest.mark.parametrize("step", STEPS)
 @pytest.mark.parametrize("heads", [(4, 2), (8, 1), (20, 1)])
-@pytest.mark.parametrize("head_dim,page,dtype,quantized", [(64, 16, BF16, False), (128, 32, F16, False), (128, 128, BF16, True), (256, 64, F16, True), (256, 16, BF16, False)])
+@pytest.mark.parametrize("head_dim,page,dtype,quantized", [(64, 16, BF16, False), (64, 32, BF16, True), (128, 32, F16, False), (128, 128, BF16, True), (256, 64, F16, True), (256, 16, BF16, False)])
 def test_key_weights(step, heads, head_dim, page, dtype, quantized):
     lengths, chunks = STEPS[step]
     b = U.batch_of(lengths, chunks, q_heads=heads[0], kv_heads=heads[1], head_dim=head_dim, page=page, dtype=dtype, quantized=quantized, seed=len(step))
