@@ -121,7 +121,7 @@ struct RotateArgs {
 // with two, 57 with four, 4.7 TB/s).
 constexpr int kHeadsAhead = 4;
 template <typename T>
-__global__ __launch_bounds__(256) void rotate_kernel(const RotateArgs a) {
+__global__ __launch_bounds__(256, 4) void rotate_kernel(const RotateArgs a) {
   chain_wait();
   chain_release();
   const int pairs = a.rotary_dim / 16, items = pairs + (a.head_dim - a.rotary_dim) / 8;
@@ -261,15 +261,17 @@ __device__ __forceinline__ float row_absmax(const float* x, int lanes) {
 
 // One CTA per new token.  head_dim / 8 lanes hold a row, eight channels each; the CTA's row slots walk
 // the token's query heads, key heads and value heads with the cosines and sines of the lane's channels
-// kept in registers (a token of 32 + 8 rotated heads would compute each of them 40 times otherwise).
+// kept in registers; they are computed once for the token (the kernel is bound by its instructions, and a third of
+// them were the sines of every lane).
 // The second channel of a pair sits in the same lane (interleaved) or in the lane half a rotated row
 // away, whose channels come by shuffle.  Codes: absolute maximum over 127, rounded to nearest even; a row of
 // zeros has scale 0, a row with an infinity or a NaN reads back as NaN.  8160 tokens of 32 + 2 x 8 heads, bf16 to codes:
 // 70 us (184 MB, 2.6 TB/s), bound by each CTA's chain of lookups and by the instructions of cosines and conversions; one
 // token of 64 requests: 8.4 us.
-constexpr int kRowsAhead = 6;  // rows of a slot on their way at once: all of a token of 32 + 2 x 8 heads of 128
+constexpr int kRowsAhead = 3;  // rows of a slot on their way at once: half of a token of 32 + 2 x 8 heads of 128
 template <typename T, bool INT8>
-__global__ __launch_bounds__(128) void append_kernel(const AppendArgs a) {
+__global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
+  __shared__ __align__(16) float cosines[128], sines[128];
   chain_wait();
   chain_release();
   const int token = blockIdx.x, lanes = a.head_dim >> 3;
@@ -321,22 +323,29 @@ __global__ __launch_bounds__(128) void append_kernel(const AppendArgs a) {
     atomicCAS(a.status, 0u, unsigned(s) + 1u);  // longer than its row of the table
   }
   const bool turned = a.turns != nullptr && channel < a.rotary_dim;
-  float cs[8], sn[8];
+  float cs[8] = {}, sn[8] = {};
   int partner = threadIdx.x & 31;
-  if (turned) {
+  if (a.turns != nullptr) {  // one thread for each pair of the token, then every lane takes those of its channels
     const int64_t position = a.positions ? position_at(a.positions, a.positions_64, token) : int64_t(place);
     const int half = a.rotary_dim >> 1;
-    const bool second = !a.interleaved && channel >= half;
-    const int pair0 = a.interleaved ? channel >> 1 : second ? channel - half : channel;
-    const int count = a.interleaved ? 4 : 8;
-    for (int i = 0; i < 8; ++i) {
-      if (i < count)
-        angle_of(position, __ldg(reinterpret_cast<const unsigned long long*>(a.turns) + pair0 + i), a.magnitude, cs[i], sn[i]);
-      else
-        cs[i] = sn[i] = 0.f;
-      if (second) sn[i] = -sn[i];  // b cos + a sin as b cos - a (-sin)
+    if (int(threadIdx.x) < half)
+      angle_of(position, __ldg(reinterpret_cast<const unsigned long long*>(a.turns) + threadIdx.x), a.magnitude, cosines[threadIdx.x], sines[threadIdx.x]);
+    __syncthreads();
+    if (turned) {
+      const bool second = !a.interleaved && channel >= half;
+      const int pair0 = a.interleaved ? channel >> 1 : second ? channel - half : channel;
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        if (a.interleaved && i == 4) break;
+        const float4 c = *reinterpret_cast<const float4*>(cosines + pair0 + i), d = *reinterpret_cast<const float4*>(sines + pair0 + i);
+        cs[i] = c.x; cs[i + 1] = c.y; cs[i + 2] = c.z; cs[i + 3] = c.w;
+        sn[i] = d.x; sn[i + 1] = d.y; sn[i + 2] = d.z; sn[i + 3] = d.w;
+      }
+      if (second)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sn[i] = -sn[i];  // b cos + a sin as b cos - a (-sin)
+      if (!a.interleaved) partner = (threadIdx.x & 31) + (second ? -(half >> 3) : (half >> 3));
     }
-    if (!a.interleaved) partner = (threadIdx.x & 31) + (second ? -(half >> 3) : (half >> 3));
   }
   const int slot_in_page = place & ((1 << a.step.page_shift) - 1);
   for (int r0 = 0; r0 < rows; r0 += slots * kRowsAhead) {
