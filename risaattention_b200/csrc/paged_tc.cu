@@ -96,6 +96,15 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
   RingPos<C::STAGES> stage;  // of both rings
   Piece piece;
   const PoolView keys{a.keys, a.key_scales, a.line.kv_heads, a.line.step.page_shift}, values{a.values, a.value_scales, a.line.kv_heads, a.line.step.page_shift};
+  // What is under way lands before the CTA ends, also when the issuer gave up on it (a stage that was never filled passes
+  // at once); `keys_ahead` is 1 where K's stage of this tile is filled and V's is not.
+  auto land = [&](int keys_ahead) {
+    copies_drain();
+    for (int i = 0; i < C::STAGES; ++i) {
+      mbar_drain(smem_u32(bars->k_full + i), i < stage.stage + keys_ahead ? stage.phase : stage.phase ^ 1);
+      mbar_drain(smem_u32(bars->v_full + i), i < stage.stage ? stage.phase : stage.phase ^ 1);
+    }
+  };
   while (pieces.next(a.line, piece)) {
     const int32_t* row = a.line.step.table + int64_t(piece.sequence) * a.line.step.width;
     const int length = piece.seq.length;
@@ -115,13 +124,8 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
         uint64_t* full = side ? bars->v_full : bars->k_full;
         uint64_t* empty = side ? bars->v_empty : bars->k_empty;
         const uint32_t to = (side ? v_ring : k_ring) + stage.stage * C::SIDE;
-        if (!mbar_wait(smem_u32(empty + stage.stage), stage.phase ^ 1, gave_up, 1001 + side)) {
-          // what is under way lands before the CTA ends (a stage that was never filled passes at once)
-          copies_drain();
-          for (int i = 0; i < C::STAGES; ++i) {
-            mbar_drain(smem_u32(bars->k_full + i), i < stage.stage + side ? stage.phase : stage.phase ^ 1);
-            mbar_drain(smem_u32(bars->v_full + i), i < stage.stage ? stage.phase : stage.phase ^ 1);
-          }
+        if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(empty + stage.stage), stage.phase ^ 1, gave_up, 1001 + side))) {
+          land(side);
           return;
         }
         if constexpr (C::INT8) {
@@ -178,7 +182,7 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
       ++issued;
     }
   }
-  copies_drain();
+  land(0);
 }
 
 // ---- the issuing warp ---------------------------------------------------------------------------------------------
@@ -252,10 +256,9 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
 }
 
 // ---- the softmax warpgroups -------------------------------------------------------------------------------------------
-// A meeting of the two warps that own the same 32 rows.  One that leaves early arrives once more on its way out, so the
-// other is never kept waiting.
+// A meeting of the two warps that own the same 32 rows.  It has no limit of its own, so nobody may stay away: after a wait
+// that ran out a warp waits for nothing more, but goes through all its tiles and meetings; its rows are marked at the end.
 __device__ __forceinline__ void meet(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
-__device__ __forceinline__ void leave(int id) { asm volatile("bar.arrive %0, 64;" ::"r"(id) : "memory"); }
 
 // Query rows of group g (half of the rows that both groups share), by the 256 threads of its two warpgroups: 16-byte pieces,
 // neighbouring threads along a row.  A
@@ -299,6 +302,9 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
   const int group_row = C::SHARED ? 0 : g * 128;  // of the group's first row in the unit
   const float call_scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // a scale of 0 must leave hidden scores at -inf
   uint32_t s_phase = 0, o_phase = 0, q_phase = 0, tile = 0, turn = 0;
+  auto wait = [&](uint32_t bar, uint32_t parity, unsigned int site) {
+    if (!mbar_test(bar, parity) && gave_up_read(gave_up) == 0) mbar_wait(bar, parity, gave_up, site);
+  };
   Piece piece;
   bool more = pieces.next(a.line, piece);
   auto mine = [&](const Piece& p) { return p.seq.count * a.line.group - p.block * C::ROWS > group_row; };
@@ -327,7 +333,7 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
 #pragma unroll 1
     for (int i = 0; i < piece.count; ++i, ++tile) {
       const int key0 = (piece.first + i) * C::KEYS + half * KEYS;
-      if (!mbar_wait(smem_u32(bars->s_full + g), s_phase, gave_up, 1020 + g)) return leave(meeting);
+      wait(smem_u32(bars->s_full + g), s_phase, 1020 + g);
       s_phase ^= 1;
       tc_fence_after();
       uint32_t x[KEYS];
@@ -425,14 +431,14 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
     const Piece done = piece;
     more = pieces.next(a.line, piece);
     if (C::SHARED) {  // and by the other group
-      if (!mbar_wait(smem_u32(&bars->q_empty), q_phase, gave_up, 1024 + g)) return leave(meeting);
+      wait(smem_u32(&bars->q_empty), q_phase, 1024 + g);
       q_phase ^= 1;
     }
     if (more && mine(piece)) fetch(piece);
     exchange->sum[g][half][r] = l;
     meet(meeting);
     l += exchange->sum[g][half ^ 1][r];
-    if (!mbar_wait(smem_u32(bars->o_full + g), o_phase, gave_up, 1022 + g)) return leave(meeting);
+    wait(smem_u32(bars->o_full + g), o_phase, 1022 + g);
     o_phase ^= 1;
     tc_fence_after();
     const bool there = row < rows;

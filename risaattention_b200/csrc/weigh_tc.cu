@@ -128,7 +128,7 @@ __device__ __forceinline__ void fetch_keys(const WeighArgs& a, Pieces pieces, Ba
     const int low = first_seen(a.line, at.seq), length = at.seq.length, key0 = (low / kBlockKeys + at.block) * kBlockKeys;
     KeyRuns runs;
     runs.look_up(row, a.line.step.page_shift, a.pages, kBlockKeys / 16, key0, low, length);
-    if (!mbar_wait(smem_u32(bars->k_empty + kb.stage), kb.phase ^ 1, gave_up, 1101)) break;
+    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(bars->k_empty + kb.stage), kb.phase ^ 1, gave_up, 1101))) break;
     if (p == 0) {
       notes->bad[block % kDepth] = runs.bad;
       if (runs.bad) atomicCAS(a.status, 0u, unsigned(at.sequence) + 1u);
@@ -190,7 +190,7 @@ __device__ __forceinline__ void fetch_queries(const WeighArgs& a, Pieces pieces,
       const float x = lse;
       if (i + 1 < now.count) lse = lse_of(now, now.first + i + 1);
       else if (more) lse = lse_of(piece, piece.first);
-      if (!mbar_wait(smem_u32(bars->q_empty + st.stage), st.phase ^ 1, gave_up, 1102)) return copies_drain();
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(bars->q_empty + st.stage), st.phase ^ 1, gave_up, 1102))) return copies_drain();
       int row = (now.first + i) * C::ROWS + r0;
       const int token = row / a.line.group;
       int h = row - token * a.line.group;
@@ -321,7 +321,7 @@ __device__ __forceinline__ void add_up(const WeighArgs& a, Pieces pieces, Barrie
     }
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     for (int i = 0; i < piece.count; ++i, ++tile) {
-      if (!mbar_wait(smem_u32(&bars->s_full[g][buffer.stage]), buffer.phase, gave_up, 1120 + g)) return;
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&bars->s_full[g][buffer.stage]), buffer.phase, gave_up, 1120 + g))) return;
       tc_fence_after();
       if (i == 0) {
         const uint32_t bad = notes->bad[block % kDepth] >> (8 * g) & 0xff;
@@ -351,7 +351,7 @@ __device__ __forceinline__ void add_up(const WeighArgs& a, Pieces pieces, Barrie
       mbar_arrive_warp(smem_u32(bars->half_full + g));
       continue;
     }
-    if (!mbar_wait(smem_u32(bars->half_full + g), parity, gave_up, 1122 + g)) return;
+    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(bars->half_full + g), parity, gave_up, 1122 + g))) return;
     total += *other;
     if (!piece.whole) {
       a.parts[(int64_t(blockIdx.x) * 2 + (piece.opens ? 1 : 0)) * kBlockKeys + g * 128 + lane] = total;
