@@ -257,7 +257,7 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
 
 // ---- the softmax warpgroups -------------------------------------------------------------------------------------------
 // A meeting of the two warps that own the same 32 rows.  It has no limit of its own, so nobody may stay away: after a wait
-// that ran out a warp waits for nothing more, but goes through all its tiles and meetings; its rows are marked at the end.
+// that ran out a warp does no more work, but comes to all the meetings that are left; its rows are marked at the end.
 __device__ __forceinline__ void meet(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
 
 // Query rows of group g (half of the rows that both groups share), by the 256 threads of its two warpgroups: 16-byte pieces,
@@ -302,9 +302,6 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
   const int group_row = C::SHARED ? 0 : g * 128;  // of the group's first row in the unit
   const float call_scale = fmaxf(fabsf(a.scale_log2), 1e-30f);  // a scale of 0 must leave hidden scores at -inf
   uint32_t s_phase = 0, o_phase = 0, q_phase = 0, tile = 0, turn = 0;
-  auto wait = [&](uint32_t bar, uint32_t parity, unsigned int site) {
-    if (!mbar_test(bar, parity) && gave_up_read(gave_up) == 0) mbar_wait(bar, parity, gave_up, site);
-  };
   Piece piece;
   bool more = pieces.next(a.line, piece);
   auto mine = [&](const Piece& p) { return p.seq.count * a.line.group - p.block * C::ROWS > group_row; };
@@ -312,6 +309,16 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
     turn ^= 1;
     load_query_rows<C>(a, p, g, q + (C::SHARED ? 0 : g * C::QUERIES), C::INT8 ? scales->row[turn][C::SHARED ? 0 : g] : nullptr);
     mbar_arrive_warp(smem_u32(bars->q_full + g));
+  };
+  auto wait = [&](uint32_t bar, uint32_t parity, unsigned int site) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, gave_up, site)); };
+  auto meet_on = [&](int meetings) {  // of the present unit, then of all that follow
+#pragma unroll 1
+    while (more) {
+#pragma unroll 1
+      for (; meetings > 0; --meetings) meet(meeting);
+      more = pieces.next(a.line, piece);
+      meetings = more && mine(piece) ? piece.count + 1 : 0;
+    }
   };
   if (more && mine(piece)) fetch(piece);
   while (more) {
@@ -333,7 +340,7 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
 #pragma unroll 1
     for (int i = 0; i < piece.count; ++i, ++tile) {
       const int key0 = (piece.first + i) * C::KEYS + half * KEYS;
-      wait(smem_u32(bars->s_full + g), s_phase, 1020 + g);
+      if (!wait(smem_u32(bars->s_full + g), s_phase, 1020 + g)) return meet_on(piece.count - i + 1);
       s_phase ^= 1;
       tc_fence_after();
       uint32_t x[KEYS];
@@ -431,14 +438,17 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
     const Piece done = piece;
     more = pieces.next(a.line, piece);
     if (C::SHARED) {  // and by the other group
-      wait(smem_u32(&bars->q_empty), q_phase, 1024 + g);
+      if (!wait(smem_u32(&bars->q_empty), q_phase, 1024 + g)) {
+        meet(meeting);
+        return meet_on(more && mine(piece) ? piece.count + 1 : 0);
+      }
       q_phase ^= 1;
     }
     if (more && mine(piece)) fetch(piece);
     exchange->sum[g][half][r] = l;
     meet(meeting);
     l += exchange->sum[g][half ^ 1][r];
-    wait(smem_u32(bars->o_full + g), o_phase, 1022 + g);
+    if (!wait(smem_u32(bars->o_full + g), o_phase, 1022 + g)) return meet_on(more && mine(piece) ? piece.count + 1 : 0);
     o_phase ^= 1;
     tc_fence_after();
     const bool there = row < rows;
