@@ -74,8 +74,8 @@ int risa_b200_cache_append(const risa_b200_cache* cache, const risa_b200_step* s
 /* softmax(scale * q K^T) V of every packed token over its sequence's cached keys; with is_causal the
  * token at place p of its sequence sees keys max(0, p - window + 1) .. p (window 0: from the start),
  * without it all of them.  q, out: dtype_code 1 or 2 (the cache's own unless that is int8).  lse: f32
- * [tokens, q_heads] or NULL.  Rows that see no key give 0 and -inf.  clear_rest: rows behind the last
- * sequence are written the same way, else left as they were. */
+ * [tokens, q_heads] or NULL.  Rows that see no key give 0 and -inf.  clear_rest: rows of no
+ * sequence are written the same way, bit 0 those of out, bit 1 those of lse, else left as they were. */
 size_t risa_b200_paged_attention_scratch_size(const risa_b200_cache* cache,
                                               const risa_b200_step* step, int q_heads);
 int risa_b200_paged_attention(const risa_b200_cache* cache, const risa_b200_step* step,

@@ -311,7 +311,7 @@ py::tuple paged_attention(const at::Tensor& q, const at::Tensor& cache_keys, con
   const Strides2 qs(qr), os(out);
   check(risa_b200_paged_attention(&cache.c, &step.s, qr.data_ptr(), qs.of, int(q.size(1)), code_of(q), out.data_ptr(), os.of,
                                   return_lse ? lse->data_ptr<float>() : nullptr, float(scale), is_causal ? 1 : 0,
-                                  window.has_value() ? int(*window) : 0, out_given.has_value() ? 0 : 1, scratch.data_ptr(), bytes,
+                                  window.has_value() ? int(*window) : 0, out_given.has_value() ? 2 : 3, scratch.data_ptr(), bytes,
                                   stream_of(stream_ptr)));
   return py::make_tuple(out, lse);
 }

@@ -343,11 +343,14 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
   chain_wait();
   chain_release();
   if (a.clear_rest && a.line.step.offsets != nullptr) {
-    const int heads = a.line.kv_heads * a.line.group;
-    for (int token = max(__ldg(a.line.step.offsets + a.line.step.batch), 0) + blockIdx.x; token < a.line.step.tokens; token += gridDim.x) {
-      for (int i = threadIdx.x; i < heads * (D / 8); i += kThreads)
+    const int heads = a.line.kv_heads * a.line.group, tokens = a.line.step.tokens;
+    // tokens in front of the first sequence, then those behind the last
+    const int front = min(max(__ldg(a.line.step.offsets), 0), tokens), back = max(__ldg(a.line.step.offsets + a.line.step.batch), front);
+    for (int n = blockIdx.x; n < front || n - front < tokens - back; n += gridDim.x) {
+      const int token = n < front ? n : n - front + back;
+      if (a.clear_rest & 1) for (int i = threadIdx.x; i < heads * (D / 8); i += kThreads)
         *reinterpret_cast<uint4*>(static_cast<T*>(a.out) + token * a.on + (i / (D / 8)) * a.oh + (i % (D / 8)) * 8) = make_uint4(0, 0, 0, 0);
-      if (a.lse != nullptr)
+      if ((a.clear_rest & 2) && a.lse != nullptr)
         for (int h = threadIdx.x; h < heads; h += kThreads) a.lse[int64_t(token) * heads + h] = -INFINITY;
     }
   }

@@ -205,8 +205,8 @@ def paged_attention(q, cache, page_table, lengths, *, query_offsets=None, scale=
     With ``is_causal`` (aligned to the end: the last new token sees all ``lengths[s]`` keys) and ``window``
     a token sees the last ``window`` keys up to its own place; without ``is_causal`` every token sees all.
     ``q_heads`` is a multiple of the cache's heads.  ``scale``: head_dim ** -0.5 unless given.  A token that
-    sees nothing gives 0 and an LSE of -inf.  Rows behind the last sequence give the same, or stay as they
-    were where ``out`` is given.  Returns the output, with ``return_lse`` also the natural logarithm of the
+    sees nothing gives 0 and an LSE of -inf.  Rows of no sequence (behind the last, in front of the first) give
+    the same; where ``out`` is given its rows stay as they were.  Returns the output, with ``return_lse`` also the natural logarithm of the
     denominators, FP32 [tokens, q_heads].
 
     Unlike ``int8_attention`` nothing is quantised on the way: scores, softmax and sums are FP32 over the

@@ -307,6 +307,17 @@ def test_attention_rows_behind_the_last_sequence_and_out():
     assert same.data_ptr() == given.data_ptr() and torch.equal(given[:4], out[:4]) and (given[4:] == 3).all()
 
 
+def test_rows_of_no_sequence_in_front_and_in_a_given_output():
+    b = U.batch_of([50, 70], [1, 60], q_heads=4, kv_heads=2, head_dim=64, page=16, extra_rows=5)
+    want, lse = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets, return_lse=True)
+    q = torch.cat([b.q[-3:], b.q])
+    for given in (None, torch.full_like(q, 3)):
+        out, got = risa.paged_attention(q, b.cache, b.table, b.lengths, query_offsets=b.offsets + 3, return_lse=True, out=given)
+        rest = 0 if given is None else 3
+        assert torch.equal(out[3:64], want[:61]) and (out[:3] == rest).all() and (out[64:] == rest).all()
+        assert torch.equal(got[3:64], lse[:61]) and torch.isneginf(got[:3]).all() and torch.isneginf(got[64:]).all()
+
+
 def test_attention_of_query_views():
     b = U.batch_of([50, 70], [7, 3], q_heads=4, kv_heads=2, head_dim=128, page=16)
     want = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets)
