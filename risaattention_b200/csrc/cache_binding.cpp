@@ -4,6 +4,7 @@
 // types TypeError, in the order shapes, types, devices.
 #include <torch/extension.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 
@@ -45,6 +46,15 @@ int code_of(const at::Tensor& t) {
 // No two elements of a tensor that is written may share memory.
 void require_distinct(const at::Tensor& t, const char* what) {
   for (int64_t i = 0; i < t.dim(); ++i) require(t.size(i) <= 1 || t.stride(i) != 0, std::string(what) + " must not be an expanded view");
+}
+
+// An output may be the input itself, row for row, or lie apart from it.  (Views with gaps that interleave are not told from
+// views that overlap.)
+void require_apart(const at::Tensor& out, const at::Tensor& in, const char* what) {
+  const bool same = out.data_ptr() == in.data_ptr();
+  const at::MemOverlapStatus overlap = at::get_overlap_status(out, in);
+  require((!same && overlap != at::MemOverlapStatus::Full && overlap != at::MemOverlapStatus::Partial) || (same && out.strides() == in.strides()),
+          std::string("out may be ") + what + " itself, not another view of its memory");
 }
 
 // Rows of eight channels that start on 16-byte boundaries: the tensor itself, or a packed copy.
@@ -172,7 +182,7 @@ at::Tensor rotate(const at::Tensor& x, const at::Tensor& positions, const at::Te
     require_distinct(*out_given, "out");
     require_type(out_given->scalar_type() == x.scalar_type(), "out must have the dtype of x");
     require(out_given->device() == x.device(), "out must be on the device of x");
-    require(out_given->data_ptr() != x.data_ptr() || out_given->strides() == x.strides(), "out may be x itself, not another view of its memory");
+    require_apart(*out_given, x, "x");
   }
   const Rotary rotary(turns, magnitude, interleaved, d, x.device());
   require(positions.device() == x.device(), "positions must be on the device of x");
@@ -279,6 +289,7 @@ void check_queries(const Cache& cache, const at::Tensor& q, const std::optional<
   require(q.dim() == 3 && q.size(2) == cache.c.head_dim, "q must have shape [tokens, q_heads, head_dim of the cache]");
   require(q.size(1) > 0 && q.size(1) % cache.c.kv_heads == 0,
           "q head count (" + std::to_string(q.size(1)) + ") must be divisible by the cache's head count (" + std::to_string(cache.c.kv_heads) + ")");
+  require(q.size(0) < ((int64_t(1) << 31) - 1024) / (q.size(1) / cache.c.kv_heads), "q has too many rows");
   require(!window.has_value() || (*window > 0 && *window < (int64_t(1) << 31)), "window must be positive");
   require(!window.has_value() || is_causal, "a window needs the causal rule");
   require_type(code_of(q) == 1 || code_of(q) == 2, "q must be float16 or bfloat16");
@@ -297,6 +308,7 @@ py::tuple paged_attention(const at::Tensor& q, const at::Tensor& cache_keys, con
             "out must have the shape of q and rows that start on 16-byte boundaries");
     require_distinct(*out_given, "out");
     require_type(out_given->scalar_type() == q.scalar_type(), "out must have the dtype of q");
+    require_apart(*out_given, q, "q");
   }
   const Step step(cache, table, lengths, offsets, q.size(0));
   require(q.device() == cache_keys.device() && (!out_given.has_value() || out_given->device() == q.device()), "q and out must be on the device of the cache");

@@ -691,7 +691,7 @@ int check_queries(const risa_b200_cache* cache, const risa_b200_step* step, cons
                "%s: query rows must start on 16-byte boundaries", what);
   RISA_REQUIRE(scale == scale && fabsf(scale) < INFINITY, "%s: the scale must be finite", what);
   RISA_REQUIRE(window >= 0 && (window == 0 || is_causal), "%s: a window needs the causal rule and at least one key", what);
-  RISA_REQUIRE(int64_t(step->tokens) * (q_heads / cache->kv_heads) < (int64_t(1) << 31), "%s: too many query rows", what);
+  RISA_REQUIRE(int64_t(step->tokens) * (q_heads / cache->kv_heads) < (int64_t(1) << 31) - 1024, "%s: too many query rows", what);
   return RISA_B200_OK;
 }
 

@@ -119,7 +119,8 @@ def rotate_positions(x, positions, rotary, *, interleaved=False, transposed=Fals
     head_dim] with ``positions`` [tokens] or [batch, tokens]; float32, float16 or bfloat16, any strides with
     contiguous rows.  ``positions``: int32 or int64 (negative ones turn backwards).  Pair i is channels
     (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where ``interleaved``.  ``transposed`` applies the transposed
-    rotation (the inverse where the table's magnitude is 1).  ``out``: where to write, ``x`` itself included.
+    rotation (the inverse where the table's magnitude is 1).  ``out``: where to write, ``x`` itself included, no other
+    view of its memory.
 
     Arithmetic is FP32 on angles reduced exactly; the gradient of ``x`` is the transposed rotation, from the
     same kernel."""
@@ -206,12 +207,14 @@ def paged_attention(q, cache, page_table, lengths, *, query_offsets=None, scale=
     a token sees the last ``window`` keys up to its own place; without ``is_causal`` every token sees all.
     ``q_heads`` is a multiple of the cache's heads.  ``scale``: head_dim ** -0.5 unless given.  A token that
     sees nothing gives 0 and an LSE of -inf.  Rows of no sequence (behind the last, in front of the first) give
-    the same; where ``out`` is given its rows stay as they were.  Returns the output, with ``return_lse`` also the natural logarithm of the
-    denominators, FP32 [tokens, q_heads].
+    the same; where ``out`` is given (``q`` itself included, no other view of its memory) its rows stay as they
+    were.  Returns the output, with ``return_lse`` also the natural logarithm of the denominators, FP32
+    [tokens, q_heads].
 
     Unlike ``int8_attention`` nothing is quantised on the way: scores, softmax and sums are FP32 over the
-    cache's 16-bit values or codes as they are; probabilities are rounded to the type of ``q`` (bf16 over a
-    cache of codes) for the product with V."""
+    cache's 16-bit values or codes as they are; probabilities are rounded to the type of ``q`` (float16 over a
+    cache of codes) for the product with V.  A value that is not finite may also reach tokens of the same call
+    that do not see its key: it is multiplied by their probability, 0."""
     _check_cache(cache)
     if scale is None:
         scale = q.shape[-1] ** -0.5

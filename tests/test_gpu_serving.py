@@ -318,6 +318,18 @@ def test_rows_of_no_sequence_in_front_and_in_a_given_output():
         assert torch.equal(got[3:64], lse[:61]) and torch.isneginf(got[:3]).all() and torch.isneginf(got[64:]).all()
 
 
+@pytest.mark.parametrize("head_dim", [64, 256])
+@pytest.mark.parametrize("lengths,chunks", [([900], [1]), ([40, 5000, 800], [1, 1, 200]), ([3000], [700])])
+def test_attention_into_its_queries(lengths, chunks, head_dim):
+    b = U.batch_of(lengths, chunks, q_heads=8, kv_heads=2, head_dim=head_dim, page=32)
+    want = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets)
+    wide = torch.zeros(b.q.shape[0], 12, head_dim, device="cuda", dtype=BF16)
+    wide[:, 2:10] = b.q
+    for q in (b.q.clone(), wide[:, 2:10]):
+        assert torch.equal(risa.paged_attention(q, b.cache, b.table, b.lengths, query_offsets=b.offsets, out=q), want) and torch.equal(q, want)
+    assert (wide[:, :2] == 0).all() and (wide[:, 10:] == 0).all()
+
+
 def test_attention_of_query_views():
     b = U.batch_of([50, 70], [7, 3], q_heads=4, kv_heads=2, head_dim=128, page=16)
     want = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets)

@@ -144,6 +144,23 @@ def test_attention_refusals(cache):
     refuses(ValueError, attend, x(3, 4, 64), cache, *step, out=x(1, 4, 64).expand(3, 4, 64), match="expanded")
 
 
+def test_outputs_that_overlap_their_input(cache):
+    memory, table = x(5, 4, 64), risa.rotary_table(64, device="cpu")
+    for out in (memory[1:4], memory[:3].view(4, 3, 64).transpose(0, 1)):
+        refuses(ValueError, risa.rotate_positions, memory[:3], ints(3), table, out=out, match="another view")
+        refuses(ValueError, risa.paged_attention, memory[:3], cache, ints(3, 2), ints(3), out=out, match="another view")
+    for out in (memory[:3], x(3, 4, 64)):
+        refuses(ValueError, risa.rotate_positions, memory[:3], ints(3), table, out=out, match="CUDA device")
+        refuses(ValueError, risa.paged_attention, memory[:3], cache, ints(3, 2), ints(3), out=out, match="CUDA device")
+
+
+def test_more_query_rows_than_31_bits(cache):
+    q, step = x(1, 1, 64).expand(2 ** 17, 2 ** 15, 64), (ints(1, 2), ints(1))
+    refuses(ValueError, risa.paged_attention, q, cache, *step, query_offsets=ints(2), match="too many rows")
+    lse = x(1, 1, dtype=torch.float32).expand(2 ** 17, 2 ** 15)
+    refuses(ValueError, risa.cached_key_weights, q, lse, cache, *step, query_offsets=ints(2), match="too many rows")
+
+
 def test_append_refusals(cache):
     append = risa.append_to_cache
     k, step = x(3, 2, 64), (ints(3, 2), ints(3))
