@@ -30,6 +30,12 @@ constexpr int kFetcher = 16, kKeyFetcher = 20, kIssuer = 24;
 // Notes and log-sum-exps of the tiles in flight.  A slot is written again kDepth tiles later, by when the sums have
 // left it: the fetchers are at most the query stages ahead of the issuer, the issuer two tiles ahead of the sums.
 constexpr int kDepth = 8;
+// Half sums on their way between the two warpgroups of a key group, each slot with a barrier of its own.  The scores of tile t
+// are issued once all eight warps have freed those of tile t - 2, and a warp frees a tile before it hands over or takes the
+// block that ends with it; so the giver is at most two blocks ahead of a warp that still has to take, three slots are in use,
+// and the giver comes back to a slot only after every taker has passed it.  (One barrier waited for by parity would need the
+// giver to be less than two phases ahead.)
+constexpr int kHalves = 4;
 // Bits of a note: first and last tile of a block, whether the block has more than 128 keys.
 constexpr uint32_t kFirst = 1u, kLast = 2u, kTwoGroups = 4u;
 
@@ -98,7 +104,7 @@ struct Shape {
 };
 
 struct Barriers {
-  uint64_t k_full[2], k_empty[2], q_full[4], q_empty[4], s_full[2][2], s_free[2][2], half_full[2], drained;
+  uint64_t k_full[2], k_empty[2], q_full[4], q_empty[4], s_full[2][2], s_free[2][2], half_full[2][kHalves], drained;
 };
 
 // Byte offset of piece `piece` of row `row` in a tile of ROWS query rows.
@@ -111,9 +117,7 @@ struct Notes {
   uint32_t tile[kDepth];
   uint32_t bad[kDepth];          // runs of 16 keys whose page is outside the pool, of the last blocks
   float minus_lse[kDepth][128];  // in units of log 2; -infinity for rows that give nothing
-  // What the second half of the rows adds to a key, of the last four blocks: the warpgroup that writes it is at most two
-  // tiles ahead of the one that reads it.
-  float half[4][2][128];
+  float half[kHalves][2][128];   // what the second half of the rows adds to a key, of the last blocks
 };
 
 // A worker's key blocks.
@@ -343,15 +347,15 @@ __device__ __forceinline__ void add_up(const WeighArgs& a, Pieces pieces, Barrie
       buffer.next();
     }
     float total = (sum[0] + sum[1]) + (sum[2] + sum[3]);
-    float* other = &notes->half[block & 3][g][lane];
-    const uint32_t parity = block & 1;
+    float* other = &notes->half[block % kHalves][g][lane];
+    const uint32_t handed = smem_u32(&bars->half_full[g][block % kHalves]), parity = block / kHalves & 1;
     ++block;
     if (half == 1) {
       *other = total;
-      mbar_arrive_warp(smem_u32(bars->half_full + g));
+      mbar_arrive_warp(handed);
       continue;
     }
-    if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(bars->half_full + g), parity, gave_up, 1122 + g))) return;
+    if (!__all_sync(0xffffffffu, mbar_wait(handed, parity, gave_up, 1122 + g))) return;
     total += *other;
     if (!piece.whole) {
       a.parts[(int64_t(blockIdx.x) * 2 + (piece.opens ? 1 : 0)) * kBlockKeys + g * 128 + lane] = total;
@@ -377,7 +381,7 @@ __global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(bars.k_full + i), 128 + 4);
       mbar_init(smem_u32(bars.k_empty + i), 1);
-      mbar_init(smem_u32(bars.half_full + i), 4);
+      for (int j = 0; j < kHalves; ++j) mbar_init(smem_u32(&bars.half_full[i][j]), 4);
       for (int g = 0; g < 2; ++g) {
         mbar_init(smem_u32(&bars.s_full[g][i]), 1);
         mbar_init(smem_u32(&bars.s_free[g][i]), 8);
