@@ -76,11 +76,11 @@ struct Exchange {
   float sum[kGroups][2][128];
 };
 // Over a cache of codes: scales of the tiles in flight (a slot is written again kScaleDepth tiles later, by when the softmax
-// that read it has handed over its probabilities), the largest of each 32 values' scales in units of log 2, and what the
-// queries' rows were divided by, of this unit and the one before.
+// that read it has handed over its probabilities), those of values also in units of log 2, and what the queries' rows were
+// divided by, of this unit and the one before.
 constexpr int kScaleDepth = 8;
 struct Scales {
-  float key[kScaleDepth][128], value[kScaleDepth][128], lift[kScaleDepth][4];
+  float key[kScaleDepth][128], value[kScaleDepth][128], lift[kScaleDepth][128];
   float row[2][kGroups][128];
 };
 
@@ -137,10 +137,8 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
             const float v = there ? __ldg(values.scales + line) : 0.f;
             scales->key[slot][p] = there ? __ldg(keys.scales + line) : 0.f;
             scales->value[slot][p] = v;
-            float most = v < INFINITY ? fmaxf(v, 0x1p-100f) : 0x1p-100f;  // one that is not finite must not let the others vanish
-#pragma unroll
-            for (int off = 16; off > 0; off >>= 1) most = fmaxf(most, __shfl_xor_sync(0xffffffffu, most, off));
-            if ((p & 31) == 0) scales->lift[slot][p >> 5] = lg2_approx(most);
+            // a row of zeros must not let its own probability overflow, nor one that is not finite let the others vanish
+            scales->lift[slot][p] = v < INFINITY ? lg2_approx(fmaxf(v, 0x1p-100f)) : 0.f;
           }
 #pragma unroll 1
           for (int from = 0; from < C::KEYS; from += CodeBatch<C::D>::ROWS) {
@@ -370,18 +368,33 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
         for (int c = 0; c < KEYS; ++c)
           if (c < lo || c >= hi || (gone >> (c >> 4) & 1)) x[c] = 0xff800000u;
       }
-      float top[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
-#pragma unroll
-      for (int c = 4; c < KEYS; c += 8)
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          top[e] = c + 4 + e < KEYS ? fmaxf(fmaxf(top[e], __uint_as_float(x[c + e])), __uint_as_float(x[c + 4 + e]))
-                                    : fmaxf(top[e], __uint_as_float(x[c + e]));
-      float best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
+      const uint64_t scale2 = pack_f32x2(scale, scale);
+      float best;
       if constexpr (C::INT8) {
-        // the maximum is that of probability times scale, or a little above it: at most 1 is rounded
-        const float4 lift = *reinterpret_cast<const float4*>(scales->lift[slot_of_tile]);
-        best += fmaxf(fmaxf(lift.x, lift.y), fmaxf(lift.z, lift.w));
+        // The maximum is that of the row's own probabilities times scales, hidden keys left out: what is rounded is at most 1
+        // (2^8 where the running maximum lags), and neither the other keys of the tile nor other rows move it.  (Against the
+        // largest scale of the tile, 1024 tokens over 8K codes, 32 heads: 271 us for 269 at 128 channels, 203 for 190 at 64.)
+        const ulonglong2* lift = reinterpret_cast<const ulonglong2*>(scales->lift[slot_of_tile] + half * KEYS);
+        float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+        for (int c = 0; c < KEYS; c += 4) {
+          const ulonglong2 of = lift[c / 4];
+          float u[4];
+          unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[c]), __uint_as_float(x[c + 1])), scale2, of.x), u[0], u[1]);
+          unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(x[c + 2]), __uint_as_float(x[c + 3])), scale2, of.y), u[2], u[3]);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) top[e] = fmaxf(top[e], u[e]);
+        }
+        best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+      } else {
+        float top[4] = {__uint_as_float(x[0]), __uint_as_float(x[1]), __uint_as_float(x[2]), __uint_as_float(x[3])};
+#pragma unroll
+        for (int c = 4; c < KEYS; c += 8)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            top[e] = c + 4 + e < KEYS ? fmaxf(fmaxf(top[e], __uint_as_float(x[c + e])), __uint_as_float(x[c + 4 + e]))
+                                      : fmaxf(top[e], __uint_as_float(x[c + e]));
+        best = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])) * scale;
       }
       // also: from here on both halves of the scores are in registers, and P may be written over them
       exchange->maximum[tile & 1][g][half][r] = best;
@@ -405,7 +418,7 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
           }
         }
       }
-      const uint64_t scale2 = pack_f32x2(scale, scale), minus_m = pack_f32x2(-m, -m);
+      const uint64_t minus_m = pack_f32x2(-m, -m);
       uint64_t sum[2] = {0, 0};
 #pragma unroll
       for (int part = 0; part < KEYS / 32; ++part) {

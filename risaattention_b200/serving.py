@@ -212,8 +212,10 @@ def paged_attention(q, cache, page_table, lengths, *, query_offsets=None, scale=
     [tokens, q_heads].
 
     Unlike ``int8_attention`` nothing is quantised on the way: scores, softmax and sums are FP32 over the
-    cache's 16-bit values or codes as they are; probabilities are rounded to the type of ``q`` (float16 over a
-    cache of codes) for the product with V.  A value that is not finite may also reach tokens of the same call
+    cache's 16-bit values or codes as they are; probabilities are rounded to the type of ``q`` for the product
+    with V.  Over a cache of codes it is probability times the key's scale that is rounded, to float16, in units
+    of the largest such product that the token sees: of two scales that differ by more than 2^24 the smaller one's
+    values may be lost in that token.  A value that is not finite may also reach tokens of the same call
     that do not see its key: it is multiplied by their probability, 0."""
     _check_cache(cache)
     if scale is None:
