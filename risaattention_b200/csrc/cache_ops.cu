@@ -655,9 +655,8 @@ extern "C" int risa_b200_rotate(const void* x, void* out, int dtype_code, int ba
   while (a.heads_each < 8 && a.heads_each < heads && threads * batch * heads / (2 * a.heads_each) >= 148 * 1024)
     a.heads_each *= 2;
   const dim3 grid(unsigned((threads + 255) / 256), unsigned((heads + a.heads_each - 1) / a.heads_each), unsigned(batch));
-  RISA_DISPATCH_FLOAT(dtype_code, T, launch_chained(wide ? rotate_kernel<T> : rotate_any_kernel<T>, grid, dim3(256), 0,
-                                                    static_cast<cudaStream_t>(stream_ptr), a));
-  return check_launch("rotate");
+  RISA_DISPATCH_FLOAT(dtype_code, T, return launched(launch_chained(wide ? rotate_kernel<T> : rotate_any_kernel<T>, grid, dim3(256), 0,
+                                                                    static_cast<cudaStream_t>(stream_ptr), a), "rotate"));
 }
 
 extern "C" int risa_b200_cache_append(const risa_b200_cache* cache, const risa_b200_step* step,
@@ -721,8 +720,7 @@ extern "C" int risa_b200_cache_append(const risa_b200_cache* cache, const risa_b
   a.status = status;
   const auto kernel = dtype_code == 1 ? (codes ? append_kernel<__half, true> : append_kernel<__half, false>)
                                       : (codes ? append_kernel<__nv_bfloat16, true> : append_kernel<__nv_bfloat16, false>);
-  launch_chained(kernel, dim3(step->tokens), dim3(128), 0, static_cast<cudaStream_t>(stream_ptr), a);
-  return check_launch("append");
+  return launched(launch_chained(kernel, dim3(step->tokens), dim3(128), 0, static_cast<cudaStream_t>(stream_ptr), a), "append");
 }
 
 extern "C" int risa_b200_cache_evict(const risa_b200_cache* cache, const risa_b200_step* step,
@@ -746,7 +744,8 @@ extern "C" int risa_b200_cache_evict(const risa_b200_cache* cache, const risa_b2
   const StepView view = view_of(*step, cache->page_size);
   const SelectArgs select{view, weights, kept, new_lengths, new_weights, cache->kv_heads, budget, recent,
                           target_width * cache->page_size};
-  launch_chained(select_kept_kernel, dim3(cache->kv_heads, step->batch), dim3(kSelectThreads), 0, stream, select);
+  if (const int bad = launched(launch_chained(select_kept_kernel, dim3(cache->kv_heads, step->batch), dim3(kSelectThreads), 0, stream, select), "evict"))
+    return bad;
   const int row_bytes = cache->head_dim * (cache->dtype_code == kInt8 ? 1 : 2);
   int shift = 0;
   while ((16 << shift) < row_bytes) ++shift;
@@ -754,6 +753,5 @@ extern "C" int risa_b200_cache_evict(const risa_b200_cache* cache, const risa_b2
                       cache->key_scales, cache->value_scales, cache->pages, cache->kv_heads, budget, target_width,
                       shift, status};
   const int rows = (256 >> shift) * kMoveRows;
-  launch_chained(move_kept_kernel, dim3((budget + rows - 1) / rows, cache->kv_heads, step->batch), dim3(256), 0, stream, move);
-  return check_launch("evict");
+  return launched(launch_chained(move_kept_kernel, dim3((budget + rows - 1) / rows, cache->kv_heads, step->batch), dim3(256), 0, stream, move), "evict");
 }

@@ -146,7 +146,10 @@ __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
 // the previous kernel drains, and wait at chain_wait() until that kernel has completed and its
 // writes are visible; chain_release() lets the next kernel's CTAs be placed as soon as every CTA of
 // this one has started.  Every kernel launched through launch_chained() must call chain_wait()
-// before its first global memory access, which also keeps the chain ordered transitively.
+// before its first global memory access, which also keeps the chain ordered transitively.  The one
+// exception are kernels that run beside the launch in front of them and call chain_wait() only at
+// their end: allowed directly behind a launch of the same call that did start, whose CTAs all wait
+// before they release and which writes nothing that such a kernel reads.
 #ifdef __CUDACC__
 __device__ __forceinline__ void chain_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void chain_release() {

@@ -773,8 +773,7 @@ extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const ris
     using C = decltype(tile);
     constexpr int bytes = kWarps * Walk<C, true>::STAGE * Walk<C, true>::STAGES;
     if (const int bad = allow_shared(paged_rows_kernel<C>, bytes, "paged attention")) return bad;
-    launch_chained(paged_rows_kernel<C>, dim3(kSms * C::CTAS), dim3(kThreads), bytes, stream, a);
-    return RISA_B200_OK;
+    return launched(launch_chained(paged_rows_kernel<C>, dim3(kSms * C::CTAS), dim3(kThreads), bytes, stream, a), "paged attention");
   });
   TcArgs t{};
   if (bad == RISA_B200_OK && tensor_cores) {
@@ -788,11 +787,10 @@ extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const ris
     bad = with_tile(dtype_code, codes, cache->head_dim, a.line.rows / 8, [&](auto tile) {
       using C = decltype(tile);
       const JoinArgs join{a.parts, a.notes, C::R, a.line.group, q_heads, out, a.on, a.oh, lse};
-      launch_chained(join_parts_kernel<typename C::T, C::D, true>, dim3(kSms * C::CTAS - 1, C::R), dim3(128), 0, stream, join);
-      return RISA_B200_OK;
+      return launched(launch_chained(join_parts_kernel<typename C::T, C::D, true>, dim3(kSms * C::CTAS - 1, C::R), dim3(128), 0, stream, join), "paged attention");
     });
   if (bad == RISA_B200_OK && tensor_cores) bad = paged_tc_join(t, dtype_code, cache->head_dim, stream);
-  return bad ? bad : check_launch("paged attention");
+  return bad;
 }
 
 extern "C" size_t risa_b200_key_weights_scratch_size(const risa_b200_cache* cache, const risa_b200_step* step, int q_heads) {
@@ -823,9 +821,7 @@ extern "C" int risa_b200_key_weights(const risa_b200_cache* cache, const risa_b2
     using C = decltype(tile);
     constexpr int bytes = kWarps * Walk<C, false>::STAGE * Walk<C, false>::STAGES;
     if (const int bad = allow_shared(weigh_rows_kernel<C>, bytes, "key weights")) return bad;
-    launch_chained(weigh_rows_kernel<C>, dim3(kSms * C::CTAS), dim3(kThreads), bytes,
-                   stream, a);
-    return RISA_B200_OK;
+    return launched(launch_chained(weigh_rows_kernel<C>, dim3(kSms * C::CTAS), dim3(kThreads), bytes, stream, a), "key weights");
   });
   if (bad == RISA_B200_OK && tensor_cores) {
     TcArgs t{};
@@ -843,5 +839,5 @@ extern "C" int risa_b200_key_weights(const risa_b200_cache* cache, const risa_b2
     t.status = status;
     bad = weigh_tc(t, lse, previous, weights, dtype_code, cache->dtype_code == kInt8, cache->head_dim, stream);
   }
-  return bad ? bad : check_launch("key weights");
+  return bad;
 }

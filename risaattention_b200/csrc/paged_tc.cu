@@ -628,8 +628,7 @@ template <typename T, int D>
 int join(const TcArgs& a, cudaStream_t stream) {
   constexpr int kRows = Shape<T, false, D>::ROWS;
   const JoinArgs join{a.parts, a.notes, kRows, a.line.group, a.line.kv_heads * a.line.group, a.out, a.on, a.oh, a.lse};
-  launch_chained(join_parts_kernel<T, D, false>, dim3(kTcWorkers - 1, kRows / 16), dim3(128), 0, stream, join);
-  return RISA_B200_OK;
+  return launched(launch_chained(join_parts_kernel<T, D, false>, dim3(kTcWorkers - 1, kRows / 16), dim3(128), 0, stream, join), "paged attention");
 }
 
 template <typename C>
@@ -647,8 +646,7 @@ int launch(const TcArgs& a, cudaStream_t stream) {
     return cudaFuncGetAttributes(&attributes, paged_tc_kernel<C>) == cudaSuccess && attributes.numRegs == kRegsLaunch;
   }();
   RISA_REQUIRE(budget, "paged attention: the tensor-core kernel was not compiled for %d registers", kRegsLaunch);
-  launch_chained(paged_tc_kernel<C>, dim3(kTcWorkers), dim3(kThreads), C::SMEM, stream, key_map, value_map, a);
-  return RISA_B200_OK;
+  return launched(launch_chained(paged_tc_kernel<C>, dim3(kTcWorkers), dim3(kThreads), C::SMEM, stream, key_map, value_map, a), "paged attention");
 }
 
 }  // namespace

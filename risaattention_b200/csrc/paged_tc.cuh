@@ -29,7 +29,7 @@ struct TcArgs {
 };
 
 size_t paged_tc_scratch(int head_dim);
-// The kernel runs beside the launch in front of it, which has to be one of the same call; the join comes behind both.
+// The kernel runs beside the launch in front of it, which has to be one of the same call that succeeded; the join comes behind both.
 TcArgs paged_tc_args(TcArgs args, int head_dim);
 int paged_tc(const TcArgs& args, int dtype_code, bool codes, int head_dim, cudaStream_t stream);
 int paged_tc_join(const TcArgs& args, int dtype_code, int head_dim, cudaStream_t stream);

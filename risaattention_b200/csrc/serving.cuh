@@ -43,6 +43,13 @@ inline int check_step(const risa_b200_step* s, const risa_b200_cache* c, const c
 
 #ifdef __CUDACC__
 
+// A launch that failed ends its call: what comes behind it reads what it would have written, or relies on its wait.
+inline int launched(cudaError_t e, const char* what) {
+  if (e == cudaSuccess) return RISA_B200_OK;
+  cudaGetLastError();
+  return fail(RISA_B200_CUDA, "%s: %s", what, cudaGetErrorString(e));
+}
+
 // A divisor known to the host: numbers below 2^31 are divided by a multiplication.
 struct Divisor {
   int value;

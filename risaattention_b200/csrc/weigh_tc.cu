@@ -484,9 +484,8 @@ int launch(WeighArgs a, cudaStream_t stream) {
   a.line.tile_rows = Divisor(C::ROWS);
   if (cudaFuncSetAttribute(weigh_tc_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
     return fail(RISA_B200_CUDA, "key weights: %s", cudaGetErrorString(cudaGetLastError()));
-  launch_chained(weigh_tc_kernel<C>, dim3(kTcWorkers), dim3(kThreads), C::SMEM, stream, a);
-  launch_chained(join_weights_kernel, dim3(kTcWorkers - 1), dim3(kBlockKeys), 0, stream, a);
-  return RISA_B200_OK;
+  if (const int bad = launched(launch_chained(weigh_tc_kernel<C>, dim3(kTcWorkers), dim3(kThreads), C::SMEM, stream, a), "key weights")) return bad;
+  return launched(launch_chained(join_weights_kernel, dim3(kTcWorkers - 1), dim3(kBlockKeys), 0, stream, a), "key weights");
 }
 template <typename T>
 int launch_for(const WeighArgs& a, bool codes, int head_dim, cudaStream_t stream) {
