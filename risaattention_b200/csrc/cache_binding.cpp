@@ -5,6 +5,7 @@
 #include <torch/extension.h>
 
 #include <ATen/MemoryOverlap.h>
+#include <c10/core/AutogradState.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 
@@ -161,10 +162,17 @@ void require_positions(const at::Tensor& p) {
   require_type(p.scalar_type() == at::kInt || p.scalar_type() == at::kLong, "positions must be int32 or int64");
 }
 
+// A tangent that rides on the tensor would be lost, whether it requires a gradient or not.
+void require_no_tangent(const at::Tensor& x) {
+  require(!c10::AutogradState::get_tls_state().get_fw_grad_mode() || !x._fw_grad(0).defined(),
+          "rotation has no forward-mode derivative: rotate the tangent itself, the map is linear");
+}
+
 // x [tokens, heads, head_dim] with positions [tokens], or [batch, heads, tokens, head_dim] with positions
 // [tokens] or [batch, tokens].
 at::Tensor rotate(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& turns, double magnitude, bool interleaved,
                   bool transposed, const MaybeTensor& out_given, uintptr_t stream_ptr) {
+  require_no_tangent(x);
   require(x.dim() == 3 || x.dim() == 4, "x must have shape [tokens, heads, head_dim] or [batch, heads, tokens, head_dim]");
   const bool packed = x.dim() == 3;
   const int64_t batch = packed ? 1 : x.size(0), heads = x.size(1), tokens = packed ? x.size(0) : x.size(2), d = x.size(-1);
@@ -230,6 +238,7 @@ struct Rotation : public torch::autograd::Function<Rotation> {
 };
 at::Tensor rotate_with_gradient(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& turns, double magnitude, bool interleaved,
                                 bool transposed) {
+  require_no_tangent(x);
   return Rotation::apply(x, positions, turns, magnitude, interleaved, transposed);
 }
 

@@ -123,7 +123,7 @@ def rotate_positions(x, positions, rotary, *, interleaved=False, transposed=Fals
     view of its memory.
 
     Arithmetic is FP32 on angles reduced exactly; the gradient of ``x`` is the transposed rotation, from the
-    same kernel."""
+    same kernel.  Tensors with a forward-mode tangent are refused (its rotation is the same call)."""
     _check_table(rotary)
     if torch.is_grad_enabled() and x.requires_grad:
         if out is not None:

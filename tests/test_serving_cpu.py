@@ -199,3 +199,16 @@ def test_weight_and_eviction_refusals(cache):
     refuses(ValueError, evict, cache, *step, weights, target, budget=17, match="hold the budget")
     refuses(ValueError, evict, cache, *step, weights, step[0], budget=8, match="other pages")
     refuses(ValueError, evict, cache, *step, weights, target, budget=8, match="CUDA device")
+
+
+def test_rotation_refuses_forward_mode():
+    """A dual tensor need not require a gradient; its tangent must not be lost on the way."""
+    table = risa.rotary_table(8, device="cpu")
+    for grad in (False, True):
+        with torch.autograd.forward_ad.dual_level():
+            dual = torch.autograd.forward_ad.make_dual(x(2, 3, 8, dtype=torch.float32).requires_grad_(grad), torch.ones(2, 3, 8))
+            refuses(ValueError, risa.rotate_positions, dual, ints(2), table, match="forward-mode")
+            with torch.no_grad():
+                refuses(ValueError, risa.rotate_positions, dual, ints(2), table, match="forward-mode")
+    # the same tensor without a tangent goes on to the next check
+    refuses(ValueError, risa.rotate_positions, x(2, 3, 8), ints(2), table, match="CUDA device")
