@@ -29,6 +29,10 @@ typedef struct {
   int pages, kv_heads, page_size, head_dim, dtype_code;
 } risa_b200_cache;
 
+/* A row of a page table leads to fewer slots than this: kernels count them in 32 bits and step past
+ * the last one by what a block of threads or a ring of tiles covers. */
+#define RISA_B200_CACHE_MOST_SLOTS (((int64_t)1 << 31) - 8192)
+
 /* One step of a batch.  The tokens of sequence s are rows query_offsets[s] .. query_offsets[s+1]-1
  * of the packed tensors (NULL: row s alone) and the last ones of the lengths[s] tokens that its row
  * of page_table [batch, table_width] leads to.  Entries of the table behind a sequence's length are

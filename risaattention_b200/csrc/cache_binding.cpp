@@ -21,6 +21,7 @@ namespace {
 
 using MaybeTensor = std::optional<at::Tensor>;
 constexpr int kInt8 = 4;
+constexpr int64_t kMostSlots = RISA_B200_CACHE_MOST_SLOTS;
 
 void check(int status) {
   if (status == RISA_B200_INVALID) throw py::value_error(risa_b200_last_error());
@@ -122,7 +123,7 @@ struct Step {
   Step(const Cache& cache, const at::Tensor& table, const at::Tensor& lengths, const MaybeTensor& offsets, int64_t tokens) {
     require(table.dim() == 2 && table.size(0) > 0 && table.size(1) > 0, "page_table must have shape [batch, pages of a sequence]");
     require(table.size(0) <= 65535, "a step takes at most 65535 sequences");
-    require(table.size(1) * cache.c.page_size < (int64_t(1) << 31) - 256, "a sequence may hold fewer than 2^31 keys");
+    require(table.size(1) * cache.c.page_size < kMostSlots, "page_table is too wide: a sequence may hold fewer than 2^31 - 8192 keys");
     require(lengths.dim() == 1 && lengths.size(0) == table.size(0), "lengths must have shape [batch]");
     require(!offsets.has_value() || (offsets->dim() == 1 && offsets->size(0) == table.size(0) + 1), "query_offsets must have shape [batch + 1]");
     require(offsets.has_value() || tokens == table.size(0), "without query_offsets there must be one token for every sequence");
@@ -383,7 +384,7 @@ py::tuple cache_evict(const at::Tensor& cache_keys, const at::Tensor& cache_valu
   require_indices(target, "target_table");
   require(budget > 0 && recent >= 0 && recent <= budget, "budget must be positive and recent between 0 and budget");
   require(target.size(1) * cache.c.page_size >= budget, "the pages of target_table do not hold the budget");
-  require(target.size(1) * cache.c.page_size < (int64_t(1) << 31) - 256, "target_table is too wide");
+  require(target.size(1) * cache.c.page_size < kMostSlots, "target_table is too wide: a sequence may hold fewer than 2^31 - 8192 keys");
   require(target.data_ptr() != table.data_ptr(), "target_table must name other pages than page_table");
   require(weights.device() == cache_keys.device() && target.device() == cache_keys.device(), "weights and target_table must be on the device of the cache");
   require_cuda(cache_keys);

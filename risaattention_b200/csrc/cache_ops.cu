@@ -730,13 +730,13 @@ extern "C" int risa_b200_cache_evict(const risa_b200_cache* cache, const risa_b2
   if (const int bad = check_cache(cache, "evict")) return bad;
   RISA_REQUIRE(step && step->page_table && step->lengths && step->batch > 0 && step->batch <= 65535 && step->table_width > 0,
                "evict: null step, or batch not in 1..65535");
-  RISA_REQUIRE(int64_t(step->table_width) * cache->page_size < (int64_t(1) << 31) - 256,
-               "evict: a sequence may hold fewer than 2^31 keys");
+  RISA_REQUIRE(int64_t(step->table_width) * cache->page_size < RISA_B200_CACHE_MOST_SLOTS,
+               "evict: a sequence may hold fewer than 2^31 - 8192 keys");
   RISA_REQUIRE(weights && target_table && kept && new_lengths && new_weights, "evict: null tensor");
   RISA_REQUIRE(cache->kv_heads <= 65535, "evict: too many heads");
   RISA_REQUIRE(budget > 0 && recent >= 0 && recent <= budget, "evict: budget must be positive and recent in 0..budget");
   RISA_REQUIRE(int64_t(target_width) * cache->page_size >= budget, "evict: the target pages do not hold the budget");
-  RISA_REQUIRE(int64_t(target_width) * cache->page_size < (int64_t(1) << 31) - 256, "evict: the target table is too wide");
+  RISA_REQUIRE(int64_t(target_width) * cache->page_size < RISA_B200_CACHE_MOST_SLOTS, "evict: the target table is too wide");
   RISA_REQUIRE(target_table != step->page_table, "evict: the target pages must not be the sequences' own");
   unsigned int* status = status_word();
   if (status == nullptr) return RISA_B200_CUDA;

@@ -33,8 +33,8 @@ inline int check_step(const risa_b200_step* s, const risa_b200_cache* c, const c
   RISA_REQUIRE(s != nullptr && s->page_table != nullptr && s->lengths != nullptr, "%s: null step", what);
   RISA_REQUIRE(s->batch > 0 && s->batch <= 65535 && s->table_width > 0,
                "%s: batch must be in 1..65535 and the page table must have columns", what);
-  RISA_REQUIRE(int64_t(s->table_width) * c->page_size < (int64_t(1) << 31) - 256,
-               "%s: a sequence may hold fewer than 2^31 keys", what);
+  RISA_REQUIRE(int64_t(s->table_width) * c->page_size < RISA_B200_CACHE_MOST_SLOTS,
+               "%s: a sequence may hold fewer than 2^31 - 8192 keys", what);
   RISA_REQUIRE(s->query_offsets != nullptr || s->tokens == s->batch,
                "%s: without query_offsets every sequence has one token", what);
   RISA_REQUIRE(s->tokens > 0, "%s: no tokens", what);

@@ -212,3 +212,17 @@ def test_rotation_refuses_forward_mode():
                 refuses(ValueError, risa.rotate_positions, dual, ints(2), table, match="forward-mode")
     # the same tensor without a tangent goes on to the next check
     refuses(ValueError, risa.rotate_positions, x(2, 3, 8), ints(2), table, match="CUDA device")
+
+
+def test_tables_that_lead_past_31_bits():
+    """Kernels count a sequence's keys in 32 bits, and step past the last one."""
+    cache = risa.allocate_key_value_cache(1, 1, 128, 64, device="cpu")
+    wide, most = ints(1, 2 ** 24 - 3), 2 ** 24 - 65  # pages of 128 keys: 2^31 - 384 keys, and as many as there may be
+    q, lse, few = x(1, 1, 64), x(1, 1, dtype=torch.float32), ints(1, 1)
+    weights = x(1, 1, 1, dtype=torch.float32)
+    for call, args in ((risa.paged_attention, (q, cache)), (risa.cached_key_weights, (q, lse, cache)), (risa.append_to_cache, (cache, q, q))):
+        refuses(ValueError, call, *args, wide, ints(1), match="2\\^31 - 8192")
+        refuses(ValueError, call, *args, wide[:, :most], ints(1), match="CUDA device")
+    refuses(ValueError, risa.evict_from_cache, cache, wide, ints(1), weights, few, budget=8, match="2\\^31 - 8192")
+    refuses(ValueError, risa.evict_from_cache, cache, few, ints(1), x(1, 1, 128, dtype=torch.float32), wide, budget=8, match="2\\^31 - 8192")
+    refuses(ValueError, risa.evict_from_cache, cache, few, ints(1), x(1, 1, 128, dtype=torch.float32), wide[:, :most], budget=8, match="CUDA device")
