@@ -672,6 +672,7 @@ extern "C" int risa_b200_cache_append(const risa_b200_cache* cache, const risa_b
   RISA_REQUIRE(dtype_code == 1 || dtype_code == 2, "append: q, k and v must be float16 or bfloat16");
   RISA_REQUIRE(codes || dtype_code == cache->dtype_code, "append: k and v must have the cache's type");
   RISA_REQUIRE(q == nullptr || rotary != nullptr, "append: q is only rotated, and there is no rotary table");
+  RISA_REQUIRE(q == nullptr || q_heads > 0, "append: q needs heads");
   if (rotary != nullptr) {
     if (const int bad = check_rotary(rotary, cache->head_dim, "append")) return bad;
     RISA_REQUIRE(rotary->rotary_dim % 16 == 0, "append: rotary_dim must be a multiple of 16");

@@ -689,7 +689,7 @@ int check_queries(const risa_b200_cache* cache, const risa_b200_step* step, cons
   RISA_REQUIRE(cache->dtype_code == kInt8 || cache->dtype_code == dtype_code, "%s: q must have the cache's type", what);
   RISA_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && qs[0] % 8 == 0 && qs[1] % 8 == 0,
                "%s: query rows must start on 16-byte boundaries", what);
-  RISA_REQUIRE(scale == scale && fabsf(scale) < INFINITY, "%s: the scale must be finite", what);
+  RISA_REQUIRE(fabsf(scale * kLog2e) < INFINITY, "%s: the scale must be finite, also in units of log 2", what);
   RISA_REQUIRE(window >= 0 && (window == 0 || is_causal), "%s: a window needs the causal rule and at least one key", what);
   RISA_REQUIRE(int64_t(step->tokens) * (q_heads / cache->kv_heads) < (int64_t(1) << 31) - 1024, "%s: too many query rows", what);
   return RISA_B200_OK;

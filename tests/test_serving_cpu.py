@@ -226,3 +226,29 @@ def test_tables_that_lead_past_31_bits():
     refuses(ValueError, risa.evict_from_cache, cache, wide, ints(1), weights, few, budget=8, match="2\\^31 - 8192")
     refuses(ValueError, risa.evict_from_cache, cache, few, ints(1), x(1, 1, 128, dtype=torch.float32), wide, budget=8, match="2\\^31 - 8192")
     refuses(ValueError, risa.evict_from_cache, cache, few, ints(1), x(1, 1, 128, dtype=torch.float32), wide[:, :most], budget=8, match="CUDA device")
+
+
+def test_c_entries_check_heads_and_scale():
+    """What the module's own checks let through or never produce; nothing is read: the addresses are aligned numbers."""
+    lib = ctypes.CDLL(str(ROOT / "risaattention_b200" / "librisa_b200.so"))
+    lib.risa_b200_last_error.restype = ctypes.c_char_p
+
+    class Cache(ctypes.Structure):
+        _fields_ = [(n, ctypes.c_void_p) for n in ("keys", "values", "key_scales", "value_scales")] + [(n, ctypes.c_int) for n in ("pages", "kv_heads", "page_size", "head_dim", "dtype_code")]
+
+    class Step(ctypes.Structure):
+        _fields_ = [(n, ctypes.c_void_p) for n in ("page_table", "lengths", "query_offsets")] + [(n, ctypes.c_int) for n in ("batch", "table_width", "tokens")]
+
+    class Rotary(ctypes.Structure):
+        _fields_ = [("turns", ctypes.c_void_p), ("rotary_dim", ctypes.c_int), ("magnitude", ctypes.c_float), ("interleaved", ctypes.c_int)]
+
+    at, strides = ctypes.c_void_p(4096), (ctypes.c_int64 * 2)(512, 128)
+    cache, step, rotary = Cache(4096, 4096, None, None, 8, 2, 16, 128, 2), Step(4096, 4096, None, 1, 8, 1), Rotary(4096, 128, 1.0, 0)
+    invalid = int(re.search(r"RISA_B200_INVALID (\d+)", (ROOT / "include" / "risa_b200.h").read_text())[1])
+    for heads in (0, -4):
+        assert lib.risa_b200_cache_append(ctypes.byref(cache), ctypes.byref(step), at, strides, at, strides, at, strides, at, strides, heads, 2, ctypes.byref(rotary), None, 0, None) == invalid
+        assert b"heads" in lib.risa_b200_last_error()
+    for scale in (3e38, math.inf, math.nan):  # 3e38 is finite, and in units of log 2 it is not
+        assert lib.risa_b200_paged_attention(ctypes.byref(cache), ctypes.byref(step), at, strides, 4, 2, at, strides, at, ctypes.c_float(scale), 1, 0, 3, at, ctypes.c_size_t(1 << 30), None) == invalid
+        assert b"scale" in lib.risa_b200_last_error()
+        assert lib.risa_b200_key_weights(ctypes.byref(cache), ctypes.byref(step), at, strides, 4, 2, at, ctypes.c_float(scale), 1, 0, None, at, at, ctypes.c_size_t(1 << 30), None) == invalid
