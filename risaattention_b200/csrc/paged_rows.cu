@@ -13,7 +13,7 @@
 // scores s but of s + log2(scale): what is rounded is at most 1, and exact relative to the largest contribution.
 //
 // Measured: 16 requests of up to 16K keys, 8 key heads of 128 bf16 channels, 110 us (6.1 TB/s, 95 % of a plain copy's rate);
-// 32 requests of up to 32K keys as codes 246 us at full clocks (5.6 TB/s), 282 in long runs, where the conversion's
+// 32 requests of up to 32K keys as codes 244 us at full clocks (5.7 TB/s), 280 in long runs, where the conversion's
 // instructions (schedulers 61 % busy) feel the lower clock.
 #include "paged_tc.cuh"
 #include "serving_plan.cuh"
