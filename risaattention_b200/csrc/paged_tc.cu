@@ -11,8 +11,8 @@
 // What bounds it: per tile and group the tensor pipe works 1024 clocks (head_dim 128) and the special-function unit 1024;
 // the chain of a group's softmax (2100: load, maxima with an exchange, exponentials, store) and products (1450) is hidden
 // by the other group's to about one half, so a tile of both takes 3850.  2048 tokens over 32K keys, 32 heads of 128 channels:
-// 1.16 ms, 916 TFLOP/s, at the clock that the power limit leaves.  One thread for a row: the same; an issue warp per group let the groups fall
-// into step (5500 clocks a tile); half of the next scores ahead of P V (N = 64 products) 4600; K and V by 128 copying threads
+// 1.16 ms, 916 TFLOP/s, at the clock that the power limit leaves.  One thread for a row: the same; an issue warp per group let
+// the groups fall into step (5500 clocks a tile); half of the next scores ahead of P V (N = 64 products) 4600; K and V by 128 copying threads
 // instead of TMA 6300; exponentials from the maximum as it stood, redone where it had moved, ran out of registers (5600).
 //
 // Heads of 256 channels leave room for the outputs of 128 rows only.  There the two groups have the same rows and half of

@@ -6,8 +6,9 @@
 // thread that owns a key adds up its row of exponentials in a register.  K is read once, nothing is written but the
 // weights.  What bounds it is the exponentials: one per (key, row) and 16 per clock and SM, 2048 clocks for 256 keys x
 // 128 rows, against 1024 of the matrix instruction at 128 channels.  A tile takes 2550; 1024 tokens over 8K keys, 32 heads:
-// 108 us in short runs (117 with the clock of long ones), of which ~10 are start-up; 16 tokens over 4 x 16K keys of 64 channels: 48.  Exponentials by polynomial on the FP32 pipes for an eighth to three eighths of them
-// cost as much issue time as they saved.
+// 108 us in short runs (117 with the clock of long ones), of which ~10 are start-up; 16 tokens over 4 x 16K keys of 64
+// channels: 48.  Exponentials by polynomial on the FP32 pipes for an eighth to three eighths of them cost as much issue time
+// as they saved.
 //
 // Warps 0-15: the sums, four warpgroups: two for each group of keys, each with half of a tile's rows (four warps a
 // scheduler hide the latencies of tensor memory and the exponential; two left a third of the time idle).  16-19: fetch
