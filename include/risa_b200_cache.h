@@ -55,6 +55,16 @@ typedef struct {
   int interleaved;
 } risa_b200_rotary;
 
+/* Positions of several axes (time, height, width): pair i follows axis axes[i] (bytes on the device;
+ * those from `count` on count as the last axis), whose positions lie `position_stride` elements
+ * behind those of the axis before it (0: all axes have the same).  count: 1 to 8. */
+typedef struct {
+  const uint8_t* axes;
+  int count;
+  int64_t position_stride;
+} risa_b200_rotary_axes;
+#define RISA_B200_MOST_AXES 8
+
 /* out = x with every [batch, heads, tokens] row of head_dim channels rotated by its position, or by
  * the transposed rotation (the gradient).  out may be x.  positions: int32 or int64 at
  * b * position_stride_b + n * position_stride_n.  Strides of the channel axis are 1. */
@@ -63,6 +73,12 @@ int risa_b200_rotate(const void* x, void* out, int dtype_code, int batch, int he
                      const void* positions, int positions_64, int64_t position_stride_b,
                      int64_t position_stride_n, const risa_b200_rotary* rotary, int transposed,
                      void* stream);
+/* The same by positions of several axes (NULL: of one). */
+int risa_b200_rotate_axes(const void* x, void* out, int dtype_code, int batch, int heads, int tokens,
+                          int head_dim, const int64_t x_strides[3], const int64_t out_strides[3],
+                          const void* positions, int positions_64, int64_t position_stride_b,
+                          int64_t position_stride_n, const risa_b200_rotary* rotary,
+                          const risa_b200_rotary_axes* axes, int transposed, void* stream);
 
 /* Writes one step's keys and values [tokens, kv_heads, head_dim] to their pages, the keys rotated
  * where rotary is given (its angle: positions[token], or the token's place in the cache where
@@ -74,6 +90,15 @@ int risa_b200_cache_append(const risa_b200_cache* cache, const risa_b200_step* s
                            const int64_t q_out_strides[2], int q_heads, int dtype_code,
                            const risa_b200_rotary* rotary, const void* positions, int positions_64,
                            void* stream);
+/* The same by positions of several axes (NULL: of one); without positions every axis has the token's
+ * place in the cache. */
+int risa_b200_cache_append_axes(const risa_b200_cache* cache, const risa_b200_step* step,
+                                const void* k, const int64_t k_strides[2], const void* v,
+                                const int64_t v_strides[2], const void* q,
+                                const int64_t q_strides[2], void* q_out,
+                                const int64_t q_out_strides[2], int q_heads, int dtype_code,
+                                const risa_b200_rotary* rotary, const risa_b200_rotary_axes* axes,
+                                const void* positions, int positions_64, void* stream);
 
 /* softmax(scale * q K^T) V of every packed token over its sequence's cached keys; with is_causal the
  * token at place p of its sequence sees keys max(0, p - window + 1) .. p (window 0: from the start),
@@ -87,6 +112,14 @@ int risa_b200_paged_attention(const risa_b200_cache* cache, const risa_b200_step
                               int dtype_code, void* out, const int64_t out_strides[2], float* lse,
                               float scale, int is_causal, int window, int clear_rest,
                               void* scratch, size_t scratch_bytes, void* stream);
+/* With a window, keys 0 .. sinks-1 of the sequence stay visible in front of it (those up to the
+ * token's own place). */
+int risa_b200_paged_attention_sinks(const risa_b200_cache* cache, const risa_b200_step* step,
+                                    const void* q, const int64_t q_strides[2], int q_heads,
+                                    int dtype_code, void* out, const int64_t out_strides[2],
+                                    float* lse, float scale, int is_causal, int window, int sinks,
+                                    int clear_rest, void* scratch, size_t scratch_bytes,
+                                    void* stream);
 
 /* weights[b, h, j] = previous[b, h, j] + sum over the sequence's new tokens and the query heads of
  * key head h of exp(scale * q . k_j - lse): the attention that key j received.  weights, previous
@@ -99,6 +132,11 @@ int risa_b200_key_weights(const risa_b200_cache* cache, const risa_b200_step* st
                           const float* lse, float scale, int is_causal, int window,
                           const float* previous, float* weights, void* scratch,
                           size_t scratch_bytes, void* stream);
+int risa_b200_key_weights_sinks(const risa_b200_cache* cache, const risa_b200_step* step,
+                                const void* q, const int64_t q_strides[2], int q_heads,
+                                int dtype_code, const float* lse, float scale, int is_causal,
+                                int window, int sinks, const float* previous, float* weights,
+                                void* scratch, size_t scratch_bytes, void* stream);
 
 /* Keeps min(length, budget) tokens of every (sequence, key head): the `recent` last ones and those of
  * the largest weights among the others (equal weights: lowest index first; NaN counts as largest),

@@ -159,6 +159,30 @@ struct Rotary {
   }
 };
 
+// The axes that a table's pairs follow, and from one axis' positions to the next one's: `positions` has the axes in front of the
+// `plain` dimensions that one axis has, or only those (all axes alike).
+struct Axes {
+  std::optional<risa_b200_rotary_axes> r;
+  at::Tensor positions;  // of the first axis
+  Axes(const MaybeTensor& axes, int64_t count, const at::Tensor& turns, const at::Tensor& all, int64_t plain) : positions(all) {
+    if (!axes.has_value()) return;
+    require_type(axes->scalar_type() == at::kByte && axes->is_contiguous(), "the axes of a rotary table must be contiguous uint8");
+    require(axes->dim() == 1 && axes->size(0) == turns.size(0), "a rotary table needs an axis for each pair");
+    require(count >= 1 && count <= RISA_B200_MOST_AXES, "a rotary table follows 1 to 8 axes");
+    require(axes->device() == turns.device(), "turns and axes of a rotary table must be on the same device");
+    r.emplace();
+    r->axes = axes->data_ptr<uint8_t>();
+    r->count = int(count);
+    r->position_stride = 0;
+    if (all.defined() && all.dim() == plain + 1) {
+      require(all.size(0) == count, "positions must have a row for each of the table's axes");
+      r->position_stride = count == 1 ? 0 : all.stride(0);
+      positions = all.select(0, 0);
+    }
+  }
+  const risa_b200_rotary_axes* get() const { return r.has_value() ? &*r : nullptr; }
+};
+
 void require_positions(const at::Tensor& p) {
   require_type(p.scalar_type() == at::kInt || p.scalar_type() == at::kLong, "positions must be int32 or int64");
 }
@@ -170,18 +194,23 @@ void require_no_tangent(const at::Tensor& x) {
 }
 
 // x [tokens, heads, head_dim] with positions [tokens], or [batch, heads, tokens, head_dim] with positions
-// [tokens] or [batch, tokens].
-at::Tensor rotate(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& turns, double magnitude, bool interleaved,
-                  bool transposed, const MaybeTensor& out_given, uintptr_t stream_ptr) {
+// [tokens] or [batch, tokens]; a table of several axes takes [tokens] for all of them, or theirs in front of the same.
+at::Tensor rotate(const at::Tensor& x, const at::Tensor& all_positions, const at::Tensor& turns, const MaybeTensor& axes_of_pairs,
+                  int64_t axis_count, double magnitude, bool interleaved, bool transposed, const MaybeTensor& out_given,
+                  uintptr_t stream_ptr) {
   require_no_tangent(x);
   require(x.dim() == 3 || x.dim() == 4, "x must have shape [tokens, heads, head_dim] or [batch, heads, tokens, head_dim]");
   const bool packed = x.dim() == 3;
   const int64_t batch = packed ? 1 : x.size(0), heads = x.size(1), tokens = packed ? x.size(0) : x.size(2), d = x.size(-1);
   require(batch > 0 && heads > 0 && tokens > 0 && d > 0, "x must not be empty");
   require(batch <= 65535 && heads <= 65535 && tokens < (int64_t(1) << 31) && d <= 65536, "x is too large");
+  // [axes, tokens], not [batch, tokens], where the table has axes
+  const Axes axes(axes_of_pairs, axis_count, turns, all_positions, all_positions.dim() - (all_positions.dim() > 1));
+  const at::Tensor& positions = axes.positions;
   require((positions.dim() == 1 && positions.size(0) == tokens) ||
               (!packed && positions.dim() == 2 && positions.size(0) == batch && positions.size(1) == tokens),
-          "positions must have shape [tokens] or, for x of four dimensions, [batch, tokens]");
+          axes.get() ? "positions must have shape [tokens], [axes, tokens] or, for x of four dimensions, [axes, batch, tokens]"
+                     : "positions must have shape [tokens] or, for x of four dimensions, [batch, tokens]");
   const int code = code_of(x);
   require_type(code >= 0 && code <= 2, "x must be float32, float16 or bfloat16");
   require_positions(positions);
@@ -206,9 +235,9 @@ at::Tensor rotate(const at::Tensor& x, const at::Tensor& positions, const at::Te
   int64_t xs[3], os[3];
   strides(x, xs);
   strides(out, os);
-  check(risa_b200_rotate(x.data_ptr(), out.data_ptr(), code, int(batch), int(heads), int(tokens), int(d), xs, os, positions.data_ptr(),
-                         positions.scalar_type() == at::kLong, positions.dim() == 2 ? positions.stride(0) : 0, positions.stride(-1),
-                         &rotary.r, transposed ? 1 : 0, stream_of(stream_ptr)));
+  check(risa_b200_rotate_axes(x.data_ptr(), out.data_ptr(), code, int(batch), int(heads), int(tokens), int(d), xs, os, positions.data_ptr(),
+                              positions.scalar_type() == at::kLong, positions.dim() == 2 ? positions.stride(0) : 0, positions.stride(-1),
+                              &rotary.r, axes.get(), transposed ? 1 : 0, stream_of(stream_ptr)));
   return out;
 }
 
@@ -221,40 +250,45 @@ struct Rotation : public torch::autograd::Function<Rotation> {
     return reinterpret_cast<uintptr_t>(devices.getStream(device).native_handle());
   }
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x, const at::Tensor& positions, const at::Tensor& turns,
-                            double magnitude, bool interleaved, bool transposed) {
-    ctx->save_for_backward({positions, turns});
+                            const MaybeTensor& axes, int64_t axis_count, double magnitude, bool interleaved, bool transposed) {
+    ctx->save_for_backward({positions, turns, axes.has_value() ? *axes : at::Tensor()});
+    ctx->saved_data["axis_count"] = axis_count;
     ctx->saved_data["magnitude"] = magnitude;
     ctx->saved_data["interleaved"] = interleaved;
     ctx->saved_data["transposed"] = transposed;
-    return rotate(x, positions, turns, magnitude, interleaved, transposed, std::nullopt, x.is_cuda() ? stream_on(x.device()) : 0);
+    return rotate(x, positions, turns, axes, axis_count, magnitude, interleaved, transposed, std::nullopt, x.is_cuda() ? stream_on(x.device()) : 0);
   }
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     // gradients of sums and broadcasts arrive as expanded views
     const at::Tensor grad = grads[0].stride(-1) == 1 ? grads[0] : grads[0].contiguous();
-    return {Rotation::apply(grad, saved[0], saved[1], ctx->saved_data["magnitude"].toDouble(), ctx->saved_data["interleaved"].toBool(),
-                            !ctx->saved_data["transposed"].toBool()),
-            at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
+    const MaybeTensor axes = saved[2].defined() ? MaybeTensor(saved[2]) : std::nullopt;
+    return {Rotation::apply(grad, saved[0], saved[1], axes, ctx->saved_data["axis_count"].toInt(), ctx->saved_data["magnitude"].toDouble(),
+                            ctx->saved_data["interleaved"].toBool(), !ctx->saved_data["transposed"].toBool()),
+            at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor(), at::Tensor()};
   }
 };
-at::Tensor rotate_with_gradient(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& turns, double magnitude, bool interleaved,
-                                bool transposed) {
+at::Tensor rotate_with_gradient(const at::Tensor& x, const at::Tensor& positions, const at::Tensor& turns, const MaybeTensor& axes,
+                                int64_t axis_count, double magnitude, bool interleaved, bool transposed) {
   require_no_tangent(x);
-  return Rotation::apply(x, positions, turns, magnitude, interleaved, transposed);
+  return Rotation::apply(x, positions, turns, axes, axis_count, magnitude, interleaved, transposed);
 }
 
 // Writes k and v [tokens, kv_heads, head_dim]; returns q rotated, or None.
 MaybeTensor cache_append(const at::Tensor& cache_keys, const at::Tensor& cache_values, const MaybeTensor& key_scales,
                          const MaybeTensor& value_scales, const at::Tensor& k, const at::Tensor& v, const at::Tensor& table,
                          const at::Tensor& lengths, const MaybeTensor& offsets, const MaybeTensor& q, const MaybeTensor& turns,
-                         double magnitude, bool interleaved, const MaybeTensor& positions, uintptr_t stream_ptr) {
+                         const MaybeTensor& axes_of_pairs, int64_t axis_count, double magnitude, bool interleaved,
+                         const MaybeTensor& positions, uintptr_t stream_ptr) {
   const Cache cache(cache_keys, cache_values, key_scales, value_scales);
   const int64_t heads = cache.c.kv_heads, d = cache.c.head_dim;
   require(k.dim() == 3 && k.size(1) == heads && k.size(2) == d && v.sizes() == k.sizes(), "k and v must have shape [tokens, kv_heads, head_dim] of the cache");
   const int64_t tokens = k.size(0);
   require(!q.has_value() || (q->dim() == 3 && q->size(0) == tokens && q->size(1) > 0 && q->size(2) == d), "q must have shape [tokens, q_heads, head_dim]");
   require(!q.has_value() || turns.has_value(), "q is only rotated: it needs a rotary table");
-  require(!positions.has_value() || (positions->dim() == 1 && positions->size(0) == tokens), "positions must have shape [tokens]");
+  require(!positions.has_value() || (positions->dim() == 1 && positions->size(0) == tokens) ||
+              (axes_of_pairs.has_value() && positions->dim() == 2 && positions->size(1) == tokens),
+          axes_of_pairs.has_value() ? "positions must have shape [tokens] or [axes, tokens]" : "positions must have shape [tokens]");
   require(!positions.has_value() || turns.has_value(), "positions need a rotary table");
   const int code = code_of(k);
   require_type(code == 1 || code == 2, "k and v must be float16 or bfloat16");
@@ -270,7 +304,9 @@ MaybeTensor cache_append(const at::Tensor& cache_keys, const at::Tensor& cache_v
               (!positions.has_value() || positions->device() == device),
           "q, k, v and positions must be on the device of the cache");
   std::optional<Rotary> rotary;
+  std::optional<Axes> axes;
   if (turns.has_value()) {
+    axes.emplace(axes_of_pairs, axis_count, *turns, positions.has_value() ? *positions : at::Tensor(), 1);
     rotary.emplace(*turns, magnitude, interleaved, d, device);
     require(rotary->r.rotary_dim % 16 == 0, "appending needs a rotary_dim that is a multiple of 16");
   }
@@ -286,32 +322,34 @@ MaybeTensor cache_append(const at::Tensor& cache_keys, const at::Tensor& cache_v
     qs.emplace(*qr);
     os.emplace(*out);
   }
-  check(risa_b200_cache_append(&cache.c, &step.s, kr.data_ptr(), ks.of, vr.data_ptr(), vs.of, qr.has_value() ? qr->data_ptr() : nullptr,
+  check(risa_b200_cache_append_axes(&cache.c, &step.s, kr.data_ptr(), ks.of, vr.data_ptr(), vs.of, qr.has_value() ? qr->data_ptr() : nullptr,
                                qs.has_value() ? qs->of : nullptr, out.has_value() ? out->data_ptr() : nullptr,
                                os.has_value() ? os->of : nullptr, q.has_value() ? int(q->size(1)) : 0, code,
-                               rotary.has_value() ? &rotary->r : nullptr, positions.has_value() ? positions->data_ptr() : nullptr,
+                               rotary.has_value() ? &rotary->r : nullptr, rotary.has_value() ? axes->get() : nullptr, positions.has_value() ? positions->data_ptr() : nullptr,
                                positions.has_value() && positions->scalar_type() == at::kLong, stream_of(stream_ptr)));
   return out;
 }
 
 // Checks that attention and key weights share.
-void check_queries(const Cache& cache, const at::Tensor& q, const std::optional<int64_t>& window, bool is_causal) {
+void check_queries(const Cache& cache, const at::Tensor& q, const std::optional<int64_t>& window, int64_t sinks, bool is_causal) {
   require(q.dim() == 3 && q.size(2) == cache.c.head_dim, "q must have shape [tokens, q_heads, head_dim of the cache]");
   require(q.size(1) > 0 && q.size(1) % cache.c.kv_heads == 0,
           "q head count (" + std::to_string(q.size(1)) + ") must be divisible by the cache's head count (" + std::to_string(cache.c.kv_heads) + ")");
   require(q.size(0) < ((int64_t(1) << 31) - 1024) / (q.size(1) / cache.c.kv_heads), "q has too many rows");
   require(!window.has_value() || (*window > 0 && *window < (int64_t(1) << 31)), "window must be positive");
   require(!window.has_value() || is_causal, "a window needs the causal rule");
+  require(sinks >= 0 && sinks < (int64_t(1) << 31), "sinks must not be negative");
+  require(sinks == 0 || window.has_value(), "sinks stay visible in front of a window, and there is none");
   require_type(code_of(q) == 1 || code_of(q) == 2, "q must be float16 or bfloat16");
   require_type(cache.c.dtype_code == kInt8 || cache.c.dtype_code == code_of(q), "q must have the dtype of the cache");
 }
 
 py::tuple paged_attention(const at::Tensor& q, const at::Tensor& cache_keys, const at::Tensor& cache_values, const MaybeTensor& key_scales,
                           const MaybeTensor& value_scales, const at::Tensor& table, const at::Tensor& lengths, const MaybeTensor& offsets,
-                          double scale, bool is_causal, std::optional<int64_t> window, bool return_lse, const MaybeTensor& out_given,
+                          double scale, bool is_causal, std::optional<int64_t> window, int64_t sinks, bool return_lse, const MaybeTensor& out_given,
                           uintptr_t stream_ptr) {
   const Cache cache(cache_keys, cache_values, key_scales, value_scales);
-  check_queries(cache, q, window, is_causal);
+  check_queries(cache, q, window, sinks, is_causal);
   if (out_given.has_value()) {
     require(out_given->sizes() == q.sizes() && out_given->stride(2) == 1 && (q.size(0) <= 1 || out_given->stride(0) % 8 == 0) &&
                 (q.size(1) <= 1 || out_given->stride(1) % 8 == 0),
@@ -331,19 +369,19 @@ py::tuple paged_attention(const at::Tensor& q, const at::Tensor& cache_keys, con
   const size_t bytes = risa_b200_paged_attention_scratch_size(&cache.c, &step.s, int(q.size(1)));
   const at::Tensor scratch = at::empty({int64_t(bytes)}, q.options().dtype(at::kByte));
   const Strides2 qs(qr), os(out);
-  check(risa_b200_paged_attention(&cache.c, &step.s, qr.data_ptr(), qs.of, int(q.size(1)), code_of(q), out.data_ptr(), os.of,
+  check(risa_b200_paged_attention_sinks(&cache.c, &step.s, qr.data_ptr(), qs.of, int(q.size(1)), code_of(q), out.data_ptr(), os.of,
                                   return_lse ? lse->data_ptr<float>() : nullptr, float(scale), is_causal ? 1 : 0,
-                                  window.has_value() ? int(*window) : 0, out_given.has_value() ? 2 : 3, scratch.data_ptr(), bytes,
+                                  window.has_value() ? int(*window) : 0, int(sinks), out_given.has_value() ? 2 : 3, scratch.data_ptr(), bytes,
                                   stream_of(stream_ptr)));
   return py::make_tuple(out, lse);
 }
 
 at::Tensor key_weights(const at::Tensor& q, const at::Tensor& lse, const at::Tensor& cache_keys, const at::Tensor& cache_values,
                        const MaybeTensor& key_scales, const MaybeTensor& value_scales, const at::Tensor& table, const at::Tensor& lengths,
-                       const MaybeTensor& offsets, double scale, bool is_causal, std::optional<int64_t> window, const MaybeTensor& previous,
+                       const MaybeTensor& offsets, double scale, bool is_causal, std::optional<int64_t> window, int64_t sinks, const MaybeTensor& previous,
                        uintptr_t stream_ptr) {
   const Cache cache(cache_keys, cache_values, key_scales, value_scales);
-  check_queries(cache, q, window, is_causal);
+  check_queries(cache, q, window, sinks, is_causal);
   require(lse.dim() == 2 && lse.size(0) == q.size(0) && lse.size(1) == q.size(1), "lse must have shape [tokens, q_heads]");
   require_type(lse.scalar_type() == at::kFloat, "lse must be float32");
   const Step step(cache, table, lengths, offsets, q.size(0));
@@ -364,8 +402,8 @@ at::Tensor key_weights(const at::Tensor& q, const at::Tensor& lse, const at::Ten
   MaybeTensor scratch;
   if (bytes) scratch = at::empty({int64_t(bytes)}, q.options().dtype(at::kByte));
   const Strides2 qs(qr);
-  check(risa_b200_key_weights(&cache.c, &step.s, qr.data_ptr(), qs.of, int(q.size(1)), code_of(q), rows.data_ptr<float>(), float(scale),
-                              is_causal ? 1 : 0, window.has_value() ? int(*window) : 0,
+  check(risa_b200_key_weights_sinks(&cache.c, &step.s, qr.data_ptr(), qs.of, int(q.size(1)), code_of(q), rows.data_ptr<float>(), float(scale),
+                              is_causal ? 1 : 0, window.has_value() ? int(*window) : 0, int(sinks),
                               previous.has_value() ? previous->data_ptr<float>() : nullptr, weights.data_ptr<float>(),
                               bytes ? scratch->data_ptr() : nullptr, bytes, stream_of(stream_ptr)));
   return weights;

@@ -112,6 +112,9 @@ struct RotateArgs {
   int batch, heads, tokens, head_dim, rotary_dim, heads_each, chunks;
   int positions_64, interleaved, transposed;
   float magnitude;
+  const uint8_t* axes;  // of the pairs, nullptr: all follow one axis
+  int64_t pa;           // from one axis' positions to the next one's
+  int last_axis;
 };
 
 // A thread owns eight pairs of one token (two runs of eight channels) in `heads_each` heads, so that
@@ -119,8 +122,9 @@ struct RotateArgs {
 // channels each.  Consecutive threads are consecutive runs of a row, then rows of consecutive tokens.  Bound by HBM: the
 // loads of four heads are on their way at once (2 x 16 heads x 16K tokens of 128 bf16 channels, half of them rotated: 78 us
 // with two, 57 with four, 4.7 TB/s).
+// With positions of several axes each of the eight pairs looks up its own (the same few cache lines).
 constexpr int kHeadsAhead = 4;
-template <typename T>
+template <typename T, bool AXES>
 __global__ __launch_bounds__(256, 4) void rotate_kernel(const RotateArgs a) {
   chain_wait();
   chain_release();
@@ -145,10 +149,14 @@ __global__ __launch_bounds__(256, 4) void rotate_kernel(const RotateArgs a) {
     }
     return;
   }
-  const int64_t position = position_at(a.positions, a.positions_64, b * a.pb + token * a.pn);
+  const int64_t at = b * a.pb + token * a.pn;
+  int64_t position = AXES ? 0 : position_at(a.positions, a.positions_64, at);
+  uint2 axes = make_uint2(0, 0);
+  if (AXES) axes = __ldg(reinterpret_cast<const uint2*>(a.axes) + item);
   float cs[8], sn[8];
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
+    if (AXES) position = position_at(a.positions, a.positions_64, at + min(int((i < 4 ? axes.x : axes.y) >> (8 * (i & 3)) & 0xff), a.last_axis) * a.pa);
     angle_of(position, __ldg(reinterpret_cast<const unsigned long long*>(a.turns) + item * 8 + i), a.magnitude, cs[i], sn[i]);
     if (a.transposed) sn[i] = -sn[i];
   }
@@ -219,7 +227,8 @@ __global__ __launch_bounds__(256) void rotate_any_kernel(const RotateArgs a) {
     for (int h = h0; h < h1; ++h) out[h * a.oh + c] = x[h * a.xh + c];
     return;
   }
-  const int64_t position = position_at(a.positions, a.positions_64, b * a.pb + token * a.pn);
+  const int64_t axis = a.axes != nullptr ? min(int(__ldg(a.axes + item)), a.last_axis) * a.pa : 0;
+  const int64_t position = position_at(a.positions, a.positions_64, b * a.pb + token * a.pn + axis);
   float c, s;
   angle_of(position, __ldg(reinterpret_cast<const unsigned long long*>(a.turns) + item), a.magnitude, c, s);
   if (a.transposed) s = -s;
@@ -246,6 +255,9 @@ struct AppendArgs {
   const void* positions;
   int rotary_dim, interleaved, positions_64;
   float magnitude;
+  const uint8_t* axes;  // of the pairs, nullptr: all follow one axis
+  int64_t axis_stride;
+  int last_axis;
   unsigned int* status;
 };
 
@@ -326,10 +338,12 @@ __global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
   float cs[8] = {}, sn[8] = {};
   int partner = threadIdx.x & 31;
   if (a.turns != nullptr) {  // one thread for each pair of the token, then every lane takes those of its channels
-    const int64_t position = a.positions ? position_at(a.positions, a.positions_64, token) : int64_t(place);
     const int half = a.rotary_dim >> 1;
-    if (int(threadIdx.x) < half)
+    if (int(threadIdx.x) < half) {
+      const int64_t axis = a.axes != nullptr ? min(int(__ldg(a.axes + threadIdx.x)), a.last_axis) * a.axis_stride : 0;
+      const int64_t position = a.positions ? position_at(a.positions, a.positions_64, token + axis) : int64_t(place);
       angle_of(position, __ldg(reinterpret_cast<const unsigned long long*>(a.turns) + threadIdx.x), a.magnitude, cosines[threadIdx.x], sines[threadIdx.x]);
+    }
     __syncthreads();
     if (turned) {
       const bool second = !a.interleaved && channel >= half;
@@ -620,6 +634,11 @@ int check_rotary(const risa_b200_rotary* r, int head_dim, const char* what) {
                "%s: rotary_dim must be even and at most head_dim", what);
   return RISA_B200_OK;
 }
+int check_axes(const risa_b200_rotary_axes* a, const char* what) {
+  RISA_REQUIRE(a == nullptr || (a->axes != nullptr && a->count >= 1 && a->count <= RISA_B200_MOST_AXES),
+               "%s: a rotary table follows 1 to 8 axes", what);
+  return RISA_B200_OK;
+}
 
 }  // namespace
 }  // namespace serving
@@ -632,21 +651,32 @@ extern "C" int risa_b200_rotate(const void* x, void* out, int dtype_code, int ba
                                 int tokens, int head_dim, const int64_t xs[3], const int64_t os[3],
                                 const void* positions, int positions_64, int64_t position_stride_b,
                                 int64_t position_stride_n, const risa_b200_rotary* rotary,
-                                int transposed, void* stream_ptr) {
+                                int transposed, void* stream) {
+  return risa_b200_rotate_axes(x, out, dtype_code, batch, heads, tokens, head_dim, xs, os, positions, positions_64, position_stride_b,
+                               position_stride_n, rotary, nullptr, transposed, stream);
+}
+
+extern "C" int risa_b200_rotate_axes(const void* x, void* out, int dtype_code, int batch, int heads,
+                                     int tokens, int head_dim, const int64_t xs[3], const int64_t os[3],
+                                     const void* positions, int positions_64, int64_t position_stride_b,
+                                     int64_t position_stride_n, const risa_b200_rotary* rotary,
+                                     const risa_b200_rotary_axes* axes, int transposed, void* stream_ptr) {
   RISA_REQUIRE(x && out && positions && rotary, "rotate: null tensor");
   RISA_REQUIRE(dtype_code >= 0 && dtype_code <= 2, "rotate: dtype must be float32, float16 or bfloat16");
   RISA_REQUIRE(batch > 0 && batch <= 65535 && heads > 0 && heads <= 65535 && tokens > 0 && head_dim > 0,
                "rotate: sizes must be positive, batch and heads at most 65535");
   if (const int bad = check_rotary(rotary, head_dim, "rotate")) return bad;
+  if (const int bad = check_axes(axes, "rotate")) return bad;
   RotateArgs a{x, out, positions, rotary->turns, xs[0], xs[1], xs[2], os[0], os[1], os[2],
                position_stride_b, position_stride_n, batch, heads, tokens, head_dim,
                rotary->rotary_dim, 1, 1, positions_64, rotary->interleaved, transposed,
-               rotary->magnitude};
+               rotary->magnitude, axes ? axes->axes : nullptr, axes ? axes->position_stride : 0, axes ? axes->count - 1 : 0};
   // eight channels at a time where every run starts on a 16-byte boundary
   const int64_t size = dtype_code == 0 ? 4 : 2;
   bool wide = rotary->rotary_dim % 16 == 0 && head_dim % 8 == 0 &&
               (reinterpret_cast<uintptr_t>(x) | reinterpret_cast<uintptr_t>(out)) % 16 == 0;
   for (int i = 0; i < 3; ++i) wide = wide && xs[i] * size % 16 == 0 && os[i] * size % 16 == 0;
+  wide = wide && reinterpret_cast<uintptr_t>(a.axes) % 8 == 0;
   const int items = wide ? rotary->rotary_dim / 16 + (head_dim - rotary->rotary_dim) / 8
                          : rotary->rotary_dim / 2 + head_dim - rotary->rotary_dim;
   const int64_t threads = int64_t(tokens) * items;
@@ -655,7 +685,7 @@ extern "C" int risa_b200_rotate(const void* x, void* out, int dtype_code, int ba
   while (a.heads_each < 8 && a.heads_each < heads && threads * batch * heads / (2 * a.heads_each) >= 148 * 1024)
     a.heads_each *= 2;
   const dim3 grid(unsigned((threads + 255) / 256), unsigned((heads + a.heads_each - 1) / a.heads_each), unsigned(batch));
-  RISA_DISPATCH_FLOAT(dtype_code, T, return launched(launch_chained(wide ? rotate_kernel<T> : rotate_any_kernel<T>, grid, dim3(256), 0,
+  RISA_DISPATCH_FLOAT(dtype_code, T, return launched(launch_chained(!wide ? rotate_any_kernel<T> : a.axes ? rotate_kernel<T, true> : rotate_kernel<T, false>, grid, dim3(256), 0,
                                                                     static_cast<cudaStream_t>(stream_ptr), a), "rotate"));
 }
 
@@ -664,7 +694,17 @@ extern "C" int risa_b200_cache_append(const risa_b200_cache* cache, const risa_b
                                       const int64_t vs[2], const void* q, const int64_t qs[2],
                                       void* q_out, const int64_t os[2], int q_heads, int dtype_code,
                                       const risa_b200_rotary* rotary, const void* positions,
-                                      int positions_64, void* stream_ptr) {
+                                      int positions_64, void* stream) {
+  return risa_b200_cache_append_axes(cache, step, k, ks, v, vs, q, qs, q_out, os, q_heads, dtype_code, rotary, nullptr, positions,
+                                     positions_64, stream);
+}
+
+extern "C" int risa_b200_cache_append_axes(const risa_b200_cache* cache, const risa_b200_step* step,
+                                           const void* k, const int64_t ks[2], const void* v,
+                                           const int64_t vs[2], const void* q, const int64_t qs[2],
+                                           void* q_out, const int64_t os[2], int q_heads, int dtype_code,
+                                           const risa_b200_rotary* rotary, const risa_b200_rotary_axes* axes,
+                                           const void* positions, int positions_64, void* stream_ptr) {
   if (const int bad = check_cache(cache, "append")) return bad;
   if (const int bad = check_step(step, cache, "append")) return bad;
   const bool codes = cache->dtype_code == kInt8;
@@ -676,6 +716,7 @@ extern "C" int risa_b200_cache_append(const risa_b200_cache* cache, const risa_b
   if (rotary != nullptr) {
     if (const int bad = check_rotary(rotary, cache->head_dim, "append")) return bad;
     RISA_REQUIRE(rotary->rotary_dim % 16 == 0, "append: rotary_dim must be a multiple of 16");
+    if (const int bad = check_axes(axes, "append")) return bad;
   }
   const void* const pointers[] = {k, v, q, q_out};
   const int64_t* const strides[] = {ks, vs, qs, os};
@@ -717,6 +758,11 @@ extern "C" int risa_b200_cache_append(const risa_b200_cache* cache, const risa_b
     a.magnitude = rotary->magnitude;
     a.positions = positions;
     a.positions_64 = positions_64;
+    if (axes != nullptr) {
+      a.axes = axes->axes;
+      a.axis_stride = axes->position_stride;
+      a.last_axis = axes->count - 1;
+    }
   }
   a.status = status;
   const auto kernel = dtype_code == 1 ? (codes ? append_kernel<__half, true> : append_kernel<__half, false>)

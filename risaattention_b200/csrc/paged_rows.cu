@@ -18,6 +18,7 @@
 #include "paged_tc.cuh"
 #include "serving_plan.cuh"
 
+#include <algorithm>
 #include <climits>
 #include <type_traits>
 
@@ -27,7 +28,7 @@ namespace {
 
 constexpr int kWarps = 4, kThreads = kWarps * 32;
 struct RowsArgs {
-  LineArgs line;
+  FrontLineArgs line;
   const void* q;
   int64_t qn, qh;
   void* out;
@@ -49,10 +50,13 @@ struct RowsArgs {
   const float* previous;
   float* weights;
 };
-
-template <typename T_, bool INT8_, int D_, int NT_>
+// FRONT: first keys stay visible in front of the window (the walk over the keys then has a gap; all others are spared its
+// instructions, which cost 32 requests of up to 32K codes 263 -> 302 us).
+template <typename T_, bool INT8_, int D_, int NT_, bool FRONT_>
 struct Tile {
   using T = T_;
+  static constexpr bool FRONT = FRONT_;
+  using Line = std::conditional_t<FRONT, FrontLineArgs, LineArgs>;
   static constexpr bool INT8 = INT8_;
   static constexpr int D = D_, NT = NT_, R = 8 * NT_;
   using M = std::conditional_t<INT8_, __half, T_>;  // type of the matrix instructions' operands
@@ -133,6 +137,13 @@ __device__ __forceinline__ uint32_t less_1152(uint32_t u) {
 __device__ __forceinline__ uint32_t pair_of_flipped(uint32_t word, int i) { return less_1152(__byte_perm(word, 0x64646464u, i ? 0x4342 : 0x4140)); }
 __device__ __forceinline__ uint32_t pair_of_halves(uint32_t pair) { return less_1152((pair & 0x00ff00ffu) ^ 0x64806480u); }
 
+// Not in front of the window, or one of the first keys.
+template <typename C>
+__device__ __forceinline__ bool outside_gap(const FrontLineArgs& line, int key, int low) {
+  if (C::FRONT) return uint32_t(key - line.sinks) >= uint32_t(max(low - line.sinks, 0));
+  return key >= low;
+}
+
 // ---- a warp's walk over its steps -----------------------------------------------------------------------
 // Steps first, first + kWarps, ... of one unit.  Page numbers are looked up 32 steps at a time, one set
 // ahead; a page outside the pool is not read (its keys are hidden and the status word says so).
@@ -141,6 +152,7 @@ struct Walk {
   const RowsArgs& a;
   const int32_t* row;  // the sequence's row of the page table
   int head, first_key, low, length, count, sequence;
+  int turn, skip;  // FRONT: from step `turn` on keys lie `skip` further, behind the first ones that stay visible
   int pages, pages_ahead;
   uint32_t base;
   unsigned int hidden;  // one bit per stage
@@ -148,7 +160,8 @@ struct Walk {
   static constexpr int STAGE = (WITH_VALUES ? 2 : 1) * C::SIDE + C::SCALES;
   static_assert(STAGES >= 2 && STAGES <= 32, "ring");
 
-  __device__ __forceinline__ int key_of(int i) const { return first_key + i * (16 * kWarps); }
+  __device__ __forceinline__ int key_of(int i) const { return first_key + i * (16 * kWarps) + (C::FRONT && i >= turn ? skip : 0); }
+  __device__ __forceinline__ bool exists(int key) const { return key < length && (outside_gap<C>(a.line, key, low)); }
   __device__ __forceinline__ int look_up(int i) const {
     const int key = key_of(i);
     return i < count && key < length ? __ldg(row + (key >> a.line.step.page_shift)) : -1;
@@ -177,23 +190,31 @@ struct Walk {
       const char* k = a.keys + line * C::ROW;
       const char* v = a.values + line * C::ROW;
       const uint32_t to = base + stage * STAGE;
+      auto copy = [&](auto whole) {
 #pragma unroll
-      for (int j = 0; j < C::CHUNKS / 2; ++j) {
-        const int index = j * 32 + lane, r = index / C::CHUNKS, piece = index % C::CHUNKS;
-        const bool there = good && key + r < length && key + r >= low;
-        const uint32_t at = to + r * C::ROW + swizzled<C>(r, piece) * 16;
-        copy16(at, k + index * 16, there);
-        if (WITH_VALUES) copy16(at + C::SIDE, v + index * 16, there);
-      }
-      if (C::INT8) {
-        const float* s = lane < 16 ? a.key_scales : a.value_scales;
-        const int r = lane & 15;
-        copy4(to + (WITH_VALUES ? 2 : 1) * C::SIDE + lane * 4, s + line + r, good && key + r < length && key + r >= low);
-      }
+        for (int j = 0; j < C::CHUNKS / 2; ++j) {
+          const int index = j * 32 + lane, r = index / C::CHUNKS, piece = index % C::CHUNKS;
+          const bool there = whole || (good && exists(key + r));
+          const uint32_t at = to + r * C::ROW + swizzled<C>(r, piece) * 16;
+          copy16(at, k + index * 16, there);
+          if (WITH_VALUES) copy16(at + C::SIDE, v + index * 16, there);
+        }
+        if (C::INT8) {
+          const float* s = lane < 16 ? a.key_scales : a.value_scales;
+          const int r = lane & 15;
+          copy4(to + (WITH_VALUES ? 2 : 1) * C::SIDE + lane * 4, s + line + r, whole || (good && exists(key + r)));
+        }
+      };
+      // nearly all steps are of 16 keys that exist
+      if (good && key >= low && key + 16 <= length) copy(std::true_type{});
+      else copy(std::false_type{});
     }
     copies_commit();
   }
 };
+
+// The first of a warp's steps that lies behind the first keys that stay visible.
+__device__ __forceinline__ int warp_turn(const Piece& piece) { return (piece.turn - int(threadIdx.x >> 5) + kWarps - 1) / kWarps; }
 
 // Query rows as the B operand: [nt][ks][2].  With codes the channels of a 64-channel run are dealt so that
 // a lane's 16 bytes of K serve four instructions: instruction 4 b + j takes channels 64 b + 16 t + 4 j ..
@@ -340,6 +361,7 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
   static_assert(R * kRowStride * 4 <= W::STAGE * W::STAGES, "a warp's output fits its ring");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = shared_address(smem) + warp * (W::STAGE * W::STAGES);
+  const typename C::Line& line = a.line;
   chain_wait();
   chain_release();
   if (a.clear_rest && a.line.step.offsets != nullptr) {
@@ -354,16 +376,16 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
         for (int h = threadIdx.x; h < heads; h += kThreads) a.lse[int64_t(token) * heads + h] = -INFINITY;
     }
   }
-  const int64_t total = line_total<kThreads>(a.line, shared);
+  const int64_t total = line_total<kThreads>(line, shared);
   const int workers = workers_of(total, gridDim.x, a.min_steps);
   if (int(blockIdx.x) >= workers) {
     if (threadIdx.x == 0) a.notes[blockIdx.x] = JoinNote{};
     return;
   }
   const int64_t begin = border(total, blockIdx.x, workers), end = border(total, blockIdx.x + 1, workers);
-  Pieces pieces{end - begin, line_place<kThreads>(a.line, begin, shared)};
+  Pieces pieces{end - begin, line_place<kThreads>(line, begin, shared)};
   Piece piece;
-  while (pieces.next(a.line, piece)) {
+  while (pieces.next(line, piece)) {
     const Sequence seq = piece.seq;
     const int s = piece.sequence, head = piece.head, row0 = piece.block * R, rows = seq.count * a.line.group, take = piece.count;
 
@@ -387,7 +409,7 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
     const int low = a.line.window > 0 ? visible(seq.length - seq.count, seq.length, true, a.line.window).lo : 0;
 
     W walk{a, a.line.step.table + int64_t(s) * a.line.step.width, head, (piece.first + warp) * 16, low, seq.length,
-           take > warp ? (take - warp + kWarps - 1) / kWarps : 0, s};
+           take > warp ? (take - warp + kWarps - 1) / kWarps : 0, s, warp_turn(piece), piece.skip * 16};
     walk.base = ring;
     walk.start();
     float m[NT][2], l[NT][2], o[NT][MT][4];
@@ -435,7 +457,7 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int k = key + g + (e >> 1) * 8;
-            if (hidden || k < lo[nt][e & 1] || k >= hi[nt][e & 1]) acc[nt][e] = -INFINITY;
+            if (hidden || !outside_gap<C>(a.line, k, lo[nt][e & 1]) || k >= hi[nt][e & 1]) acc[nt][e] = -INFINITY;
           }
       }
       uint32_t p[NT][2];
@@ -541,7 +563,7 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
     }
     __syncthreads();
   }
-  if (threadIdx.x == 0) a.notes[blockIdx.x] = join_note(a.line, piece, total, end, blockIdx.x, workers);
+  if (threadIdx.x == 0) a.notes[blockIdx.x] = join_note(line, piece, total, end, blockIdx.x, workers);
 }
 
 // ---- key weights -------------------------------------------------------------------------------------------
@@ -556,32 +578,33 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void weigh_rows_kernel(const Row
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   const uint32_t ring = shared_address(smem) + warp * (W::STAGE * W::STAGES);
   const int slots = a.line.step.width << a.line.step.page_shift, heads = a.line.kv_heads * a.line.group;
+  const typename C::Line& line = a.line;
   chain_wait();
   chain_release();
-  // what no step covers: in front of the window, behind the length
+  // what no step covers: in front of the window (but for the first keys that stay visible), behind the length
   for (int64_t u = blockIdx.x; u < int64_t(a.line.step.batch) * a.line.kv_heads; u += gridDim.x) {
     const Sequence seq = sequence_of(a.line.step, int(u / a.line.kv_heads));
     const int rows = seq.count * a.line.group;
     if (rows > a.line.max_rows) continue;
-    const StepRange range = rows == 0 ? StepRange{0, 0} : steps_of(a.line, seq, 0);
-    const int from = min(range.first * 16, slots), to = min((range.first + range.count) * 16, slots);
-    for (int i = threadIdx.x; i < slots - (to - from); i += kThreads) {
+    const StepRange range = rows == 0 ? StepRange{0, 0} : steps_of(line, seq, 0);
+    const int front = range.front * 16, from = min(range.first * 16, slots), to = min((range.first + range.count - range.front) * 16, slots);
+    for (int i = front + threadIdx.x; i < slots - (to - from); i += kThreads) {
       const int key = i < from ? i : i + (to - from);
       a.weights[u * slots + key] = a.previous != nullptr ? a.previous[u * slots + key] : 0.f;
     }
   }
-  const int64_t total = line_total<kThreads>(a.line, shared);
+  const int64_t total = line_total<kThreads>(line, shared);
   const int workers = workers_of(total, gridDim.x, a.min_steps);
   if (int(blockIdx.x) >= workers) return;
   const int64_t begin = border(total, blockIdx.x, workers);
-  Pieces pieces{border(total, blockIdx.x + 1, workers) - begin, line_place<kThreads>(a.line, begin, shared)};
+  Pieces pieces{border(total, blockIdx.x + 1, workers) - begin, line_place<kThreads>(line, begin, shared)};
   Piece piece;
-  while (pieces.next(a.line, piece)) {
+  while (pieces.next(line, piece)) {
     const Sequence seq = piece.seq;
     const int s = piece.sequence, head = piece.head, rows = seq.count * a.line.group, blocks = (rows + R - 1) / R, take = piece.count;
     const int low = a.line.window > 0 ? visible(seq.length - seq.count, seq.length, true, a.line.window).lo : 0;
     W walk{a, a.line.step.table + int64_t(s) * a.line.step.width, head, (piece.first + warp) * 16, low, seq.length,
-           take > warp ? (take - warp + kWarps - 1) / kWarps : 0, s};
+           take > warp ? (take - warp + kWarps - 1) / kWarps : 0, s, warp_turn(piece), piece.skip * 16};
     walk.base = ring;
     walk.start();
 #pragma unroll
@@ -630,7 +653,7 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void weigh_rows_kernel(const Row
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int k = key + g + (e >> 1) * 8;
-            const bool seen = !hidden && k >= lo[nt][e & 1] && k < hi[nt][e & 1];
+            const bool seen = !hidden && outside_gap<C>(a.line, k, lo[nt][e & 1]) && k < hi[nt][e & 1];
             const float f = C::INT8 ? (e < 2 ? ks0 : ks1) * factor[nt][e & 1] : factor[nt][e & 1];
             const float w = seen ? ex2_approx(fmaf(acc[nt][e], f, -lse2[nt][e & 1])) : 0.f;
             if (e < 2) sum0 += w; else sum1 += w;
@@ -658,9 +681,10 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void weigh_rows_kernel(const Row
 constexpr int kSms = 148, kMaxWorkers = kSms * 3;
 
 template <typename F>
-int with_tile(int dtype_code, bool codes, int head_dim, int column_blocks, F&& f) {
-#define RISA_TILE(T, I8, D)                                              \
-  return column_blocks == 1 ? f(Tile<T, I8, D, 1>{}) : f(Tile<T, I8, D, 2>{})
+int with_tile(int dtype_code, bool codes, int head_dim, int column_blocks, bool front, F&& f) {
+#define RISA_TILE(T, I8, D)                                                                                 \
+  return column_blocks == 1 ? (front ? f(Tile<T, I8, D, 1, true>{}) : f(Tile<T, I8, D, 1, false>{}))        \
+                            : (front ? f(Tile<T, I8, D, 2, true>{}) : f(Tile<T, I8, D, 2, false>{}))
 #define RISA_TILE_DIM(T, I8)                      \
   do {                                            \
     if (head_dim == 64) RISA_TILE(T, I8, 64);     \
@@ -680,7 +704,7 @@ int with_tile(int dtype_code, bool codes, int head_dim, int column_blocks, F&& f
 int column_blocks_of(const risa_b200_step& step, int group) { return step.query_offsets == nullptr && group <= 8 ? 1 : 2; }
 
 int check_queries(const risa_b200_cache* cache, const risa_b200_step* step, const void* q, const int64_t qs[2], int q_heads,
-                  int dtype_code, float scale, int is_causal, int window, const char* what) {
+                  int dtype_code, float scale, int is_causal, int window, int sinks, const char* what) {
   if (const int bad = check_cache(cache, what)) return bad;
   if (const int bad = check_step(step, cache, what)) return bad;
   RISA_REQUIRE(q != nullptr, "%s: null tensor", what);
@@ -691,16 +715,18 @@ int check_queries(const risa_b200_cache* cache, const risa_b200_step* step, cons
                "%s: query rows must start on 16-byte boundaries", what);
   RISA_REQUIRE(fabsf(scale * kLog2e) < INFINITY, "%s: the scale must be finite, also in units of log 2", what);
   RISA_REQUIRE(window >= 0 && (window == 0 || is_causal), "%s: a window needs the causal rule and at least one key", what);
+  RISA_REQUIRE(sinks >= 0 && (sinks == 0 || window > 0), "%s: first keys stay visible in front of a window", what);
   RISA_REQUIRE(int64_t(step->tokens) * (q_heads / cache->kv_heads) < (int64_t(1) << 31) - 1024, "%s: too many query rows", what);
   return RISA_B200_OK;
 }
 
 RowsArgs rows_args(const risa_b200_cache* cache, const risa_b200_step* step, const void* q, const int64_t qs[2], int q_heads,
-                   float scale, int is_causal, int window, unsigned int* status) {
+                   float scale, int is_causal, int window, int sinks, unsigned int* status) {
   RowsArgs a{};
   const int group = q_heads / cache->kv_heads;
-  a.line = {view_of(*step, cache->page_size), cache->kv_heads, Divisor(group), Divisor(8 * column_blocks_of(*step, group)), 1, INT_MAX, Divisor(16),
-            is_causal != 0, window};
+  a.line = {{view_of(*step, cache->page_size), cache->kv_heads, Divisor(group), Divisor(8 * column_blocks_of(*step, group)), 1, INT_MAX, Divisor(16),
+             is_causal != 0, window},
+            std::min(sinks, int(RISA_B200_CACHE_MOST_SLOTS))};
   a.q = q;
   a.qn = qs[0];
   a.qh = qs[1];
@@ -748,8 +774,16 @@ extern "C" size_t risa_b200_paged_attention_scratch_size(const risa_b200_cache* 
 extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const risa_b200_step* step, const void* q,
                                          const int64_t q_strides[2], int q_heads, int dtype_code, void* out,
                                          const int64_t out_strides[2], float* lse, float scale, int is_causal, int window,
-                                         int clear_rest, void* scratch, size_t scratch_bytes, void* stream_ptr) {
-  if (const int bad = check_queries(cache, step, q, q_strides, q_heads, dtype_code, scale, is_causal, window, "paged attention")) return bad;
+                                         int clear_rest, void* scratch, size_t scratch_bytes, void* stream) {
+  return risa_b200_paged_attention_sinks(cache, step, q, q_strides, q_heads, dtype_code, out, out_strides, lse, scale, is_causal, window, 0,
+                                         clear_rest, scratch, scratch_bytes, stream);
+}
+
+extern "C" int risa_b200_paged_attention_sinks(const risa_b200_cache* cache, const risa_b200_step* step, const void* q,
+                                               const int64_t q_strides[2], int q_heads, int dtype_code, void* out,
+                                               const int64_t out_strides[2], float* lse, float scale, int is_causal, int window,
+                                               int sinks, int clear_rest, void* scratch, size_t scratch_bytes, void* stream_ptr) {
+  if (const int bad = check_queries(cache, step, q, q_strides, q_heads, dtype_code, scale, is_causal, window, sinks, "paged attention")) return bad;
   RISA_REQUIRE(out != nullptr && reinterpret_cast<uintptr_t>(out) % 16 == 0 && out_strides[0] % 8 == 0 && out_strides[1] % 8 == 0,
                "paged attention: output rows must start on 16-byte boundaries");
   RISA_REQUIRE(scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 16 == 0 &&
@@ -757,7 +791,7 @@ extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const ris
                "paged attention: the scratch is too small");
   unsigned int* status = status_word();
   if (status == nullptr) return RISA_B200_CUDA;
-  RowsArgs a = rows_args(cache, step, q, q_strides, q_heads, scale, is_causal, window, status);
+  RowsArgs a = rows_args(cache, step, q, q_strides, q_heads, scale, is_causal, window, sinks, status);
   a.out = out;
   a.on = out_strides[0];
   a.oh = out_strides[1];
@@ -769,7 +803,7 @@ extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const ris
   const bool tensor_cores = takes_tensor_cores(*step, a.line.group);
   if (tensor_cores) a.line.max_rows = kTcFewestRows - 1;
   const bool codes = cache->dtype_code == kInt8;
-  int bad = with_tile(dtype_code, codes, cache->head_dim, a.line.rows / 8, [&](auto tile) {
+  int bad = with_tile(dtype_code, codes, cache->head_dim, a.line.rows / 8, sinks > 0, [&](auto tile) {
     using C = decltype(tile);
     constexpr int bytes = kWarps * Walk<C, true>::STAGE * Walk<C, true>::STAGES;
     if (const int bad = allow_shared(paged_rows_kernel<C>, bytes, "paged attention")) return bad;
@@ -784,7 +818,7 @@ extern "C" int risa_b200_paged_attention(const risa_b200_cache* cache, const ris
     bad = paged_tc(t, dtype_code, codes, cache->head_dim, stream);
   }
   if (bad == RISA_B200_OK)
-    bad = with_tile(dtype_code, codes, cache->head_dim, a.line.rows / 8, [&](auto tile) {
+    bad = with_tile(dtype_code, codes, cache->head_dim, a.line.rows / 8, false, [&](auto tile) {
       using C = decltype(tile);
       const JoinArgs join{a.parts, a.notes, C::R, a.line.group, q_heads, out, a.on, a.oh, lse};
       return launched(launch_chained(join_parts_kernel<typename C::T, C::D, true>, dim3(kSms * C::CTAS - 1, C::R), dim3(128), 0, stream, join), "paged attention");
@@ -801,12 +835,20 @@ extern "C" size_t risa_b200_key_weights_scratch_size(const risa_b200_cache* cach
 extern "C" int risa_b200_key_weights(const risa_b200_cache* cache, const risa_b200_step* step, const void* q,
                                      const int64_t q_strides[2], int q_heads, int dtype_code, const float* lse, float scale,
                                      int is_causal, int window, const float* previous, float* weights, void* scratch,
-                                     size_t scratch_bytes, void* stream_ptr) {
-  if (const int bad = check_queries(cache, step, q, q_strides, q_heads, dtype_code, scale, is_causal, window, "key weights")) return bad;
+                                     size_t scratch_bytes, void* stream) {
+  return risa_b200_key_weights_sinks(cache, step, q, q_strides, q_heads, dtype_code, lse, scale, is_causal, window, 0, previous, weights,
+                                     scratch, scratch_bytes, stream);
+}
+
+extern "C" int risa_b200_key_weights_sinks(const risa_b200_cache* cache, const risa_b200_step* step, const void* q,
+                                           const int64_t q_strides[2], int q_heads, int dtype_code, const float* lse, float scale,
+                                           int is_causal, int window, int sinks, const float* previous, float* weights, void* scratch,
+                                           size_t scratch_bytes, void* stream_ptr) {
+  if (const int bad = check_queries(cache, step, q, q_strides, q_heads, dtype_code, scale, is_causal, window, sinks, "key weights")) return bad;
   RISA_REQUIRE(lse != nullptr && weights != nullptr, "key weights: null tensor");
   unsigned int* status = status_word();
   if (status == nullptr) return RISA_B200_CUDA;
-  RowsArgs a = rows_args(cache, step, q, q_strides, q_heads, scale, is_causal, window, status);
+  RowsArgs a = rows_args(cache, step, q, q_strides, q_heads, scale, is_causal, window, sinks, status);
   const int column_blocks = a.line.rows / 8;
   a.line.rows = Divisor(1 << 30);  // all rows of a key head are one unit
   const bool tensor_cores = takes_tensor_cores(*step, a.line.group);
@@ -817,7 +859,7 @@ extern "C" int risa_b200_key_weights(const risa_b200_cache* cache, const risa_b2
   a.row_lse = lse;
   a.previous = previous;
   a.weights = weights;
-  int bad = with_tile(dtype_code, cache->dtype_code == kInt8, cache->head_dim, column_blocks, [&](auto tile) {
+  int bad = with_tile(dtype_code, cache->dtype_code == kInt8, cache->head_dim, column_blocks, sinks > 0, [&](auto tile) {
     using C = decltype(tile);
     constexpr int bytes = kWarps * Walk<C, false>::STAGE * Walk<C, false>::STAGES;
     if (const int bad = allow_shared(weigh_rows_kernel<C>, bytes, "key weights")) return bad;

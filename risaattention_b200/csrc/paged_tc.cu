@@ -90,7 +90,7 @@ struct Scales {
 // front of a window, pages outside the pool) are copied piece by piece with zeros in place of what is not there.
 template <typename C>
 __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* key_map, const CUtensorMap* value_map, Pieces pieces, Barriers* bars,
-                                            volatile uint32_t* notes, Scales* scales, uint32_t k_ring, uint32_t v_ring, uint32_t gave_up) {
+                                            volatile uint32_t* notes, volatile int* tile_keys, Scales* scales, uint32_t k_ring, uint32_t v_ring, uint32_t gave_up) {
   const int p = threadIdx.x - kProducer * 32;
   uint32_t issued = 0;
   RingPos<C::STAGES> stage;  // of both rings
@@ -111,14 +111,14 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
     const int low = a.line.window > 0 ? visible(piece.seq.length - piece.seq.count, length, true, a.line.window).lo : 0;
     const uint32_t two = C::SHARED || piece.seq.count * a.line.group - piece.block * C::ROWS > 128 ? kTwoGroups : 0u;
     KeyRuns ahead;
-    ahead.look_up(row, a.line.step.page_shift, a.pages, C::KEYS / 16, piece.first * C::KEYS, low, length);
+    ahead.look_up(row, a.line.step.page_shift, a.pages, C::KEYS / 16, piece.step(0) * C::KEYS, low, a.line.sinks, length);
     // over codes: the next batch is on its way while one is converted
     CodeBatch<C::D> batch;
     if (C::INT8) batch.load(keys, ahead, piece.head, 0, p);
 #pragma unroll 1
     for (int i = 0; i < piece.count; ++i) {
       const KeyRuns runs = ahead;
-      if (i + 1 < piece.count) ahead.look_up(row, a.line.step.page_shift, a.pages, C::KEYS / 16, runs.key0 + C::KEYS, low, length);
+      if (i + 1 < piece.count) ahead.look_up(row, a.line.step.page_shift, a.pages, C::KEYS / 16, piece.step(i + 1) * C::KEYS, low, a.line.sinks, length);
 #pragma unroll 1
       for (int side = 0; side < 2; ++side) {  // K, then V
         uint64_t* full = side ? bars->v_full : bars->k_full;
@@ -132,7 +132,7 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
           // codes as they are; the softmax multiplies scores and probabilities by their keys' scales, in 32 bits
           if (side == 0) {
             const int key = runs.key0 + p, page = __shfl_sync(0xffffffffu, runs.id, p >> 4), slot = issued % kScaleDepth;
-            const bool there = page >= 0 && key >= low && key < length;
+            const bool there = page >= 0 && runs.has(key);
             const int64_t line = there ? keys.line(page, piece.head, key) : 0;
             const float v = there ? __ldg(values.scales + line) : 0.f;
             scales->key[slot][p] = there ? __ldg(keys.scales + line) : 0.f;
@@ -171,6 +171,7 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
           mbar_arrive(smem_u32(full + stage.stage));
         }
         if (side == 0 && p == 0) {
+          tile_keys[issued % kNotes] = runs.key0;
           notes[issued % kNotes] = runs.bad | (i == 0 ? kFirst : 0u) | (i + 1 == piece.count ? kLast : 0u) | two;
           if (runs.bad) atomicCAS(a.status, 0u, unsigned(piece.sequence) + 1u);
           mbar_arrive(smem_u32(bars->k_full + stage.stage));  // the note is there
@@ -254,6 +255,9 @@ __device__ __forceinline__ void issue_products(int tiles, Barriers* bars, const 
 }
 
 // ---- the softmax warpgroups -------------------------------------------------------------------------------------------
+// The n lowest bits (none below 0, all from 32 on).
+__device__ __forceinline__ uint32_t low_bits(int n) { return n >= 32 ? 0xffffffffu : (1u << max(n, 0)) - 1u; }
+
 // A meeting of the two warps that own the same 32 rows.  It has no limit of its own, so nobody may stay away: after a wait
 // that ran out a warp does no more work, but comes to all the meetings that are left; its rows are marked at the end.
 __device__ __forceinline__ void meet(int id) { asm volatile("bar.sync %0, 64;" ::"r"(id) : "memory"); }
@@ -291,7 +295,7 @@ __device__ __forceinline__ void load_query_rows(const TcArgs& a, const Piece& pi
 
 template <typename C>
 __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Barriers* bars, Exchange* exchange, Scales* scales, uint32_t tmem, uint32_t q, int g, int half,
-                                             const volatile uint32_t* notes, uint32_t gave_up) {
+                                             const volatile uint32_t* notes, const volatile int* tile_keys, uint32_t gave_up) {
   constexpr int D = C::D, KEYS = C::KEYS / 2, OUT = C::OUT;
   using T = typename C::T;
   const int r = threadIdx.x & 127, meeting = 1 + g * 4 + (r >> 5);
@@ -337,13 +341,13 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
     const uint32_t mine_turn = turn;
 #pragma unroll 1
     for (int i = 0; i < piece.count; ++i, ++tile) {
-      const int key0 = (piece.first + i) * C::KEYS + half * KEYS;
       if (!wait(smem_u32(bars->s_full + g), s_phase, 1020 + g)) return meet_on(piece.count - i + 1);
       s_phase ^= 1;
       tc_fence_after();
       uint32_t x[KEYS];
 #pragma unroll
       for (int c = 0; c < KEYS; c += 32) tmem_load32(s_columns + half * KEYS + c, x + c);
+      const int key0 = tile_keys[tile % kNotes] + half * KEYS;
       const uint32_t gone = notes[tile % kNotes] >> (half * (KEYS / 16)) & ((1u << (KEYS / 16)) - 1);
       tmem_load_wait();
       tmem_regs_ready<KEYS>(x);
@@ -363,10 +367,17 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
       }
       if (gone != 0 || key0 < all_lo || key0 + KEYS > all_hi) {
         asm volatile("" ::: "memory");  // a branch of its own: as selects in the common path it cost a quarter of the time
-        const int lo = seen.lo - key0, hi = seen.hi - key0;
+        // hidden: in front of the window but for the first keys, behind the row's own place, on a page that is not there
+        const int lo = seen.lo - key0, hi = seen.hi - key0, front = a.line.sinks - key0;
 #pragma unroll
-        for (int c = 0; c < KEYS; ++c)
-          if (c < lo || c >= hi || (gone >> (c >> 4) & 1)) x[c] = 0xff800000u;
+        for (int c0 = 0; c0 < KEYS; c0 += 32) {
+          uint32_t hidden = (low_bits(lo - c0) & ~low_bits(front - c0)) | ~low_bits(hi - c0);
+          if (gone >> (c0 >> 4) & 1) hidden |= 0xffffu;
+          if (gone >> (c0 >> 4) & 2) hidden |= 0xffff0000u;
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (hidden >> c & 1) x[c0 + c] = 0xff800000u;
+        }
       }
       const uint64_t scale2 = pack_f32x2(scale, scale);
       float best;
@@ -516,6 +527,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
   __shared__ LineShared<kThreads> shared;
   __shared__ uint32_t tmem_base, gave_up_word;
   __shared__ volatile uint32_t notes[kNotes];
+  __shared__ volatile int tile_keys[kNotes];  // their first keys
   const int warp = threadIdx.x >> 5;
   const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
   const uint32_t q = smem, v_ring = q + C::Q, k_ring = v_ring + C::STAGES * C::SIDE, gave_up = smem_u32(&gave_up_word);
@@ -557,10 +569,10 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
   const uint32_t tmem = tmem_base;
   if (warp < kProducer) {
     regs_inc<kRegsSoftmax>();
-    softmax_rows<C>(a, pieces, &bars, &exchange, scales, tmem, q, warp >> 3, (warp >> 2) & 1, notes, gave_up);
+    softmax_rows<C>(a, pieces, &bars, &exchange, scales, tmem, q, warp >> 3, (warp >> 2) & 1, notes, tile_keys, gave_up);
   } else if (warp < kIssuer) {
     regs_dec<kRegsProducer>();
-    fetch_tiles<C>(a, &key_map, &value_map, pieces, &bars, notes, scales, k_ring, v_ring, gave_up);
+    fetch_tiles<C>(a, &key_map, &value_map, pieces, &bars, notes, tile_keys, scales, k_ring, v_ring, gave_up);
   } else {
     regs_dec<kRegsIssuer>();
     if (warp == kIssuer + 1 && (threadIdx.x & 31) == 0) {

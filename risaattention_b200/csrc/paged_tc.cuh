@@ -10,7 +10,7 @@ constexpr int kTcWorkers = 148;  // one CTA per SM
 constexpr int kTcFewestRows = 33;
 
 struct TcArgs {
-  LineArgs line;  // rows, keys and notes are the kernel's own: paged_tc_args
+  FrontLineArgs line;  // rows, keys and notes are the kernel's own: paged_tc_args
   const void* q;
   int64_t qn, qh;
   void* out;

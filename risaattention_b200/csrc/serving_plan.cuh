@@ -5,6 +5,8 @@
 // launch joins them in order.  Equal shares whatever the lengths, at most two partial results per worker,
 // and the same division (so the same bits) every time.
 #pragma once
+#include <type_traits>
+
 #include "serving.cuh"
 
 namespace risa_b200 {
@@ -19,10 +21,15 @@ struct LineArgs {
   Divisor keys;            // keys of a step
   int causal, window;
 };
+// The same with first keys that stay visible in front of the window.  A type of its own, so that kernels whose blocks have no
+// gap are compiled without it.
+struct FrontLineArgs : LineArgs {
+  int sinks;
+};
 
-// Steps [first, first + count) of a block.
+// The `count` steps of a block: [0, front), and from step `first` on.
 struct StepRange {
-  int first, count;
+  int first, count, front = 0;
 };
 // How many blocks a sequence has per key head (0: nothing to do).  The functions of a line that know what its
 // blocks and steps are: blocks_of and steps_of; here blocks of query rows and steps of keys.
@@ -39,6 +46,12 @@ __device__ __forceinline__ StepRange steps_of(const LineArgs& a, const Sequence&
   const KeyRange newest = visible(q.length - q.count + token1, q.length, a.causal, a.window);
   const int first = oldest.lo / a.keys, end = (newest.hi + a.keys - 1) / a.keys;
   return {first, max(end - first, 1)};
+}
+// In front of them those of the first keys that stay visible, as far as they lie in front of the window's.
+__device__ __forceinline__ StepRange steps_of(const FrontLineArgs& a, const Sequence& q, int block) {
+  const StepRange window = steps_of(static_cast<const LineArgs&>(a), q, block);
+  const int front = min((a.sinks + a.keys.value - 1) / a.keys, window.first);
+  return {window.first, front + window.count, front};
 }
 
 // Quotients of numbers that are rarely past 32 bits (a 64-bit division is some hundred instructions).
@@ -190,7 +203,9 @@ struct Piece {
   Sequence seq;
   int sequence, head, block;
   int first, count;
+  int turn, skip;  // from the piece's step `turn` on it goes on `skip` steps further
   bool whole, opens;
+  __device__ __forceinline__ int step(int i) const { return first + i + (i >= turn ? skip : 0); }
 };
 // Walks the pieces of one worker; every role of a CTA keeps a walk of its own.
 struct Pieces {
@@ -215,6 +230,15 @@ struct Pieces {
     p.head = at.head;
     p.block = at.block;
     p.first = range.first + at.inside;
+    p.turn = p.skip = 0;
+    if (std::is_same<L, FrontLineArgs>::value) {
+      p.first -= range.front;
+      if (at.inside < range.front) {
+        p.turn = range.front - at.inside;
+        p.skip = range.first - range.front;
+        p.first = at.inside;
+      }
+    }
     p.count = int(min(int64_t(range.count - at.inside), left));
     p.opens = at.inside == 0;
     p.whole = p.count == range.count;
@@ -255,7 +279,8 @@ struct JoinArgs {
 };
 
 // Written once the walk over the pieces has come to its end (`at` behind the last step, `done` the last piece).
-__device__ __forceinline__ JoinNote join_note(const LineArgs& a, const Piece& last, int64_t total, int64_t end, int worker, int workers) {
+template <typename L>
+__device__ __forceinline__ JoinNote join_note(const L& a, const Piece& last, int64_t total, int64_t end, int worker, int workers) {
   if (!last.opens || last.whole) return {0, 0, 0, 0, 0, 0};
   const int64_t unit_end = end - last.count + steps_of(a, last.seq, last.block).count;
   return {last.seq.first, last.seq.count * a.group, last.head, last.block, min(worker_from(total, unit_end, workers), workers) - worker, last.sequence};

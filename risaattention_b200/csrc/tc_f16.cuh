@@ -122,17 +122,21 @@ struct PoolView {
     return ((int64_t(id) * kv_heads + head) << page_shift) + (key & ((1 << page_shift) - 1));
   }
 };
-// Keys [low, length) of a sequence exist.  Lane i of every warp knows the page of the i-th run of 16 keys from key0 on, -1
+// Keys [low, length) of a sequence exist, and its first `sinks`.  Lane i of every warp knows the page of the i-th run of 16 keys from key0 on, -1
 // where there is none; `bad`: runs whose page is outside the pool although a key of theirs exists.
 struct KeyRuns {
-  int key0, low, length, id;
+  int key0, low, sinks, length, id;
   uint32_t bad;
-  __device__ __forceinline__ void look_up(const int32_t* row, int page_shift, int pages, int runs, int first_key, int first_existing, int sequence_length) {
+  // all but the keys [sinks, low) between the first ones and the window
+  __device__ __forceinline__ bool has(int key) const { return key < length && uint32_t(key - sinks) >= uint32_t(max(low - sinks, 0)); }
+  __device__ __forceinline__ void look_up(const int32_t* row, int page_shift, int pages, int runs, int first_key, int first_existing, int first_keys,
+                                          int sequence_length) {
     key0 = first_key;
     low = first_existing;
+    sinks = first_keys;
     length = sequence_length;
     const int lane = threadIdx.x & 31, key = key0 + 16 * lane;
-    const bool exists = lane < runs && key < length && key + 16 > low;
+    const bool exists = lane < runs && key < length && (key + 16 > low || key < sinks);
     id = exists ? __ldg(row + (key >> page_shift)) : -1;
     bad = __ballot_sync(0xffffffffu, exists && (id < 0 || id >= pages));
     if (id >= pages) id = -1;
@@ -148,7 +152,7 @@ __device__ __forceinline__ void copy_keys(const PoolView& pool, const KeyRuns& k
 #pragma unroll 4
   for (int r = thread / PIECES; r < ROWS; r += EACH) {
     const int key = k.key0 + r, page = __shfl_sync(0xffffffffu, k.id, r >> 4);
-    const bool there = page >= 0 && key >= k.low && key < k.length;
+    const bool there = page >= 0 && k.has(key);
     const int64_t line = there ? pool.line(page, head, key) : 0;
     copy16(to + (ROWS > 128 ? (r >> 7) * tile_bytes : 0) + tile_offset<(ROWS > 128 ? 128 : ROWS)>(r & 127, piece), pool.rows + line * (D * 2) + piece * 16, there);
   }
@@ -163,7 +167,7 @@ struct CodeBatch {
 #pragma unroll
     for (int n = 0; n < COUNT; ++n) {
       const int r = from + thread / PIECES + n * EACH, key = k.key0 + r, page = __shfl_sync(0xffffffffu, k.id, r >> 4);
-      const bool there = page >= 0 && key >= k.low && key < k.length;
+      const bool there = page >= 0 && k.has(key);
       codes[n] = there ? *reinterpret_cast<const uint4*>(pool.rows + pool.line(page, head, key) * D + piece * 16) : make_uint4(0, 0, 0, 0);
     }
   }

@@ -48,13 +48,22 @@ struct WeighLine {
   int min_rows;
   Divisor tile_rows;  // query rows of a step
   int causal, window;
+  int sinks;          // first keys that stay visible in front of a window
 };
 __device__ __forceinline__ int first_seen(const WeighLine& a, const Sequence& q) {
   return a.window > 0 ? visible(q.length - q.count, q.length, true, a.window).lo : 0;
 }
+// Blocks of the first keys that stay visible, as far as they lie in front of the window's.
+__device__ __forceinline__ int front_blocks(const WeighLine& a, const Sequence& q) {
+  return min((a.sinks + kBlockKeys - 1) / kBlockKeys, first_seen(a, q) / kBlockKeys);
+}
 __device__ __forceinline__ int blocks_of(const WeighLine& a, const Sequence& q) {
   if (q.count == 0 || q.count * a.group < a.min_rows || q.length == 0) return 0;
-  return (q.length + kBlockKeys - 1) / kBlockKeys - first_seen(a, q) / kBlockKeys;
+  return front_blocks(a, q) + (q.length + kBlockKeys - 1) / kBlockKeys - first_seen(a, q) / kBlockKeys;
+}
+__device__ __forceinline__ int first_key_of(const WeighLine& a, const Sequence& q, int block) {
+  const int front = front_blocks(a, q);
+  return (block < front ? block : first_seen(a, q) / kBlockKeys + block - front) * kBlockKeys;
 }
 // Rows [lo, hi) of the sequence that see a key; hi is INT_MAX where no window ends them.
 struct RowRange {
@@ -64,13 +73,13 @@ __device__ __forceinline__ RowRange rows_of(const WeighLine& a, const Sequence& 
   if (!a.causal) return {0, INT_MAX};
   const int base = q.length - q.count;  // place of the first new token
   const int lo = min(max(key - base, 0), q.count) * a.group;
-  if (a.window == 0) return {lo, INT_MAX};
+  if (a.window == 0 || key < a.sinks) return {lo, INT_MAX};
   const int64_t end = int64_t(key) + a.window - base;
   return {lo, end <= 0 ? 0 : end >= q.count ? INT_MAX : int(end) * a.group};
 }
 __device__ __forceinline__ StepRange steps_of(const WeighLine& a, const Sequence& q, int block) {
-  const int key0 = (first_seen(a, q) / kBlockKeys + block) * kBlockKeys;
-  const int rows = q.count * a.group, from = rows_of(a, q, key0).lo, to = min(rows_of(a, q, key0 + kBlockKeys - 1).hi, rows);
+  const int key0 = first_key_of(a, q, block);
+  const int rows = q.count * a.group, from = rows_of(a, q, key0).lo, to = min(rows_of(a, q, key0 < a.sinks ? key0 : key0 + kBlockKeys - 1).hi, rows);
   const int first = min(from, rows - 1) / a.tile_rows, end = (to + a.tile_rows - 1) / a.tile_rows;
   return {first, max(end - first, 1)};
 }
@@ -130,9 +139,9 @@ __device__ __forceinline__ void fetch_keys(const WeighArgs& a, Pieces pieces, Ba
   Piece at;
   while (pieces.next(a.line, at)) {
     const int32_t* row = a.line.step.table + int64_t(at.sequence) * a.line.step.width;
-    const int low = first_seen(a.line, at.seq), length = at.seq.length, key0 = (low / kBlockKeys + at.block) * kBlockKeys;
+    const int low = first_seen(a.line, at.seq), length = at.seq.length, key0 = first_key_of(a.line, at.seq, at.block);
     KeyRuns runs;
-    runs.look_up(row, a.line.step.page_shift, a.pages, kBlockKeys / 16, key0, low, length);
+    runs.look_up(row, a.line.step.page_shift, a.pages, kBlockKeys / 16, key0, low, a.line.sinks, length);
     if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(bars->k_empty + kb.stage), kb.phase ^ 1, gave_up, 1101))) break;
     if (p == 0) {
       notes->bad[block % kDepth] = runs.bad;
@@ -183,7 +192,7 @@ __device__ __forceinline__ void fetch_queries(const WeighArgs& a, Pieces pieces,
   while (more) {
     const Piece now = piece;
     const Sequence& seq = now.seq;
-    const int key0 = (first_seen(a.line, seq) / kBlockKeys + now.block) * kBlockKeys, rows = seq.count * a.line.group;
+    const int key0 = first_key_of(a.line, seq, now.block), rows = seq.count * a.line.group;
     more = pieces.next(a.line, piece);
     constexpr int PIECES = C::D / 8, ROWS_EACH = 128 / PIECES;  // rows that the warpgroup copies at a time
     constexpr int COPIES = C::ROWS / ROWS_EACH;
@@ -313,14 +322,16 @@ __device__ __forceinline__ void add_up(const WeighArgs& a, Pieces pieces, Barrie
   Piece piece;
   while (pieces.next(a.line, piece)) {
     const Sequence& seq = piece.seq;
-    const int low = first_seen(a.line, seq), key0 = (low / kBlockKeys + piece.block) * kBlockKeys + g * 128, key = key0 + lane;
+    const int low = first_seen(a.line, seq), key0 = first_key_of(a.line, seq, piece.block) + g * 128, key = key0 + lane;
+    const bool exists = (key >= low || key < a.line.sinks) && key < seq.length;
     const bool takes_part = g == 0 || seq.length - key0 > 0;
     RowRange mine = rows_of(a.line, seq, key);
-    const int all_lo = rows_of(a.line, seq, key0 + 127).lo, all_hi = rows_of(a.line, seq, key0).hi;
-    bool whole_group = key0 >= low && key0 + 128 <= seq.length;
-    if (key < low || key >= seq.length) mine.hi = 0;
+    // the first to lose sight of a key of the group are those of its first key that is not always visible
+    const int all_lo = rows_of(a.line, seq, key0 + 127).lo, all_hi = rows_of(a.line, seq, min(max(key0, a.line.sinks), key0 + 127)).hi;
+    bool whole_group = (key0 >= low || key0 + 128 <= a.line.sinks) && key0 + 128 <= seq.length;
+    if (!exists) mine.hi = 0;
     float factor = a.scale_log2;
-    if (C::INT8 && key >= low && key < seq.length) {
+    if (C::INT8 && exists) {
       const int id = __ldg(a.line.step.table + int64_t(piece.sequence) * a.line.step.width + (key >> a.line.step.page_shift));
       if (id >= 0 && id < a.pages) factor *= __ldg(a.keys.scales + a.keys.line(id, piece.head, key));
     }
@@ -396,14 +407,15 @@ __global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a
     mbar_init_fence();
   }
   chain_release();  // and no wait: see paged_tc_kernel
-  // what no block covers: in front of the window, behind the length
+  // what no block covers: in front of the window (but for the first keys that stay visible), behind the length
   const int slots = a.line.step.width << a.line.step.page_shift;
   for (int64_t u = blockIdx.x; u < int64_t(a.line.step.batch) * a.line.kv_heads; u += gridDim.x) {
     const Sequence seq = sequence_of(a.line.step, int(u / a.line.kv_heads));
     if (seq.count * a.line.group < a.line.min_rows) continue;
     const int blocks = blocks_of(a.line, seq), block0 = first_seen(a.line, seq) / kBlockKeys;
-    const int from = blocks == 0 ? 0 : block0 * kBlockKeys, to = blocks == 0 ? 0 : min((block0 + blocks) * kBlockKeys, slots);
-    for (int i = threadIdx.x; i < slots - (to - from); i += kThreads) {
+    const int front = blocks == 0 ? 0 : front_blocks(a.line, seq), from = blocks == 0 ? 0 : block0 * kBlockKeys;
+    const int to = blocks == 0 ? 0 : min((block0 + blocks - front) * kBlockKeys, slots);
+    for (int i = front * kBlockKeys + threadIdx.x; i < slots - (to - from); i += kThreads) {
       const int64_t index = u * slots + (i < from ? i : i + (to - from));
       a.weights[index] = a.previous != nullptr ? a.previous[index] : 0.f;
     }
@@ -436,7 +448,7 @@ __global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a
       JoinNote note{};
       if (last.opens && !last.whole) {
         const int64_t end = finish - last.count + steps_of(a.line, last.seq, last.block).count;
-        note = {last.seq.first, (first_seen(a.line, last.seq) / kBlockKeys + last.block) * kBlockKeys, last.head, last.block,
+        note = {last.seq.first, first_key_of(a.line, last.seq, last.block), last.head, last.block,
                 min(worker_from(total, end, workers), workers) - int(blockIdx.x), last.sequence};
       }
       a.notes[blockIdx.x] = note;
@@ -458,7 +470,7 @@ __global__ __launch_bounds__(kThreads, 1) void weigh_tc_kernel(const WeighArgs a
     Pieces all = pieces;
     Piece piece;
     while (all.next(a.line, piece)) {
-      const int key = (first_seen(a.line, piece.seq) / kBlockKeys + piece.block) * kBlockKeys + threadIdx.x;
+      const int key = first_key_of(a.line, piece.seq, piece.block) + threadIdx.x;
       if (!piece.whole) a.parts[(int64_t(blockIdx.x) * 2 + (piece.opens ? 1 : 0)) * kBlockKeys + threadIdx.x] = NAN;
       else if (key < slots) a.weights[(int64_t(piece.sequence) * a.line.kv_heads + piece.head) * slots + key] = NAN;
     }
@@ -501,7 +513,7 @@ size_t weigh_tc_scratch() { return size_t(kTcWorkers) * (2 * kBlockKeys * sizeof
 
 int weigh_tc(const TcArgs& t, const float* row_lse, const float* previous, float* weights, int dtype_code, bool codes, int head_dim,
              cudaStream_t stream) {
-  const WeighArgs a{{t.line.step, t.line.kv_heads, t.line.group, t.line.min_rows, Divisor(), t.line.causal, t.line.window},
+  const WeighArgs a{{t.line.step, t.line.kv_heads, t.line.group, t.line.min_rows, Divisor(), t.line.causal, t.line.window, t.line.sinks},
                     t.q, t.qn, t.qh, row_lse, {t.keys, t.key_scales, t.line.kv_heads, t.line.step.page_shift}, t.pages, t.scale_log2,
                     previous, weights, t.parts, reinterpret_cast<JoinNote*>(t.parts + size_t(kTcWorkers) * 2 * kBlockKeys), t.min_steps, t.status};
   return dtype_code == 1 ? launch_for<__half>(a, codes, head_dim, stream) : launch_for<__nv_bfloat16>(a, codes, head_dim, stream);

@@ -24,6 +24,7 @@ from ._validation import UNAVAILABLE, is_available
 
 PAGE_SIZES = (16, 32, 64, 128)
 CACHE_HEAD_DIMS = (64, 128, 256)
+MOST_AXES = 8
 ROTARY_SCALINGS = (None, "linear", "base", "parts")
 
 
@@ -45,14 +46,21 @@ class RotaryTable:
     """Angle per position of every rotated pair of channels, ``turns`` int64 [rotary_dim / 2] in units of
     2^-64 turns (an angle matters modulo one turn, and positions are whole numbers, so the product with a
     position wraps exactly where the angle does and far positions lose nothing), and the factor that
-    multiplies cosines and sines."""
+    multiplies cosines and sines.  Where positions have several axes, ``axes`` uint8 [rotary_dim / 2] says
+    which of the ``axis_count`` each pair follows."""
 
     turns: torch.Tensor
     magnitude: float = 1.0
+    axes: torch.Tensor | None = None
+    axis_count: int = 1
 
     @property
     def rotary_dim(self) -> int:
         return 2 * self.turns.shape[0]
+
+    @property
+    def _arguments(self):
+        return self.turns, self.axes, self.axis_count, self.magnitude
 
 
 def rotary_frequencies(rotary_dim, *, base=10000.0, scaling=None, factor=1.0, original_length=None,
@@ -93,17 +101,45 @@ def rotary_frequencies(rotary_dim, *, base=10000.0, scaling=None, factor=1.0, or
 
 
 def rotary_table(rotary_dim, *, base=10000.0, scaling=None, factor=1.0, original_length=None,
-                 slow_turns=1.0, fast_turns=32.0, magnitude=1.0, device="cuda") -> RotaryTable:
+                 slow_turns=1.0, fast_turns=32.0, magnitude=1.0, sections=None, dealt=False, restart=False,
+                 device="cuda") -> RotaryTable:
     """The table of ``rotary_frequencies`` on a device.  ``magnitude`` multiplies cosines and sines (some
-    long-context scalings raise it above 1)."""
+    long-context scalings raise it above 1).
+
+    ``sections``, for positions of several axes (time, height and width of a video, say): how many pairs
+    follow each axis, ``rotary_dim / 2`` together.  The sections lie one behind the other or, ``dealt``, the
+    pairs go to the axes in turn while their sections last.  The frequencies run on through all pairs or,
+    with ``restart``, each axis has those of a ``rotary_dim`` of its own."""
     if not math.isfinite(magnitude):
         raise ValueError(f"magnitude must be finite, got {magnitude}")
-    frequencies = rotary_frequencies(rotary_dim, base=base, scaling=scaling, factor=factor,
-                                     original_length=original_length, slow_turns=slow_turns,
-                                     fast_turns=fast_turns)
+    options = dict(base=base, scaling=scaling, factor=factor, original_length=original_length,
+                   slow_turns=slow_turns, fast_turns=fast_turns)
+    frequencies, axes = rotary_frequencies(rotary_dim, **options), None
+    if sections is None:
+        if dealt or restart:
+            raise ValueError("dealt and restart need sections")
+    else:
+        axes = _axes_of_pairs(rotary_dim, sections, dealt)
+        if restart:
+            own = [iter(rotary_frequencies(2 * n, **options)) for n in sections]
+            frequencies = [next(own[axis]) for axis in axes]
     units = [round(f / (2 * math.pi) * 2.0 ** 64) % 2 ** 64 for f in frequencies]
     signed = [u - 2 ** 64 if u >= 2 ** 63 else u for u in units]
-    return RotaryTable(torch.tensor(signed, dtype=torch.int64, device=device), float(magnitude))
+    turns = torch.tensor(signed, dtype=torch.int64, device=device)
+    if axes is None:
+        return RotaryTable(turns, float(magnitude))
+    return RotaryTable(turns, float(magnitude), torch.tensor(axes, dtype=torch.uint8, device=device), len(sections))
+
+
+def _axes_of_pairs(rotary_dim, sections, dealt):
+    sections = list(sections)
+    if not 1 <= len(sections) <= MOST_AXES or any(not isinstance(n, int) or n <= 0 for n in sections):
+        raise ValueError(f"sections must be 1 to {MOST_AXES} positive numbers of pairs, got {sections}")
+    if 2 * sum(sections) != rotary_dim:
+        raise ValueError(f"sections must add up to rotary_dim / 2 = {rotary_dim // 2}, got {sum(sections)}")
+    if not dealt:
+        return [axis for axis, n in enumerate(sections) for _ in range(n)]
+    return [axis for turn in range(max(sections)) for axis, n in enumerate(sections) if turn < n]
 
 
 def _check_table(rotary):
@@ -117,7 +153,8 @@ def rotate_positions(x, positions, rotary, *, interleaved=False, transposed=Fals
 
     ``x``: packed tokens [tokens, heads, head_dim] with ``positions`` [tokens], or [batch, heads, tokens,
     head_dim] with ``positions`` [tokens] or [batch, tokens]; float32, float16 or bfloat16, any strides with
-    contiguous rows.  ``positions``: int32 or int64 (negative ones turn backwards).  Pair i is channels
+    contiguous rows.  ``positions``: int32 or int64 (negative ones turn backwards); of a table with sections
+    [axes, tokens] or [axes, batch, tokens], or [tokens] where all axes have the same.  Pair i is channels
     (i, i + rotary_dim / 2), or (2 i, 2 i + 1) where ``interleaved``.  ``transposed`` applies the transposed
     rotation (the inverse where the table's magnitude is 1).  ``out``: where to write, ``x`` itself included, no other
     view of its memory.
@@ -128,10 +165,10 @@ def rotate_positions(x, positions, rotary, *, interleaved=False, transposed=Fals
     if torch.is_grad_enabled() and x.requires_grad:
         if out is not None:
             raise ValueError("out cannot be given where x requires a gradient")
-        return _native(x.device).rotate_with_gradient(x, positions, rotary.turns, rotary.magnitude,
-                                                      bool(interleaved), bool(transposed))
-    return _native(x.device).rotate(x, positions, rotary.turns, rotary.magnitude, bool(interleaved),
-                                    bool(transposed), out, _stream(x.device))
+        return _native(x.device).rotate_with_gradient(x, positions, *rotary._arguments, bool(interleaved),
+                                                      bool(transposed))
+    return _native(x.device).rotate(x, positions, *rotary._arguments, bool(interleaved), bool(transposed), out,
+                                    _stream(x.device))
 
 
 # ---- the cache --------------------------------------------------------------------------------------------
@@ -182,7 +219,8 @@ def append_to_cache(cache, k, v, page_table, lengths, *, query_offsets=None, q=N
     """Writes a step's keys and values [tokens, kv_heads, head_dim] to their places: token i of the n new
     ones of sequence s is token ``lengths[s] - n + i`` of it.
 
-    With ``rotary`` the keys are rotated first, by ``positions`` [tokens] or, without them, by those places;
+    With ``rotary`` the keys are rotated first, by ``positions`` [tokens] (of a table with sections also
+    [axes, tokens]) or, without them, by those places;
     ``q`` [tokens, q_heads, head_dim] is rotated in the same launch and returned (None without it; rows
     behind the last sequence give 0).  An int8 cache stores absmax / 127 as a token's scale and the codes
     rounded to nearest even.  Tokens that their sequence is too short for are not written; a page outside
@@ -193,18 +231,20 @@ def append_to_cache(cache, k, v, page_table, lengths, *, query_offsets=None, q=N
         _check_table(rotary)
     device = cache.keys.device
     return _native(device).cache_append(
-        *cache.tensors, k, v, page_table, lengths, query_offsets, q, None if rotary is None else rotary.turns,
-        1.0 if rotary is None else rotary.magnitude, bool(interleaved), positions, _stream(device))
+        *cache.tensors, k, v, page_table, lengths, query_offsets, q,
+        *((None, None, 1, 1.0) if rotary is None else rotary._arguments), bool(interleaved), positions, _stream(device))
 
 
 def paged_attention(q, cache, page_table, lengths, *, query_offsets=None, scale=None, is_causal=True,
-                    window=None, return_lse=False, out=None):
+                    window=None, sinks=0, return_lse=False, out=None):
     """Attention of a step's new tokens ``q`` [tokens, q_heads, head_dim] over the cached keys of their
     sequences, the tokens' own included (append them first).  One token of each sequence, chunks of a
     prompt, or both in one call.
 
     With ``is_causal`` (aligned to the end: the last new token sees all ``lengths[s]`` keys) and ``window``
-    a token sees the last ``window`` keys up to its own place; without ``is_causal`` every token sees all.
+    a token sees the last ``window`` keys up to its own place and, of those in front of them, the first ``sinks``
+    of the sequence; keys between them are not read, nor are their entries of the page table.  Without
+    ``is_causal`` every token sees all.
     ``q_heads`` is a multiple of the cache's heads.  ``scale``: head_dim ** -0.5 unless given.  A token that
     sees nothing gives 0 and an LSE of -inf.  Rows of no sequence (behind the last, in front of the first) give
     the same; where ``out`` is given (``q`` itself included, no other view of its memory) its rows stay as they
@@ -222,12 +262,12 @@ def paged_attention(q, cache, page_table, lengths, *, query_offsets=None, scale=
         scale = q.shape[-1] ** -0.5
     output, lse = _native(q.device).paged_attention(
         q, *cache.tensors, page_table, lengths, query_offsets, float(scale), bool(is_causal), window,
-        bool(return_lse), out, _stream(q.device))
+        int(sinks), bool(return_lse), out, _stream(q.device))
     return (output, lse) if return_lse else output
 
 
 def cached_key_weights(q, lse, cache, page_table, lengths, *, query_offsets=None, scale=None, is_causal=True,
-                       window=None, previous=None):
+                       window=None, sinks=0, previous=None):
     """The attention that each cached key received from a step's tokens: FP32 [batch, kv_heads, pages of a
     sequence * page_size], the sum of the probabilities over the sequence's new tokens and the query heads
     of the key's head.  ``q``, ``lse`` and the options as in ``paged_attention(..., return_lse=True)``;
@@ -238,7 +278,7 @@ def cached_key_weights(q, lse, cache, page_table, lengths, *, query_offsets=None
         scale = q.shape[-1] ** -0.5
     return _native(q.device).key_weights(
         q, lse, *cache.tensors, page_table, lengths, query_offsets, float(scale), bool(is_causal), window,
-        previous, _stream(q.device))
+        int(sinks), previous, _stream(q.device))
 
 
 class Eviction(NamedTuple):
