@@ -7,7 +7,8 @@
  * status code with risa_b200_last_error(), no allocation, no host synchronisation.  Everything that
  * changes from step to step (lengths, offsets, page table) is read on the device, so a captured
  * graph replays with new contents.
- * dtype codes: 0 = float32, 1 = float16, 2 = bfloat16, 4 = int8 codes with a scale per token and head.
+ * dtype codes: 0 = float32, 1 = float16, 2 = bfloat16, 4 = int8 codes with a scale per token and head,
+ * 5 = 4-bit codes with a scale per token and head and one per 16 channels.
  */
 #ifndef RISA_B200_CACHE_H
 #define RISA_B200_CACHE_H
@@ -19,8 +20,14 @@ extern "C" {
 #endif
 
 /* Pages of keys and values: [pages, kv_heads, page_size, head_dim] contiguous, 16-byte aligned;
- * scales f32 [pages, kv_heads, page_size] (int8 only, else NULL).  page_size: 16, 32, 64 or 128;
- * head_dim: 64, 128 or 256; dtype_code: 1, 2 or 4. */
+ * scales f32 [pages, kv_heads, page_size] (int8; NULL for 16-bit values).  page_size: 16, 32, 64 or
+ * 128; head_dim: 64, 128 or 256; dtype_code: 1, 2, 4 or 5.
+ * 4-bit codes: a value is code * group scale * token scale.  Rows of head_dim / 2 bytes; channel
+ * 8 w + 2 i + j as code + 8 (codes -7..7) in bits 16 j + 4 i of the row's 32-bit word w.  The scale
+ * pointers lead to bytes [pages, kv_heads, page_size * (1 + head_dim / 16)], 16-byte aligned: of each
+ * page and head first the token scales, powers of two as the exponent field of a float (0: a scale of
+ * zero, 255: a row that is not finite), then for each token the scales of its groups of 16 channels,
+ * e4m3 numbers that are not negative. */
 typedef struct {
   void* keys;
   void* values;
@@ -100,9 +107,17 @@ int risa_b200_cache_append_axes(const risa_b200_cache* cache, const risa_b200_st
                                 const risa_b200_rotary* rotary, const risa_b200_rotary_axes* axes,
                                 const void* positions, int positions_64, void* stream);
 
+/* The step's keys and values [tokens, kv_heads, head_dim] as they lie in the cache, codes as the values
+ * that they stand for, rounded to dtype_code (1 or 2; a 16-bit cache's own).  Rows of no sequence, or
+ * whose sequence is too short for them, give 0.  Strides are of (token, head) in elements, multiples of 8;
+ * pointers are 16-byte aligned. */
+int risa_b200_cache_read(const risa_b200_cache* cache, const risa_b200_step* step, void* k,
+                         const int64_t k_strides[2], void* v, const int64_t v_strides[2],
+                         int dtype_code, void* stream);
+
 /* softmax(scale * q K^T) V of every packed token over its sequence's cached keys; with is_causal the
  * token at place p of its sequence sees keys max(0, p - window + 1) .. p (window 0: from the start),
- * without it all of them.  q, out: dtype_code 1 or 2 (the cache's own unless that is int8).  lse: f32
+ * without it all of them.  q, out: dtype_code 1 or 2 (the cache's own unless that holds codes).  lse: f32
  * [tokens, q_heads] or NULL.  Rows that see no key give 0 and -inf.  clear_rest: rows of no
  * sequence are written the same way, bit 0 those of out, bit 1 those of lse, else left as they were. */
 size_t risa_b200_paged_attention_scratch_size(const risa_b200_cache* cache,

@@ -20,7 +20,7 @@ namespace py = pybind11;
 namespace {
 
 using MaybeTensor = std::optional<at::Tensor>;
-constexpr int kInt8 = 4;
+constexpr int kInt8 = 4, kInt4 = 5;
 constexpr int64_t kMostSlots = RISA_B200_CACHE_MOST_SLOTS;
 
 void check(int status) {
@@ -41,6 +41,7 @@ int code_of(const at::Tensor& t) {
     case at::kHalf: return 1;
     case at::kBFloat16: return 2;
     case at::kChar: return kInt8;
+    case at::kByte: return kInt4;
     default: return -1;
   }
 }
@@ -80,17 +81,26 @@ struct Cache {
   Cache(const at::Tensor& k, const at::Tensor& v, const MaybeTensor& ks, const MaybeTensor& vs)
       : keys(k), values(v), key_scales(ks), value_scales(vs) {
     require(k.dim() == 4 && v.sizes() == k.sizes(),
-            "cache keys and values must both have shape [pages, kv_heads, page_size, head_dim]");
+            "cache keys and values must both have shape [pages, kv_heads, page_size, head_dim] (half of it where a byte holds two 4-bit codes)");
+    const int code = code_of(k);
+    const int64_t head_dim = k.size(3) * (code == kInt4 ? 2 : 1);
     require(k.size(0) > 0 && k.size(1) > 0, "the cache needs pages and heads");
     require(k.size(0) < (int64_t(1) << 31) && k.size(1) <= 65535, "the cache has too many pages or heads");
     require(k.size(2) == 16 || k.size(2) == 32 || k.size(2) == 64 || k.size(2) == 128, "page_size must be 16, 32, 64 or 128");
-    require(k.size(3) == 64 || k.size(3) == 128 || k.size(3) == 256, "head_dim of a cache must be 64, 128 or 256");
-    const int code = code_of(k);
-    require_type(code == 1 || code == 2 || code == kInt8, "cache keys and values must be float16, bfloat16 or int8");
+    require(head_dim == 64 || head_dim == 128 || head_dim == 256, "head_dim of a cache must be 64, 128 or 256");
+    require_type(code == 1 || code == 2 || code == kInt8 || code == kInt4, "cache keys and values must be float16, bfloat16, int8 or uint8 (4-bit codes)");
     require_type(v.scalar_type() == k.scalar_type(), "cache keys and values must have the same dtype");
     require(k.is_contiguous() && v.is_contiguous(), "cache keys and values must be contiguous");
-    require((code == kInt8) == ks.has_value() && (code == kInt8) == vs.has_value(),
-            "an int8 cache needs key_scales and value_scales, any other has none");
+    const bool codes = code == kInt8 || code == kInt4;
+    require(codes == ks.has_value() && codes == vs.has_value(), "a cache of codes needs key_scales and value_scales, any other has none");
+    if (code == kInt4) {
+      for (const at::Tensor* s : {&*ks, &*vs}) {
+        require_type(s->scalar_type() == at::kByte, "scales of 4-bit codes must be uint8");
+        require(s->dim() == 3 && s->size(0) == k.size(0) && s->size(1) == k.size(1) && s->size(2) == k.size(2) * (1 + head_dim / 16) && s->is_contiguous(),
+                "scales of 4-bit codes must be contiguous [pages, kv_heads, page_size * (1 + head_dim / 16)]");
+        require(s->device() == k.device(), "scales must be on the device of the cache");
+      }
+    }
     if (code == kInt8) {
       for (const at::Tensor* s : {&*ks, &*vs}) {
         require_type(s->scalar_type() == at::kFloat, "scales must be float32");
@@ -102,12 +112,12 @@ struct Cache {
     require(v.device() == k.device(), "cache keys and values must be on the same device");
     c.keys = k.data_ptr();
     c.values = v.data_ptr();
-    c.key_scales = code == kInt8 ? ks->data_ptr<float>() : nullptr;
-    c.value_scales = code == kInt8 ? vs->data_ptr<float>() : nullptr;
+    c.key_scales = codes ? static_cast<float*>(ks->data_ptr()) : nullptr;
+    c.value_scales = codes ? static_cast<float*>(vs->data_ptr()) : nullptr;
     c.pages = int(k.size(0));
     c.kv_heads = int(k.size(1));
     c.page_size = int(k.size(2));
-    c.head_dim = int(k.size(3));
+    c.head_dim = int(head_dim);
     c.dtype_code = code;
   }
 };
@@ -293,7 +303,7 @@ MaybeTensor cache_append(const at::Tensor& cache_keys, const at::Tensor& cache_v
   const int code = code_of(k);
   require_type(code == 1 || code == 2, "k and v must be float16 or bfloat16");
   require_type(v.scalar_type() == k.scalar_type() && (!q.has_value() || q->scalar_type() == k.scalar_type()), "q, k and v must have the same dtype");
-  require_type(cache.c.dtype_code == kInt8 || cache.c.dtype_code == code, "k and v must have the dtype of the cache");
+  require_type(cache.c.dtype_code >= kInt8 || cache.c.dtype_code == code, "k and v must have the dtype of the cache");
   if (positions.has_value()) {
     require_positions(*positions);
     require(positions->is_contiguous(), "positions must be contiguous");
@@ -330,6 +340,24 @@ MaybeTensor cache_append(const at::Tensor& cache_keys, const at::Tensor& cache_v
   return out;
 }
 
+// Keys and values [tokens, kv_heads, head_dim] of a step's tokens, as the cache holds them.
+py::tuple cache_read(const at::Tensor& cache_keys, const at::Tensor& cache_values, const MaybeTensor& key_scales, const MaybeTensor& value_scales,
+                     const at::Tensor& table, const at::Tensor& lengths, const MaybeTensor& offsets, int64_t tokens,
+                     std::optional<at::ScalarType> dtype, uintptr_t stream_ptr) {
+  const Cache cache(cache_keys, cache_values, key_scales, value_scales);
+  const at::ScalarType type = dtype.value_or(cache_keys.scalar_type());
+  require(dtype.has_value() || cache.c.dtype_code < kInt8, "a cache of codes is read as float16 or bfloat16: say which");
+  require_type(type == at::kHalf || type == at::kBFloat16, "keys and values are read as float16 or bfloat16");
+  require_type(cache.c.dtype_code >= kInt8 || type == cache_keys.scalar_type(), "keys and values must be read in the dtype of the cache");
+  const Step step(cache, table, lengths, offsets, tokens);
+  require_cuda(cache_keys);
+  const c10::DeviceGuard on_device(cache_keys.device());
+  const at::Tensor k = at::empty({tokens, cache.c.kv_heads, cache.c.head_dim}, cache_keys.options().dtype(type)), v = at::empty_like(k);
+  const Strides2 ks(k), vs(v);
+  check(risa_b200_cache_read(&cache.c, &step.s, k.data_ptr(), ks.of, v.data_ptr(), vs.of, code_of(k), stream_of(stream_ptr)));
+  return py::make_tuple(k, v);
+}
+
 // Checks that attention and key weights share.
 void check_queries(const Cache& cache, const at::Tensor& q, const std::optional<int64_t>& window, int64_t sinks, bool is_causal) {
   require(q.dim() == 3 && q.size(2) == cache.c.head_dim, "q must have shape [tokens, q_heads, head_dim of the cache]");
@@ -341,7 +369,7 @@ void check_queries(const Cache& cache, const at::Tensor& q, const std::optional<
   require(sinks >= 0 && sinks < (int64_t(1) << 31), "sinks must not be negative");
   require(sinks == 0 || window.has_value(), "sinks stay visible in front of a window, and there is none");
   require_type(code_of(q) == 1 || code_of(q) == 2, "q must be float16 or bfloat16");
-  require_type(cache.c.dtype_code == kInt8 || cache.c.dtype_code == code_of(q), "q must have the dtype of the cache");
+  require_type(cache.c.dtype_code >= kInt8 || cache.c.dtype_code == code_of(q), "q must have the dtype of the cache");
 }
 
 py::tuple paged_attention(const at::Tensor& q, const at::Tensor& cache_keys, const at::Tensor& cache_values, const MaybeTensor& key_scales,
@@ -441,6 +469,7 @@ void bind_cache(py::module_& m) {
   m.def("rotate", &rotate);
   m.def("rotate_with_gradient", &rotate_with_gradient);
   m.def("cache_append", &cache_append);
+  m.def("cache_read", &cache_read);
   m.def("paged_attention", &paged_attention);
   m.def("key_weights", &key_weights);
   m.def("cache_evict", &cache_evict);

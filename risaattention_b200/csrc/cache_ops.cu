@@ -1,5 +1,6 @@
 // Rotary positions, the append that fills a paged key/value cache, and eviction from it: the serving
 // operators that move data.  All are bounded by memory traffic (large) or by launch latency (steps).
+#include "four_bits.cuh"
 #include "paged_tc.cuh"
 #include "serving.cuh"
 
@@ -271,6 +272,104 @@ __device__ __forceinline__ float row_absmax(const float* x, int lanes) {
   return m;
 }
 
+// A row in 4 bits (four_bits.cuh): this lane's eight channels, the scale of its group and the token's exponent.
+struct Row4 {
+  uint32_t word, group;
+  int exponent;
+};
+// The token's scale is the smallest power of two, 2^-126 at least, of which the row's largest value is at most 3136 = 7 * 448.
+constexpr uint32_t kAbove3136 = 0x7fffffu - 0x440000u;  // carries into the exponent where the mantissa is above that of 3136
+__device__ __forceinline__ uint32_t e4m3_pair(float hi, float lo) {
+  uint16_t r;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// Channel 2 i + j in bits 16 j + 4 i.
+__device__ __forceinline__ uint32_t code_bits(int code, int channel) { return uint32_t(min(max(code, -7), 7) + 8) << (16 * (channel & 1) + 4 * (channel >> 1)); }
+
+// Group scale: the largest value of the group over 7 token scales, rounded to e4m3.  Code: the value over both scales, rounded
+// to nearest even.  Values of 16 bits meet the borders between codes (and between scales) exactly or not nearly, so that
+// for rows as they came this is decided in 32 bits: the quotient by 7 is correctly rounded, and a value's distance from the
+// border below it comes from one fused multiply-add, whose sign is right.  Rotated values are off by 2^-20 of the row's largest
+// value at most (cosine and sine 2^-22 each, of a pair whose length is sqrt(2) times that at most); `doubtful` says that one of
+// them lies within twice that of a border.
+__device__ __forceinline__ Row4 row4_of(const float (&x)[8], int lanes, bool& doubtful) {
+  Row4 r;
+  float group = fabsf(x[0]);
+#pragma unroll
+  for (int i = 1; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(group) : "f"(fabsf(x[i])));
+  asm("max.NaN.f32 %0, %0, %1;" : "+f"(group) : "f"(__shfl_xor_sync(0xffffffffu, group, 1)));
+  float most = group;
+  for (int off = lanes >> 1; off > 1; off >>= 1)
+    asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(__shfl_xor_sync(0xffffffffu, most, off)));
+  const uint32_t bits = __float_as_uint(most) + kAbove3136;
+  r.exponent = most == 0.f ? 0 : !(most < INFINITY) ? 255 : max(int(bits >> 23) - 11, 1);
+  r.word = 0x88888888u;
+  r.group = 0;
+  doubtful = false;
+  if (r.exponent == 0 || r.exponent == 255) return r;
+  const float to_units = __uint_as_float(uint32_t(254 - r.exponent) << 23), slack = most * to_units * 0x1p-19f;
+  const float ratio = __fdiv_rn(group * to_units, 7.0f);
+  r.group = e4m3_pair(0.f, ratio) & 0xffu;
+  const uint32_t around = e4m3_pair(ratio + slack, fmaxf(ratio - slack, 0.f));
+  doubtful = (around & 0xffu) != around >> 8 || (bits - 16) >> 23 != (bits + 16) >> 23;
+  if (r.group == 0) return r;
+  const uint32_t half_bits = r.group << 7;
+  const float scale = __half2float(__ushort_as_half(uint16_t(half_bits))) * kGroupUnit, inverse = 1.0f / scale;
+  r.word = 0;
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const float y = x[i] * to_units, below = floorf(y * inverse), past = fmaf(-(below + 0.5f), scale, y);
+    const int code = int(below);
+    r.word |= code_bits(code + (past > 0.f || (past == 0.f && (code & 1)) ? 1 : 0), i);
+    doubtful = doubtful || fabsf(past) < slack;
+  }
+  return r;
+}
+// The same for a rotated row that came too near a border, in 64 bits: from the channels as they came (`own`, and `other` of a
+// lane half a rotated row away).  About one row in a hundred.
+template <typename T>
+__device__ __noinline__ Row4 row4_of_rotated(const AppendArgs& a, Run<T> own, Run<T> other, int64_t token, int place, int lanes, int channel) {
+  float u[8], v[8];
+  own.values(u);
+  other.values(v);
+  double x[8], most = 0.0;
+  const int half = a.rotary_dim >> 1;
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) {
+    const int c = channel + i;
+    x[i] = u[i];
+    if (c < a.rotary_dim) {
+      const bool second = a.interleaved ? c & 1 : c >= half;
+      const int pair = a.interleaved ? c >> 1 : second ? c - half : c;
+      const int64_t axis = a.axes != nullptr ? min(int(__ldg(a.axes + pair)), a.last_axis) * a.axis_stride : 0;
+      const int64_t position = a.positions ? position_at(a.positions, a.positions_64, token + axis) : int64_t(place);
+      const uint64_t angle = uint64_t(position) * __ldg(reinterpret_cast<const unsigned long long*>(a.turns) + pair);
+      double sine, cosine;
+      sincospi(double(int64_t(angle)) * 0x1p-63, &sine, &cosine);
+      const double partner = a.interleaved ? u[i ^ 1] : v[i];
+      x[i] = double(a.magnitude) * (u[i] * cosine + (second ? partner : -partner) * sine);
+    }
+    most = fmax(most, fabs(x[i]));
+  }
+  const double group = fmax(most, __shfl_xor_sync(0xffffffffu, most, 1));
+  most = group;
+  for (int off = lanes >> 1; off > 1; off >>= 1) most = fmax(most, __shfl_xor_sync(0xffffffffu, most, off));
+  Row4 r{0x88888888u, 0, 0};
+  if (most == 0.0) return r;
+  r.exponent = max(int((__double_as_longlong(most) + (0xfffffffffffffll - 0x8800000000000ll)) >> 52) - 1023 - 11 + 127, 1);
+  const double to_units = __longlong_as_double(int64_t(1023 + 127 - r.exponent) << 52), ratio = group * to_units / 7.0;
+  // steps of 2^-3 of the leading bit, 2^-9 at least
+  const double step = __longlong_as_double(int64_t(max(int(__double_as_longlong(ratio) >> 52) - 3, 1023 - 9)) << 52);
+  const double scale = rint(ratio / step) * step;
+  r.group = e4m3_pair(0.f, float(scale)) & 0xffu;
+  if (scale == 0.0) return r;
+  r.word = 0;
+#pragma unroll 1
+  for (int i = 0; i < 8; ++i) r.word |= code_bits(int(rint(x[i] * to_units / scale)), i);
+  return r;
+}
+
 // One CTA per new token.  head_dim / 8 lanes hold a row, eight channels each; the CTA's row slots walk
 // the token's query heads, key heads and value heads with the cosines and sines of the lane's channels
 // kept in registers.  A thread computes those of one pair for the whole token (8160 tokens below: 70 us where every lane
@@ -281,7 +380,7 @@ __device__ __forceinline__ float row_absmax(const float* x, int lanes) {
 // 56 us (184 MB, 3.3 TB/s), bound by each CTA's chain of lookups and by the instructions of conversions; one token of 64
 // requests, with the call: 11.5 to 12.4 us.
 constexpr int kRowsAhead = 3;  // rows of a slot on their way at once: half of a token of 32 + 2 x 8 heads of 128
-template <typename T, bool INT8>
+template <typename T, int BITS>
 __global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
   __shared__ __align__(16) float cosines[128], sines[128];
   chain_wait();
@@ -373,6 +472,8 @@ __global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
       const int h = kind == 0 ? r : kind == 1 ? r - a.q_heads : r - a.q_heads - a.kv_heads;
       float x[8];
       run[j].values(x);
+      Run<T> other;
+      other.zero();
       if (a.turns != nullptr && __any_sync(0xffffffffu, kind < 2)) {
         if (a.interleaved) {
           if (turned && kind < 2) {
@@ -384,7 +485,6 @@ __global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
             }
           }
         } else {
-          Run<T> other;
           other.raw.x = __shfl_sync(0xffffffffu, run[j].raw.x, partner);
           other.raw.y = __shfl_sync(0xffffffffu, run[j].raw.y, partner);
           other.raw.z = __shfl_sync(0xffffffffu, run[j].raw.z, partner);
@@ -398,7 +498,22 @@ __global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
         }
       }
       const int64_t row = ((page * a.kv_heads + h) << a.step.page_shift) + slot_in_page;
-      if (INT8 && __any_sync(0xffffffffu, kind > 0)) {
+      if (BITS == 4 && __any_sync(0xffffffffu, kind > 0)) {
+        bool doubtful;
+        Row4 r4 = row4_of(x, lanes, doubtful);
+        if (a.turns != nullptr && __any_sync(0xffffffffu, doubtful && there && kind == 1)) {
+          const Row4 sure = row4_of_rotated<T>(a, run[j], other, token, place, lanes, channel);
+          if (kind == 1 && r4.exponent != 255) r4 = sure;
+        }
+        if (there && kind > 0 && page >= 0) {
+          reinterpret_cast<uint32_t*>(kind == 1 ? a.keys : a.values)[row * lanes + lane] = r4.word;
+          const int groups = lanes >> 1;
+          uint8_t* scales = reinterpret_cast<uint8_t*>(kind == 1 ? a.key_scales : a.value_scales) + (((page * a.kv_heads + h) * (1 + groups)) << a.step.page_shift);
+          if (lane == 0) scales[slot_in_page] = uint8_t(r4.exponent);
+          if ((lane & 1) == 0) scales[(1 << a.step.page_shift) + slot_in_page * groups + (lane >> 1)] = uint8_t(r4.group);
+        }
+      }
+      if (BITS == 8 && __any_sync(0xffffffffu, kind > 0)) {
         const float most = row_absmax(x, lanes), scale = most / 127.0f;
         if (there && kind > 0 && page >= 0) {
           // one reciprocal for the row; rows so small that it would overflow are divided
@@ -411,11 +526,94 @@ __global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
               make_uint2(pack4_s8(c[0], c[1], c[2], c[3]), pack4_s8(c[4], c[5], c[6], c[7]));
           if (lane == 0) (kind == 1 ? a.key_scales : a.value_scales)[row] = scale;
         }
-      } else if (!INT8 && there && kind > 0 && page >= 0) {
+      }
+      if (BITS == 16 && there && kind > 0 && page >= 0) {
         store8(static_cast<T*>(kind == 1 ? a.keys : a.values) + row * a.head_dim + channel, x);
       }
       if (there && kind == 0) store8(static_cast<T*>(a.q_out) + token * a.on + h * a.oh + channel, x);
     }
+  }
+}
+
+// ---- reading back -----------------------------------------------------------------------------------------
+struct ReadArgs {
+  StepView step;
+  const void* keys;
+  const void* values;
+  const float* key_scales;
+  const float* value_scales;
+  void *k, *v;
+  int64_t kn, kh, vn, vh;
+  int pages, kv_heads, head_dim;
+  unsigned int* status;
+};
+
+// One CTA per token of a step, as append has them; head_dim / 8 lanes hold a row.
+template <typename T, int BITS>
+__global__ __launch_bounds__(128) void read_kernel(const ReadArgs a) {
+  chain_wait();
+  chain_release();
+  const int token = blockIdx.x, lanes = a.head_dim >> 3;
+  const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes, slots = 128 / lanes;
+  int s = token;
+  if (a.step.offsets != nullptr) {
+    s = 0;
+    for (int i = 0; i < a.step.batch; i += 128)
+      s += __syncthreads_count(i + int(threadIdx.x) < a.step.batch && __ldg(a.step.offsets + i + threadIdx.x + 1) <= token);
+  }
+  int64_t page = -1;
+  int place = -1;
+  if (s < a.step.batch && (a.step.offsets == nullptr || token >= __ldg(a.step.offsets + s))) {
+    place = __ldg(a.step.lengths + s) - ((a.step.offsets ? __ldg(a.step.offsets + s + 1) : s + 1) - token);
+    if (place >= 0) {
+      if ((place >> a.step.page_shift) < a.step.width) page = __ldg(a.step.table + int64_t(s) * a.step.width + (place >> a.step.page_shift));
+      if (page < 0 || page >= a.pages) {
+        page = -1;
+        if (threadIdx.x == 0) atomicCAS(a.status, 0u, unsigned(s) + 1u);
+      }
+    }
+  }
+  const int in_page = place & ((1 << a.step.page_shift) - 1);
+#pragma unroll 4
+  for (int r = slot; r < 2 * a.kv_heads; r += slots) {
+    const bool is_key = r < a.kv_heads;
+    const int h = is_key ? r : r - a.kv_heads;
+    T* out = (is_key ? static_cast<T*>(a.k) + token * a.kn + h * a.kh : static_cast<T*>(a.v) + token * a.vn + h * a.vh) + lane * 8;
+    uint4 raw = make_uint4(0, 0, 0, 0);
+    if (page >= 0) {
+      const int64_t row = ((page * a.kv_heads + h) << a.step.page_shift) + in_page;
+      const void* pool = is_key ? a.keys : a.values;
+      const float* scales = is_key ? a.key_scales : a.value_scales;
+      if (BITS == 16) {
+        raw = reinterpret_cast<const uint4*>(pool)[row * lanes + lane];
+      } else {
+        float x[8], scale;
+        if (BITS == 8) {
+          const uint2 w = reinterpret_cast<const uint2*>(pool)[row * lanes + lane];
+          scale = __ldg(scales + row);
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = float(int8_t((i < 4 ? w.x : w.y) >> (8 * (i & 3))));
+        } else {
+          const uint32_t w = reinterpret_cast<const uint32_t*>(pool)[row * lanes + lane];
+          const int groups = lanes >> 1;
+          const uint8_t* of = reinterpret_cast<const uint8_t*>(scales) + (((page * a.kv_heads + h) * (1 + groups)) << a.step.page_shift);
+          const GroupScale<__half> group(twice(__ldg(of + (1 << a.step.page_shift) + in_page * groups + (lane >> 1))));
+          scale = power_of(__ldg(of + in_page)) * kGroupUnit;
+          uint32_t pairs[4];
+          scaled_codes(w, group, pairs);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 f = Half2<__half>::unpack(pairs[i]);
+            x[2 * i] = f.x;
+            x[2 * i + 1] = f.y;
+          }
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] *= scale;
+        store8(reinterpret_cast<T*>(&raw), x);
+      }
+    }
+    *reinterpret_cast<uint4*>(out) = raw;
   }
 }
 
@@ -565,6 +763,7 @@ struct MoveArgs {
   float* key_scales;
   float* value_scales;
   int pages, kv_heads, budget, target_width, row_shift;  // a row is 16 << row_shift bytes
+  int groups;                                            // 4-bit codes: of a row
   unsigned int* status;
 };
 
@@ -620,7 +819,17 @@ __global__ __launch_bounds__(256) void move_kept_kernel(const MoveArgs a) {
       const int64_t byte = (to[i] << (a.row_shift + 4)) + piece * 16;
       *reinterpret_cast<uint4*>(a.keys + byte) = key[i];
       *reinterpret_cast<uint4*>(a.values + byte) = value[i];
-      if (a.key_scales != nullptr && piece == 0) {
+      if (a.groups > 0 && piece < 2) {  // the first two threads of a row take the scales of a pool each
+        auto scales = [&](int64_t row) {
+          return reinterpret_cast<uint8_t*>(piece == 0 ? a.key_scales : a.value_scales) + (((row >> a.step.page_shift) * (1 + a.groups)) << a.step.page_shift);
+        };
+        uint8_t *f = scales(from[i]), *t = scales(to[i]);
+        const int fs = int(from[i]) & in_page, ts = int(to[i]) & in_page;
+        t[ts] = f[fs];
+        f += (1 << a.step.page_shift) + fs * a.groups;
+        t += (1 << a.step.page_shift) + ts * a.groups;
+        for (int g = 0; g < a.groups; g += 4) *reinterpret_cast<uint32_t*>(t + g) = *reinterpret_cast<const uint32_t*>(f + g);
+      } else if (a.key_scales != nullptr && a.groups == 0 && piece == 0) {
         a.key_scales[to[i]] = a.key_scales[from[i]];
         a.value_scales[to[i]] = a.value_scales[from[i]];
       }
@@ -707,10 +916,10 @@ extern "C" int risa_b200_cache_append_axes(const risa_b200_cache* cache, const r
                                            const void* positions, int positions_64, void* stream_ptr) {
   if (const int bad = check_cache(cache, "append")) return bad;
   if (const int bad = check_step(step, cache, "append")) return bad;
-  const bool codes = cache->dtype_code == kInt8;
+  const int bits = bits_of(*cache);
   RISA_REQUIRE(k && v && (q == nullptr) == (q_out == nullptr), "append: null tensor");
   RISA_REQUIRE(dtype_code == 1 || dtype_code == 2, "append: q, k and v must be float16 or bfloat16");
-  RISA_REQUIRE(codes || dtype_code == cache->dtype_code, "append: k and v must have the cache's type");
+  RISA_REQUIRE(bits < 16 || dtype_code == cache->dtype_code, "append: k and v must have the cache's type");
   RISA_REQUIRE(q == nullptr || rotary != nullptr, "append: q is only rotated, and there is no rotary table");
   RISA_REQUIRE(q == nullptr || q_heads > 0, "append: q needs heads");
   if (rotary != nullptr) {
@@ -765,9 +974,28 @@ extern "C" int risa_b200_cache_append_axes(const risa_b200_cache* cache, const r
     }
   }
   a.status = status;
-  const auto kernel = dtype_code == 1 ? (codes ? append_kernel<__half, true> : append_kernel<__half, false>)
-                                      : (codes ? append_kernel<__nv_bfloat16, true> : append_kernel<__nv_bfloat16, false>);
+  const auto kernel = dtype_code == 1 ? (bits == 4 ? append_kernel<__half, 4> : bits == 8 ? append_kernel<__half, 8> : append_kernel<__half, 16>)
+                                      : (bits == 4 ? append_kernel<__nv_bfloat16, 4> : bits == 8 ? append_kernel<__nv_bfloat16, 8> : append_kernel<__nv_bfloat16, 16>);
   return launched(launch_chained(kernel, dim3(step->tokens), dim3(128), 0, static_cast<cudaStream_t>(stream_ptr), a), "append");
+}
+
+extern "C" int risa_b200_cache_read(const risa_b200_cache* cache, const risa_b200_step* step, void* k, const int64_t ks[2], void* v,
+                                    const int64_t vs[2], int dtype_code, void* stream_ptr) {
+  if (const int bad = check_cache(cache, "read")) return bad;
+  if (const int bad = check_step(step, cache, "read")) return bad;
+  const int bits = bits_of(*cache);
+  RISA_REQUIRE(k && v, "read: null tensor");
+  RISA_REQUIRE(dtype_code == 1 || dtype_code == 2, "read: keys and values are read as float16 or bfloat16");
+  RISA_REQUIRE(bits < 16 || dtype_code == cache->dtype_code, "read: keys and values must have the cache's type");
+  RISA_REQUIRE((reinterpret_cast<uintptr_t>(k) | reinterpret_cast<uintptr_t>(v)) % 16 == 0 && (ks[0] | ks[1] | vs[0] | vs[1]) % 8 == 0,
+               "read: rows must start on 16-byte boundaries");
+  unsigned int* status = status_word();
+  if (status == nullptr) return RISA_B200_CUDA;
+  const ReadArgs a{view_of(*step, cache->page_size), cache->keys, cache->values, cache->key_scales, cache->value_scales, k, v,
+                   ks[0], ks[1], vs[0], vs[1], cache->pages, cache->kv_heads, cache->head_dim, status};
+  const auto kernel = dtype_code == 1 ? (bits == 4 ? read_kernel<__half, 4> : bits == 8 ? read_kernel<__half, 8> : read_kernel<__half, 16>)
+                                      : (bits == 4 ? read_kernel<__nv_bfloat16, 4> : bits == 8 ? read_kernel<__nv_bfloat16, 8> : read_kernel<__nv_bfloat16, 16>);
+  return launched(launch_chained(kernel, dim3(step->tokens), dim3(128), 0, static_cast<cudaStream_t>(stream_ptr), a), "read");
 }
 
 extern "C" int risa_b200_cache_evict(const risa_b200_cache* cache, const risa_b200_step* step,
@@ -793,12 +1021,12 @@ extern "C" int risa_b200_cache_evict(const risa_b200_cache* cache, const risa_b2
                           target_width * cache->page_size};
   if (const int bad = launched(launch_chained(select_kept_kernel, dim3(cache->kv_heads, step->batch), dim3(kSelectThreads), 0, stream, select), "evict"))
     return bad;
-  const int row_bytes = cache->head_dim * (cache->dtype_code == kInt8 ? 1 : 2);
+  const int row_bytes = cache->head_dim * bits_of(*cache) / 8;
   int shift = 0;
   while ((16 << shift) < row_bytes) ++shift;
   const MoveArgs move{view, target_table, kept, static_cast<char*>(cache->keys), static_cast<char*>(cache->values),
                       cache->key_scales, cache->value_scales, cache->pages, cache->kv_heads, budget, target_width,
-                      shift, status};
+                      shift, cache->dtype_code == kInt4 ? cache->head_dim / 16 : 0, status};
   const int rows = (256 >> shift) * kMoveRows;
   return launched(launch_chained(move_kept_kernel, dim3((budget + rows - 1) / rows, cache->kv_heads, step->batch), dim3(256), 0, stream, move), "evict");
 }

@@ -15,6 +15,7 @@
 // Measured: 16 requests of up to 16K keys, 8 key heads of 128 bf16 channels, 110 us (6.1 TB/s, 95 % of a plain copy's rate);
 // 32 requests of up to 32K keys as codes 244 us at full clocks (5.7 TB/s), 280 in long runs, where the conversion's
 // instructions (schedulers 61 % busy) feel the lower clock.
+#include "four_bits.cuh"
 #include "paged_tc.cuh"
 #include "serving_plan.cuh"
 
@@ -52,38 +53,44 @@ struct RowsArgs {
 };
 // FRONT: first keys stay visible in front of the window (the walk over the keys then has a gap; all others are spared its
 // instructions, which cost 32 requests of up to 32K codes 263 -> 302 us).
-template <typename T_, bool INT8_, int D_, int NT_, bool FRONT_>
+template <typename T_, int BITS_, int D_, int NT_, bool FRONT_>
 struct Tile {
   using T = T_;
   static constexpr bool FRONT = FRONT_;
   using Line = std::conditional_t<FRONT, FrontLineArgs, LineArgs>;
-  static constexpr bool INT8 = INT8_;
+  static constexpr int BITS = BITS_;
+  static constexpr bool CODES = BITS < 16;
   static constexpr int D = D_, NT = NT_, R = 8 * NT_;
-  using M = std::conditional_t<INT8_, __half, T_>;  // type of the matrix instructions' operands
-  static constexpr int ROW = D * (INT8 ? 1 : 2);  // bytes of a key
+  using M = std::conditional_t<CODES, __half, T_>;  // type of the matrix instructions' operands
+  static constexpr int ROW = D * BITS / 8;  // bytes of a key
   static constexpr int CHUNKS = ROW / 16;
   static constexpr int SIDE = 16 * ROW;  // the 16 keys (or values) of a step
-  static constexpr int SCALES = INT8 ? 128 : 0;
+  // bytes of the scales of a step's keys (or values)
+  static constexpr int SCALES = BITS == 8 ? 16 * 4 : BITS == 4 ? 16 * token_scale_bytes<D>() : 0;
   static constexpr int KS = D / 16;
   // CTAs of four warps that share an SM's shared memory: what hides the latency of HBM is bytes in flight, 96 KB or
   // more per SM.  Codes, whose conversion keeps the schedulers busy, gain from a third CTA (32 requests of up to 32K
   // keys: 280 us with two, 247 with three, 267 with four); 16-bit rows of 256 channels leave room for one.
-  static constexpr int CTAS = D == 256 && !INT8 ? 1 : INT8 && D <= 128 && NT == 1 ? 3 : 2;
+  static constexpr int CTAS = D == 256 && !CODES ? 1 : CODES && D <= 128 && NT == 1 ? 3 : 2;
   static constexpr int BUDGET = 48 * 1024 / CTAS;  // per warp
   __host__ __device__ static constexpr int stages(int sides) {
-    const int n = BUDGET / (sides * SIDE + SCALES);
+    const int n = BUDGET / (sides * (SIDE + SCALES));
     return n > 8 ? 8 : n;
   }
 };
 
 // 16-byte pieces of a row are permuted so that the reads below are free of bank conflicts.  16-bit rows:
 // ldmatrix takes one piece of eight consecutive rows.  Codes: for K eight lanes read four pieces of two
-// consecutive rows, for V two pieces of every other row.
+// consecutive rows, for V two pieces of every other row.  4-bit rows are read the same way, but several of them share 128 bytes
+// (the width of the banks): there the pieces of a line are permuted by the line's number.
 template <typename C>
-__device__ __forceinline__ int swizzled(int row, int piece) {
-  if (!C::INT8) return piece ^ (row & 7);
-  if (C::CHUNKS < 8) return piece;
-  return piece ^ (((row & 1) << 2) ^ (((row >> 1) & 3) << 1));
+__device__ __forceinline__ int offset_of(int row, int piece) {
+  if (C::BITS == 16) return row * C::ROW + (piece ^ (row & 7)) * 16;
+  if (C::ROW >= 128) return row * C::ROW + (piece ^ (((row & 1) << 2) ^ (((row >> 1) & 3) << 1))) * 16;
+  if (C::BITS == 8) return row * C::ROW + piece * 16;
+  constexpr int EACH = 128 / C::ROW;  // rows of a line: 2 or 4
+  const int line = row / EACH, slot = row % EACH * C::CHUNKS + piece;
+  return line * 128 + (slot ^ ((line & (EACH == 2 ? 3 : 1)) << 1)) * 16;
 }
 
 __device__ __forceinline__ uint32_t shared_address(const void* p) {
@@ -121,6 +128,22 @@ __device__ __forceinline__ uint2 read8(uint32_t address) {
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(address) : "memory");
   return v;
 }
+__device__ __forceinline__ uint32_t read4(uint32_t address) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(address) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t read2(uint32_t address) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(address) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t read1(uint32_t address) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(address) : "memory");
+  return v;
+}
+__device__ __forceinline__ void write1(uint32_t address, uint32_t v) { asm volatile("st.shared.u8 [%0], %1;" ::"r"(address), "r"(v) : "memory"); }
 __device__ __forceinline__ float read_float(uint32_t address) {
   float v;
   asm volatile("ld.shared.f32 %0, [%1];" : "=f"(v) : "r"(address) : "memory");
@@ -157,7 +180,8 @@ struct Walk {
   uint32_t base;
   unsigned int hidden;  // one bit per stage
   static constexpr int STAGES = C::stages(WITH_VALUES ? 2 : 1);
-  static constexpr int STAGE = (WITH_VALUES ? 2 : 1) * C::SIDE + C::SCALES;
+  static constexpr int SIDES = WITH_VALUES ? 2 : 1;
+  static constexpr int STAGE = SIDES * (C::SIDE + C::SCALES);  // keys, values, scales of the keys, of the values
   static_assert(STAGES >= 2 && STAGES <= 32, "ring");
 
   __device__ __forceinline__ int key_of(int i) const { return first_key + i * (16 * kWarps) + (C::FRONT && i >= turn ? skip : 0); }
@@ -195,21 +219,47 @@ struct Walk {
         for (int j = 0; j < C::CHUNKS / 2; ++j) {
           const int index = j * 32 + lane, r = index / C::CHUNKS, piece = index % C::CHUNKS;
           const bool there = whole || (good && exists(key + r));
-          const uint32_t at = to + r * C::ROW + swizzled<C>(r, piece) * 16;
+          const uint32_t at = to + offset_of<C>(r, piece);
           copy16(at, k + index * 16, there);
           if (WITH_VALUES) copy16(at + C::SIDE, v + index * 16, there);
         }
-        if (C::INT8) {
+        if (C::BITS == 8 && (WITH_VALUES || lane < 16)) {
           const float* s = lane < 16 ? a.key_scales : a.value_scales;
           const int r = lane & 15;
-          copy4(to + (WITH_VALUES ? 2 : 1) * C::SIDE + lane * 4, s + line + r, whole || (good && exists(key + r)));
+          copy4(to + SIDES * C::SIDE + lane * 4, s + line + r, whole || (good && exists(key + r)));
         }
       };
+      if (C::BITS == 4) {  // exponents, then group scales; those of keys that do not exist are cleared by who reads them
+        constexpr int PIECES = C::SCALES / 16;
+        const int slot = key & ((1 << a.line.step.page_shift) - 1);
+        const int64_t block = good ? scales4<C::D>(nullptr, page, a.line.kv_heads, head, a.line.step.page_shift) - static_cast<const uint8_t*>(nullptr) : 0;
+#pragma unroll
+        for (int j = 0; j < (SIDES * PIECES + 31) / 32; ++j) {
+          const int index = j * 32 + lane, piece = index < PIECES ? index : index - PIECES;
+          const char* from = reinterpret_cast<const char*>(index < PIECES ? a.key_scales : a.value_scales) + block;
+          from += piece == 0 ? slot : (1 << a.line.step.page_shift) + slot * (C::D / 16) + (piece - 1) * 16;
+          if (index < SIDES * PIECES) copy16(to + SIDES * C::SIDE + index * 16, from, good);
+        }
+      }
       // nearly all steps are of 16 keys that exist
       if (good && key >= low && key + 16 <= length) copy(std::true_type{});
       else copy(std::false_type{});
     }
     copies_commit();
+  }
+  // Scales of 4-bit keys that do not exist (they lie beside those that do) become zeros.
+  __device__ __forceinline__ void clear_missing(uint32_t data, int key) const {
+    const int lane = threadIdx.x & 31;
+    if (lane < 16 && !exists(key + lane)) {
+#pragma unroll
+      for (int side = 0; side < SIDES; ++side) {
+        const uint32_t scales = data + SIDES * C::SIDE + side * C::SCALES;
+        write1(scales + lane, 0);
+#pragma unroll
+        for (int i = 0; i < C::D / 16; ++i) write1(scales + 16 + lane * (C::D / 16) + i, 0);
+      }
+    }
+    __syncwarp();
   }
 };
 
@@ -233,13 +283,14 @@ __device__ __forceinline__ void load_queries(const RowsArgs& a, const Sequence& 
                              int64_t(head * a.line.group + h) * a.qh;
 #pragma unroll
     for (int ks = 0; ks < C::KS; ++ks) {
-      const int c0 = C::INT8 ? (ks >> 2) * 64 + t * 16 + (ks & 3) * 4 : ks * 16 + t * 2;
-      const int c1 = C::INT8 ? c0 + 2 : c0 + 8;
+      constexpr int RUN = C::BITS == 4 && C::D >= 128 ? 32 : 16;  // channels that a lane takes at once
+      const int c0 = C::CODES ? ks / (RUN / 4) * (4 * RUN) + t * RUN + ks % (RUN / 4) * 4 : ks * 16 + t * 2;
+      const int c1 = C::CODES ? c0 + 2 : c0 + 8;
       qf[nt][ks][0] = there ? *reinterpret_cast<const uint32_t*>(q + c0) : 0u;
       qf[nt][ks][1] = there ? *reinterpret_cast<const uint32_t*>(q + c1) : 0u;
     }
     factor[nt][0] = factor[nt][1] = a.scale_log2;
-    if constexpr (C::INT8 && std::is_same<typename C::T, __nv_bfloat16>::value) {
+    if constexpr (C::CODES && std::is_same<typename C::T, __nv_bfloat16>::value) {
       uint32_t most = 0;  // bits of the largest magnitude
 #pragma unroll
       for (int ks = 0; ks < C::KS; ++ks)
@@ -263,19 +314,56 @@ __device__ __forceinline__ void load_queries(const RowsArgs& a, const Sequence& 
   }
 }
 
-// acc[nt]: raw scores of keys g and g + 8 against query rows 2 t and 2 t + 1 (of column block nt).
+// acc[nt]: raw scores of keys g and g + 8 against query rows 2 t and 2 t + 1 (of column block nt); scales: of 4-bit keys.
 template <typename C>
-__device__ __forceinline__ void score_step(uint32_t keys, const uint32_t (&qf)[C::NT][C::KS][2], float (&acc)[C::NT][4]) {
+__device__ __forceinline__ void score_step(uint32_t keys, uint32_t scales, const uint32_t (&qf)[C::NT][C::KS][2], float (&acc)[C::NT][4]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
 #pragma unroll
   for (int nt = 0; nt < C::NT; ++nt)
 #pragma unroll
     for (int i = 0; i < 4; ++i) acc[nt][i] = 0.f;
-  if constexpr (C::INT8) {
+  if constexpr (C::BITS == 4) {
+    // a lane takes 16 channels (a group) of heads of 64, else 32 (two groups) at a time
+    constexpr int RUNS = C::D == 256 ? 2 : 1, WORDS = C::D == 64 ? 2 : 4, GROUPS = WORDS / 2;
+#pragma unroll
+    for (int run = 0; run < RUNS; ++run) {
+      uint32_t w[2][WORDS], scale[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int key = g + 8 * i;
+        if constexpr (WORDS == 4) {
+          const uint4 v = read16(keys + offset_of<C>(key, run * 4 + t));
+          w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
+          scale[i] = read2(scales + 16 + key * (C::D / 16) + run * 8 + t * 2);
+        } else {
+          const uint2 v = read8(keys + offset_of<C>(key, t >> 1) + (t & 1) * 8);
+          w[i][0] = v.x; w[i][1] = v.y;
+          scale[i] = read1(scales + 16 + key * (C::D / 16) + t);
+        }
+      }
+#pragma unroll
+      for (int group = 0; group < GROUPS; ++group) {
+        const GroupScale<__half> lo(twice(GROUPS == 1 ? scale[0] : group ? scale[0] >> 8 : scale[0] & 0xffu));
+        const GroupScale<__half> hi(twice(GROUPS == 1 ? scale[1] : group ? scale[1] >> 8 : scale[1] & 0xffu));
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          uint32_t l[4], h[4];
+          scaled_codes(w[0][2 * group + j], lo, l);
+          scaled_codes(w[1][2 * group + j], hi, h);
+#pragma unroll
+          for (int half = 0; half < 2; ++half) {
+            const uint32_t af[4] = {l[2 * half], h[2 * half], l[2 * half + 1], h[2 * half + 1]};
+#pragma unroll
+            for (int nt = 0; nt < C::NT; ++nt) mma16816<__half>(acc[nt], af, qf[nt][run * 8 + group * 4 + j * 2 + half]);
+          }
+        }
+      }
+    }
+  } else if constexpr (C::BITS == 8) {
 #pragma unroll
     for (int b = 0; b < C::D / 64; ++b) {
-      const uint4 lo = read16(keys + g * C::ROW + swizzled<C>(g, b * 4 + t) * 16);
-      const uint4 hi = read16(keys + (g + 8) * C::ROW + swizzled<C>(g + 8, b * 4 + t) * 16);
+      const uint4 lo = read16(keys + offset_of<C>(g, b * 4 + t));
+      const uint4 hi = read16(keys + offset_of<C>(g + 8, b * 4 + t));
       const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -290,7 +378,7 @@ __device__ __forceinline__ void score_step(uint32_t keys, const uint32_t (&qf)[C
 #pragma unroll
     for (int ks = 0; ks < C::KS; ++ks) {
       uint32_t af[4];
-      ldmatrix4(af, keys + r * C::ROW + swizzled<C>(r, 2 * ks + (lane >> 4)) * 16);
+      ldmatrix4(af, keys + offset_of<C>(r, 2 * ks + (lane >> 4)));
 #pragma unroll
       for (int nt = 0; nt < C::NT; ++nt) mma16816<typename C::T>(acc[nt], af, qf[nt][ks]);
     }
@@ -298,11 +386,51 @@ __device__ __forceinline__ void score_step(uint32_t keys, const uint32_t (&qf)[C
 }
 
 // out[nt][mt] += V^T P^T.  16-bit values: block mt holds channels 16 mt + g (and + 8).  Codes: a lane takes
-// the channels of its own 16-byte pieces (8 bytes at 64 channels), two per instruction: see channel_of.
+// the channels of its own 16-byte pieces (8 bytes at 64 channels; 4-bit codes half of that), two per instruction: see channel_of.
 template <typename C>
-__device__ __forceinline__ void value_step(uint32_t values, const uint32_t (&p)[C::NT][2], float (&out)[C::NT][C::D / 16][4]) {
+__device__ __forceinline__ void value_step(uint32_t values, uint32_t scales, const uint32_t (&p)[C::NT][2], float (&out)[C::NT][C::D / 16][4]) {
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
-  if constexpr (C::INT8) {
+  if constexpr (C::BITS == 4) {
+    constexpr int WORDS = C::D / 64;  // of a key: half a group, a group or two groups
+    uint32_t w[4][WORDS], scale[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int key = 2 * t + (i & 1) + (i >> 1) * 8;
+      const uint32_t of = scales + 16 + key * (C::D / 16);
+      if constexpr (WORDS == 4) {
+        const uint4 v = read16(values + offset_of<C>(key, g));
+        w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
+        scale[i] = read2(of + 2 * g);
+      } else if constexpr (WORDS == 2) {
+        const uint2 v = read8(values + offset_of<C>(key, g >> 1) + (g & 1) * 8);
+        w[i][0] = v.x; w[i][1] = v.y;
+        scale[i] = read1(of + g);
+      } else {
+        w[i][0] = read4(values + offset_of<C>(key, g >> 2) + (g & 3) * 4);
+        scale[i] = read1(of + (g >> 1));
+      }
+    }
+#pragma unroll
+    for (int group = 0; group < (WORDS + 1) / 2; ++group) {
+      // the scales of keys 2 t and 2 t + 1, of 2 t + 8 and 2 t + 9
+      const GroupScale<__half> near(__byte_perm(scale[0], scale[1], WORDS < 4 ? 0x7470 : group ? 0x3531 : 0x3430) & 0x00ff00ffu);
+      const GroupScale<__half> far(__byte_perm(scale[2], scale[3], WORDS < 4 ? 0x7470 : group ? 0x3531 : 0x3430) & 0x00ff00ffu);
+#pragma unroll
+      for (int j = 2 * group; j < 2 * group + 2 && j < WORDS; ++j) {
+        uint32_t x[4][4];  // even channels of near keys, odd ones; of far keys
+        scaled_codes(__byte_perm(w[0][j], w[1][j], 0x5410), near, x[0]);
+        scaled_codes(__byte_perm(w[0][j], w[1][j], 0x7632), near, x[1]);
+        scaled_codes(__byte_perm(w[2][j], w[3][j], 0x5410), far, x[2]);
+        scaled_codes(__byte_perm(w[2][j], w[3][j], 0x7632), far, x[3]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {  // channels 2 e and 2 e + 1 of the word
+          const uint32_t af[4] = {x[0][e], x[1][e], x[2][e], x[3][e]};
+#pragma unroll
+          for (int nt = 0; nt < C::NT; ++nt) mma16816<__half>(out[nt][j * 4 + e], af, p[nt]);
+        }
+      }
+    }
+  } else if constexpr (C::BITS == 8) {
     constexpr int RUNS = C::D == 256 ? 2 : 1, WORDS = C::D == 64 ? 2 : 4;
 #pragma unroll
     for (int run = 0; run < RUNS; ++run) {
@@ -311,7 +439,7 @@ __device__ __forceinline__ void value_step(uint32_t values, const uint32_t (&p)[
       for (int i = 0; i < 4; ++i) {
         const int key = 2 * t + (i & 1) + (i >> 1) * 8;
         if constexpr (WORDS == 4) {
-          const uint4 v = read16(values + key * C::ROW + swizzled<C>(key, g + 8 * run) * 16);
+          const uint4 v = read16(values + offset_of<C>(key, g + 8 * run));
           w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
         } else {
           const uint2 v = read8(values + key * C::ROW + g * 8);
@@ -334,7 +462,7 @@ __device__ __forceinline__ void value_step(uint32_t values, const uint32_t (&p)[
 #pragma unroll
     for (int mt = 0; mt < C::D / 16; ++mt) {
       uint32_t af[4];
-      ldmatrix4_transposed(af, values + r * C::ROW + swizzled<C>(r, 2 * mt + ((lane >> 3) & 1)) * 16);
+      ldmatrix4_transposed(af, values + offset_of<C>(r, 2 * mt + ((lane >> 3) & 1)));
 #pragma unroll
       for (int nt = 0; nt < C::NT; ++nt) mma16816<typename C::T>(out[nt][mt], af, p[nt]);
     }
@@ -343,8 +471,9 @@ __device__ __forceinline__ void value_step(uint32_t values, const uint32_t (&p)[
 template <typename C>
 __device__ __forceinline__ int channel_of(int mt, int second) {
   const int g = (threadIdx.x & 31) >> 2;
-  if (!C::INT8) return mt * 16 + g + second * 8;
+  if (!C::CODES) return mt * 16 + g + second * 8;
   if (C::D == 64) return g * 8 + 2 * mt + second;
+  if (C::BITS == 4) return g * (C::D / 8) + 2 * mt + second;
   return (g + 8 * (mt >> 3)) * 16 + 2 * (mt & 7) + second;
 }
 
@@ -436,13 +565,24 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
       const int key = walk.key_of(i);
       const bool hidden = walk.hidden >> stage & 1;
       float acc[NT][4];
-      score_step<C>(data, qf, acc);
+      const uint32_t key_scales = data + 2 * C::SIDE, value_scales = key_scales + C::SCALES;
+      if (C::BITS == 4 && (key < low || key + 16 > seq.length)) walk.clear_missing(data, key);
+      score_step<C>(data, key_scales, qf, acc);
       float ks0 = 1.f, ks1 = 1.f, vs0 = 1.f, vs1 = 1.f, lift0 = 0.f, lift1 = 0.f;
-      if (C::INT8) {
-        ks0 = read_float(data + 2 * C::SIDE + g * 4);
-        ks1 = read_float(data + 2 * C::SIDE + (g + 8) * 4);
-        vs0 = read_float(data + 2 * C::SIDE + 64 + g * 4);
-        vs1 = read_float(data + 2 * C::SIDE + 64 + (g + 8) * 4);
+      if (C::BITS == 4) {
+        const uint32_t e0 = read1(value_scales + g), e1 = read1(value_scales + g + 8);
+        ks0 = power_of(read1(key_scales + g));
+        ks1 = power_of(read1(key_scales + g + 8));
+        vs0 = power_of(e0) * kGroupUnit;
+        vs1 = power_of(e1) * kGroupUnit;
+        lift0 = lift_of(e0);
+        lift1 = lift_of(e1);
+      }
+      if (C::BITS == 8) {
+        ks0 = read_float(key_scales + g * 4);
+        ks1 = read_float(key_scales + (g + 8) * 4);
+        vs0 = read_float(value_scales + g * 4);
+        vs1 = read_float(value_scales + (g + 8) * 4);
         // a row of zeros must not let its own probability overflow, nor one that is not finite let the others vanish
         lift0 = vs0 < INFINITY ? lg2_approx(fmaxf(vs0, 0x1p-100f)) : 0.f;
         lift1 = vs1 < INFINITY ? lg2_approx(fmaxf(vs1, 0x1p-100f)) : 0.f;
@@ -450,7 +590,7 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[nt][e] *= C::INT8 ? (e < 2 ? ks0 : ks1) * factor[nt][e & 1] : factor[nt][e & 1];
+        for (int e = 0; e < 4; ++e) acc[nt][e] *= C::CODES ? (e < 2 ? ks0 : ks1) * factor[nt][e & 1] : factor[nt][e & 1];
       if (hidden || key < all_lo || key + 16 > all_hi) {
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -494,10 +634,10 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
         l[nt][0] += e[0] + e[2];
         l[nt][1] += e[1] + e[3];
         // Probabilities (times scales) leave 32 bits here: half a step, 2^-8 of the value in bf16, 2^-11 in fp16.
-        p[nt][0] = transposed8x8(Half2<typename C::M>::pack(C::INT8 ? e[0] * vs0 : e[0], C::INT8 ? e[1] * vs0 : e[1]));
-        p[nt][1] = transposed8x8(Half2<typename C::M>::pack(C::INT8 ? e[2] * vs1 : e[2], C::INT8 ? e[3] * vs1 : e[3]));
+        p[nt][0] = transposed8x8(Half2<typename C::M>::pack(C::CODES ? e[0] * vs0 : e[0], C::CODES ? e[1] * vs0 : e[1]));
+        p[nt][1] = transposed8x8(Half2<typename C::M>::pack(C::CODES ? e[2] * vs1 : e[2], C::CODES ? e[3] * vs1 : e[3]));
       }
-      value_step<C>(data + C::SIDE, p, o);
+      value_step<C>(data + C::SIDE, value_scales, p, o);
       stage = stage + 1 == W::STAGES ? 0 : stage + 1;
     }
     copies_wait<0>();
@@ -639,7 +779,12 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void weigh_rows_kernel(const Row
       const int key = walk.key_of(i);
       const bool hidden = walk.hidden >> stage & 1;
       float ks0 = 1.f, ks1 = 1.f;
-      if (C::INT8) {
+      if (C::BITS == 4) {
+        if (key < low || key + 16 > seq.length) walk.clear_missing(data, key);
+        ks0 = power_of(read1(data + C::SIDE + g));
+        ks1 = power_of(read1(data + C::SIDE + g + 8));
+      }
+      if (C::BITS == 8) {
         ks0 = read_float(data + C::SIDE + g * 4);
         ks1 = read_float(data + C::SIDE + (g + 8) * 4);
       }
@@ -647,14 +792,14 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void weigh_rows_kernel(const Row
       for (int block = 0; block < blocks; ++block) {
         if (blocks > 1) load_block(block);
         float acc[NT][4];
-        score_step<C>(data, qf, acc);
+        score_step<C>(data, data + C::SIDE, qf, acc);
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
             const int k = key + g + (e >> 1) * 8;
             const bool seen = !hidden && outside_gap<C>(a.line, k, lo[nt][e & 1]) && k < hi[nt][e & 1];
-            const float f = C::INT8 ? (e < 2 ? ks0 : ks1) * factor[nt][e & 1] : factor[nt][e & 1];
+            const float f = C::CODES ? (e < 2 ? ks0 : ks1) * factor[nt][e & 1] : factor[nt][e & 1];
             const float w = seen ? ex2_approx(fmaf(acc[nt][e], f, -lse2[nt][e & 1])) : 0.f;
             if (e < 2) sum0 += w; else sum1 += w;
           }
@@ -681,22 +826,25 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void weigh_rows_kernel(const Row
 constexpr int kSms = 148, kMaxWorkers = kSms * 3;
 
 template <typename F>
-int with_tile(int dtype_code, bool codes, int head_dim, int column_blocks, bool front, F&& f) {
-#define RISA_TILE(T, I8, D)                                                                                 \
-  return column_blocks == 1 ? (front ? f(Tile<T, I8, D, 1, true>{}) : f(Tile<T, I8, D, 1, false>{}))        \
-                            : (front ? f(Tile<T, I8, D, 2, true>{}) : f(Tile<T, I8, D, 2, false>{}))
-#define RISA_TILE_DIM(T, I8)                      \
-  do {                                            \
-    if (head_dim == 64) RISA_TILE(T, I8, 64);     \
-    if (head_dim == 128) RISA_TILE(T, I8, 128);   \
-    RISA_TILE(T, I8, 256);                        \
+int with_tile(int dtype_code, int bits, int head_dim, int column_blocks, bool front, F&& f) {
+#define RISA_TILE(T, BITS, D)                                                                                   \
+  return column_blocks == 1 ? (front ? f(Tile<T, BITS, D, 1, true>{}) : f(Tile<T, BITS, D, 1, false>{}))        \
+                            : (front ? f(Tile<T, BITS, D, 2, true>{}) : f(Tile<T, BITS, D, 2, false>{}))
+#define RISA_TILE_DIM(T, BITS)                      \
+  do {                                              \
+    if (head_dim == 64) RISA_TILE(T, BITS, 64);     \
+    if (head_dim == 128) RISA_TILE(T, BITS, 128);   \
+    RISA_TILE(T, BITS, 256);                        \
   } while (0)
-  if (dtype_code == 1) {
-    if (codes) RISA_TILE_DIM(__half, true);
-    RISA_TILE_DIM(__half, false);
-  }
-  if (codes) RISA_TILE_DIM(__nv_bfloat16, true);
-  RISA_TILE_DIM(__nv_bfloat16, false);
+#define RISA_TILE_BITS(T)                 \
+  do {                                    \
+    if (bits == 4) RISA_TILE_DIM(T, 4);   \
+    if (bits == 8) RISA_TILE_DIM(T, 8);   \
+    RISA_TILE_DIM(T, 16);                 \
+  } while (0)
+  if (dtype_code == 1) RISA_TILE_BITS(__half);
+  RISA_TILE_BITS(__nv_bfloat16);
+#undef RISA_TILE_BITS
 #undef RISA_TILE_DIM
 #undef RISA_TILE
 }
@@ -710,10 +858,11 @@ int check_queries(const risa_b200_cache* cache, const risa_b200_step* step, cons
   RISA_REQUIRE(q != nullptr, "%s: null tensor", what);
   RISA_REQUIRE(q_heads > 0 && q_heads % cache->kv_heads == 0, "%s: the query heads must be a multiple of the key heads", what);
   RISA_REQUIRE(dtype_code == 1 || dtype_code == 2, "%s: q must be float16 or bfloat16", what);
-  RISA_REQUIRE(cache->dtype_code == kInt8 || cache->dtype_code == dtype_code, "%s: q must have the cache's type", what);
+  RISA_REQUIRE(bits_of(*cache) < 16 || cache->dtype_code == dtype_code, "%s: q must have the cache's type", what);
   RISA_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && qs[0] % 8 == 0 && qs[1] % 8 == 0,
                "%s: query rows must start on 16-byte boundaries", what);
   RISA_REQUIRE(fabsf(scale * kLog2e) < INFINITY, "%s: the scale must be finite, also in units of log 2", what);
+  RISA_REQUIRE(bits_of(*cache) != 4 || fabsf(scale * kLog2e * kGroupUnit) < INFINITY, "%s: the scale is too large for 4-bit codes", what);
   RISA_REQUIRE(window >= 0 && (window == 0 || is_causal), "%s: a window needs the causal rule and at least one key", what);
   RISA_REQUIRE(sinks >= 0 && (sinks == 0 || window > 0), "%s: first keys stay visible in front of a window", what);
   RISA_REQUIRE(int64_t(step->tokens) * (q_heads / cache->kv_heads) < (int64_t(1) << 31) - 1024, "%s: too many query rows", what);
@@ -735,7 +884,7 @@ RowsArgs rows_args(const risa_b200_cache* cache, const risa_b200_step* step, con
   a.key_scales = cache->key_scales;
   a.value_scales = cache->value_scales;
   a.pages = cache->pages;
-  a.scale_log2 = scale * kLog2e;
+  a.scale_log2 = scale * kLog2e * (bits_of(*cache) == 4 ? kGroupUnit : 1.0f);
   a.min_steps = 16;  // one token over 8K keys: 16.8 us with 8 (256 workers), 15.5 with 16
   a.status = status;
   return a;
@@ -802,8 +951,8 @@ extern "C" int risa_b200_paged_attention_sinks(const risa_b200_cache* cache, con
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   const bool tensor_cores = takes_tensor_cores(*step, a.line.group);
   if (tensor_cores) a.line.max_rows = kTcFewestRows - 1;
-  const bool codes = cache->dtype_code == kInt8;
-  int bad = with_tile(dtype_code, codes, cache->head_dim, a.line.rows / 8, sinks > 0, [&](auto tile) {
+  const int bits = bits_of(*cache);
+  int bad = with_tile(dtype_code, bits, cache->head_dim, a.line.rows / 8, sinks > 0, [&](auto tile) {
     using C = decltype(tile);
     constexpr int bytes = kWarps * Walk<C, true>::STAGE * Walk<C, true>::STAGES;
     if (const int bad = allow_shared(paged_rows_kernel<C>, bytes, "paged attention")) return bad;
@@ -815,10 +964,10 @@ extern "C" int risa_b200_paged_attention_sinks(const risa_b200_cache* cache, con
                              a.parts + rows_scratch(*cache, *step, a.line.group) / sizeof(float), nullptr, 2, status}, cache->head_dim);
     t.line.min_rows = kTcFewestRows;
     t.line.max_rows = INT_MAX;
-    bad = paged_tc(t, dtype_code, codes, cache->head_dim, stream);
+    bad = paged_tc(t, dtype_code, bits, cache->head_dim, stream);
   }
   if (bad == RISA_B200_OK)
-    bad = with_tile(dtype_code, codes, cache->head_dim, a.line.rows / 8, false, [&](auto tile) {
+    bad = with_tile(dtype_code, bits, cache->head_dim, a.line.rows / 8, false, [&](auto tile) {
       using C = decltype(tile);
       const JoinArgs join{a.parts, a.notes, C::R, a.line.group, q_heads, out, a.on, a.oh, lse};
       return launched(launch_chained(join_parts_kernel<typename C::T, C::D, true>, dim3(kSms * C::CTAS - 1, C::R), dim3(128), 0, stream, join), "paged attention");
@@ -859,7 +1008,7 @@ extern "C" int risa_b200_key_weights_sinks(const risa_b200_cache* cache, const r
   a.row_lse = lse;
   a.previous = previous;
   a.weights = weights;
-  int bad = with_tile(dtype_code, cache->dtype_code == kInt8, cache->head_dim, column_blocks, sinks > 0, [&](auto tile) {
+  int bad = with_tile(dtype_code, bits_of(*cache), cache->head_dim, column_blocks, sinks > 0, [&](auto tile) {
     using C = decltype(tile);
     constexpr int bytes = kWarps * Walk<C, false>::STAGE * Walk<C, false>::STAGES;
     if (const int bad = allow_shared(weigh_rows_kernel<C>, bytes, "key weights")) return bad;
@@ -879,7 +1028,7 @@ extern "C" int risa_b200_key_weights_sinks(const risa_b200_cache* cache, const r
     t.parts = static_cast<float*>(scratch);
     t.min_steps = 2;
     t.status = status;
-    bad = weigh_tc(t, lse, previous, weights, dtype_code, cache->dtype_code == kInt8, cache->head_dim, stream);
+    bad = weigh_tc(t, lse, previous, weights, dtype_code, bits_of(*cache), cache->head_dim, stream);
   }
   return bad;
 }

@@ -49,11 +49,12 @@ constexpr uint32_t kHiddenRuns = 0xff, kFirst = 1u << 8, kLast = 1u << 9, kTwoGr
 // most 256, which 16-bit types hold with the same relative precision, and the output in tensor memory stays as it is.
 constexpr float kStale = 8.0f;
 
-template <typename T_, bool INT8_, int D_>
+template <typename T_, int BITS_, int D_>
 struct Shape {
   using T = T_;
-  using M = std::conditional_t<INT8_, __half, T_>;  // type of the matrix instructions' operands
-  static constexpr bool INT8 = INT8_;
+  static constexpr int BITS = BITS_;
+  static constexpr bool CODES = BITS < 16;
+  using M = std::conditional_t<CODES, __half, T_>;  // type of the matrix instructions' operands
   static constexpr int D = D_;
   static constexpr bool SHARED = D == 256;             // both groups have the same rows
   static constexpr int KEYS = SHARED ? 64 : 128;       // of a tile
@@ -113,8 +114,9 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
     KeyRuns ahead;
     ahead.look_up(row, a.line.step.page_shift, a.pages, C::KEYS / 16, piece.step(0) * C::KEYS, low, a.line.sinks, length);
     // over codes: the next batch is on its way while one is converted
-    CodeBatch<C::D> batch;
-    if (C::INT8) batch.load(keys, ahead, piece.head, 0, p);
+    using Batch = CodeBatch<C::D, C::CODES ? C::BITS : 8>;
+    Batch batch;
+    if (C::CODES) batch.load(keys, ahead, piece.head, 0, p);
 #pragma unroll 1
     for (int i = 0; i < piece.count; ++i) {
       const KeyRuns runs = ahead;
@@ -128,22 +130,31 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
           land(side);
           return;
         }
-        if constexpr (C::INT8) {
+        if constexpr (C::CODES) {
           // codes as they are; the softmax multiplies scores and probabilities by their keys' scales, in 32 bits
           if (side == 0) {
             const int key = runs.key0 + p, page = __shfl_sync(0xffffffffu, runs.id, p >> 4), slot = issued % kScaleDepth;
             const bool there = page >= 0 && runs.has(key);
-            const int64_t line = there ? keys.line(page, piece.head, key) : 0;
-            const float v = there ? __ldg(values.scales + line) : 0.f;
-            scales->key[slot][p] = there ? __ldg(keys.scales + line) : 0.f;
-            scales->value[slot][p] = v;
-            // a row of zeros must not let its own probability overflow, nor one that is not finite let the others vanish
-            scales->lift[slot][p] = v < INFINITY ? lg2_approx(fmaxf(v, 0x1p-100f)) : 0.f;
+            if (C::BITS == 4) {
+              const int in_page = key & ((1 << a.line.step.page_shift) - 1);
+              const uint32_t k = there ? __ldg(scales4<C::D>(keys.scales, page, a.line.kv_heads, piece.head, a.line.step.page_shift) + in_page) : 0;
+              const uint32_t v = there ? __ldg(scales4<C::D>(values.scales, page, a.line.kv_heads, piece.head, a.line.step.page_shift) + in_page) : 0;
+              scales->key[slot][p] = power_of(k);
+              scales->value[slot][p] = power_of(v) * kGroupUnit;
+              scales->lift[slot][p] = lift_of(v);
+            } else {
+              const int64_t line = there ? keys.line(page, piece.head, key) : 0;
+              const float v = there ? __ldg(values.scales + line) : 0.f;
+              scales->key[slot][p] = there ? __ldg(keys.scales + line) : 0.f;
+              scales->value[slot][p] = v;
+              // a row of zeros must not let its own probability overflow, nor one that is not finite let the others vanish
+              scales->lift[slot][p] = v < INFINITY ? lg2_approx(fmaxf(v, 0x1p-100f)) : 0.f;
+            }
           }
 #pragma unroll 1
-          for (int from = 0; from < C::KEYS; from += CodeBatch<C::D>::ROWS) {
-            CodeBatch<C::D> next = batch;
-            if (from + CodeBatch<C::D>::ROWS < C::KEYS) next.load(side ? values : keys, runs, piece.head, from + CodeBatch<C::D>::ROWS, p);
+          for (int from = 0; from < C::KEYS; from += Batch::ROWS) {
+            Batch next = batch;
+            if (from + Batch::ROWS < C::KEYS) next.load(side ? values : keys, runs, piece.head, from + Batch::ROWS, p);
             else if (side == 0) next.load(values, runs, piece.head, 0, p);
             else if (i + 1 < piece.count) next.load(keys, ahead, piece.head, 0, p);
             batch.template store<__half, C::KEYS>(to, 0, from, p);
@@ -280,7 +291,7 @@ __device__ __forceinline__ void load_query_rows(const TcArgs& a, const Piece& pi
       v = *reinterpret_cast<const uint4*>(static_cast<const typename C::T*>(a.q) + int64_t(piece.seq.first + token) * a.qn +
                                           int64_t(piece.head * a.line.group + h) * a.qh + c * 8);
     }
-    if constexpr (C::INT8 && std::is_same<typename C::T, __nv_bfloat16>::value) {
+    if constexpr (C::CODES && std::is_same<typename C::T, __nv_bfloat16>::value) {
       const float down = row_to_half<PIECES>(v);
       if (c == 0) row_scale[r] = down;
     }
@@ -309,7 +320,7 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
   auto mine = [&](const Piece& p) { return p.seq.count * a.line.group - p.block * C::ROWS > group_row; };
   auto fetch = [&](const Piece& p) {
     turn ^= 1;
-    load_query_rows<C>(a, p, g, q + (C::SHARED ? 0 : g * C::QUERIES), C::INT8 ? scales->row[turn][C::SHARED ? 0 : g] : nullptr);
+    load_query_rows<C>(a, p, g, q + (C::SHARED ? 0 : g * C::QUERIES), C::CODES ? scales->row[turn][C::SHARED ? 0 : g] : nullptr);
     mbar_arrive_warp(smem_u32(bars->q_full + g));
   };
   auto wait = [&](uint32_t bar, uint32_t parity, unsigned int site) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, gave_up, site)); };
@@ -352,7 +363,7 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
       tmem_load_wait();
       tmem_regs_ready<KEYS>(x);
       const int slot_of_tile = tile % kScaleDepth;
-      if constexpr (C::INT8) {
+      if constexpr (C::CODES) {
         if (std::is_same<T, __nv_bfloat16>::value && i == 0) scale = call_scale * scales->row[mine_turn][C::SHARED ? 0 : g][r];
         const ulonglong2* k = reinterpret_cast<const ulonglong2*>(scales->key[slot_of_tile] + half * KEYS);
 #pragma unroll
@@ -381,7 +392,7 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
       }
       const uint64_t scale2 = pack_f32x2(scale, scale);
       float best;
-      if constexpr (C::INT8) {
+      if constexpr (C::CODES) {
         // The maximum is that of the row's own probabilities times scales, hidden keys left out: what is rounded is at most 1
         // (2^8 where the running maximum lags), and neither the other keys of the tile nor other rows move it.  (Against the
         // largest scale of the tile, 1024 tokens over 8K codes, 32 heads: 271 us for 269 at 128 channels, 203 for 190 at 64.)
@@ -442,7 +453,7 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
           u = ex2_approx(u);
           w = ex2_approx(w);
           sum[c & 1] = add_f32x2(sum[c & 1], pack_f32x2(u, w));
-          if constexpr (C::INT8) {
+          if constexpr (C::CODES) {
             const float2 v = *reinterpret_cast<const float2*>(scales->value[slot_of_tile] + half * KEYS + at);
             u *= v.x;
             w *= v.y;
@@ -522,7 +533,7 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
   extern __shared__ char smem_raw[];
   __shared__ Barriers bars;
   __shared__ Exchange exchange;
-  __shared__ __align__(16) typename std::conditional<C::INT8, Scales, char>::type scales_memory;
+  __shared__ __align__(16) typename std::conditional<C::CODES, Scales, char>::type scales_memory;
   Scales* scales = reinterpret_cast<Scales*>(&scales_memory);
   __shared__ LineShared<kThreads> shared;
   __shared__ uint32_t tmem_base, gave_up_word;
@@ -638,7 +649,7 @@ bool pool_map(CUtensorMap* map, const char* pool, const TcArgs& a) {
 
 template <typename T, int D>
 int join(const TcArgs& a, cudaStream_t stream) {
-  constexpr int kRows = Shape<T, false, D>::ROWS;
+  constexpr int kRows = Shape<T, 16, D>::ROWS;
   const JoinArgs join{a.parts, a.notes, kRows, a.line.group, a.line.kv_heads * a.line.group, a.out, a.on, a.oh, a.lse};
   return launched(launch_chained(join_parts_kernel<T, D, false>, dim3(kTcWorkers - 1, kRows / 16), dim3(128), 0, stream, join), "paged attention");
 }
@@ -647,7 +658,7 @@ template <typename C>
 int launch(const TcArgs& a, cudaStream_t stream) {
   CUtensorMap key_map{}, value_map{};
   RISA_REQUIRE(int64_t(a.pages) * a.line.kv_heads < (int64_t(1) << 31), "paged attention: the pool has too many pages");
-  if (!C::INT8)
+  if (!C::CODES)
     if (encode_fn() == nullptr || !pool_map<C>(&key_map, a.keys, a) || !pool_map<C>(&value_map, a.values, a))
       return fail(RISA_B200_CUDA, "paged attention: no tensor map of the pool");
   if (cudaFuncSetAttribute(paged_tc_kernel<C>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM) != cudaSuccess)
@@ -664,12 +675,14 @@ int launch(const TcArgs& a, cudaStream_t stream) {
 }  // namespace
 
 namespace {
-int rows_of_unit(int head_dim) { return head_dim == 256 ? Shape<__half, false, 256>::ROWS : Shape<__half, false, 128>::ROWS; }
+int rows_of_unit(int head_dim) { return head_dim == 256 ? Shape<__half, 16, 256>::ROWS : Shape<__half, 16, 128>::ROWS; }
+template <typename T, int BITS>
+int launch_bits(const TcArgs& a, int head_dim, cudaStream_t stream) {
+  return head_dim == 64 ? launch<Shape<T, BITS, 64>>(a, stream) : head_dim == 128 ? launch<Shape<T, BITS, 128>>(a, stream) : launch<Shape<T, BITS, 256>>(a, stream);
+}
 template <typename T>
-int launch_for(const TcArgs& a, bool codes, int head_dim, cudaStream_t stream) {
-  if (head_dim == 64) return codes ? launch<Shape<T, true, 64>>(a, stream) : launch<Shape<T, false, 64>>(a, stream);
-  if (head_dim == 128) return codes ? launch<Shape<T, true, 128>>(a, stream) : launch<Shape<T, false, 128>>(a, stream);
-  return codes ? launch<Shape<T, true, 256>>(a, stream) : launch<Shape<T, false, 256>>(a, stream);
+int launch_for(const TcArgs& a, int bits, int head_dim, cudaStream_t stream) {
+  return bits == 4 ? launch_bits<T, 4>(a, head_dim, stream) : bits == 8 ? launch_bits<T, 8>(a, head_dim, stream) : launch_bits<T, 16>(a, head_dim, stream);
 }
 template <typename T>
 int join_for(const TcArgs& a, int head_dim, cudaStream_t stream) {
@@ -682,12 +695,12 @@ size_t paged_tc_scratch(int head_dim) {
 }
 TcArgs paged_tc_args(TcArgs a, int head_dim) {
   a.line.rows = Divisor(rows_of_unit(head_dim));
-  a.line.keys = Divisor(head_dim == 256 ? Shape<__half, false, 256>::KEYS : Shape<__half, false, 128>::KEYS);
+  a.line.keys = Divisor(head_dim == 256 ? Shape<__half, 16, 256>::KEYS : Shape<__half, 16, 128>::KEYS);
   a.notes = reinterpret_cast<JoinNote*>(a.parts + size_t(kTcWorkers) * 2 * slot_floats(a.line.rows, head_dim));
   return a;
 }
-int paged_tc(const TcArgs& a, int dtype_code, bool codes, int head_dim, cudaStream_t stream) {
-  return dtype_code == 1 ? launch_for<__half>(a, codes, head_dim, stream) : launch_for<__nv_bfloat16>(a, codes, head_dim, stream);
+int paged_tc(const TcArgs& a, int dtype_code, int bits, int head_dim, cudaStream_t stream) {
+  return dtype_code == 1 ? launch_for<__half>(a, bits, head_dim, stream) : launch_for<__nv_bfloat16>(a, bits, head_dim, stream);
 }
 int paged_tc_join(const TcArgs& a, int dtype_code, int head_dim, cudaStream_t stream) {
   return dtype_code == 1 ? join_for<__half>(a, head_dim, stream) : join_for<__nv_bfloat16>(a, head_dim, stream);

@@ -31,13 +31,13 @@ struct TcArgs {
 size_t paged_tc_scratch(int head_dim);
 // The kernel runs beside the launch in front of it, which has to be one of the same call that succeeded; the join comes behind both.
 TcArgs paged_tc_args(TcArgs args, int head_dim);
-int paged_tc(const TcArgs& args, int dtype_code, bool codes, int head_dim, cudaStream_t stream);
+int paged_tc(const TcArgs& args, int dtype_code, int bits, int head_dim, cudaStream_t stream);
 int paged_tc_join(const TcArgs& args, int dtype_code, int head_dim, cudaStream_t stream);
 int paged_tc_wait_status();
 
 // Key weights (weigh_tc.cu), likewise beside the launch in front; `out`, `lse` and `values` of the arguments are not used.
 size_t weigh_tc_scratch();
-int weigh_tc(const TcArgs& args, const float* row_lse, const float* previous, float* weights, int dtype_code, bool codes, int head_dim,
+int weigh_tc(const TcArgs& args, const float* row_lse, const float* previous, float* weights, int dtype_code, int bits, int head_dim,
              cudaStream_t stream);
 int weigh_tc_wait_status();
 

@@ -7,7 +7,10 @@
 namespace risa_b200 {
 namespace serving {
 
-constexpr int kInt8 = 4;  // dtype code of a cache of codes
+constexpr int kInt8 = 4, kInt4 = 5;  // dtype codes of caches of codes
+
+// Bits of a cached value.
+inline int bits_of(const risa_b200_cache& c) { return c.dtype_code == kInt8 ? 8 : c.dtype_code == kInt4 ? 4 : 16; }
 
 // Address on the current device of the word that records a page outside the pool (sequence + 1 of the
 // first one seen); nullptr with the error set where it cannot be had.  Defined in cache_ops.cu.
@@ -20,10 +23,11 @@ inline int check_cache(const risa_b200_cache* c, const char* what) {
                "%s: page_size must be 16, 32, 64 or 128", what);
   RISA_REQUIRE(c->head_dim == 64 || c->head_dim == 128 || c->head_dim == 256,
                "%s: head_dim must be 64, 128 or 256", what);
-  RISA_REQUIRE(c->dtype_code == 1 || c->dtype_code == 2 || c->dtype_code == kInt8,
-               "%s: the cache holds float16, bfloat16 or int8", what);
-  RISA_REQUIRE(c->dtype_code != kInt8 || (c->key_scales != nullptr && c->value_scales != nullptr),
-               "%s: an int8 cache needs scales", what);
+  RISA_REQUIRE(c->dtype_code == 1 || c->dtype_code == 2 || c->dtype_code == kInt8 || c->dtype_code == kInt4,
+               "%s: the cache holds float16, bfloat16 or codes of 8 or 4 bits", what);
+  RISA_REQUIRE(bits_of(*c) == 16 || (c->key_scales != nullptr && c->value_scales != nullptr), "%s: a cache of codes needs scales", what);
+  RISA_REQUIRE(c->dtype_code != kInt4 || (reinterpret_cast<uintptr_t>(c->key_scales) | reinterpret_cast<uintptr_t>(c->value_scales)) % 16 == 0,
+               "%s: scales of 4-bit codes must be 16-byte aligned", what);
   RISA_REQUIRE((reinterpret_cast<uintptr_t>(c->keys) | reinterpret_cast<uintptr_t>(c->values)) % 16 == 0,
                "%s: pages must be 16-byte aligned", what);
   return RISA_B200_OK;

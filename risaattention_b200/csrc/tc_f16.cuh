@@ -3,6 +3,7 @@
 #pragma once
 #include <type_traits>
 
+#include "four_bits.cuh"
 #include "serving.cuh"
 #include "tc_ptx.cuh"
 
@@ -157,9 +158,11 @@ __device__ __forceinline__ void copy_keys(const PoolView& pool, const KeyRuns& k
     copy16(to + (ROWS > 128 ? (r >> 7) * tile_bytes : 0) + tile_offset<(ROWS > 128 ? 128 : ROWS)>(r & 127, piece), pool.rows + line * (D * 2) + piece * 16, there);
   }
 }
-// Codes, 16 of them per load; a batch is what a thread has on its way at once, from row `from` of the tile on.
+// Codes, 16 bytes of them per load; a batch is what a thread has on its way at once, from row `from` of the tile on.
+template <int D, int BITS>
+struct CodeBatch;
 template <int D>
-struct CodeBatch {
+struct CodeBatch<D, 8> {
   static constexpr int PIECES = D / 16, EACH = 128 / PIECES, COUNT = 4, ROWS = COUNT * EACH;
   uint4 codes[COUNT];
   __device__ __forceinline__ void load(const PoolView& pool, const KeyRuns& k, int head, int from, int thread) {
@@ -179,6 +182,44 @@ struct CodeBatch {
     for (int n = 0; n < COUNT; ++n) {
       const int r = from + thread / PIECES + n * EACH;
       store_codes<M, TILE>(to + r / TILE * tile_bytes, r % TILE, piece, codes[n]);
+    }
+  }
+};
+// 4 bits: 32 codes and the scales of their two groups.
+template <int D>
+struct CodeBatch<D, 4> {
+  static constexpr int PIECES = D / 32, EACH = 128 / PIECES, COUNT = EACH == 64 ? 2 : 4, ROWS = COUNT * EACH;
+  uint4 codes[COUNT];
+  uint32_t groups[COUNT];
+  __device__ __forceinline__ void load(const PoolView& pool, const KeyRuns& k, int head, int from, int thread) {
+    const int piece = thread % PIECES;
+#pragma unroll
+    for (int n = 0; n < COUNT; ++n) {
+      const int r = from + thread / PIECES + n * EACH, key = k.key0 + r, page = __shfl_sync(0xffffffffu, k.id, r >> 4);
+      const bool there = page >= 0 && k.has(key);
+      codes[n] = make_uint4(0, 0, 0, 0);
+      groups[n] = 0;
+      if (there) {
+        codes[n] = *reinterpret_cast<const uint4*>(pool.rows + pool.line(page, head, key) * (D / 2) + piece * 16);
+        const uint8_t* of = groups4<D>(scales4<D>(pool.scales, page, pool.kv_heads, head, pool.page_shift), pool.page_shift, key & ((1 << pool.page_shift) - 1));
+        groups[n] = __ldg(reinterpret_cast<const uint16_t*>(of) + piece);
+      }
+    }
+  }
+  template <typename M, int TILE>
+  __device__ __forceinline__ void store(uint32_t to, int tile_bytes, int from, int thread) const {
+    const int piece = thread % PIECES;
+#pragma unroll
+    for (int n = 0; n < COUNT; ++n) {
+      const int r = from + thread / PIECES + n * EACH;
+      const uint32_t w[4] = {codes[n].x, codes[n].y, codes[n].z, codes[n].w};
+      const GroupScale<M> first(twice(groups[n] & 0xffu)), second(twice(groups[n] >> 8));
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        uint32_t x[4];
+        scaled_codes(w[i], i < 2 ? first : second, x);
+        store16(to + r / TILE * tile_bytes + tile_offset<TILE>(r % TILE, 4 * piece + i), make_uint4(x[0], x[1], x[2], x[3]));
+      }
     }
   }
 };

@@ -100,10 +100,11 @@ struct WeighArgs {
   unsigned int* status;
 };
 
-template <typename T_, bool INT8_, int D_>
+template <typename T_, int BITS_, int D_>
 struct Shape {
   using T = T_;
-  static constexpr bool INT8 = INT8_;
+  static constexpr int BITS = BITS_;
+  static constexpr bool CODES = BITS < 16;
   static constexpr int D = D_;
   static constexpr int ROWS = D == 256 ? 64 : 128;  // query rows of a tile
   static constexpr int GROUP = 128 * D * 2;         // 128 keys
@@ -149,19 +150,20 @@ __device__ __forceinline__ void fetch_keys(const WeighArgs& a, Pieces pieces, Ba
     }
     const uint32_t to = keys + kb.stage * C::KEYS;
     // codes as they are: a key's scale multiplies its scores in 32 bits
-    if constexpr (C::INT8) {
-      CodeBatch<C::D> batch, next;
+    if constexpr (C::CODES) {
+      using Batch = CodeBatch<C::D, C::BITS>;
+      Batch batch, next;
       batch.load(a.keys, runs, at.head, 0, p);
 #pragma unroll 1
-      for (int from = 0; from < kBlockKeys; from += CodeBatch<C::D>::ROWS) {
-        if (from + CodeBatch<C::D>::ROWS < kBlockKeys) next.load(a.keys, runs, at.head, from + CodeBatch<C::D>::ROWS, p);
+      for (int from = 0; from < kBlockKeys; from += Batch::ROWS) {
+        if (from + Batch::ROWS < kBlockKeys) next.load(a.keys, runs, at.head, from + Batch::ROWS, p);
         batch.template store<typename C::T, 128>(to, C::GROUP, from, p);
         batch = next;
       }
     } else {
       copy_keys<C::D, kBlockKeys>(a.keys, runs, at.head, to, C::GROUP, p);
     }
-    if (C::INT8) {
+    if (C::CODES) {
       fence_async_smem();
       mbar_arrive(smem_u32(bars->k_full + kb.stage));
     } else {
@@ -331,9 +333,14 @@ __device__ __forceinline__ void add_up(const WeighArgs& a, Pieces pieces, Barrie
     bool whole_group = (key0 >= low || key0 + 128 <= a.line.sinks) && key0 + 128 <= seq.length;
     if (!exists) mine.hi = 0;
     float factor = a.scale_log2;
-    if (C::INT8 && exists) {
+    if (C::CODES && exists) {
       const int id = __ldg(a.line.step.table + int64_t(piece.sequence) * a.line.step.width + (key >> a.line.step.page_shift));
-      if (id >= 0 && id < a.pages) factor *= __ldg(a.keys.scales + a.keys.line(id, piece.head, key));
+      if (id >= 0 && id < a.pages) {
+        if (C::BITS == 4)
+          factor *= power_of(__ldg(scales4<C::D>(a.keys.scales, id, a.keys.kv_heads, piece.head, a.keys.page_shift) + (key & ((1 << a.keys.page_shift) - 1))));
+        else
+          factor *= __ldg(a.keys.scales + a.keys.line(id, piece.head, key));
+      }
     }
     float sum[4] = {0.f, 0.f, 0.f, 0.f};
     for (int i = 0; i < piece.count; ++i, ++tile) {
@@ -500,23 +507,25 @@ int launch(WeighArgs a, cudaStream_t stream) {
   if (const int bad = launched(launch_chained(weigh_tc_kernel<C>, dim3(kTcWorkers), dim3(kThreads), C::SMEM, stream, a), "key weights")) return bad;
   return launched(launch_chained(join_weights_kernel, dim3(kTcWorkers - 1), dim3(kBlockKeys), 0, stream, a), "key weights");
 }
+template <typename T, int BITS>
+int launch_bits(const WeighArgs& a, int head_dim, cudaStream_t stream) {
+  return head_dim == 64 ? launch<Shape<T, BITS, 64>>(a, stream) : head_dim == 128 ? launch<Shape<T, BITS, 128>>(a, stream) : launch<Shape<T, BITS, 256>>(a, stream);
+}
 template <typename T>
-int launch_for(const WeighArgs& a, bool codes, int head_dim, cudaStream_t stream) {
-  if (head_dim == 64) return codes ? launch<Shape<T, true, 64>>(a, stream) : launch<Shape<T, false, 64>>(a, stream);
-  if (head_dim == 128) return codes ? launch<Shape<T, true, 128>>(a, stream) : launch<Shape<T, false, 128>>(a, stream);
-  return codes ? launch<Shape<T, true, 256>>(a, stream) : launch<Shape<T, false, 256>>(a, stream);
+int launch_for(const WeighArgs& a, int bits, int head_dim, cudaStream_t stream) {
+  return bits == 4 ? launch_bits<T, 4>(a, head_dim, stream) : bits == 8 ? launch_bits<T, 8>(a, head_dim, stream) : launch_bits<T, 16>(a, head_dim, stream);
 }
 
 }  // namespace
 
 size_t weigh_tc_scratch() { return size_t(kTcWorkers) * (2 * kBlockKeys * sizeof(float) + sizeof(JoinNote)); }
 
-int weigh_tc(const TcArgs& t, const float* row_lse, const float* previous, float* weights, int dtype_code, bool codes, int head_dim,
+int weigh_tc(const TcArgs& t, const float* row_lse, const float* previous, float* weights, int dtype_code, int bits, int head_dim,
              cudaStream_t stream) {
   const WeighArgs a{{t.line.step, t.line.kv_heads, t.line.group, t.line.min_rows, Divisor(), t.line.causal, t.line.window, t.line.sinks},
                     t.q, t.qn, t.qh, row_lse, {t.keys, t.key_scales, t.line.kv_heads, t.line.step.page_shift}, t.pages, t.scale_log2,
                     previous, weights, t.parts, reinterpret_cast<JoinNote*>(t.parts + size_t(kTcWorkers) * 2 * kBlockKeys), t.min_steps, t.status};
-  return dtype_code == 1 ? launch_for<__half>(a, codes, head_dim, stream) : launch_for<__nv_bfloat16>(a, codes, head_dim, stream);
+  return dtype_code == 1 ? launch_for<__half>(a, bits, head_dim, stream) : launch_for<__nv_bfloat16>(a, bits, head_dim, stream);
 }
 
 int weigh_tc_wait_status() {

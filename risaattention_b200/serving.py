@@ -176,7 +176,14 @@ def rotate_positions(x, positions, rotary, *, interleaved=False, transposed=Fals
 class KeyValueCache:
     """Pages of keys and values, [pages, kv_heads, page_size, head_dim] contiguous: float16 or bfloat16, or
     int8 codes with one FP32 scale per token and head, [pages, kv_heads, page_size].  Pages hold 16, 32, 64
-    or 128 tokens of 64, 128 or 256 channels.  Which sequence owns which page is the caller's page table."""
+    or 128 tokens of 64, 128 or 256 channels.  Which sequence owns which page is the caller's page table.
+
+    Or 4-bit codes -7..7, two in a byte: uint8 [pages, kv_heads, page_size, head_dim / 2] with scales uint8
+    [pages, kv_heads, page_size * (1 + head_dim / 16)].  A value is code * group scale * token scale.  Of each
+    page and head the scales are first those of the tokens, powers of two as the exponent field of a float32
+    (0: a scale of zero; 255: infinity, which makes the row NaN), then for each token those of its groups of
+    16 channels, float8_e4m3fn.  Channel 8 w + 2 i + j of a row is ``code + 8`` in bits 16 j + 4 i of its
+    32-bit word w."""
 
     keys: torch.Tensor
     values: torch.Tensor
@@ -196,13 +203,20 @@ class KeyValueCache:
         return self.keys.shape[2]
 
     @property
+    def head_dim(self) -> int:
+        return self.keys.shape[3] * (2 if self.keys.dtype == torch.uint8 else 1)
+
+    @property
     def quantized(self) -> bool:
-        return self.keys.dtype == torch.int8
+        return self.key_scales is not None
 
 
 def allocate_key_value_cache(pages, kv_heads, page_size, head_dim, *, dtype=torch.bfloat16, device="cuda") -> KeyValueCache:
-    """An empty cache; ``dtype`` torch.int8 allocates scales beside the codes."""
+    """An empty cache; ``dtype`` torch.int8 allocates scales beside the codes, torch.uint8 is a cache in 4 bits."""
     shape = (pages, kv_heads, page_size, head_dim)
+    if dtype == torch.uint8:
+        shapes = ((*shape[:3], head_dim // 2),) * 2 + ((*shape[:2], page_size * (1 + head_dim // 16)),) * 2
+        return KeyValueCache(*(torch.zeros(s, dtype=dtype, device=device) for s in shapes))
     keys, values = torch.zeros(shape, dtype=dtype, device=device), torch.zeros(shape, dtype=dtype, device=device)
     if dtype != torch.int8:
         return KeyValueCache(keys, values)
@@ -223,7 +237,9 @@ def append_to_cache(cache, k, v, page_table, lengths, *, query_offsets=None, q=N
     [axes, tokens]) or, without them, by those places;
     ``q`` [tokens, q_heads, head_dim] is rotated in the same launch and returned (None without it; rows
     behind the last sequence give 0).  An int8 cache stores absmax / 127 as a token's scale and the codes
-    rounded to nearest even.  Tokens that their sequence is too short for are not written; a page outside
+    rounded to nearest even.  One in 4 bits takes as a token's scale the smallest power of two (2^-126 at
+    least) of which its largest value is at most 7 * 448, as a group's the group's largest value over 7 of them,
+    rounded to e4m3, and codes rounded to nearest even: those of the exactly rotated keys.  Tokens that their sequence is too short for are not written; a page outside
     the pool is not written either, and ``device_status()`` of the native module reports it.  Two sequences of
     a step must not share the pages they write to."""
     _check_cache(cache)
@@ -233,6 +249,20 @@ def append_to_cache(cache, k, v, page_table, lengths, *, query_offsets=None, q=N
     return _native(device).cache_append(
         *cache.tensors, k, v, page_table, lengths, query_offsets, q,
         *((None, None, 1, 1.0) if rotary is None else rotary._arguments), bool(interleaved), positions, _stream(device))
+
+
+def read_from_cache(cache, page_table, lengths, *, query_offsets=None, tokens=None, dtype=None):
+    """Keys and values of a step's tokens as they lie in the cache, each [tokens, kv_heads, head_dim] (the step
+    may be whole sequences).  Codes are read as the values they stand for, in ``dtype`` float16 or bfloat16.
+    ``tokens``: rows of the result where ``query_offsets`` are given; those of no sequence, or that their sequence
+    is too short for, give 0."""
+    _check_cache(cache)
+    if tokens is None:
+        if query_offsets is not None:
+            raise ValueError("with query_offsets the number of tokens must be given")
+        tokens = page_table.shape[0]
+    device = cache.keys.device
+    return _native(device).cache_read(*cache.tensors, page_table, lengths, query_offsets, int(tokens), dtype, _stream(device))
 
 
 def paged_attention(q, cache, page_table, lengths, *, query_offsets=None, scale=None, is_causal=True,
@@ -255,7 +285,7 @@ def paged_attention(q, cache, page_table, lengths, *, query_offsets=None, scale=
     cache's 16-bit values or codes as they are; probabilities are rounded to the type of ``q`` for the product
     with V.  Over a cache of codes it is probability times the key's scale that is rounded, to float16, in units
     of the largest such product that the token sees: of two scales that differ by more than 2^24 the smaller one's
-    values may be lost in that token.  A value that is not finite may also reach tokens of the same call
+    values may be lost in that token.  (4-bit codes enter multiplied by their group's scale, exactly.)  A value that is not finite may also reach tokens of the same call
     that do not see its key: it is multiplied by their probability, 0."""
     _check_cache(cache)
     if scale is None:

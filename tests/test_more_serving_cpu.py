@@ -76,3 +76,43 @@ def test_sinks_refusals():
         refuses(ValueError, call, *args, *step, window=8, sinks=2 ** 31, match="sinks")
         refuses(ValueError, call, *args, *step, window=8, sinks=4, is_causal=False, match="causal")
         refuses(ValueError, call, *args, *step, window=8, sinks=4, match="CUDA device")
+
+
+# ---- a cache in 4 bits ---------------------------------------------------------------------------------------
+U8 = torch.uint8
+
+
+def test_four_bit_caches():
+    cache = risa.allocate_key_value_cache(3, 2, 32, 128, dtype=U8, device="cpu")
+    assert cache.quantized and cache.page_size == 32 and cache.head_dim == 128
+    assert cache.keys.shape == (3, 2, 32, 64) and cache.key_scales.shape == (3, 2, 32 * 9) and cache.value_scales.dtype == U8
+    make, rows, scales = risa.KeyValueCache, x(2, 1, 16, 32, dtype=U8), x(2, 1, 16 * 5, dtype=U8)
+    make(rows, rows, scales, scales)
+    for args, error in [((rows, rows), ValueError), ((rows, rows, scales[..., :64], scales), ValueError), ((rows, rows, scales, x(2, 1, 80, dtype=torch.int8)), TypeError),
+                        ((rows, rows, scales, x(2, 80, 1, dtype=U8).transpose(1, 2)), None), ((rows, rows, scales, x(2, 80, 2, dtype=U8).transpose(1, 2)[:, :1]), ValueError),
+                        ((x(2, 1, 16, 64, dtype=U8),) * 2 + (scales, scales), ValueError), ((x(2, 1, 16, 16, dtype=U8),) * 2 + (scales, scales), ValueError),
+                        ((rows, rows.to(torch.int8), scales, scales), TypeError), ((x(2, 1, 16, 64, dtype=torch.int8),) * 2 + (scales, scales), TypeError)]:
+        if error is None:
+            make(*args)
+            continue
+        refuses(error, make, *args)
+
+
+def test_four_bit_refusals():
+    cache, step = risa.allocate_key_value_cache(4, 2, 16, 64, dtype=U8, device="cpu"), (ints(3, 2), ints(3))
+    refuses(ValueError, risa.paged_attention, x(3, 4, 32), cache, *step, match="q must have shape")
+    refuses(TypeError, risa.paged_attention, x(3, 4, 64, dtype=torch.float32), cache, *step, match="float16 or bfloat16")
+    refuses(ValueError, risa.append_to_cache, cache, x(3, 2, 32), x(3, 2, 32), *step, match="k and v")
+    refuses(ValueError, risa.paged_attention, x(3, 4, 64), cache, *step, match="CUDA device")
+    refuses(ValueError, risa.append_to_cache, cache, x(3, 2, 64), x(3, 2, 64), *step, match="CUDA device")
+    read = risa.read_from_cache
+    refuses(ValueError, read, cache, *step, match="say which")
+    refuses(TypeError, read, cache, *step, dtype=torch.float32, match="float16 or bfloat16")
+    refuses(ValueError, read, cache, *step, query_offsets=ints(4), dtype=BF16, match="number of tokens")
+    refuses(ValueError, read, cache, *step, tokens=5, dtype=BF16, match="one token")
+    refuses(ValueError, read, cache, *step, query_offsets=ints(4), tokens=0, dtype=BF16, match="tokens")
+    refuses(ValueError, read, cache, *step, dtype=BF16, match="CUDA device")
+    refuses(TypeError, read, cache.keys, *step, dtype=BF16, match="KeyValueCache")
+    plain = risa.allocate_key_value_cache(4, 2, 16, 64, device="cpu")
+    refuses(TypeError, read, plain, *step, dtype=torch.float16, match="dtype of the cache")
+    refuses(ValueError, read, plain, *step, match="CUDA device")
