@@ -165,6 +165,40 @@ int risa_b200_cache_evict(const risa_b200_cache* cache, const risa_b200_step* st
                           int budget, int recent, int32_t* kept, int32_t* new_lengths,
                           float* new_weights, void* stream);
 
+/* ---- pages shared, handed out, given back and moved ----------------------------------------------
+ * references: int32 [pages], how many entries of page tables lead to each page; 0: the page is free.
+ * Entries behind a sequence's length are not read; one that leads outside the pool is not counted, and
+ * risa_b200_device_status() reports it. */
+
+/* Row c of table [children, table_width] and lengths[c] become those of sequence parents[c] of the
+ * step, -1 behind the length (a parent outside 0..batch-1: an empty sequence); references counts the
+ * new entries.  step->query_offsets and tokens are not used here and in compact. */
+int risa_b200_fork_sequences(const risa_b200_cache* cache, int32_t* references,
+                             const risa_b200_step* step, const int32_t* parents, int children,
+                             int32_t* table, int32_t* lengths, void* stream);
+
+/* Brings every sequence from lengths[s] to new_lengths[s] tokens (at most what its row of the table
+ * holds).  A longer one gets pages: the lowest that were free, in the order of the sequences; where its
+ * last page is not full and has more than one reference it first gets a page in place of that, with a
+ * copy of its tokens.  A shorter one gives back the pages behind its length (their entries become
+ * -1); they are handed out from the next call on.  granted[s]: the length that the pages found allow
+ * (a sequence whose shared page could not be replaced keeps its length). */
+size_t risa_b200_resize_scratch_size(const risa_b200_cache* cache, int batch);
+int risa_b200_resize_sequences(const risa_b200_cache* cache, int32_t* references,
+                               int32_t* page_table, int table_width, const int32_t* lengths,
+                               const int32_t* new_lengths, int batch, int32_t* granted,
+                               void* scratch, size_t scratch_bytes, void* stream);
+
+/* Copies the pages in use (references > 0), in their order, to the first pages of another pool whose
+ * pages are of the same kind; table: the step's page table for that pool (-1 behind the lengths),
+ * target_references its counts, used[0] the number of pages in use.  Pages that the target has no room for are
+ * not copied, and their entries become -1. */
+size_t risa_b200_compact_scratch_size(const risa_b200_cache* cache);
+int risa_b200_cache_compact(const risa_b200_cache* cache, const int32_t* references,
+                            const risa_b200_step* step, const risa_b200_cache* target,
+                            int32_t* table, int32_t* target_references, int32_t* used,
+                            void* scratch, size_t scratch_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

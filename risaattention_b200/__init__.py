@@ -8,9 +8,9 @@ from .attention import (PrequantizedInt8Attention, RetainedMassPattern,
                         prequantize_int8_attention, sparse_int8_attention)
 from .host_pipeline import int8_attention_from_host
 from .permutation import KVPermutation, prepare_kv_permutation
-from .serving import (Eviction, KeyValueCache, RotaryTable, allocate_key_value_cache, append_to_cache,
-                      cached_key_weights, evict_from_cache, paged_attention, read_from_cache,
-                      rotary_frequencies, rotary_table, rotate_positions)
+from .serving import (Compaction, Eviction, KeyValueCache, RotaryTable, allocate_key_value_cache, append_to_cache,
+                      cached_key_weights, compact_cache, evict_from_cache, fork_sequences, paged_attention,
+                      read_from_cache, resize_sequences, rotary_frequencies, rotary_table, rotate_positions)
 
 __all__ = [
     "KVPermutation", "prepare_kv_permutation", "PrequantizedInt8Attention", "RetainedMassPattern",
@@ -19,6 +19,7 @@ __all__ = [
     "int8_attention_from_host", "int8_attention_from_prequantized", "int8_attention_is_available", "measure_pattern_recall",
     "prequantize_int8_attention", "sparse_int8_attention", "Eviction", "KeyValueCache", "RotaryTable",
     "allocate_key_value_cache", "append_to_cache", "cached_key_weights", "evict_from_cache",
+    "Compaction", "compact_cache", "fork_sequences", "resize_sequences",
     "paged_attention", "read_from_cache", "rotary_frequencies", "rotary_table", "rotate_positions",
 ]
 __version__ = "0.1.0"

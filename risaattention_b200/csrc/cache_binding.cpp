@@ -463,6 +463,88 @@ py::tuple cache_evict(const at::Tensor& cache_keys, const at::Tensor& cache_valu
   return py::make_tuple(kept, new_lengths, new_weights);
 }
 
+// ---- pages ----------------------------------------------------------------------------------------------------
+// Page table and lengths of sequences, without a step's tokens.
+Step sequences_of(const Cache& cache, const at::Tensor& table, const at::Tensor& lengths) {
+  return Step(cache, table, lengths, std::nullopt, table.dim() == 2 ? table.size(0) : 0);
+}
+void require_counts(const Cache& cache, const at::Tensor& references) {
+  require(references.dim() == 1 && references.size(0) == cache.c.pages, "references must have shape [pages of the cache]");
+  require_indices(references, "references");
+  require(references.device() == cache.keys.device(), "references must be on the device of the cache");
+}
+
+py::tuple fork_sequences(const at::Tensor& cache_keys, const at::Tensor& cache_values, const MaybeTensor& key_scales, const MaybeTensor& value_scales,
+                         const at::Tensor& references, const at::Tensor& table, const at::Tensor& lengths, const at::Tensor& parents,
+                         uintptr_t stream_ptr) {
+  const Cache cache(cache_keys, cache_values, key_scales, value_scales);
+  require_counts(cache, references);
+  const Step step = sequences_of(cache, table, lengths);
+  require(parents.dim() == 1 && parents.size(0) > 0 && parents.size(0) < (int64_t(1) << 31), "parents must have shape [children]");
+  require_indices(parents, "parents");
+  require(table.size(1) <= 65535 * 256, "page_table is too wide");
+  require(parents.device() == cache_keys.device(), "parents must be on the device of the cache");
+  require_cuda(cache_keys);
+  const c10::DeviceGuard on_device(cache_keys.device());
+  const at::Tensor new_table = at::empty({parents.size(0), table.size(1)}, table.options()), new_lengths = at::empty({parents.size(0)}, table.options());
+  check(risa_b200_fork_sequences(&cache.c, references.data_ptr<int32_t>(), &step.s, parents.data_ptr<int32_t>(), int(parents.size(0)),
+                                 new_table.data_ptr<int32_t>(), new_lengths.data_ptr<int32_t>(), stream_of(stream_ptr)));
+  return py::make_tuple(new_table, new_lengths);
+}
+
+at::Tensor resize_sequences(const at::Tensor& cache_keys, const at::Tensor& cache_values, const MaybeTensor& key_scales,
+                            const MaybeTensor& value_scales, const at::Tensor& references, const at::Tensor& table, const at::Tensor& lengths,
+                            const at::Tensor& new_lengths, uintptr_t stream_ptr) {
+  const Cache cache(cache_keys, cache_values, key_scales, value_scales);
+  require_counts(cache, references);
+  const Step step = sequences_of(cache, table, lengths);
+  require(new_lengths.dim() == 1 && new_lengths.size(0) == table.size(0), "new_lengths must have shape [batch]");
+  require_indices(new_lengths, "new_lengths");
+  require(new_lengths.device() == cache_keys.device(), "new_lengths must be on the device of the cache");
+  require_cuda(cache_keys);
+  const c10::DeviceGuard on_device(cache_keys.device());
+  const at::Tensor granted = at::empty({table.size(0)}, table.options());
+  const size_t bytes = risa_b200_resize_scratch_size(&cache.c, step.s.batch);
+  const at::Tensor scratch = at::empty({int64_t(bytes)}, table.options().dtype(at::kByte));
+  check(risa_b200_resize_sequences(&cache.c, references.data_ptr<int32_t>(), table.data_ptr<int32_t>(), step.s.table_width, step.s.lengths,
+                                   new_lengths.data_ptr<int32_t>(), step.s.batch, granted.data_ptr<int32_t>(), scratch.data_ptr(), bytes,
+                                   stream_of(stream_ptr)));
+  return granted;
+}
+
+// Whether two tensors share memory (both are contiguous).
+bool share_memory(const at::Tensor& a, const at::Tensor& b) {
+  const char *p = static_cast<const char*>(a.data_ptr()), *q = static_cast<const char*>(b.data_ptr());
+  return p < q + b.nbytes() && q < p + a.nbytes();
+}
+
+py::tuple cache_compact(const at::Tensor& cache_keys, const at::Tensor& cache_values, const MaybeTensor& key_scales, const MaybeTensor& value_scales,
+                        const at::Tensor& references, const at::Tensor& table, const at::Tensor& lengths, const at::Tensor& target_keys,
+                        const at::Tensor& target_values, const MaybeTensor& target_key_scales, const MaybeTensor& target_value_scales,
+                        uintptr_t stream_ptr) {
+  const Cache cache(cache_keys, cache_values, key_scales, value_scales), target(target_keys, target_values, target_key_scales, target_value_scales);
+  require_counts(cache, references);
+  const Step step = sequences_of(cache, table, lengths);
+  require_type(target.c.dtype_code == cache.c.dtype_code, "target must have the dtype of the cache");
+  require(target.c.kv_heads == cache.c.kv_heads && target.c.page_size == cache.c.page_size && target.c.head_dim == cache.c.head_dim,
+          "target must have pages of the same kind as the cache");
+  require(target_keys.device() == cache_keys.device(), "target must be on the device of the cache");
+  for (const at::Tensor* from : {&cache_keys, &cache_values})
+    for (const at::Tensor* to : {&target_keys, &target_values}) require(!share_memory(*from, *to), "target must be another pool: it shares memory with the cache");
+  if (key_scales.has_value())
+    for (const at::Tensor* from : {&*key_scales, &*value_scales})
+      for (const at::Tensor* to : {&*target_key_scales, &*target_value_scales})
+        require(!share_memory(*from, *to), "target must be another pool: its scales share memory with the cache's");
+  require_cuda(cache_keys);
+  const c10::DeviceGuard on_device(cache_keys.device());
+  const at::Tensor new_table = at::empty_like(table), counts = at::empty({target.c.pages}, table.options()), used = at::empty({1}, table.options());
+  const size_t bytes = risa_b200_compact_scratch_size(&cache.c);
+  const at::Tensor scratch = at::empty({int64_t(bytes)}, table.options().dtype(at::kByte));
+  check(risa_b200_cache_compact(&cache.c, references.data_ptr<int32_t>(), &step.s, &target.c, new_table.data_ptr<int32_t>(),
+                                counts.data_ptr<int32_t>(), used.data_ptr<int32_t>(), scratch.data_ptr(), bytes, stream_of(stream_ptr)));
+  return py::make_tuple(new_table, counts, used);
+}
+
 }  // namespace
 
 void bind_cache(py::module_& m) {
@@ -473,5 +555,8 @@ void bind_cache(py::module_& m) {
   m.def("paged_attention", &paged_attention);
   m.def("key_weights", &key_weights);
   m.def("cache_evict", &cache_evict);
+  m.def("fork_sequences", &fork_sequences);
+  m.def("resize_sequences", &resize_sequences);
+  m.def("cache_compact", &cache_compact);
   m.def("check_cache", [](const at::Tensor& k, const at::Tensor& v, const MaybeTensor& ks, const MaybeTensor& vs) { Cache(k, v, ks, vs); });
 }

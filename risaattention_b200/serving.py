@@ -336,3 +336,49 @@ def evict_from_cache(cache, page_table, lengths, weights, target_table, *, budge
     device = cache.keys.device
     return Eviction(*_native(device).cache_evict(*cache.tensors, page_table, lengths, weights, target_table,
                                                  int(budget), int(recent), _stream(device)))
+
+
+# ---- pages --------------------------------------------------------------------------------------------------
+# ``references`` int32 [pages] counts for each page how many entries of page tables lead to it; a page with
+# none is free.  (zeros for a new cache; every table whose pages are counted goes through these calls.)
+def fork_sequences(cache, references, page_table, lengths, parents):
+    """Sequences that begin as copies of others and share their pages (several answers to a prompt, beams):
+    ``parents`` int32 [children] names a row of ``page_table`` for each (or none, -1: an empty sequence).
+    Returns their page table [children, pages of a sequence], -1 behind their lengths, and their lengths;
+    ``references`` counts the new entries.  Nothing is copied until one of them grows (``resize_sequences``)."""
+    _check_cache(cache)
+    device = cache.keys.device
+    return _native(device).fork_sequences(*cache.tensors, references, page_table, lengths, parents, _stream(device))
+
+
+def resize_sequences(cache, references, page_table, lengths, new_lengths):
+    """Brings sequences to ``new_lengths`` int32 [batch] (at most what a row of ``page_table`` holds) and
+    returns the lengths that were granted; ``page_table`` and ``references`` are changed in place.
+
+    Before tokens are appended: a longer sequence gets the lowest free pages, in the order of the sequences;
+    where its last page is not full and shared, a page of its own in place of that, with a copy of its
+    tokens.  If pages run out it is granted the length that its pages hold (the old one, where a shared page
+    could not be replaced).  A shorter one, or length 0, gives its pages back; they may be handed out from
+    the next call on, by when nobody else may lead to them uncounted."""
+    _check_cache(cache)
+    device = cache.keys.device
+    return _native(device).resize_sequences(*cache.tensors, references, page_table, lengths, new_lengths, _stream(device))
+
+
+class Compaction(NamedTuple):
+    """``page_table`` for the target's pages, -1 behind the lengths; ``references`` int32 [pages of the target];
+    ``used`` int32 [1]: how many pages were in use."""
+
+    page_table: torch.Tensor
+    references: torch.Tensor
+    used: torch.Tensor
+
+
+def compact_cache(cache, references, page_table, lengths, target) -> Compaction:
+    """Copies the pages in use, shared ones once and all in their order, to the front of ``target``, another
+    cache with pages of the same kind (a smaller one, say, when most requests have left).  Where the target
+    has fewer pages than ``used`` tells, the last ones are not copied and entries that led to them are -1."""
+    _check_cache(cache)
+    _check_cache(target)
+    device = cache.keys.device
+    return Compaction(*_native(device).cache_compact(*cache.tensors, references, page_table, lengths, *target.tensors, _stream(device)))

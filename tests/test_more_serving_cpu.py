@@ -116,3 +116,33 @@ def test_four_bit_refusals():
     plain = risa.allocate_key_value_cache(4, 2, 16, 64, device="cpu")
     refuses(TypeError, read, plain, *step, dtype=torch.float16, match="dtype of the cache")
     refuses(ValueError, read, plain, *step, match="CUDA device")
+
+
+# ---- pages -----------------------------------------------------------------------------------------------------
+def test_page_refusals():
+    cache, table, lengths, references = risa.allocate_key_value_cache(4, 2, 16, 64, device="cpu"), ints(3, 2), ints(3), ints(4)
+    other = risa.allocate_key_value_cache(2, 2, 16, 64, device="cpu")
+    calls = [(risa.fork_sequences, (ints(5),)), (risa.resize_sequences, (ints(3),)), (risa.compact_cache, (other,))]
+    for call, rest in calls:
+        refuses(TypeError, call, cache.keys, references, table, lengths, *rest, match="KeyValueCache")
+        refuses(ValueError, call, cache, ints(5), table, lengths, *rest, match="references")
+        refuses(TypeError, call, cache, references.long(), table, lengths, *rest, match="references")
+        refuses(ValueError, call, cache, ints(8)[::2], table, lengths, *rest, match="references")
+        refuses(ValueError, call, cache, references, ints(3), lengths, *rest, match="page_table")
+        refuses(ValueError, call, cache, references, table, ints(2), *rest, match="lengths")
+        refuses(TypeError, call, cache, references, table.long(), lengths, *rest, match="int32")
+        refuses(ValueError, call, cache, references, table, lengths, *rest, match="CUDA device")
+    step = (cache, references, table, lengths)
+    refuses(ValueError, risa.fork_sequences, *step, ints(0), match="parents")
+    refuses(ValueError, risa.fork_sequences, *step, ints(2, 1), match="parents")
+    refuses(TypeError, risa.fork_sequences, *step, ints(2).long(), match="int32")
+    refuses(ValueError, risa.resize_sequences, *step, ints(4), match="new_lengths")
+    refuses(TypeError, risa.resize_sequences, *step, ints(3).long(), match="int32")
+    refuses(TypeError, risa.compact_cache, *step, other.keys, match="KeyValueCache")
+    for make, error in ((dict(dtype=torch.float16), TypeError), (dict(dtype=torch.int8), TypeError)):
+        refuses(error, risa.compact_cache, *step, risa.allocate_key_value_cache(4, 2, 16, 64, device="cpu", **make), match="dtype")
+    for shape in ((4, 1, 16, 64), (4, 2, 32, 64), (4, 2, 16, 128)):
+        refuses(ValueError, risa.compact_cache, *step, risa.allocate_key_value_cache(*shape, device="cpu"), match="same kind")
+    refuses(ValueError, risa.compact_cache, *step, cache, match="another pool")
+    refuses(ValueError, risa.compact_cache, *step, risa.KeyValueCache(cache.keys[1:], other.values.repeat(2, 1, 1, 1)[1:]), match="another pool")
+    refuses(ValueError, risa.compact_cache, *step, risa.KeyValueCache(other.keys, cache.keys[:2]), match="another pool")
