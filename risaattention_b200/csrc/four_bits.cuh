@@ -29,9 +29,10 @@ __device__ __forceinline__ const uint8_t* groups4(const uint8_t* scales, int pag
   return scales + (1 << page_shift) + slot * (D / 16);
 }
 __device__ __forceinline__ float power_of(uint32_t exponent) { return __uint_as_float(exponent << 23); }
-// Its logarithm in units of group scales as they are read; a scale of zero must not let its key's own probability overflow, nor
-// one that is not finite let the others vanish.
-__device__ __forceinline__ float lift_of(uint32_t exponent) { return exponent == 255u ? 0.f : float(max(int(exponent) - 119, -100)); }
+// Its logarithm in units of group scales as they are read, for the running maximum of probabilities times scales.  A scale of zero
+// must not let its key's own probability overflow, nor one that is not finite let the others vanish, nor the largest ones (up to
+// 2^125) leave denominators no room above 2^-126: probabilities times scales then grow to 2^15, which fp16 holds.
+__device__ __forceinline__ float lift_of(uint32_t exponent) { return exponent == 255u ? 0.f : float(min(max(int(exponent) - 119, -100), 110)); }
 
 // Group scales as a pair of 16-bit numbers, and what multiplies the bias of codes + 8 + 2^n.
 template <typename M> struct GroupScale;
@@ -47,11 +48,13 @@ template <> struct GroupScale<__half> {
 };
 template <> struct GroupScale<__nv_bfloat16> {
   __nv_bfloat162 s, c0;
-  __device__ __forceinline__ explicit GroupScale(uint32_t pair) {
-    const uint32_t bits = pair << 4;  // 2^-120 of the scale, then 2^-8
-    s = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&bits), __float2bfloat162_rn(0x1p112f));
+  // times 2^(exponent - 127) beside that 2^-8: the token's scale, for whom that range of exponents is no matter
+  __device__ __forceinline__ GroupScale(uint32_t pair, float power) {
+    const uint32_t bits = pair << 4;  // 2^-120 of the scale
+    s = __hmul2(__hmul2(*reinterpret_cast<const __nv_bfloat162*>(&bits), __float2bfloat162_rn(0x1p112f)), __float2bfloat162_rn(power));
     c0 = __hmul2(s, __float2bfloat162_rn(-136.f));  // exact: 17 times four bits
   }
+  __device__ __forceinline__ explicit GroupScale(uint32_t pair) : GroupScale(pair, 1.0f) {}
 };
 __device__ __forceinline__ uint32_t twice(uint32_t byte) { return byte * 0x00010001u; }
 

@@ -21,7 +21,8 @@
 //
 // Warps 0-15: softmax, query loads and epilogue, four for each half of the columns of each row group.  16-19: fetch K
 // and V tiles from the pages (cp.async, or codes converted on the way) into the 128-byte-swizzled layout of the matrix
-// instructions.  20: issues them (and owns tensor memory).  21-23 idle, so that registers can be dealt per warpgroup.
+// instructions.  20: issues them (and owns tensor memory).  21: notes for the join.  22: over a cache in 4 bits, brings its codes.
+// 23 idle, so that registers can be dealt per warpgroup.
 #include "serving_plan.cuh"
 #include "paged_tc.cuh"
 #include "tc_f16.cuh"
@@ -54,7 +55,10 @@ struct Shape {
   using T = T_;
   static constexpr int BITS = BITS_;
   static constexpr bool CODES = BITS < 16;
-  using M = std::conditional_t<CODES, __half, T_>;  // type of the matrix instructions' operands
+  // 4-bit codes that meet bf16 queries become bf16 with all their scales, exactly; other codes become fp16 and the softmax
+  // multiplies scores and probabilities by their tokens' scales.
+  static constexpr bool SCALED = BITS == 8 || (BITS == 4 && std::is_same<T, __half>::value);
+  using M = std::conditional_t<SCALED, __half, T_>;  // type of the matrix instructions' operands
   static constexpr int D = D_;
   static constexpr bool SHARED = D == 256;             // both groups have the same rows
   static constexpr int KEYS = SHARED ? 64 : 128;       // of a tile
@@ -64,11 +68,13 @@ struct Shape {
   static constexpr int BLOCK = KEYS * 128;             // 64 channels of it
   static constexpr int STAGES = D == 64 ? 4 : 2;
   static constexpr int QUERIES = 128 * D * 2, Q = (SHARED ? 1 : kGroups) * QUERIES;
-  static constexpr int SMEM = Q + 2 * STAGES * SIDE + 1024;  // + alignment
+  static constexpr int RAW = BITS == 4 ? RawTile<D, KEYS>::BYTES : 0;  // a tile's keys (or values) as they come from the pages
+  static constexpr int SMEM = Q + 2 * STAGES * SIDE + 2 * RAW + 1024;  // + alignment
 };
 
 struct Barriers {
   uint64_t k_full[4], k_empty[4], v_full[4], v_empty[4];
+  uint64_t raw_full[2], raw_empty[2];  // of 4-bit keys, of values
   uint64_t q_full[kGroups], s_full[kGroups], p_full[kGroups], o_full[kGroups], o_free[kGroups], q_empty, drained;
 };
 // What the two threads of a row tell each other: maxima (of tiles in turn) and sums.
@@ -76,14 +82,105 @@ struct Exchange {
   float maximum[2][kGroups][2][128];
   float sum[kGroups][2][128];
 };
-// Over a cache of codes: scales of the tiles in flight (a slot is written again kScaleDepth tiles later, by when the softmax
-// that read it has handed over its probabilities), those of values also in units of log 2, and what the queries' rows were
-// divided by, of this unit and the one before.
-constexpr int kScaleDepth = 8;
+// Over a cache of codes: scales of the tiles in flight, those of values also in units of log 2, and what the queries' rows were
+// divided by, of this unit and the one before.  A tile's slot is written once K's stage is free, that is after the scores STAGES
+// tiles back, which were issued behind the product with the probabilities before them: STAGES + 1 tiles need slots.
+template <int STAGES>
 struct Scales {
-  float key[kScaleDepth][128], value[kScaleDepth][128], lift[kScaleDepth][128];
+  static constexpr int DEPTH = 2 * STAGES;
+  static_assert(DEPTH > STAGES, "a slot outlives its readers");
+  float key[DEPTH][128], value[DEPTH][128], lift[DEPTH][128];
   float row[2][kGroups][128];
 };
+
+// ---- 4-bit codes ------------------------------------------------------------------------------------------------
+// A warp brings each tile's keys, then its values, as they lie in the pages, while the fetching warpgroup turns those in front of
+// them into the tiles of the matrix instructions: one slot for keys and one for values, so that half a tile's time is left for a
+// copy to land.  (Loads into registers one batch ahead: 1024 tokens of a prompt with a window of 8192, 32 heads of 128,
+// 361 us.)
+template <typename C>
+__device__ __forceinline__ void fetch_raw(const TcArgs& a, Pieces pieces, Barriers* bars, uint32_t raw, uint32_t gave_up) {
+  const PoolView keys{a.keys, a.key_scales, a.line.kv_heads, a.line.step.page_shift}, values{a.values, a.value_scales, a.line.kv_heads, a.line.step.page_shift};
+  uint32_t phase = 0, filled = 0;  // of both slots; how many copies were started
+  Piece piece;
+  bool going = true;
+  while (going && pieces.next(a.line, piece)) {
+    const int32_t* row = a.line.step.table + int64_t(piece.sequence) * a.line.step.width;
+    const int length = piece.seq.length;
+    const int low = a.line.window > 0 ? visible(piece.seq.length - piece.seq.count, length, true, a.line.window).lo : 0;
+    KeyRuns ahead;
+    ahead.look_up(row, a.line.step.page_shift, a.pages, C::KEYS / 16, piece.step(0) * C::KEYS, low, a.line.sinks, length);
+    for (int i = 0; going && i < piece.count; ++i) {
+      const KeyRuns runs = ahead;
+      if (i + 1 < piece.count) ahead.look_up(row, a.line.step.page_shift, a.pages, C::KEYS / 16, piece.step(i + 1) * C::KEYS, low, a.line.sinks, length);
+      for (int side = 0; going && side < 2; ++side) {
+        going = __all_sync(0xffffffffu, mbar_wait(smem_u32(bars->raw_empty + side), phase ^ 1, gave_up, 1003 + side));
+        if (!going) break;
+        RawTile<C::D, C::KEYS>::fetch(side ? values : keys, runs, piece.head, raw + side * C::RAW, smem_u32(bars->raw_full + side));
+        ++filled;
+      }
+      phase ^= 1;
+    }
+  }
+  // what was started lands before the CTA ends, also when a wait ran out
+  for (int side = 0; side < 2; ++side) {
+    const uint32_t rounds = (filled + 1 - side) / 2;
+    if (rounds > 0) mbar_drain(smem_u32(bars->raw_full + side), (rounds - 1) & 1);
+  }
+}
+template <typename C>
+__device__ __forceinline__ void convert_tiles(const TcArgs& a, Pieces pieces, Barriers* bars, volatile uint32_t* notes, volatile int* tile_keys, Scales<C::STAGES>* scales,
+                                              uint32_t k_ring, uint32_t v_ring, uint32_t raw, uint32_t gave_up) {
+  using Raw = RawTile<C::D, C::KEYS>;
+  const int p = threadIdx.x - kProducer * 32;
+  uint32_t issued = 0, phase = 0;
+  RingPos<C::STAGES> stage;  // of both rings
+  Piece piece;
+  auto wait = [&](uint64_t* bar, uint32_t parity, unsigned int site) { return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, gave_up, site)); };
+  while (pieces.next(a.line, piece)) {
+    const int32_t* row = a.line.step.table + int64_t(piece.sequence) * a.line.step.width;
+    const int length = piece.seq.length;
+    const int low = a.line.window > 0 ? visible(piece.seq.length - piece.seq.count, length, true, a.line.window).lo : 0;
+    const uint32_t two = C::SHARED || piece.seq.count * a.line.group - piece.block * C::ROWS > 128 ? kTwoGroups : 0u;
+    KeyRuns ahead;
+    ahead.look_up(row, a.line.step.page_shift, a.pages, C::KEYS / 16, piece.step(0) * C::KEYS, low, a.line.sinks, length);
+#pragma unroll 1
+    for (int i = 0; i < piece.count; ++i) {
+      const KeyRuns runs = ahead;
+      if (i + 1 < piece.count) ahead.look_up(row, a.line.step.page_shift, a.pages, C::KEYS / 16, piece.step(i + 1) * C::KEYS, low, a.line.sinks, length);
+#pragma unroll 1
+      for (int side = 0; side < 2; ++side) {  // K, then V
+        uint64_t* full = side ? bars->v_full : bars->k_full;
+        uint64_t* empty = side ? bars->v_empty : bars->k_empty;
+        if (!wait(bars->raw_full + side, phase, 1005 + side) || !wait(empty + stage.stage, stage.phase ^ 1, 1001 + side)) return;
+        if (C::SCALED && side == 0) {
+          if (!wait(bars->raw_full + 1, phase, 1007)) return;  // the softmax goes by the values' scales too
+          const int slot = issued % Scales<C::STAGES>::DEPTH;
+          if (p < C::KEYS) {
+            const bool there = __shfl_sync(0xffffffffu, runs.id, p >> 4) >= 0 && runs.has(runs.key0 + p);
+            const uint32_t k = there ? Raw::exponent(raw, p) : 0, v = there ? Raw::exponent(raw + C::RAW, p) : 0;
+            scales->key[slot][p] = power_of(k);
+            scales->value[slot][p] = power_of(v) * kGroupUnit;
+            scales->lift[slot][p] = lift_of(v);
+          }
+        }
+        Raw::template convert<typename C::M>(raw + side * C::RAW, runs, (side ? v_ring : k_ring) + stage.stage * C::SIDE, p);
+        fence_async_smem();
+        mbar_arrive(smem_u32(full + stage.stage));
+        mbar_arrive_warp(smem_u32(bars->raw_empty + side));
+        if (side == 0 && p == 0) {
+          tile_keys[issued % kNotes] = runs.key0;
+          notes[issued % kNotes] = runs.bad | (i == 0 ? kFirst : 0u) | (i + 1 == piece.count ? kLast : 0u) | two;
+          if (runs.bad) atomicCAS(a.status, 0u, unsigned(piece.sequence) + 1u);
+          mbar_arrive(smem_u32(bars->k_full + stage.stage));  // the note is there
+        }
+      }
+      stage.next();
+      phase ^= 1;
+      ++issued;
+    }
+  }
+}
 
 // ---- the fetching warpgroup -----------------------------------------------------------------------------------
 // Tiles of 16-bit rows that all exist come by TMA, a box of 64 channels x a page at a time: 128 threads that copy 16
@@ -91,7 +188,7 @@ struct Scales {
 // front of a window, pages outside the pool) are copied piece by piece with zeros in place of what is not there.
 template <typename C>
 __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* key_map, const CUtensorMap* value_map, Pieces pieces, Barriers* bars,
-                                            volatile uint32_t* notes, volatile int* tile_keys, Scales* scales, uint32_t k_ring, uint32_t v_ring, uint32_t gave_up) {
+                                            volatile uint32_t* notes, volatile int* tile_keys, Scales<C::STAGES>* scales, uint32_t k_ring, uint32_t v_ring, uint32_t gave_up) {
   const int p = threadIdx.x - kProducer * 32;
   uint32_t issued = 0;
   RingPos<C::STAGES> stage;  // of both rings
@@ -114,7 +211,7 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
     KeyRuns ahead;
     ahead.look_up(row, a.line.step.page_shift, a.pages, C::KEYS / 16, piece.step(0) * C::KEYS, low, a.line.sinks, length);
     // over codes: the next batch is on its way while one is converted
-    using Batch = CodeBatch<C::D, C::CODES ? C::BITS : 8>;
+    using Batch = CodeBatch<C::D, 8>;
     Batch batch;
     if (C::CODES) batch.load(keys, ahead, piece.head, 0, p);
 #pragma unroll 1
@@ -133,23 +230,14 @@ __device__ __forceinline__ void fetch_tiles(const TcArgs& a, const CUtensorMap* 
         if constexpr (C::CODES) {
           // codes as they are; the softmax multiplies scores and probabilities by their keys' scales, in 32 bits
           if (side == 0) {
-            const int key = runs.key0 + p, page = __shfl_sync(0xffffffffu, runs.id, p >> 4), slot = issued % kScaleDepth;
+            const int key = runs.key0 + p, page = __shfl_sync(0xffffffffu, runs.id, p >> 4), slot = issued % Scales<C::STAGES>::DEPTH;
             const bool there = page >= 0 && runs.has(key);
-            if (C::BITS == 4) {
-              const int in_page = key & ((1 << a.line.step.page_shift) - 1);
-              const uint32_t k = there ? __ldg(scales4<C::D>(keys.scales, page, a.line.kv_heads, piece.head, a.line.step.page_shift) + in_page) : 0;
-              const uint32_t v = there ? __ldg(scales4<C::D>(values.scales, page, a.line.kv_heads, piece.head, a.line.step.page_shift) + in_page) : 0;
-              scales->key[slot][p] = power_of(k);
-              scales->value[slot][p] = power_of(v) * kGroupUnit;
-              scales->lift[slot][p] = lift_of(v);
-            } else {
-              const int64_t line = there ? keys.line(page, piece.head, key) : 0;
-              const float v = there ? __ldg(values.scales + line) : 0.f;
-              scales->key[slot][p] = there ? __ldg(keys.scales + line) : 0.f;
-              scales->value[slot][p] = v;
-              // a row of zeros must not let its own probability overflow, nor one that is not finite let the others vanish
-              scales->lift[slot][p] = v < INFINITY ? lg2_approx(fmaxf(v, 0x1p-100f)) : 0.f;
-            }
+            const int64_t line = there ? keys.line(page, piece.head, key) : 0;
+            const float v = there ? __ldg(values.scales + line) : 0.f;
+            scales->key[slot][p] = there ? __ldg(keys.scales + line) : 0.f;
+            scales->value[slot][p] = v;
+            // a row of zeros must not let its own probability overflow, nor one that is not finite let the others vanish
+            scales->lift[slot][p] = v < INFINITY ? lg2_approx(fmaxf(v, 0x1p-100f)) : 0.f;
           }
 #pragma unroll 1
           for (int from = 0; from < C::KEYS; from += Batch::ROWS) {
@@ -291,7 +379,7 @@ __device__ __forceinline__ void load_query_rows(const TcArgs& a, const Piece& pi
       v = *reinterpret_cast<const uint4*>(static_cast<const typename C::T*>(a.q) + int64_t(piece.seq.first + token) * a.qn +
                                           int64_t(piece.head * a.line.group + h) * a.qh + c * 8);
     }
-    if constexpr (C::CODES && std::is_same<typename C::T, __nv_bfloat16>::value) {
+    if constexpr (C::SCALED && std::is_same<typename C::T, __nv_bfloat16>::value) {
       const float down = row_to_half<PIECES>(v);
       if (c == 0) row_scale[r] = down;
     }
@@ -305,7 +393,7 @@ __device__ __forceinline__ void load_query_rows(const TcArgs& a, const Piece& pi
 }
 
 template <typename C>
-__device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Barriers* bars, Exchange* exchange, Scales* scales, uint32_t tmem, uint32_t q, int g, int half,
+__device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Barriers* bars, Exchange* exchange, Scales<C::STAGES>* scales, uint32_t tmem, uint32_t q, int g, int half,
                                              const volatile uint32_t* notes, const volatile int* tile_keys, uint32_t gave_up) {
   constexpr int D = C::D, KEYS = C::KEYS / 2, OUT = C::OUT;
   using T = typename C::T;
@@ -320,7 +408,7 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
   auto mine = [&](const Piece& p) { return p.seq.count * a.line.group - p.block * C::ROWS > group_row; };
   auto fetch = [&](const Piece& p) {
     turn ^= 1;
-    load_query_rows<C>(a, p, g, q + (C::SHARED ? 0 : g * C::QUERIES), C::CODES ? scales->row[turn][C::SHARED ? 0 : g] : nullptr);
+    load_query_rows<C>(a, p, g, q + (C::SHARED ? 0 : g * C::QUERIES), C::SCALED ? scales->row[turn][C::SHARED ? 0 : g] : nullptr);
     mbar_arrive_warp(smem_u32(bars->q_full + g));
   };
   auto wait = [&](uint32_t bar, uint32_t parity, unsigned int site) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, gave_up, site)); };
@@ -362,8 +450,8 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
       const uint32_t gone = notes[tile % kNotes] >> (half * (KEYS / 16)) & ((1u << (KEYS / 16)) - 1);
       tmem_load_wait();
       tmem_regs_ready<KEYS>(x);
-      const int slot_of_tile = tile % kScaleDepth;
-      if constexpr (C::CODES) {
+      const int slot_of_tile = tile % Scales<C::STAGES>::DEPTH;
+      if constexpr (C::SCALED) {
         if (std::is_same<T, __nv_bfloat16>::value && i == 0) scale = call_scale * scales->row[mine_turn][C::SHARED ? 0 : g][r];
         const ulonglong2* k = reinterpret_cast<const ulonglong2*>(scales->key[slot_of_tile] + half * KEYS);
 #pragma unroll
@@ -392,7 +480,7 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
       }
       const uint64_t scale2 = pack_f32x2(scale, scale);
       float best;
-      if constexpr (C::CODES) {
+      if constexpr (C::SCALED) {
         // The maximum is that of the row's own probabilities times scales, hidden keys left out: what is rounded is at most 1
         // (2^8 where the running maximum lags), and neither the other keys of the tile nor other rows move it.  (Against the
         // largest scale of the tile, 1024 tokens over 8K codes, 32 heads: 271 us for 269 at 128 channels, 203 for 190 at 64.)
@@ -453,7 +541,7 @@ __device__ __forceinline__ void softmax_rows(const TcArgs& a, Pieces pieces, Bar
           u = ex2_approx(u);
           w = ex2_approx(w);
           sum[c & 1] = add_f32x2(sum[c & 1], pack_f32x2(u, w));
-          if constexpr (C::CODES) {
+          if constexpr (C::SCALED) {
             const float2 v = *reinterpret_cast<const float2*>(scales->value[slot_of_tile] + half * KEYS + at);
             u *= v.x;
             w *= v.y;
@@ -533,15 +621,15 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
   extern __shared__ char smem_raw[];
   __shared__ Barriers bars;
   __shared__ Exchange exchange;
-  __shared__ __align__(16) typename std::conditional<C::CODES, Scales, char>::type scales_memory;
-  Scales* scales = reinterpret_cast<Scales*>(&scales_memory);
+  __shared__ __align__(16) typename std::conditional<C::SCALED, Scales<C::STAGES>, char>::type scales_memory;
+  Scales<C::STAGES>* scales = reinterpret_cast<Scales<C::STAGES>*>(&scales_memory);
   __shared__ LineShared<kThreads> shared;
   __shared__ uint32_t tmem_base, gave_up_word;
   __shared__ volatile uint32_t notes[kNotes];
   __shared__ volatile int tile_keys[kNotes];  // their first keys
   const int warp = threadIdx.x >> 5;
   const uint32_t smem = (smem_u32(smem_raw) + 1023) & ~1023u;
-  const uint32_t q = smem, v_ring = q + C::Q, k_ring = v_ring + C::STAGES * C::SIDE, gave_up = smem_u32(&gave_up_word);
+  const uint32_t q = smem, v_ring = q + C::Q, k_ring = v_ring + C::STAGES * C::SIDE, raw = k_ring + C::STAGES * C::SIDE, gave_up = smem_u32(&gave_up_word);
   if (threadIdx.x == 0) {
     gave_up_word = 0;
     for (int i = 0; i < 4; ++i) {
@@ -556,6 +644,10 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
       mbar_init(smem_u32(bars.p_full + g), 8);
       mbar_init(smem_u32(bars.o_full + g), 1);
       mbar_init(smem_u32(bars.o_free + g), 8);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(bars.raw_full + i), 1);
+      mbar_init(smem_u32(bars.raw_empty + i), 4);
     }
     mbar_init(smem_u32(&bars.q_empty), 1);
     mbar_init(smem_u32(&bars.drained), 1);
@@ -583,7 +675,8 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
     softmax_rows<C>(a, pieces, &bars, &exchange, scales, tmem, q, warp >> 3, (warp >> 2) & 1, notes, tile_keys, gave_up);
   } else if (warp < kIssuer) {
     regs_dec<kRegsProducer>();
-    fetch_tiles<C>(a, &key_map, &value_map, pieces, &bars, notes, tile_keys, scales, k_ring, v_ring, gave_up);
+    if constexpr (C::BITS == 4) convert_tiles<C>(a, pieces, &bars, notes, tile_keys, scales, k_ring, v_ring, raw, gave_up);
+    else fetch_tiles<C>(a, &key_map, &value_map, pieces, &bars, notes, tile_keys, scales, k_ring, v_ring, gave_up);
   } else {
     regs_dec<kRegsIssuer>();
     if (warp == kIssuer + 1 && (threadIdx.x & 31) == 0) {
@@ -592,6 +685,8 @@ __global__ __launch_bounds__(kThreads, 1) void paged_tc_kernel(const __grid_cons
       while (all.next(a.line, piece)) {}
       a.notes[blockIdx.x] = join_note(a.line, piece, total, finish, blockIdx.x, workers);
     }
+    if constexpr (C::BITS == 4)
+      if (warp == kIssuer + 2) fetch_raw<C>(a, pieces, &bars, raw, gave_up);
     if (warp == kIssuer) {
       issue_products<C>(int(pieces.left), &bars, notes, tmem, q, k_ring, v_ring, gave_up);
       __syncwarp();
@@ -699,7 +794,9 @@ TcArgs paged_tc_args(TcArgs a, int head_dim) {
   a.notes = reinterpret_cast<JoinNote*>(a.parts + size_t(kTcWorkers) * 2 * slot_floats(a.line.rows, head_dim));
   return a;
 }
-int paged_tc(const TcArgs& a, int dtype_code, int bits, int head_dim, cudaStream_t stream) {
+int paged_tc(const TcArgs& args, int dtype_code, int bits, int head_dim, cudaStream_t stream) {
+  TcArgs a = args;
+  if (bits == 4 && dtype_code == 2) a.scale_log2 /= kGroupUnit;  // bf16 takes group scales as they are
   return dtype_code == 1 ? launch_for<__half>(a, bits, head_dim, stream) : launch_for<__nv_bfloat16>(a, bits, head_dim, stream);
 }
 int paged_tc_join(const TcArgs& a, int dtype_code, int head_dim, cudaStream_t stream) {

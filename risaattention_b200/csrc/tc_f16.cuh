@@ -185,6 +185,79 @@ struct CodeBatch<D, 8> {
     }
   }
 };
+// Codes and scales of a tile's rows as they lie in the pages: rows of D / 2 bytes, the tokens' exponents, the groups' scales.  A
+// run of 16 keys is contiguous in each of the three, so one bulk copy brings it.
+template <int D, int KEYS>
+struct RawTile {
+  static constexpr int EXPONENTS = KEYS * (D / 2), GROUPS = EXPONENTS + KEYS, BYTES = GROUPS + KEYS * (D / 16);
+  static constexpr int RUN = 16 * (D / 2 + token_scale_bytes<D>());  // bytes of a run
+
+  // By a converged warp: the runs that exist, lane i the i-th; their bytes are announced on the barrier.
+  static __device__ __forceinline__ void fetch(const PoolView& pool, const KeyRuns& k, int head, uint32_t to, uint32_t barrier) {
+    const int lane = threadIdx.x & 31;
+    const bool there = k.id >= 0;
+    const uint32_t runs = __ballot_sync(0xffffffffu, there);
+    if (lane == 0) tc::mbar_expect_tx(barrier, __popc(runs) * RUN);
+    __syncwarp();
+    if (!there) return;
+    const int key = k.key0 + 16 * lane, slot = key & ((1 << pool.page_shift) - 1);
+    const uint8_t* scales = scales4<D>(pool.scales, k.id, pool.kv_heads, head, pool.page_shift);
+    tc::bulk_load(to + lane * 16 * (D / 2), pool.rows + pool.line(k.id, head, key) * (D / 2), 16 * (D / 2), barrier);
+    tc::bulk_load(to + EXPONENTS + lane * 16, scales + slot, 16, barrier);
+    tc::bulk_load(to + GROUPS + lane * D, groups4<D>(scales, pool.page_shift, slot), D, barrier);
+  }
+  static __device__ __forceinline__ uint32_t exponent(uint32_t tile, int row) {
+    uint32_t v;
+    asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(tile + EXPONENTS + row) : "memory");
+    return v;
+  }
+  // As the matrix instructions read them, by the 128 threads of a warpgroup; keys that do not exist become zeros.  In bf16 the
+  // token's scale is multiplied in (exactly: seven bits and the exponents of fp32), in fp16 it is left to the reader.
+  template <typename M>
+  static __device__ __forceinline__ void convert(uint32_t tile, const KeyRuns& k, uint32_t to, int thread) {
+    constexpr int PIECES = D / 32, EACH = 128 / PIECES;
+    const int piece = thread % PIECES;
+#pragma unroll 1
+    for (int r = thread / PIECES; r < KEYS; r += EACH) {
+      const bool there = __shfl_sync(0xffffffffu, k.id, r >> 4) >= 0 && k.has(k.key0 + r);
+      uint4 codes = make_uint4(0, 0, 0, 0);
+      uint16_t groups = 0;
+      uint32_t power = 0;
+      if (there) {
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(codes.x), "=r"(codes.y), "=r"(codes.z), "=r"(codes.w) : "r"(tile + r * (D / 2) + piece * 16) : "memory");
+        asm volatile("ld.shared.u16 %0, [%1];" : "=h"(groups) : "r"(tile + GROUPS + r * (D / 16) + piece * 2) : "memory");
+        power = exponent(tile, r);
+      }
+      const uint32_t w[4] = {codes.x, codes.y, codes.z, codes.w};
+      auto store = [&](const GroupScale<M>& first, const GroupScale<M>& second, auto&& finish) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          uint32_t x[4];
+          scaled_codes(w[i], i < 2 ? first : second, x);
+          finish(x);
+          store16(to + tile_offset<KEYS>(r, 4 * piece + i), make_uint4(x[0], x[1], x[2], x[3]));
+        }
+      };
+      const uint32_t first = twice(groups & 0xffu), second = twice(groups >> 8);
+      if constexpr (std::is_same<M, __half>::value) {
+        store(GroupScale<M>(first), GroupScale<M>(second), [](uint32_t (&)[4]) {});
+      } else {
+        const float unit = power_of(power) * kGroupUnit;
+        if (power <= 230) {
+          store(GroupScale<M>(first, unit), GroupScale<M>(second, unit), [](uint32_t (&)[4]) {});
+        } else {  // 136 times the scale would overflow: codes times group scales first
+          store(GroupScale<M>(first), GroupScale<M>(second), [&](uint32_t (&x)[4]) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const __nv_bfloat162 v = __hmul2(*reinterpret_cast<const __nv_bfloat162*>(&x[e]), __float2bfloat162_rn(unit));
+              x[e] = *reinterpret_cast<const uint32_t*>(&v);
+            }
+          });
+        }
+      }
+    }
+  }
+};
 // 4 bits: 32 codes and the scales of their two groups.
 template <int D>
 struct CodeBatch<D, 4> {

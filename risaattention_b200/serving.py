@@ -285,7 +285,8 @@ def paged_attention(q, cache, page_table, lengths, *, query_offsets=None, scale=
     cache's 16-bit values or codes as they are; probabilities are rounded to the type of ``q`` for the product
     with V.  Over a cache of codes it is probability times the key's scale that is rounded, to float16, in units
     of the largest such product that the token sees: of two scales that differ by more than 2^24 the smaller one's
-    values may be lost in that token.  (4-bit codes enter multiplied by their group's scale, exactly.)  A value that is not finite may also reach tokens of the same call
+    values may be lost in that token.  (4-bit codes enter multiplied by their group's scale, exactly; where 33
+    rows or more of bfloat16 queries meet them by all their scales, and probabilities are rounded to bfloat16.)  A value that is not finite may also reach tokens of the same call
     that do not see its key: it is multiplied by their probability, 0."""
     _check_cache(cache)
     if scale is None:

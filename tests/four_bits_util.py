@@ -89,3 +89,18 @@ def batch_of(lengths, chunks, *, q_heads, kv_heads, head_dim, page, dtype=torch.
         tensors[1].append(torch.cat((exponents, groups.flatten(-2)), -1))
     b.cache = risa.KeyValueCache(*tensors[0], *tensors[1])
     return b
+
+
+def assert_attention(batch, out, lse, **options):
+    """``serving_util.assert_attention`` for 4-bit caches: codes enter exactly, and a probability (times its key's scale) is rounded to
+    fp16 or, where bf16 queries are many, to bf16: half a step of the queries' type covers both."""
+    want, want_lse, spread, size = U.attention(batch, **options)
+    half = torch.finfo(out.dtype).eps / 2
+    score = size * out.shape[-1] * 2.0 ** -23 + 2.0 ** -20 * (1 + size)
+    assert torch.equal(torch.isneginf(lse.double()), torch.isneginf(want_lse))
+    visible = ~torch.isneginf(want_lse)
+    assert bool(((lse.double() - want_lse).abs()[visible] <= (score + 2.0 ** -22 * (1 + want_lse.abs()))[visible]).all())
+    bound = half * want.abs() + spread * (half + 2.1 * score[..., None]) + torch.finfo(out.dtype).tiny
+    error = (out.double() - want).abs()
+    assert bool((error <= bound).all()), f"{float((error / bound.clamp_min(1e-300)).max()):.2f} of the bound"
+    assert not bool(out[~visible].any())

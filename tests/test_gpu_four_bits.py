@@ -61,7 +61,7 @@ def test_attention(case, dtype, monkeypatch):
     offsets = None if set(chunks) == {1} else b.offsets
     out, lse = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=offsets, return_lse=True, **options)
     plain = {("causal" if k == "is_causal" else k): v for k, v in options.items() if k != "sinks"}
-    U.assert_attention(b, out, lse, **plain)
+    F.assert_attention(b, out, lse, **plain)
     # the weights that keys receive, for the rows' own denominators
     previous = torch.rand(len(lengths), kv_heads, b.table.shape[1] * page, device="cuda")
     got = risa.cached_key_weights(b.q, lse, b.cache, b.table, b.lengths, query_offsets=offsets, previous=previous, **options)
@@ -72,10 +72,10 @@ def test_attention(case, dtype, monkeypatch):
     assert bool(((got.double() - previous.double() - want).abs() <= bound).all())
 
 
-@pytest.mark.parametrize("chunk", [1, 40])
-def test_scales_of_every_size(chunk):
+@pytest.mark.parametrize("chunk,dtype", [(1, BF16), (40, BF16), (40, F16)])
+def test_scales_of_every_size(chunk, dtype):
     """Tokens whose scales differ by 2^40, scales of zero, groups of zero: small values are lost beside large ones, nothing else."""
-    b = F.batch_of([300, 64], [chunk, chunk], q_heads=4, kv_heads=2, head_dim=128, page=16, spread=0)
+    b = F.batch_of([300, 64], [chunk, chunk], q_heads=4, kv_heads=2, head_dim=128, page=16, spread=0, dtype=dtype)
     for scales, rest in ((b.cache.key_scales, 0), (b.cache.value_scales, 1)):
         exponents = scales[..., :16]
         used = exponents != 255
@@ -85,12 +85,13 @@ def test_scales_of_every_size(chunk):
         exponents[~used] = 255
         scales[..., 16 + 8 * 2:16 + 8 * 3][used.any(-1)] = 0  # all groups of the third token of a page
     out, lse = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets, return_lse=True)
-    U.assert_attention(b, out, lse)
+    F.assert_attention(b, out, lse)
 
 
-def test_a_row_that_is_not_finite_is_nan_for_those_who_see_it():
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_a_row_that_is_not_finite_is_nan_for_those_who_see_it(dtype):
     for chunk in (1, 40):
-        b = F.batch_of([200, 150], [chunk, chunk], q_heads=2, kv_heads=1, head_dim=128, page=16)
+        b = F.batch_of([200, 150], [chunk, chunk], q_heads=2, kv_heads=1, head_dim=128, page=16, dtype=dtype)
         want = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets)
         b.cache.value_scales[int(b.table[0, 3]), 0, 5] = 255
         out = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets)
@@ -228,6 +229,18 @@ def test_eviction(head_dim, page):
                 assert torch.equal(now[h], before[3 * w + s][h][chosen])
 
 
+@pytest.mark.parametrize("chunk", [2, 33])
+def test_the_largest_rows(chunk):
+    """Keys of up to 2^117 against queries as small, and such values: sums of 100 of them in 32 bits end at 2^124.  (Values of 2^126
+    themselves would overflow any such sum.)"""
+    b = F.batch_of([100], [chunk], q_heads=1, kv_heads=1, head_dim=128, page=16)
+    x = torch.randn(100, 1, 128, device="cuda").clamp(-3, 3) * 2.0 ** 115
+    risa.append_to_cache(b.cache, x.bfloat16(), x.flip(0).bfloat16(), b.table, b.lengths, query_offsets=torch.tensor([0, 100], dtype=torch.int32, device="cuda"))
+    b.q *= 2.0 ** -115
+    out, lse = risa.paged_attention(b.q, b.cache, b.table, b.lengths, query_offsets=b.offsets, return_lse=True)
+    F.assert_attention(b, out, lse)
+
+
 def test_a_conversation(monkeypatch):
     """Prompts taken in, tokens drawn, keys weighed and the conversation shortened, twice, with a window at the end."""
     d, page = 128, 16
@@ -246,14 +259,14 @@ def test_a_conversation(monkeypatch):
         q = risa.append_to_cache(cache, k, v, table, lengths, query_offsets=offsets, q=q, rotary=rotary, positions=positions)
         out, lse = risa.paged_attention(q, cache, table, lengths, query_offsets=offsets, return_lse=True)
         b = U.Batch(cache, table, lengths, offsets, chunks, q, 0)
-        U.assert_attention(b, out, lse)
+        F.assert_attention(b, out, lse)
         weights = risa.cached_key_weights(q, lse, cache, table, lengths, query_offsets=offsets, previous=weights)
     target = torch.arange(40, 48, dtype=torch.int32, device="cuda").view(2, 4)
     _, lengths, _ = risa.evict_from_cache(cache, table, lengths, weights, target, budget=60, recent=10)
     q = torch.randn(2, 4, d, device="cuda", generator=g).bfloat16()
     out, lse = risa.paged_attention(q, cache, target, lengths, window=20, sinks=3, return_lse=True)
     with_sinks(monkeypatch, 3)
-    U.assert_attention(U.Batch(cache, target, lengths, torch.tensor([0, 1, 2]), [1, 1], q, 0), out, lse, window=20)
+    F.assert_attention(U.Batch(cache, target, lengths, torch.tensor([0, 1, 2]), [1, 1], q, 0), out, lse, window=20)
 
 
 def test_pages_outside_the_pool():
@@ -297,4 +310,4 @@ def test_replayed_on_another_stream():
             side.wait_stream(torch.cuda.current_stream())
             graph.replay()
         torch.cuda.synchronize()
-        U.assert_attention(b, out, lse)
+        F.assert_attention(b, out, lse)

@@ -260,7 +260,7 @@ def test_children_of_a_prompt(kind, monkeypatch):
 
     def check():
         torch.cuda.synchronize()
-        U.assert_attention(U.Batch(cache, tables, sizes, torch.arange(5), [1] * 4, q, 0), out, lse)
+        F.assert_attention(U.Batch(cache, tables, sizes, torch.arange(5), [1] * 4, q, 0), out, lse)
         keys, values = risa.read_from_cache(cache, tables, sizes, dtype=torch.bfloat16)
         for s in range(4):
             own[s].append((keys[s].clone(), values[s].clone()))
@@ -287,6 +287,6 @@ def test_children_of_a_prompt(kind, monkeypatch):
     assert int(used) == 5 and counts.tolist() == [1] * 5 + [0]
     out, lse = risa.paged_attention(q, target, new, left, return_lse=True)
     assert left.tolist() == [0, 68, 0, 0]
-    U.assert_attention(U.Batch(target, new, left, torch.arange(5), [1] * 4, q, 0), out, lse)
+    F.assert_attention(U.Batch(target, new, left, torch.arange(5), [1] * 4, q, 0), out, lse)
     again = risa.read_from_cache(target, new, left, query_offsets=ints([0, 0, 68, 68, 68]), tokens=68, dtype=torch.bfloat16)
     assert torch.equal(again[0], keys[68:136]) and torch.equal(again[1], values[68:136])
