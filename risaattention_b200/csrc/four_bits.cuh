@@ -30,15 +30,17 @@ __device__ __forceinline__ const uint8_t* groups4(const uint8_t* scales, int pag
 }
 __device__ __forceinline__ float power_of(uint32_t exponent) { return __uint_as_float(exponent << 23); }
 // Its logarithm in units of group scales as they are read, for the running maximum of probabilities times scales.  A scale of zero
-// must not let its key's own probability overflow, nor one that is not finite let the others vanish, nor the largest ones (up to
-// 2^125) leave denominators no room above 2^-126: probabilities times scales then grow to 2^15, which fp16 holds.
-__device__ __forceinline__ float lift_of(uint32_t exponent) { return exponent == 255u ? 0.f : float(min(max(int(exponent) - 119, -100), 110)); }
+// must not let its key's own probability overflow, nor may the largest ones (up to 2^125) leave denominators no room above
+// 2^-126: probabilities times scales then grow to 2^15, which fp16 holds.  (Rows that see one that is not finite become NaN.)
+__device__ __forceinline__ float lift_of(uint32_t exponent) {
+  return fminf(fmaxf(__uint_as_float(0x4b000000u | exponent) - (8388608.0f + 119.0f), -100.f), 110.f);
+}
 
 // Group scales as a pair of 16-bit numbers, and what multiplies the bias of codes + 8 + 2^n.
 template <typename M> struct GroupScale;
 template <> struct GroupScale<__half> {
   __half2 s, c0, c1;
-  // pair: two e4m3 numbers in the low bytes of the halves
+  // pair: two e4m3 numbers in the low bytes of the halves, zeros above
   __device__ __forceinline__ explicit GroupScale(uint32_t pair) {
     const uint32_t bits = pair << 7;
     s = *reinterpret_cast<const __half2*>(&bits);
@@ -58,12 +60,18 @@ template <> struct GroupScale<__nv_bfloat16> {
 };
 __device__ __forceinline__ uint32_t twice(uint32_t byte) { return byte * 0x00010001u; }
 
+// (a & mask) | bits: one instruction (left to itself the compiler takes two).
+__device__ __forceinline__ uint32_t masked(uint32_t a, uint32_t mask, uint32_t bits) {
+  uint32_t r;
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(r) : "r"(a), "r"(mask), "r"(bits));
+  return r;
+}
 // Codes times scales: element i of the result holds field i of both halves of the word.  fp16: 0x6400 + u is 1024 + u, and
 // 0x5400 + 16 u is 64 + u; one fused multiply-add removes the bias and scales, exactly.
 __device__ __forceinline__ void scaled_codes(uint32_t word, const GroupScale<__half>& g, uint32_t (&x)[4]) {
   const uint32_t above = word >> 8;
-  const uint32_t b[4] = {(word & 0x000f000fu) | 0x64006400u, (word & 0x00f000f0u) | 0x54005400u, (above & 0x000f000fu) | 0x64006400u,
-                         (above & 0x00f000f0u) | 0x54005400u};
+  const uint32_t b[4] = {masked(word, 0x000f000fu, 0x64006400u), masked(word, 0x00f000f0u, 0x54005400u), masked(above, 0x000f000fu, 0x64006400u),
+                         masked(above, 0x00f000f0u, 0x54005400u)};
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const __half2 v = __hfma2(*reinterpret_cast<const __half2*>(&b[i]), g.s, i & 1 ? g.c1 : g.c0);
@@ -74,7 +82,7 @@ __device__ __forceinline__ void scaled_codes(uint32_t word, const GroupScale<__h
 __device__ __forceinline__ void scaled_codes(uint32_t word, const GroupScale<__nv_bfloat16>& g, uint32_t (&x)[4]) {
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
-    const uint32_t b = ((word >> (4 * i)) & 0x000f000fu) | 0x43004300u;
+    const uint32_t b = masked(word >> (4 * i), 0x000f000fu, 0x43004300u);
     const __nv_bfloat162 v = __hfma2(*reinterpret_cast<const __nv_bfloat162*>(&b), g.s, g.c0);
     x[i] = *reinterpret_cast<const uint32_t*>(&v);
   }

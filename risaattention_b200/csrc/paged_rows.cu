@@ -72,6 +72,8 @@ struct Tile {
   // more per SM.  Codes, whose conversion keeps the schedulers busy, gain from a third CTA (32 requests of up to 32K
   // keys: 280 us with two, 247 with three, 267 with four); 16-bit rows of 256 channels leave room for one.
   static constexpr int CTAS = D == 256 && !CODES ? 1 : CODES && D <= 128 && NT == 1 ? 3 : 2;
+  // Steps that share a maximum: with half of the bytes for the same instructions, 4-bit codes gain from halving the softmax's.
+  static constexpr int SUB = BITS == 4 && NT == 1 ? 2 : 1;
   static constexpr int BUDGET = 48 * 1024 / CTAS;  // per warp
   __host__ __device__ static constexpr int stages(int sides) {
     const int n = BUDGET / (sides * (SIDE + SCALES));
@@ -102,6 +104,11 @@ __device__ __forceinline__ void copy16(uint32_t to, const void* from, bool there
 __device__ __forceinline__ void copy4(uint32_t to, const void* from, bool there) {
   asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(to), "l"(from), "r"(there ? 4 : 0) : "memory");
 }
+// A copy whose offsets are known to the compiler (as operands of their own they cost three instructions).
+template <int TO, int FROM>
+__device__ __forceinline__ void copy16_at(uint32_t to, const void* from) {
+  asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(to), "l"(from), "n"(TO), "n"(FROM) : "memory");
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
@@ -118,6 +125,37 @@ __device__ __forceinline__ uint32_t transposed8x8(uint32_t v) {
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
 }
+// Reads at an offset known to the compiler.
+template <int AT>
+__device__ __forceinline__ uint4 read16_at(uint32_t address) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4 + %5];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(address), "n"(AT) : "memory");
+  return v;
+}
+template <int AT>
+__device__ __forceinline__ uint2 read8_at(uint32_t address) {
+  uint2 v;
+  asm volatile("ld.shared.v2.u32 {%0,%1}, [%2 + %3];" : "=r"(v.x), "=r"(v.y) : "r"(address), "n"(AT) : "memory");
+  return v;
+}
+template <int AT>
+__device__ __forceinline__ uint32_t read4_at(uint32_t address) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1 + %2];" : "=r"(v) : "r"(address), "n"(AT) : "memory");
+  return v;
+}
+template <int AT>
+__device__ __forceinline__ uint32_t read2_at(uint32_t address) {
+  uint16_t v;
+  asm volatile("ld.shared.u16 %0, [%1 + %2];" : "=h"(v) : "r"(address), "n"(AT) : "memory");
+  return v;
+}
+template <int AT>
+__device__ __forceinline__ uint32_t read1_at(uint32_t address) {
+  uint32_t v;
+  asm volatile("ld.shared.u8 %0, [%1 + %2];" : "=r"(v) : "r"(address), "n"(AT) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint4 read16(uint32_t address) {
   uint4 v;
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(address) : "memory");
@@ -126,21 +164,6 @@ __device__ __forceinline__ uint4 read16(uint32_t address) {
 __device__ __forceinline__ uint2 read8(uint32_t address) {
   uint2 v;
   asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(address) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t read4(uint32_t address) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(address) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t read2(uint32_t address) {
-  uint16_t v;
-  asm volatile("ld.shared.u16 %0, [%1];" : "=h"(v) : "r"(address) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t read1(uint32_t address) {
-  uint32_t v;
-  asm volatile("ld.shared.u8 %0, [%1];" : "=r"(v) : "r"(address) : "memory");
   return v;
 }
 __device__ __forceinline__ void write1(uint32_t address, uint32_t v) { asm volatile("st.shared.u8 [%0], %1;" ::"r"(address), "r"(v) : "memory"); }
@@ -178,6 +201,9 @@ struct Walk {
   int turn, skip;  // FRONT: from step `turn` on keys lie `skip` further, behind the first ones that stay visible
   int pages, pages_ahead;
   uint32_t base;
+  // 4-bit codes: this lane's pieces of the sequence's head in page 0, and bytes of a page
+  const char *key_rows, *value_rows, *scales[2];
+  int scale_each[2], page_rows, page_scales;
   unsigned int hidden;  // one bit per stage
   static constexpr int STAGES = C::stages(WITH_VALUES ? 2 : 1);
   static constexpr int SIDES = WITH_VALUES ? 2 : 1;
@@ -195,6 +221,67 @@ struct Walk {
     pages = look_up(lane);
     pages_ahead = look_up(32 + lane);
     hidden = 0;
+    if constexpr (C::BITS == 4) {
+      const int shift = a.line.step.page_shift, block = token_scale_bytes<C::D>() << shift;
+      page_rows = (a.line.kv_heads << shift) * C::ROW;
+      page_scales = a.line.kv_heads * block;
+      const int64_t of_head = (int64_t(head) << shift) * C::ROW + lane * 16;
+      key_rows = a.keys + of_head;
+      value_rows = a.values + of_head;
+#pragma unroll
+      for (int j = 0; j < SCALE_ROUNDS; ++j) {  // exponents, then group scales, of the keys, then of the values
+        const int index = j * 32 + lane, piece = index < C::SCALES / 16 ? index : index - C::SCALES / 16;
+        scales[j] = reinterpret_cast<const char*>(index < C::SCALES / 16 ? a.key_scales : a.value_scales) + int64_t(head) * block +
+                    (piece == 0 ? 0 : (1 << shift) + (piece - 1) * 16);
+        scale_each[j] = piece == 0 ? 1 : C::D / 16;
+      }
+    }
+  }
+  static constexpr int SCALE_ROUNDS = (SIDES * C::SCALES / 16 + 31) / 32;
+  // 16 keys that exist.
+  __device__ __forceinline__ void fetch_codes4(int key, int page, uint32_t to) {
+    const int lane = threadIdx.x & 31, slot = key & ((1 << a.line.step.page_shift) - 1);
+    const int64_t off = int64_t(page) * page_rows + slot * C::ROW;
+    const char *k = key_rows + off, *v = value_rows + off;
+    // 512 bytes further rows lie alike in the swizzle, but for heads of 256 channels: there every other 512
+    const int first = offset_of<C>(lane / C::CHUNKS, lane % C::CHUNKS);
+    const uint32_t at = to + first, odd = C::D == 256 ? to + (first ^ 64) : at;
+    copy16_at<0, 0>(at, k);
+    if constexpr (C::CHUNKS >= 4) copy16_at<512, 512>(odd, k);
+    if constexpr (C::CHUNKS == 8) copy16_at<1024, 1024>(at, k);
+    if constexpr (C::CHUNKS == 8) copy16_at<1536, 1536>(odd, k);
+    if constexpr (WITH_VALUES) {
+      copy16_at<C::SIDE, 0>(at, v);
+      if constexpr (C::CHUNKS >= 4) copy16_at<C::SIDE + 512, 512>(odd, v);
+      if constexpr (C::CHUNKS == 8) copy16_at<C::SIDE + 1024, 1024>(at, v);
+      if constexpr (C::CHUNKS == 8) copy16_at<C::SIDE + 1536, 1536>(odd, v);
+    }
+    const uint32_t scales_at = to + lane * 16;
+#pragma unroll
+    for (int j = 0; j < SCALE_ROUNDS; ++j)
+      if (j * 32 + lane < SIDES * C::SCALES / 16) {
+        const char* from = scales[j] + (int64_t(page) * page_scales + slot * scale_each[j]);
+        if (j == 0) copy16_at<SIDES * C::SIDE, 0>(scales_at, from);
+        else copy16_at<SIDES * C::SIDE + 512, 0>(scales_at, from);
+      }
+  }
+  // Some of the 16 (or none: good false) exist; the others become zeros, their scales are cleared by who reads them.
+  __device__ __forceinline__ void fetch_some_codes4(int key, int page, bool good, uint32_t to) {
+    const int lane = threadIdx.x & 31, slot = key & ((1 << a.line.step.page_shift) - 1);
+    const int64_t off = good ? int64_t(page) * page_rows + slot * C::ROW : 0;
+    const char *k = key_rows + off, *v = value_rows + off;
+#pragma unroll 1
+    for (int j = 0; j < C::CHUNKS / 2; ++j) {
+      const int r = (j * 32 + lane) / C::CHUNKS;
+      const uint32_t at = to + offset_of<C>(r, lane % C::CHUNKS);
+      const bool there = good && exists(key + r);
+      copy16(at, k + j * 512, there);
+      if (WITH_VALUES) copy16(at + C::SIDE, v + j * 512, there);
+    }
+#pragma unroll
+    for (int j = 0; j < SCALE_ROUNDS; ++j)
+      if (j * 32 + lane < SIDES * C::SCALES / 16)
+        copy16(to + SIDES * C::SIDE + (j * 32 + lane) * 16, scales[j] + (good ? int64_t(page) * page_scales + slot * scale_each[j] : 0), good);
   }
   // Fetches step i into stage i % STAGES (its stage number is given) and closes a copy group either way.
   __device__ __forceinline__ void fetch(int i, int stage) {
@@ -205,9 +292,23 @@ struct Walk {
       }
       const int lane = threadIdx.x & 31, key = key_of(i);
       const int page = __shfl_sync(0xffffffffu, pages, i & 31);
+      if constexpr (C::BITS == 4) {
+        // nearly all steps are of 16 keys that exist
+        if (uint32_t(page) < uint32_t(a.pages) && key >= low && key + 16 <= length) {
+          fetch_codes4(key, page, base + stage * STAGE);
+          if (hidden != 0) hidden &= ~(1u << stage);
+          copies_commit();
+          return;
+        }
+      }
       const bool good = key < length && page >= 0 && page < a.pages;
       if (key < length && !good && lane == 0) atomicCAS(a.status, 0u, unsigned(sequence) + 1u);
       hidden = good ? hidden & ~(1u << stage) : hidden | (1u << stage);
+      if constexpr (C::BITS == 4) {
+        fetch_some_codes4(key, page, good, base + stage * STAGE);
+        copies_commit();
+        return;
+      }
       const int64_t line = good ? (((int64_t(page) * a.line.kv_heads + head) << a.line.step.page_shift) +
                                    (key & ((1 << a.line.step.page_shift) - 1)))
                                 : 0;
@@ -229,28 +330,16 @@ struct Walk {
           copy4(to + SIDES * C::SIDE + lane * 4, s + line + r, whole || (good && exists(key + r)));
         }
       };
-      if (C::BITS == 4) {  // exponents, then group scales; those of keys that do not exist are cleared by who reads them
-        constexpr int PIECES = C::SCALES / 16;
-        const int slot = key & ((1 << a.line.step.page_shift) - 1);
-        const int64_t block = good ? scales4<C::D>(nullptr, page, a.line.kv_heads, head, a.line.step.page_shift) - static_cast<const uint8_t*>(nullptr) : 0;
-#pragma unroll
-        for (int j = 0; j < (SIDES * PIECES + 31) / 32; ++j) {
-          const int index = j * 32 + lane, piece = index < PIECES ? index : index - PIECES;
-          const char* from = reinterpret_cast<const char*>(index < PIECES ? a.key_scales : a.value_scales) + block;
-          from += piece == 0 ? slot : (1 << a.line.step.page_shift) + slot * (C::D / 16) + (piece - 1) * 16;
-          if (index < SIDES * PIECES) copy16(to + SIDES * C::SIDE + index * 16, from, good);
-        }
-      }
       // nearly all steps are of 16 keys that exist
       if (good && key >= low && key + 16 <= length) copy(std::true_type{});
       else copy(std::false_type{});
     }
     copies_commit();
   }
-  // Scales of 4-bit keys that do not exist (they lie beside those that do) become zeros.
-  __device__ __forceinline__ void clear_missing(uint32_t data, int key) const {
+  // Scales of 4-bit keys that do not exist (they lie beside those that do), or of a step that does not, become zeros.
+  __device__ __forceinline__ void clear_missing(uint32_t data, int key, bool all) const {
     const int lane = threadIdx.x & 31;
-    if (lane < 16 && !exists(key + lane)) {
+    if (lane < 16 && (all || !exists(key + lane))) {
 #pragma unroll
       for (int side = 0; side < SIDES; ++side) {
         const uint32_t scales = data + SIDES * C::SIDE + side * C::SCALES;
@@ -327,24 +416,27 @@ __device__ __forceinline__ void score_step(uint32_t keys, uint32_t scales, const
     constexpr int RUNS = C::D == 256 ? 2 : 1, WORDS = C::D == 64 ? 2 : 4, GROUPS = WORDS / 2;
 #pragma unroll
     for (int run = 0; run < RUNS; ++run) {
+      // keys g and g + 8 lie alike in the swizzle
+      constexpr int EIGHT = 8 * C::ROW, SCALE_EIGHT = 8 * (C::D / 16);
       uint32_t w[2][WORDS], scale[2];
-#pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        const int key = g + 8 * i;
-        if constexpr (WORDS == 4) {
-          const uint4 v = read16(keys + offset_of<C>(key, run * 4 + t));
-          w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
-          scale[i] = read2(scales + 16 + key * (C::D / 16) + run * 8 + t * 2);
-        } else {
-          const uint2 v = read8(keys + offset_of<C>(key, t >> 1) + (t & 1) * 8);
-          w[i][0] = v.x; w[i][1] = v.y;
-          scale[i] = read1(scales + 16 + key * (C::D / 16) + t);
-        }
+      if constexpr (WORDS == 4) {
+        const uint32_t at = keys + offset_of<C>(g, run * 4 + t), of = scales + g * (C::D / 16) + t * 2;
+        const uint4 u = read16_at<0>(at), v = read16_at<EIGHT>(at);
+        w[0][0] = u.x; w[0][1] = u.y; w[0][2] = u.z; w[0][3] = u.w;
+        w[1][0] = v.x; w[1][1] = v.y; w[1][2] = v.z; w[1][3] = v.w;
+        scale[0] = run ? read2_at<16 + 8>(of) : read2_at<16>(of);
+        scale[1] = run ? read2_at<16 + 8 + SCALE_EIGHT>(of) : read2_at<16 + SCALE_EIGHT>(of);
+      } else {
+        const uint32_t at = keys + offset_of<C>(g, t >> 1) + (t & 1) * 8, of = scales + g * (C::D / 16) + t;
+        const uint2 u = read8_at<0>(at), v = read8_at<EIGHT>(at);
+        w[0][0] = u.x; w[0][1] = u.y;
+        w[1][0] = v.x; w[1][1] = v.y;
+        scale[0] = read1_at<16>(of);
+        scale[1] = read1_at<16 + SCALE_EIGHT>(of);
       }
 #pragma unroll
       for (int group = 0; group < GROUPS; ++group) {
-        const GroupScale<__half> lo(twice(GROUPS == 1 ? scale[0] : group ? scale[0] >> 8 : scale[0] & 0xffu));
-        const GroupScale<__half> hi(twice(GROUPS == 1 ? scale[1] : group ? scale[1] >> 8 : scale[1] & 0xffu));
+        const GroupScale<__half> lo(__byte_perm(scale[0], 0, group ? 0x4141 : 0x4040)), hi(__byte_perm(scale[1], 0, group ? 0x4141 : 0x4040));
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
           uint32_t l[4], h[4];
@@ -392,23 +484,36 @@ __device__ __forceinline__ void value_step(uint32_t values, uint32_t scales, con
   const int lane = threadIdx.x & 31, g = lane >> 2, t = lane & 3;
   if constexpr (C::BITS == 4) {
     constexpr int WORDS = C::D / 64;  // of a key: half a group, a group or two groups
+    // keys 2 t and 2 t + 1, and those eight further, which lie alike in the swizzle
+    constexpr int EIGHT = 8 * C::ROW, GROUP_BYTES = C::D / 16;
     uint32_t w[4][WORDS], scale[4];
+    const uint32_t of = scales + 2 * t * GROUP_BYTES + (WORDS == 4 ? 2 * g : WORDS == 2 ? g : g >> 1);
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int key = 2 * t + (i & 1) + (i >> 1) * 8;
-      const uint32_t of = scales + 16 + key * (C::D / 16);
+    for (int i = 0; i < 2; ++i) {
+      const uint32_t at = values + offset_of<C>(2 * t + i, WORDS == 4 ? g : WORDS == 2 ? g >> 1 : g >> 2) + (WORDS == 4 ? 0 : WORDS == 2 ? (g & 1) * 8 : (g & 3) * 4);
       if constexpr (WORDS == 4) {
-        const uint4 v = read16(values + offset_of<C>(key, g));
-        w[i][0] = v.x; w[i][1] = v.y; w[i][2] = v.z; w[i][3] = v.w;
-        scale[i] = read2(of + 2 * g);
+        const uint4 u = read16_at<0>(at), v = read16_at<EIGHT>(at);
+        w[i][0] = u.x; w[i][1] = u.y; w[i][2] = u.z; w[i][3] = u.w;
+        w[i + 2][0] = v.x; w[i + 2][1] = v.y; w[i + 2][2] = v.z; w[i + 2][3] = v.w;
       } else if constexpr (WORDS == 2) {
-        const uint2 v = read8(values + offset_of<C>(key, g >> 1) + (g & 1) * 8);
-        w[i][0] = v.x; w[i][1] = v.y;
-        scale[i] = read1(of + g);
+        const uint2 u = read8_at<0>(at), v = read8_at<EIGHT>(at);
+        w[i][0] = u.x; w[i][1] = u.y;
+        w[i + 2][0] = v.x; w[i + 2][1] = v.y;
       } else {
-        w[i][0] = read4(values + offset_of<C>(key, g >> 2) + (g & 3) * 4);
-        scale[i] = read1(of + (g >> 1));
+        w[i][0] = read4_at<0>(at);
+        w[i + 2][0] = read4_at<EIGHT>(at);
       }
+    }
+    if constexpr (WORDS == 4) {
+      scale[0] = read2_at<16>(of);
+      scale[1] = read2_at<16 + GROUP_BYTES>(of);
+      scale[2] = read2_at<16 + 8 * GROUP_BYTES>(of);
+      scale[3] = read2_at<16 + 9 * GROUP_BYTES>(of);
+    } else {
+      scale[0] = read1_at<16>(of);
+      scale[1] = read1_at<16 + GROUP_BYTES>(of);
+      scale[2] = read1_at<16 + 8 * GROUP_BYTES>(of);
+      scale[3] = read1_at<16 + 9 * GROUP_BYTES>(of);
     }
 #pragma unroll
     for (int group = 0; group < (WORDS + 1) / 2; ++group) {
@@ -551,62 +656,76 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
 #pragma unroll
         for (int i = 0; i < 4; ++i) o[nt][mt][i] = 0.f;
     }
+    constexpr int SUB = C::SUB;
+    static_assert(W::STAGES >= 2 * SUB, "ring");
 #pragma unroll
-    for (int i = 0; i < W::STAGES - 1; ++i) walk.fetch(i, i);
+    for (int i = 0; i < W::STAGES - SUB; ++i) walk.fetch(i, i);
     int stage = 0;
-    for (int i = 0; i < walk.count; ++i) {
-      {
-        const int next = stage == 0 ? W::STAGES - 1 : stage - 1;  // the stage of step i + STAGES - 1
-        copies_wait<W::STAGES - 2>();
-        __syncwarp();
-        walk.fetch(i + W::STAGES - 1, next);
-      }
-      const uint32_t data = ring + stage * W::STAGE;
-      const int key = walk.key_of(i);
-      const bool hidden = walk.hidden >> stage & 1;
-      float acc[NT][4];
-      const uint32_t key_scales = data + 2 * C::SIDE, value_scales = key_scales + C::SCALES;
-      if (C::BITS == 4 && (key < low || key + 16 > seq.length)) walk.clear_missing(data, key);
-      score_step<C>(data, key_scales, qf, acc);
-      float ks0 = 1.f, ks1 = 1.f, vs0 = 1.f, vs1 = 1.f, lift0 = 0.f, lift1 = 0.f;
-      if (C::BITS == 4) {
-        const uint32_t e0 = read1(value_scales + g), e1 = read1(value_scales + g + 8);
-        ks0 = power_of(read1(key_scales + g));
-        ks1 = power_of(read1(key_scales + g + 8));
-        vs0 = power_of(e0) * kGroupUnit;
-        vs1 = power_of(e1) * kGroupUnit;
-        lift0 = lift_of(e0);
-        lift1 = lift_of(e1);
-      }
-      if (C::BITS == 8) {
-        ks0 = read_float(key_scales + g * 4);
-        ks1 = read_float(key_scales + (g + 8) * 4);
-        vs0 = read_float(value_scales + g * 4);
-        vs1 = read_float(value_scales + (g + 8) * 4);
-        // a row of zeros must not let its own probability overflow, nor one that is not finite let the others vanish
-        lift0 = vs0 < INFINITY ? lg2_approx(fmaxf(vs0, 0x1p-100f)) : 0.f;
-        lift1 = vs1 < INFINITY ? lg2_approx(fmaxf(vs1, 0x1p-100f)) : 0.f;
-      }
+    for (int i = 0; i < walk.count; i += SUB) {
+      int next = stage < SUB ? stage + W::STAGES - SUB : stage - SUB;  // the stages of the steps in front of i, free by now
+      copies_wait<W::STAGES - 2 * SUB>();
+      __syncwarp();
 #pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
+      for (int u = 0; u < SUB; ++u) {
+        walk.fetch(i + W::STAGES - SUB + u, next);
+        next = next + 1 == W::STAGES ? 0 : next + 1;
+      }
+      uint32_t data[SUB];
+      float acc[SUB][NT][4], vs[SUB][2], lift[SUB][2];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) acc[nt][e] *= C::CODES ? (e < 2 ? ks0 : ks1) * factor[nt][e & 1] : factor[nt][e & 1];
-      if (hidden || key < all_lo || key + 16 > all_hi) {
+      for (int u = 0; u < SUB; ++u) {
+        data[u] = ring + stage * W::STAGE;
+        const int key = walk.key_of(i + u);
+        // the last step may stand alone
+        const bool alone = SUB > 1 && i + u >= walk.count, hidden = alone || (walk.hidden >> stage & 1);
+        const uint32_t key_scales = data[u] + 2 * C::SIDE, value_scales = key_scales + C::SCALES;
+        if (C::BITS == 4 && (alone || key < low || key + 16 > seq.length)) walk.clear_missing(data[u], key, alone);
+        score_step<C>(data[u], key_scales, qf, acc[u]);
+        float ks0 = 1.f, ks1 = 1.f;
+        vs[u][0] = vs[u][1] = 1.f;
+        lift[u][0] = lift[u][1] = 0.f;
+        if (C::BITS == 4) {
+          const uint32_t of = key_scales + g, e0 = read1_at<C::SCALES>(of), e1 = read1_at<C::SCALES + 8>(of);
+          ks0 = power_of(read1_at<0>(of));
+          ks1 = power_of(read1_at<8>(of));
+          vs[u][0] = power_of(e0) * kGroupUnit;
+          vs[u][1] = power_of(e1) * kGroupUnit;
+          lift[u][0] = lift_of(e0);
+          lift[u][1] = lift_of(e1);
+        }
+        if (C::BITS == 8) {
+          ks0 = read_float(key_scales + g * 4);
+          ks1 = read_float(key_scales + (g + 8) * 4);
+          vs[u][0] = read_float(value_scales + g * 4);
+          vs[u][1] = read_float(value_scales + (g + 8) * 4);
+          // a row of zeros must not let its own probability overflow, nor one that is not finite let the others vanish
+#pragma unroll
+          for (int e = 0; e < 2; ++e) lift[u][e] = vs[u][e] < INFINITY ? lg2_approx(fmaxf(vs[u][e], 0x1p-100f)) : 0.f;
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const int k = key + g + (e >> 1) * 8;
-            if (hidden || !outside_gap<C>(a.line, k, lo[nt][e & 1]) || k >= hi[nt][e & 1]) acc[nt][e] = -INFINITY;
-          }
+          for (int e = 0; e < 4; ++e) acc[u][nt][e] *= C::CODES ? (e < 2 ? ks0 : ks1) * factor[nt][e & 1] : factor[nt][e & 1];
+        if (hidden || key < all_lo || key + 16 > all_hi) {
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              const int k = key + g + (e >> 1) * 8;
+              if (hidden || !outside_gap<C>(a.line, k, lo[nt][e & 1]) || k >= hi[nt][e & 1]) acc[u][nt][e] = -INFINITY;
+            }
+        }
+        stage = stage + 1 == W::STAGES ? 0 : stage + 1;
       }
-      uint32_t p[NT][2];
+      uint32_t p[SUB][NT][2];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt) {
         float top[2], keep[2];
 #pragma unroll
         for (int i2 = 0; i2 < 2; ++i2) {
-          float x = fmaxf(acc[nt][i2] + lift0, acc[nt][2 + i2] + lift1);
+          float x = fmaxf(acc[0][nt][i2] + lift[0][0], acc[0][nt][2 + i2] + lift[0][1]);
+#pragma unroll
+          for (int u = 1; u < SUB; ++u) x = fmaxf(x, fmaxf(acc[u][nt][i2] + lift[u][0], acc[u][nt][2 + i2] + lift[u][1]));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
           x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
@@ -628,17 +747,20 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
             o[nt][mt][3] *= keep[1];
           }
         }
-        float e[4];
 #pragma unroll
-        for (int i2 = 0; i2 < 4; ++i2) e[i2] = ex2_approx(acc[nt][i2] - m[nt][i2 & 1]);
-        l[nt][0] += e[0] + e[2];
-        l[nt][1] += e[1] + e[3];
-        // Probabilities (times scales) leave 32 bits here: half a step, 2^-8 of the value in bf16, 2^-11 in fp16.
-        p[nt][0] = transposed8x8(Half2<typename C::M>::pack(C::CODES ? e[0] * vs0 : e[0], C::CODES ? e[1] * vs0 : e[1]));
-        p[nt][1] = transposed8x8(Half2<typename C::M>::pack(C::CODES ? e[2] * vs1 : e[2], C::CODES ? e[3] * vs1 : e[3]));
+        for (int u = 0; u < SUB; ++u) {
+          float e[4];
+#pragma unroll
+          for (int i2 = 0; i2 < 4; ++i2) e[i2] = ex2_approx(acc[u][nt][i2] - m[nt][i2 & 1]);
+          l[nt][0] += e[0] + e[2];
+          l[nt][1] += e[1] + e[3];
+          // Probabilities (times scales) leave 32 bits here: half a step, 2^-8 of the value in bf16, 2^-11 in fp16.
+          p[u][nt][0] = transposed8x8(Half2<typename C::M>::pack(C::CODES ? e[0] * vs[u][0] : e[0], C::CODES ? e[1] * vs[u][0] : e[1]));
+          p[u][nt][1] = transposed8x8(Half2<typename C::M>::pack(C::CODES ? e[2] * vs[u][1] : e[2], C::CODES ? e[3] * vs[u][1] : e[3]));
+        }
       }
-      value_step<C>(data + C::SIDE, value_scales, p, o);
-      stage = stage + 1 == W::STAGES ? 0 : stage + 1;
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) value_step<C>(data[u] + C::SIDE, data[u] + 2 * C::SIDE + C::SCALES, p[u], o);
     }
     copies_wait<0>();
     __syncwarp();
@@ -780,9 +902,9 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void weigh_rows_kernel(const Row
       const bool hidden = walk.hidden >> stage & 1;
       float ks0 = 1.f, ks1 = 1.f;
       if (C::BITS == 4) {
-        if (key < low || key + 16 > seq.length) walk.clear_missing(data, key);
-        ks0 = power_of(read1(data + C::SIDE + g));
-        ks1 = power_of(read1(data + C::SIDE + g + 8));
+        if (key < low || key + 16 > seq.length) walk.clear_missing(data, key, false);
+        ks0 = power_of(read1_at<C::SIDE>(data + g));
+        ks1 = power_of(read1_at<C::SIDE + 8>(data + g));
       }
       if (C::BITS == 8) {
         ks0 = read_float(data + C::SIDE + g * 4);
