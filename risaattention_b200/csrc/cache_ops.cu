@@ -289,10 +289,10 @@ __device__ __forceinline__ uint32_t code_bits(int code, int channel) { return ui
 
 // Group scale: the largest value of the group over 7 token scales, rounded to e4m3.  Code: the value over both scales, rounded
 // to nearest even.  Values of 16 bits meet the borders between codes (and between scales) exactly or not nearly, so that
-// for rows as they came this is decided in 32 bits: the quotient by 7 is correctly rounded, and a value's distance from the
-// border below it comes from one fused multiply-add, whose sign is right.  Rotated values are off by 2^-20 of the row's largest
-// value at most (cosine and sine 2^-22 each, of a pair whose length is sqrt(2) times that at most); `doubtful` says that one of
-// them lies within twice that of a border.
+// for rows as they came this is decided in 32 bits: a quotient near a border of scales is divided correctly, and a value's
+// quotient, corrected by its remainder, is exact where it is half of a whole number.  Rotated values are off by 2^-21 of
+// the row's largest value at most (cosine and sine 2^-22.8 each, of a pair whose length is sqrt(2) times that at most); `doubtful`
+// says that one of them lies within twice that of a border.
 __device__ __forceinline__ Row4 row4_of(const float (&x)[8], int lanes, bool& doubtful) {
   Row4 r;
   float group = fabsf(x[0]);
@@ -308,22 +308,33 @@ __device__ __forceinline__ Row4 row4_of(const float (&x)[8], int lanes, bool& do
   r.group = 0;
   doubtful = false;
   if (r.exponent == 0 || r.exponent == 255) return r;
-  const float to_units = __uint_as_float(uint32_t(254 - r.exponent) << 23), slack = most * to_units * 0x1p-19f;
-  const float ratio = __fdiv_rn(group * to_units, 7.0f);
-  r.group = e4m3_pair(0.f, ratio) & 0xffu;
-  const uint32_t around = e4m3_pair(ratio + slack, fmaxf(ratio - slack, 0.f));
+  const float to_units = __uint_as_float(uint32_t(254 - r.exponent) << 23), slack = most * to_units * 0x1p-20f;
+  float ratio = group * to_units;
+  uint32_t around = e4m3_pair(fmaf(ratio, 1.0f / 7.0f, slack), fmaxf(fmaf(ratio, 1.0f / 7.0f, -slack), 0.f));
   doubtful = (around & 0xffu) != around >> 8 || (bits - 16) >> 23 != (bits + 16) >> 23;
+  if ((around & 0xffu) != around >> 8) around = e4m3_pair(0.f, __fdiv_rn(ratio, 7.0f));
+  r.group = around & 0xffu;
   if (r.group == 0) return r;
-  const uint32_t half_bits = r.group << 7;
-  const float scale = __half2float(__ushort_as_half(uint16_t(half_bits))) * kGroupUnit, inverse = 1.0f / scale;
-  r.word = 0;
+  const float scale = __half2float(__ushort_as_half(uint16_t(r.group << 7))) * kGroupUnit;
+  float inverse;
+  asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
+  float code[8], nearest = 1.f;
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
-    const float y = x[i] * to_units, below = floorf(y * inverse), past = fmaf(-(below + 0.5f), scale, y);
-    const int code = int(below);
-    r.word |= code_bits(code + (past > 0.f || (past == 0.f && (code & 1)) ? 1 : 0), i);
-    doubtful = doubtful || fabsf(past) < slack;
+    const float y = x[i] * to_units, guess = y * inverse;
+    const float quotient = fmaf(fmaf(-guess, scale, y), inverse, guess);  // exact where it is half of a whole number
+    code[i] = (quotient + 12582912.0f) - 12582912.0f;
+    nearest = fminf(nearest, fabsf(fabsf(quotient - code[i]) - 0.5f));
   }
+  doubtful = doubtful || nearest * scale < slack;
+  if (r.group < 8) {  // scales below 2^-6 are rounded coarsely: quotients past 7
+#pragma unroll
+    for (int i = 0; i < 8; ++i) code[i] = fminf(fmaxf(code[i], -7.f), 7.f);
+  }
+  float half_words[2] = {8388608.0f + 0x8888, 8388608.0f + 0x8888};  // four codes + 8 in the low bits
+#pragma unroll
+  for (int i = 0; i < 8; ++i) half_words[i & 1] = fmaf(code[i], float(1 << (4 * (i >> 1))), half_words[i & 1]);
+  r.word = __byte_perm(__float_as_uint(half_words[0]), __float_as_uint(half_words[1]), 0x5410);
   return r;
 }
 // The same for a rotated row that came too near a border, in 64 bits: from the channels as they came (`own`, and `other` of a
@@ -357,6 +368,8 @@ __device__ __noinline__ Row4 row4_of_rotated(const AppendArgs& a, Run<T> own, Ru
   for (int off = lanes >> 1; off > 1; off >>= 1) most = fmax(most, __shfl_xor_sync(0xffffffffu, most, off));
   Row4 r{0x88888888u, 0, 0};
   if (most == 0.0) return r;
+  r.exponent = 255;  // not finite (fmax passes over a NaN, whose row the other form has stored)
+  if (!(most < double(INFINITY))) return r;
   r.exponent = max(int((__double_as_longlong(most) + (0xfffffffffffffll - 0x8800000000000ll)) >> 52) - 1023 - 11 + 127, 1);
   const double to_units = __longlong_as_double(int64_t(1023 + 127 - r.exponent) << 52), ratio = group * to_units / 7.0;
   // steps of 2^-3 of the leading bit, 2^-9 at least
@@ -370,6 +383,15 @@ __device__ __noinline__ Row4 row4_of_rotated(const AppendArgs& a, Run<T> own, Ru
   return r;
 }
 
+__device__ __forceinline__ void store_row4(const AppendArgs& a, bool key, const Row4& r, int64_t page, int h, int slot_in_page, int lanes, int lane) {
+  const int64_t of_head = page * a.kv_heads + h;
+  const int groups = lanes >> 1;
+  reinterpret_cast<uint32_t*>(key ? a.keys : a.values)[((of_head << a.step.page_shift) + slot_in_page) * lanes + lane] = r.word;
+  uint8_t* scales = reinterpret_cast<uint8_t*>(key ? a.key_scales : a.value_scales) + ((of_head * (1 + groups)) << a.step.page_shift);
+  if (lane == 0) scales[slot_in_page] = uint8_t(r.exponent);
+  if ((lane & 1) == 0) scales[(1 << a.step.page_shift) + slot_in_page * groups + (lane >> 1)] = uint8_t(r.group);
+}
+
 // One CTA per new token.  head_dim / 8 lanes hold a row, eight channels each; the CTA's row slots walk
 // the token's query heads, key heads and value heads with the cosines and sines of the lane's channels
 // kept in registers.  A thread computes those of one pair for the whole token (8160 tokens below: 70 us where every lane
@@ -381,7 +403,7 @@ __device__ __noinline__ Row4 row4_of_rotated(const AppendArgs& a, Run<T> own, Ru
 // requests, with the call: 11.5 to 12.4 us.
 constexpr int kRowsAhead = 3;  // rows of a slot on their way at once: half of a token of 32 + 2 x 8 heads of 128
 template <typename T, int BITS>
-__global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
+__global__ __launch_bounds__(128, BITS == 4 ? 6 : 8) void append_kernel(const AppendArgs a) {
   __shared__ __align__(16) float cosines[128], sines[128];
   chain_wait();
   chain_release();
@@ -461,6 +483,7 @@ __global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
     }
   }
   const int slot_in_page = place & ((1 << a.step.page_shift) - 1);
+  uint32_t again = 0;  // 4 bits: passes (modulo 32) of this warp whose keys came too near a border
   for (int r0 = 0; r0 < rows; r0 += slots * kRowsAhead) {
     if (r0 > 0) load_rows(r0);
 #pragma unroll
@@ -472,8 +495,6 @@ __global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
       const int h = kind == 0 ? r : kind == 1 ? r - a.q_heads : r - a.q_heads - a.kv_heads;
       float x[8];
       run[j].values(x);
-      Run<T> other;
-      other.zero();
       if (a.turns != nullptr && __any_sync(0xffffffffu, kind < 2)) {
         if (a.interleaved) {
           if (turned && kind < 2) {
@@ -485,6 +506,7 @@ __global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
             }
           }
         } else {
+          Run<T> other;
           other.raw.x = __shfl_sync(0xffffffffu, run[j].raw.x, partner);
           other.raw.y = __shfl_sync(0xffffffffu, run[j].raw.y, partner);
           other.raw.z = __shfl_sync(0xffffffffu, run[j].raw.z, partner);
@@ -500,18 +522,9 @@ __global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
       const int64_t row = ((page * a.kv_heads + h) << a.step.page_shift) + slot_in_page;
       if (BITS == 4 && __any_sync(0xffffffffu, kind > 0)) {
         bool doubtful;
-        Row4 r4 = row4_of(x, lanes, doubtful);
-        if (a.turns != nullptr && __any_sync(0xffffffffu, doubtful && there && kind == 1)) {
-          const Row4 sure = row4_of_rotated<T>(a, run[j], other, token, place, lanes, channel);
-          if (kind == 1 && r4.exponent != 255) r4 = sure;
-        }
-        if (there && kind > 0 && page >= 0) {
-          reinterpret_cast<uint32_t*>(kind == 1 ? a.keys : a.values)[row * lanes + lane] = r4.word;
-          const int groups = lanes >> 1;
-          uint8_t* scales = reinterpret_cast<uint8_t*>(kind == 1 ? a.key_scales : a.value_scales) + (((page * a.kv_heads + h) * (1 + groups)) << a.step.page_shift);
-          if (lane == 0) scales[slot_in_page] = uint8_t(r4.exponent);
-          if ((lane & 1) == 0) scales[(1 << a.step.page_shift) + slot_in_page * groups + (lane >> 1)] = uint8_t(r4.group);
-        }
+        const Row4 r4 = row4_of(x, lanes, doubtful);
+        if (there && kind > 0 && page >= 0) store_row4(a, kind == 1, r4, page, h, slot_in_page, lanes, lane);
+        if (a.turns != nullptr && __any_sync(0xffffffffu, doubtful && there && kind == 1)) again |= 1u << (r0 / slots + j & 31);
       }
       if (BITS == 8 && __any_sync(0xffffffffu, kind > 0)) {
         const float most = row_absmax(x, lanes), scale = most / 127.0f;
@@ -533,6 +546,24 @@ __global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
       if (there && kind == 0) store8(static_cast<T*>(a.q_out) + token * a.on + h * a.oh + channel, x);
     }
   }
+  if (BITS == 4 && again != 0) {
+    // such rows once more, in 64 bits.  (Called from within the passes this cost every row 26 us of 116: registers kept for the call.)
+#pragma unroll 1
+    for (int pass = 0; pass * slots < rows; ++pass) {
+      if (!(again >> (pass & 31) & 1)) continue;
+      const int r = pass * slots + slot, h = r - a.q_heads;
+      const bool is_key = h >= 0 && h < a.kv_heads;
+      Run<T> own, other;
+      own.zero();
+      if (is_key) own.load(static_cast<const T*>(a.k) + token * a.kn + h * a.kh + channel);
+      other.raw.x = __shfl_sync(0xffffffffu, own.raw.x, partner);
+      other.raw.y = __shfl_sync(0xffffffffu, own.raw.y, partner);
+      other.raw.z = __shfl_sync(0xffffffffu, own.raw.z, partner);
+      other.raw.w = __shfl_sync(0xffffffffu, own.raw.w, partner);
+      const Row4 r4 = row4_of_rotated<T>(a, own, other, token, place, lanes, channel);
+      if (is_key && page >= 0 && r4.exponent != 255) store_row4(a, true, r4, page, h, slot_in_page, lanes, lane);
+    }
+  }
 }
 
 // ---- reading back -----------------------------------------------------------------------------------------
@@ -548,18 +579,26 @@ struct ReadArgs {
   unsigned int* status;
 };
 
-// One CTA per token of a step, as append has them; head_dim / 8 lanes hold a row.
+// A warp per token of a step, tokens as append has them; head_dim / 8 lanes hold a row, and as many rows as fit the warp are
+// taken at once, four times over before the first is stored.  (A CTA per token, 8160 tokens of 2 x 8 heads of 128 from 4 bits: 20 us,
+// most of it the search for the sequence.)
+constexpr int kReadWarps = 4, kReadAhead = 4;
 template <typename T, int BITS>
-__global__ __launch_bounds__(128) void read_kernel(const ReadArgs a) {
+__global__ __launch_bounds__(kReadWarps * 32) void read_kernel(const ReadArgs a) {
   chain_wait();
   chain_release();
-  const int token = blockIdx.x, lanes = a.head_dim >> 3;
-  const int lane = threadIdx.x & (lanes - 1), slot = threadIdx.x / lanes, slots = 128 / lanes;
+  const int token = blockIdx.x * kReadWarps + (threadIdx.x >> 5);
+  if (token >= a.step.tokens) return;
+  const int lanes = a.head_dim >> 3, lane = threadIdx.x & (lanes - 1), slot = (threadIdx.x & 31) / lanes, slots = 32 / lanes;
   int s = token;
   if (a.step.offsets != nullptr) {
     s = 0;
-    for (int i = 0; i < a.step.batch; i += 128)
-      s += __syncthreads_count(i + int(threadIdx.x) < a.step.batch && __ldg(a.step.offsets + i + threadIdx.x + 1) <= token);
+    for (int i = 0; i < a.step.batch; i += 32) {
+      const int at = i + int(threadIdx.x & 31);
+      const unsigned int in_front = __ballot_sync(0xffffffffu, at < a.step.batch && __ldg(a.step.offsets + at + 1) <= token);
+      s += __popc(in_front);
+      if (in_front != 0xffffffffu) break;
+    }
   }
   int64_t page = -1;
   int place = -1;
@@ -569,51 +608,74 @@ __global__ __launch_bounds__(128) void read_kernel(const ReadArgs a) {
       if ((place >> a.step.page_shift) < a.step.width) page = __ldg(a.step.table + int64_t(s) * a.step.width + (place >> a.step.page_shift));
       if (page < 0 || page >= a.pages) {
         page = -1;
-        if (threadIdx.x == 0) atomicCAS(a.status, 0u, unsigned(s) + 1u);
+        if ((threadIdx.x & 31) == 0) atomicCAS(a.status, 0u, unsigned(s) + 1u);
       }
     }
   }
-  const int in_page = place & ((1 << a.step.page_shift) - 1);
-#pragma unroll 4
-  for (int r = slot; r < 2 * a.kv_heads; r += slots) {
-    const bool is_key = r < a.kv_heads;
-    const int h = is_key ? r : r - a.kv_heads;
-    T* out = (is_key ? static_cast<T*>(a.k) + token * a.kn + h * a.kh : static_cast<T*>(a.v) + token * a.vn + h * a.vh) + lane * 8;
-    uint4 raw = make_uint4(0, 0, 0, 0);
-    if (page >= 0) {
-      const int64_t row = ((page * a.kv_heads + h) << a.step.page_shift) + in_page;
+  const int in_page = place & ((1 << a.step.page_shift) - 1), groups = lanes >> 1, rows = 2 * a.kv_heads;
+  struct Row {
+    uint4 raw;          // as stored
+    uint32_t exponent;  // of a token in 4 bits
+    float scale;        // of a token in 8; the group's bits in 4
+  };
+  for (int r0 = slot; r0 < rows; r0 += slots * kReadAhead) {
+    Row row[kReadAhead];
+#pragma unroll
+    for (int j = 0; j < kReadAhead; ++j) {
+      const int r = r0 + j * slots;
+      row[j].raw = make_uint4(0, 0, 0, 0);
+      row[j].exponent = 0;
+      row[j].scale = 0.f;
+      if (r >= rows || page < 0) continue;
+      const bool is_key = r < a.kv_heads;
+      const int64_t of_head = page * a.kv_heads + (is_key ? r : r - a.kv_heads), at = (of_head << a.step.page_shift) + in_page;
       const void* pool = is_key ? a.keys : a.values;
       const float* scales = is_key ? a.key_scales : a.value_scales;
       if (BITS == 16) {
-        raw = reinterpret_cast<const uint4*>(pool)[row * lanes + lane];
+        row[j].raw = __ldg(reinterpret_cast<const uint4*>(pool) + at * lanes + lane);
+      } else if (BITS == 8) {
+        const uint2 w = __ldg(reinterpret_cast<const uint2*>(pool) + at * lanes + lane);
+        row[j].raw.x = w.x;
+        row[j].raw.y = w.y;
+        row[j].scale = __ldg(scales + at);
       } else {
-        float x[8], scale;
-        if (BITS == 8) {
-          const uint2 w = reinterpret_cast<const uint2*>(pool)[row * lanes + lane];
-          scale = __ldg(scales + row);
+        row[j].raw.x = __ldg(reinterpret_cast<const uint32_t*>(pool) + at * lanes + lane);
+        const uint8_t* of = reinterpret_cast<const uint8_t*>(scales) + ((of_head * (1 + groups)) << a.step.page_shift);
+        row[j].exponent = __ldg(of + in_page);
+        row[j].raw.y = __ldg(of + (1 << a.step.page_shift) + in_page * groups + (lane >> 1));
+      }
+    }
 #pragma unroll
-          for (int i = 0; i < 8; ++i) x[i] = float(int8_t((i < 4 ? w.x : w.y) >> (8 * (i & 3))));
+    for (int j = 0; j < kReadAhead; ++j) {
+      const int r = r0 + j * slots;
+      if (r >= rows) break;
+      const bool is_key = r < a.kv_heads;
+      const int h = is_key ? r : r - a.kv_heads;
+      T* out = (is_key ? static_cast<T*>(a.k) + token * a.kn + h * a.kh : static_cast<T*>(a.v) + token * a.vn + h * a.vh) + lane * 8;
+      uint4 raw = row[j].raw;
+      if (BITS < 16) {
+        float x[8];
+        if (BITS == 8) {
+#pragma unroll
+          for (int i = 0; i < 8; ++i) x[i] = float(int8_t((i < 4 ? raw.x : raw.y) >> (8 * (i & 3)))) * row[j].scale;
         } else {
-          const uint32_t w = reinterpret_cast<const uint32_t*>(pool)[row * lanes + lane];
-          const int groups = lanes >> 1;
-          const uint8_t* of = reinterpret_cast<const uint8_t*>(scales) + (((page * a.kv_heads + h) * (1 + groups)) << a.step.page_shift);
-          const GroupScale<__half> group(twice(__ldg(of + (1 << a.step.page_shift) + in_page * groups + (lane >> 1))));
-          scale = power_of(__ldg(of + in_page)) * kGroupUnit;
+          const float scale = power_of(row[j].exponent) * kGroupUnit;
           uint32_t pairs[4];
-          scaled_codes(w, group, pairs);
+          scaled_codes(raw.x, GroupScale<__half>(twice(raw.y)), pairs);
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const float2 f = Half2<__half>::unpack(pairs[i]);
-            x[2 * i] = f.x;
-            x[2 * i + 1] = f.y;
+            x[2 * i] = f.x * scale;
+            x[2 * i + 1] = f.y * scale;
           }
-        }
+          if (page < 0)
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] *= scale;
+            for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        }
         store8(reinterpret_cast<T*>(&raw), x);
       }
+      *reinterpret_cast<uint4*>(out) = raw;
     }
-    *reinterpret_cast<uint4*>(out) = raw;
   }
 }
 
@@ -995,7 +1057,7 @@ extern "C" int risa_b200_cache_read(const risa_b200_cache* cache, const risa_b20
                    ks[0], ks[1], vs[0], vs[1], cache->pages, cache->kv_heads, cache->head_dim, status};
   const auto kernel = dtype_code == 1 ? (bits == 4 ? read_kernel<__half, 4> : bits == 8 ? read_kernel<__half, 8> : read_kernel<__half, 16>)
                                       : (bits == 4 ? read_kernel<__nv_bfloat16, 4> : bits == 8 ? read_kernel<__nv_bfloat16, 8> : read_kernel<__nv_bfloat16, 16>);
-  return launched(launch_chained(kernel, dim3(step->tokens), dim3(128), 0, static_cast<cudaStream_t>(stream_ptr), a), "read");
+  return launched(launch_chained(kernel, dim3((step->tokens + kReadWarps - 1) / kReadWarps), dim3(kReadWarps * 32), 0, static_cast<cudaStream_t>(stream_ptr), a), "read");
 }
 
 extern "C" int risa_b200_cache_evict(const risa_b200_cache* cache, const risa_b200_step* step,
