@@ -193,7 +193,7 @@ int risa_b200_resize_sequences(const risa_b200_cache* cache, int32_t* references
  * pages are of the same kind; table: the step's page table for that pool (-1 behind the lengths),
  * target_references its counts, used[0] the number of pages in use.  Pages that the target has no room for are
  * not copied, and their entries become -1. */
-size_t risa_b200_compact_scratch_size(const risa_b200_cache* cache);
+size_t risa_b200_compact_scratch_size(const risa_b200_cache* cache, const risa_b200_cache* target);
 int risa_b200_cache_compact(const risa_b200_cache* cache, const int32_t* references,
                             const risa_b200_step* step, const risa_b200_cache* target,
                             int32_t* table, int32_t* target_references, int32_t* used,

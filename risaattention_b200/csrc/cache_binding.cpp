@@ -538,7 +538,7 @@ py::tuple cache_compact(const at::Tensor& cache_keys, const at::Tensor& cache_va
   require_cuda(cache_keys);
   const c10::DeviceGuard on_device(cache_keys.device());
   const at::Tensor new_table = at::empty_like(table), counts = at::empty({target.c.pages}, table.options()), used = at::empty({1}, table.options());
-  const size_t bytes = risa_b200_compact_scratch_size(&cache.c);
+  const size_t bytes = risa_b200_compact_scratch_size(&cache.c, &target.c);
   const at::Tensor scratch = at::empty({int64_t(bytes)}, table.options().dtype(at::kByte));
   check(risa_b200_cache_compact(&cache.c, references.data_ptr<int32_t>(), &step.s, &target.c, new_table.data_ptr<int32_t>(),
                                 counts.data_ptr<int32_t>(), used.data_ptr<int32_t>(), scratch.data_ptr(), bytes, stream_of(stream_ptr)));

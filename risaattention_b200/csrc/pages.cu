@@ -102,10 +102,7 @@ __device__ __forceinline__ Change change_of(const ResizeArgs& a, int s) {
 
 // One CTA: what each sequence needs, added up in order; then free pages, lowest first, until there are enough (16 K a round); then
 // what each sequence is granted.
-__global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(const ResizeArgs a) {
-  __shared__ int warp_sums[32];
-  chain_wait();
-  chain_release();
+__device__ __forceinline__ void plan_resize(const ResizeArgs& a, int* warp_sums) {
   int needed = 0;
   for (int s0 = 0; s0 < a.batch; s0 += kPlanThreads) {
     const int s = s0 + threadIdx.x;
@@ -152,24 +149,22 @@ __global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(const ResizeA
   }
 }
 
-// Grid (sequence, part): part 0 writes entries and counts, all parts copy the rows of a page that was shared.
-__global__ __launch_bounds__(256) void resize_apply_kernel(const ResizeArgs a) {
-  chain_wait();
-  chain_release();
-  const int s = blockIdx.x, part = blockIdx.y, parts = gridDim.y;
+// Part 0 of a sequence's CTAs writes entries and counts, all parts copy the rows of a page that was shared.
+__device__ __forceinline__ void apply_resize(const ResizeArgs& a, int s, int part, int parts) {
+  const int threads = blockDim.x;
   Change c = change_of(a, s);
   c.shared = a.left[s];
   const int found = a.counts[0], before = a.before[s], given = max(min(found - before, c.need()), 0);
   const bool copies = c.shared >= 0 && given > 0;
   int32_t* row = a.table + int64_t(s) * a.width;
   if (part == 0) {
-    for (int i = threadIdx.x; i < given; i += 256) {
+    for (int i = threadIdx.x; i < given; i += threads) {
       const int page = a.fresh[before + i], column = copies ? c.held - 1 + i : c.held + i;
       a.references[page] = 1;
       row[column] = page;
     }
     if (copies && threadIdx.x == 0) atomicAdd(a.references + c.shared, -1);
-    for (int i = c.needed + threadIdx.x; i < c.held; i += 256) {  // given back
+    for (int i = c.needed + threadIdx.x; i < c.held; i += threads) {  // given back
       const int page = row[i];
       if (page >= 0 && page < a.pages) atomicAdd(a.references + page, -1);
       else atomicCAS(a.status, 0u, unsigned(s) + 1u);
@@ -179,7 +174,7 @@ __global__ __launch_bounds__(256) void resize_apply_kernel(const ResizeArgs a) {
   if (!copies) return;
   const int64_t from = int64_t(c.shared) * a.kv_heads, to = int64_t(a.fresh[before]) * a.kv_heads;
   const int rows = c.length & ((1 << a.page_shift) - 1), pieces = a.row_bytes >> 4, each = rows * pieces;  // of a head
-  for (int i = part * 256 + threadIdx.x; i < a.kv_heads * each; i += parts * 256) {
+  for (int i = part * threads + threadIdx.x; i < a.kv_heads * each; i += parts * threads) {
     const int h = i / each;
     const int64_t in_head = int64_t(i - h * each) * 16, head_bytes = int64_t(a.row_bytes) << a.page_shift;
     const uint4 k = *reinterpret_cast<const uint4*>(a.keys + (from + h) * head_bytes + in_head);
@@ -191,7 +186,7 @@ __global__ __launch_bounds__(256) void resize_apply_kernel(const ResizeArgs a) {
   // scales byte by byte: of the tokens, then (behind those of all the page's tokens) of their groups
   const int64_t block = int64_t(a.token_scales + a.group_scales) << a.page_shift;
   const int of_tokens = rows * a.token_scales, of_head = of_tokens + rows * a.group_scales;
-  for (int i = part * 256 + threadIdx.x; i < a.kv_heads * of_head; i += parts * 256) {
+  for (int i = part * threads + threadIdx.x; i < a.kv_heads * of_head; i += parts * threads) {
     const int h = i / of_head, j = i - h * of_head;
     const int64_t at = j < of_tokens ? j : (int64_t(a.token_scales) << a.page_shift) + j - of_tokens;
     a.key_scales[(to + h) * block + at] = a.key_scales[(from + h) * block + at];
@@ -199,11 +194,35 @@ __global__ __launch_bounds__(256) void resize_apply_kernel(const ResizeArgs a) {
   }
 }
 
+__global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(const ResizeArgs a) {
+  __shared__ int warp_sums[32];
+  chain_wait();
+  chain_release();
+  plan_resize(a, warp_sums);
+}
+__global__ __launch_bounds__(256) void resize_apply_kernel(const ResizeArgs a) {
+  chain_wait();
+  chain_release();
+  apply_resize(a, blockIdx.x, blockIdx.y, gridDim.y);
+}
+// Both in one launch where there is little to copy: a cluster of eight CTAs, of which the first one plans.
+constexpr int kResizeCtas = 8;
+constexpr int64_t kLittle = 4 << 20;  // bytes that all sequences together can have copied
+__global__ __cluster_dims__(kResizeCtas, 1, 1) __launch_bounds__(kPlanThreads) void resize_kernel(const ResizeArgs a) {
+  __shared__ int warp_sums[32];
+  chain_wait();
+  chain_release();
+  if (blockIdx.x == 0) plan_resize(a, warp_sums);
+  asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+  for (int s = blockIdx.x; s < a.batch; s += kResizeCtas) apply_resize(a, s, 0, 1);
+}
+
 // ---- compact ------------------------------------------------------------------------------------------------
 struct CompactArgs {
   StepView step;
   const int32_t* references;
-  int32_t* place;  // of each page in the target, -1: nowhere
+  int32_t* place;   // of each page in the target, -1: nowhere
+  int32_t* source;  // the page that goes to each place, -1: none
   int32_t* table;
   int32_t* target_references;
   int32_t* used;
@@ -212,6 +231,7 @@ struct CompactArgs {
   char* to[4];
   int units[2];         // of a page: 16-byte pieces of rows, 4-byte pieces of scales
   int pages_each;       // pages that a copying CTA takes where they are small
+  unsigned int parts[2], copies[2];  // CTAs of such a group of pages, CTAs in all, of rows and of scales
   unsigned int* status;
 };
 
@@ -236,22 +256,31 @@ __global__ __launch_bounds__(kPlanThreads) void compact_plan_kernel(const Compac
   for (int i = 0; i < kPlanEach && first + i < a.pages; ++i) {
     const bool moves = (in_use >> i & 1) && rank < a.target_pages;
     a.place[first + i] = moves ? rank : -1;
-    if (moves) a.target_references[rank] = __ldg(a.references + first + i);
+    if (moves) {
+      a.source[rank] = first + i;
+      a.target_references[rank] = __ldg(a.references + first + i);
+    }
     rank += in_use >> i & 1;
   }
   if (blockIdx.x == gridDim.x - 1) {
     if (threadIdx.x == 0) *a.used = base + total;
-    for (int p = base + total + threadIdx.x; p < a.target_pages; p += kPlanThreads) a.target_references[p] = 0;
+    for (int p = base + total + threadIdx.x; p < a.target_pages; p += kPlanThreads) {
+      a.source[p] = -1;
+      a.target_references[p] = 0;
+    }
   }
 }
 
-// Grid z: 0 copies rows, 1 scales, the last one rewrites the tables.  Eight loads of a thread are on their way at once.
+// CTAs that copy rows to places of the target, then those that copy scales, then those that rewrite the tables.  Eight loads of a
+// thread are on their way at once.  (CTAs of pages that stand empty, and as many for the tables as for rows: 32 requests in half
+// of a pool, 671 MB, 256 us.)
 constexpr int kCopyAhead = 4;
 template <typename V>
-__device__ __forceinline__ void copy_pages(const CompactArgs& a, int kind) {
+__device__ __forceinline__ void copy_pages(const CompactArgs& a, int kind, unsigned int block) {
   const int units = a.units[kind];
-  const int64_t page0 = int64_t(blockIdx.x) * a.pages_each;
-  // units of the pages [page0, page0 + pages_each), 256 * kCopyAhead of them for each y
+  const unsigned int group = block / a.parts[kind], part = block - group * a.parts[kind];
+  const int64_t place0 = int64_t(group) * a.pages_each;
+  // units of the places [place0, place0 + pages_each), 256 * kCopyAhead of them for each part
   const V* from_k = reinterpret_cast<const V*>(a.from[2 * kind]);
   const V* from_v = reinterpret_cast<const V*>(a.from[2 * kind + 1]);
   V* to_k = reinterpret_cast<V*>(a.to[2 * kind]);
@@ -260,14 +289,14 @@ __device__ __forceinline__ void copy_pages(const CompactArgs& a, int kind) {
   int64_t to[kCopyAhead];
 #pragma unroll
   for (int i = 0; i < kCopyAhead; ++i) {
-    const int64_t u = (int64_t(blockIdx.y) * kCopyAhead + i) * 256 + threadIdx.x;
+    const int64_t u = (int64_t(part) * kCopyAhead + i) * 256 + threadIdx.x;
     to[i] = -1;
-    const int64_t in_group = a.pages_each == 1 ? 0 : u / units, page = page0 + in_group;
+    const int64_t in_group = a.pages_each == 1 ? 0 : u / units, place = place0 + in_group;
     const int64_t in_page = u - in_group * units;
-    if (in_group < a.pages_each && in_page < units && page < a.pages) {
-      const int place = __ldg(a.place + page);
-      if (place >= 0) {
-        to[i] = int64_t(place) * units + in_page;
+    if (in_group < a.pages_each && in_page < units && place < a.target_pages) {
+      const int64_t page = __ldg(a.source + place);
+      if (page >= 0) {
+        to[i] = place * units + in_page;
         k[i] = __ldg(from_k + page * units + in_page);
         v[i] = __ldg(from_v + page * units + in_page);
       }
@@ -283,13 +312,11 @@ __device__ __forceinline__ void copy_pages(const CompactArgs& a, int kind) {
 __global__ __launch_bounds__(256) void compact_copy_kernel(const CompactArgs a) {
   chain_wait();
   chain_release();
-  if (blockIdx.z + 1 < gridDim.z) {
-    if (blockIdx.z == 0) copy_pages<uint4>(a, 0);
-    else copy_pages<uint32_t>(a, 1);
-    return;
-  }
-  const int64_t entries = int64_t(a.step.batch) * a.step.width, threads = int64_t(gridDim.x) * gridDim.y * 256;
-  for (int64_t i = (int64_t(blockIdx.y) * gridDim.x + blockIdx.x) * 256 + threadIdx.x; i < entries; i += threads) {
+  if (blockIdx.x < a.copies[0]) return copy_pages<uint4>(a, 0, blockIdx.x);
+  const unsigned int behind = blockIdx.x - a.copies[0];
+  if (behind < a.copies[1]) return copy_pages<uint32_t>(a, 1, behind);
+  const int64_t entries = int64_t(a.step.batch) * a.step.width, threads = int64_t(gridDim.x - a.copies[0] - a.copies[1]) * 256;
+  for (int64_t i = int64_t(behind - a.copies[1]) * 256 + threadIdx.x; i < entries; i += threads) {
     const int s = int(i / a.step.width), column = int(i - int64_t(s) * a.step.width);
     const int length = min(max(__ldg(a.step.lengths + s), 0), a.step.width << a.step.page_shift);
     int place = -1;
@@ -362,6 +389,8 @@ extern "C" int risa_b200_resize_sequences(const risa_b200_cache* cache, int32_t*
                      static_cast<char*>(cache->keys), static_cast<char*>(cache->values), reinterpret_cast<char*>(cache->key_scales),
                      reinterpret_cast<char*>(cache->value_scales), cache->kv_heads, row_bytes, token_scale_of(*cache), group_scales_of(*cache), status};
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
+  if (2 * int64_t(batch) * cache->kv_heads * cache->page_size * row_bytes <= kLittle)
+    return launched(launch_chained(resize_kernel, dim3(kResizeCtas), dim3(kPlanThreads), 0, stream, a), "resize");
   if (const int bad = launched(launch_chained(resize_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a), "resize")) return bad;
   // parts: 16 bytes of keys and values for each thread in turn, as many as fill the SMs and as a page has work for
   const int64_t work = (int64_t(cache->kv_heads) * cache->page_size * row_bytes / 16 + 255) / 256;
@@ -369,8 +398,9 @@ extern "C" int risa_b200_resize_sequences(const risa_b200_cache* cache, int32_t*
   return launched(launch_chained(resize_apply_kernel, dim3(batch, parts), dim3(256), 0, stream, a), "resize");
 }
 
-extern "C" size_t risa_b200_compact_scratch_size(const risa_b200_cache* cache) {
-  return cache == nullptr ? 0 : sizeof(int32_t) * size_t(std::max(cache->pages, 0));
+extern "C" size_t risa_b200_compact_scratch_size(const risa_b200_cache* cache, const risa_b200_cache* target) {
+  if (cache == nullptr || target == nullptr) return 0;
+  return sizeof(int32_t) * (size_t(std::max(cache->pages, 0)) + size_t(std::max(target->pages, 0)));
 }
 
 extern "C" int risa_b200_cache_compact(const risa_b200_cache* cache, const int32_t* references, const risa_b200_step* step, const risa_b200_cache* target,
@@ -383,27 +413,28 @@ extern "C" int risa_b200_cache_compact(const risa_b200_cache* cache, const int32
   RISA_REQUIRE(cache->kv_heads == target->kv_heads && cache->page_size == target->page_size && cache->head_dim == target->head_dim &&
                    cache->dtype_code == target->dtype_code, "compact: both caches must have pages of the same kind");
   RISA_REQUIRE(cache->keys != target->keys && cache->values != target->values, "compact: the target must be another pool");
-  RISA_REQUIRE(scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 4 == 0 && scratch_bytes >= risa_b200_compact_scratch_size(cache),
+  RISA_REQUIRE(scratch != nullptr && reinterpret_cast<uintptr_t>(scratch) % 4 == 0 && scratch_bytes >= risa_b200_compact_scratch_size(cache, target),
                "compact: the scratch is too small");
   const int64_t rows = int64_t(cache->kv_heads) * cache->page_size;
   const int64_t row_units = rows * cache->head_dim * bits_of(*cache) / 8 / 16, scale_units = rows * (token_scale_of(*cache) + group_scales_of(*cache)) / 4;
-  RISA_REQUIRE(std::max(row_units, scale_units) < int64_t(65535) * 256 * kCopyAhead, "compact: a page is too large");
+  const int per_plan = kPlanThreads * kPlanEach, per_copy = 256 * kCopyAhead;
+  const int64_t pages_each = std::max<int64_t>(1, per_copy / std::max(row_units, scale_units)), groups = (target->pages + pages_each - 1) / pages_each;
+  const int64_t row_parts = (row_units * pages_each + per_copy - 1) / per_copy, scale_parts = (scale_units * pages_each + per_copy - 1) / per_copy;
+  const int64_t table_blocks = std::min<int64_t>((int64_t(step->batch) * step->table_width + 2047) / 2048, 1024);
+  RISA_REQUIRE(std::max(row_units, scale_units) < (int64_t(1) << 31) && groups * (row_parts + scale_parts) + table_blocks < (int64_t(1) << 31),
+               "compact: the target has too many pages, or too large ones");
   unsigned int* status = status_word();
   if (status == nullptr) return RISA_B200_CUDA;
-  CompactArgs a{{step->page_table, step->lengths, nullptr, step->batch, step->table_width, 0, shift_of(cache->page_size)},
-                references, static_cast<int32_t*>(scratch), table, target_references, used, cache->pages, target->pages,
+  const CompactArgs a{{step->page_table, step->lengths, nullptr, step->batch, step->table_width, 0, shift_of(cache->page_size)},
+                references, static_cast<int32_t*>(scratch), static_cast<int32_t*>(scratch) + cache->pages, table, target_references, used, cache->pages, target->pages,
                 {static_cast<const char*>(cache->keys), static_cast<const char*>(cache->values), reinterpret_cast<const char*>(cache->key_scales),
                  reinterpret_cast<const char*>(cache->value_scales)},
                 {static_cast<char*>(target->keys), static_cast<char*>(target->values), reinterpret_cast<char*>(target->key_scales),
                  reinterpret_cast<char*>(target->value_scales)},
-                {int(row_units), int(scale_units)}, 1, status};
+                {int(row_units), int(scale_units)}, int(pages_each), {unsigned(row_parts), unsigned(std::max<int64_t>(scale_parts, 1))},
+                {unsigned(groups * row_parts), unsigned(groups * scale_parts)}, status};
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  const int per_plan = kPlanThreads * kPlanEach, per_copy = 256 * kCopyAhead;
   if (const int bad = launched(launch_chained(compact_plan_kernel, dim3((cache->pages + per_plan - 1) / per_plan), dim3(kPlanThreads), 0, stream, a), "compact"))
     return bad;
-  const int64_t units = std::max(row_units, scale_units);
-  a.pages_each = int(std::max<int64_t>(1, per_copy / units));
-  const dim3 grid(unsigned((cache->pages + a.pages_each - 1) / a.pages_each), unsigned((units * a.pages_each + per_copy - 1) / per_copy),
-                  scale_units > 0 ? 3 : 2);
-  return launched(launch_chained(compact_copy_kernel, grid, dim3(256), 0, stream, a), "compact");
+  return launched(launch_chained(compact_copy_kernel, dim3(unsigned(a.copies[0] + a.copies[1] + table_blocks)), dim3(256), 0, stream, a), "compact");
 }
