@@ -289,32 +289,26 @@ __device__ __forceinline__ uint32_t code_bits(int code, int channel) { return ui
 
 // Group scale: the largest value of the group over 7 token scales, rounded to e4m3.  Code: the value over both scales, rounded
 // to nearest even.  Values of 16 bits meet the borders between codes (and between scales) exactly or not nearly, so that
-// for rows as they came this is decided in 32 bits: a quotient near a border of scales is divided correctly, and a value's
-// quotient, corrected by its remainder, is exact where it is half of a whole number.  Rotated values are off by 2^-21 of
+// for rows as they came this is decided in 32 bits: quotients corrected by their remainders are exact where they meet one.  Rotated values are off by 2^-21 of
 // the row's largest value at most (cosine and sine 2^-22.8 each, of a pair whose length is sqrt(2) times that at most); `doubtful`
 // says that one of them lies within twice that of a border.
-__device__ __forceinline__ Row4 row4_of(const float (&x)[8], int lanes, bool& doubtful) {
-  Row4 r;
+template <int LANES, bool ROTATED>
+__device__ __forceinline__ Row4 row4_of(const float (&x)[8], bool& doubtful) {
   float group = fabsf(x[0]);
 #pragma unroll
   for (int i = 1; i < 8; ++i) asm("max.NaN.f32 %0, %0, %1;" : "+f"(group) : "f"(fabsf(x[i])));
   asm("max.NaN.f32 %0, %0, %1;" : "+f"(group) : "f"(__shfl_xor_sync(0xffffffffu, group, 1)));
   float most = group;
-  for (int off = lanes >> 1; off > 1; off >>= 1)
+#pragma unroll
+  for (int off = LANES / 2; off > 1; off >>= 1)
     asm("max.NaN.f32 %0, %0, %1;" : "+f"(most) : "f"(__shfl_xor_sync(0xffffffffu, most, off)));
   const uint32_t bits = __float_as_uint(most) + kAbove3136;
-  r.exponent = most == 0.f ? 0 : !(most < INFINITY) ? 255 : max(int(bits >> 23) - 11, 1);
-  r.word = 0x88888888u;
-  r.group = 0;
-  doubtful = false;
-  if (r.exponent == 0 || r.exponent == 255) return r;
-  const float to_units = __uint_as_float(uint32_t(254 - r.exponent) << 23), slack = most * to_units * 0x1p-20f;
-  float ratio = group * to_units;
-  uint32_t around = e4m3_pair(fmaf(ratio, 1.0f / 7.0f, slack), fmaxf(fmaf(ratio, 1.0f / 7.0f, -slack), 0.f));
-  doubtful = (around & 0xffu) != around >> 8 || (bits - 16) >> 23 != (bits + 16) >> 23;
-  if ((around & 0xffu) != around >> 8) around = e4m3_pair(0.f, __fdiv_rn(ratio, 7.0f));
-  r.group = around & 0xffu;
-  if (r.group == 0) return r;
+  const bool usable = most > 0.f && most < INFINITY;
+  Row4 r;
+  r.exponent = usable ? max(int(bits >> 23) - 11, 1) : most == 0.f ? 0 : 255;
+  const float to_units = __uint_as_float(uint32_t(254 - r.exponent) << 23), size = group * to_units, third = size * (1.0f / 7.0f);
+  const float ratio = fmaf(fmaf(-third, 7.0f, size), 1.0f / 7.0f, third);  // exact where a border of scales is met
+  r.group = e4m3_pair(0.f, ratio) & 0xffu;
   const float scale = __half2float(__ushort_as_half(uint16_t(r.group << 7))) * kGroupUnit;
   float inverse;
   asm("rcp.approx.f32 %0, %1;" : "=f"(inverse) : "f"(scale));
@@ -324,17 +318,22 @@ __device__ __forceinline__ Row4 row4_of(const float (&x)[8], int lanes, bool& do
     const float y = x[i] * to_units, guess = y * inverse;
     const float quotient = fmaf(fmaf(-guess, scale, y), inverse, guess);  // exact where it is half of a whole number
     code[i] = (quotient + 12582912.0f) - 12582912.0f;
-    nearest = fminf(nearest, fabsf(fabsf(quotient - code[i]) - 0.5f));
+    if (ROTATED) nearest = fminf(nearest, fabsf(fabsf(quotient - code[i]) - 0.5f));
   }
-  doubtful = doubtful || nearest * scale < slack;
-  if (r.group < 8) {  // scales below 2^-6 are rounded coarsely: quotients past 7
+  if (ROTATED) {
+    const float slack = most * to_units * 0x1p-20f;
+    const uint32_t around = e4m3_pair(ratio + slack, fmaxf(ratio - slack, 0.f));
+    doubtful = usable && (nearest * scale < slack || (around & 0xffu) != around >> 8 || (bits - 16) >> 23 != (bits + 16) >> 23);
+  }
+  if (__any_sync(0xffffffffu, r.group < 8)) {  // scales below 2^-6 are rounded coarsely: quotients past 7
 #pragma unroll
     for (int i = 0; i < 8; ++i) code[i] = fminf(fmaxf(code[i], -7.f), 7.f);
   }
   float half_words[2] = {8388608.0f + 0x8888, 8388608.0f + 0x8888};  // four codes + 8 in the low bits
 #pragma unroll
   for (int i = 0; i < 8; ++i) half_words[i & 1] = fmaf(code[i], float(1 << (4 * (i >> 1))), half_words[i & 1]);
-  r.word = __byte_perm(__float_as_uint(half_words[0]), __float_as_uint(half_words[1]), 0x5410);
+  r.word = usable && r.group != 0 ? __byte_perm(__float_as_uint(half_words[0]), __float_as_uint(half_words[1]), 0x5410) : 0x88888888u;
+  r.group = usable ? r.group : 0;
   return r;
 }
 // The same for a rotated row that came too near a border, in 64 bits: from the channels as they came (`own`, and `other` of a
@@ -344,6 +343,7 @@ __device__ __noinline__ Row4 row4_of_rotated(const AppendArgs& a, Run<T> own, Ru
   float u[8], v[8];
   own.values(u);
   other.values(v);
+  auto larger = [](double m, double x) { return x > m || x != x ? x : m; };
   double x[8], most = 0.0;
   const int half = a.rotary_dim >> 1;
 #pragma unroll 1
@@ -361,14 +361,14 @@ __device__ __noinline__ Row4 row4_of_rotated(const AppendArgs& a, Run<T> own, Ru
       const double partner = a.interleaved ? u[i ^ 1] : v[i];
       x[i] = double(a.magnitude) * (u[i] * cosine + (second ? partner : -partner) * sine);
     }
-    most = fmax(most, fabs(x[i]));
+    most = larger(most, fabs(x[i]));
   }
-  const double group = fmax(most, __shfl_xor_sync(0xffffffffu, most, 1));
+  const double group = larger(most, __shfl_xor_sync(0xffffffffu, most, 1));
   most = group;
-  for (int off = lanes >> 1; off > 1; off >>= 1) most = fmax(most, __shfl_xor_sync(0xffffffffu, most, off));
+  for (int off = lanes >> 1; off > 1; off >>= 1) most = larger(most, __shfl_xor_sync(0xffffffffu, most, off));
   Row4 r{0x88888888u, 0, 0};
   if (most == 0.0) return r;
-  r.exponent = 255;  // not finite (fmax passes over a NaN, whose row the other form has stored)
+  r.exponent = 255;  // not finite
   if (!(most < double(INFINITY))) return r;
   r.exponent = max(int((__double_as_longlong(most) + (0xfffffffffffffll - 0x8800000000000ll)) >> 52) - 1023 - 11 + 127, 1);
   const double to_units = __longlong_as_double(int64_t(1023 + 127 - r.exponent) << 52), ratio = group * to_units / 7.0;
@@ -383,15 +383,6 @@ __device__ __noinline__ Row4 row4_of_rotated(const AppendArgs& a, Run<T> own, Ru
   return r;
 }
 
-__device__ __forceinline__ void store_row4(const AppendArgs& a, bool key, const Row4& r, int64_t page, int h, int slot_in_page, int lanes, int lane) {
-  const int64_t of_head = page * a.kv_heads + h;
-  const int groups = lanes >> 1;
-  reinterpret_cast<uint32_t*>(key ? a.keys : a.values)[((of_head << a.step.page_shift) + slot_in_page) * lanes + lane] = r.word;
-  uint8_t* scales = reinterpret_cast<uint8_t*>(key ? a.key_scales : a.value_scales) + ((of_head * (1 + groups)) << a.step.page_shift);
-  if (lane == 0) scales[slot_in_page] = uint8_t(r.exponent);
-  if ((lane & 1) == 0) scales[(1 << a.step.page_shift) + slot_in_page * groups + (lane >> 1)] = uint8_t(r.group);
-}
-
 // One CTA per new token.  head_dim / 8 lanes hold a row, eight channels each; the CTA's row slots walk
 // the token's query heads, key heads and value heads with the cosines and sines of the lane's channels
 // kept in registers.  A thread computes those of one pair for the whole token (8160 tokens below: 70 us where every lane
@@ -403,7 +394,7 @@ __device__ __forceinline__ void store_row4(const AppendArgs& a, bool key, const 
 // requests, with the call: 11.5 to 12.4 us.
 constexpr int kRowsAhead = 3;  // rows of a slot on their way at once: half of a token of 32 + 2 x 8 heads of 128
 template <typename T, int BITS>
-__global__ __launch_bounds__(128, BITS == 4 ? 6 : 8) void append_kernel(const AppendArgs a) {
+__global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
   __shared__ __align__(16) float cosines[128], sines[128];
   chain_wait();
   chain_release();
@@ -483,7 +474,6 @@ __global__ __launch_bounds__(128, BITS == 4 ? 6 : 8) void append_kernel(const Ap
     }
   }
   const int slot_in_page = place & ((1 << a.step.page_shift) - 1);
-  uint32_t again = 0;  // 4 bits: passes (modulo 32) of this warp whose keys came too near a border
   for (int r0 = 0; r0 < rows; r0 += slots * kRowsAhead) {
     if (r0 > 0) load_rows(r0);
 #pragma unroll
@@ -520,12 +510,6 @@ __global__ __launch_bounds__(128, BITS == 4 ? 6 : 8) void append_kernel(const Ap
         }
       }
       const int64_t row = ((page * a.kv_heads + h) << a.step.page_shift) + slot_in_page;
-      if (BITS == 4 && __any_sync(0xffffffffu, kind > 0)) {
-        bool doubtful;
-        const Row4 r4 = row4_of(x, lanes, doubtful);
-        if (there && kind > 0 && page >= 0) store_row4(a, kind == 1, r4, page, h, slot_in_page, lanes, lane);
-        if (a.turns != nullptr && __any_sync(0xffffffffu, doubtful && there && kind == 1)) again |= 1u << (r0 / slots + j & 31);
-      }
       if (BITS == 8 && __any_sync(0xffffffffu, kind > 0)) {
         const float most = row_absmax(x, lanes), scale = most / 127.0f;
         if (there && kind > 0 && page >= 0) {
@@ -546,23 +530,176 @@ __global__ __launch_bounds__(128, BITS == 4 ? 6 : 8) void append_kernel(const Ap
       if (there && kind == 0) store8(static_cast<T*>(a.q_out) + token * a.on + h * a.oh + channel, x);
     }
   }
-  if (BITS == 4 && again != 0) {
-    // such rows once more, in 64 bits.  (Called from within the passes this cost every row 26 us of 116: registers kept for the call.)
-#pragma unroll 1
-    for (int pass = 0; pass * slots < rows; ++pass) {
-      if (!(again >> (pass & 31) & 1)) continue;
-      const int r = pass * slots + slot, h = r - a.q_heads;
-      const bool is_key = h >= 0 && h < a.kv_heads;
-      Run<T> own, other;
-      own.zero();
-      if (is_key) own.load(static_cast<const T*>(a.k) + token * a.kn + h * a.kh + channel);
-      other.raw.x = __shfl_sync(0xffffffffu, own.raw.x, partner);
-      other.raw.y = __shfl_sync(0xffffffffu, own.raw.y, partner);
-      other.raw.z = __shfl_sync(0xffffffffu, own.raw.z, partner);
-      other.raw.w = __shfl_sync(0xffffffffu, own.raw.w, partner);
-      const Row4 r4 = row4_of_rotated<T>(a, own, other, token, place, lanes, channel);
-      if (is_key && page >= 0 && r4.exponent != 255) store_row4(a, true, r4, page, h, slot_in_page, lanes, lane);
+}
+
+// In 4 bits: a kernel of its own, in which a CTA's row slots walk the token's query heads, then its keys, then its values (what is
+// computed of a row in 4 bits is three times as much as of a rotated one).  8160 tokens of 32 + 2 x 8 heads of 128: 72 us, 87 in
+// the kernel for all kinds of cache, whose every row paid for the registers of the call that decides doubtful ones.
+constexpr int kQueriesAhead = 4;
+template <typename T, int LANES>
+__global__ __launch_bounds__(128, 7) void append4_kernel(const AppendArgs a) {
+  __shared__ __align__(16) float cosines[128], sines[128];
+  chain_wait();
+  chain_release();
+  constexpr int SLOTS = 128 / LANES, GROUPS = LANES / 2;
+  const int token = blockIdx.x, lane = threadIdx.x % LANES, slot = threadIdx.x / LANES, channel = lane * 8;
+  const T* const k0 = static_cast<const T*>(a.k) + token * a.kn + channel;
+  const T* const v0 = static_cast<const T*>(a.v) + token * a.vn + channel;
+  const T* const q0 = static_cast<const T*>(a.q) + token * a.qn + channel;
+  T* const o0 = static_cast<T*>(a.q_out) + token * a.on + channel;
+  // the first rows are on their way before their place is looked up
+  Run<T> q[kQueriesAhead], k, v;
+  auto load_queries = [&](int h0) {
+#pragma unroll
+    for (int j = 0; j < kQueriesAhead; ++j) {
+      const int h = h0 + j * SLOTS + slot;
+      q[j].zero();
+      if (h < a.q_heads) q[j].load(q0 + h * a.qh);
     }
+  };
+  load_queries(0);
+  k.zero();
+  v.zero();
+  if (slot < a.kv_heads) {
+    k.load(k0 + slot * a.kh);
+    v.load(v0 + slot * a.vh);
+  }
+  int s = token;
+  if (a.step.offsets != nullptr) {
+    s = 0;
+    for (int i = 0; i < a.step.batch; i += 128)
+      s += __syncthreads_count(i + int(threadIdx.x) < a.step.batch && __ldg(a.step.offsets + i + threadIdx.x + 1) <= token);
+  }
+  int place = -1;
+  bool belongs = false;
+  if (s < a.step.batch) {
+    const int first = a.step.offsets ? __ldg(a.step.offsets + s) : s;
+    const int end = a.step.offsets ? __ldg(a.step.offsets + s + 1) : s + 1;
+    belongs = token >= first;
+    place = __ldg(a.step.lengths + s) - (end - token);
+  }
+  if (!belongs) {  // a row behind the last sequence
+    for (int h = slot; h < a.q_heads; h += SLOTS) *reinterpret_cast<uint4*>(o0 + h * a.oh) = make_uint4(0, 0, 0, 0);
+    return;
+  }
+  int64_t page = -1;
+  if (place >= 0) {
+    if ((place >> a.step.page_shift) < a.step.width) page = __ldg(a.step.table + int64_t(s) * a.step.width + (place >> a.step.page_shift));
+    if (page < 0 || page >= a.pages) {  // outside the pool, or the sequence is longer than its row of the table
+      page = -1;
+      if (threadIdx.x == 0) atomicCAS(a.status, 0u, unsigned(s) + 1u);
+    }
+  }
+  const bool turns = a.turns != nullptr, turned = turns && channel < a.rotary_dim;
+  float cs[8] = {}, sn[8] = {};
+  int partner = threadIdx.x & 31;
+  if (turns) {  // one thread for each pair of the token, then every lane takes those of its channels
+    const int half = a.rotary_dim >> 1;
+    if (int(threadIdx.x) < half) {
+      const int64_t axis = a.axes != nullptr ? min(int(__ldg(a.axes + threadIdx.x)), a.last_axis) * a.axis_stride : 0;
+      const int64_t position = a.positions ? position_at(a.positions, a.positions_64, token + axis) : int64_t(place);
+      angle_of(position, __ldg(reinterpret_cast<const unsigned long long*>(a.turns) + threadIdx.x), a.magnitude, cosines[threadIdx.x], sines[threadIdx.x]);
+    }
+    __syncthreads();
+    if (turned) {
+      const bool second = !a.interleaved && channel >= half;
+      const int pair0 = a.interleaved ? channel >> 1 : second ? channel - half : channel;
+#pragma unroll
+      for (int i = 0; i < 8; i += 4) {
+        if (a.interleaved && i == 4) break;
+        const float4 c = *reinterpret_cast<const float4*>(cosines + pair0 + i), d = *reinterpret_cast<const float4*>(sines + pair0 + i);
+        cs[i] = c.x; cs[i + 1] = c.y; cs[i + 2] = c.z; cs[i + 3] = c.w;
+        sn[i] = d.x; sn[i + 1] = d.y; sn[i + 2] = d.z; sn[i + 3] = d.w;
+      }
+      if (second)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sn[i] = -sn[i];  // b cos + a sin as b cos - a (-sin)
+      if (!a.interleaved) partner = (threadIdx.x & 31) + (second ? -(half >> 3) : (half >> 3));
+    }
+  }
+  auto partner_of = [&](const Run<T>& run) {
+    Run<T> other;
+    other.raw.x = __shfl_sync(0xffffffffu, run.raw.x, partner);
+    other.raw.y = __shfl_sync(0xffffffffu, run.raw.y, partner);
+    other.raw.z = __shfl_sync(0xffffffffu, run.raw.z, partner);
+    other.raw.w = __shfl_sync(0xffffffffu, run.raw.w, partner);
+    return other;
+  };
+  auto turn = [&](const Run<T>& run, float (&x)[8]) {  // by the whole warp
+    run.values(x);
+    if (a.interleaved) {
+      if (turned) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float p = x[2 * i], q = x[2 * i + 1];
+          x[2 * i] = p * cs[i] - q * sn[i];
+          x[2 * i + 1] = q * cs[i] + p * sn[i];
+        }
+      }
+    } else {
+      float y[8];
+      partner_of(run).values(y);
+      if (turned) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = x[i] * cs[i] - y[i] * sn[i];
+      }
+    }
+  };
+  for (int h0 = 0; h0 < a.q_heads; h0 += SLOTS * kQueriesAhead) {
+    if (h0 > 0) load_queries(h0);
+#pragma unroll
+    for (int j = 0; j < kQueriesAhead; ++j) {
+      if (h0 + j * SLOTS >= a.q_heads) break;  // the same for the whole CTA
+      float x[8];
+      turn(q[j], x);
+      const int h = h0 + j * SLOTS + slot;
+      if (h < a.q_heads) store8(o0 + h * a.oh, x);
+    }
+  }
+  if (page < 0) return;
+  // where this lane's word of head 0 lies, and the scales of the token
+  const int in_page = place & ((1 << a.step.page_shift) - 1);
+  const int64_t of_page = page * a.kv_heads;
+  const int64_t word0 = ((of_page << a.step.page_shift) + in_page) * LANES + lane, scales0 = (of_page * (1 + GROUPS)) << a.step.page_shift;
+  auto store = [&](void* codes, float* scales, int h, const Row4& r) {
+    static_cast<uint32_t*>(codes)[word0 + int64_t(h) * (LANES << a.step.page_shift)] = r.word;
+    uint8_t* of = reinterpret_cast<uint8_t*>(scales) + scales0 + int64_t(h) * ((1 + GROUPS) << a.step.page_shift);
+    if (lane == 0) of[in_page] = uint8_t(r.exponent);
+    if ((lane & 1) == 0) of[(1 << a.step.page_shift) + in_page * GROUPS + (lane >> 1)] = uint8_t(r.group);
+  };
+  uint32_t again = 0;  // rounds (modulo 32) of this warp whose keys came too near a border
+  for (int h0 = 0, round = 0; h0 < a.kv_heads; h0 += SLOTS, ++round) {
+    const int h = h0 + slot;
+    if (h0 > 0) {
+      k.zero();
+      v.zero();
+      if (h < a.kv_heads) {
+        k.load(k0 + h * a.kh);
+        v.load(v0 + h * a.vh);
+      }
+    }
+    float x[8];
+    bool doubtful = false;
+    if (turns) turn(k, x);
+    else k.values(x);
+    const Row4 of_key = row4_of<LANES, true>(x, doubtful);
+    if (turns && __any_sync(0xffffffffu, doubtful && h < a.kv_heads)) again |= 1u << (round & 31);
+    v.values(x);
+    const Row4 of_value = row4_of<LANES, false>(x, doubtful);
+    if (h < a.kv_heads) {
+      store(a.keys, a.key_scales, h, of_key);
+      store(a.values, a.value_scales, h, of_value);
+    }
+  }
+  // such rows once more, in 64 bits
+#pragma unroll 1
+  for (int h0 = 0, round = 0; again != 0 && h0 < a.kv_heads; h0 += SLOTS, ++round) {
+    if (!(again >> (round & 31) & 1)) continue;
+    const int h = h0 + slot;
+    k.zero();
+    if (h < a.kv_heads) k.load(k0 + h * a.kh);
+    const Row4 r = row4_of_rotated<T>(a, k, partner_of(k), token, place, LANES, channel);
+    if (h < a.kv_heads && r.exponent != 255) store(a.keys, a.key_scales, h, r);
   }
 }
 
@@ -899,6 +1036,9 @@ __global__ __launch_bounds__(256) void move_kept_kernel(const MoveArgs a) {
   }
 }
 
+template <typename T>
+auto append4_for(int head_dim) { return head_dim == 64 ? append4_kernel<T, 8> : head_dim == 128 ? append4_kernel<T, 16> : append4_kernel<T, 32>; }
+
 int check_rotary(const risa_b200_rotary* r, int head_dim, const char* what) {
   RISA_REQUIRE(r->turns != nullptr, "%s: null rotary table", what);
   RISA_REQUIRE(r->rotary_dim > 0 && r->rotary_dim % 2 == 0 && r->rotary_dim <= head_dim,
@@ -1036,8 +1176,8 @@ extern "C" int risa_b200_cache_append_axes(const risa_b200_cache* cache, const r
     }
   }
   a.status = status;
-  const auto kernel = dtype_code == 1 ? (bits == 4 ? append_kernel<__half, 4> : bits == 8 ? append_kernel<__half, 8> : append_kernel<__half, 16>)
-                                      : (bits == 4 ? append_kernel<__nv_bfloat16, 4> : bits == 8 ? append_kernel<__nv_bfloat16, 8> : append_kernel<__nv_bfloat16, 16>);
+  const auto kernel = dtype_code == 1 ? (bits == 4 ? append4_for<__half>(a.head_dim) : bits == 8 ? append_kernel<__half, 8> : append_kernel<__half, 16>)
+                                      : (bits == 4 ? append4_for<__nv_bfloat16>(a.head_dim) : bits == 8 ? append_kernel<__nv_bfloat16, 8> : append_kernel<__nv_bfloat16, 16>);
   return launched(launch_chained(kernel, dim3(step->tokens), dim3(128), 0, static_cast<cudaStream_t>(stream_ptr), a), "append");
 }
 

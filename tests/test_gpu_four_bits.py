@@ -194,6 +194,26 @@ def test_append_of_extreme_rows(dtype):
     assert bool(keys[4:6].isnan().all()) and bool(keys[[0, 1, 2, 3, 6, 7, 8, 9, 10, 11]].isfinite().all())
 
 
+def test_rows_beside_ones_that_are_not_finite():
+    """Rotated keys of which every other head is not finite: the others are those of the formula, also where they are decided in 64
+    bits (many rows, so that some of them are)."""
+    n, d = 600, 128
+    cache = risa.allocate_key_value_cache(38, 4, 16, d, dtype=torch.uint8)
+    table, length = torch.arange(38, dtype=torch.int32, device="cuda")[None], torch.tensor([n], dtype=torch.int32, device="cuda")
+    k = torch.randn(n, 4, d, device="cuda").bfloat16()
+    k[::2, 1, 5], k[1::2, 1, 100], k[:, 3, 64] = torch.nan, torch.inf, -torch.inf
+    rotary = risa.rotary_table(d)
+    risa.append_to_cache(cache, k, k, table, length, query_offsets=torch.tensor([0, n], dtype=torch.int32, device="cuda"), rotary=rotary)
+    place = torch.arange(n, device="cuda")
+    frequencies = [u % 2 ** 64 / 2 ** 64 * 2 * torch.pi for u in rotary.turns.tolist()]
+    codes, groups, exponents = F.quantized(U.turned(k, place[:, None].expand(n, 4), frequencies, 1.0, False))
+    e, s = F.scales_of(cache.key_scales, 16)
+    got = F.unpacked(cache.keys)
+    at = (place // 16, slice(None), place % 16)
+    assert torch.equal(e[at], exponents) and torch.equal(s[at], groups) and torch.equal(got[at], codes)
+    assert bool((exponents[:, 1::2] == 255).all()) and bool((exponents[:, ::2] < 255).all())
+
+
 @pytest.mark.parametrize("kind", [BF16, F16, torch.int8])
 def test_reading_other_caches(kind):
     quantized = kind == torch.int8
