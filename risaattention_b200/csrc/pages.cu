@@ -2,7 +2,7 @@
 // tokens.  `references` counts for each page how many entries of page tables lead to it; a page with none is free.  All of it
 // happens on the device in a fixed order, so results do not depend on timing: the lowest free pages go first, to the sequences
 // in their order.
-#include "serving.cuh"
+#include "serving_plan.cuh"
 
 #include <algorithm>
 
@@ -102,7 +102,11 @@ __device__ __forceinline__ Change change_of(const ResizeArgs& a, int s) {
 
 // One CTA: what each sequence needs, added up in order; then free pages, lowest first, until there are enough (16 K a round); then
 // what each sequence is granted.
-__device__ __forceinline__ void plan_resize(const ResizeArgs& a, int* warp_sums) {
+struct PlanShared {
+  BlockScan<kPlanThreads> scan;  // needs can add up past 32 bits
+  int warp_sums[32];
+};
+__device__ __forceinline__ void plan_resize(const ResizeArgs& a, PlanShared& shared) {
   int needed = 0;
   for (int s0 = 0; s0 < a.batch; s0 += kPlanThreads) {
     const int s = s0 + threadIdx.x;
@@ -117,10 +121,10 @@ __device__ __forceinline__ void plan_resize(const ResizeArgs& a, int* warp_sums)
       need = c.need();
       a.left[s] = c.shared;
     }
-    int total;
-    const int before = needed + block_prefix(need, warp_sums, total);
-    if (s < a.batch) a.before[s] = before;
-    needed = min(needed + total, a.pages);  // more than there are: nobody behind gets any
+    int64_t total;
+    const int64_t before = needed + block_inclusive_scan<kPlanThreads>(need, shared.scan, total) - need;
+    if (s < a.batch) a.before[s] = int(min(before, int64_t(a.pages)));
+    needed = int(min(needed + total, int64_t(a.pages)));  // more than there are: nobody behind gets any
   }
   int found = 0;
   for (int p0 = 0; p0 < a.pages && found < needed; p0 += kPlanThreads * kPlanEach) {
@@ -129,7 +133,7 @@ __device__ __forceinline__ void plan_resize(const ResizeArgs& a, int* warp_sums)
 #pragma unroll
     for (int i = 0; i < kPlanEach; ++i)
       if (first + i < a.pages && a.references[first + i] == 0) free_pages |= 1u << i;
-    int total, rank = found + block_prefix(__popc(free_pages), warp_sums, total);
+    int total, rank = found + block_prefix(__popc(free_pages), shared.warp_sums, total);
     for (; free_pages != 0 && rank < needed; free_pages &= free_pages - 1) a.fresh[rank++] = first + __ffs(free_pages) - 1;
     found += total;
   }
@@ -195,10 +199,10 @@ __device__ __forceinline__ void apply_resize(const ResizeArgs& a, int s, int par
 }
 
 __global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(const ResizeArgs a) {
-  __shared__ int warp_sums[32];
+  __shared__ PlanShared shared;
   chain_wait();
   chain_release();
-  plan_resize(a, warp_sums);
+  plan_resize(a, shared);
 }
 __global__ __launch_bounds__(256) void resize_apply_kernel(const ResizeArgs a) {
   chain_wait();
@@ -209,10 +213,10 @@ __global__ __launch_bounds__(256) void resize_apply_kernel(const ResizeArgs a) {
 constexpr int kResizeCtas = 8;
 constexpr int64_t kLittle = 4 << 20;  // bytes that all sequences together can have copied
 __global__ __cluster_dims__(kResizeCtas, 1, 1) __launch_bounds__(kPlanThreads) void resize_kernel(const ResizeArgs a) {
-  __shared__ int warp_sums[32];
+  __shared__ PlanShared shared;
   chain_wait();
   chain_release();
-  if (blockIdx.x == 0) plan_resize(a, warp_sums);
+  if (blockIdx.x == 0) plan_resize(a, shared);
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
   for (int s = blockIdx.x; s < a.batch; s += kResizeCtas) apply_resize(a, s, 0, 1);
 }

@@ -26,6 +26,7 @@ inline int check_cache(const risa_b200_cache* c, const char* what) {
   RISA_REQUIRE(c->dtype_code == 1 || c->dtype_code == 2 || c->dtype_code == kInt8 || c->dtype_code == kInt4,
                "%s: the cache holds float16, bfloat16 or codes of 8 or 4 bits", what);
   RISA_REQUIRE(bits_of(*c) == 16 || (c->key_scales != nullptr && c->value_scales != nullptr), "%s: a cache of codes needs scales", what);
+  RISA_REQUIRE(c->dtype_code != kInt4 || c->kv_heads <= 65535, "%s: a cache in 4 bits has at most 65535 heads", what);  // bytes of a page in 32 bits
   RISA_REQUIRE(c->dtype_code != kInt4 || (reinterpret_cast<uintptr_t>(c->key_scales) | reinterpret_cast<uintptr_t>(c->value_scales)) % 16 == 0,
                "%s: scales of 4-bit codes must be 16-byte aligned", what);
   RISA_REQUIRE((reinterpret_cast<uintptr_t>(c->keys) | reinterpret_cast<uintptr_t>(c->values)) % 16 == 0,
