@@ -671,15 +671,26 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
         next = next + 1 == W::STAGES ? 0 : next + 1;
       }
       uint32_t data[SUB];
+      int key[SUB];
+      bool alone[SUB], hidden[SUB], masked = false, partial = false;
       float acc[SUB][NT][4], vs[SUB][2], lift[SUB][2];
 #pragma unroll
       for (int u = 0; u < SUB; ++u) {
         data[u] = ring + stage * W::STAGE;
-        const int key = walk.key_of(i + u);
-        // the last step may stand alone
-        const bool alone = SUB > 1 && i + u >= walk.count, hidden = alone || (walk.hidden >> stage & 1);
+        key[u] = walk.key_of(i + u);
+        alone[u] = SUB > 1 && i + u >= walk.count;  // the last step may stand alone
+        hidden[u] = alone[u] || (walk.hidden >> stage & 1);
+        masked = masked || hidden[u] || key[u] < all_lo || key[u] + 16 > all_hi;
+        partial = partial || alone[u] || key[u] < low || key[u] + 16 > seq.length;
+        stage = stage + 1 == W::STAGES ? 0 : stage + 1;
+      }
+      if (C::BITS == 4 && partial)
+#pragma unroll
+        for (int u = 0; u < SUB; ++u) walk.clear_missing(data[u], key[u], alone[u]);
+      // no branch from here to the mask, so that the steps' chains of products run side by side
+#pragma unroll
+      for (int u = 0; u < SUB; ++u) {
         const uint32_t key_scales = data[u] + 2 * C::SIDE, value_scales = key_scales + C::SCALES;
-        if (C::BITS == 4 && (alone || key < low || key + 16 > seq.length)) walk.clear_missing(data[u], key, alone);
         score_step<C>(data[u], key_scales, qf, acc[u]);
         float ks0 = 1.f, ks1 = 1.f;
         vs[u][0] = vs[u][1] = 1.f;
@@ -706,16 +717,17 @@ __global__ __launch_bounds__(kThreads, C::CTAS) void paged_rows_kernel(const Row
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
           for (int e = 0; e < 4; ++e) acc[u][nt][e] *= C::CODES ? (e < 2 ? ks0 : ks1) * factor[nt][e & 1] : factor[nt][e & 1];
-        if (hidden || key < all_lo || key + 16 > all_hi) {
+      }
+      if (masked) {
+#pragma unroll
+        for (int u = 0; u < SUB; ++u)
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) {
-              const int k = key + g + (e >> 1) * 8;
-              if (hidden || !outside_gap<C>(a.line, k, lo[nt][e & 1]) || k >= hi[nt][e & 1]) acc[u][nt][e] = -INFINITY;
+              const int k = key[u] + g + (e >> 1) * 8;
+              if (hidden[u] || !outside_gap<C>(a.line, k, lo[nt][e & 1]) || k >= hi[nt][e & 1]) acc[u][nt][e] = -INFINITY;
             }
-        }
-        stage = stage + 1 == W::STAGES ? 0 : stage + 1;
       }
       uint32_t p[SUB][NT][2];
 #pragma unroll
