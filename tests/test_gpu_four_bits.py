@@ -106,6 +106,9 @@ APPENDS = [
     ([16, 70], [16, 65], (4, 4), 128, 64, None),
     ([1000, 500], [999, 400], (8, 8), 128, 16, dict(rotary_dim=96, magnitude=1.3)),
     ([3, 20], [7, 2], (2, 2), 64, 16, None),   # more tokens than the sequence has
+    ([60, 9], [50, 9], (40, 40), 128, 16, dict(rotary_dim=128)),   # more heads than a block of threads takes at once
+    ([40], [33], (80, 20), 64, 32, dict(rotary_dim=64)),
+    ([40], [33], (9, 9), 256, 16, dict(rotary_dim=128, sections=(24, 40), dealt=True)),
 ]
 
 
@@ -129,7 +132,7 @@ def test_append(case, dtype, interleaved):
     options, want_k = {}, k.double()
     place, owner = places_of(lengths, chunks)
     if rotary is not None:
-        table = risa.rotary_table(**rotary)
+        table = risa.rotary_table(**rotary)  # of several axes: without positions all of them have the place
         frequencies = [u % 2 ** 64 / 2 ** 64 * 2 * torch.pi for u in table.turns.tolist()]
         options = dict(q=b.q, rotary=table, interleaved=interleaved)
         positions = torch.cat((place, place.new_zeros(2)))
@@ -287,6 +290,50 @@ def test_a_conversation(monkeypatch):
     out, lse = risa.paged_attention(q, cache, target, lengths, window=20, sinks=3, return_lse=True)
     with_sinks(monkeypatch, 3)
     F.assert_attention(U.Batch(cache, target, lengths, torch.tensor([0, 1, 2]), [1, 1], q, 0), out, lse, window=20)
+
+
+def test_pools_past_32_bits():
+    """Pages that lie 4 GB into a pool give what they give at its front, in every call."""
+    d, page, heads, lengths, chunks = 256, 128, 8, [500, 131], [40, 1]
+    b = F.batch_of(lengths, chunks, q_heads=16, kv_heads=heads, head_dim=d, page=page, dtype=F16)
+    few, far = b.cache.keys.shape[0], 34000
+    big = risa.allocate_key_value_cache(far + 2 * few, heads, page, d, dtype=torch.uint8)
+    assert big.keys[far:].data_ptr() - big.keys.data_ptr() > 2 ** 32
+    for to, source in zip(big.tensors, b.cache.tensors):
+        to[far:far + few] = source
+    table = torch.where(b.table >= 0, b.table + far, -1)
+    k, v = (torch.randn(41, heads, d, device="cuda").half() for _ in range(2))
+    got = []
+    for cache, rows in ((b.cache, b.table), (big, table)):
+        step = (cache, rows, b.lengths)
+        risa.append_to_cache(cache, k, v, *step[1:], query_offsets=b.offsets)
+        out, lse = risa.paged_attention(b.q, *step, query_offsets=b.offsets, window=300, sinks=9, return_lse=True)
+        weights = risa.cached_key_weights(b.q, lse, *step, query_offsets=b.offsets)
+        got.append((out, lse, weights, *risa.read_from_cache(*step, query_offsets=b.offsets, tokens=41, dtype=F16)))
+    assert all(torch.equal(x, y) for x, y in zip(*got))
+    # a page that is shared is copied, and all pages in use move to another pool
+    references = torch.ones(far + 2 * few, dtype=torch.int32, device="cuda")
+    references[far + few:] = 0
+    children, sizes = risa.fork_sequences(big, references, table, b.lengths, torch.tensor([1, 0], dtype=torch.int32, device="cuda"))
+    sizes = risa.resize_sequences(big, references, children, sizes, sizes + 1) - 1
+    assert bool((children == far + few).any()) and bool((children == far + few + 1).any())
+    references[:far] = 0
+    target = risa.allocate_key_value_cache(2 * few, heads, page, d, dtype=torch.uint8)
+    moved, _, used = risa.compact_cache(big, references, children, sizes, target)
+    offsets = torch.tensor([0, 131, 631], dtype=torch.int32, device="cuda")
+    want = risa.read_from_cache(b.cache, b.table.flip(0), b.lengths.flip(0), query_offsets=offsets, tokens=631, dtype=F16)
+    for cache, rows in ((big, children), (target, moved)):
+        now = risa.read_from_cache(cache, rows, sizes, query_offsets=offsets, tokens=631, dtype=F16)
+        assert torch.equal(now[0], want[0]) and torch.equal(now[1], want[1])
+    assert int(used) == few + 2
+    # and eviction copies to its end
+    goal = torch.arange(far + few, far + few + 2, dtype=torch.int32, device="cuda").view(2, 1)
+    kept, left, _ = risa.evict_from_cache(big, table, b.lengths, got[1][2], goal, budget=100, recent=20)
+    now = risa.read_from_cache(big, goal, left, query_offsets=torch.tensor([0, 100, 200], dtype=torch.int32, device="cuda"), tokens=200, dtype=F16)
+    whole = risa.read_from_cache(b.cache, b.table, b.lengths, query_offsets=torch.tensor([0, 500, 631], dtype=torch.int32, device="cuda"), tokens=631, dtype=F16)
+    for s, start in enumerate((0, 500)):
+        for h in range(heads):
+            assert torch.equal(now[0][100 * s:100 * s + 100, h], whole[0][start + kept[s, h].long(), h])
 
 
 def test_pages_outside_the_pool():

@@ -290,3 +290,14 @@ def test_children_of_a_prompt(kind, monkeypatch):
     F.assert_attention(U.Batch(target, new, left, torch.arange(5), [1] * 4, q, 0), out, lse)
     again = risa.read_from_cache(target, new, left, query_offsets=ints([0, 0, 68, 68, 68]), tokens=68, dtype=torch.bfloat16)
     assert torch.equal(again[0], keys[68:136]) and torch.equal(again[1], values[68:136])
+
+
+@pytest.mark.skipif(torch.cuda.device_count() < 2, reason="needs two GPUs")
+def test_on_another_device_than_the_current_one():
+    for device in ("cuda:0", "cuda:1"):
+        cache = risa.allocate_key_value_cache(9, 2, 16, 64, dtype=torch.uint8, device=device)
+        references, table = torch.zeros(9, dtype=torch.int32, device=device), torch.full((2, 3), -1, dtype=torch.int32, device=device)
+        sizes = risa.resize_sequences(cache, references, table, torch.zeros(2, dtype=torch.int32, device=device), torch.tensor([20, 40], dtype=torch.int32, device=device))
+        children, lengths = risa.fork_sequences(cache, references, table, sizes, torch.tensor([1], dtype=torch.int32, device=device))
+        moved = risa.compact_cache(cache, references, children, lengths, risa.allocate_key_value_cache(5, 2, 16, 64, dtype=torch.uint8, device=device))
+        assert table.tolist() == [[0, 1, -1], [2, 3, 4]] and children.tolist() == [[2, 3, 4]] and moved.page_table.tolist() == [[2, 3, 4]]
