@@ -109,6 +109,10 @@ template <int TO, int FROM>
 __device__ __forceinline__ void copy16_at(uint32_t to, const void* from) {
   asm volatile("cp.async.cg.shared.global [%0 + %2], [%1 + %3], 16;" ::"r"(to), "l"(from), "n"(TO), "n"(FROM) : "memory");
 }
+template <int TO>
+__device__ __forceinline__ void copy4_at(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0 + %2], [%1], 4;" ::"r"(to), "l"(from), "n"(TO) : "memory");
+}
 __device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
 template <int N> __device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
@@ -181,7 +185,11 @@ __device__ __forceinline__ uint32_t less_1152(uint32_t u) {
   return *reinterpret_cast<const uint32_t*>(&d);
 }
 __device__ __forceinline__ uint32_t pair_of_flipped(uint32_t word, int i) { return less_1152(__byte_perm(word, 0x64646464u, i ? 0x4342 : 0x4140)); }
-__device__ __forceinline__ uint32_t pair_of_halves(uint32_t pair) { return less_1152((pair & 0x00ff00ffu) ^ 0x64806480u); }
+__device__ __forceinline__ uint32_t pair_of_halves(uint32_t pair) {
+  uint32_t u;  // (pair & 0x00ff00ff) ^ 0x64806480: one instruction, of which the compiler makes two
+  asm("lop3.b32 %0, %1, %2, %3, 0x6a;" : "=r"(u) : "r"(pair), "r"(0x00ff00ffu), "r"(0x64806480u));
+  return less_1152(u);
+}
 
 // Not in front of the window, or one of the first keys.
 template <typename C>
@@ -201,9 +209,10 @@ struct Walk {
   int turn, skip;  // FRONT: from step `turn` on keys lie `skip` further, behind the first ones that stay visible
   int pages, pages_ahead;
   uint32_t base;
-  // 4-bit codes: this lane's pieces of the sequence's head in page 0, and bytes of a page
+  // codes: this lane's pieces of the sequence's head in page 0, and bytes of a page
   const char *key_rows, *value_rows, *scales[2];
-  int scale_each[2], page_rows, page_scales;
+  int scale_each[2];
+  std::conditional_t<C::BITS == 4, int, int64_t> page_rows, page_scales;
   unsigned int hidden;  // one bit per stage
   static constexpr int STAGES = C::stages(WITH_VALUES ? 2 : 1);
   static constexpr int SIDES = WITH_VALUES ? 2 : 1;
@@ -221,47 +230,46 @@ struct Walk {
     pages = look_up(lane);
     pages_ahead = look_up(32 + lane);
     hidden = 0;
-    if constexpr (C::BITS == 4) {
-      const int shift = a.line.step.page_shift, block = token_scale_bytes<C::D>() << shift;
-      page_rows = (a.line.kv_heads << shift) * C::ROW;
-      page_scales = a.line.kv_heads * block;
+    if constexpr (C::CODES) {
+      const int shift = a.line.step.page_shift, block = (C::BITS == 4 ? token_scale_bytes<C::D>() : 4) << shift;
+      page_rows = (decltype(page_rows)(a.line.kv_heads) << shift) * C::ROW;
+      page_scales = decltype(page_rows)(a.line.kv_heads) * block;
       const int64_t of_head = (int64_t(head) << shift) * C::ROW + lane * 16;
       key_rows = a.keys + of_head;
       value_rows = a.values + of_head;
 #pragma unroll
-      for (int j = 0; j < SCALE_ROUNDS; ++j) {  // exponents, then group scales, of the keys, then of the values
-        const int index = j * 32 + lane, piece = index < C::SCALES / 16 ? index : index - C::SCALES / 16;
-        scales[j] = reinterpret_cast<const char*>(index < C::SCALES / 16 ? a.key_scales : a.value_scales) + int64_t(head) * block +
-                    (piece == 0 ? 0 : (1 << shift) + (piece - 1) * 16);
-        scale_each[j] = piece == 0 ? 1 : C::D / 16;
+      for (int j = 0; j < SCALE_ROUNDS; ++j) {  // of the keys, then of the values; 4 bits: exponents, then group scales
+        const int index = j * 32 + lane, piece = index < SCALE_PIECES ? index : index - SCALE_PIECES;
+        scales[j] = reinterpret_cast<const char*>(index < SCALE_PIECES ? a.key_scales : a.value_scales) + int64_t(head) * block +
+                    (C::BITS == 8 ? piece * 4 : piece == 0 ? 0 : (1 << shift) + (piece - 1) * 16);
+        scale_each[j] = C::BITS == 8 ? 4 : piece == 0 ? 1 : C::D / 16;
       }
     }
   }
-  static constexpr int SCALE_ROUNDS = (SIDES * C::SCALES / 16 + 31) / 32;
+  static constexpr int SCALE_BYTES = C::BITS == 8 ? 4 : 16, SCALE_PIECES = C::SCALES / SCALE_BYTES;  // of a copy, copies of a side
+  static constexpr int SCALE_ROUNDS = (SIDES * SCALE_PIECES + 31) / 32;
+  // What 512 bytes of a step further in the swizzle flip (offset_of's rows are 512 bytes apart by its lines).
+  static constexpr int flip(int j) {
+    return C::ROW == 128 ? (j & 1) * 64 : C::ROW == 256 ? (j & 3) * 32 : 0;
+  }
+  template <int J>
+  __device__ __forceinline__ void copy_codes(uint32_t to, int first, const char* k, const char* v) {
+    copy16_at<J * 512, J * 512>(to + (first ^ flip(J)), k);
+    if constexpr (WITH_VALUES) copy16_at<C::SIDE + J * 512, J * 512>(to + (first ^ flip(J)), v);
+    if constexpr (J + 1 < C::CHUNKS / 2) copy_codes<J + 1>(to, first, k, v);
+  }
   // 16 keys that exist.
-  __device__ __forceinline__ void fetch_codes4(int key, int page, uint32_t to) {
+  __device__ __forceinline__ void fetch_codes(int key, int page, uint32_t to) {
     const int lane = threadIdx.x & 31, slot = key & ((1 << a.line.step.page_shift) - 1);
     const int64_t off = int64_t(page) * page_rows + slot * C::ROW;
-    const char *k = key_rows + off, *v = value_rows + off;
-    // 512 bytes further rows lie alike in the swizzle, but for heads of 256 channels: there every other 512
-    const int first = offset_of<C>(lane / C::CHUNKS, lane % C::CHUNKS);
-    const uint32_t at = to + first, odd = C::D == 256 ? to + (first ^ 64) : at;
-    copy16_at<0, 0>(at, k);
-    if constexpr (C::CHUNKS >= 4) copy16_at<512, 512>(odd, k);
-    if constexpr (C::CHUNKS == 8) copy16_at<1024, 1024>(at, k);
-    if constexpr (C::CHUNKS == 8) copy16_at<1536, 1536>(odd, k);
-    if constexpr (WITH_VALUES) {
-      copy16_at<C::SIDE, 0>(at, v);
-      if constexpr (C::CHUNKS >= 4) copy16_at<C::SIDE + 512, 512>(odd, v);
-      if constexpr (C::CHUNKS == 8) copy16_at<C::SIDE + 1024, 1024>(at, v);
-      if constexpr (C::CHUNKS == 8) copy16_at<C::SIDE + 1536, 1536>(odd, v);
-    }
-    const uint32_t scales_at = to + lane * 16;
+    copy_codes<0>(to, offset_of<C>(lane / C::CHUNKS, lane % C::CHUNKS), key_rows + off, value_rows + off);
+    const uint32_t scales_at = to + lane * SCALE_BYTES;
 #pragma unroll
     for (int j = 0; j < SCALE_ROUNDS; ++j)
-      if (j * 32 + lane < SIDES * C::SCALES / 16) {
+      if (SIDES * SCALE_PIECES >= (j + 1) * 32 || j * 32 + lane < SIDES * SCALE_PIECES) {
         const char* from = scales[j] + (int64_t(page) * page_scales + slot * scale_each[j]);
-        if (j == 0) copy16_at<SIDES * C::SIDE, 0>(scales_at, from);
+        if constexpr (C::BITS == 8) copy4_at<SIDES * C::SIDE>(scales_at, from);
+        else if (j == 0) copy16_at<SIDES * C::SIDE, 0>(scales_at, from);
         else copy16_at<SIDES * C::SIDE + 512, 0>(scales_at, from);
       }
   }
@@ -280,7 +288,7 @@ struct Walk {
     }
 #pragma unroll
     for (int j = 0; j < SCALE_ROUNDS; ++j)
-      if (j * 32 + lane < SIDES * C::SCALES / 16)
+      if (j * 32 + lane < SIDES * SCALE_PIECES)
         copy16(to + SIDES * C::SIDE + (j * 32 + lane) * 16, scales[j] + (good ? int64_t(page) * page_scales + slot * scale_each[j] : 0), good);
   }
   // Fetches step i into stage i % STAGES (its stage number is given) and closes a copy group either way.
@@ -292,10 +300,10 @@ struct Walk {
       }
       const int lane = threadIdx.x & 31, key = key_of(i);
       const int page = __shfl_sync(0xffffffffu, pages, i & 31);
-      if constexpr (C::BITS == 4) {
+      if constexpr (C::CODES) {
         // nearly all steps are of 16 keys that exist
         if (uint32_t(page) < uint32_t(a.pages) && key >= low && key + 16 <= length) {
-          fetch_codes4(key, page, base + stage * STAGE);
+          fetch_codes(key, page, base + stage * STAGE);
           if (hidden != 0) hidden &= ~(1u << stage);
           copies_commit();
           return;
@@ -454,8 +462,8 @@ __device__ __forceinline__ void score_step(uint32_t keys, uint32_t scales, const
   } else if constexpr (C::BITS == 8) {
 #pragma unroll
     for (int b = 0; b < C::D / 64; ++b) {
-      const uint4 lo = read16(keys + offset_of<C>(g, b * 4 + t));
-      const uint4 hi = read16(keys + offset_of<C>(g + 8, b * 4 + t));
+      const uint32_t at = keys + offset_of<C>(g, b * 4 + t);  // keys g and g + 8 lie alike in the swizzle
+      const uint4 lo = read16_at<0>(at), hi = read16_at<8 * C::ROW>(at);
       const uint32_t wl[4] = {lo.x, lo.y, lo.z, lo.w}, wh[4] = {hi.x, hi.y, hi.z, hi.w};
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
