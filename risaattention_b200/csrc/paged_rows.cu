@@ -13,8 +13,9 @@
 // scores s but of s + log2(scale): what is rounded is at most 1, and exact relative to the largest contribution.
 //
 // Measured: 16 requests of up to 16K keys, 8 key heads of 128 bf16 channels, 110 us (6.1 TB/s, 95 % of a plain copy's rate);
-// 32 requests of up to 32K keys as codes 244 us at full clocks (5.7 TB/s), 280 in long runs, where the conversion's
-// instructions (schedulers 61 % busy) feel the lower clock.
+// 32 requests of up to 32K keys as codes 238 us at full clocks (5.9 TB/s), more in long runs, where the conversion's
+// instructions feel the lower clock; in 4 bits 202 (3.9 TB/s): 360 instructions a step, 160 of them conversion, at 57 % of the
+// issue slots, with three warps a scheduler.
 #include "four_bits.cuh"
 #include "paged_tc.cuh"
 #include "serving_plan.cuh"
@@ -72,8 +73,9 @@ struct Tile {
   // more per SM.  Codes, whose conversion keeps the schedulers busy, gain from a third CTA (32 requests of up to 32K
   // keys: 280 us with two, 247 with three, 267 with four); 16-bit rows of 256 channels leave room for one.
   static constexpr int CTAS = D == 256 && !CODES ? 1 : CODES && D <= 128 && NT == 1 ? 3 : 2;
-  // Steps that share a maximum: with half of the bytes for the same instructions, 4-bit codes gain from halving the softmax's.
-  static constexpr int SUB = BITS == 4 && NT == 1 ? 2 : 1;
+  // Steps that share a maximum: with half of the bytes for the same instructions, 4-bit codes gain from halving the softmax's
+  // (32 requests of up to 32K keys 264 -> 246 us when it was brought in, with 16 rows 311 -> 282); 16 rows of 256 channels have no registers for it.
+  static constexpr int SUB = BITS == 4 && (NT == 1 || D <= 128) ? 2 : 1;
   static constexpr int BUDGET = 48 * 1024 / CTAS;  // per warp
   __host__ __device__ static constexpr int stages(int sides) {
     const int n = BUDGET / (sides * (SIDE + SCALES));
