@@ -289,9 +289,10 @@ __device__ __forceinline__ uint32_t code_bits(int code, int channel) { return ui
 
 // Group scale: the largest value of the group over 7 token scales, rounded to e4m3.  Code: the value over both scales, rounded
 // to nearest even.  Values of 16 bits meet the borders between codes (and between scales) exactly or not nearly, so that
-// for rows as they came this is decided in 32 bits: quotients corrected by their remainders are exact where they meet one.  Rotated values are off by 2^-21 of
-// the row's largest value at most (cosine and sine 2^-22.8 each, of a pair whose length is sqrt(2) times that at most); `doubtful`
-// says that one of them lies within twice that of a border.
+// for rows as they came this is decided in 32 bits: quotients corrected by their remainders are exact where they meet one.  Rotated
+// values are off by 2^-20.9 of the row's largest value at most: the angle is rounded to 2^-25 of half a turn and sincospi gives two
+// units in the last place, 2^-22.2 of a pair whose length is sqrt(2) times that value at most, and two roundings follow; the quotient
+// adds 2^-22.8.  `doubtful` says that one of them lies within 1.5 x 2^-20, more than twice the sum, of a border.
 template <int LANES, bool ROTATED>
 __device__ __forceinline__ Row4 row4_of(const float (&x)[8], bool& doubtful) {
   float group = fabsf(x[0]);
@@ -321,9 +322,9 @@ __device__ __forceinline__ Row4 row4_of(const float (&x)[8], bool& doubtful) {
     if (ROTATED) nearest = fminf(nearest, fabsf(fabsf(quotient - code[i]) - 0.5f));
   }
   if (ROTATED) {
-    const float slack = most * to_units * 0x1p-20f;
+    const float slack = most * to_units * 0x1.8p-20f;
     const uint32_t around = e4m3_pair(ratio + slack, fmaxf(ratio - slack, 0.f));
-    doubtful = usable && (nearest * scale < slack || (around & 0xffu) != around >> 8 || (bits - 16) >> 23 != (bits + 16) >> 23);
+    doubtful = usable && (nearest * scale < slack || (around & 0xffu) != around >> 8 || (bits - 24) >> 23 != (bits + 24) >> 23);
   }
   if (__any_sync(0xffffffffu, r.group < 8)) {  // scales below 2^-6 are rounded coarsely: quotients past 7
 #pragma unroll
