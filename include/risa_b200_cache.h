@@ -182,7 +182,8 @@ int risa_b200_fork_sequences(const risa_b200_cache* cache, int32_t* references,
  * last page is not full and has more than one reference it first gets a page in place of that, with a
  * copy of its tokens.  A shorter one gives back the pages behind its length (their entries become
  * -1); they are handed out from the next call on.  granted[s]: the length that the pages found allow
- * (a sequence whose shared page could not be replaced keeps its length). */
+ * (a sequence whose shared page could not be replaced keeps its length); it may be lengths or
+ * new_lengths itself. */
 size_t risa_b200_resize_scratch_size(const risa_b200_cache* cache, int batch);
 int risa_b200_resize_sequences(const risa_b200_cache* cache, int32_t* references,
                                int32_t* page_table, int table_width, const int32_t* lengths,

@@ -76,7 +76,10 @@ struct ResizeArgs {
   int32_t* granted;
   int32_t* references;
   int batch, width, page_shift, pages;
-  // the plan: pages that sequences in front of each one need, the shared page that it leaves, and the pages handed out
+  // the plan: both lengths of each sequence as they were (`granted` may lie over them), pages that sequences in front of it need,
+  // the shared page that it leaves, and the pages handed out
+  int32_t* was;
+  int32_t* asked;
   int32_t* before;
   int32_t* left;
   int32_t* fresh;
@@ -89,16 +92,11 @@ struct ResizeArgs {
   unsigned int* status;
 };
 
-__device__ __forceinline__ Change change_of(const ResizeArgs& a, int s) {
-  const int most = a.width << a.page_shift;
-  Change c;
-  c.length = min(max(__ldg(a.lengths + s), 0), most);
-  c.wanted = min(max(__ldg(a.wanted + s), 0), most);
-  c.held = pages_for(c.length, a.page_shift);
-  c.needed = pages_for(c.wanted, a.page_shift);
-  c.shared = -1;
-  return c;
+__device__ __forceinline__ Change change_of(const ResizeArgs& a, int length, int wanted, int shared) {
+  return {length, wanted, pages_for(length, a.page_shift), pages_for(wanted, a.page_shift), shared};
 }
+// As planned.
+__device__ __forceinline__ Change planned_change(const ResizeArgs& a, int s) { return change_of(a, a.was[s], a.asked[s], a.left[s]); }
 
 // One CTA: what each sequence needs, added up in order; then free pages, lowest first, until there are enough (16 K a round); then
 // what each sequence is granted.
@@ -112,13 +110,16 @@ __device__ __forceinline__ void plan_resize(const ResizeArgs& a, PlanShared& sha
     const int s = s0 + threadIdx.x;
     int need = 0;
     if (s < a.batch) {
-      Change c = change_of(a, s);
+      const int most = a.width << a.page_shift;
+      Change c = change_of(a, min(max(a.lengths[s], 0), most), min(max(a.wanted[s], 0), most), -1);
       if (c.wanted > c.length && (c.length & ((1 << a.page_shift) - 1)) != 0) {
         const int last = a.table[int64_t(s) * a.width + c.held - 1];
         if (last < 0 || last >= a.pages) atomicCAS(a.status, 0u, unsigned(s) + 1u);
         else if (a.references[last] > 1) c.shared = last;
       }
       need = c.need();
+      a.was[s] = c.length;
+      a.asked[s] = c.wanted;
       a.left[s] = c.shared;
     }
     int64_t total;
@@ -140,8 +141,7 @@ __device__ __forceinline__ void plan_resize(const ResizeArgs& a, PlanShared& sha
   if (threadIdx.x == 0) a.counts[0] = min(found, needed);
   found = min(found, needed);
   for (int s = threadIdx.x; s < a.batch; s += kPlanThreads) {
-    Change c = change_of(a, s);
-    c.shared = a.left[s];
+    const Change c = planned_change(a, s);
     const int need = c.need(), given = max(min(found - a.before[s], need), 0);
     int length = c.wanted;
     if (given < need) {
@@ -156,8 +156,7 @@ __device__ __forceinline__ void plan_resize(const ResizeArgs& a, PlanShared& sha
 // Part 0 of a sequence's CTAs writes entries and counts, all parts copy the rows of a page that was shared.
 __device__ __forceinline__ void apply_resize(const ResizeArgs& a, int s, int part, int parts) {
   const int threads = blockDim.x;
-  Change c = change_of(a, s);
-  c.shared = a.left[s];
+  const Change c = planned_change(a, s);
   const int found = a.counts[0], before = a.before[s], given = max(min(found - before, c.need()), 0);
   const bool copies = c.shared >= 0 && given > 0;
   int32_t* row = a.table + int64_t(s) * a.width;
@@ -371,7 +370,7 @@ extern "C" int risa_b200_fork_sequences(const risa_b200_cache* cache, int32_t* r
 
 extern "C" size_t risa_b200_resize_scratch_size(const risa_b200_cache* cache, int batch) {
   if (cache == nullptr || batch <= 0) return 0;
-  return sizeof(int32_t) * (2 * size_t(batch) + size_t(std::max(cache->pages, 0)) + 1);
+  return sizeof(int32_t) * (4 * size_t(batch) + size_t(std::max(cache->pages, 0)) + 1);
 }
 
 extern "C" int risa_b200_resize_sequences(const risa_b200_cache* cache, int32_t* references, int32_t* page_table, int table_width,
@@ -389,7 +388,7 @@ extern "C" int risa_b200_resize_sequences(const risa_b200_cache* cache, int32_t*
   if (status == nullptr) return RISA_B200_CUDA;
   int32_t* words = static_cast<int32_t*>(scratch);
   const ResizeArgs a{page_table, lengths, new_lengths, granted, references, batch, table_width, shift_of(cache->page_size), cache->pages,
-                     words + 1, words + 1 + batch, words + 1 + 2 * int64_t(batch), words,
+                     words + 1, words + 1 + batch, words + 1 + 2 * int64_t(batch), words + 1 + 3 * int64_t(batch), words + 1 + 4 * int64_t(batch), words,
                      static_cast<char*>(cache->keys), static_cast<char*>(cache->values), reinterpret_cast<char*>(cache->key_scales),
                      reinterpret_cast<char*>(cache->value_scales), cache->kv_heads, row_bytes, token_scale_of(*cache), group_scales_of(*cache), status};
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
