@@ -158,7 +158,7 @@ int risa_b200_key_weights_sinks(const risa_b200_cache* cache, const risa_b200_st
  * and copies them in their order to the pages of target_table [batch, target_width], which must hold
  * the budget and share no page with what is read.  step->query_offsets and tokens are not used.
  * weights: f32 [batch, kv_heads, table_width * page_size].  kept: int32 [batch, kv_heads, budget],
- * -1 behind the last; new_lengths: int32 [batch]; new_weights: f32 [batch, kv_heads,
+ * -1 behind the last; new_lengths: int32 [batch], may be the step's lengths; new_weights: f32 [batch, kv_heads,
  * target_width * page_size], 0 behind the last. */
 int risa_b200_cache_evict(const risa_b200_cache* cache, const risa_b200_step* step,
                           const float* weights, const int32_t* target_table, int target_width,

@@ -829,7 +829,6 @@ struct SelectArgs {
   StepView step;
   const float* weights;
   int32_t* kept;
-  int32_t* new_lengths;
   float* new_weights;
   int kv_heads, budget, recent, target_slots;
 };
@@ -857,7 +856,6 @@ __global__ __launch_bounds__(kSelectThreads) void select_kept_kernel(const Selec
   int32_t* kept = a.kept + row * a.budget;
   float* new_weights = a.new_weights + row * a.target_slots;
   const int count = min(length, a.budget), recent = min(a.recent, count);
-  if (head == 0 && tid == 0) a.new_lengths[s] = count;
   const int open = length - recent;         // tokens that compete
   const unsigned int wanted = count - recent;  // of which so many stay
   const int rounds = ((length + 31) / 32 + 31) / 32, begin = warp * rounds * 32;
@@ -958,6 +956,7 @@ struct MoveArgs {
   StepView step;
   const int32_t* target;
   const int32_t* kept;
+  int32_t* new_lengths;
   char* keys;
   char* values;
   float* key_scales;
@@ -977,7 +976,9 @@ __global__ __launch_bounds__(256) void move_kept_kernel(const MoveArgs a) {
   chain_release();
   const int s = blockIdx.z, head = blockIdx.y;
   const int slots = a.step.width << a.step.page_shift;
-  const int count = min(min(max(__ldg(a.step.lengths + s), 0), slots), a.budget);
+  // (the new length may lie over the old one: whichever a CTA reads, the count is the same)
+  const int count = min(min(max(a.step.lengths[s], 0), slots), a.budget);
+  if (blockIdx.x == 0 && head == 0 && threadIdx.x == 0) a.new_lengths[s] = count;
   const int per_pass = 256 >> a.row_shift, piece = threadIdx.x & ((1 << a.row_shift) - 1);
   const int j0 = blockIdx.x * per_pass * kMoveRows + (threadIdx.x >> a.row_shift);
   const int32_t* kept = a.kept + (int64_t(s) * a.kv_heads + head) * a.budget;
@@ -1220,14 +1221,14 @@ extern "C" int risa_b200_cache_evict(const risa_b200_cache* cache, const risa_b2
   if (status == nullptr) return RISA_B200_CUDA;
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
   const StepView view = view_of(*step, cache->page_size);
-  const SelectArgs select{view, weights, kept, new_lengths, new_weights, cache->kv_heads, budget, recent,
+  const SelectArgs select{view, weights, kept, new_weights, cache->kv_heads, budget, recent,
                           target_width * cache->page_size};
   if (const int bad = launched(launch_chained(select_kept_kernel, dim3(cache->kv_heads, step->batch), dim3(kSelectThreads), 0, stream, select), "evict"))
     return bad;
   const int row_bytes = cache->head_dim * bits_of(*cache) / 8;
   int shift = 0;
   while ((16 << shift) < row_bytes) ++shift;
-  const MoveArgs move{view, target_table, kept, static_cast<char*>(cache->keys), static_cast<char*>(cache->values),
+  const MoveArgs move{view, target_table, kept, new_lengths, static_cast<char*>(cache->keys), static_cast<char*>(cache->values),
                       cache->key_scales, cache->value_scales, cache->pages, cache->kv_heads, budget, target_width,
                       shift, cache->dtype_code == kInt4 ? cache->head_dim / 16 : 0, status};
   const int rows = (256 >> shift) * kMoveRows;

@@ -69,3 +69,20 @@ def test_lengths_resized_in_place(granted_is, heads, page):
             assert torch.equal(cache.keys[to, :, :n], was[0][source, :, :n]) and torch.equal(cache.values[to, :, :n], was[1][source, :, :n])
         lengths = granted
         assert step != 2 or len(account.copies) > 10
+
+
+def test_lengths_evicted_in_place():
+    """Heads whose largest weights lie behind the budget, so that a head which took the new length for the old one would keep others."""
+    lib, heads, page, width, budget = library(), 64, 16, 40, 48
+    batch = 30
+    cache = filled(batch * (width + 3), heads, page, 64, torch.bfloat16)
+    table = torch.arange(batch * width, dtype=torch.int32, device="cuda").view(batch, width)
+    target = torch.arange(batch * width, batch * (width + 3), dtype=torch.int32, device="cuda").view(batch, 3)
+    lengths = torch.arange(11, 11 + 20 * batch, 20, dtype=torch.int32, device="cuda")
+    weights = torch.rand(batch, heads, width * page, device="cuda") + torch.arange(width * page, device="cuda")
+    want = risa.evict_from_cache(cache, table, lengths, weights, target, budget=budget, recent=5)
+    kept, new_weights = torch.empty_like(want.kept), torch.empty_like(want.weights)
+    step = Step(table.data_ptr(), lengths.data_ptr(), None, batch, width, batch)
+    assert lib.risa_b200_cache_evict(ctypes.byref(Cache(cache)), ctypes.byref(step), at(weights), at(target), 3, budget, 5, at(kept), at(lengths), at(new_weights),
+                                     ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    assert torch.equal(lengths, want.lengths) and torch.equal(kept, want.kept) and torch.equal(new_weights, want.weights)
