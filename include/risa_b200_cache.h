@@ -7,6 +7,8 @@
  * status code with risa_b200_last_error(), no allocation, no host synchronisation.  Everything that
  * changes from step to step (lengths, offsets, page table) is read on the device, so a captured
  * graph replays with new contents.
+ * What a call writes lies apart from all that it reads, unless it is said below that it may be one
+ * of its inputs itself: CTAs write while others still read, and addresses are not compared.
  * dtype codes: 0 = float32, 1 = float16, 2 = bfloat16, 4 = int8 codes with a scale per token and head,
  * 5 = 4-bit codes with a scale per token and head and one per 16 channels.
  */
@@ -117,7 +119,8 @@ int risa_b200_cache_read(const risa_b200_cache* cache, const risa_b200_step* ste
 
 /* softmax(scale * q K^T) V of every packed token over its sequence's cached keys; with is_causal the
  * token at place p of its sequence sees keys max(0, p - window + 1) .. p (window 0: from the start),
- * without it all of them.  q, out: dtype_code 1 or 2 (the cache's own unless that holds codes).  lse: f32
+ * without it all of them.  q, out: dtype_code 1 or 2 (the cache's own unless that holds codes); out
+ * may be q itself, with its strides.  lse: f32
  * [tokens, q_heads] or NULL.  Rows that see no key give 0 and -inf.  clear_rest: rows of no
  * sequence are written the same way, bit 0 those of out, bit 1 those of lse, else left as they were. */
 size_t risa_b200_paged_attention_scratch_size(const risa_b200_cache* cache,
@@ -168,7 +171,9 @@ int risa_b200_cache_evict(const risa_b200_cache* cache, const risa_b200_step* st
 /* ---- pages shared, handed out, given back and moved ----------------------------------------------
  * references: int32 [pages], how many entries of page tables lead to each page; 0: the page is free.
  * Entries behind a sequence's length are not read; one that leads outside the pool is not counted, and
- * risa_b200_device_status() reports it. */
+ * risa_b200_device_status() reports it.  Tables and lengths that fork returns are others than the
+ * step's, and compact's target_references others than references; compact's table may be the
+ * step's page_table itself. */
 
 /* Row c of table [children, table_width] and lengths[c] become those of sequence parents[c] of the
  * step, -1 behind the length (a parent outside 0..batch-1: an empty sequence); references counts the

@@ -86,3 +86,20 @@ def test_lengths_evicted_in_place():
     assert lib.risa_b200_cache_evict(ctypes.byref(Cache(cache)), ctypes.byref(step), at(weights), at(target), 3, budget, 5, at(kept), at(lengths), at(new_weights),
                                      ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
     assert torch.equal(lengths, want.lengths) and torch.equal(kept, want.kept) and torch.equal(new_weights, want.weights)
+
+
+def test_a_table_compacted_in_place():
+    lib, pages, heads, page, width, batch = library(), 700, 2, 16, 12, 50
+    lib.risa_b200_compact_scratch_size.restype = ctypes.c_size_t
+    cache, target = filled(pages, heads, page, 64, torch.int8), filled(batch * width, heads, page, 64, torch.int8, seed=2)
+    references, table = ints([0] * pages), ints([[-1] * width] * batch)
+    lengths = risa.resize_sequences(cache, references, table, ints([0] * batch), ints([s * 4 for s in range(batch)]))
+    lengths = risa.resize_sequences(cache, references, table, lengths, ints([s * 4 if s % 3 else 0 for s in range(batch)]))
+    want = risa.compact_cache(cache, references, table, lengths, target)
+    here, there = Cache(cache), Cache(target)
+    scratch = torch.empty(lib.risa_b200_compact_scratch_size(ctypes.byref(here), ctypes.byref(there)), dtype=torch.uint8, device="cuda")
+    counts, used = torch.empty_like(want.references), torch.empty_like(want.used)
+    step = Step(table.data_ptr(), lengths.data_ptr(), None, batch, width, batch)
+    assert lib.risa_b200_cache_compact(ctypes.byref(here), at(references), ctypes.byref(step), ctypes.byref(there), at(table), at(counts), at(used), at(scratch),
+                                       ctypes.c_size_t(scratch.numel()), ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+    assert torch.equal(table, want.page_table) and torch.equal(counts, want.references) and torch.equal(used, want.used)
