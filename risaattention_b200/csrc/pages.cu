@@ -153,31 +153,28 @@ __device__ __forceinline__ void plan_resize(const ResizeArgs& a, PlanShared& sha
   }
 }
 
-// Part 0 of a sequence's CTAs writes entries and counts, all parts copy the rows of a page that was shared.
-__device__ __forceinline__ void apply_resize(const ResizeArgs& a, int s, int part, int parts) {
-  const int threads = blockDim.x;
+// By `step` threads, of which this is the `first`-th: entries and counts, then the rows of a page that was shared.
+__device__ __forceinline__ void apply_resize(const ResizeArgs& a, int s, int first, int step) {
   const Change c = planned_change(a, s);
   const int found = a.counts[0], before = a.before[s], given = max(min(found - before, c.need()), 0);
   const bool copies = c.shared >= 0 && given > 0;
   int32_t* row = a.table + int64_t(s) * a.width;
-  if (part == 0) {
-    for (int i = threadIdx.x; i < given; i += threads) {
-      const int page = a.fresh[before + i], column = copies ? c.held - 1 + i : c.held + i;
-      a.references[page] = 1;
-      row[column] = page;
-    }
-    if (copies && threadIdx.x == 0) atomicAdd(a.references + c.shared, -1);
-    for (int i = c.needed + threadIdx.x; i < c.held; i += threads) {  // given back
-      const int page = row[i];
-      if (page >= 0 && page < a.pages) atomicAdd(a.references + page, -1);
-      else atomicCAS(a.status, 0u, unsigned(s) + 1u);
-      row[i] = -1;
-    }
+  for (int i = first; i < given; i += step) {
+    const int page = a.fresh[before + i], column = copies ? c.held - 1 + i : c.held + i;
+    a.references[page] = 1;
+    row[column] = page;
+  }
+  if (copies && first == 0) atomicAdd(a.references + c.shared, -1);
+  for (int i = c.needed + first; i < c.held; i += step) {  // given back
+    const int page = row[i];
+    if (page >= 0 && page < a.pages) atomicAdd(a.references + page, -1);
+    else atomicCAS(a.status, 0u, unsigned(s) + 1u);
+    row[i] = -1;
   }
   if (!copies) return;
   const int64_t from = int64_t(c.shared) * a.kv_heads, to = int64_t(a.fresh[before]) * a.kv_heads;
   const int rows = c.length & ((1 << a.page_shift) - 1), pieces = a.row_bytes >> 4, each = rows * pieces;  // of a head
-  for (int i = part * threads + threadIdx.x; i < a.kv_heads * each; i += parts * threads) {
+  for (int i = first; i < a.kv_heads * each; i += step) {
     const int h = i / each;
     const int64_t in_head = int64_t(i - h * each) * 16, head_bytes = int64_t(a.row_bytes) << a.page_shift;
     const uint4 k = *reinterpret_cast<const uint4*>(a.keys + (from + h) * head_bytes + in_head);
@@ -189,7 +186,7 @@ __device__ __forceinline__ void apply_resize(const ResizeArgs& a, int s, int par
   // scales byte by byte: of the tokens, then (behind those of all the page's tokens) of their groups
   const int64_t block = int64_t(a.token_scales + a.group_scales) << a.page_shift;
   const int of_tokens = rows * a.token_scales, of_head = of_tokens + rows * a.group_scales;
-  for (int i = part * threads + threadIdx.x; i < a.kv_heads * of_head; i += parts * threads) {
+  for (int i = first; i < a.kv_heads * of_head; i += step) {
     const int h = i / of_head, j = i - h * of_head;
     const int64_t at = j < of_tokens ? j : (int64_t(a.token_scales) << a.page_shift) + j - of_tokens;
     a.key_scales[(to + h) * block + at] = a.key_scales[(from + h) * block + at];
@@ -206,18 +203,23 @@ __global__ __launch_bounds__(kPlanThreads) void resize_plan_kernel(const ResizeA
 __global__ __launch_bounds__(256) void resize_apply_kernel(const ResizeArgs a) {
   chain_wait();
   chain_release();
-  apply_resize(a, blockIdx.x, blockIdx.y, gridDim.y);
+  apply_resize(a, blockIdx.x, blockIdx.y * blockDim.x + threadIdx.x, gridDim.y * blockDim.x);
 }
-// Both in one launch where there is little to copy: a cluster of eight CTAs, of which the first one plans.
-constexpr int kResizeCtas = 8;
-constexpr int64_t kLittle = 4 << 20;  // bytes that all sequences together can have copied
+// Both in one launch where there is little to do: a cluster of eight CTAs, of which the first one plans.  Its warps are dealt to
+// the sequences, so that the chains of look-ups of as many run side by side (64 sequences that grow within their pages 5.0 us on
+// the GPU, 4.5 as two launches; calls in a row, which the host bounds, 8.3 and 10.4).  More sequences than warps, and more bytes
+// than this that all together can have copied, are for two launches: 4096 sequences 20.7 and 15.9 us, 256 with 4 MB to copy 21.8
+// and 8.9, with 1 MB 10.2 and 8.0.
+constexpr int kResizeCtas = 8, kResizeWarps = kResizeCtas * kPlanThreads / 32;
+constexpr int64_t kLittle = 4 << 20;
 __global__ __cluster_dims__(kResizeCtas, 1, 1) __launch_bounds__(kPlanThreads) void resize_kernel(const ResizeArgs a) {
   __shared__ PlanShared shared;
   chain_wait();
   chain_release();
   if (blockIdx.x == 0) plan_resize(a, shared);
   asm volatile("barrier.cluster.arrive.release.aligned;\nbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-  for (int s = blockIdx.x; s < a.batch; s += kResizeCtas) apply_resize(a, s, 0, 1);
+  const int thread = blockIdx.x * kPlanThreads + threadIdx.x, each = kResizeWarps / a.batch * 32, s = thread / each;
+  if (s < a.batch) apply_resize(a, s, thread - s * each, each);
 }
 
 // ---- compact ------------------------------------------------------------------------------------------------
@@ -392,7 +394,7 @@ extern "C" int risa_b200_resize_sequences(const risa_b200_cache* cache, int32_t*
                      static_cast<char*>(cache->keys), static_cast<char*>(cache->values), reinterpret_cast<char*>(cache->key_scales),
                      reinterpret_cast<char*>(cache->value_scales), cache->kv_heads, row_bytes, token_scale_of(*cache), group_scales_of(*cache), status};
   const cudaStream_t stream = static_cast<cudaStream_t>(stream_ptr);
-  if (2 * int64_t(batch) * cache->kv_heads * cache->page_size * row_bytes <= kLittle)
+  if (batch <= kResizeWarps && 2 * int64_t(batch) * cache->kv_heads * cache->page_size * row_bytes <= kLittle)
     return launched(launch_chained(resize_kernel, dim3(kResizeCtas), dim3(kPlanThreads), 0, stream, a), "resize");
   if (const int bad = launched(launch_chained(resize_plan_kernel, dim3(1), dim3(kPlanThreads), 0, stream, a), "resize")) return bad;
   // parts: 16 bytes of keys and values for each thread in turn, as many as fill the SMs and as a page has work for

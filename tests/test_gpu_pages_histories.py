@@ -88,9 +88,9 @@ def test_much_to_copy(kind, heads, page, d, children):
 
 
 @pytest.mark.parametrize("kind", KINDS)
-@pytest.mark.parametrize("batch", [1, 7, 31, 32, 33, 100, 257, 600])
+@pytest.mark.parametrize("batch", [1, 7, 31, 32, 33, 100, 129, 256, 257, 600])
 def test_little_to_copy(kind, batch):
-    """Histories of one launch, of fewer and of more sequences than it has warps."""
+    """Histories of one launch, where a sequence has several warps or one, and of more sequences than it has warps."""
     page, width = 16, 3
     pages = 3 * batch + 5
     history = History(filled(pages, 1, page, 64, kind), width, batch)
