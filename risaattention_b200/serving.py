@@ -119,6 +119,7 @@ def rotary_table(rotary_dim, *, base=10000.0, scaling=None, factor=1.0, original
         if dealt or restart:
             raise ValueError("dealt and restart need sections")
     else:
+        sections = list(sections)
         axes = _axes_of_pairs(rotary_dim, sections, dealt)
         if restart:
             own = [iter(rotary_frequencies(2 * n, **options)) for n in sections]
@@ -132,7 +133,6 @@ def rotary_table(rotary_dim, *, base=10000.0, scaling=None, factor=1.0, original
 
 
 def _axes_of_pairs(rotary_dim, sections, dealt):
-    sections = list(sections)
     if not 1 <= len(sections) <= MOST_AXES or any(not isinstance(n, int) or n <= 0 for n in sections):
         raise ValueError(f"sections must be 1 to {MOST_AXES} positive numbers of pairs, got {sections}")
     if 2 * sum(sections) != rotary_dim:
