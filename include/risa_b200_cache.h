@@ -29,7 +29,8 @@ extern "C" {
  * pointers lead to bytes [pages, kv_heads, page_size * (1 + head_dim / 16)], 16-byte aligned: of each
  * page and head first the token scales, powers of two as the exponent field of a float (0: a scale of
  * zero, 255: a row that is not finite), then for each token the scales of its groups of 16 channels,
- * e4m3 numbers that are not negative. */
+ * e4m3 numbers from 0 to 448: neither a sign bit nor e4m3's NaN, which are read by their bits and
+ * not checked (append writes none). */
 typedef struct {
   void* keys;
   void* values;
@@ -161,8 +162,8 @@ int risa_b200_key_weights_sinks(const risa_b200_cache* cache, const risa_b200_st
  * and copies them in their order to the pages of target_table [batch, target_width], which must hold
  * the budget and share no page with what is read.  step->query_offsets and tokens are not used.
  * weights: f32 [batch, kv_heads, table_width * page_size].  kept: int32 [batch, kv_heads, budget],
- * -1 behind the last; new_lengths: int32 [batch], may be the step's lengths; new_weights: f32 [batch, kv_heads,
- * target_width * page_size], 0 behind the last. */
+ * -1 behind the last; new_lengths: int32 [batch], may be the step's lengths; new_weights: f32
+ * [batch, kv_heads, target_width * page_size], 0 behind the last. */
 int risa_b200_cache_evict(const risa_b200_cache* cache, const risa_b200_step* step,
                           const float* weights, const int32_t* target_table, int target_width,
                           int budget, int recent, int32_t* kept, int32_t* new_lengths,
@@ -185,8 +186,9 @@ int risa_b200_fork_sequences(const risa_b200_cache* cache, int32_t* references,
 /* Brings every sequence from lengths[s] to new_lengths[s] tokens (at most what its row of the table
  * holds).  A longer one gets pages: the lowest that were free, in the order of the sequences; where its
  * last page is not full and has more than one reference it first gets a page in place of that, with a
- * copy of its tokens.  A shorter one gives back the pages behind its length (their entries become
- * -1); they are handed out from the next call on.  granted[s]: the length that the pages found allow
+ * copy of its tokens (each sequence that shares it, also where all of them grow in one call).  A
+ * shorter one gives back the pages behind its length (their entries become -1); they are handed out
+ * from the next call on.  granted[s]: the length that the pages found allow
  * (a sequence whose shared page could not be replaced keeps its length); it may be lengths or
  * new_lengths itself. */
 size_t risa_b200_resize_scratch_size(const risa_b200_cache* cache, int batch);

@@ -123,7 +123,9 @@ struct RotateArgs {
 // channels each.  Consecutive threads are consecutive runs of a row, then rows of consecutive tokens.  Bound by HBM: the
 // loads of four heads are on their way at once (2 x 16 heads x 16K tokens of 128 bf16 channels, half of them rotated: 78 us
 // with two, 57 with four, 4.7 TB/s).
-// With positions of several axes each of the eight pairs looks up its own (the same few cache lines).
+// With positions of several axes each of the eight pairs looks up its own (the same few cache lines).  In FP32 the rows of four heads
+// are 64 registers of the 64 that a thread has: 572 bytes of spill stores and 956 of loads, and 134 us for 2 x 16 heads x 16K rows of
+// 128 channels (4.0 TB/s; 16-bit rows spill 48 and 100 bytes, 47 us, 5.7 TB/s).
 constexpr int kHeadsAhead = 4;
 template <typename T, bool AXES>
 __global__ __launch_bounds__(256, 4) void rotate_kernel(const RotateArgs a) {
@@ -340,7 +342,7 @@ __device__ __forceinline__ Row4 row4_of(const float (&x)[8], bool turned, bool& 
 }
 // The same for a rotated row that came too near a border, in 64 bits: from the channels as they came (`own`, and `other` of a
 // lane half a rotated row away).  0.4 % of Gaussian rows of 128; nearly all rows with a turned group of 2^-18 to 2^-12 of the row's largest
-// value, whose codes are hardly wider than the rotation's own error (8160 tokens of such keys 125 us, others 62).
+// value, whose codes are hardly wider than the rotation's own error (8160 tokens of such keys 127 us, others 62).
 template <typename T>
 __device__ __noinline__ Row4 row4_of_rotated(const AppendArgs& a, Run<T> own, Run<T> other, int64_t token, int place, int lanes, int channel) {
   float u[8], v[8];
@@ -536,8 +538,11 @@ __global__ __launch_bounds__(128, 8) void append_kernel(const AppendArgs a) {
 }
 
 // In 4 bits: a kernel of its own, in which a CTA's row slots walk the token's query heads, then its keys, then its values (what is
-// computed of a row in 4 bits is three times as much as of a rotated one).  8160 tokens of 32 + 2 x 8 heads of 128: 72 us, 87 in
-// the kernel for all kinds of cache, whose every row paid for the registers of the call that decides doubtful ones.
+// computed of a row in 4 bits is three times as much as of a rotated one).  8160 tokens of 32 + 2 x 8 heads of 128: 67 us with
+// positions of three axes (184 MB, 2.7 TB/s), 62 with those of one; 87 in the kernel for all kinds of cache, whose every row paid for
+// the registers of the call that decides doubtful ones.  Latency bounds it: of the 6.4 warps that a scheduler has, 1.1 wait for
+// global memory (the look-ups in front of a token's rows, with nothing of another token on its way in that CTA), 1.4 for shared memory
+// and shuffles, 1.0 for results of fixed latency and 0.6 at barriers; 56 % of the issue slots are used, HBM at 32 %.
 constexpr int kQueriesAhead = 4;
 template <typename T, int LANES>
 __global__ __launch_bounds__(128, 7) void append4_kernel(const AppendArgs a) {
@@ -721,7 +726,8 @@ struct ReadArgs {
 
 // A warp per token of a step, tokens as append has them; head_dim / 8 lanes hold a row, and as many rows as fit the warp are
 // taken at once, four times over before the first is stored.  (A CTA per token, 8160 tokens of 2 x 8 heads of 128 from 4 bits: 20 us,
-// most of it the search for the sequence.)
+// most of it the search for the sequence; so 13.)  Eight sequences of 8192 tokens: 84 us from bf16 (6.4 TB/s), 69 from INT8
+// (5.9), 94 from 4 bits (3.7), whose copies are of 4 bytes a lane.
 constexpr int kReadWarps = 4, kReadAhead = 4;
 template <typename T, int BITS>
 __global__ __launch_bounds__(kReadWarps * 32) void read_kernel(const ReadArgs a) {

@@ -13,9 +13,10 @@
 // scores s but of s + log2(scale): what is rounded is at most 1, and exact relative to the largest contribution.
 //
 // Measured: 16 requests of up to 16K keys, 8 key heads of 128 bf16 channels, 110 us (6.1 TB/s, 95 % of a plain copy's rate);
-// 32 requests of up to 32K keys as codes 238 us at full clocks (5.9 TB/s), more in long runs, where the conversion's
-// instructions feel the lower clock; in 4 bits 202 (3.9 TB/s): 360 instructions a step, 160 of them conversion, at 57 % of the
-// issue slots, with three warps a scheduler.
+// 32 requests of up to 32K keys as codes 221 us in short runs (6.3 TB/s), 251 in long ones; in 4 bits 192 and 209 (3.7 TB/s): 360
+// instructions a step, 160 of them conversion.  Neither HBM nor the issue slots (57 %) are full there: of the 2.8 warps that a
+// scheduler has, 0.6 wait for a result of fixed latency, 0.3 for a math pipe, 0.4 for dispatch or instructions and 0.3 for
+// memory, so that none is ready in four cycles of ten; a fourth CTA's warps have no registers.
 #include "four_bits.cuh"
 #include "paged_tc.cuh"
 #include "serving_plan.cuh"

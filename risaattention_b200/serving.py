@@ -182,8 +182,9 @@ class KeyValueCache:
     [pages, kv_heads, page_size * (1 + head_dim / 16)].  A value is code * group scale * token scale.  Of each
     page and head the scales are first those of the tokens, powers of two as the exponent field of a float32
     (0: a scale of zero; 255: infinity, which makes the row NaN), then for each token those of its groups of
-    16 channels, float8_e4m3fn.  Channel 8 w + 2 i + j of a row is ``code + 8`` in bits 16 j + 4 i of its
-    32-bit word w."""
+    16 channels: float8_e4m3fn numbers from 0 to 448, so neither a sign bit nor the NaN of that type (whoever
+    fills a cache without ``append_to_cache`` sees to that; they are read by their bits and not checked).
+    Channel 8 w + 2 i + j of a row is ``code + 8`` in bits 16 j + 4 i of its 32-bit word w."""
 
     keys: torch.Tensor
     values: torch.Tensor
@@ -234,14 +235,19 @@ def append_to_cache(cache, k, v, page_table, lengths, *, query_offsets=None, q=N
     ones of sequence s is token ``lengths[s] - n + i`` of it.
 
     With ``rotary`` the keys are rotated first, by ``positions`` [tokens] (of a table with sections also
-    [axes, tokens]) or, without them, by those places;
-    ``q`` [tokens, q_heads, head_dim] is rotated in the same launch and returned (None without it; rows
-    behind the last sequence give 0).  An int8 cache stores absmax / 127 as a token's scale and the codes
-    rounded to nearest even.  One in 4 bits takes as a token's scale the smallest power of two (2^-126 at
-    least) of which its largest value is at most 7 * 448, as a group's the group's largest value over 7 of them,
-    rounded to e4m3, and codes rounded to nearest even: those of the exactly rotated keys.  Tokens that their sequence is too short for are not written; a page outside
-    the pool is not written either, and ``device_status()`` of the native module reports it.  Two sequences of
-    a step must not share the pages they write to."""
+    [axes, tokens]) or, without them, by those places; ``q`` [tokens, q_heads, head_dim] is rotated in the
+    same launch and returned (None without it; rows behind the last sequence give 0).
+
+    An int8 cache stores absmax / 127 as a token's scale and the codes rounded to nearest even.  A cache in 4
+    bits stores the codes of the exactly rotated keys:
+
+    token scale t  the smallest power of two, 2^-126 at least, with absmax <= 7 * 448 * t
+    group scale g  the group's absmax / (7 t), rounded to e4m3
+    code           x / (g t), rounded to nearest even, -7..7
+
+    Tokens that their sequence is too short for are not written; a page outside the pool is not written
+    either, and ``device_status()`` of the native module reports it.  Two sequences of a step must not share
+    the pages they write to."""
     _check_cache(cache)
     if rotary is not None:
         _check_table(rotary)
@@ -273,8 +279,10 @@ def paged_attention(q, cache, page_table, lengths, *, query_offsets=None, scale=
 
     With ``is_causal`` (aligned to the end: the last new token sees all ``lengths[s]`` keys) and ``window``
     a token sees the last ``window`` keys up to its own place and, of those in front of them, the first ``sinks``
-    of the sequence; keys between them are not read, nor are their entries of the page table.  Without
-    ``is_causal`` every token sees all.
+    of the sequence; keys between them are not read, nor are their entries of the page table.  (Keys keep the
+    rotation that they were appended with: in an endless conversation the distance to the first ones grows past
+    what a model was trained on, unless the ``positions`` given to ``append_to_cache`` stay within it.)
+    Without ``is_causal`` every token sees all.
     ``q_heads`` is a multiple of the cache's heads.  ``scale``: head_dim ** -0.5 unless given.  A token that
     sees nothing gives 0 and an LSE of -inf.  Rows of no sequence (behind the last, in front of the first) give
     the same; where ``out`` is given (``q`` itself included, no other view of its memory) its rows stay as they
@@ -282,12 +290,17 @@ def paged_attention(q, cache, page_table, lengths, *, query_offsets=None, scale=
     [tokens, q_heads].
 
     Unlike ``int8_attention`` nothing is quantised on the way: scores, softmax and sums are FP32 over the
-    cache's 16-bit values or codes as they are; probabilities are rounded to the type of ``q`` for the product
-    with V.  Over a cache of codes it is probability times the key's scale that is rounded, to float16, in units
-    of the largest such product that the token sees: of two scales that differ by more than 2^24 the smaller one's
-    values may be lost in that token.  (4-bit codes enter multiplied by their group's scale, exactly; where 33
-    rows or more of bfloat16 queries meet them by all their scales, and probabilities are rounded to bfloat16.)  A value that is not finite may also reach tokens of the same call
-    that do not see its key: it is multiplied by their probability, 0."""
+    cache's 16-bit values or codes as they are.  What is rounded for the product with V:
+
+    * over 16-bit values the probability, to the type of ``q``;
+    * over codes the probability times the key's scale, to float16, in units of the largest such product that
+      the token sees: of two scales that differ by more than 2^24 the smaller one's values may be lost in that
+      token (codes of 4 bits enter times their group's scale, which is exact);
+    * over codes of 4 bits with bfloat16 queries, where a key head has 33 query rows or more of a sequence, the
+      probability, to bfloat16 (the codes enter times all their scales, which is exact).
+
+    A value that is not finite may also reach tokens of the same call that do not see its key: it is multiplied
+    by their probability, 0."""
     _check_cache(cache)
     if scale is None:
         scale = q.shape[-1] ** -0.5
@@ -358,9 +371,10 @@ def resize_sequences(cache, references, page_table, lengths, new_lengths):
 
     Before tokens are appended: a longer sequence gets the lowest free pages, in the order of the sequences;
     where its last page is not full and shared, a page of its own in place of that, with a copy of its
-    tokens.  If pages run out it is granted the length that its pages hold (the old one, where a shared page
-    could not be replaced).  A shorter one, or length 0, gives its pages back; they may be handed out from
-    the next call on, by when nobody else may lead to them uncounted."""
+    tokens (each of those that share it, also where all of them grow in one call).  If pages run out it is
+    granted the length that its pages hold (the old one, where a shared page could not be replaced).  A
+    shorter one, or length 0, gives its pages back; they may be handed out from the next call on, by when
+    nobody else may lead to them uncounted."""
     _check_cache(cache)
     device = cache.keys.device
     return _native(device).resize_sequences(*cache.tensors, references, page_table, lengths, new_lengths, _stream(device))
