@@ -295,7 +295,9 @@ __device__ __forceinline__ uint32_t code_bits(int code, int channel) { return ui
 // values are off by 2^-20.9 of the row's largest value at most: the angle is rounded to 2^-25 of half a turn and sincospi gives two
 // units in the last place, 2^-22.2 of a pair whose length is sqrt(2) times that value at most, and two roundings follow; the quotient
 // adds 2^-22.8.  `doubtful` says that one of them lies within 1.5 x 2^-20, more than twice the sum, of a border: of its token's scale,
-// and where this lane's channels were `turned` (a group is, or is not) of its group's scale, or between codes of a group that has any.
+// and where this lane's channels were `turned` (a group is, or is not) of its group's scale, or between codes of a group that has any;
+// or that the row is not finite, which a finite one of bf16 can become in 32 bits.  (Values below 2^-126 are whole multiples of 2^-149
+// and so are the borders between their codes and scales: what is off by less than that meets a border or stays on its side.)
 template <int LANES, bool ROTATED>
 __device__ __forceinline__ Row4 row4_of(const float (&x)[8], bool turned, bool& doubtful) {
   float group = fabsf(x[0]);
@@ -327,7 +329,8 @@ __device__ __forceinline__ Row4 row4_of(const float (&x)[8], bool turned, bool& 
   if (ROTATED) {
     const float slack = most * to_units * 0x1.8p-20f;
     const uint32_t around = e4m3_pair(fmaf(slack, 1.0f / 7.0f, ratio), fmaxf(fmaf(slack, -1.0f / 7.0f, ratio), 0.f));
-    doubtful = usable && ((turned && ((r.group != 0 && nearest * scale < slack) || (around & 0xffu) != around >> 8)) || (bits - 24) >> 23 != (bits + 24) >> 23);
+    doubtful = !(most < INFINITY) || (usable && ((turned && ((r.group != 0 && nearest * scale < slack) || (around & 0xffu) != around >> 8)) ||
+                                                 (bits - 24) >> 23 != (bits + 24) >> 23));
   }
   if (__any_sync(0xffffffffu, r.group < 8)) {  // scales below 2^-6 are rounded coarsely: quotients past 7
 #pragma unroll
@@ -373,8 +376,8 @@ __device__ __noinline__ Row4 row4_of_rotated(const AppendArgs& a, Run<T> own, Ru
   for (int off = lanes >> 1; off > 1; off >>= 1) most = larger(most, __shfl_xor_sync(0xffffffffu, most, off));
   Row4 r{0x88888888u, 0, 0};
   if (most == 0.0) return r;
-  r.exponent = 255;  // not finite
-  if (!(most < double(INFINITY))) return r;
+  r.exponent = 255;  // not finite, or larger (by the table's magnitude) than any 7 * 448 token scales that readers take times 2^8
+  if (!(most <= 3136.0 * 0x1p119)) return r;
   r.exponent = max(int((__double_as_longlong(most) + (0xfffffffffffffll - 0x8800000000000ll)) >> 52) - 1023 - 11 + 127, 1);
   const double to_units = __longlong_as_double(int64_t(1023 + 127 - r.exponent) << 52), ratio = group * to_units / 7.0;
   // steps of 2^-3 of the leading bit, 2^-9 at least
@@ -707,7 +710,7 @@ __global__ __launch_bounds__(128, 7) void append4_kernel(const AppendArgs a) {
     k.zero();
     if (h < a.kv_heads) k.load(k0 + h * a.kh);
     const Row4 r = row4_of_rotated<T>(a, k, partner_of(k), token, place, LANES, channel);
-    if (h < a.kv_heads && r.exponent != 255) store(a.keys, a.key_scales, h, r);
+    if (h < a.kv_heads) store(a.keys, a.key_scales, h, r);
   }
 }
 

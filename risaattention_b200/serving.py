@@ -245,6 +245,8 @@ def append_to_cache(cache, k, v, page_table, lengths, *, query_offsets=None, q=N
     group scale g  the group's absmax / (7 t), rounded to e4m3
     code           x / (g t), rounded to nearest even, -7..7
 
+    (a row that is not finite, or whose absmax needs a token scale above 2^119, becomes NaN)
+
     Tokens that their sequence is too short for are not written; a page outside the pool is not written
     either, and ``device_status()`` of the native module reports it.  Two sequences of a step must not share
     the pages they write to."""
