@@ -31,7 +31,9 @@ __device__ __forceinline__ const uint8_t* groups4(const uint8_t* scales, int pag
 __device__ __forceinline__ float power_of(uint32_t exponent) { return __uint_as_float(exponent << 23); }
 // Its logarithm in units of group scales as they are read, for the running maximum of probabilities times scales.  A scale of zero
 // must not let its key's own probability overflow, nor may the largest ones (up to 2^125) leave denominators no room above
-// 2^-126: probabilities times scales then grow to 2^15, which fp16 holds.  (Rows that see one that is not finite become NaN.)
+// 2^-126: probabilities times scales then grow to 2^15, which fp16 holds.  (Rows that see one that is not finite become NaN.  Where all
+// scales that a row sees are below 2^-108 its largest product is below 1, and fp16's smallest numbers leave errors of 2^-133 of a
+// probability times scale, 2^-121 of a value, for each key.)
 __device__ __forceinline__ float lift_of(uint32_t exponent) {
   return fminf(fmaxf(__uint_as_float(0x4b000000u | exponent) - (8388608.0f + 119.0f), -100.f), 110.f);
 }
